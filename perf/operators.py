@@ -327,8 +327,13 @@ def _results(case, x):
     return {"out": (tuple(x["q"].shape), t), "lse": ((case["batch"], case["heads"], case["queries"]), torch.float32)}
 
 
+class _Buffer:
+    """A node's memory, for torch to look at."""
+
+
 class _Program:
-    """A context that holds a case's nodes and the operator linked to them; given back together."""
+    """A context that holds a case's nodes and the operator linked to them; given back together, when nothing looks at a node
+    any more (every view keeps its program)."""
 
     def __init__(self, case, x):
         global _device
@@ -336,7 +341,7 @@ class _Program:
         from ocannl_b200.low_level import Tnode
         if _device is None:
             _device = bk.Device(0)
-        self.context = None
+        self.context = self.operator = None
         kinds = {torch.float32: "single", torch.float16: "half", torch.bfloat16: "bfloat16", torch.int32: "int32"}
         nodes = [(n, tuple(v.shape), v.dtype) for n, v in x.items()] + [(n, d, t) for n, (d, t) in _results(case, x).items()]
         self.context = bk.Context(_device).allocate([Tnode(i + 1, n, kinds[t], d) for i, (n, d, t) in enumerate(nodes)])
@@ -346,7 +351,6 @@ class _Program:
             self.view(n).copy_(v)
         torch.cuda.synchronize()
         self.operator = self.link(case, self.context, x)
-        self.outputs = {n: self.view(n) for n in _results(case, x)}
 
     def link(self, case, ctx, x):
         if case["kind"] == "norm":
@@ -370,14 +374,14 @@ class _Program:
         pool, offset, t = self.context.arrays[ident]
         address, _ = _device.pool_address(pool)
 
-        class Buffer:
-            program = self
-            __cuda_array_interface__ = {"shape": tuple(t.dims), "data": (address + offset, False), "version": 3, "strides": None,
-                                        "typestr": {"single": "<f4", "half": "<f2", "bfloat16": "<i2", "int32": "<i4"}[t.prec]}
-        return torch.as_tensor(Buffer(), device="cuda").view(self.types[ident])
+        buffer = _Buffer()
+        buffer.program = self
+        buffer.__cuda_array_interface__ = {"shape": tuple(t.dims), "data": (address + offset, False), "version": 3, "strides": None,
+                                           "typestr": {"single": "<f4", "half": "<f2", "bfloat16": "<i2", "int32": "<i4"}[t.prec]}
+        return torch.as_tensor(buffer, device="cuda").view(self.types[ident])
 
-    def free(self):
-        if self.context is not None:
+    def __del__(self):
+        if self.context is not None and getattr(self, "operator", None) is not None:
             _device.await_()
             self.operator.free()
             for pool in {p for p, _, _ in self.context.arrays.values()}:
@@ -386,10 +390,7 @@ class _Program:
 
 
 class _State:
-    def __del__(self):
-        if own:
-            self.outputs = None
-            self.program.free()
+    pass
 
 
 def prepare(case, seed):
@@ -398,7 +399,8 @@ def prepare(case, seed):
     if own:
         # the nodes lie in the context's pool, the operator is linked to them
         s.program = _Program(case, s.x)
-        s.x, s.outputs = None, s.program.outputs
+        s.outputs = {n: s.program.view(n) for n in _results(case, s.x)}
+        s.x = None
     return s
 
 
