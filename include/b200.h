@@ -189,6 +189,100 @@ int b200_comm_free(b200_comm* comm);
 int b200_sum_f32_static(b200_dev* dev, int in_pool, size_t in_offset, size_t count, int out_pool,
                         size_t out_offset);
 
+/* ---- operators: what a decoder layer (lib/nn_blocks.ml:209-285) does between its contractions, as kernels of their own
+ *      beside the fused stages that b200_compile finds in a routine.  No counterpart in the reference, which spells them as
+ *      assignments.  An operator is linked to nodes once, like a routine -- arguments are checked, the kernels and the
+ *      workspace chosen -- and keeps their addresses: free it before their pools.  A run queues kernels on the device's
+ *      stream, in order with routines and copies; it allocates nothing, waits for nothing and may be captured into a CUDA graph.
+ *      Every linked operator has a workspace of its own; runs of ONE operator may not overlap on the GPU.
+ *      Nodes are row-major and need only be aligned to their element size (16 bytes are faster).  An output may not overlap
+ *      another operand, but where it says so.  Sums, statistics and softmax are held in single precision; 16-bit outputs are
+ *      rounded once.  The same inputs give the same bits. */
+typedef struct b200_operator b200_operator;
+#define B200_F16 2               /* beside B200_F32 and B200_BF16 */
+typedef struct {
+  int32_t pool_id;               /* negative: not given */
+  uint64_t offset;
+} b200_operand;
+int b200_operator_run(b200_operator* op);
+int b200_operator_free(b200_operator* op);   /* waits for the device's stream */
+
+/* Layer norm of rows of n elements (1 <= n <= 2^30) with a scale and a shift:
+ *   h = x + residual;  mean = sum(h) / n;  rstd = 1 / sqrt(sum((h - mean)^2) / n + eps);  y = (h - mean) * rstd * gamma + beta
+ * and, of the gradient dy of y, with u = (h - mean) * rstd and g = dy * gamma,
+ *   dx = rstd * (g - sum(g) / n - u * sum(g * u) / n) + d_total;  dgamma = sum_rows(dy * u);  dbeta = sum_rows(dy).
+ * (lib/nn_blocks.ml:251-258 divides the distance from the SUM by n; this is the usual norm.) */
+typedef struct {
+  int64_t rows, n;
+  int32_t dtype;                 /* x, residual, y, total, dy, d_total, dx */
+  int32_t weight_dtype;          /* gamma, beta: B200_F32 or `dtype` */
+  float eps;
+  b200_operand x;                /* gradient: h, that is `total` where there was a residual */
+  b200_operand residual;         /* forward, optional */
+  b200_operand gamma, beta;      /* [n], optional: 1 and 0 */
+  b200_operand y;                /* forward */
+  b200_operand total;            /* forward, optional, with a residual: h */
+  b200_operand mean, rstd;       /* [rows] single: written by the forward pass (optional), read by the gradient */
+  b200_operand dy, d_total;      /* gradient; d_total (optional): what reaches h from elsewhere */
+  b200_operand dx;               /* gradient: of x, and of the residual as well */
+  b200_operand dgamma, dbeta;    /* gradient, [n] single, each optional */
+} b200_layer_norm;
+int b200_layer_norm_link(b200_dev* dev, const b200_layer_norm* spec, b200_operator** out);
+int b200_layer_norm_grad_link(b200_dev* dev, const b200_layer_norm* spec, b200_operator** out);
+
+/* Rotary positions: of the first 2 * pairs elements of every head, pair i turns by the angle position * frequency[i] and is
+ * multiplied by `magnitude`; the head's other elements are copied.  Pairs are (i, i + pairs) or, interleaved, (2i, 2i + 1).
+ * x is [batch, seq, heads, d]; y has the same shape and may be x itself.  A second tensor (keys beside queries, with heads of its own) may
+ * go with the first.  inverse: the angle negated, which is the gradient's form (dy in the place of x).  Angles are kept in 64
+ * bits of a turn: far positions lose nothing. */
+typedef struct {
+  int64_t batch, seq;
+  int32_t heads[2];              /* heads[1] 0: one tensor */
+  int32_t d;
+  int32_t pairs;                 /* 2 * pairs <= d */
+  int32_t dtype;
+  int32_t interleaved, inverse;
+  float magnitude;
+  const double* frequencies;     /* host, [pairs]: radians per position; copied at link */
+  int64_t first_position;        /* of index 0 in seq, where no positions are given */
+  b200_operand positions;        /* int32 [batch, seq], optional */
+  b200_operand x[2], y[2];
+} b200_rotary;
+int b200_rotary_link(b200_dev* dev, const b200_rotary* spec, b200_operator** out);
+
+/* Attention of `queries` rows over `keys` keys (the chain of lib/nn_blocks.ml:222-236 at any length, nothing of it kept):
+ *   x_rj = scale * <q_r, k_j>;  c = cap * tanh(x / cap) (cap > 0) or x;  s = c - slope[h] * |position_r - j|
+ *   out_r = sum_j softmax_j(s_rj) v_j over the keys j that r sees, lse_r = log(sum_j exp(s_rj));  no key: 0 and -infinity
+ * q, out are [batch, queries, heads, d], k, v [batch, keys, kv_heads, d] (each key head serves heads / kv_heads query heads
+ * in a row), 1 <= d <= 128.  Query r of sequence b lies at position len_b - queries + r, where len_b is lengths[b] (taken
+ * between 0 and `keys`) or `keys`.  It sees key j if j < len_b, and
+ *   B200_MASK_CAUSAL: j <= position;   B200_MASK_PREFIX: j <= position or j < prefix[b];
+ *   and, with documents: key_documents[b, j] == query_documents[b, r] >= 0 (a negative document is padding).
+ * What lies at a key or a query that is not seen has no influence, whatever it holds.
+ * The gradient takes out and lse of the forward pass and gives, with p = exp(s - lse),
+ *   dv_j = sum_r p_rj d_out_r;  ds_rj = p_rj (<d_out_r, v_j> - <d_out_r, out_r>);  dx = ds (1 - (c / cap)^2)
+ *   dq_r = scale * sum_j dx_rj k_j;  dk_j = scale * sum_r dx_rj q_r
+ * where a key head's sums run over the query heads it serves.  slopes are constants: they get no gradient. */
+#define B200_MASK_NONE 0
+#define B200_MASK_CAUSAL 1
+#define B200_MASK_PREFIX 2
+typedef struct {
+  int64_t batch, queries, keys;
+  int32_t heads, kv_heads, d;
+  int32_t dtype;                 /* q, k, v, out and their gradients */
+  int32_t mask;
+  float scale, cap;              /* cap 0: none */
+  b200_operand q, k, v, out;
+  b200_operand lse;              /* [batch, heads, queries] single; optional in the forward pass */
+  b200_operand lengths, prefix;  /* int32 [batch] */
+  b200_operand query_documents;  /* int32 [batch, queries], and ... */
+  b200_operand key_documents;    /* int32 [batch, keys]: both or neither; may be one node */
+  b200_operand slopes;           /* single [heads] */
+  b200_operand d_out, dq, dk, dv;
+} b200_attention;
+int b200_attention_link(b200_dev* dev, const b200_attention* spec, b200_operator** out);
+int b200_attention_grad_link(b200_dev* dev, const b200_attention* spec, b200_operator** out);
+
 #ifdef __cplusplus
 }
 #endif

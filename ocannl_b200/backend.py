@@ -251,8 +251,90 @@ class Code:
             self.h = None
 
 
+# ------------------------------------------------------------------ operators
+class Operand(ctypes.Structure):
+    _fields_ = [("pool_id", ctypes.c_int32), ("offset", ctypes.c_uint64)]
+
+
+def _spec(name: str, *fields):
+    """A struct of include/b200.h; operands that are not set are not given."""
+    cls = type(name, (ctypes.Structure,), {"_fields_": [(f, t) for f, t in fields]})
+
+    def init(self, **values):
+        ctypes.Structure.__init__(self)
+        for f, t in fields:
+            if t is Operand:
+                setattr(self, f, Operand(-1, 0))
+            elif t is Operand * 2:
+                setattr(self, f, t(Operand(-1, 0), Operand(-1, 0)))
+        for k, v in values.items():
+            setattr(self, k, v)
+    cls.__init__ = init
+    return cls
+
+
+_i32, _i64, _f32 = ctypes.c_int32, ctypes.c_int64, ctypes.c_float
+LayerNormSpec = _spec("LayerNormSpec", ("rows", _i64), ("n", _i64), ("dtype", _i32), ("weight_dtype", _i32), ("eps", _f32),
+                      *((n, Operand) for n in ("x", "residual", "gamma", "beta", "y", "total", "mean", "rstd", "dy", "d_total", "dx",
+                                               "dgamma", "dbeta")))
+RotarySpec = _spec("RotarySpec", ("batch", _i64), ("seq", _i64), ("heads", _i32 * 2), ("d", _i32), ("pairs", _i32), ("dtype", _i32),
+                   ("interleaved", _i32), ("inverse", _i32), ("magnitude", _f32), ("frequencies", ctypes.POINTER(ctypes.c_double)),
+                   ("first_position", _i64), ("positions", Operand), ("x", Operand * 2), ("y", Operand * 2))
+AttentionSpec = _spec("AttentionSpec", ("batch", _i64), ("queries", _i64), ("keys", _i64), ("heads", _i32), ("kv_heads", _i32), ("d", _i32),
+                      ("dtype", _i32), ("mask", _i32), ("scale", _f32), ("cap", _f32),
+                      *((n, Operand) for n in ("q", "k", "v", "out", "lse", "lengths", "prefix", "query_documents", "key_documents",
+                                               "slopes", "d_out", "dq", "dk", "dv")))
+DTYPE = {"single": 0, "bfloat16": 1, "half": 2}   # B200_F32, B200_BF16, B200_F16
+MASKS = {"none": 0, "causal": 1, "prefix": 2}
+
+
+class Operator:
+    """A linked operator (`b200_operator`): `run` queues it on the device's stream.  Like a routine it keeps the addresses of
+    its nodes; free it before their pools."""
+
+    def __init__(self, device: Device, entry: str, spec):
+        self.h = ctypes.c_void_p()
+        check(getattr(lib(), entry)(device.h, ctypes.byref(spec), ctypes.byref(self.h)))
+        self._run = lib().b200_operator_run
+
+    def run(self):
+        rc = self._run(self.h)
+        if rc:
+            check(rc)
+
+    def free(self):
+        if self.h:
+            check(lib().b200_operator_free(self.h))
+            self.h = None
+
+
 def compile(ir: IrRoutine, options: Optional[str] = None) -> Code:  # noqa: A001 (mirrors Backend.compile)
     return Code(ir, options)
+
+
+def rotary_frequencies(dims: int, theta: float = 10000.0, scaling: str = "none", factor: float = 1.0, original: int = 4096,
+                       fast: float = 32.0, slow: float = 1.0) -> Tuple[np.ndarray, float]:
+    """Radians per position of the dims / 2 pairs of `Context.rotary`, and the magnitude: theta^(-2i / dims), for long contexts
+    "linear" (positions shrink by `factor`), "ntk" (the base grows, so that the slowest pair shrinks by `factor` and the
+    fastest stays) or "yarn" (pairs that turn more than `fast` times over the `original` context stay, those that turn less
+    than `slow` times shrink by `factor`, a ramp between; magnitude 0.1 ln(factor) + 1)."""
+    if dims < 0 or dims % 2 or theta <= 0 or factor <= 0:
+        raise UserError(-5, "rotary_frequencies: an even number of dims, a positive base and factor")
+    m = dims // 2
+    i = np.arange(m, dtype=np.float64)
+    f = theta ** (-i / max(m, 1))
+    if scaling == "none":
+        return f, 1.0
+    if scaling == "linear":
+        return f / factor, 1.0
+    if scaling == "ntk":
+        return (theta * factor ** (m / max(1, m - 1))) ** (-i / max(m, 1)), 1.0
+    if scaling != "yarn":
+        raise UserError(-5, "rotary_frequencies: unknown scaling '%s'" % scaling)
+    low, high = (m * np.log(original / (2.0 * np.pi * turns)) / np.log(theta) for turns in (fast, slow))
+    low, high = max(0.0, np.floor(low)), min(m - 1.0, np.ceil(high))
+    ramp = np.clip((i - low) / max(1e-3, high - low), 0.0, 1.0)
+    return f * (1.0 - ramp) + f / factor * ramp, float(0.1 * np.log(factor) + 1.0)
 
 
 POOL_CAP = 0x1_0000_0000   # bytes per pool while offsets are 32-bit (arrayjit/lib/backends.ml:536)
@@ -378,6 +460,116 @@ class Context:
         h = ctypes.c_void_p()
         check(lib().b200_link(dev.h, code.h, binds, ctypes.c_int(len(params)), ctypes.byref(h)))
         return Routine(self._child(arrays), code, h)
+
+    # ---- operators over nodes of this context (b200_layer_norm_link and its kin in include/b200.h, which define them)
+    def _operand(self, what: str, ident: Optional[str], prec, dims) -> Operand:
+        """The node's location, its precision and shape checked; dims None: any, "*" in dims: any extent."""
+        if ident is None:
+            return Operand(-1, 0)
+        if ident not in self.arrays:
+            raise UserError(-5, "%s: the context holds no node '%s'" % (what, ident))
+        pool, off, t = self.arrays[ident]
+        if t.prec not in ((prec,) if isinstance(prec, str) else prec):
+            raise UserError(-5, "%s: node '%s' is of precision %s, not %s" % (what, ident, t.prec, prec))
+        if dims is not None and tuple(t.dims) != tuple(dims):
+            raise UserError(-5, "%s: node '%s' has dims %s, not %s" % (what, ident, tuple(t.dims), tuple(dims)))
+        return Operand(pool, off)
+
+    def _node(self, what: str, ident: str) -> Tnode:
+        if ident not in self.arrays:
+            raise UserError(-5, "%s: the context holds no node '%s'" % (what, ident))
+        t = self.arrays[ident][2]
+        if t.prec not in DTYPE:
+            raise UserError(-5, "%s: node '%s' of precision %s: single, bfloat16 or half is wanted" % (what, ident, t.prec))
+        return t
+
+    def _norm(self, what: str, x: str, gamma: Optional[str], beta: Optional[str], eps: float, rows_like, weights, stats, sums) -> Operator:
+        t = self._node(what, x)
+        if not t.dims:
+            raise UserError(-5, "%s: node '%s' has no axis" % (what, x))
+        n = t.dims[-1]
+        given = {self._node(what, w).prec for w in (gamma, beta) if w is not None}
+        if len(given) > 1:
+            raise UserError(-5, "%s: gamma and beta are of one precision" % what)
+        wprec = given.pop() if given else "single"
+        spec = LayerNormSpec(rows=t.num_elems // n if n else 0, n=n, dtype=DTYPE[t.prec], weight_dtype=DTYPE[wprec], eps=eps)
+        for names, prec, dims in ((dict(rows_like, x=x), t.prec, t.dims), (weights, wprec, (n,)), (stats, "single", t.dims[:-1]),
+                                  (sums, "single", (n,))):
+            for field, ident in names.items():
+                setattr(spec, field, self._operand(what, ident, prec, dims))
+        return Operator(self.device, "b200_%s_link" % what, spec)
+
+    def layer_norm(self, x: str, y: str, gamma: Optional[str] = None, beta: Optional[str] = None, residual: Optional[str] = None,
+                   total: Optional[str] = None, mean: Optional[str] = None, rstd: Optional[str] = None, eps: float = 1e-5) -> Operator:
+        """y = the norm of x (+ residual, their sum kept in `total`) along the last axis, scaled by gamma, shifted by beta.
+        mean, rstd (single, the shape of x without its last axis) are what `layer_norm_grad` reads."""
+        return self._norm("layer_norm", x, gamma, beta, eps, dict(y=y, residual=residual, total=total), dict(gamma=gamma, beta=beta),
+                          dict(mean=mean, rstd=rstd), {})
+
+    def layer_norm_grad(self, x: str, dy: str, dx: str, mean: str, rstd: str, gamma: Optional[str] = None, dgamma: Optional[str] = None,
+                        dbeta: Optional[str] = None, d_total: Optional[str] = None) -> Operator:
+        """The gradients of `layer_norm`: x is its input, `total` where there was a residual (whose gradient is dx too);
+        d_total is added to dx; dgamma and dbeta (single) are sums over all rows."""
+        return self._norm("layer_norm_grad", x, gamma, None, 0.0, dict(dy=dy, dx=dx, d_total=d_total), dict(gamma=gamma),
+                          dict(mean=mean, rstd=rstd), dict(dgamma=dgamma, dbeta=dbeta))
+
+    def rotary(self, tensors: Sequence[Tuple[str, str]], frequencies: Sequence[float], magnitude: float = 1.0,
+               positions: Optional[str] = None, first_position: int = 0, layout: str = "half", inverse: bool = False) -> Operator:
+        """Turns the pairs of one or two tensors [batch, seq, heads, d], given as (from, to) (which may be one node), by
+        position * frequencies[pair] (radians, `rotary_frequencies`).  layout: "half" pairs element i with
+        i + len(frequencies), "interleaved" 2i with 2i + 1.  inverse: the other way, as gradients go."""
+        if not 1 <= len(tensors) <= 2:
+            raise UserError(-5, "rotary: one or two tensors")
+        if layout not in ("half", "interleaved"):
+            raise UserError(-5, "rotary: unknown layout '%s'" % layout)
+        t = self._node("rotary", tensors[0][0])
+        if len(t.dims) != 4:
+            raise UserError(-5, "rotary: node '%s' is not [batch, seq, heads, d]" % tensors[0][0])
+        f = np.ascontiguousarray(frequencies, dtype=np.float64).reshape(-1)
+        spec = RotarySpec(batch=t.dims[0], seq=t.dims[1], d=t.dims[3], pairs=f.size, dtype=DTYPE[t.prec], interleaved=int(layout == "interleaved"),
+                          inverse=int(inverse), magnitude=magnitude, frequencies=f.ctypes.data_as(ctypes.POINTER(ctypes.c_double)),
+                          first_position=first_position, positions=self._operand("rotary", positions, "int32", t.dims[:2]))
+        for i, (src, dst) in enumerate(tensors):
+            u = self._node("rotary", src)
+            dims = (t.dims[0], t.dims[1], u.dims[2] if len(u.dims) == 4 else -1, t.dims[3])
+            spec.heads[i] = dims[2]
+            spec.x[i], spec.y[i] = self._operand("rotary", src, t.prec, dims), self._operand("rotary", dst, t.prec, dims)
+        return Operator(self.device, "b200_rotary_link", spec)
+
+    def _attention(self, what: str, q: str, k: str, rows_like, keys_like, lse, mask, prefix, documents, lengths, slopes, scale, cap) -> Operator:
+        t, u = self._node(what, q), self._node(what, k)
+        if len(t.dims) != 4 or len(u.dims) != 4:
+            raise UserError(-5, "%s: q is [batch, queries, heads, d], k and v are [batch, keys, kv_heads, d]" % what)
+        if mask not in MASKS:
+            raise UserError(-5, "%s: unknown mask '%s'" % (what, mask))
+        (b, s, h, d), (n, hk) = t.dims, u.dims[1:3]
+        spec = AttentionSpec(batch=b, queries=s, keys=n, heads=h, kv_heads=hk, d=d, dtype=DTYPE[t.prec], mask=MASKS[mask],
+                             scale=1.0 / np.sqrt(d) if scale is None and d else scale or 0.0, cap=cap)
+        qdoc, kdoc = (documents, documents) if documents is None or isinstance(documents, str) else documents
+        for names, prec, dims in ((dict(rows_like, q=q), t.prec, t.dims), (dict(keys_like, k=k), t.prec, (b, n, hk, d)),
+                                  (dict(lse=lse), "single", (b, h, s)), (dict(prefix=prefix, lengths=lengths), "int32", (b,)),
+                                  (dict(query_documents=qdoc), "int32", (b, s)), (dict(key_documents=kdoc), "int32", (b, n)),
+                                  (dict(slopes=slopes), "single", (h,))):
+            for field, ident in names.items():
+                setattr(spec, field, self._operand(what, ident, prec, dims))
+        return Operator(self.device, "b200_%s_link" % what, spec)
+
+    def attention(self, q: str, k: str, v: str, out: str, lse: Optional[str] = None, mask: str = "causal", prefix: Optional[str] = None,
+                  documents=None, lengths: Optional[str] = None, slopes: Optional[str] = None, scale: Optional[float] = None,
+                  cap: float = 0.0) -> Operator:
+        """out = softmax over the visible keys of the scores, times v; lse (single [batch, heads, queries]) is what
+        `attention_grad` reads.  The queries are the last ones of each sequence's `lengths` (or all) keys.  mask: "none",
+        "causal" or "prefix" (keys before prefix[b] are seen by all).  documents: an int32 node of numbers per key -- or two, of
+        queries and keys; queries see keys of their own document, a negative number is padding.  slopes: bias by distance,
+        -slopes[h] * |position - key|.  scale: 1 / sqrt(d) by default.  cap: scores become cap * tanh(score / cap)."""
+        return self._attention("attention", q, k, dict(out=out), dict(v=v), lse, mask, prefix, documents, lengths, slopes, scale, cap)
+
+    def attention_grad(self, q: str, k: str, v: str, out: str, lse: str, d_out: str, dq: str, dk: str, dv: str, mask: str = "causal",
+                       prefix: Optional[str] = None, documents=None, lengths: Optional[str] = None, slopes: Optional[str] = None,
+                       scale: Optional[float] = None, cap: float = 0.0) -> Operator:
+        """The gradients of `attention`, from its inputs, its out and lse, and the gradient d_out of out."""
+        return self._attention("attention_grad", q, k, dict(out=out, d_out=d_out, dq=dq), dict(v=v, dk=dk, dv=dv), lse, mask, prefix,
+                               documents, lengths, slopes, scale, cap)
 
     # ---- host access (Context.set_values / get_values, arrayjit/lib/context.ml:322-395)
     def from_host(self, ident: str, arr: np.ndarray):

@@ -23,7 +23,7 @@ CUDA = os.environ.get("CUDA_HOME", "/usr/local/cuda")
 
 HOST_SOURCES = ["ir.cpp", "emit.cpp", "compile.cpp", "gemm_match.cpp", "attn_match.cpp", "driver.cpp", "runtime.cpp",
                 "gemm_launch.cpp", "api.cpp"]
-CUDA_SOURCES = ["sum_static.cu"]
+CUDA_SOURCES = ["sum_static.cu", "op_norm.cu", "op_rotary.cu", "op_attention.cu"]
 EMBED = {"kNumericsSource": "kernels/numerics.cuh", "kTcSource": "kernels/tc_sm100.cuh",
          "kGemmSource": "kernels/gemm_sm100.cuh", "kAttnSource": "kernels/attn_sm100.cuh",
          "kAttnRowsSource": "kernels/attn_rows.cuh"}

@@ -17,6 +17,7 @@
 
 #include "compile.hpp"
 #include "driver.hpp"
+#include "operators.hpp"
 #include "runtime.hpp"
 
 using namespace b200;
@@ -845,5 +846,26 @@ int b200_comm_free(b200_comm* comm) {
     if (comm->comm && !comm->aborted) nccl().ncclCommDestroy_(comm->comm);
     if (comm->stream) cu().cuStreamDestroy_(comm->stream);
     delete comm;
+  });
+}
+
+// ---------------------------------------------------------------- operators
+int b200_operator_run(b200_operator* op) {
+  return guard([&] {
+    if (!op) throw Error(B200_E_INVALID, "null operator");
+    op->dev->make_current(/*join=*/false);
+    if (op->dev->uploads_pending)
+      for (int p : op->pools_used) op->dev->join_pool_id(p);
+    op->run((cudaStream_t)op->dev->stream);
+  });
+}
+
+int b200_operator_free(b200_operator* op) {
+  return guard([&] {
+    if (!op) return;
+    op->dev->make_current(/*join=*/false);
+    cu_check(cu().cuStreamSynchronize_(op->dev->stream), "cuStreamSynchronize");
+    if (op->workspace) cu_check(cu().cuMemFree_(op->workspace), "cuMemFree(operator workspace)");
+    delete op;
   });
 }

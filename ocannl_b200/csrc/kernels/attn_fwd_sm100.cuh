@@ -1,0 +1,471 @@
+// Attention for 16-bit heads on the tensor cores, any number of keys: softmax with a running maximum and sum.
+//
+// A CTA takes NQ tiles of 128 queries of one (sequence, head).  Roles: a warp that copies (TMA: the queries once, then tiles of
+// 128 keys and values through rings), a warp that issues tcgen05.mma, and four warps per query tile that do the softmax, a thread
+// a row.  Scores of a tile lie in tensor memory (128 columns); the thread loads its row of 128, applies cap, bias and mask, takes
+// the maximum, writes the weights exp2(s - m) in 16 bits over the scores, and they are the A operand of the second product, which adds
+// to the output accumulators in tensor memory.  The accumulators are only multiplied by 2^(m_old - m_new) when a row's maximum has
+// grown by more than 2^8 (weights stay below that, sums and accumulators are single precision, so nothing is lost): after the
+// first tiles hardly ever.  With NQ = 2 the two tiles take turns on the tensor cores and on the arithmetic; with NQ = 1 two CTAs of an SM do.
+//
+// Key tiles that no query of a tile sees are skipped, and those that all see take no mask: the classes of all key tiles are made
+// first, from the rows' last keys and the range of document numbers in each tile.
+#ifndef B200_ATTN_FWD_SM100_CUH
+#define B200_ATTN_FWD_SM100_CUH
+#include "attn_terms.cuh"
+#ifndef B200_ELEM_BYTES
+#define B200_ELEM_BYTES 2
+#endif
+#include "tc_sm100.cuh"
+#include <type_traits>
+
+namespace b200 {
+
+constexpr unsigned int kTileBytes64 = 128 * 128;   // 128 rows x 64 elements of 16 bits: one swizzled panel
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// tanh x = 1 - 2 / (e^2x + 1), of which 2 x log2(e) is given; off by a few 2^-24 (absolute), which a cap multiplies
+__device__ __forceinline__ float tanh_of(float two_x_log2e) { return fmaf(-2.f, rcp(ex2(two_x_log2e) + 1.f), 1.f); }
+
+// A from tensor memory: 16-bit elements, two to a column
+__device__ __forceinline__ void umma_ts(unsigned int d, unsigned int a, unsigned long long b, unsigned int idesc, unsigned int accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_st16(unsigned int taddr, const unsigned int* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr), "r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
+      "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void named_barrier(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+
+template <class T>
+__host__ __device__ constexpr unsigned int idesc_of(int m, int n, bool a_mn, bool b_mn) {
+  const unsigned int f = sizeof(T) == 2 ? (std::is_same<T, __nv_bfloat16>::value ? 1u : 0u) : 0u;
+  return (1u << 4) | (f << 7) | (f << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) | ((unsigned int)(n / 8) << 17) | ((unsigned int)(m / 16) << 24);
+}
+
+// what a tile of rows sees: the least and the greatest last key, the range of documents
+struct AttnSpan {
+  int last_min, last_max, doc_min, doc_max;
+};
+__device__ __forceinline__ AttnSpan span_of(bool ok, const AttnRow& w) {
+  AttnSpan s;
+  s.last_min = __reduce_min_sync(0xffffffffu, ok ? w.last : 0x7fffffff);
+  s.last_max = __reduce_max_sync(0xffffffffu, ok ? w.last : -1);
+  s.doc_min = __reduce_min_sync(0xffffffffu, ok ? w.doc : 0x7fffffff);
+  s.doc_max = __reduce_max_sync(0xffffffffu, ok ? w.doc : -0x7fffffff - 1);
+  return s;
+}
+// 0: no row sees a key of the tile, 1: every row sees every key, 2: some
+__device__ __forceinline__ unsigned int tile_class(const AttnSpan& s, int j0, bool docs, int kmin, int kmax, bool negative) {
+  if (j0 > s.last_max) return 0u;
+  if (!docs) return j0 + 127 <= s.last_min ? 1u : 2u;
+  if (kmax < s.doc_min || kmin > s.doc_max) return 0u;
+  return (j0 + 127 <= s.last_min && !negative && kmin == kmax && s.doc_min == s.doc_max && s.doc_min == kmin) ? 1u : 2u;
+}
+// range of the non-negative documents of keys j0 .. j0 + 127 (a warp); `negative`: some are padding
+__device__ __forceinline__ void key_documents(const AttnArgs& a, int b, int j0, unsigned int lane, int& kmin, int& kmax, bool& negative) {
+  int lo = 0x7fffffff, hi = -1, bad = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int j = j0 + (int)lane + 32 * i;
+    if (j < a.T) {
+      const int d = a.kdoc[(long long)b * a.T + j];
+      if (d < 0) bad = 1;
+      else { lo = min(lo, d); hi = max(hi, d); }
+    }
+  }
+  kmin = __reduce_min_sync(0xffffffffu, lo);
+  kmax = __reduce_max_sync(0xffffffffu, hi);
+  negative = __any_sync(0xffffffffu, bad);
+}
+// Which of the 128 keys from j0 the lane's row sees, a bit each.  The rows of a warp belong to one document or a few: one round each.
+__device__ __forceinline__ void visible_words(const AttnArgs& a, int b, int j0, const AttnRow& w, unsigned int lane, unsigned int (&bits)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int n = w.last + 1 - (j0 + 32 * i);       // keys of this word up to the last one
+    bits[i] = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
+  }
+  if (!a.kdoc) return;
+  int d[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int j = j0 + (int)lane + 32 * i;
+    d[i] = j < a.T ? a.kdoc[(long long)b * a.T + j] : -1;
+  }
+  unsigned int todo = 0xffffffffu;
+  while (todo) {
+    const int doc = __shfl_sync(0xffffffffu, w.doc, __ffs(todo) - 1);
+    const bool mine = w.doc == doc;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const unsigned int same = __ballot_sync(0xffffffffu, d[i] == doc);
+      if (mine) bits[i] &= same;
+    }
+    todo &= ~__ballot_sync(0xffffffffu, mine);
+  }
+}
+
+template <int DP, int NQ>
+struct FwdShape {
+  static constexpr int kPanels = DP / 64;
+  static constexpr unsigned int kTile = kPanels * kTileBytes64;
+  // two slots each for keys and values; one, where two CTAs of 96 KB share an SM
+  static constexpr int kSlots = (DP == 128 && NQ == 1) ? 1 : 2;
+  static constexpr unsigned int kThreads = NQ * 128 + 64;
+  static constexpr unsigned int kBytes = NQ * kTile + 2 * kSlots * kTile;
+  static constexpr unsigned int kColumns = NQ * (128 + DP) <= 256 ? 256 : 512;
+  static constexpr size_t smem(int tiles) { return 1024 + kBytes + 256 + (size_t)tiles; }
+};
+
+template <class T, int DP, int NQ, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(NQ * 128 + 64, NQ == 1 ? 2 : 1)
+attn_forward_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant__ b200_tmap map_k, const __grid_constant__ b200_tmap map_v,
+                const __grid_constant__ b200_tmap map_o, const __grid_constant__ AttnArgs a) {
+  typedef FwdShape<DP, NQ> Sh;
+  extern __shared__ unsigned char dyn[];
+  const unsigned int base = (b200_smem_addr(dyn) + 1023u) & ~1023u;
+  unsigned char* const gen = dyn + (base - b200_smem_addr(dyn));
+  const unsigned int q_at = base, k_at = base + NQ * Sh::kTile, v_at = k_at + Sh::kSlots * Sh::kTile;
+  unsigned long long* bars = (unsigned long long*)(gen + Sh::kBytes);
+  const unsigned int bar0 = b200_smem_addr(bars);
+  const unsigned int bar_q = bar0, bar_kf = bar0 + 8, bar_ke = bar0 + 24, bar_vf = bar0 + 40, bar_ve = bar0 + 56;   // two each but bar_q
+  const unsigned int bar_s = bar0 + 72, bar_p = bar0 + 88, bar_o = bar0 + 104;                                       // a query tile each
+  volatile unsigned int* tmem_slot = (volatile unsigned int*)(bars + 16);
+  volatile unsigned int* abort_flag = tmem_slot + 1;
+  volatile unsigned int* repair = tmem_slot + 2;      // [2]: some row of the query tile came out infinite or undefined
+  AttnSpan* spans = (AttnSpan*)(bars + 18);           // [2], 16 bytes each
+  unsigned char* classes = (unsigned char*)(gen + Sh::kBytes + 256);
+
+  asm volatile("griddepcontrol.launch_dependents;");
+  const unsigned int warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+  const unsigned int kLoad = NQ * 4, kMma = NQ * 4 + 1;
+  if (threadIdx.x == 0) {
+    b200_mbar_init(bar_q, 1);
+    for (int i = 0; i < 2; ++i) {
+      b200_mbar_init(bar_kf + 8 * i, 1);
+      b200_mbar_init(bar_ke + 8 * i, 1);
+      b200_mbar_init(bar_vf + 8 * i, 1);
+      b200_mbar_init(bar_ve + 8 * i, 1);
+      b200_mbar_init(bar_s + 8 * i, 1);
+      b200_mbar_init(bar_p + 8 * i, 128);
+      b200_mbar_init(bar_o + 8 * i, 1);
+      repair[i] = 0u;
+      spans[i].last_min = spans[i].doc_min = 0x7fffffff;
+      spans[i].last_max = -1;
+      spans[i].doc_max = -0x7fffffff - 1;
+    }
+    *abort_flag = 0u;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kMma) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(b200_smem_addr((const void*)tmem_slot)), "r"(Sh::kColumns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  // this CTA's queries: the last ones first, which under a causal mask see the most keys
+  const unsigned int heads = (unsigned int)a.B * (unsigned int)a.H;
+  const unsigned int tiles_q = (a.S + 128 * NQ - 1) / (128 * NQ);
+  const int r0 = (int)(tiles_q - 1 - blockIdx.x / heads) * 128 * NQ;
+  const unsigned int bh = blockIdx.x % heads;
+  const int b = (int)(bh / (unsigned int)a.H), h = (int)(bh % (unsigned int)a.H), hk = h / a.group;
+  const unsigned int g = warp >> 2;                        // query tile of a softmax warp
+  const int r = r0 + (int)threadIdx.x;                     // row of a softmax thread
+  AttnRow row;
+  row.pos = 0; row.last = -1; row.doc = 0;
+  tc_before();
+  __syncthreads();
+  tc_after();
+  if (warp < kLoad) {
+    if (r < a.S) row = attn_row(a, b, r);
+    const AttnSpan s = span_of(r < a.S, row);
+    if (lane == 0) {
+      atomicMin(&spans[g].last_min, s.last_min);
+      atomicMax(&spans[g].last_max, s.last_max);
+      atomicMin(&spans[g].doc_min, s.doc_min);
+      atomicMax(&spans[g].doc_max, s.doc_max);
+    }
+  }
+  __syncthreads();
+  int n_tiles = 0;
+#pragma unroll
+  for (int i = 0; i < NQ; ++i) n_tiles = max(n_tiles, (spans[i].last_max + 128) / 128);
+  for (int t = (int)warp; t < n_tiles; t += (int)(Sh::kThreads / 32)) {
+    int kmin = 0, kmax = 0;
+    bool negative = false;
+    if (a.kdoc) key_documents(a, b, t * 128, lane, kmin, kmax, negative);
+    unsigned int c = 0;
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) c |= tile_class(spans[i], t * 128, a.kdoc != nullptr, kmin, kmax, negative) << (2 * i);
+    if (lane == 0) classes[t] = (unsigned char)c;
+  }
+  __syncthreads();
+  const unsigned int tmem = *tmem_slot;
+  const unsigned int acc_o = tmem + NQ * 128;              // output accumulators behind the scores
+
+  if (warp == kLoad) {
+    if (b200_elect()) {
+      b200_mbar_expect_tx(bar_q, NQ * Sh::kTile);
+#pragma unroll
+      for (int i = 0; i < NQ; ++i)
+#pragma unroll
+        for (int p = 0; p < Sh::kPanels; ++p) b200_tma_load_4d(q_at + i * Sh::kTile + p * kTileBytes64, &map_q, bar_q, p * 64, r0 + 128 * i, h, b);
+      unsigned int n = 0;
+      bool live = true;
+      for (int t = 0; t < n_tiles && live; ++t) {
+        if (!classes[t]) continue;
+        const unsigned int slot = n % Sh::kSlots, use = n / Sh::kSlots;
+        if (use) live = b200_wait(bar_ke + 8 * slot, (use - 1) & 1u, abort_flag, a.status, 21u);
+        if (!live) break;
+        b200_mbar_expect_tx(bar_kf + 8 * slot, Sh::kTile);
+#pragma unroll
+        for (int p = 0; p < Sh::kPanels; ++p) b200_tma_load_4d(k_at + slot * Sh::kTile + p * kTileBytes64, &map_k, bar_kf + 8 * slot, p * 64, t * 128, hk, b);
+        if (use) live = b200_wait(bar_ve + 8 * slot, (use - 1) & 1u, abort_flag, a.status, 22u);
+        if (!live) break;
+        b200_mbar_expect_tx(bar_vf + 8 * slot, Sh::kTile);
+#pragma unroll
+        for (int p = 0; p < Sh::kPanels; ++p) b200_tma_load_4d(v_at + slot * Sh::kTile + p * kTileBytes64, &map_v, bar_vf + 8 * slot, p * 64, t * 128, hk, b);
+        ++n;
+      }
+      // the copies under way land before shared memory is given up, whatever happened to the others
+      if (n && *abort_flag) {
+        for (unsigned int i = 0; i < Sh::kSlots && i < n; ++i) {
+          const unsigned int last = (n - 1 - i) / Sh::kSlots, slot = (n - 1 - i) % Sh::kSlots;
+          for (int tries = 0; tries < 1 << 20 && !b200_mbar_try(bar_kf + 8 * slot, last & 1u); ++tries) {}
+          for (int tries = 0; tries < 1 << 20 && !b200_mbar_try(bar_vf + 8 * slot, last & 1u); ++tries) {}
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == kMma) {
+    if (b200_elect()) {
+      constexpr unsigned int idesc_s = idesc_of<T>(128, 128, false, false), idesc_o = idesc_of<T>(128, DP, false, true);
+      bool live = b200_wait(bar_q, 0u, abort_flag, a.status, 23u);
+      auto scores = [&](int i, unsigned int slot) {
+#pragma unroll
+        for (int p = 0; p < Sh::kPanels; ++p) {
+          const unsigned long long dq = b200_smem_desc(q_at + i * Sh::kTile + p * kTileBytes64, 16u, 1024u);
+          const unsigned long long dk = b200_smem_desc(k_at + slot * Sh::kTile + p * kTileBytes64, 16u, 1024u);
+#pragma unroll
+          for (unsigned int ks = 0; ks < 4; ++ks) b200_umma(tmem + i * 128, dq + ks * 2, dk + ks * 2, idesc_s, (p || ks) ? 1u : 0u);
+        }
+        b200_umma_commit(bar_s + 8 * i);
+      };
+      unsigned int done[NQ];                     // tiles whose weights have been multiplied
+      int last[NQ];                              // the last tile of keys that a query tile sees: its product is awaited
+#pragma unroll
+      for (int i = 0; i < NQ; ++i) {
+        done[i] = 0;
+        for (last[i] = n_tiles - 1; last[i] >= 0 && !((classes[last[i]] >> (2 * i)) & 3u); --last[i]) {}
+      }
+      // the scores of a tile are queued behind the products of the tile before it, query tile by query tile
+      int t = 0, next = 0;
+      unsigned int n = 0;
+      while (next < n_tiles && !classes[next]) ++next;
+      if (live && next < n_tiles) {
+        live = b200_wait(bar_kf, 0u, abort_flag, a.status, 24u);
+        tc_after();
+        if (live) {
+#pragma unroll
+          for (int i = 0; i < NQ; ++i)
+            if ((classes[next] >> (2 * i)) & 3u) scores(i, 0);
+          b200_umma_commit(bar_ke);
+        }
+      }
+      while (live && next < n_tiles) {
+        t = next;
+        for (++next; next < n_tiles && !classes[next]; ++next) {}
+        const unsigned int slot = n % Sh::kSlots, ph = (n / Sh::kSlots) & 1u, slot1 = (n + 1) % Sh::kSlots, ph1 = ((n + 1) / Sh::kSlots) & 1u;
+        live = b200_wait(bar_vf + 8 * slot, ph, abort_flag, a.status, 25u);
+        if (live && next < n_tiles) live = b200_wait(bar_kf + 8 * slot1, ph1, abort_flag, a.status, 26u);
+        tc_after();
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) {
+          if (!live) break;
+          if ((classes[t] >> (2 * i)) & 3u) {
+            live = b200_wait(bar_p + 8 * i, done[i] & 1u, abort_flag, a.status, 27u);
+            tc_after();
+            if (!live) break;
+            const unsigned long long dv = b200_smem_desc(v_at + slot * Sh::kTile, kTileBytes64, 1024u);
+#pragma unroll
+            for (unsigned int ks = 0; ks < 8; ++ks)
+              umma_ts(acc_o + i * DP, tmem + i * 128 + ks * 8, dv + ks * 128, idesc_o, (done[i] || ks) ? 1u : 0u);
+            if (t == last[i]) b200_umma_commit(bar_o + 8 * i);
+            ++done[i];
+          }
+          if (i == NQ - 1) b200_umma_commit(bar_ve + 8 * slot);
+          if (next < n_tiles && ((classes[next] >> (2 * i)) & 3u)) scores(i, slot1);
+        }
+        if (!live) break;
+        if (next < n_tiles) b200_umma_commit(bar_ke + 8 * slot1);
+        ++n;
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---------------------------------------------------------------- softmax: a thread a row
+    const unsigned int mine = tmem + g * 128 + ((warp & 3u) << 21), mine_o = acc_o + g * DP + ((warp & 3u) << 21);
+    const float c = CAP ? a.cap * kLog2e : a.scale * kLog2e;
+    const float to_tanh = CAP ? 2.f * kLog2e * a.scale / a.cap : 0.f;
+    const float slope2 = BIAS ? a.slopes[h] * kLog2e : 0.f;
+    float m = -INFINITY, l = 0.f;      // m: in log 2 units without bias or cap scaled by c, see `unit`
+    const float unit = BIAS ? 1.f : c;
+    unsigned int seen = 0;
+    bool live = true;
+    for (int t = 0; t < n_tiles && live; ++t) {
+      const unsigned int cls = (classes[t] >> (2 * g)) & 3u;
+      if (!cls) continue;
+      live = b200_wait(bar_s + 8 * g, seen & 1u, abort_flag, a.status, 28u);
+      if (!live) break;
+      tc_after();
+      // first pass: the row's maximum, 32 scores at a time; what cap, bias or mask have changed goes back
+      unsigned int bits[4] = {0u, 0u, 0u, 0u};
+      if (cls == 2u) visible_words(a, b, t * 128, row, lane, bits);
+      float x[2][32], top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      b200_tmem_ld32(mine, (unsigned int*)x[0]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float* y = x[k & 1];
+        tmem_wait_ld();
+        if (k < 3) b200_tmem_ld32(mine + 32 * (k + 1), (unsigned int*)x[(k + 1) & 1]);
+        if constexpr (CAP) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) y[j] = tanh_of(y[j] * to_tanh);
+        }
+        if constexpr (BIAS) {
+          const float from = (float)(row.pos - t * 128 - 32 * k);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) y[j] = fmaf(-slope2, fabsf(from - (float)j), y[j] * c);
+        }
+        if (cls == 2u) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) y[j] = (bits[k] >> j) & 1u ? y[j] : -INFINITY;
+        }
+#pragma unroll
+        for (int j = 0; j < 32; ++j) top[j & 3] = fmaxf(top[j & 3], y[j]);
+        if (CAP || BIAS || cls == 2u) b200_tmem_st32(mine + 32 * k, (const unsigned int*)y);
+      }
+      if (CAP || BIAS || cls == 2u) tmem_wait_st();
+      b200_tmem_ld32(mine, (unsigned int*)x[0]);
+      const float m_tile = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * unit;
+      // the maximum in use moves when some row of the warp has outgrown it (or has had none)
+      if (__any_sync(0xffffffffu, m_tile > m + 8.f || (m == -INFINITY && m_tile != -INFINITY))) {
+        const float m_new = fmaxf(m, m_tile);
+        const float by = m == -INFINITY ? 0.f : ex2(m - m_new);
+        if (seen) {
+#pragma unroll
+          for (int e = 0; e < DP; e += 32) {
+            float o[32];
+            b200_tmem_ld32(mine_o + e, (unsigned int*)o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] = by == 0.f ? 0.f : o[j] * by;
+            b200_tmem_st32(mine_o + e, (unsigned int*)o);
+          }
+        }
+        l *= by;
+        m = m_new;
+      }
+      const float off = m == -INFINITY ? 0.f : -m;
+      float part[4] = {0.f, 0.f, 0.f, 0.f};
+      // second pass: the weights, over the scores that have been read
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float* y = x[k & 1];
+        tmem_wait_ld();
+        if (k < 3) b200_tmem_ld32(mine + 32 * (k + 1), (unsigned int*)x[(k + 1) & 1]);
+        unsigned int w[16];
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) {
+          const float p0 = ex2(fmaf(y[j], unit, off)), p1 = ex2(fmaf(y[j + 1], unit, off));
+          part[j & 2] += p0;
+          part[(j & 2) + 1] += p1;
+          w[j / 2] = pack2(p0, p1, T());
+        }
+        tmem_st16(mine + 16 * k, w);
+      }
+      l += (part[0] + part[1]) + (part[2] + part[3]);
+      tmem_wait_st();
+      tc_before();
+      b200_mbar_arrive(bar_p + 8 * g);
+      ++seen;
+    }
+    // ---------------------------------------------------------------- output
+    if (live && seen) live = b200_wait(bar_o + 8 * g, 0u, abort_flag, a.status, 29u);
+    tc_after();
+    const float by = l > 0.f || l != l ? 1.f / l : 0.f;
+    float bad = 0.f;
+    unsigned char* tile = gen + g * Sh::kTile;     // the queries' tile: its last product is done
+    const unsigned int in = (warp & 3u) * 32 + lane;
+#pragma unroll
+    for (int e = 0; e < DP; e += 32) {
+      float o[32];
+      if (live && seen) {
+        b200_tmem_ld32(mine_o + e, (unsigned int*)o);
+        tmem_wait_ld();
+      }
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        o[j] = by == 0.f ? 0.f : o[j] * by;
+        bad = fmaf(o[j], 0.f, bad);
+      }
+      unsigned char* line = tile + (e >> 6) * kTileBytes64 + in * 128;
+      const unsigned int piece0 = (e & 63) >> 3;
+#pragma unroll
+      for (int p = 0; p < 4; ++p)
+        *(uint4*)(line + (((piece0 + p) ^ (in & 7u)) << 4)) =
+            make_uint4(pack2(o[8 * p], o[8 * p + 1], T()), pack2(o[8 * p + 2], o[8 * p + 3], T()), pack2(o[8 * p + 4], o[8 * p + 5], T()), pack2(o[8 * p + 6], o[8 * p + 7], T()));
+    }
+    const bool mend = live && r < a.S && bad != 0.f;     // (NaN)
+    if (mend) repair[g] = 1u;
+    if (live && r < a.S && a.lse) a.lse[((long long)b * a.H + h) * a.S + r] = l > 0.f || l != l ? (m + log2f(l)) * kLn2 : -INFINITY;
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    named_barrier(1 + (int)g, 128);
+    if ((threadIdx.x & 127u) == 0 && live) {
+#pragma unroll
+      for (int p = 0; p < Sh::kPanels; ++p)
+        if (p * 64 < a.D && r0 + 128 * (int)g < a.S) b200_tma_store_4d(&map_o, b200_smem_addr(tile) + p * kTileBytes64, p * 64, r0 + 128 * (int)g, h, b);
+      if (repair[g]) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+      else b200_tma_store_read_wait<0>();
+    }
+    if (repair[g]) {
+      named_barrier(1 + (int)g, 128);
+      for (unsigned int todo = __ballot_sync(0xffffffffu, mend); todo; todo &= todo - 1) attn_forward_row<T>(a, b, h, r0 + (int)(warp * 32) + __ffs(todo) - 1, lane);
+    }
+  }
+  // ------------------------------------------------------------------ teardown
+  __syncwarp();
+  if (*abort_flag) {
+    const unsigned long long t0 = b200_now_ns();
+    while (b200_now_ns() - t0 < 200000ull) __nanosleep(1000);
+  }
+  tc_before();
+  __syncthreads();
+  if (warp == kMma) {
+    tc_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Sh::kColumns) : "memory");
+  }
+}
+
+}  // namespace b200
+#endif

@@ -1,0 +1,520 @@
+// Layer norm of the rows of a [rows, n] node, and its gradients.
+//
+//   forward    h = x + r;  mean = sum(h) / n;  rstd = 1 / sqrt(sum((h - mean)^2) / n + eps)
+//              y = (h - mean) * rstd * gamma + beta
+//   gradients  u = (h - mean) * rstd;  g = dy * gamma
+//              dx = rstd * (g - sum(g) / n - u * sum(g * u) / n) (+ dh);  dgamma = sum_rows(dy * u);  dbeta = sum_rows(dy)
+//
+// Both are bound by memory: every plane of the rows crosses it once.  A group of 8, 32, 128 or 512 threads keeps its row in
+// registers, at most 16 elements a thread, so that the squares of the distances from the mean are summed in a second pass over
+// registers (no difference of large sums).  The groups stride over the rows; the scale and the shift stay in registers, and
+// so do, in the gradient, a thread's sums over the rows of its columns, which meet in shared memory once per block and then in a
+// second kernel that adds the blocks' partial sums in their order: the same bits every time.  Rows of more than 8192 elements
+// are read again for each pass, by 1024 threads (they come from L2 then), their column sums by a kernel of its own.
+#include "kernels/op_common.cuh"
+#include "operators.hpp"
+
+using namespace b200;
+
+namespace {
+
+struct NormArgs {
+  const void *x, *r, *gamma, *beta, *dy, *dh;
+  void *y, *h, *dx;
+  float *mean, *rstd;              // written by the forward pass, read by the gradient
+  float *partial;                  // gradient: [2][blocks][n]
+  unsigned long long rows;
+  unsigned int n;
+  int weight_f32;                  // gamma and beta in single precision, or in the rows' type
+  float eps, inv_n;
+};
+
+constexpr unsigned int kBlock = 256;
+
+template <class T>
+__device__ __forceinline__ float weight_at(const void* p, int f32, unsigned int i, float otherwise) {
+  if (!p) return otherwise;
+  return f32 ? ((const float*)p)[i] : to_float(((const T*)p)[i]);
+}
+
+// Sums of K values over the TPR threads of a row.  `sh`: [2][K][threads / 32], the halves used in turn, so that one barrier a
+// sum is enough.
+template <int TPR, int K>
+__device__ __forceinline__ void row_sum(float (&v)[K], float* sh, int half) {
+  constexpr int W = TPR < 32 ? TPR : 32;
+#pragma unroll
+  for (int o = W / 2; o > 0; o >>= 1)
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+  if constexpr (TPR > 32) {
+    const unsigned int warps = blockDim.x / 32, warp = threadIdx.x / 32, first = threadIdx.x / TPR * (TPR / 32);
+    float* s = sh + half * K * 32;
+    if ((threadIdx.x & 31u) == 0)
+#pragma unroll
+      for (int k = 0; k < K; ++k) s[k * 32 + warp] = v[k];
+    __syncthreads();
+    (void)warps;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      float t = 0.f;
+#pragma unroll
+      for (int w = 0; w < TPR / 32; ++w) t += s[k * 32 + first + w];
+      v[k] = t;
+    }
+  }
+}
+
+template <class T, int VEC, int NV, int TPR>
+__global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_rows(const NormArgs a) {
+  constexpr int E = NV * VEC;
+  __shared__ float sh[2 * 32];
+  grid_begin();
+  const unsigned int t = threadIdx.x % TPR, sub = threadIdx.x / TPR, per_block = blockDim.x / TPR;
+  float ga[E], be[E];
+#pragma unroll
+  for (int c = 0; c < NV; ++c)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const unsigned int e = (c * TPR + t) * VEC + i;
+      ga[c * VEC + i] = e < a.n ? weight_at<T>(a.gamma, a.weight_f32, e, 1.f) : 0.f;
+      be[c * VEC + i] = e < a.n ? weight_at<T>(a.beta, a.weight_f32, e, 0.f) : 0.f;
+    }
+  for (unsigned long long first = (unsigned long long)blockIdx.x * per_block; first < a.rows; first += (unsigned long long)gridDim.x * per_block) {
+    const unsigned long long row = first + sub;
+    const bool on = row < a.rows;
+    const unsigned long long at = row * a.n;
+    float h[E];
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+      const unsigned int e = (c * TPR + t) * VEC;
+      const bool ok = on && e < a.n;
+      float v[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[i] = 0.f;
+      if (ok) Vec<T, VEC>::load((const T*)a.x + at + e, v);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) h[c * VEC + i] = v[i];
+    }
+    if (a.r) {
+#pragma unroll
+      for (int c = 0; c < NV; ++c) {
+        const unsigned int e = (c * TPR + t) * VEC;
+        if (!(on && e < a.n)) continue;
+        float v[VEC];
+        Vec<T, VEC>::load((const T*)a.r + at + e, v);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) h[c * VEC + i] += v[i];
+      }
+    }
+    float s[1] = {0.f};
+#pragma unroll
+    for (int i = 0; i < E; ++i) s[0] += h[i];
+    row_sum<TPR>(s, sh, 0);
+    const float mean = s[0] * a.inv_n;
+    float q[1] = {0.f};
+#pragma unroll
+    for (int c = 0; c < NV; ++c)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const float d = (c * TPR + t) * VEC + i < a.n ? h[c * VEC + i] - mean : 0.f;
+        q[0] = fmaf(d, d, q[0]);
+      }
+    row_sum<TPR>(q, sh, 1);
+    const float rstd = 1.f / sqrtf(fmaf(q[0], a.inv_n, a.eps));
+    if (!on) continue;
+    if (t == 0) {
+      if (a.mean) a.mean[row] = mean;
+      if (a.rstd) a.rstd[row] = rstd;
+    }
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+      const unsigned int e = (c * TPR + t) * VEC;
+      if (e >= a.n) continue;
+      float v[VEC];
+      if (a.h) Vec<T, VEC>::store((T*)a.h + at + e, h + c * VEC);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[i] = fmaf((h[c * VEC + i] - mean) * rstd, ga[c * VEC + i], be[c * VEC + i]);
+      Vec<T, VEC>::store((T*)a.y + at + e, v);
+    }
+  }
+}
+
+template <class T, int VEC, int NV, int TPR>
+__global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_grad_rows(const NormArgs a) {
+  constexpr int E = NV * VEC;
+  __shared__ float sh[2 * 2 * 32];
+  extern __shared__ float columns[];        // [2][rows of the block at a time][n]
+  grid_begin();
+  const unsigned int t = threadIdx.x % TPR, sub = threadIdx.x / TPR, per_block = blockDim.x / TPR;
+  float ga[E], dg[E], db[E];
+#pragma unroll
+  for (int c = 0; c < NV; ++c)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const unsigned int e = (c * TPR + t) * VEC + i;
+      ga[c * VEC + i] = e < a.n ? weight_at<T>(a.gamma, a.weight_f32, e, 1.f) : 0.f;
+      dg[c * VEC + i] = db[c * VEC + i] = 0.f;
+    }
+  int half = 0;
+  for (unsigned long long first = (unsigned long long)blockIdx.x * per_block; first < a.rows; first += (unsigned long long)gridDim.x * per_block) {
+    const unsigned long long row = first + sub;
+    const bool on = row < a.rows;
+    const unsigned long long at = row * a.n;
+    float u[E], dy[E];
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+      const unsigned int e = (c * TPR + t) * VEC;
+      float v[VEC], w[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[i] = w[i] = 0.f;
+      if (on && e < a.n) {
+        Vec<T, VEC>::load((const T*)a.x + at + e, v);
+        Vec<T, VEC>::load((const T*)a.dy + at + e, w);
+      }
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) { u[c * VEC + i] = v[i]; dy[c * VEC + i] = w[i]; }
+    }
+    const float mean = on ? a.mean[row] : 0.f, rstd = on ? a.rstd[row] : 0.f;
+    float s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < NV; ++c)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const int k = c * VEC + i;
+        u[k] = on && (c * TPR + t) * VEC + i < a.n ? (u[k] - mean) * rstd : 0.f;
+        const float g = dy[k] * ga[k];
+        s[0] += g;
+        s[1] = fmaf(g, u[k], s[1]);
+        dg[k] = fmaf(dy[k], u[k], dg[k]);
+        db[k] += dy[k];
+      }
+    row_sum<TPR>(s, sh, half);
+    half ^= 1;
+    if (!on) continue;
+    const float m0 = s[0] * a.inv_n, m1 = s[1] * a.inv_n;
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+      const unsigned int e = (c * TPR + t) * VEC;
+      if (e >= a.n) continue;
+      float v[VEC], w[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) w[i] = 0.f;
+      if (a.dh) Vec<T, VEC>::load((const T*)a.dh + at + e, w);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const int k = c * VEC + i;
+        v[i] = fmaf(rstd, dy[k] * ga[k] - m0 - u[k] * m1, w[i]);
+      }
+      Vec<T, VEC>::store((T*)a.dx + at + e, v);
+    }
+  }
+  if (!a.partial) return;
+  // the block's groups of threads meet: columns[which][group][column]
+  const unsigned int plane = per_block * a.n;
+  if (per_block > 1) {
+#pragma unroll
+    for (int c = 0; c < NV; ++c)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const unsigned int e = (c * TPR + t) * VEC + i;
+        if (e >= a.n) continue;
+        columns[sub * a.n + e] = dg[c * VEC + i];
+        columns[plane + sub * a.n + e] = db[c * VEC + i];
+      }
+    __syncthreads();
+    for (unsigned int e = threadIdx.x; e < 2 * a.n; e += blockDim.x) {
+      const unsigned int which = e >= a.n, col = e - which * a.n;
+      float v = 0.f;
+      for (unsigned int g = 0; g < per_block; ++g) v += columns[which * plane + g * a.n + col];
+      a.partial[((unsigned long long)which * gridDim.x + blockIdx.x) * a.n + col] = v;
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < NV; ++c)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const unsigned int e = (c * TPR + t) * VEC + i;
+        if (e >= a.n) continue;
+        a.partial[(unsigned long long)blockIdx.x * a.n + e] = dg[c * VEC + i];
+        a.partial[((unsigned long long)gridDim.x + blockIdx.x) * a.n + e] = db[c * VEC + i];
+      }
+  }
+}
+
+// ---- rows of more than 8192 elements: a block of 1024 threads each, read again for every pass
+template <class T, int VEC>
+__global__ void __launch_bounds__(1024) norm_wide(const NormArgs a) {
+  __shared__ float sh[2 * 32];
+  grid_begin();
+  for (unsigned long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const T *x = (const T*)a.x + row * a.n, *r = a.r ? (const T*)a.r + row * a.n : nullptr;
+    auto load = [&](unsigned int e, float* v) {
+      Vec<T, VEC>::load(x + e, v);
+      if (r) {
+        float w[VEC];
+        Vec<T, VEC>::load(r + e, w);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[i] += w[i];
+      }
+    };
+    float s[1] = {0.f}, q[1] = {0.f};
+    for (unsigned int e = threadIdx.x * VEC; e < a.n; e += 1024 * VEC) {
+      float v[VEC];
+      load(e, v);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) s[0] += v[i];
+    }
+    row_sum<1024>(s, sh, 0);
+    const float mean = s[0] * a.inv_n;
+    for (unsigned int e = threadIdx.x * VEC; e < a.n; e += 1024 * VEC) {
+      float v[VEC];
+      load(e, v);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) q[0] = fmaf(v[i] - mean, v[i] - mean, q[0]);
+    }
+    row_sum<1024>(q, sh, 1);
+    const float rstd = 1.f / sqrtf(fmaf(q[0], a.inv_n, a.eps));
+    if (threadIdx.x == 0) {
+      if (a.mean) a.mean[row] = mean;
+      if (a.rstd) a.rstd[row] = rstd;
+    }
+    for (unsigned int e = threadIdx.x * VEC; e < a.n; e += 1024 * VEC) {
+      float v[VEC];
+      load(e, v);
+      if (a.h) Vec<T, VEC>::store((T*)a.h + row * a.n + e, v);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i)
+        v[i] = fmaf((v[i] - mean) * rstd, weight_at<T>(a.gamma, a.weight_f32, e + i, 1.f), weight_at<T>(a.beta, a.weight_f32, e + i, 0.f));
+      Vec<T, VEC>::store((T*)a.y + row * a.n + e, v);
+    }
+  }
+}
+
+template <class T, int VEC>
+__global__ void __launch_bounds__(1024) norm_grad_wide(const NormArgs a) {
+  __shared__ float sh[2 * 2 * 32];
+  grid_begin();
+  int half = 0;
+  for (unsigned long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const unsigned long long at = row * a.n;
+    const float mean = a.mean[row], rstd = a.rstd[row];
+    float s[2] = {0.f, 0.f};
+    for (unsigned int e = threadIdx.x * VEC; e < a.n; e += 1024 * VEC) {
+      float v[VEC], w[VEC];
+      Vec<T, VEC>::load((const T*)a.x + at + e, v);
+      Vec<T, VEC>::load((const T*)a.dy + at + e, w);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const float g = w[i] * weight_at<T>(a.gamma, a.weight_f32, e + i, 1.f);
+        s[0] += g;
+        s[1] = fmaf(g, (v[i] - mean) * rstd, s[1]);
+      }
+    }
+    row_sum<1024>(s, sh, half);
+    half ^= 1;
+    const float m0 = s[0] * a.inv_n, m1 = s[1] * a.inv_n;
+    for (unsigned int e = threadIdx.x * VEC; e < a.n; e += 1024 * VEC) {
+      float v[VEC], w[VEC], d[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) d[i] = 0.f;
+      Vec<T, VEC>::load((const T*)a.x + at + e, v);
+      Vec<T, VEC>::load((const T*)a.dy + at + e, w);
+      if (a.dh) Vec<T, VEC>::load((const T*)a.dh + at + e, d);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const float g = w[i] * weight_at<T>(a.gamma, a.weight_f32, e + i, 1.f);
+        v[i] = fmaf(rstd, g - m0 - (v[i] - mean) * rstd * m1, d[i]);
+      }
+      Vec<T, VEC>::store((T*)a.dx + at + e, v);
+    }
+  }
+}
+
+// column sums of wide rows: a thread per column, a slice of the rows per block; partial sums as above
+template <class T>
+__global__ void __launch_bounds__(256) norm_grad_columns(const NormArgs a, unsigned int slices) {
+  grid_begin();
+  const unsigned int col = blockIdx.x * 256 + threadIdx.x, slice = blockIdx.y;
+  if (col >= a.n) return;
+  const unsigned long long first = a.rows * slice / slices, last = a.rows * (slice + 1) / slices;
+  float dg = 0.f, db = 0.f;
+#pragma unroll 4
+  for (unsigned long long row = first; row < last; ++row) {
+    const float dy = to_float(((const T*)a.dy)[row * a.n + col]);
+    const float u = (to_float(((const T*)a.x)[row * a.n + col]) - a.mean[row]) * a.rstd[row];
+    dg = fmaf(dy, u, dg);
+    db += dy;
+  }
+  a.partial[(unsigned long long)slice * a.n + col] = dg;
+  a.partial[((unsigned long long)slices + slice) * a.n + col] = db;
+}
+
+// Partial sums of `blocks` blocks, added in their order: 32 columns x 32 runs of blocks, then the runs.
+__global__ void __launch_bounds__(1024) norm_grad_join(const float* partial, unsigned int blocks, unsigned int n, float* dgamma, float* dbeta) {
+  __shared__ float sh[32][33];
+  grid_begin();
+  const unsigned int col = blockIdx.x * 32 + threadIdx.x, which = blockIdx.y;
+  float* out = which ? dbeta : dgamma;
+  float v = 0.f;
+  if (out && col < n) {
+    const float* p = partial + (unsigned long long)which * blocks * n + col;
+#pragma unroll 4
+    for (unsigned int b = threadIdx.y; b < blocks; b += 32) v += p[(unsigned long long)b * n];
+  }
+  sh[threadIdx.y][threadIdx.x] = v;
+  __syncthreads();
+  if (threadIdx.y == 0 && out && col < n) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) s += sh[i][threadIdx.x];
+    out[col] = s;
+  }
+}
+
+typedef void (*NormKernel)(const NormArgs);
+
+struct NormPlan {
+  NormKernel kernel = nullptr;
+  unsigned int block = 0, tpr = 0;
+};
+
+template <class T, int VEC, int NV>
+NormPlan rows_of(bool grad, unsigned int n) {
+  const unsigned int e = VEC * NV;
+  if (n <= 8 * e) return {grad ? norm_grad_rows<T, VEC, NV, 8> : norm_rows<T, VEC, NV, 8>, kBlock, 8};
+  if (n <= 32 * e) return {grad ? norm_grad_rows<T, VEC, NV, 32> : norm_rows<T, VEC, NV, 32>, kBlock, 32};
+  if (n <= 128 * e) return {grad ? norm_grad_rows<T, VEC, NV, 128> : norm_rows<T, VEC, NV, 128>, kBlock, 128};
+  return {grad ? norm_grad_rows<T, VEC, NV, 512> : norm_rows<T, VEC, NV, 512>, 512, 512};
+}
+
+// The group of threads is the smallest that holds a row at 16 elements a thread; rows of at most half of what it holds
+// take 8 a thread.
+template <class T>
+NormPlan plan_of(bool grad, unsigned int n, bool vec) {
+  constexpr int V = 16 / (int)sizeof(T);
+  if (n > 8192) {
+    if (vec) return {grad ? norm_grad_wide<T, V> : norm_wide<T, V>, 1024, 1024};
+    return {grad ? norm_grad_wide<T, 1> : norm_wide<T, 1>, 1024, 1024};
+  }
+  if (!vec) return rows_of<T, 1, 16>(grad, n);
+  const unsigned int g = n <= 128 ? 8 : n <= 512 ? 32 : n <= 2048 ? 128 : 512;
+  return n <= g * 8 ? rows_of<T, V, 8 / V>(grad, n) : rows_of<T, V, 16 / V>(grad, n);
+}
+
+struct NormOperator : b200_operator {
+  NormArgs a = {};
+  NormPlan plan;
+  int dtype = 0;
+  bool grad = false;
+  size_t smem = 0;
+  unsigned int grid = 0, slices = 0;
+  float *dgamma = nullptr, *dbeta = nullptr;
+
+  void choose() {
+    const size_t size = dtype_bytes(dtype);
+    bool vec = (size_t)a.n * size % 16 == 0;
+    for (const void* p : {a.x, a.r, a.dy, a.dh, (const void*)a.y, (const void*)a.h, (const void*)a.dx}) vec &= ((size_t)p & 15) == 0;
+    plan = dtype == B200_F32 ? plan_of<float>(grad, a.n, vec) : dtype == B200_BF16 ? plan_of<__nv_bfloat16>(grad, a.n, vec) : plan_of<__half>(grad, a.n, vec);
+    const unsigned int per_block = plan.block / plan.tpr;
+    const bool wide = plan.tpr == 1024;
+    smem = grad && per_block > 1 ? 2 * (size_t)per_block * a.n * 4 : 0;
+    ready(plan.kernel, smem);
+    int resident = 0;
+    rt_check(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, plan.kernel, (int)plan.block, smem), "occupancy");
+    const unsigned long long blocks = (a.rows + per_block - 1) / per_block;
+    grid = (unsigned int)std::min<unsigned long long>(blocks, (unsigned long long)std::max(1, resident) * (unsigned)dev->sm_count);
+    if (grad && (dgamma || dbeta)) {
+      ready(norm_grad_join);
+      unsigned int partials = grid;
+      if (wide) {
+        // enough blocks for the machine, at least 32 rows each
+        const unsigned int across = (a.n + 255) / 256;
+        slices = (unsigned int)std::max<unsigned long long>(1, std::min<unsigned long long>(a.rows / 32, (8u * dev->sm_count + across - 1) / across));
+        partials = slices;
+        if (dtype == B200_F32) ready(norm_grad_columns<float>);
+        else if (dtype == B200_BF16) ready(norm_grad_columns<__nv_bfloat16>);
+        else ready(norm_grad_columns<__half>);
+      }
+      take_workspace((size_t)2 * std::max(1u, partials) * a.n * 4);
+      a.partial = (float*)workspace;
+    }
+  }
+
+  void run(cudaStream_t s) override {
+    if (grid) launch(plan.kernel, grid, plan.block, smem, s, a);
+    if (!a.partial) return;
+    unsigned int partials = grid;
+    if (plan.tpr == 1024 && a.rows) {
+      const dim3 g((a.n + 255) / 256, slices);
+      if (dtype == B200_F32) launch(norm_grad_columns<float>, g, 256, 0, s, a, slices);
+      else if (dtype == B200_BF16) launch(norm_grad_columns<__nv_bfloat16>, g, 256, 0, s, a, slices);
+      else launch(norm_grad_columns<__half>, g, 256, 0, s, a, slices);
+      partials = slices;
+    }
+    // (no rows: no partial sums, zeros)
+    launch(norm_grad_join, dim3((a.n + 31) / 32, 2), dim3(32, 32), 0, s, (const float*)workspace, a.rows ? partials : 0u, a.n, dgamma, dbeta);
+  }
+};
+
+void check_norm(const b200_layer_norm& p, const Operands& ops) {
+  ops.dtype(p.dtype);
+  if (p.weight_dtype != B200_F32 && p.weight_dtype != p.dtype) ops.refuse("gamma and beta are single precision or of the rows' type");
+  if (p.rows < 0 || p.n < 1 || p.n > (1ll << 30)) ops.refuse("rows must not be negative, n between 1 and 2^30");
+  if (!(p.eps >= 0.f)) ops.refuse("eps must not be negative");
+}
+
+}  // namespace
+
+extern "C" int b200_layer_norm_link(b200_dev* dev, const b200_layer_norm* p, b200_operator** out) {
+  return link_operator<NormOperator>(dev, p, out, [&](NormOperator* op) {
+    Operands ops(op, "layer_norm");
+    check_norm(*p, ops);
+    const unsigned long long count = extent_product({p->rows, p->n}, "layer_norm");
+    const size_t size = dtype_bytes(p->dtype), wsize = dtype_bytes(p->weight_dtype);
+    op->dtype = p->dtype;
+    NormArgs& a = op->a;
+    a.x = (const void*)ops.in(p->x, "x", count, size);
+    a.r = (const void*)ops.in(p->residual, "residual", count, size, false);
+    a.gamma = (const void*)ops.in(p->gamma, "gamma", p->n, wsize, false);
+    a.beta = (const void*)ops.in(p->beta, "beta", p->n, wsize, false);
+    a.y = (void*)ops.out(p->y, "y", count, size);
+    a.h = (void*)ops.out(p->total, "total", count, size, false);
+    a.mean = (float*)ops.out(p->mean, "mean", p->rows, 4, false);
+    a.rstd = (float*)ops.out(p->rstd, "rstd", p->rows, 4, false);
+    if (a.h && !a.r) ops.refuse("'total' is the sum with a residual, which is not given");
+    ops.check_overlaps();
+    a.rows = (unsigned long long)p->rows;
+    a.n = (unsigned int)p->n;
+    a.weight_f32 = p->weight_dtype == B200_F32;
+    a.eps = p->eps;
+    a.inv_n = 1.f / (float)p->n;
+    op->choose();
+  });
+}
+
+extern "C" int b200_layer_norm_grad_link(b200_dev* dev, const b200_layer_norm* p, b200_operator** out) {
+  return link_operator<NormOperator>(dev, p, out, [&](NormOperator* op) {
+    Operands ops(op, "layer_norm_grad");
+    check_norm(*p, ops);
+    const unsigned long long count = extent_product({p->rows, p->n}, "layer_norm_grad");
+    const size_t size = dtype_bytes(p->dtype), wsize = dtype_bytes(p->weight_dtype);
+    op->dtype = p->dtype;
+    op->grad = true;
+    NormArgs& a = op->a;
+    a.x = (const void*)ops.in(p->x, "x", count, size);
+    a.gamma = (const void*)ops.in(p->gamma, "gamma", p->n, wsize, false);
+    a.mean = (float*)ops.in(p->mean, "mean", p->rows, 4);
+    a.rstd = (float*)ops.in(p->rstd, "rstd", p->rows, 4);
+    a.dy = (const void*)ops.in(p->dy, "dy", count, size);
+    a.dh = (const void*)ops.in(p->d_total, "d_total", count, size, false);
+    a.dx = (void*)ops.out(p->dx, "dx", count, size);
+    op->dgamma = (float*)ops.out(p->dgamma, "dgamma", p->n, 4, false);
+    op->dbeta = (float*)ops.out(p->dbeta, "dbeta", p->n, 4, false);
+    ops.check_overlaps();
+    a.rows = (unsigned long long)p->rows;
+    a.n = (unsigned int)p->n;
+    a.weight_f32 = p->weight_dtype == B200_F32;
+    a.inv_n = 1.f / (float)p->n;
+    op->choose();
+  });
+}
