@@ -70,6 +70,7 @@ def build_library(verbose=False) -> str:
             subprocess.run(cmd, check=True)
         objs.append(o)
     # translation units that hold ahead-of-time kernels: nvcc, sm_100a only
+    hdrs += [os.path.join(CSRC, "kernels", h) for h in os.listdir(os.path.join(CSRC, "kernels")) if h.endswith(".cuh")]
     for s in CUDA_SOURCES:
         src = os.path.join(CSRC, s)
         o = os.path.join(OUT, s[:-3] + ".o")

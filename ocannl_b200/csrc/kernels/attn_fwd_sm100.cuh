@@ -411,7 +411,8 @@ attn_forward_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant__
       ++seen;
     }
     // ---------------------------------------------------------------- output
-    if (live && seen) live = b200_wait(bar_o + 8 * g, 0u, abort_flag, a.status, 29u);
+    // (the output goes through the queries' tile, which has to have arrived even where nobody reads it)
+    if (live) live = b200_wait(seen ? bar_o + 8 * g : bar_q, 0u, abort_flag, a.status, 29u);
     tc_after();
     const float by = l > 0.f || l != l ? 1.f / l : 0.f;
     float bad = 0.f;

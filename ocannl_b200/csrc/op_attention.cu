@@ -132,7 +132,7 @@ struct AttnOperator : b200_operator {
     head = a.D;
     for (int i = 0; i < 4; ++i) ready(kernel(i));
     ready(attn_copy_rows);
-    tc = false;
+    tc = dtype != B200_F32 && rows && key_rows && !grad;
     if (grad) {
       take_workspace((size_t)rows * 4);
       a.delta = (float*)workspace;
