@@ -1,0 +1,682 @@
+// The gradients of attention for 16-bit heads on the tensor cores.
+//
+// Two kernels, each of which owns its outputs and adds to them in a fixed order (no atomic additions: the same bits every time), at
+// the price of forming the scores and their gradients twice: seven products a pair of tiles instead of five.
+//
+//   keys     a CTA has 128 keys of one key head and walks the tiles of 128 queries that see them, of all query heads it
+//            serves.  s^T = k q^T and dp^T = v do^T have a thread per key; p^T and ds^T go back to tensor memory in 16 bits, as the
+//            A operand of dv += p^T do and dk += ds^T q.
+//   queries  a CTA has 128 queries of one head and walks the tiles of keys they see: s = q k^T, dp = do v^T, dq += ds k.
+//
+// Eight warps do the arithmetic, two threads a row, 64 columns each; one warp copies, one issues the products.  Weights are
+// formed while the second product runs, the score gradients while the next tile's scores are: with 512 columns of tensor memory
+// in use a CTA has an SM to itself.
+#ifndef B200_ATTN_BWD_SM100_CUH
+#define B200_ATTN_BWD_SM100_CUH
+#include "attn_fwd_sm100.cuh"
+
+namespace b200 {
+
+template <int DP>
+struct BwdShape {
+  static constexpr int kPanels = DP / 64;
+  static constexpr unsigned int kTile = kPanels * kTileBytes64;
+  static constexpr unsigned int kThreads = 320;
+  static constexpr unsigned int kStage = 2 * kTile + 1024;        // two tiles, and a tile of row statistics
+  static constexpr unsigned int kBytes = 2 * kTile + 2 * kStage;
+  static constexpr size_t smem(int tiles) { return 1024 + kBytes + 256 + (size_t)tiles; }
+};
+
+// Half gradients of scores are multiplied by a power of two before they are rounded, so that those of 2^-20 of the largest
+// row of d_out still lie in the normal range: 2^6 over the largest norm of a row of d_out (of the rows that see something).
+// `norms`: the squares of the largest norms, one a block of the statistics kernel.
+template <class T>
+__device__ __forceinline__ float gradient_unit(const AttnArgs& a, float* sh) {
+  if constexpr (std::is_same<T, __half>::value) {
+    float m = 0.f;
+    for (int i = (int)threadIdx.x; i < a.n_norms; i += (int)blockDim.x) m = fmaxf(m, a.norms[i]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if ((threadIdx.x & 31u) == 0) sh[threadIdx.x >> 5] = m;
+    __syncthreads();
+    for (unsigned int i = 0; i < blockDim.x / 32; ++i) m = fmaxf(m, sh[i]);
+    __syncthreads();
+    return m > 0.f && m < INFINITY ? exp2f(fminf(fmaxf(floorf(6.f - 0.5f * log2f(m)), -60.f), 60.f)) : 1.f;
+  }
+  return 1.f;
+}
+
+__device__ __forceinline__ void bulk_load(unsigned int dst, const void* src, unsigned int bytes, unsigned int bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
+// Which of the 64 queries from r0 see key j, a bit each (bits of queries behind the last one are of no account: their weights are zero).
+// Without documents a key is seen from one query on.
+__device__ __forceinline__ void visible_queries(const AttnArgs& a, int b, int r0, int j, unsigned int lane, unsigned int (&bits)[2]) {
+  const int len = a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
+  int first = 0;
+  if (j >= len) first = 0x7fffffff;
+  else if (a.mask == B200_MASK_CAUSAL || (a.mask == B200_MASK_PREFIX && j >= a.prefix[b])) first = max(0, j - (len - a.S));
+  int doc = 0;
+  if (a.kdoc) {
+    doc = j < a.T ? a.kdoc[(long long)b * a.T + j] : -1;
+    if (doc < 0) first = 0x7fffffff;
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int n = first - (r0 + 32 * i);     // queries of this word before the first
+    bits[i] = n <= 0 ? 0xffffffffu : n >= 32 ? 0u : 0xffffffffu << n;
+  }
+  if (!a.kdoc) return;
+  int d[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = r0 + (int)lane + 32 * i;
+    d[i] = r < a.S ? a.qdoc[(long long)b * a.S + r] : -1;
+  }
+  unsigned int todo = 0xffffffffu;
+  while (todo) {
+    const int k = __shfl_sync(0xffffffffu, doc, __ffs(todo) - 1);
+    const bool mine = doc == k;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const unsigned int same = __ballot_sync(0xffffffffu, d[i] == k);
+      if (mine) bits[i] &= same;
+    }
+    todo &= ~__ballot_sync(0xffffffffu, mine);
+  }
+}
+
+// 32 accumulator columns of a row into the swizzled 16-bit tile that leaves by TMA; false where a value is infinite or undefined
+template <class T>
+__device__ __forceinline__ bool store_columns(unsigned char* tile, unsigned int in, int e, const float* o) {
+  float bad = 0.f;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) bad = fmaf(o[j], 0.f, bad);
+  unsigned char* line = tile + (e >> 6) * kTileBytes64 + in * 128;
+  const unsigned int piece0 = (e & 63) >> 3;
+#pragma unroll
+  for (int p = 0; p < 4; ++p)
+    *(uint4*)(line + (((piece0 + p) ^ (in & 7u)) << 4)) =
+        make_uint4(pack2(o[8 * p], o[8 * p + 1], T()), pack2(o[8 * p + 2], o[8 * p + 3], T()), pack2(o[8 * p + 4], o[8 * p + 5], T()), pack2(o[8 * p + 6], o[8 * p + 7], T()));
+  return bad == 0.f;
+}
+
+// Score of one pair from the product: `z` in units of log 2, `slack` = 1 - tanh^2
+template <bool CAP, bool BIAS>
+__device__ __forceinline__ float pair_score(float x, float c, float to_tanh, float slope2, float far, float& slack) {
+  if constexpr (CAP) {
+    x = tanh_of(x * to_tanh);
+    slack = fmaf(-x, x, 1.f);
+  }
+  x *= c;
+  if constexpr (BIAS) x = fmaf(-slope2, fabsf(far), x);
+  return x;
+}
+
+// ------------------------------------------------------------------ keys
+template <class T, int DP, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(320, 1)
+attn_grad_keys_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant__ b200_tmap map_k, const __grid_constant__ b200_tmap map_v,
+                  const __grid_constant__ b200_tmap map_do, const __grid_constant__ b200_tmap map_dk, const __grid_constant__ b200_tmap map_dv,
+                  const __grid_constant__ AttnArgs a) {
+  typedef BwdShape<DP> Sh;
+  extern __shared__ unsigned char dyn[];
+  const unsigned int base = (b200_smem_addr(dyn) + 1023u) & ~1023u;
+  unsigned char* const gen = dyn + (base - b200_smem_addr(dyn));
+  const unsigned int k_at = base, v_at = base + Sh::kTile, ring = base + 2 * Sh::kTile;
+  unsigned long long* bars = (unsigned long long*)(gen + Sh::kBytes);
+  const unsigned int bar0 = b200_smem_addr(bars);
+  const unsigned int bar_kv = bar0, bar_full = bar0 + 8, bar_empty = bar0 + 24;      // two each
+  const unsigned int bar_s = bar0 + 40, bar_dp = bar0 + 48, bar_p = bar0 + 56, bar_ds = bar0 + 64, bar_done = bar0 + 72;
+  volatile unsigned int* tmem_slot = (volatile unsigned int*)(bars + 10);
+  volatile unsigned int* abort_flag = tmem_slot + 1;
+  volatile unsigned int* repair = tmem_slot + 2;          // [2]: dv, dk
+  float* scratch = (float*)(bars + 12);                   // [10]
+  unsigned char* classes = (unsigned char*)(gen + Sh::kBytes + 256);
+
+  asm volatile("griddepcontrol.launch_dependents;");
+  const unsigned int warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+  if (threadIdx.x == 0) {
+    b200_mbar_init(bar_kv, 1);
+    for (int i = 0; i < 2; ++i) {
+      b200_mbar_init(bar_full + 8 * i, 1);
+      b200_mbar_init(bar_empty + 8 * i, 1);
+      repair[i] = 0u;
+    }
+    b200_mbar_init(bar_s, 1);
+    b200_mbar_init(bar_dp, 1);
+    b200_mbar_init(bar_p, 256);
+    b200_mbar_init(bar_ds, 256);
+    b200_mbar_init(bar_done, 1);
+    *abort_flag = 0u;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(b200_smem_addr((const void*)tmem_slot)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  // this CTA's keys: the first ones first, which under a causal mask are seen by the most queries
+  const unsigned int heads = (unsigned int)a.B * (unsigned int)a.HK;
+  const int j0 = (int)(blockIdx.x / heads) * 128;
+  const unsigned int bh = blockIdx.x % heads;
+  const int b = (int)(bh / (unsigned int)a.HK), hk = (int)(bh % (unsigned int)a.HK);
+  const int tiles = (a.S + 127) / 128;
+  tc_before();
+  __syncthreads();
+  tc_after();
+  const float grad_unit = gradient_unit<T>(a, scratch);
+  {
+    int kmin = 0, kmax = 0;
+    bool negative = false;
+    if (a.kdoc) key_documents(a, b, j0, lane, kmin, kmax, negative);
+    for (int t = (int)warp; t < tiles; t += 10) {
+      AttnSpan s;
+      s.last_min = s.doc_min = 0x7fffffff;
+      s.last_max = -1;
+      s.doc_max = -0x7fffffff - 1;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = t * 128 + 32 * i + (int)lane;
+        AttnRow w;
+        w.last = w.doc = 0;
+        if (r < a.S) w = attn_row(a, b, r);
+        const AttnSpan p = span_of(r < a.S, w);
+        s.last_min = min(s.last_min, p.last_min);
+        s.last_max = max(s.last_max, p.last_max);
+        s.doc_min = min(s.doc_min, p.doc_min);
+        s.doc_max = max(s.doc_max, p.doc_max);
+      }
+      if (lane == 0) classes[t] = (unsigned char)tile_class(s, j0, a.kdoc != nullptr, kmin, kmax, negative);
+    }
+  }
+  __syncthreads();
+  const unsigned int tmem = *tmem_slot;
+  const unsigned int t_s = tmem, t_dp = tmem + 128, t_dv = tmem + 256, t_dk = tmem + 256 + DP;
+
+  if (warp == 8) {
+    if (b200_elect()) {
+      b200_mbar_expect_tx(bar_kv, 2 * Sh::kTile);
+#pragma unroll
+      for (int p = 0; p < Sh::kPanels; ++p) {
+        b200_tma_load_4d(k_at + p * kTileBytes64, &map_k, bar_kv, p * 64, j0, hk, b);
+        b200_tma_load_4d(v_at + p * kTileBytes64, &map_v, bar_kv, p * 64, j0, hk, b);
+      }
+      unsigned int n = 0;
+      bool live = true;
+      for (int h = hk * a.group; h < (hk + 1) * a.group && live; ++h)
+        for (int t = 0; t < tiles; ++t) {
+          if (!classes[t]) continue;
+          const unsigned int slot = n & 1u, use = n >> 1, at = ring + slot * Sh::kStage, bar = bar_full + 8 * slot;
+          if (use) live = b200_wait(bar_empty + 8 * slot, (use - 1) & 1u, abort_flag, a.status, 31u);
+          if (!live) break;
+          b200_mbar_expect_tx(bar, Sh::kStage);
+#pragma unroll
+          for (int p = 0; p < Sh::kPanels; ++p) {
+            b200_tma_load_4d(at + p * kTileBytes64, &map_q, bar, p * 64, t * 128, h, b);
+            b200_tma_load_4d(at + Sh::kTile + p * kTileBytes64, &map_do, bar, p * 64, t * 128, h, b);
+          }
+          bulk_load(at + 2 * Sh::kTile, a.stat + (((long long)b * a.H + h) * tiles + t) * 256, 1024, bar);
+          ++n;
+        }
+      if (*abort_flag)
+        for (unsigned int i = 0; i < 2 && i < n; ++i)
+          for (int tries = 0; tries < 1 << 20 && !b200_mbar_try(bar_full + 8 * ((n - 1 - i) & 1u), ((n - 1 - i) >> 1) & 1u); ++tries) {}
+    }
+    __syncwarp();
+  } else if (warp == 9) {
+    if (b200_elect()) {
+      constexpr unsigned int idesc_s = idesc_of<T>(128, 128, false, false), idesc_g = idesc_of<T>(128, DP, false, true);
+      // 128 x 128 of two k-major tiles
+      auto square = [&](unsigned int d, unsigned int x, unsigned int y) {
+#pragma unroll
+        for (int p = 0; p < Sh::kPanels; ++p) {
+          const unsigned long long dx = b200_smem_desc(x + p * kTileBytes64, 16u, 1024u), dy = b200_smem_desc(y + p * kTileBytes64, 16u, 1024u);
+#pragma unroll
+          for (unsigned int ks = 0; ks < 4; ++ks) b200_umma(d, dx + ks * 2, dy + ks * 2, idesc_s, (p || ks) ? 1u : 0u);
+        }
+      };
+      // += (16-bit rows in tensor memory, the halves 64 columns apart) x (tile read along its rows)
+      auto product = [&](unsigned int d, unsigned int x, unsigned int y, bool add) {
+        const unsigned long long dy = b200_smem_desc(y, kTileBytes64, 1024u);
+#pragma unroll
+        for (unsigned int ks = 0; ks < 8; ++ks) umma_ts(d, x + (ks >> 2) * 64 + (ks & 3u) * 8, dy + ks * 128, idesc_g, (add || ks) ? 1u : 0u);
+      };
+      int total = 0;
+      for (int t = 0; t < tiles; ++t) total += classes[t] != 0;
+      total *= a.group;
+      bool live = b200_wait(bar_kv, 0u, abort_flag, a.status, 32u);
+      if (live && total) {
+        live = b200_wait(bar_full, 0u, abort_flag, a.status, 33u);
+        tc_after();
+        if (live) {
+          square(t_s, k_at, ring);
+          b200_umma_commit(bar_s);
+          square(t_dp, v_at, ring + Sh::kTile);
+          b200_umma_commit(bar_dp);
+        }
+      }
+      for (int n = 0; live && n < total; ++n) {
+        const unsigned int at = ring + (n & 1) * Sh::kStage, next = ring + ((n + 1) & 1) * Sh::kStage;
+        live = b200_wait(bar_p, n & 1, abort_flag, a.status, 34u);
+        if (!live) break;
+        tc_after();
+        product(t_dv, t_s, at + Sh::kTile, n != 0);
+        if (n + 1 < total) {
+          live = b200_wait(bar_full + 8 * ((n + 1) & 1), ((n + 1) >> 1) & 1, abort_flag, a.status, 35u);
+          if (!live) break;
+          tc_after();
+          square(t_s, k_at, next);
+          b200_umma_commit(bar_s);
+        }
+        live = b200_wait(bar_ds, n & 1, abort_flag, a.status, 36u);
+        if (!live) break;
+        tc_after();
+        product(t_dk, t_dp, at, n != 0);
+        b200_umma_commit(bar_empty + 8 * (n & 1));
+        if (n + 1 < total) {
+          square(t_dp, v_at, next + Sh::kTile);
+          b200_umma_commit(bar_dp);
+        } else {
+          b200_umma_commit(bar_done);
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+    const unsigned int half = warp >> 2, in = (warp & 3u) * 32 + lane, lanes = (warp & 3u) << 21;
+    const unsigned int my_s = t_s + 64 * half + lanes, my_dp = t_dp + 64 * half + lanes;
+    const float c = CAP ? a.cap * kLog2e : a.scale * kLog2e, to_tanh = CAP ? 2.f * kLog2e * a.scale / a.cap : 0.f;
+    const int j = j0 + (int)in;
+    const int len = a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
+    unsigned int n = 0;
+    bool live = true;
+    for (int h = hk * a.group; h < (hk + 1) * a.group && live; ++h) {
+      const float slope2 = BIAS ? a.slopes[h] * kLog2e : 0.f;
+      for (int t = 0; t < tiles; ++t) {
+        const unsigned int cls = classes[t];
+        if (!cls) continue;
+        const float* stat = (const float*)(gen + 2 * Sh::kTile + (n & 1u) * Sh::kStage + 2 * Sh::kTile) + 64 * half;
+        unsigned int bits[2] = {0xffffffffu, 0xffffffffu};
+        const int r0 = t * 128 + 64 * (int)half;
+        if (cls == 2u) visible_queries(a, b, r0, j, lane, bits);
+        live = b200_wait(bar_full + 8 * (n & 1u), (n >> 1) & 1u, abort_flag, a.status, 37u) && b200_wait(bar_s, n & 1u, abort_flag, a.status, 38u);
+        if (!live) break;
+        tc_after();
+        float w[64];            // weights, times 1 - tanh^2 with a cap
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          float x[32];
+          unsigned int u[16];
+          b200_tmem_ld32(my_s + 32 * k, (unsigned int*)x);
+          const float far = BIAS ? (float)(len - a.S + r0 + 32 * k - j) : 0.f;
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            const float4 l = *(const float4*)(stat + 32 * k + i);
+            const float lse2[4] = {l.x, l.y, l.z, l.w};
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              float slack = 1.f, p;
+              if constexpr (!CAP && !BIAS) p = ex2(fmaf(x[i + q], c, -lse2[q]));
+              else p = ex2(pair_score<CAP, BIAS>(x[i + q], c, to_tanh, slope2, far + (float)(i + q), slack) - lse2[q]);
+              if (cls == 2u) p = (bits[k] >> (i + q)) & 1u ? p : 0.f;
+              x[i + q] = p;
+              w[32 * k + i + q] = CAP ? p * slack : p;
+            }
+            u[i / 2] = pack2(x[i], x[i + 1], T());
+            u[i / 2 + 1] = pack2(x[i + 2], x[i + 3], T());
+          }
+          tmem_st16(my_s + 16 * k, u);
+        }
+        tmem_wait_st();
+        tc_before();
+        b200_mbar_arrive(bar_p);
+        live = b200_wait(bar_dp, n & 1u, abort_flag, a.status, 39u);
+        if (!live) break;
+        tc_after();
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          float x[32];
+          unsigned int u[16];
+          b200_tmem_ld32(my_dp + 32 * k, (unsigned int*)x);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            const float4 l = *(const float4*)(stat + 128 + 32 * k + i);
+            const float delta[4] = {l.x, l.y, l.z, l.w};
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              float ds = w[32 * k + i + q] * (x[i + q] - delta[q]);
+              if constexpr (std::is_same<T, __half>::value) ds *= grad_unit;
+              if (cls == 2u) ds = (bits[k] >> (i + q)) & 1u ? ds : 0.f;
+              x[i + q] = ds;
+            }
+            u[i / 2] = pack2(x[i], x[i + 1], T());
+            u[i / 2 + 1] = pack2(x[i + 2], x[i + 3], T());
+          }
+          tmem_st16(my_dp + 16 * k, u);
+        }
+        tmem_wait_st();
+        tc_before();
+        b200_mbar_arrive(bar_ds);
+        ++n;
+      }
+    }
+    // ---- dv by the first four warps, dk by the others, through the tiles of v and k
+    if (live) live = b200_wait(n ? bar_done : bar_kv, 0u, abort_flag, a.status, 40u);
+    tc_after();
+    const unsigned int from = (half ? t_dk : t_dv) + lanes;
+    unsigned char* tile = gen + (half ? 0 : Sh::kTile);
+    const float by = half ? a.scale / grad_unit : 1.f;
+    bool fine = true;
+#pragma unroll
+    for (int e = 0; e < DP; e += 32) {
+      float o[32];
+      if (live && n) {
+        b200_tmem_ld32(from + e, (unsigned int*)o);
+        tmem_wait_ld();
+      }
+#pragma unroll
+      for (int i = 0; i < 32; ++i) o[i] = n ? o[i] * by : 0.f;
+      fine &= store_columns<T>(tile, in, e, o);
+    }
+    const bool mend = live && j < a.T && !fine;
+    if (mend) repair[half] = 1u;
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    named_barrier(1 + (int)half, 128);
+    if ((threadIdx.x & 127u) == 0 && live) {
+#pragma unroll
+      for (int p = 0; p < Sh::kPanels; ++p)
+        if (p * 64 < a.D) b200_tma_store_4d(half ? &map_dk : &map_dv, b200_smem_addr(tile) + p * kTileBytes64, p * 64, j0, hk, b);
+      if (repair[half]) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+      else b200_tma_store_read_wait<0>();
+    }
+    if (repair[half]) {
+      named_barrier(1 + (int)half, 128);
+      for (unsigned int todo = __ballot_sync(0xffffffffu, mend); todo; todo &= todo - 1)
+        attn_dkv_row<T>(a, b, hk, j0 + (int)((warp & 3u) * 32) + __ffs(todo) - 1, lane, half ? 1 : 2);
+    }
+  }
+  __syncwarp();
+  if (*abort_flag) {
+    const unsigned long long t0 = b200_now_ns();
+    while (b200_now_ns() - t0 < 200000ull) __nanosleep(1000);
+  }
+  tc_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  }
+}
+
+// ------------------------------------------------------------------ queries
+template <class T, int DP, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(320, 1)
+attn_grad_queries_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant__ b200_tmap map_k, const __grid_constant__ b200_tmap map_v,
+                     const __grid_constant__ b200_tmap map_do, const __grid_constant__ b200_tmap map_dq, const __grid_constant__ AttnArgs a) {
+  typedef BwdShape<DP> Sh;
+  extern __shared__ unsigned char dyn[];
+  const unsigned int base = (b200_smem_addr(dyn) + 1023u) & ~1023u;
+  unsigned char* const gen = dyn + (base - b200_smem_addr(dyn));
+  const unsigned int q_at = base, do_at = base + Sh::kTile, ring = base + 2 * Sh::kTile;
+  unsigned long long* bars = (unsigned long long*)(gen + Sh::kBytes);
+  const unsigned int bar0 = b200_smem_addr(bars);
+  const unsigned int bar_q = bar0, bar_full = bar0 + 8, bar_empty = bar0 + 24, bar_s = bar0 + 40;      // two each but bar_q
+  const unsigned int bar_dp = bar0 + 56, bar_ds = bar0 + 64, bar_done = bar0 + 72;
+  volatile unsigned int* tmem_slot = (volatile unsigned int*)(bars + 10);
+  volatile unsigned int* abort_flag = tmem_slot + 1;
+  volatile unsigned int* repair = tmem_slot + 2;
+  float* scratch = (float*)(bars + 12);
+  AttnSpan* span = (AttnSpan*)(bars + 18);
+  unsigned char* classes = (unsigned char*)(gen + Sh::kBytes + 256);
+
+  asm volatile("griddepcontrol.launch_dependents;");
+  const unsigned int warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+  if (threadIdx.x == 0) {
+    b200_mbar_init(bar_q, 1);
+    for (int i = 0; i < 2; ++i) {
+      b200_mbar_init(bar_full + 8 * i, 1);
+      b200_mbar_init(bar_empty + 8 * i, 1);
+      b200_mbar_init(bar_s + 8 * i, 1);
+    }
+    b200_mbar_init(bar_dp, 1);
+    b200_mbar_init(bar_ds, 256);
+    b200_mbar_init(bar_done, 1);
+    *repair = 0u;
+    span->last_min = span->doc_min = 0x7fffffff;
+    span->last_max = -1;
+    span->doc_max = -0x7fffffff - 1;
+    *abort_flag = 0u;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(b200_smem_addr((const void*)tmem_slot)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  const unsigned int heads = (unsigned int)a.B * (unsigned int)a.H;
+  const int tiles_q = (a.S + 127) / 128;
+  const int t_q = tiles_q - 1 - (int)(blockIdx.x / heads), r0 = t_q * 128;
+  const unsigned int bh = blockIdx.x % heads;
+  const int b = (int)(bh / (unsigned int)a.H), h = (int)(bh % (unsigned int)a.H), hk = h / a.group;
+  const unsigned int half = warp >> 2, in = (warp & 3u) * 32 + lane;
+  const int r = r0 + (int)in;
+  AttnRow row;
+  row.pos = 0; row.last = -1; row.doc = 0;
+  tc_before();
+  __syncthreads();
+  tc_after();
+  const float grad_unit = gradient_unit<T>(a, scratch);
+  if (warp < 8) {
+    if (r < a.S) row = attn_row(a, b, r);
+    const AttnSpan s = span_of(r < a.S, row);
+    if (lane == 0) {
+      atomicMin(&span->last_min, s.last_min);
+      atomicMax(&span->last_max, s.last_max);
+      atomicMin(&span->doc_min, s.doc_min);
+      atomicMax(&span->doc_max, s.doc_max);
+    }
+  }
+  __syncthreads();
+  const int tiles = (span->last_max + 128) / 128;
+  for (int t = (int)warp; t < tiles; t += 10) {
+    int kmin = 0, kmax = 0;
+    bool negative = false;
+    if (a.kdoc) key_documents(a, b, t * 128, lane, kmin, kmax, negative);
+    const unsigned int cls = tile_class(*span, t * 128, a.kdoc != nullptr, kmin, kmax, negative);
+    if (lane == 0) classes[t] = (unsigned char)cls;
+  }
+  __syncthreads();
+  const unsigned int tmem = *tmem_slot;
+  const unsigned int t_dp = tmem + 256, t_dq = tmem + 384;     // two tiles of scores ahead of them
+
+  if (warp == 8) {
+    if (b200_elect()) {
+      b200_mbar_expect_tx(bar_q, 2 * Sh::kTile);
+#pragma unroll
+      for (int p = 0; p < Sh::kPanels; ++p) {
+        b200_tma_load_4d(q_at + p * kTileBytes64, &map_q, bar_q, p * 64, r0, h, b);
+        b200_tma_load_4d(do_at + p * kTileBytes64, &map_do, bar_q, p * 64, r0, h, b);
+      }
+      unsigned int n = 0;
+      bool live = true;
+      for (int t = 0; t < tiles; ++t) {
+        if (!classes[t]) continue;
+        const unsigned int slot = n & 1u, use = n >> 1, at = ring + slot * Sh::kStage, bar = bar_full + 8 * slot;
+        if (use) live = b200_wait(bar_empty + 8 * slot, (use - 1) & 1u, abort_flag, a.status, 41u);
+        if (!live) break;
+        b200_mbar_expect_tx(bar, 2 * Sh::kTile);
+#pragma unroll
+        for (int p = 0; p < Sh::kPanels; ++p) {
+          b200_tma_load_4d(at + p * kTileBytes64, &map_k, bar, p * 64, t * 128, hk, b);
+          b200_tma_load_4d(at + Sh::kTile + p * kTileBytes64, &map_v, bar, p * 64, t * 128, hk, b);
+        }
+        ++n;
+      }
+      if (*abort_flag)
+        for (unsigned int i = 0; i < 2 && i < n; ++i)
+          for (int tries = 0; tries < 1 << 20 && !b200_mbar_try(bar_full + 8 * ((n - 1 - i) & 1u), ((n - 1 - i) >> 1) & 1u); ++tries) {}
+    }
+    __syncwarp();
+  } else if (warp == 9) {
+    if (b200_elect()) {
+      constexpr unsigned int idesc_s = idesc_of<T>(128, 128, false, false), idesc_g = idesc_of<T>(128, DP, false, true);
+      auto square = [&](unsigned int d, unsigned int x, unsigned int y) {
+#pragma unroll
+        for (int p = 0; p < Sh::kPanels; ++p) {
+          const unsigned long long dx = b200_smem_desc(x + p * kTileBytes64, 16u, 1024u), dy = b200_smem_desc(y + p * kTileBytes64, 16u, 1024u);
+#pragma unroll
+          for (unsigned int ks = 0; ks < 4; ++ks) b200_umma(d, dx + ks * 2, dy + ks * 2, idesc_s, (p || ks) ? 1u : 0u);
+        }
+      };
+      int total = 0;
+      for (int t = 0; t < tiles; ++t) total += classes[t] != 0;
+      bool live = b200_wait(bar_q, 0u, abort_flag, a.status, 42u);
+      if (live && total) {
+        live = b200_wait(bar_full, 0u, abort_flag, a.status, 43u);
+        tc_after();
+        if (live) {
+          square(tmem, q_at, ring);
+          b200_umma_commit(bar_s);
+          square(t_dp, do_at, ring + Sh::kTile);
+          b200_umma_commit(bar_dp);
+        }
+      }
+      for (int n = 0; live && n < total; ++n) {
+        const unsigned int at = ring + (n & 1) * Sh::kStage, next = ring + ((n + 1) & 1) * Sh::kStage;
+        if (n + 1 < total) {
+          live = b200_wait(bar_full + 8 * ((n + 1) & 1), ((n + 1) >> 1) & 1, abort_flag, a.status, 44u);
+          if (!live) break;
+          tc_after();
+          square(tmem + 128 * ((n + 1) & 1), q_at, next);
+          b200_umma_commit(bar_s + 8 * ((n + 1) & 1));
+        }
+        live = b200_wait(bar_ds, n & 1, abort_flag, a.status, 45u);
+        if (!live) break;
+        tc_after();
+        const unsigned long long dk = b200_smem_desc(at, kTileBytes64, 1024u);
+#pragma unroll
+        for (unsigned int ks = 0; ks < 8; ++ks) umma_ts(t_dq, t_dp + (ks >> 2) * 64 + (ks & 3u) * 8, dk + ks * 128, idesc_g, (n || ks) ? 1u : 0u);
+        b200_umma_commit(bar_empty + 8 * (n & 1));
+        if (n + 1 < total) {
+          square(t_dp, do_at, next + Sh::kTile);
+          b200_umma_commit(bar_dp);
+        } else {
+          b200_umma_commit(bar_done);
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+    const unsigned int lanes = (warp & 3u) << 21;
+    const unsigned int my_dp = t_dp + 64 * half + lanes;
+    const float c = CAP ? a.cap * kLog2e : a.scale * kLog2e, to_tanh = CAP ? 2.f * kLog2e * a.scale / a.cap : 0.f;
+    const float slope2 = BIAS ? a.slopes[h] * kLog2e : 0.f;
+    const float* stat = a.stat + (((long long)b * a.H + h) * tiles_q + t_q) * 256 + in;
+    const float lse2 = stat[0], delta = stat[128];
+    unsigned int n = 0;
+    bool live = true;
+    for (int t = 0; t < tiles; ++t) {
+      const unsigned int cls = classes[t];
+      if (!cls) continue;
+      unsigned int all[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+      if (cls == 2u) visible_words(a, b, t * 128, row, lane, all);
+      const unsigned int bits[2] = {half ? all[2] : all[0], half ? all[3] : all[1]};
+      live = b200_wait(bar_s + 8 * (n & 1u), (n >> 1) & 1u, abort_flag, a.status, 46u);
+      if (!live) break;
+      tc_after();
+      float w[64];
+      const unsigned int my_s = tmem + 128 * (n & 1u) + 64 * half + lanes;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        float x[32];
+        b200_tmem_ld32(my_s + 32 * k, (unsigned int*)x);
+        const float far = BIAS ? (float)(row.pos - t * 128 - 64 * (int)half - 32 * k) : 0.f;
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          float slack = 1.f, p;
+          if constexpr (!CAP && !BIAS) p = ex2(fmaf(x[i], c, -lse2));
+          else p = ex2(pair_score<CAP, BIAS>(x[i], c, to_tanh, slope2, far - (float)i, slack) - lse2);
+          if (cls == 2u) p = (bits[k] >> i) & 1u ? p : 0.f;
+          if constexpr (std::is_same<T, __half>::value) p *= grad_unit;
+          w[32 * k + i] = CAP ? p * slack : p;
+        }
+      }
+      live = b200_wait(bar_dp, n & 1u, abort_flag, a.status, 47u);
+      if (!live) break;
+      tc_after();
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        float x[32];
+        unsigned int u[16];
+        b200_tmem_ld32(my_dp + 32 * k, (unsigned int*)x);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          x[i] = w[32 * k + i] * (x[i] - delta);
+          if (cls == 2u) x[i] = (bits[k] >> i) & 1u ? x[i] : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) u[i / 2] = pack2(x[i], x[i + 1], T());
+        tmem_st16(my_dp + 16 * k, u);
+      }
+      tmem_wait_st();
+      tc_before();
+      b200_mbar_arrive(bar_ds);
+      ++n;
+    }
+    // ---- dq through the queries' tile, half of a row's elements a thread
+    if (live) live = b200_wait(n ? bar_done : bar_q, 0u, abort_flag, a.status, 48u);
+    tc_after();
+    const float by = a.scale / grad_unit;
+    bool fine = true;
+#pragma unroll
+    for (int e = 0; e < DP / 2; e += 32) {
+      float o[32];
+      const int col = (int)half * (DP / 2) + e;
+      if (live && n) {
+        b200_tmem_ld32(t_dq + lanes + col, (unsigned int*)o);
+        tmem_wait_ld();
+      }
+#pragma unroll
+      for (int i = 0; i < 32; ++i) o[i] = n ? o[i] * by : 0.f;
+      fine &= store_columns<T>(gen, in, col, o);
+    }
+    const bool mend = live && r < a.S && !fine;
+    if (mend) *repair = 1u;
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    named_barrier(1, 256);
+    if (threadIdx.x == 0 && live) {
+#pragma unroll
+      for (int p = 0; p < Sh::kPanels; ++p)
+        if (p * 64 < a.D) b200_tma_store_4d(&map_dq, q_at + p * kTileBytes64, p * 64, r0, h, b);
+      if (*repair) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+      else b200_tma_store_read_wait<0>();
+    }
+    if (*repair) {
+      named_barrier(1, 256);
+      // (a row whose halves are both to be mended is done twice, with the same result)
+      for (unsigned int todo = __ballot_sync(0xffffffffu, mend); todo; todo &= todo - 1) attn_dq_row<T>(a, b, h, r0 + (int)((warp & 3u) * 32) + __ffs(todo) - 1, lane);
+    }
+  }
+  __syncwarp();
+  if (*abort_flag) {
+    const unsigned long long t0 = b200_now_ns();
+    while (b200_now_ns() - t0 < 200000ull) __nanosleep(1000);
+  }
+  tc_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  }
+}
+
+}  // namespace b200
+#endif

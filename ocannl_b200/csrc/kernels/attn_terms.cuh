@@ -13,7 +13,10 @@ namespace b200 {
 struct AttnArgs {
   const void *q, *k, *v, *o, *d_out;     // o: the forward pass's output, read by the gradient
   void *out, *dq, *dk, *dv;
-  float *lse, *delta;                    // [batch, heads, queries]; delta: <d_out_r, out_r>
+  float* lse;                            // [batch, heads, queries]
+  float* stat;                           // gradient: a tile of 128 queries of a head: lse / log 2 of each, then <d_out, out>
+  float* norms;                          // gradient, half: largest squares of a row of d_out, n_norms of them
+  int n_norms;
   const int *lengths, *prefix, *qdoc, *kdoc;
   const float* slopes;
   unsigned int* status;
@@ -58,6 +61,11 @@ __device__ __forceinline__ float attn_score(const AttnArgs& a, float x, float sl
     s = x * (a.scale * kLog2e);
   }
   return fmaf(-slope2, fabsf((float)(pos - j)), s);
+}
+
+// Where a row's statistics lie: its lse (log 2 units; +infinity for a row that sees nothing: all weights are zero), 128 further <d_out, out>
+__device__ __forceinline__ long long attn_stat_at(const AttnArgs& a, int b, int h, int r) {
+  return (((long long)b * a.H + h) * ((a.S + 127) / 128) + (r >> 7)) * 256 + (r & 127);
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -125,8 +133,8 @@ __device__ __noinline__ void attn_dq_row(const AttnArgs& a, int b, int h, int r,
   const AttnRow w = attn_row(a, b, r);
   const float slope2 = a.slopes ? a.slopes[h] * kLog2e : 0.f;
   const int hk = h / a.group;
-  const long long at = attn_q_at(a, b, r, h), stat = ((long long)b * a.H + h) * a.S + r;
-  const float lse2 = a.lse[stat] == -INFINITY ? 0.f : a.lse[stat] * kLog2e, delta = a.delta[stat];
+  const long long at = attn_q_at(a, b, r, h), stat = attn_stat_at(a, b, h, r);
+  const float lse2 = a.stat[stat], delta = a.stat[stat + 128];
   float q[4], k[4], v[4], go[4], g[4] = {0.f, 0.f, 0.f, 0.f}, p, dx;
   attn_load_row<T>(a, a.q, at, lane, q);
   attn_load_row<T>(a, a.d_out, at, lane, go);
@@ -155,11 +163,10 @@ __device__ __noinline__ void attn_dkv_row(const AttnArgs& a, int b, int hk, int 
     for (int r = 0; r < a.S; ++r) {
       const AttnRow w = attn_row(a, b, r);
       if (j > w.last || (a.kdoc && doc != w.doc)) continue;
-      const long long at = attn_q_at(a, b, r, h), stat = ((long long)b * a.H + h) * a.S + r;
+      const long long at = attn_q_at(a, b, r, h), stat = attn_stat_at(a, b, h, r);
       attn_load_row<T>(a, a.q, at, lane, q);
       attn_load_row<T>(a, a.d_out, at, lane, go);
-      const float lse2 = a.lse[stat] == -INFINITY ? 0.f : a.lse[stat] * kLog2e;
-      attn_pair(a, attn_dot(q, k), attn_dot(go, v), slope2, w.pos, j, lse2, a.delta[stat], p, dx);
+      attn_pair(a, attn_dot(q, k), attn_dot(go, v), slope2, w.pos, j, a.stat[stat], a.stat[stat + 128], p, dx);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         gk[i] = fmaf(dx, q[i], gk[i]);

@@ -3,6 +3,7 @@
 #include <cstring>
 
 #include "operators.hpp"
+#include "kernels/attn_bwd_sm100.cuh"
 #include "kernels/attn_fwd_sm100.cuh"
 #include "kernels/attn_terms.cuh"
 
@@ -21,20 +22,58 @@ __global__ void __launch_bounds__(256) attn_forward_rows(const __grid_constant__
     attn_forward_row<T>(a, (int)(bs / a.S), (int)(i - bs * a.H), (int)(bs % a.S), lane);
   }
 }
-// delta_r = <d_out_r, out_r>
-template <class T>
-__global__ void __launch_bounds__(256) attn_delta(const __grid_constant__ AttnArgs a) {
+// What the gradients need of every row: its lse and <d_out, out>, tile by tile of 128 queries, G threads a row.  Bound by memory: out and
+// d_out are read once.  Rows behind the last one and rows that see nothing get weights of zero.
+template <class T, int VEC, int G>
+__global__ void __launch_bounds__(256) attn_statistics(const __grid_constant__ AttnArgs a) {
+  __shared__ float sh[8];
   grid_begin();
-  const unsigned int lane = threadIdx.x & 31u;
-  const long long n = (long long)a.B * a.S * a.H;
-  for (long long i = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); i < n; i += (long long)gridDim.x * 8) {
+  const int lane = (int)threadIdx.x % G, padded = (a.S + 127) / 128 * 128;
+  const long long n = (long long)a.B * padded * a.H, step = (long long)gridDim.x * (256 / G);
+  float top = 0.f;
+  for (long long base = (long long)blockIdx.x * (256 / G); base < n; base += step) {
+    const long long i = base + threadIdx.x / G;
+    if (i >= n) continue;
     const long long bs = i / a.H;
-    const int b = (int)(bs / a.S), h = (int)(i - bs * a.H), r = (int)(bs % a.S);
-    float x[4], y[4];
-    attn_load_row<T>(a, a.o, attn_q_at(a, b, r, h), lane, x);
-    attn_load_row<T>(a, a.d_out, attn_q_at(a, b, r, h), lane, y);
-    const float s = attn_dot(x, y);
-    if (lane == 0) a.delta[((long long)b * a.H + h) * a.S + r] = s;
+    const int h = (int)(i - bs * a.H), b = (int)(bs / padded), r = (int)(bs % padded);
+    float lse2 = INFINITY, delta = 0.f, square = 0.f;
+    const float lse = r < a.S ? a.lse[((long long)b * a.H + h) * a.S + r] : -INFINITY;
+    if (lse != -INFINITY) {
+      const long long at = attn_q_at(a, b, r, h);
+      for (int e = lane * VEC; e < a.D; e += G * VEC) {
+        float x[VEC], y[VEC];
+        Vec<T, VEC>::load((const T*)a.o + at + e, x);
+        Vec<T, VEC>::load((const T*)a.d_out + at + e, y);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          if (e + k >= a.D) continue;      // (padded copies)
+          delta = fmaf(x[k], y[k], delta);
+          square = fmaf(y[k], y[k], square);
+        }
+      }
+      lse2 = lse * kLog2e;
+    }
+    const unsigned int group = G == 32 ? 0xffffffffu : ((1u << G) - 1u) << (threadIdx.x % 32 / G * G);
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1) {
+      delta += __shfl_xor_sync(group, delta, o);
+      square += __shfl_xor_sync(group, square, o);
+    }
+    top = fmaxf(top, square);
+    if (lane == 0) {
+      const long long at = attn_stat_at(a, b, h, r);
+      a.stat[at] = lse2;
+      a.stat[at + 128] = delta;
+    }
+  }
+  if (!a.norms) return;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if ((threadIdx.x & 31u) == 0) sh[threadIdx.x / 32] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 8; ++i) top = fmaxf(top, sh[i]);
+    a.norms[blockIdx.x] = top;
   }
 }
 template <class T>
@@ -67,6 +106,20 @@ __global__ void __launch_bounds__(256) attn_copy_rows(const unsigned short* src,
     const int e = (int)(i - row * d);
     dst[row * to + e] = src[row * from + e];
   }
+}
+
+typedef void (*KeysKernel)(const b200_tmap, const b200_tmap, const b200_tmap, const b200_tmap, const b200_tmap, const b200_tmap, const AttnArgs);
+typedef void (*QueriesKernel)(const b200_tmap, const b200_tmap, const b200_tmap, const b200_tmap, const b200_tmap, const AttnArgs);
+
+template <class T, int DP>
+KeysKernel keys_of(bool cap, bool bias) {
+  if (cap) return bias ? attn_grad_keys_tc<T, DP, true, true> : attn_grad_keys_tc<T, DP, true, false>;
+  return bias ? attn_grad_keys_tc<T, DP, false, true> : attn_grad_keys_tc<T, DP, false, false>;
+}
+template <class T, int DP>
+QueriesKernel queries_of(bool cap, bool bias) {
+  if (cap) return bias ? attn_grad_queries_tc<T, DP, true, true> : attn_grad_queries_tc<T, DP, true, false>;
+  return bias ? attn_grad_queries_tc<T, DP, false, true> : attn_grad_queries_tc<T, DP, false, false>;
 }
 
 typedef void (*AttnKernel)(const AttnArgs);
@@ -106,12 +159,16 @@ struct AttnOperator : b200_operator {
   int dtype = 0;
   bool grad = false;
   long long rows = 0, key_rows = 0;
+  AttnKernel statistics = nullptr;
+  unsigned int statistics_grid = 0;
   // tensor-core form
   bool tc = false;
   ForwardKernel forward = nullptr;
-  b200_tmap map_q, map_k, map_v, map_o;
-  unsigned int threads = 0, grid = 0;
-  size_t smem = 0;
+  KeysKernel keys = nullptr;
+  QueriesKernel queries = nullptr;
+  b200_tmap map_q, map_k, map_v, map_o, map_do, map_dq, map_dk, map_dv;
+  unsigned int threads = 0, grid = 0, keys_grid = 0;
+  size_t smem = 0, keys_smem = 0;
   // padded copies: what is copied before and after the kernels
   struct Copy {
     const void* src;
@@ -121,57 +178,98 @@ struct AttnOperator : b200_operator {
   };
   std::vector<Copy> before, after;
   int head = 0;                // elements of a head that the caller's nodes have
+  size_t reserved = 0;         // of the workspace, while the operator is put together
 
   AttnKernel kernel(int which) const {
     return by_type(dtype, [&](auto t) -> AttnKernel {
       typedef decltype(t) T;
-      return which == 0 ? attn_forward_rows<T> : which == 1 ? attn_delta<T> : which == 2 ? attn_dq_rows<T> : attn_dkv_rows<T>;
+      return which == 0 ? attn_forward_rows<T> : which == 1 ? attn_dq_rows<T> : attn_dkv_rows<T>;
     });
+  }
+  size_t reserve(size_t bytes) {
+    const size_t here = reserved;
+    reserved += (bytes + 255) & ~(size_t)255;
+    return here;
   }
   void choose() {
     head = a.D;
-    for (int i = 0; i < 4; ++i) ready(kernel(i));
-    ready(attn_copy_rows);
-    tc = dtype != B200_F32 && rows && key_rows && !grad;
-    if (grad) {
-      take_workspace((size_t)rows * 4);
-      a.delta = (float*)workspace;
+    tc = dtype != B200_F32 && rows && key_rows;
+    if (!tc)
+      for (int i = 0; i < 3; ++i) ready(kernel(i));
+    // Heads whose rows or addresses are no multiples of 16 bytes go through copies with padded rows.
+    struct Padded {
+      const void* node;
+      bool written, of_keys;
+      size_t at;
+    };
+    std::vector<Padded> nodes;
+    for (auto& n : {Padded{a.q, false, false, 0}, {a.k, false, true, 0}, {a.v, false, true, 0}, {a.o, false, false, 0}, {a.d_out, false, false, 0},
+                    {a.out, true, false, 0}, {a.dq, true, false, 0}, {a.dk, true, true, 0}, {a.dv, true, true, 0}})
+      if (n.node) nodes.push_back(n);
+    bool plain = a.D % 8 == 0;
+    for (auto& n : nodes) plain &= ((size_t)n.node & 15) == 0;
+    const int ld = (a.D + 7) / 8 * 8;
+    const bool pad = tc && !plain;
+    if (pad)
+      for (auto& n : nodes) n.at = reserve((size_t)(n.of_keys ? key_rows : rows) * ld * 2);
+    size_t stat = 0, norms = 0;
+    if (grad && rows) {
+      const long long padded = (long long)a.B * a.H * ((a.S + 127) / 128) * 128;
+      const int size = (int)dtype_bytes(dtype);
+      const bool vec = tc || (a.D * size % 16 == 0 && (((size_t)a.o | (size_t)a.d_out) & 15) == 0);
+      const bool narrow = a.D * size <= 128;
+      statistics = by_type(dtype, [&](auto t) -> AttnKernel {
+        typedef decltype(t) T;
+        constexpr int V = 16 / (int)sizeof(T);
+        if (!vec) return attn_statistics<T, 1, 16>;
+        return narrow ? attn_statistics<T, V, 8> : attn_statistics<T, V, 16>;
+      });
+      ready(statistics);
+      statistics_grid = (unsigned int)std::min<long long>((padded + (256 / 16) - 1) / (256 / 16), 8ll * dev->sm_count);
+      stat = reserve((size_t)padded * 8);
+      if (dtype == B200_F16) norms = reserve((size_t)statistics_grid * 4);
+    }
+    take_workspace(reserved);
+    if (grad && rows) {
+      a.stat = (float*)(workspace + stat);
+      if (dtype == B200_F16) {
+        a.norms = (float*)(workspace + norms);
+        a.n_norms = (int)statistics_grid;
+      }
+    }
+    if (pad) {
+      ready(attn_copy_rows);
+      for (auto& n : nodes) {
+        void* copy = (void*)(workspace + n.at);
+        const long long many = n.of_keys ? key_rows : rows;
+        if (n.written) after.push_back({copy, (void*)n.node, many, ld, a.D});
+        else before.push_back({n.node, copy, many, a.D, ld});
+        for (const void** p : {&a.q, &a.k, &a.v, &a.o, &a.d_out, (const void**)&a.out, (const void**)&a.dq, (const void**)&a.dk, (const void**)&a.dv})
+          if (*p == n.node) *p = copy;
+      }
+      a.ld = ld;
     }
     if (tc) choose_tc();
   }
-  // Heads whose rows or addresses are no multiples of 16 bytes go through copies with padded rows.
-  void pad() {
-    bool plain = a.D % 8 == 0;
-    for (const void* p : {a.q, a.k, a.v, (const void*)a.out}) plain &= ((size_t)p & 15) == 0;
-    if (plain) return;
-    const int ld = (a.D + 7) / 8 * 8;
-    size_t at = 0;
-    auto room = [&](long long n) {
-      const size_t here = at;
-      at += ((size_t)n * ld * 2 + 255) & ~(size_t)255;
-      return here;
-    };
-    const size_t q = room(rows), k = room(key_rows), v = room(key_rows), o = room(rows);
-    take_workspace(at);
-    auto in = [&](const void*& p, size_t where, long long n) {
-      before.push_back({p, (void*)(workspace + where), n, a.D, ld});
-      p = (const void*)(workspace + where);
-    };
-    in(a.q, q, rows);
-    in(a.k, k, key_rows);
-    in(a.v, v, key_rows);
-    after.push_back({(const void*)(workspace + o), a.out, rows, ld, a.D});
-    a.out = (void*)(workspace + o);
-    a.ld = ld;
+  unsigned int blocks_of(long long n) const {
+    if (n >> 31) throw Error(B200_E_UNSUPPORTED, "attention: too many rows");
+    return (unsigned int)n;
   }
   void choose_tc() {
-    pad();
-    map_q = head_map(a.q, dtype, a.B, a.S, a.H, a.D, a.ld);
-    map_k = head_map(a.k, dtype, a.B, a.T, a.HK, a.D, a.ld);
-    map_v = head_map(a.v, dtype, a.B, a.T, a.HK, a.D, a.ld);
-    map_o = head_map(a.out, dtype, a.B, a.S, a.H, a.D, a.ld);
-    const bool cap = a.cap > 0.f, bias = a.slopes != nullptr;
-    const int tiles = (a.T + 127) / 128;
+    auto of_queries = [&](const void* p) { return head_map(p, dtype, a.B, a.S, a.H, a.D, a.ld); };
+    auto of_keys = [&](const void* p) { return head_map(p, dtype, a.B, a.T, a.HK, a.D, a.ld); };
+    map_q = of_queries(a.q);
+    map_k = of_keys(a.k);
+    map_v = of_keys(a.v);
+    if (grad) {
+      map_do = of_queries(a.d_out);
+      map_dq = of_queries(a.dq);
+      map_dk = of_keys(a.dk);
+      map_dv = of_keys(a.dv);
+    } else {
+      map_o = of_queries(a.out);
+    }
+    const int tiles = (a.T + 127) / 128, tiles_q = (a.S + 127) / 128;
     const long long heads = (long long)a.B * a.H;
     // Heads of more than 64 elements: two query tiles a CTA share each key tile (64 KB per tile of 128 x 128 would otherwise
     // come in from L2 for 1024 cycles of products), unless that leaves SMs without work.
@@ -179,23 +277,40 @@ struct AttnOperator : b200_operator {
     by_type(dtype, [&](auto t) {
       typedef decltype(t) T;
       if constexpr (sizeof(T) == 2) {
-        if (a.D <= 64) set<T, 64, 1>(cap, bias, tiles);
-        else if (two) set<T, 128, 2>(cap, bias, tiles);
-        else set<T, 128, 1>(cap, bias, tiles);
+        if (grad) {
+          if (a.D <= 64) set_grad<T, 64>(tiles, tiles_q);
+          else set_grad<T, 128>(tiles, tiles_q);
+        } else {
+          if (a.D <= 64) set<T, 64, 1>(tiles);
+          else if (two) set<T, 128, 2>(tiles);
+          else set<T, 128, 1>(tiles);
+        }
       }
       return 0;
     });
-    const long long n = heads * ((a.S + 128 * (two ? 2 : 1) - 1) / (128 * (two ? 2 : 1)));
-    if (n >> 31) throw Error(B200_E_UNSUPPORTED, "attention: too many rows");
-    grid = (unsigned int)n;
-    if (smem > 227 * 1024) throw Error(B200_E_UNSUPPORTED, "attention: too many keys");
-    ready(forward, smem);
+    grid = blocks_of(heads * ((a.S + 128 * (!grad && two ? 2 : 1) - 1) / (128 * (!grad && two ? 2 : 1))));
+    if (grad) keys_grid = blocks_of((long long)a.B * a.HK * tiles);
+    if (std::max(smem, keys_smem) > 227 * 1024) throw Error(B200_E_UNSUPPORTED, "attention: too many keys or queries");
+    if (grad) {
+      ready(keys, keys_smem);
+      ready(queries, smem);
+    } else {
+      ready(forward, smem);
+    }
   }
   template <class T, int DP, int NQ>
-  void set(bool cap, bool bias, int tiles) {
-    forward = forward_of<T, DP, NQ>(cap, bias);
+  void set(int tiles) {
+    forward = forward_of<T, DP, NQ>(a.cap > 0.f, a.slopes != nullptr);
     threads = FwdShape<DP, NQ>::kThreads;
     smem = FwdShape<DP, NQ>::smem(tiles);
+  }
+  template <class T, int DP>
+  void set_grad(int tiles, int tiles_q) {
+    keys = keys_of<T, DP>(a.cap > 0.f, a.slopes != nullptr);
+    queries = queries_of<T, DP>(a.cap > 0.f, a.slopes != nullptr);
+    threads = BwdShape<DP>::kThreads;
+    smem = BwdShape<DP>::smem(tiles);
+    keys_smem = BwdShape<DP>::smem(tiles_q);
   }
   void copy(const std::vector<Copy>& list, cudaStream_t s) {
     for (auto& c : list)
@@ -204,21 +319,20 @@ struct AttnOperator : b200_operator {
   }
   unsigned int blocks(long long n) const { return (unsigned int)std::min<long long>((n + 7) / 8, 16ll * dev->sm_count); }
   void run(cudaStream_t s) override {
-    if (tc) {
-      copy(before, s);
+    copy(before, s);
+    if (grad && rows) launch(statistics, statistics_grid, 256, 0, s, a);
+    if (tc && grad) {
+      launch(keys, keys_grid, threads, keys_smem, s, map_q, map_k, map_v, map_do, map_dk, map_dv, a);
+      launch(queries, grid, threads, smem, s, map_q, map_k, map_v, map_do, map_dq, a);
+    } else if (tc) {
       launch(forward, grid, threads, smem, s, map_q, map_k, map_v, map_o, a);
-      copy(after, s);
-      return;
+    } else if (grad) {
+      if (rows) launch(kernel(1), blocks(rows), 256, 0, s, a);
+      if (key_rows) launch(kernel(2), blocks(key_rows), 256, 0, s, a);
+    } else if (rows) {
+      launch(kernel(0), blocks(rows), 256, 0, s, a);
     }
-    if (!grad) {
-      if (rows) launch(kernel(0), blocks(rows), 256, 0, s, a);
-      return;
-    }
-    if (rows) {
-      launch(kernel(1), blocks(rows), 256, 0, s, a);
-      launch(kernel(2), blocks(rows), 256, 0, s, a);
-    }
-    if (key_rows) launch(kernel(3), blocks(key_rows), 256, 0, s, a);
+    copy(after, s);
   }
 };
 
