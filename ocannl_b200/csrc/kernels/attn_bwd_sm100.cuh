@@ -121,7 +121,7 @@ attn_grad_keys_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant
                   const __grid_constant__ b200_tmap map_do, const __grid_constant__ b200_tmap map_dk, const __grid_constant__ b200_tmap map_dv,
                   const __grid_constant__ AttnArgs a) {
   typedef BwdShape<DP> Sh;
-  extern __shared__ unsigned char dyn[];
+  extern __shared__ __align__(128) unsigned char dyn[];
   const unsigned int base = (b200_smem_addr(dyn) + 1023u) & ~1023u;
   unsigned char* const gen = dyn + (base - b200_smem_addr(dyn));
   const unsigned int k_at = base, v_at = base + Sh::kTile, ring = base + 2 * Sh::kTile;
@@ -419,7 +419,7 @@ __global__ void __launch_bounds__(320, 1)
 attn_grad_queries_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant__ b200_tmap map_k, const __grid_constant__ b200_tmap map_v,
                      const __grid_constant__ b200_tmap map_do, const __grid_constant__ b200_tmap map_dq, const __grid_constant__ AttnArgs a) {
   typedef BwdShape<DP> Sh;
-  extern __shared__ unsigned char dyn[];
+  extern __shared__ __align__(128) unsigned char dyn[];
   const unsigned int base = (b200_smem_addr(dyn) + 1023u) & ~1023u;
   unsigned char* const gen = dyn + (base - b200_smem_addr(dyn));
   const unsigned int q_at = base, do_at = base + Sh::kTile, ring = base + 2 * Sh::kTile;

@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(NQ * 128 + 64, NQ == 1 ? 2 : 1)
 attn_forward_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant__ b200_tmap map_k, const __grid_constant__ b200_tmap map_v,
                 const __grid_constant__ b200_tmap map_o, const __grid_constant__ AttnArgs a) {
   typedef FwdShape<DP, NQ> Sh;
-  extern __shared__ unsigned char dyn[];
+  extern __shared__ __align__(128) unsigned char dyn[];
   const unsigned int base = (b200_smem_addr(dyn) + 1023u) & ~1023u;
   unsigned char* const gen = dyn + (base - b200_smem_addr(dyn));
   const unsigned int q_at = base, k_at = base + NQ * Sh::kTile, v_at = k_at + Sh::kSlots * Sh::kTile;

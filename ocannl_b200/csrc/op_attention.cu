@@ -4,7 +4,9 @@
 
 #include "operators.hpp"
 #include "kernels/attn_bwd_sm100.cuh"
+#include "kernels/attn_few_sm100.cuh"
 #include "kernels/attn_fwd_sm100.cuh"
+#include "kernels/attn_single.cuh"
 #include "kernels/attn_terms.cuh"
 
 using namespace b200;
@@ -111,6 +113,14 @@ __global__ void __launch_bounds__(256) attn_copy_rows(const unsigned short* src,
 typedef void (*KeysKernel)(const b200_tmap, const b200_tmap, const b200_tmap, const b200_tmap, const b200_tmap, const b200_tmap, const AttnArgs);
 typedef void (*QueriesKernel)(const b200_tmap, const b200_tmap, const b200_tmap, const b200_tmap, const b200_tmap, const AttnArgs);
 
+typedef void (*SingleKernel)(const AttnArgs, int);
+typedef void (*FewKernel)(const AttnArgs, const FewArgs);
+
+template <class T, int DP>
+FewKernel few_of(bool cap, bool bias) {
+  if (cap) return bias ? attn_forward_few<T, DP, true, true> : attn_forward_few<T, DP, true, false>;
+  return bias ? attn_forward_few<T, DP, false, true> : attn_forward_few<T, DP, false, false>;
+}
 template <class T, int DP>
 KeysKernel keys_of(bool cap, bool bias) {
   if (cap) return bias ? attn_grad_keys_tc<T, DP, true, true> : attn_grad_keys_tc<T, DP, true, false>;
@@ -166,6 +176,11 @@ struct AttnOperator : b200_operator {
   ForwardKernel forward = nullptr;
   KeysKernel keys = nullptr;
   QueriesKernel queries = nullptr;
+  SingleKernel single[2] = {nullptr, nullptr};      // forward, or the gradients' two
+  size_t single_smem[2] = {0, 0};
+  int vec = 0;
+  FewKernel few = nullptr;
+  FewArgs few_args = {};
   b200_tmap map_q, map_k, map_v, map_o, map_do, map_dq, map_dk, map_dv;
   unsigned int threads = 0, grid = 0, keys_grid = 0;
   size_t smem = 0, keys_smem = 0;
@@ -194,7 +209,8 @@ struct AttnOperator : b200_operator {
   void choose() {
     head = a.D;
     tc = dtype != B200_F32 && rows && key_rows;
-    if (!tc)
+    if (dtype == B200_F32 && rows && key_rows) choose_single();
+    else if (!tc)
       for (int i = 0; i < 3; ++i) ready(kernel(i));
     // Heads whose rows or addresses are no multiples of 16 bytes go through copies with padded rows.
     struct Padded {
@@ -212,7 +228,8 @@ struct AttnOperator : b200_operator {
     const bool pad = tc && !plain;
     if (pad)
       for (auto& n : nodes) n.at = reserve((size_t)(n.of_keys ? key_rows : rows) * ld * 2);
-    size_t stat = 0, norms = 0;
+    size_t stat = 0, norms = 0, parts = 0, tickets = 0;
+    if (tc && !grad && few_rows()) choose_few(&parts, &tickets);
     if (grad && rows) {
       const long long padded = (long long)a.B * a.H * ((a.S + 127) / 128) * 128;
       const int size = (int)dtype_bytes(dtype);
@@ -249,7 +266,53 @@ struct AttnOperator : b200_operator {
       }
       a.ld = ld;
     }
-    if (tc) choose_tc();
+    if (few) {
+      few_args.parts = (float*)(workspace + parts);
+      few_args.tickets = (unsigned int*)(workspace + tickets);
+      cu_check(cu().cuMemsetD8Async_(workspace + tickets, 0, (size_t)grid * 4, dev->stream), "cuMemsetD8Async(tickets)");
+      ready(few, smem);
+    } else if (tc) {
+      choose_tc();
+    }
+  }
+  // A tile of the tensor-core kernel has 128 queries of one head.  Up to 16 queries go sixteen rows at a time (of all heads that
+  // share the keys), the keys split over the machine.
+  bool few_rows() const { return a.S <= 16; }
+  void choose_few(size_t* parts, size_t* tickets) {
+    const long long pairs = (long long)a.B * a.HK * ((a.group * a.S + kFewRows - 1) / kFewRows);
+    grid = blocks_of(pairs);
+    by_type(dtype, [&](auto t) {
+      typedef decltype(t) T;
+      if constexpr (sizeof(T) == 2) {
+        few = a.D <= 64 ? few_of<T, 64>(a.cap > 0.f, a.slopes != nullptr) : few_of<T, 128>(a.cap > 0.f, a.slopes != nullptr);
+        smem = a.D <= 64 ? FewShape<64>::smem() : FewShape<128>::smem();
+      }
+      return 0;
+    });
+    // Ranges of at least 256 keys, as many as give every SM four blocks: sequences of different lengths even out.
+    const long long most = (a.T + 255) / 256, want = (4ll * dev->sm_count + pairs - 1) / pairs;
+    const int step = kFewStep * kFewWarps, splits = (int)std::max<long long>(1, std::min<long long>(std::min(most, want), kFewMost));
+    few_args.per_split = ((a.T + splits - 1) / splits + step - 1) / step * step;
+    few_args.splits = (a.T + few_args.per_split - 1) / few_args.per_split;
+    const int width = a.D <= 64 ? FewShape<64>::kWidth : FewShape<128>::kWidth;
+    *parts = reserve(few_args.splits > 1 ? (size_t)pairs * few_args.splits * kFewRows * width * 4 : 0);
+    *tickets = reserve((size_t)pairs * 4);
+  }
+  void choose_single() {
+    vec = a.D % 4 == 0;
+    for (const void* p : {a.q, a.k, a.v, a.d_out}) vec &= ((size_t)p & 15) == 0;
+    if (grad) {
+      single[0] = a.D <= 64 ? attn_grad_keys_single<1> : attn_grad_keys_single<2>;
+      single[1] = a.D <= 64 ? attn_grad_queries_single<1> : attn_grad_queries_single<2>;
+      single_smem[0] = single_smem[1] = SingleShape::smem(a.D, 4);
+      keys_grid = blocks_of((long long)a.B * a.HK * ((a.T + kSide - 1) / kSide));
+    } else {
+      single[0] = a.D <= 64 ? attn_forward_single<1> : attn_forward_single<2>;
+      single_smem[0] = SingleShape::smem(a.D, 3);
+    }
+    grid = blocks_of((long long)a.B * a.H * ((a.S + kSide - 1) / kSide));
+    for (int i = 0; i < 2; ++i)
+      if (single[i]) ready(single[i], single_smem[i]);
   }
   unsigned int blocks_of(long long n) const {
     if (n >> 31) throw Error(B200_E_UNSUPPORTED, "attention: too many rows");
@@ -324,8 +387,13 @@ struct AttnOperator : b200_operator {
     if (tc && grad) {
       launch(keys, keys_grid, threads, keys_smem, s, map_q, map_k, map_v, map_do, map_dk, map_dv, a);
       launch(queries, grid, threads, smem, s, map_q, map_k, map_v, map_do, map_dq, a);
+    } else if (few) {
+      launch(few, dim3(grid, (unsigned int)few_args.splits), kFewWarps * 32, smem, s, a, few_args);
     } else if (tc) {
       launch(forward, grid, threads, smem, s, map_q, map_k, map_v, map_o, a);
+    } else if (single[0]) {
+      launch(single[0], grad ? keys_grid : grid, 256, single_smem[0], s, a, vec);
+      if (grad) launch(single[1], grid, 256, single_smem[1], s, a, vec);
     } else if (grad) {
       if (rows) launch(kernel(1), blocks(rows), 256, 0, s, a);
       if (key_rows) launch(kernel(2), blocks(key_rows), 256, 0, s, a);
