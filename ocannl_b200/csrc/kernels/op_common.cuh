@@ -5,6 +5,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 namespace b200 {
 
 __device__ __forceinline__ void grid_begin() {
@@ -60,6 +62,48 @@ struct Vec {
       *(uint4*)p = make_uint4(pack2(v[0], v[1], T()), pack2(v[2], v[3], T()), pack2(v[4], v[5], T()), pack2(v[6], v[7], T()));
     }
   }
+};
+
+// The same access in two steps, so that a load can be under way while other work is done.
+template <class T, int VEC>
+struct Raw {
+  typename std::conditional<VEC == 1, T, uint4>::type r;
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (VEC == 1) r = *p;
+    else r = *(const uint4*)p;
+  }
+  __device__ __forceinline__ void clear() {
+    if constexpr (VEC == 1) from_float(0.f, r);
+    else r = make_uint4(0u, 0u, 0u, 0u);
+  }
+  __device__ __forceinline__ void values(float* v) const {
+    if constexpr (VEC == 1) {
+      v[0] = to_float(r);
+    } else {
+      const unsigned int w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4) {
+          v[i] = __uint_as_float(w[i]);
+        } else {
+          const float2 f = unpack2(w[i], T());
+          v[2 * i] = f.x; v[2 * i + 1] = f.y;
+        }
+      }
+    }
+  }
+};
+
+// Quotients by a number known at link (1 <= d < 2^31), for numerators below 2^31: one multiplication and a shift.
+// With s = ceil(log2 d) and m = ceil(2^(31 + s) / d), floor(n m / 2^(31 + s)) is the quotient: m d exceeds 2^(31 + s) by less than 2^s.
+struct Divisor {
+  unsigned int d, m, s;
+  Divisor() : d(1), m(0x80000000u), s(0) {}
+  explicit Divisor(unsigned int by) : d(by), m(0), s(0) {
+    while ((1ull << s) < by) ++s;
+    m = (unsigned int)(((1ull << (31 + s)) + by - 1) / by);
+  }
+  __device__ __forceinline__ unsigned int of(unsigned int n) const { return (unsigned int)(((unsigned long long)n * m) >> (31 + s)); }
 };
 
 }  // namespace b200

@@ -25,47 +25,72 @@ __global__ void __launch_bounds__(256) attn_forward_rows(const __grid_constant__
   }
 }
 // What the gradients need of every row: its lse and <d_out, out>, tile by tile of 128 queries, G threads a row.  Bound by memory: out and
-// d_out are read once.  Rows behind the last one and rows that see nothing get weights of zero.
+// d_out are read once, kRowsAtOnce rows of a thread under way together.  Rows behind the last one and rows that see nothing get
+// weights of zero.
+constexpr int kRowsAtOnce = 4;
+
 template <class T, int VEC, int G>
-__global__ void __launch_bounds__(256) attn_statistics(const __grid_constant__ AttnArgs a) {
+__global__ void __launch_bounds__(256) attn_statistics(const __grid_constant__ AttnArgs a, const Divisor by_heads, const Divisor by_padded) {
   __shared__ float sh[8];
   grid_begin();
-  const int lane = (int)threadIdx.x % G, padded = (a.S + 127) / 128 * 128;
-  const long long n = (long long)a.B * padded * a.H, step = (long long)gridDim.x * (256 / G);
+  constexpr int rows = 256 / G, chunks = VEC > 1 ? 1 : 128 / G;
+  const int lane = (int)threadIdx.x % G;
+  const unsigned int padded = by_padded.d, n = (unsigned int)a.B * padded * (unsigned int)a.H, step = gridDim.x * rows * kRowsAtOnce;
   float top = 0.f;
-  for (long long base = (long long)blockIdx.x * (256 / G); base < n; base += step) {
-    const long long i = base + threadIdx.x / G;
-    if (i >= n) continue;
-    const long long bs = i / a.H;
-    const int h = (int)(i - bs * a.H), b = (int)(bs / padded), r = (int)(bs % padded);
-    float lse2 = INFINITY, delta = 0.f, square = 0.f;
-    const float lse = r < a.S ? a.lse[((long long)b * a.H + h) * a.S + r] : -INFINITY;
-    if (lse != -INFINITY) {
-      const long long at = attn_q_at(a, b, r, h);
-      for (int e = lane * VEC; e < a.D; e += G * VEC) {
-        float x[VEC], y[VEC];
-        Vec<T, VEC>::load((const T*)a.o + at + e, x);
-        Vec<T, VEC>::load((const T*)a.d_out + at + e, y);
+  for (unsigned int base = blockIdx.x * rows * kRowsAtOnce; base < n; base += step) {
+    Raw<T, VEC> x[kRowsAtOnce][chunks], y[kRowsAtOnce][chunks];
+    float lse[kRowsAtOnce];
+    long long stat[kRowsAtOnce];
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-          if (e + k >= a.D) continue;      // (padded copies)
-          delta = fmaf(x[k], y[k], delta);
-          square = fmaf(y[k], y[k], square);
+    for (int k = 0; k < kRowsAtOnce; ++k) {
+      const unsigned int i = base + k * rows + threadIdx.x / G;
+      lse[k] = -INFINITY;
+      stat[k] = -1;
+#pragma unroll
+      for (int c = 0; c < chunks; ++c) {
+        x[k][c].clear();
+        y[k][c].clear();
+      }
+      if (i >= n) continue;
+      const unsigned int bs = by_heads.of(i), h = i - bs * (unsigned int)a.H, b = by_padded.of(bs), r = bs - b * padded;
+      stat[k] = attn_stat_at(a, (int)b, (int)h, (int)r);
+      if (r >= (unsigned int)a.S) continue;
+      lse[k] = a.lse[((long long)b * a.H + h) * a.S + r];
+      const long long at = attn_q_at(a, (int)b, (int)r, (int)h);
+#pragma unroll
+      for (int c = 0; c < chunks; ++c) {
+        const int e = (c * G + lane) * VEC;
+        if (e >= a.D) continue;
+        x[k][c].load((const T*)a.o + at + e);
+        y[k][c].load((const T*)a.d_out + at + e);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kRowsAtOnce; ++k) {
+      float delta = 0.f, square = 0.f;
+#pragma unroll
+      for (int c = 0; c < chunks; ++c) {
+        float u[VEC], w[VEC];
+        x[k][c].values(u);
+        y[k][c].values(w);
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) {
+          if (VEC > 1 && (c * G + lane) * VEC + q >= a.D) continue;      // (padded copies)
+          delta = fmaf(u[q], w[q], delta);
+          square = fmaf(w[q], w[q], square);
         }
       }
-      lse2 = lse * kLog2e;
-    }
-    const unsigned int group = G == 32 ? 0xffffffffu : ((1u << G) - 1u) << (threadIdx.x % 32 / G * G);
 #pragma unroll
-    for (int o = G / 2; o > 0; o >>= 1) {
-      delta += __shfl_xor_sync(group, delta, o);
-      square += __shfl_xor_sync(group, square, o);
-    }
-    top = fmaxf(top, square);
-    if (lane == 0) {
-      const long long at = attn_stat_at(a, b, h, r);
-      a.stat[at] = lse2;
-      a.stat[at + 128] = delta;
+      for (int o = G / 2; o > 0; o >>= 1) {
+        delta += __shfl_xor_sync(0xffffffffu, delta, o);
+        square += __shfl_xor_sync(0xffffffffu, square, o);
+      }
+      const bool empty = lse[k] == -INFINITY;
+      if (!empty) top = fmaxf(top, square);
+      if (lane == 0 && stat[k] >= 0) {
+        a.stat[stat[k]] = empty ? INFINITY : lse[k] * kLog2e;
+        a.stat[stat[k] + 128] = empty ? 0.f : delta;
+      }
     }
   }
   if (!a.norms) return;
@@ -78,6 +103,8 @@ __global__ void __launch_bounds__(256) attn_statistics(const __grid_constant__ A
     a.norms[blockIdx.x] = top;
   }
 }
+typedef void (*StatisticsKernel)(const AttnArgs, const Divisor, const Divisor);
+
 template <class T>
 __global__ void __launch_bounds__(256) attn_dq_rows(const __grid_constant__ AttnArgs a) {
   grid_begin();
@@ -169,8 +196,9 @@ struct AttnOperator : b200_operator {
   int dtype = 0;
   bool grad = false;
   long long rows = 0, key_rows = 0;
-  AttnKernel statistics = nullptr;
+  StatisticsKernel statistics = nullptr;
   unsigned int statistics_grid = 0;
+  Divisor by_heads, by_padded;
   // tensor-core form
   bool tc = false;
   ForwardKernel forward = nullptr;
@@ -234,15 +262,20 @@ struct AttnOperator : b200_operator {
       const long long padded = (long long)a.B * a.H * ((a.S + 127) / 128) * 128;
       const int size = (int)dtype_bytes(dtype);
       const bool vec = tc || (a.D * size % 16 == 0 && (((size_t)a.o | (size_t)a.d_out) & 15) == 0);
-      const bool narrow = a.D * size <= 128;
-      statistics = by_type(dtype, [&](auto t) -> AttnKernel {
+      if (padded >> 31) throw Error(B200_E_UNSUPPORTED, "attention: too many rows");
+      int group = 32;
+      statistics = by_type(dtype, [&](auto t) -> StatisticsKernel {
         typedef decltype(t) T;
-        constexpr int V = 16 / (int)sizeof(T);
-        if (!vec) return attn_statistics<T, 1, 16>;
-        return narrow ? attn_statistics<T, V, 8> : attn_statistics<T, V, 16>;
+        constexpr int V = 16 / (int)sizeof(T), G = 128 / V;
+        if (!vec) return attn_statistics<T, 1, 32>;
+        group = a.D <= 64 ? G / 2 : G;
+        return a.D <= 64 ? attn_statistics<T, V, G / 2> : attn_statistics<T, V, G>;
       });
       ready(statistics);
-      statistics_grid = (unsigned int)std::min<long long>((padded + (256 / 16) - 1) / (256 / 16), 8ll * dev->sm_count);
+      by_heads = Divisor((unsigned int)a.H);
+      by_padded = Divisor((unsigned int)((a.S + 127) / 128 * 128));
+      const long long at_once = 256 / group * kRowsAtOnce;
+      statistics_grid = (unsigned int)std::min<long long>((padded + at_once - 1) / at_once, 8ll * dev->sm_count);
       stat = reserve((size_t)padded * 8);
       if (dtype == B200_F16) norms = reserve((size_t)statistics_grid * 4);
     }
@@ -383,7 +416,7 @@ struct AttnOperator : b200_operator {
   unsigned int blocks(long long n) const { return (unsigned int)std::min<long long>((n + 7) / 8, 16ll * dev->sm_count); }
   void run(cudaStream_t s) override {
     copy(before, s);
-    if (grad && rows) launch(statistics, statistics_grid, 256, 0, s, a);
+    if (grad && rows) launch(statistics, statistics_grid, 256, 0, s, a, by_heads, by_padded);
     if (tc && grad) {
       launch(keys, keys_grid, threads, keys_smem, s, map_q, map_k, map_v, map_do, map_dk, map_dv, a);
       launch(queries, grid, threads, smem, s, map_q, map_k, map_v, map_do, map_dq, a);

@@ -7,9 +7,9 @@
 //
 // Both are bound by memory: every plane of the rows crosses it once.  A group of 8, 32, 128 or 512 threads keeps its row in
 // registers, at most 16 elements a thread, so that the squares of the distances from the mean are summed in a second pass over
-// registers (no difference of large sums).  The groups stride over the rows; the scale and the shift stay in registers, and
-// so do, in the gradient, a thread's sums over the rows of its columns, which meet in shared memory once per block and then in a
-// second kernel that adds the blocks' partial sums in their order: the same bits every time.  Rows of more than 8192 elements
+// registers (no difference of large sums).  The groups stride over the rows, the next row's loads under way while one is worked
+// on; the scale and the shift stay in shared memory.  In the gradient a thread keeps its sums over the rows of its columns in
+// registers; they meet in shared memory once per block and then in a second kernel that adds the blocks' partial sums in their order: the same bits every time.  Rows of more than 8192 elements
 // are read again for each pass, by 1024 threads (they come from L2 then), their column sums by a kernel of its own.
 #include "kernels/op_common.cuh"
 #include "operators.hpp"
@@ -28,8 +28,6 @@ struct NormArgs {
   int weight_f32;                  // gamma and beta in single precision, or in the rows' type
   float eps, inv_n;
 };
-
-constexpr unsigned int kBlock = 256;
 
 template <class T>
 __device__ __forceinline__ float weight_at(const void* p, int f32, unsigned int i, float otherwise) {
@@ -65,47 +63,51 @@ __device__ __forceinline__ void row_sum(float (&v)[K], float* sh, int half) {
 }
 
 template <class T, int VEC, int NV, int TPR>
-__global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_rows(const NormArgs a) {
+__global__ void __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 1 : 3) norm_rows(const NormArgs a) {
   constexpr int E = NV * VEC;
   __shared__ float sh[2 * 32];
+  extern __shared__ __align__(16) float weights[];      // scale and shift
   grid_begin();
   const unsigned int t = threadIdx.x % TPR, sub = threadIdx.x / TPR, per_block = blockDim.x / TPR;
-  float ga[E], be[E];
+  constexpr unsigned int kSpan = TPR * E;
+  for (unsigned int e = threadIdx.x; e < kSpan; e += blockDim.x) {
+    weights[e] = e < a.n ? weight_at<T>(a.gamma, a.weight_f32, e, 1.f) : 0.f;
+    weights[kSpan + e] = e < a.n ? weight_at<T>(a.beta, a.weight_f32, e, 0.f) : 0.f;
+  }
+  // the next row is on its way while this one is worked on
+  Raw<T, VEC> rx[NV], rr[NV];
+  const unsigned long long step = (unsigned long long)gridDim.x * per_block;
+  auto fetch = [&](unsigned long long row) {
 #pragma unroll
-  for (int c = 0; c < NV; ++c)
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      const unsigned int e = (c * TPR + t) * VEC + i;
-      ga[c * VEC + i] = e < a.n ? weight_at<T>(a.gamma, a.weight_f32, e, 1.f) : 0.f;
-      be[c * VEC + i] = e < a.n ? weight_at<T>(a.beta, a.weight_f32, e, 0.f) : 0.f;
+    for (int c = 0; c < NV; ++c) {
+      const unsigned int e = (c * TPR + t) * VEC;
+      if (row < a.rows && e < a.n) {
+        rx[c].load((const T*)a.x + row * a.n + e);
+        if (a.r) rr[c].load((const T*)a.r + row * a.n + e);
+      }
     }
-  for (unsigned long long first = (unsigned long long)blockIdx.x * per_block; first < a.rows; first += (unsigned long long)gridDim.x * per_block) {
+  };
+#pragma unroll
+  for (int c = 0; c < NV; ++c) {
+    rx[c].clear();
+    rr[c].clear();
+  }
+  fetch((unsigned long long)blockIdx.x * per_block + sub);
+  __syncthreads();
+  for (unsigned long long first = (unsigned long long)blockIdx.x * per_block; first < a.rows; first += step) {
     const unsigned long long row = first + sub;
     const bool on = row < a.rows;
     const unsigned long long at = row * a.n;
     float h[E];
 #pragma unroll
     for (int c = 0; c < NV; ++c) {
-      const unsigned int e = (c * TPR + t) * VEC;
-      const bool ok = on && e < a.n;
-      float v[VEC];
+      float w[VEC];
+      rx[c].values(h + c * VEC);
+      rr[c].values(w);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) v[i] = 0.f;
-      if (ok) Vec<T, VEC>::load((const T*)a.x + at + e, v);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) h[c * VEC + i] = v[i];
+      for (int i = 0; i < VEC; ++i) h[c * VEC + i] += w[i];
     }
-    if (a.r) {
-#pragma unroll
-      for (int c = 0; c < NV; ++c) {
-        const unsigned int e = (c * TPR + t) * VEC;
-        if (!(on && e < a.n)) continue;
-        float v[VEC];
-        Vec<T, VEC>::load((const T*)a.r + at + e, v);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) h[c * VEC + i] += v[i];
-      }
-    }
+    fetch(row + step);
     float s[1] = {0.f};
 #pragma unroll
     for (int i = 0; i < E; ++i) s[0] += h[i];
@@ -133,61 +135,74 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_rows(const NormArg
       float v[VEC];
       if (a.h) Vec<T, VEC>::store((T*)a.h + at + e, h + c * VEC);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) v[i] = fmaf((h[c * VEC + i] - mean) * rstd, ga[c * VEC + i], be[c * VEC + i]);
+      for (int i = 0; i < VEC; ++i) v[i] = fmaf((h[c * VEC + i] - mean) * rstd, weights[e + i], weights[kSpan + e + i]);
       Vec<T, VEC>::store((T*)a.y + at + e, v);
     }
   }
 }
 
 template <class T, int VEC, int NV, int TPR>
-__global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_grad_rows(const NormArgs a) {
+__global__ void __launch_bounds__(512, 1) norm_grad_rows(const NormArgs a) {
   constexpr int E = NV * VEC;
   __shared__ float sh[2 * 2 * 32];
-  extern __shared__ float columns[];        // [2][rows of the block at a time][n]
+  extern __shared__ __align__(16) float weights[];      // the scale; at the end [2][rows of the block at a time][n] sums
+  float* columns = weights;
   grid_begin();
   const unsigned int t = threadIdx.x % TPR, sub = threadIdx.x / TPR, per_block = blockDim.x / TPR;
-  float ga[E], dg[E], db[E];
+  constexpr unsigned int kSpan = TPR * E;
+  for (unsigned int e = threadIdx.x; e < kSpan; e += blockDim.x) weights[e] = e < a.n ? weight_at<T>(a.gamma, a.weight_f32, e, 1.f) : 0.f;
+  float dg[E], db[E];
 #pragma unroll
-  for (int c = 0; c < NV; ++c)
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      const unsigned int e = (c * TPR + t) * VEC + i;
-      ga[c * VEC + i] = e < a.n ? weight_at<T>(a.gamma, a.weight_f32, e, 1.f) : 0.f;
-      dg[c * VEC + i] = db[c * VEC + i] = 0.f;
-    }
-  int half = 0;
-  for (unsigned long long first = (unsigned long long)blockIdx.x * per_block; first < a.rows; first += (unsigned long long)gridDim.x * per_block) {
-    const unsigned long long row = first + sub;
+  for (int i = 0; i < E; ++i) dg[i] = db[i] = 0.f;
+  // the next row is on its way while this one is worked on; a row's values are taken from its bits twice, before and after the sums
+  struct Row {
+    Raw<T, VEC> x[NV], dy[NV], dh[NV];
+    float mean, rstd;
+  } next, now;
+  const unsigned long long step = (unsigned long long)gridDim.x * per_block;
+  auto fetch = [&](unsigned long long row) {
     const bool on = row < a.rows;
-    const unsigned long long at = row * a.n;
-    float u[E], dy[E];
+    next.mean = on ? a.mean[row] : 0.f;
+    next.rstd = on ? a.rstd[row] : 0.f;
 #pragma unroll
     for (int c = 0; c < NV; ++c) {
       const unsigned int e = (c * TPR + t) * VEC;
-      float v[VEC], w[VEC];
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) v[i] = w[i] = 0.f;
+      next.x[c].clear();
+      next.dy[c].clear();
+      next.dh[c].clear();
       if (on && e < a.n) {
-        Vec<T, VEC>::load((const T*)a.x + at + e, v);
-        Vec<T, VEC>::load((const T*)a.dy + at + e, w);
+        next.x[c].load((const T*)a.x + row * a.n + e);
+        next.dy[c].load((const T*)a.dy + row * a.n + e);
+        if (a.dh) next.dh[c].load((const T*)a.dh + row * a.n + e);
       }
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) { u[c * VEC + i] = v[i]; dy[c * VEC + i] = w[i]; }
     }
-    const float mean = on ? a.mean[row] : 0.f, rstd = on ? a.rstd[row] : 0.f;
+  };
+  int half = 0;
+  fetch((unsigned long long)blockIdx.x * per_block + sub);
+  __syncthreads();
+  for (unsigned long long first = (unsigned long long)blockIdx.x * per_block; first < a.rows; first += step) {
+    const unsigned long long row = first + sub;
+    const bool on = row < a.rows;
+    now = next;
+    fetch(row + step);
     float s[2] = {0.f, 0.f};
 #pragma unroll
-    for (int c = 0; c < NV; ++c)
+    for (int c = 0; c < NV; ++c) {
+      float u[VEC], dy[VEC];
+      now.x[c].values(u);
+      now.dy[c].values(dy);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
         const int k = c * VEC + i;
-        u[k] = on && (c * TPR + t) * VEC + i < a.n ? (u[k] - mean) * rstd : 0.f;
-        const float g = dy[k] * ga[k];
+        // (behind the row's end dy and gamma are zero)
+        u[i] = (u[i] - now.mean) * now.rstd;
+        const float g = dy[i] * weights[(c * TPR + t) * VEC + i];
         s[0] += g;
-        s[1] = fmaf(g, u[k], s[1]);
-        dg[k] = fmaf(dy[k], u[k], dg[k]);
-        db[k] += dy[k];
+        s[1] = fmaf(g, u[i], s[1]);
+        dg[k] = fmaf(dy[i], u[i], dg[k]);
+        db[k] += dy[i];
       }
+    }
     row_sum<TPR>(s, sh, half);
     half ^= 1;
     if (!on) continue;
@@ -196,22 +211,20 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_grad_rows(const No
     for (int c = 0; c < NV; ++c) {
       const unsigned int e = (c * TPR + t) * VEC;
       if (e >= a.n) continue;
-      float v[VEC], w[VEC];
+      float v[VEC], dy[VEC], w[VEC];
+      now.x[c].values(v);
+      now.dy[c].values(dy);
+      now.dh[c].values(w);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) w[i] = 0.f;
-      if (a.dh) Vec<T, VEC>::load((const T*)a.dh + at + e, w);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const int k = c * VEC + i;
-        v[i] = fmaf(rstd, dy[k] * ga[k] - m0 - u[k] * m1, w[i]);
-      }
-      Vec<T, VEC>::store((T*)a.dx + at + e, v);
+      for (int i = 0; i < VEC; ++i) v[i] = fmaf(now.rstd, dy[i] * weights[e + i] - m0 - (v[i] - now.mean) * now.rstd * m1, w[i]);
+      Vec<T, VEC>::store((T*)a.dx + row * a.n + e, v);
     }
   }
   if (!a.partial) return;
   // the block's groups of threads meet: columns[which][group][column]
   const unsigned int plane = per_block * a.n;
   if (per_block > 1) {
+    __syncthreads();
 #pragma unroll
     for (int c = 0; c < NV; ++c)
 #pragma unroll
@@ -375,16 +388,18 @@ typedef void (*NormKernel)(const NormArgs);
 
 struct NormPlan {
   NormKernel kernel = nullptr;
-  unsigned int block = 0, tpr = 0;
+  unsigned int block = 0, tpr = 0, elements = 0;       // elements a thread
 };
 
 template <class T, int VEC, int NV>
 NormPlan rows_of(bool grad, unsigned int n) {
   const unsigned int e = VEC * NV;
-  if (n <= 8 * e) return {grad ? norm_grad_rows<T, VEC, NV, 8> : norm_rows<T, VEC, NV, 8>, kBlock, 8};
-  if (n <= 32 * e) return {grad ? norm_grad_rows<T, VEC, NV, 32> : norm_rows<T, VEC, NV, 32>, kBlock, 32};
-  if (n <= 128 * e) return {grad ? norm_grad_rows<T, VEC, NV, 128> : norm_rows<T, VEC, NV, 128>, kBlock, 128};
-  return {grad ? norm_grad_rows<T, VEC, NV, 512> : norm_rows<T, VEC, NV, 512>, 512, 512};
+  // (a gradient's blocks are larger: each leaves a row of partial sums)
+  const unsigned int block = grad ? 512 : 256;
+  if (n <= 8 * e) return {grad ? norm_grad_rows<T, VEC, NV, 8> : norm_rows<T, VEC, NV, 8>, block, 8, e};
+  if (n <= 32 * e) return {grad ? norm_grad_rows<T, VEC, NV, 32> : norm_rows<T, VEC, NV, 32>, block, 32, e};
+  if (n <= 128 * e) return {grad ? norm_grad_rows<T, VEC, NV, 128> : norm_rows<T, VEC, NV, 128>, block, 128, e};
+  return {grad ? norm_grad_rows<T, VEC, NV, 512> : norm_rows<T, VEC, NV, 512>, 512, 512, e};
 }
 
 // The group of threads is the smallest that holds a row at 16 elements a thread; rows of at most half of what it holds
@@ -393,10 +408,11 @@ template <class T>
 NormPlan plan_of(bool grad, unsigned int n, bool vec) {
   constexpr int V = 16 / (int)sizeof(T);
   if (n > 8192) {
-    if (vec) return {grad ? norm_grad_wide<T, V> : norm_wide<T, V>, 1024, 1024};
-    return {grad ? norm_grad_wide<T, 1> : norm_wide<T, 1>, 1024, 1024};
+    if (vec) return {grad ? norm_grad_wide<T, V> : norm_wide<T, V>, 1024, 1024, 0};
+    return {grad ? norm_grad_wide<T, 1> : norm_wide<T, 1>, 1024, 1024, 0};
   }
-  if (!vec) return rows_of<T, 1, 16>(grad, n);
+  // (single elements: 16 of them a thread, twice for the next row, would not fit its registers)
+  if (!vec) return n <= 4096 ? rows_of<T, 1, 8>(grad, n) : rows_of<T, 1, 16>(grad, n);
   const unsigned int g = n <= 128 ? 8 : n <= 512 ? 32 : n <= 2048 ? 128 : 512;
   return n <= g * 8 ? rows_of<T, V, 8 / V>(grad, n) : rows_of<T, V, 16 / V>(grad, n);
 }
@@ -417,7 +433,8 @@ struct NormOperator : b200_operator {
     plan = dtype == B200_F32 ? plan_of<float>(grad, a.n, vec) : dtype == B200_BF16 ? plan_of<__nv_bfloat16>(grad, a.n, vec) : plan_of<__half>(grad, a.n, vec);
     const unsigned int per_block = plan.block / plan.tpr;
     const bool wide = plan.tpr == 1024;
-    smem = grad && per_block > 1 ? 2 * (size_t)per_block * a.n * 4 : 0;
+    smem = wide ? 0 : (size_t)plan.tpr * plan.elements * 4 * (grad ? 1 : 2);
+    if (grad && per_block > 1 && !wide) smem = std::max(smem, 2 * (size_t)per_block * a.n * 4);
     ready(plan.kernel, smem);
     int resident = 0;
     rt_check(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, plan.kernel, (int)plan.block, smem), "occupancy");

@@ -25,9 +25,12 @@ struct RotaryArgs {
   unsigned int heads[2], d, pairs;
   unsigned int per_block;              // tokens
   unsigned int turn_items, items;      // of a head: accesses that turn, all accesses
+  Divisor by_pairs, by_items, by_heads;
   float magnitude;
   int inverse;
 };
+
+constexpr int kAtOnce = 4;             // accesses of a thread under way together
 
 template <class T, int VEC, bool INTERLEAVED>
 __global__ void __launch_bounds__(256) rotary(const RotaryArgs a) {
@@ -35,8 +38,37 @@ __global__ void __launch_bounds__(256) rotary(const RotaryArgs a) {
   grid_begin();
   const unsigned long long first = (unsigned long long)blockIdx.x * a.per_block;
   const unsigned int n = (unsigned int)min((unsigned long long)a.per_block, a.tokens - first);
+  const unsigned int heads = a.heads[0] + a.heads[1], total = n * heads * a.items;
+  // One access: where it lies, and its elements.  Half pairs have their second elements `pairs` further.
+  struct Item {
+    T* y;
+    const T* x;
+    unsigned int tok, item;
+    Raw<T, VEC> u, v;
+  } it[kAtOnce];
+  auto fetch = [&](unsigned int i, Item& t) {
+    if (i >= total) return;
+    const unsigned int row = a.by_items.of(i), tok = a.by_heads.of(row), head = row - tok * heads;
+    t.item = i - row * a.items;
+    t.tok = tok;
+    const bool second = head >= a.heads[0];
+    const unsigned long long at = ((first + tok) * a.heads[second] + (second ? head - a.heads[0] : head)) * a.d;
+    unsigned int e;
+    if (t.item >= a.turn_items) e = 2 * a.pairs + (t.item - a.turn_items) * VEC;
+    else e = INTERLEAVED && VEC == 1 ? 2 * t.item : t.item * VEC;
+    t.x = (const T*)a.x[second] + at + e;
+    t.y = (T*)a.y[second] + at + e;
+    t.u.load(t.x);
+    if (t.item < a.turn_items) {
+      if constexpr (!INTERLEAVED) t.v.load(t.x + a.pairs);
+      else if constexpr (VEC == 1) t.v.load(t.x + 1);
+    }
+  };
+  // the first accesses are under way while the table is made
+#pragma unroll
+  for (int k = 0; k < kAtOnce; ++k) fetch(threadIdx.x + 256 * k, it[k]);
   for (unsigned int i = threadIdx.x; i < n * a.pairs; i += 256) {
-    const unsigned int tok = i / a.pairs, pair = i - tok * a.pairs;
+    const unsigned int tok = a.by_pairs.of(i), pair = i - tok * a.pairs;
     const unsigned long long t = first + tok;
     const long long p = a.positions ? (long long)a.positions[t] : a.first_position + (long long)(t % a.seq);
     unsigned long long turn = (unsigned long long)p * a.turns[pair];
@@ -48,50 +80,44 @@ __global__ void __launch_bounds__(256) rotary(const RotaryArgs a) {
     table[i] = make_float2(c * a.magnitude, s * a.magnitude);
   }
   __syncthreads();
-  const unsigned int heads = a.heads[0] + a.heads[1], total = n * heads * a.items;
-#pragma unroll 2
-  for (unsigned int i = threadIdx.x; i < total; i += 256) {
-    const unsigned int row = i / a.items, item = i - row * a.items;
-    const unsigned int tok = row / heads, head = row - tok * heads;
-    const bool second = head >= a.heads[0];
-    const unsigned long long at = ((first + tok) * a.heads[second] + (second ? head - a.heads[0] : head)) * a.d;
-    const T* x = (const T*)a.x[second] + at;
-    T* y = (T*)a.y[second] + at;
-    const float2* cs = table + tok * a.pairs;
-    if (item >= a.turn_items) {          // elements that do not turn
-      const unsigned int e = 2 * a.pairs + (item - a.turn_items) * VEC;
-      if constexpr (VEC == 1) y[e] = x[e];
-      else *(uint4*)(y + e) = *(const uint4*)(x + e);
-    } else if constexpr (INTERLEAVED) {
-      constexpr int P = VEC == 1 ? 1 : VEC / 2;
-      float v[2 * P];
-      const unsigned int e = item * 2 * P;
-      if constexpr (VEC == 1) { v[0] = to_float(x[e]); v[1] = to_float(x[e + 1]); }
-      else Vec<T, VEC>::load(x + e, v);
+  for (unsigned int base = 0; base < total; base += 256 * kAtOnce) {
 #pragma unroll
-      for (int k = 0; k < P; ++k) {
-        const float2 w = cs[item * P + k];
-        const float u0 = v[2 * k], u1 = v[2 * k + 1];
-        v[2 * k] = u0 * w.x - u1 * w.y;
-        v[2 * k + 1] = u0 * w.y + u1 * w.x;
+    for (int k = 0; k < kAtOnce; ++k) {
+      const unsigned int i = base + threadIdx.x + 256 * k;
+      if (i >= total) continue;
+      const Item& t = it[k];
+      if (t.item >= a.turn_items) {          // elements that do not turn
+        if constexpr (VEC == 1) *t.y = t.u.r;
+        else *(uint4*)t.y = t.u.r;
+        continue;
       }
-      if constexpr (VEC == 1) { from_float(v[0], y[e]); from_float(v[1], y[e + 1]); }
-      else Vec<T, VEC>::store(y + e, v);
-    } else {
+      const float2* cs = table + t.tok * a.pairs;
       float u[VEC], v[VEC];
-      const unsigned int e = item * VEC;
-      Vec<T, VEC>::load(x + e, u);
-      Vec<T, VEC>::load(x + a.pairs + e, v);
+      t.u.values(u);
+      if constexpr (INTERLEAVED && VEC > 1) {
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) {
-        const float2 w = cs[e + k];
-        const float u0 = u[k], u1 = v[k];
-        u[k] = u0 * w.x - u1 * w.y;
-        v[k] = u0 * w.y + u1 * w.x;
+        for (int q = 0; q < VEC / 2; ++q) {
+          const float2 w = cs[t.item * (VEC / 2) + q];
+          v[2 * q] = u[2 * q] * w.x - u[2 * q + 1] * w.y;
+          v[2 * q + 1] = u[2 * q] * w.y + u[2 * q + 1] * w.x;
+        }
+        Vec<T, VEC>::store(t.y, v);
+      } else {
+        t.v.values(v);
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) {
+          const float2 w = cs[t.item * VEC + q];
+          const float u0 = u[q], u1 = v[q];
+          u[q] = u0 * w.x - u1 * w.y;
+          v[q] = u0 * w.y + u1 * w.x;
+        }
+        Vec<T, VEC>::store(t.y, u);
+        Vec<T, VEC>::store(INTERLEAVED ? t.y + 1 : t.y + a.pairs, v);
       }
-      Vec<T, VEC>::store(y + e, u);
-      Vec<T, VEC>::store(y + a.pairs + e, v);
     }
+    if (base + 256 * kAtOnce < total)
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) fetch(base + 256 * (kAtOnce + k) + threadIdx.x, it[k]);
   }
 }
 
@@ -158,6 +184,9 @@ extern "C" int b200_rotary_link(b200_dev* dev, const b200_rotary* p, b200_operat
     unsigned long long tok = std::max(1ull, 1024ull / per_token);
     tok = std::min(tok, std::max(1ull, tokens / (2ull * (unsigned)dev->sm_count)));
     if (a.pairs) tok = std::min(tok, std::max(1ull, 4096ull / a.pairs));
+    a.by_pairs = Divisor(std::max(1u, a.pairs));
+    a.by_items = Divisor(a.items);
+    a.by_heads = Divisor(a.heads[0] + a.heads[1]);
     if (tok * per_token >> 31) ops.refuse("a token has too many elements", B200_E_UNSUPPORTED);
     a.per_block = (unsigned int)tok;
     op->grid = (tokens + tok - 1) / tok;
