@@ -8,22 +8,26 @@
 //            A operand of dv += p^T do and dk += ds^T q.
 //   queries  a CTA has 128 queries of one head and walks the tiles of keys they see: s = q k^T, dp = do v^T, dq += ds k.
 //
-// Eight warps do the arithmetic, two threads a row, 64 columns each; one warp copies, one issues the products.  Weights are
-// formed while the second product runs, the score gradients while the next tile's scores are: with 512 columns of tensor memory
-// in use a CTA has an SM to itself.
+// A thread does 64 columns of a row; one warp copies, one issues the products.  Weights are formed while the second product runs, the
+// score gradients while the next tile's scores are.  Heads of more than 64 elements take tiles of 128 columns, two threads a row, and
+// all of tensor memory; those of up to 64 tiles of 64 columns, a thread a row, and half of it, so that two CTAs share an SM (short
+// sequences are bound by the chain from a CTA's start to its end).  Copies start before anything else.
 #ifndef B200_ATTN_BWD_SM100_CUH
 #define B200_ATTN_BWD_SM100_CUH
 #include "attn_fwd_sm100.cuh"
 
 namespace b200 {
 
-template <int DP>
+// CW: columns of a tile, that is queries (or keys) of one step; 64 a thread.
+template <int DP, int CW>
 struct BwdShape {
-  static constexpr int kPanels = DP / 64;
-  static constexpr unsigned int kTile = kPanels * kTileBytes64;
-  static constexpr unsigned int kThreads = 320;
-  static constexpr unsigned int kStage = 2 * kTile + 1024;        // two tiles, and a tile of row statistics
+  static constexpr int kPanels = DP / 64, kGroups = CW / 64;                 // groups of four warps
+  static constexpr unsigned int kTile = kPanels * kTileBytes64;              // the CTA's own rows
+  static constexpr unsigned int kPanel = CW * 128, kStep = kPanels * kPanel; // a tile of the others
+  static constexpr unsigned int kThreads = kGroups * 128 + 64, kWarps = kThreads / 32;
+  static constexpr unsigned int kStage = 2 * kStep + 1024;                   // two tiles, and the queries' statistics (8 bytes each)
   static constexpr unsigned int kBytes = 2 * kTile + 2 * kStage;
+  static constexpr unsigned int kColumns = 2 * CW + 2 * DP <= 256 && 3 * CW + DP <= 256 ? 256 : 512;
   static constexpr size_t smem(int tiles) { return 1024 + kBytes + 256 + (size_t)tiles; }
 };
 
@@ -102,25 +106,21 @@ __device__ __forceinline__ bool store_columns(unsigned char* tile, unsigned int 
   return bad == 0.f;
 }
 
-// Score of one pair from the product: `z` in units of log 2, `slack` = 1 - tanh^2
-template <bool CAP, bool BIAS>
-__device__ __forceinline__ float pair_score(float x, float c, float to_tanh, float slope2, float far, float& slack) {
-  if constexpr (CAP) {
-    x = tanh_of(x * to_tanh);
-    slack = fmaf(-x, x, 1.f);
-  }
+// Score of one pair in units of log 2, from tanh(x / cap) or x
+template <bool BIAS>
+__device__ __forceinline__ float pair_score(float x, float c, float slope2, float far) {
   x *= c;
   if constexpr (BIAS) x = fmaf(-slope2, fabsf(far), x);
   return x;
 }
 
 // ------------------------------------------------------------------ keys
-template <class T, int DP, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(320, 1)
+template <class T, int DP, int CW, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(BwdShape<DP, CW>::kThreads, CW == 64 ? 2 : 1)
 attn_grad_keys_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant__ b200_tmap map_k, const __grid_constant__ b200_tmap map_v,
                   const __grid_constant__ b200_tmap map_do, const __grid_constant__ b200_tmap map_dk, const __grid_constant__ b200_tmap map_dv,
                   const __grid_constant__ AttnArgs a) {
-  typedef BwdShape<DP> Sh;
+  typedef BwdShape<DP, CW> Sh;
   extern __shared__ __align__(128) unsigned char dyn[];
   const unsigned int base = (b200_smem_addr(dyn) + 1023u) & ~1023u;
   unsigned char* const gen = dyn + (base - b200_smem_addr(dyn));
@@ -131,55 +131,81 @@ attn_grad_keys_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant
   const unsigned int bar_s = bar0 + 40, bar_dp = bar0 + 48, bar_p = bar0 + 56, bar_ds = bar0 + 64, bar_done = bar0 + 72;
   volatile unsigned int* tmem_slot = (volatile unsigned int*)(bars + 10);
   volatile unsigned int* abort_flag = tmem_slot + 1;
-  volatile unsigned int* repair = tmem_slot + 2;          // [2]: dv, dk
   float* scratch = (float*)(bars + 12);                   // [10]
   unsigned char* classes = (unsigned char*)(gen + Sh::kBytes + 256);
 
   asm volatile("griddepcontrol.launch_dependents;");
   const unsigned int warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-  if (threadIdx.x == 0) {
-    b200_mbar_init(bar_kv, 1);
-    for (int i = 0; i < 2; ++i) {
-      b200_mbar_init(bar_full + 8 * i, 1);
-      b200_mbar_init(bar_empty + 8 * i, 1);
-      repair[i] = 0u;
-    }
-    b200_mbar_init(bar_s, 1);
-    b200_mbar_init(bar_dp, 1);
-    b200_mbar_init(bar_p, 256);
-    b200_mbar_init(bar_ds, 256);
-    b200_mbar_init(bar_done, 1);
-    *abort_flag = 0u;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  if (warp == 9) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(b200_smem_addr((const void*)tmem_slot)), "r"(512u) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-
+  constexpr unsigned int kLoad = Sh::kWarps - 2, kMma = Sh::kWarps - 1;
   // this CTA's keys: the first ones first, which under a causal mask are seen by the most queries
   const unsigned int heads = (unsigned int)a.B * (unsigned int)a.HK;
   const int j0 = (int)(blockIdx.x / heads) * 128;
   const unsigned int bh = blockIdx.x % heads;
   const int b = (int)(bh / (unsigned int)a.HK), hk = (int)(bh % (unsigned int)a.HK);
-  const int tiles = (a.S + 127) / 128;
+  const int tiles = (a.S + CW - 1) / CW, stat_tiles = (a.S + 127) / 128;
+  const bool docs = a.kdoc != nullptr;
+  if (threadIdx.x == kLoad * 32) {
+    b200_mbar_init(bar_kv, 1);
+    for (int i = 0; i < 2; ++i) {
+      b200_mbar_init(bar_full + 8 * i, 1);
+      b200_mbar_init(bar_empty + 8 * i, 1);
+    }
+    b200_mbar_init(bar_s, 1);
+    b200_mbar_init(bar_dp, 1);
+    b200_mbar_init(bar_p, Sh::kGroups * 128);
+    b200_mbar_init(bar_ds, Sh::kGroups * 128);
+    b200_mbar_init(bar_done, 1);
+    *abort_flag = 0u;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kMma) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(b200_smem_addr((const void*)tmem_slot)), "r"(Sh::kColumns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const AttnSeq seq = attn_seq(a, b);
+  if (threadIdx.x == kLoad * 32) {
+    b200_mbar_expect_tx(bar_kv, 2 * Sh::kTile);
+#pragma unroll
+    for (int p = 0; p < Sh::kPanels; ++p) {
+      b200_tma_load_4d(k_at + p * kTileBytes64, &map_k, bar_kv, p * 64, j0, hk, b);
+      b200_tma_load_4d(v_at + p * kTileBytes64, &map_v, bar_kv, p * 64, j0, hk, b);
+    }
+  }
+  // queries: a tile of CW; `n`: tiles taken so far
+  auto load = [&](int h, int t, unsigned int n) {
+    const unsigned int slot = n & 1u, at = ring + slot * Sh::kStage, bar = bar_full + 8 * slot;
+    b200_mbar_expect_tx(bar, 2 * Sh::kStep + CW * 8);
+#pragma unroll
+    for (int p = 0; p < Sh::kPanels; ++p) {
+      b200_tma_load_4d(at + p * Sh::kPanel, &map_q, bar, p * 64, t * CW, h, b);
+      b200_tma_load_4d(at + Sh::kStep + p * Sh::kPanel, &map_do, bar, p * 64, t * CW, h, b);
+    }
+    const float* stat = a.stat + (((long long)b * a.H + h) * stat_tiles + t * CW / 128) * 256 + t * CW % 128;
+    bulk_load(at + 2 * Sh::kStep, stat, CW * 4, bar);
+    bulk_load(at + 2 * Sh::kStep + CW * 4, stat + 128, CW * 4, bar);
+  };
+  auto class_without = [&](int t) { return tile_class(plain_span(a, seq, t * CW, CW), j0, 128, false, 0, 0, false); };
+  int early = -1;             // the tile that is on its way before the others are known
+  if (!docs)
+    for (early = 0; early < tiles && !class_without(early); ++early) {}
+  if (threadIdx.x == kLoad * 32 && early >= 0 && early < tiles) load(hk * a.group, early, 0);
   tc_before();
   __syncthreads();
   tc_after();
   const float grad_unit = gradient_unit<T>(a, scratch);
-  {
+  if (docs) {
     int kmin = 0, kmax = 0;
     bool negative = false;
-    if (a.kdoc) key_documents(a, b, j0, lane, kmin, kmax, negative);
-    for (int t = (int)warp; t < tiles; t += 10) {
+    key_documents<128>(a, b, j0, lane, kmin, kmax, negative);
+    for (int t = (int)warp; t < tiles; t += (int)Sh::kWarps) {
       AttnSpan s;
       s.last_min = s.doc_min = 0x7fffffff;
       s.last_max = -1;
       s.doc_max = -0x7fffffff - 1;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = t * 128 + 32 * i + (int)lane;
+      for (int i = 0; i < CW / 32; ++i) {
+        const int r = t * CW + 32 * i + (int)lane;
         AttnRow w;
         w.last = w.doc = 0;
         if (r < a.S) w = attn_row(a, b, r);
@@ -189,63 +215,57 @@ attn_grad_keys_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant
         s.doc_min = min(s.doc_min, p.doc_min);
         s.doc_max = max(s.doc_max, p.doc_max);
       }
-      if (lane == 0) classes[t] = (unsigned char)tile_class(s, j0, a.kdoc != nullptr, kmin, kmax, negative);
+      if (lane == 0) classes[t] = (unsigned char)tile_class(s, j0, 128, true, kmin, kmax, negative);
     }
+    __syncthreads();
   }
-  __syncthreads();
+  auto class_of = [&](int t) { return docs ? (unsigned int)classes[t] : class_without(t); };
+  const int begin = docs ? 0 : early;       // (without documents the tiles that see the keys are the last ones)
   const unsigned int tmem = *tmem_slot;
-  const unsigned int t_s = tmem, t_dp = tmem + 128, t_dv = tmem + 256, t_dk = tmem + 256 + DP;
+  const unsigned int t_s = tmem, t_dp = tmem + CW, t_dv = tmem + 2 * CW, t_dk = tmem + 2 * CW + DP;
 
-  if (warp == 8) {
-    if (b200_elect()) {
-      b200_mbar_expect_tx(bar_kv, 2 * Sh::kTile);
-#pragma unroll
-      for (int p = 0; p < Sh::kPanels; ++p) {
-        b200_tma_load_4d(k_at + p * kTileBytes64, &map_k, bar_kv, p * 64, j0, hk, b);
-        b200_tma_load_4d(v_at + p * kTileBytes64, &map_v, bar_kv, p * 64, j0, hk, b);
-      }
+  if (warp == kLoad) {
+    if (lane == 0) {
       unsigned int n = 0;
       bool live = true;
       for (int h = hk * a.group; h < (hk + 1) * a.group && live; ++h)
-        for (int t = 0; t < tiles; ++t) {
-          if (!classes[t]) continue;
-          const unsigned int slot = n & 1u, use = n >> 1, at = ring + slot * Sh::kStage, bar = bar_full + 8 * slot;
-          if (use) live = b200_wait(bar_empty + 8 * slot, (use - 1) & 1u, abort_flag, a.status, 31u);
-          if (!live) break;
-          b200_mbar_expect_tx(bar, Sh::kStage);
-#pragma unroll
-          for (int p = 0; p < Sh::kPanels; ++p) {
-            b200_tma_load_4d(at + p * kTileBytes64, &map_q, bar, p * 64, t * 128, h, b);
-            b200_tma_load_4d(at + Sh::kTile + p * kTileBytes64, &map_do, bar, p * 64, t * 128, h, b);
+        for (int t = begin; t < tiles; ++t) {
+          if (!class_of(t)) continue;
+          if (docs || n) {
+            if (n > 1) live = b200_wait(bar_empty + 8 * (n & 1u), ((n >> 1) - 1) & 1u, abort_flag, a.status, 31u);
+            if (!live) break;
+            load(h, t, n);
           }
-          bulk_load(at + 2 * Sh::kTile, a.stat + (((long long)b * a.H + h) * tiles + t) * 256, 1024, bar);
           ++n;
         }
-      if (*abort_flag)
+      // the copies under way land before shared memory is given up, whatever happened to the others
+      if (*abort_flag) {
+        for (int tries = 0; tries < 1 << 20 && !b200_mbar_try(bar_kv, 0u); ++tries) {}
         for (unsigned int i = 0; i < 2 && i < n; ++i)
           for (int tries = 0; tries < 1 << 20 && !b200_mbar_try(bar_full + 8 * ((n - 1 - i) & 1u), ((n - 1 - i) >> 1) & 1u); ++tries) {}
+      }
     }
     __syncwarp();
-  } else if (warp == 9) {
+  } else if (warp == kMma) {
     if (b200_elect()) {
-      constexpr unsigned int idesc_s = idesc_of<T>(128, 128, false, false), idesc_g = idesc_of<T>(128, DP, false, true);
-      // 128 x 128 of two k-major tiles
+      constexpr unsigned int idesc_s = idesc_of<T>(128, CW, false, false), idesc_g = idesc_of<T>(128, DP, false, true);
+      // 128 x CW of two k-major tiles
       auto square = [&](unsigned int d, unsigned int x, unsigned int y) {
 #pragma unroll
         for (int p = 0; p < Sh::kPanels; ++p) {
-          const unsigned long long dx = b200_smem_desc(x + p * kTileBytes64, 16u, 1024u), dy = b200_smem_desc(y + p * kTileBytes64, 16u, 1024u);
+          const unsigned long long dx = b200_smem_desc(x + p * kTileBytes64, 16u, 1024u), dy = b200_smem_desc(y + p * Sh::kPanel, 16u, 1024u);
 #pragma unroll
           for (unsigned int ks = 0; ks < 4; ++ks) b200_umma(d, dx + ks * 2, dy + ks * 2, idesc_s, (p || ks) ? 1u : 0u);
         }
       };
-      // += (16-bit rows in tensor memory, the halves 64 columns apart) x (tile read along its rows)
+      // += (16-bit rows in tensor memory, 64 columns of the tile in each 64) x (tile read along its rows)
       auto product = [&](unsigned int d, unsigned int x, unsigned int y, bool add) {
-        const unsigned long long dy = b200_smem_desc(y, kTileBytes64, 1024u);
+        const unsigned long long dy = b200_smem_desc(y, Sh::kPanel, 1024u);
 #pragma unroll
-        for (unsigned int ks = 0; ks < 8; ++ks) umma_ts(d, x + (ks >> 2) * 64 + (ks & 3u) * 8, dy + ks * 128, idesc_g, (add || ks) ? 1u : 0u);
+        for (unsigned int ks = 0; ks < CW / 16; ++ks) umma_ts(d, x + (ks >> 2) * 64 + (ks & 3u) * 8, dy + ks * 128, idesc_g, (add || ks) ? 1u : 0u);
       };
       int total = 0;
-      for (int t = 0; t < tiles; ++t) total += classes[t] != 0;
+      for (int t = begin; t < tiles; ++t) total += class_of(t) != 0;
       total *= a.group;
       bool live = b200_wait(bar_kv, 0u, abort_flag, a.status, 32u);
       if (live && total) {
@@ -254,7 +274,7 @@ attn_grad_keys_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant
         if (live) {
           square(t_s, k_at, ring);
           b200_umma_commit(bar_s);
-          square(t_dp, v_at, ring + Sh::kTile);
+          square(t_dp, v_at, ring + Sh::kStep);
           b200_umma_commit(bar_dp);
         }
       }
@@ -263,7 +283,7 @@ attn_grad_keys_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant
         live = b200_wait(bar_p, n & 1, abort_flag, a.status, 34u);
         if (!live) break;
         tc_after();
-        product(t_dv, t_s, at + Sh::kTile, n != 0);
+        product(t_dv, t_s, at + Sh::kStep, n != 0);
         if (n + 1 < total) {
           live = b200_wait(bar_full + 8 * ((n + 1) & 1), ((n + 1) >> 1) & 1, abort_flag, a.status, 35u);
           if (!live) break;
@@ -277,7 +297,7 @@ attn_grad_keys_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant
         product(t_dk, t_dp, at, n != 0);
         b200_umma_commit(bar_empty + 8 * (n & 1));
         if (n + 1 < total) {
-          square(t_dp, v_at, next + Sh::kTile);
+          square(t_dp, v_at, next + Sh::kStep);
           b200_umma_commit(bar_dp);
         } else {
           b200_umma_commit(bar_done);
@@ -288,117 +308,134 @@ attn_grad_keys_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant
   } else {
     const unsigned int half = warp >> 2, in = (warp & 3u) * 32 + lane, lanes = (warp & 3u) << 21;
     const unsigned int my_s = t_s + 64 * half + lanes, my_dp = t_dp + 64 * half + lanes;
-    const float c = CAP ? a.cap * kLog2e : a.scale * kLog2e, to_tanh = CAP ? 2.f * kLog2e * a.scale / a.cap : 0.f;
+    const float c = CAP ? a.cap * kLog2e : a.scale * kLog2e, to_tanh = CAP ? a.scale / a.cap : 0.f;
     const int j = j0 + (int)in;
-    const int len = a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
     unsigned int n = 0;
     bool live = true;
     for (int h = hk * a.group; h < (hk + 1) * a.group && live; ++h) {
       const float slope2 = BIAS ? a.slopes[h] * kLog2e : 0.f;
-      for (int t = 0; t < tiles; ++t) {
-        const unsigned int cls = classes[t];
+      for (int t = begin; t < tiles; ++t) {
+        const unsigned int cls = class_of(t);
         if (!cls) continue;
-        const float* stat = (const float*)(gen + 2 * Sh::kTile + (n & 1u) * Sh::kStage + 2 * Sh::kTile) + 64 * half;
+        const float* stat = (const float*)(gen + 2 * Sh::kTile + (n & 1u) * Sh::kStage + 2 * Sh::kStep) + 64 * half;
         unsigned int bits[2] = {0xffffffffu, 0xffffffffu};
-        const int r0 = t * 128 + 64 * (int)half;
+        const int r0 = t * CW + 64 * (int)half;
         if (cls == 2u) visible_queries(a, b, r0, j, lane, bits);
         live = b200_wait(bar_full + 8 * (n & 1u), (n >> 1) & 1u, abort_flag, a.status, 37u) && b200_wait(bar_s, n & 1u, abort_flag, a.status, 38u);
         if (!live) break;
         tc_after();
         float w[64];            // weights, times 1 - tanh^2 with a cap
+        // (two forms: the mask costs three instructions an element)
+        auto weights = [&](auto masked) {
+          constexpr bool M = decltype(masked)::value;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          float x[32];
-          unsigned int u[16];
-          b200_tmem_ld32(my_s + 32 * k, (unsigned int*)x);
-          const float far = BIAS ? (float)(len - a.S + r0 + 32 * k - j) : 0.f;
-          tmem_wait_ld();
+          for (int k = 0; k < 2; ++k) {
+            float x[32];
+            unsigned int u[16];
+            b200_tmem_ld32(my_s + 32 * k, (unsigned int*)x);
+            [[maybe_unused]] const float far = BIAS ? (float)(seq.len - a.S + r0 + 32 * k - j) : 0.f;
+            tmem_wait_ld();
+            if constexpr (CAP) tanh_chunk(x, to_tanh);
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            const float4 l = *(const float4*)(stat + 32 * k + i);
-            const float lse2[4] = {l.x, l.y, l.z, l.w};
+            for (int i = 0; i < 32; i += 4) {
+              const float4 l = *(const float4*)(stat + 32 * k + i);
+              const float lse2[4] = {l.x, l.y, l.z, l.w};
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              float slack = 1.f, p;
-              if constexpr (!CAP && !BIAS) p = ex2(fmaf(x[i + q], c, -lse2[q]));
-              else p = ex2(pair_score<CAP, BIAS>(x[i + q], c, to_tanh, slope2, far + (float)(i + q), slack) - lse2[q]);
-              if (cls == 2u) p = (bits[k] >> (i + q)) & 1u ? p : 0.f;
-              x[i + q] = p;
-              w[32 * k + i + q] = CAP ? p * slack : p;
+              for (int q = 0; q < 4; ++q) {
+                float p;
+                if constexpr (!BIAS) p = ex2(fmaf(x[i + q], c, -lse2[q]));
+                else p = ex2(pair_score<BIAS>(x[i + q], c, slope2, far + (float)(i + q)) - lse2[q]);
+                if constexpr (M) p = (bits[k] >> (i + q)) & 1u ? p : 0.f;
+                w[32 * k + i + q] = CAP ? p * fmaf(-x[i + q], x[i + q], 1.f) : p;
+                x[i + q] = p;
+              }
+              u[i / 2] = pack2(x[i], x[i + 1], T());
+              u[i / 2 + 1] = pack2(x[i + 2], x[i + 3], T());
             }
-            u[i / 2] = pack2(x[i], x[i + 1], T());
-            u[i / 2 + 1] = pack2(x[i + 2], x[i + 3], T());
+            tmem_st16(my_s + 16 * k, u);
           }
-          tmem_st16(my_s + 16 * k, u);
-        }
+        };
+        if (cls == 2u) weights(std::true_type());
+        else weights(std::false_type());
         tmem_wait_st();
         tc_before();
         b200_mbar_arrive(bar_p);
         live = b200_wait(bar_dp, n & 1u, abort_flag, a.status, 39u);
         if (!live) break;
         tc_after();
+        auto gradients = [&](auto masked) {
+          constexpr bool M = decltype(masked)::value;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          float x[32];
-          unsigned int u[16];
-          b200_tmem_ld32(my_dp + 32 * k, (unsigned int*)x);
-          tmem_wait_ld();
+          for (int k = 0; k < 2; ++k) {
+            float x[32];
+            unsigned int u[16];
+            b200_tmem_ld32(my_dp + 32 * k, (unsigned int*)x);
+            tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            const float4 l = *(const float4*)(stat + 128 + 32 * k + i);
-            const float delta[4] = {l.x, l.y, l.z, l.w};
+            for (int i = 0; i < 32; i += 4) {
+              const float4 l = *(const float4*)(stat + CW + 32 * k + i);
+              const float delta[4] = {l.x, l.y, l.z, l.w};
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              float ds = w[32 * k + i + q] * (x[i + q] - delta[q]);
-              if constexpr (std::is_same<T, __half>::value) ds *= grad_unit;
-              if (cls == 2u) ds = (bits[k] >> (i + q)) & 1u ? ds : 0.f;
-              x[i + q] = ds;
+              for (int q = 0; q < 4; ++q) {
+                float ds = w[32 * k + i + q] * (x[i + q] - delta[q]);
+                if constexpr (std::is_same<T, __half>::value) ds *= grad_unit;
+                if constexpr (M) ds = (bits[k] >> (i + q)) & 1u ? ds : 0.f;
+                x[i + q] = ds;
+              }
+              u[i / 2] = pack2(x[i], x[i + 1], T());
+              u[i / 2 + 1] = pack2(x[i + 2], x[i + 3], T());
             }
-            u[i / 2] = pack2(x[i], x[i + 1], T());
-            u[i / 2 + 1] = pack2(x[i + 2], x[i + 3], T());
+            tmem_st16(my_dp + 16 * k, u);
           }
-          tmem_st16(my_dp + 16 * k, u);
-        }
+        };
+        if (cls == 2u) gradients(std::true_type());
+        else gradients(std::false_type());
         tmem_wait_st();
         tc_before();
         b200_mbar_arrive(bar_ds);
         ++n;
       }
     }
-    // ---- dv by the first four warps, dk by the others, through the tiles of v and k
+    // ---- dv and dk, 32 rows a warp, through the tiles of v and k: by the first four warps and the others, or one after the other
     if (live) live = b200_wait(n ? bar_done : bar_kv, 0u, abort_flag, a.status, 40u);
     tc_after();
-    const unsigned int from = (half ? t_dk : t_dv) + lanes;
-    unsigned char* tile = gen + (half ? 0 : Sh::kTile);
-    const float by = half ? a.scale / grad_unit : 1.f;
-    bool fine = true;
+    const int first = j0 + (int)(warp & 3u) * 32;
+    unsigned int mend[2] = {0u, 0u};           // rows of dv, of dk that are to be done again
 #pragma unroll
-    for (int e = 0; e < DP; e += 32) {
-      float o[32];
-      if (live && n) {
-        b200_tmem_ld32(from + e, (unsigned int*)o);
-        tmem_wait_ld();
+    for (int which = 0; which < 2; ++which) {
+      if (Sh::kGroups == 2 && which != (int)half) continue;
+      const unsigned int from = (which ? t_dk : t_dv) + lanes;
+      unsigned char* tile = gen + (which ? 0 : Sh::kTile);
+      const float by = which ? a.scale / grad_unit : 1.f;
+      bool fine = true;
+#pragma unroll
+      for (int e = 0; e < DP; e += 32) {
+        float o[32];
+        if (live && n) {
+          b200_tmem_ld32(from + e, (unsigned int*)o);
+          tmem_wait_ld();
+        }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = n ? o[i] * by : 0.f;
+        fine &= store_columns<T>(tile, in, e, o);
       }
+      mend[which] = __ballot_sync(0xffffffffu, live && j < a.T && !fine);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0 && live && first < a.T) {
 #pragma unroll
-      for (int i = 0; i < 32; ++i) o[i] = n ? o[i] * by : 0.f;
-      fine &= store_columns<T>(tile, in, e, o);
+        for (int p = 0; p < Sh::kPanels; ++p)
+          if (p * 64 < a.D) b200_tma_store_4d(which ? &map_dk : &map_dv, b200_smem_addr(tile) + p * kTileBytes64 + (warp & 3u) * 4096, p * 64, first, hk, b);
+      }
     }
-    const bool mend = live && j < a.T && !fine;
-    if (mend) repair[half] = 1u;
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    named_barrier(1 + (int)half, 128);
-    if ((threadIdx.x & 127u) == 0 && live) {
-#pragma unroll
-      for (int p = 0; p < Sh::kPanels; ++p)
-        if (p * 64 < a.D) b200_tma_store_4d(half ? &map_dk : &map_dv, b200_smem_addr(tile) + p * kTileBytes64, p * 64, j0, hk, b);
-      if (repair[half]) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    if (lane == 0 && live) {
+      if (mend[0] | mend[1]) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
       else b200_tma_store_read_wait<0>();
     }
-    if (repair[half]) {
-      named_barrier(1 + (int)half, 128);
-      for (unsigned int todo = __ballot_sync(0xffffffffu, mend); todo; todo &= todo - 1)
-        attn_dkv_row<T>(a, b, hk, j0 + (int)((warp & 3u) * 32) + __ffs(todo) - 1, lane, half ? 1 : 2);
-    }
+    __syncwarp();
+#pragma unroll
+    for (int which = 0; which < 2; ++which)
+      for (unsigned int todo = mend[which]; todo; todo &= todo - 1) attn_dkv_row<T>(a, b, hk, first + __ffs(todo) - 1, lane, which ? 1 : 2);
   }
   __syncwarp();
   if (*abort_flag) {
@@ -407,18 +444,18 @@ attn_grad_keys_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant
   }
   tc_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == kMma) {
     tc_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Sh::kColumns) : "memory");
   }
 }
 
 // ------------------------------------------------------------------ queries
-template <class T, int DP, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(320, 1)
+template <class T, int DP, int CW, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(BwdShape<DP, CW>::kThreads, CW == 64 ? 2 : 1)
 attn_grad_queries_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant__ b200_tmap map_k, const __grid_constant__ b200_tmap map_v,
                      const __grid_constant__ b200_tmap map_do, const __grid_constant__ b200_tmap map_dq, const __grid_constant__ AttnArgs a) {
-  typedef BwdShape<DP> Sh;
+  typedef BwdShape<DP, CW> Sh;
   extern __shared__ __align__(128) unsigned char dyn[];
   const unsigned int base = (b200_smem_addr(dyn) + 1023u) & ~1023u;
   unsigned char* const gen = dyn + (base - b200_smem_addr(dyn));
@@ -429,14 +466,20 @@ attn_grad_queries_tc(const __grid_constant__ b200_tmap map_q, const __grid_const
   const unsigned int bar_dp = bar0 + 56, bar_ds = bar0 + 64, bar_done = bar0 + 72;
   volatile unsigned int* tmem_slot = (volatile unsigned int*)(bars + 10);
   volatile unsigned int* abort_flag = tmem_slot + 1;
-  volatile unsigned int* repair = tmem_slot + 2;
   float* scratch = (float*)(bars + 12);
   AttnSpan* span = (AttnSpan*)(bars + 18);
   unsigned char* classes = (unsigned char*)(gen + Sh::kBytes + 256);
 
   asm volatile("griddepcontrol.launch_dependents;");
   const unsigned int warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-  if (threadIdx.x == 0) {
+  constexpr unsigned int kLoad = Sh::kWarps - 2, kMma = Sh::kWarps - 1;
+  const unsigned int heads = (unsigned int)a.B * (unsigned int)a.H;
+  const int tiles_q = (a.S + 127) / 128;
+  const int t_q = tiles_q - 1 - (int)(blockIdx.x / heads), r0 = t_q * 128;
+  const unsigned int bh = blockIdx.x % heads;
+  const int b = (int)(bh / (unsigned int)a.H), h = (int)(bh % (unsigned int)a.H), hk = h / a.group;
+  const bool docs = a.kdoc != nullptr;
+  if (threadIdx.x == kLoad * 32) {
     b200_mbar_init(bar_q, 1);
     for (int i = 0; i < 2; ++i) {
       b200_mbar_init(bar_full + 8 * i, 1);
@@ -444,98 +487,106 @@ attn_grad_queries_tc(const __grid_constant__ b200_tmap map_q, const __grid_const
       b200_mbar_init(bar_s + 8 * i, 1);
     }
     b200_mbar_init(bar_dp, 1);
-    b200_mbar_init(bar_ds, 256);
+    b200_mbar_init(bar_ds, Sh::kGroups * 128);
     b200_mbar_init(bar_done, 1);
-    *repair = 0u;
     span->last_min = span->doc_min = 0x7fffffff;
     span->last_max = -1;
     span->doc_max = -0x7fffffff - 1;
     *abort_flag = 0u;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 9) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(b200_smem_addr((const void*)tmem_slot)), "r"(512u) : "memory");
+  if (warp == kMma) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(b200_smem_addr((const void*)tmem_slot)), "r"(Sh::kColumns) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
-
-  const unsigned int heads = (unsigned int)a.B * (unsigned int)a.H;
-  const int tiles_q = (a.S + 127) / 128;
-  const int t_q = tiles_q - 1 - (int)(blockIdx.x / heads), r0 = t_q * 128;
-  const unsigned int bh = blockIdx.x % heads;
-  const int b = (int)(bh / (unsigned int)a.H), h = (int)(bh % (unsigned int)a.H), hk = h / a.group;
+  const AttnSpan plain = plain_span(a, attn_seq(a, b), r0, 128);
+  int tiles = (plain.last_max + CW) / CW;
+  auto load = [&](int t, unsigned int n) {
+    const unsigned int slot = n & 1u, at = ring + slot * Sh::kStage, bar = bar_full + 8 * slot;
+    b200_mbar_expect_tx(bar, 2 * Sh::kStep);
+#pragma unroll
+    for (int p = 0; p < Sh::kPanels; ++p) {
+      b200_tma_load_4d(at + p * Sh::kPanel, &map_k, bar, p * 64, t * CW, hk, b);
+      b200_tma_load_4d(at + Sh::kStep + p * Sh::kPanel, &map_v, bar, p * 64, t * CW, hk, b);
+    }
+  };
+  if (threadIdx.x == kLoad * 32) {
+    b200_mbar_expect_tx(bar_q, 2 * Sh::kTile);
+#pragma unroll
+    for (int p = 0; p < Sh::kPanels; ++p) {
+      b200_tma_load_4d(q_at + p * kTileBytes64, &map_q, bar_q, p * 64, r0, h, b);
+      b200_tma_load_4d(do_at + p * kTileBytes64, &map_do, bar_q, p * 64, r0, h, b);
+    }
+    if (!docs && tiles) load(0, 0);
+  }
   const unsigned int half = warp >> 2, in = (warp & 3u) * 32 + lane;
   const int r = r0 + (int)in;
   AttnRow row;
   row.pos = 0; row.last = -1; row.doc = 0;
+  if (warp < kLoad && r < a.S) row = attn_row(a, b, r);
   tc_before();
   __syncthreads();
   tc_after();
   const float grad_unit = gradient_unit<T>(a, scratch);
-  if (warp < 8) {
-    if (r < a.S) row = attn_row(a, b, r);
-    const AttnSpan s = span_of(r < a.S, row);
-    if (lane == 0) {
-      atomicMin(&span->last_min, s.last_min);
-      atomicMax(&span->last_max, s.last_max);
-      atomicMin(&span->doc_min, s.doc_min);
-      atomicMax(&span->doc_max, s.doc_max);
-    }
-  }
-  __syncthreads();
-  const int tiles = (span->last_max + 128) / 128;
-  for (int t = (int)warp; t < tiles; t += 10) {
-    int kmin = 0, kmax = 0;
-    bool negative = false;
-    if (a.kdoc) key_documents(a, b, t * 128, lane, kmin, kmax, negative);
-    const unsigned int cls = tile_class(*span, t * 128, a.kdoc != nullptr, kmin, kmax, negative);
-    if (lane == 0) classes[t] = (unsigned char)cls;
-  }
-  __syncthreads();
-  const unsigned int tmem = *tmem_slot;
-  const unsigned int t_dp = tmem + 256, t_dq = tmem + 384;     // two tiles of scores ahead of them
-
-  if (warp == 8) {
-    if (b200_elect()) {
-      b200_mbar_expect_tx(bar_q, 2 * Sh::kTile);
-#pragma unroll
-      for (int p = 0; p < Sh::kPanels; ++p) {
-        b200_tma_load_4d(q_at + p * kTileBytes64, &map_q, bar_q, p * 64, r0, h, b);
-        b200_tma_load_4d(do_at + p * kTileBytes64, &map_do, bar_q, p * 64, r0, h, b);
+  if (docs) {
+    if (warp < 4) {
+      const AttnSpan s = span_of(r < a.S, row);
+      if (lane == 0) {
+        atomicMin(&span->last_min, s.last_min);
+        atomicMax(&span->last_max, s.last_max);
+        atomicMin(&span->doc_min, s.doc_min);
+        atomicMax(&span->doc_max, s.doc_max);
       }
+    }
+    __syncthreads();
+    tiles = (span->last_max + CW) / CW;
+    for (int t = (int)warp; t < tiles; t += (int)Sh::kWarps) {
+      int kmin = 0, kmax = 0;
+      bool negative = false;
+      key_documents<CW>(a, b, t * CW, lane, kmin, kmax, negative);
+      const unsigned int cls = tile_class(*span, t * CW, CW, true, kmin, kmax, negative);
+      if (lane == 0) classes[t] = (unsigned char)cls;
+    }
+    __syncthreads();
+  }
+  auto class_of = [&](int t) { return docs ? (unsigned int)classes[t] : tile_class(plain, t * CW, CW, false, 0, 0, false); };
+  const unsigned int tmem = *tmem_slot;
+  const unsigned int t_dp = tmem + 2 * CW, t_dq = tmem + 3 * CW;     // two tiles of scores ahead of them
+
+  if (warp == kLoad) {
+    if (lane == 0) {
       unsigned int n = 0;
       bool live = true;
       for (int t = 0; t < tiles; ++t) {
-        if (!classes[t]) continue;
-        const unsigned int slot = n & 1u, use = n >> 1, at = ring + slot * Sh::kStage, bar = bar_full + 8 * slot;
-        if (use) live = b200_wait(bar_empty + 8 * slot, (use - 1) & 1u, abort_flag, a.status, 41u);
-        if (!live) break;
-        b200_mbar_expect_tx(bar, 2 * Sh::kTile);
-#pragma unroll
-        for (int p = 0; p < Sh::kPanels; ++p) {
-          b200_tma_load_4d(at + p * kTileBytes64, &map_k, bar, p * 64, t * 128, hk, b);
-          b200_tma_load_4d(at + Sh::kTile + p * kTileBytes64, &map_v, bar, p * 64, t * 128, hk, b);
+        if (!class_of(t)) continue;
+        if (docs || n) {
+          if (n > 1) live = b200_wait(bar_empty + 8 * (n & 1u), ((n >> 1) - 1) & 1u, abort_flag, a.status, 41u);
+          if (!live) break;
+          load(t, n);
         }
         ++n;
       }
-      if (*abort_flag)
+      if (*abort_flag) {
+        for (int tries = 0; tries < 1 << 20 && !b200_mbar_try(bar_q, 0u); ++tries) {}
         for (unsigned int i = 0; i < 2 && i < n; ++i)
           for (int tries = 0; tries < 1 << 20 && !b200_mbar_try(bar_full + 8 * ((n - 1 - i) & 1u), ((n - 1 - i) >> 1) & 1u); ++tries) {}
+      }
     }
     __syncwarp();
-  } else if (warp == 9) {
+  } else if (warp == kMma) {
     if (b200_elect()) {
-      constexpr unsigned int idesc_s = idesc_of<T>(128, 128, false, false), idesc_g = idesc_of<T>(128, DP, false, true);
+      constexpr unsigned int idesc_s = idesc_of<T>(128, CW, false, false), idesc_g = idesc_of<T>(128, DP, false, true);
       auto square = [&](unsigned int d, unsigned int x, unsigned int y) {
 #pragma unroll
         for (int p = 0; p < Sh::kPanels; ++p) {
-          const unsigned long long dx = b200_smem_desc(x + p * kTileBytes64, 16u, 1024u), dy = b200_smem_desc(y + p * kTileBytes64, 16u, 1024u);
+          const unsigned long long dx = b200_smem_desc(x + p * kTileBytes64, 16u, 1024u), dy = b200_smem_desc(y + p * Sh::kPanel, 16u, 1024u);
 #pragma unroll
           for (unsigned int ks = 0; ks < 4; ++ks) b200_umma(d, dx + ks * 2, dy + ks * 2, idesc_s, (p || ks) ? 1u : 0u);
         }
       };
       int total = 0;
-      for (int t = 0; t < tiles; ++t) total += classes[t] != 0;
+      for (int t = 0; t < tiles; ++t) total += class_of(t) != 0;
       bool live = b200_wait(bar_q, 0u, abort_flag, a.status, 42u);
       if (live && total) {
         live = b200_wait(bar_full, 0u, abort_flag, a.status, 43u);
@@ -543,7 +594,7 @@ attn_grad_queries_tc(const __grid_constant__ b200_tmap map_q, const __grid_const
         if (live) {
           square(tmem, q_at, ring);
           b200_umma_commit(bar_s);
-          square(t_dp, do_at, ring + Sh::kTile);
+          square(t_dp, do_at, ring + Sh::kStep);
           b200_umma_commit(bar_dp);
         }
       }
@@ -553,18 +604,18 @@ attn_grad_queries_tc(const __grid_constant__ b200_tmap map_q, const __grid_const
           live = b200_wait(bar_full + 8 * ((n + 1) & 1), ((n + 1) >> 1) & 1, abort_flag, a.status, 44u);
           if (!live) break;
           tc_after();
-          square(tmem + 128 * ((n + 1) & 1), q_at, next);
+          square(tmem + CW * ((n + 1) & 1), q_at, next);
           b200_umma_commit(bar_s + 8 * ((n + 1) & 1));
         }
         live = b200_wait(bar_ds, n & 1, abort_flag, a.status, 45u);
         if (!live) break;
         tc_after();
-        const unsigned long long dk = b200_smem_desc(at, kTileBytes64, 1024u);
+        const unsigned long long dk = b200_smem_desc(at, Sh::kPanel, 1024u);
 #pragma unroll
-        for (unsigned int ks = 0; ks < 8; ++ks) umma_ts(t_dq, t_dp + (ks >> 2) * 64 + (ks & 3u) * 8, dk + ks * 128, idesc_g, (n || ks) ? 1u : 0u);
+        for (unsigned int ks = 0; ks < CW / 16; ++ks) umma_ts(t_dq, t_dp + (ks >> 2) * 64 + (ks & 3u) * 8, dk + ks * 128, idesc_g, (n || ks) ? 1u : 0u);
         b200_umma_commit(bar_empty + 8 * (n & 1));
         if (n + 1 < total) {
-          square(t_dp, do_at, next + Sh::kTile);
+          square(t_dp, do_at, next + Sh::kStep);
           b200_umma_commit(bar_dp);
         } else {
           b200_umma_commit(bar_done);
@@ -575,71 +626,83 @@ attn_grad_queries_tc(const __grid_constant__ b200_tmap map_q, const __grid_const
   } else {
     const unsigned int lanes = (warp & 3u) << 21;
     const unsigned int my_dp = t_dp + 64 * half + lanes;
-    const float c = CAP ? a.cap * kLog2e : a.scale * kLog2e, to_tanh = CAP ? 2.f * kLog2e * a.scale / a.cap : 0.f;
+    const float c = CAP ? a.cap * kLog2e : a.scale * kLog2e, to_tanh = CAP ? a.scale / a.cap : 0.f;
     const float slope2 = BIAS ? a.slopes[h] * kLog2e : 0.f;
     const float* stat = a.stat + (((long long)b * a.H + h) * tiles_q + t_q) * 256 + in;
     const float lse2 = stat[0], delta = stat[128];
     unsigned int n = 0;
     bool live = true;
     for (int t = 0; t < tiles; ++t) {
-      const unsigned int cls = classes[t];
+      const unsigned int cls = class_of(t);
       if (!cls) continue;
-      unsigned int all[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
-      if (cls == 2u) visible_words(a, b, t * 128, row, lane, all);
-      const unsigned int bits[2] = {half ? all[2] : all[0], half ? all[3] : all[1]};
+      unsigned int bits[2] = {0xffffffffu, 0xffffffffu};
+      if (cls == 2u) visible_words<2>(a, b, t * CW + 64 * (int)half, row, lane, bits);
       live = b200_wait(bar_s + 8 * (n & 1u), (n >> 1) & 1u, abort_flag, a.status, 46u);
       if (!live) break;
       tc_after();
       float w[64];
-      const unsigned int my_s = tmem + 128 * (n & 1u) + 64 * half + lanes;
+      const unsigned int my_s = tmem + CW * (n & 1u) + 64 * half + lanes;
+      auto weights = [&](auto masked) {
+        constexpr bool M = decltype(masked)::value;
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        float x[32];
-        b200_tmem_ld32(my_s + 32 * k, (unsigned int*)x);
-        const float far = BIAS ? (float)(row.pos - t * 128 - 64 * (int)half - 32 * k) : 0.f;
-        tmem_wait_ld();
+        for (int k = 0; k < 2; ++k) {
+          float x[32];
+          b200_tmem_ld32(my_s + 32 * k, (unsigned int*)x);
+          [[maybe_unused]] const float far = BIAS ? (float)(row.pos - t * CW - 64 * (int)half - 32 * k) : 0.f;
+          tmem_wait_ld();
+          if constexpr (CAP) tanh_chunk(x, to_tanh);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          float slack = 1.f, p;
-          if constexpr (!CAP && !BIAS) p = ex2(fmaf(x[i], c, -lse2));
-          else p = ex2(pair_score<CAP, BIAS>(x[i], c, to_tanh, slope2, far - (float)i, slack) - lse2);
-          if (cls == 2u) p = (bits[k] >> i) & 1u ? p : 0.f;
-          if constexpr (std::is_same<T, __half>::value) p *= grad_unit;
-          w[32 * k + i] = CAP ? p * slack : p;
+          for (int i = 0; i < 32; ++i) {
+            float p;
+            if constexpr (!BIAS) p = ex2(fmaf(x[i], c, -lse2));
+            else p = ex2(pair_score<BIAS>(x[i], c, slope2, far - (float)i) - lse2);
+            if constexpr (M) p = (bits[k] >> i) & 1u ? p : 0.f;
+            if constexpr (std::is_same<T, __half>::value) p *= grad_unit;
+            w[32 * k + i] = CAP ? p * fmaf(-x[i], x[i], 1.f) : p;
+          }
         }
-      }
+      };
+      if (cls == 2u) weights(std::true_type());
+      else weights(std::false_type());
       live = b200_wait(bar_dp, n & 1u, abort_flag, a.status, 47u);
       if (!live) break;
       tc_after();
+      auto gradients = [&](auto masked) {
+        constexpr bool M = decltype(masked)::value;
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        float x[32];
-        unsigned int u[16];
-        b200_tmem_ld32(my_dp + 32 * k, (unsigned int*)x);
-        tmem_wait_ld();
+        for (int k = 0; k < 2; ++k) {
+          float x[32];
+          unsigned int u[16];
+          b200_tmem_ld32(my_dp + 32 * k, (unsigned int*)x);
+          tmem_wait_ld();
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          x[i] = w[32 * k + i] * (x[i] - delta);
-          if (cls == 2u) x[i] = (bits[k] >> i) & 1u ? x[i] : 0.f;
+          for (int i = 0; i < 32; ++i) {
+            x[i] = w[32 * k + i] * (x[i] - delta);
+            if constexpr (M) x[i] = (bits[k] >> i) & 1u ? x[i] : 0.f;
+          }
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) u[i / 2] = pack2(x[i], x[i + 1], T());
+          tmem_st16(my_dp + 16 * k, u);
         }
-#pragma unroll
-        for (int i = 0; i < 32; i += 2) u[i / 2] = pack2(x[i], x[i + 1], T());
-        tmem_st16(my_dp + 16 * k, u);
-      }
+      };
+      if (cls == 2u) gradients(std::true_type());
+      else gradients(std::false_type());
       tmem_wait_st();
       tc_before();
       b200_mbar_arrive(bar_ds);
       ++n;
     }
-    // ---- dq through the queries' tile, half of a row's elements a thread
+    // ---- dq through the queries' tile: 32 rows a warp, half of a row's elements where two threads share it
     if (live) live = b200_wait(n ? bar_done : bar_q, 0u, abort_flag, a.status, 48u);
     tc_after();
     const float by = a.scale / grad_unit;
+    const int first = r0 + (int)(warp & 3u) * 32;
+    constexpr int kMine = DP / Sh::kGroups;
     bool fine = true;
 #pragma unroll
-    for (int e = 0; e < DP / 2; e += 32) {
+    for (int e = 0; e < kMine; e += 32) {
       float o[32];
-      const int col = (int)half * (DP / 2) + e;
+      const int col = (int)half * kMine + e;
       if (live && n) {
         b200_tmem_ld32(t_dq + lanes + col, (unsigned int*)o);
         tmem_wait_ld();
@@ -648,22 +711,33 @@ attn_grad_queries_tc(const __grid_constant__ b200_tmap map_q, const __grid_const
       for (int i = 0; i < 32; ++i) o[i] = n ? o[i] * by : 0.f;
       fine &= store_columns<T>(gen, in, col, o);
     }
-    const bool mend = live && r < a.S && !fine;
-    if (mend) *repair = 1u;
+    unsigned int mend = __ballot_sync(0xffffffffu, live && r < a.S && !fine);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    named_barrier(1, 256);
-    if (threadIdx.x == 0 && live) {
+    __syncwarp();
+    if (lane == 0 && live && first < a.S) {
 #pragma unroll
-      for (int p = 0; p < Sh::kPanels; ++p)
-        if (p * 64 < a.D) b200_tma_store_4d(&map_dq, q_at + p * kTileBytes64, p * 64, r0, h, b);
-      if (*repair) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+      for (int p = (int)half * kMine / 64; p < ((int)half + 1) * kMine / 64; ++p)
+        if (p * 64 < a.D) b200_tma_store_4d(&map_dq, q_at + p * kTileBytes64 + (warp & 3u) * 4096, p * 64, first, h, b);
+    }
+    bool all_out = mend != 0u;         // whether the copies have to be complete, not only read
+    if (Sh::kGroups == 2) {
+      // two warps share their rows: a row to be done again is done by the first, when both halves are out
+      volatile unsigned int* mends = (volatile unsigned int*)(bars + 22);
+      if (lane == 0) mends[warp] = mend;
+      named_barrier(1 + (int)(warp & 3u), 64);
+      mend |= mends[warp ^ 4u];
+      all_out = mend != 0u;
+    }
+    if (lane == 0 && live) {
+      if (all_out) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
       else b200_tma_store_read_wait<0>();
     }
-    if (*repair) {
-      named_barrier(1, 256);
-      // (a row whose halves are both to be mended is done twice, with the same result)
-      for (unsigned int todo = __ballot_sync(0xffffffffu, mend); todo; todo &= todo - 1) attn_dq_row<T>(a, b, h, r0 + (int)((warp & 3u) * 32) + __ffs(todo) - 1, lane);
+    __syncwarp();
+    if (Sh::kGroups == 2 && all_out) {
+      named_barrier(1 + (int)(warp & 3u), 64);
+      if (half) mend = 0u;
     }
+    for (unsigned int todo = mend; todo; todo &= todo - 1) attn_dq_row<T>(a, b, h, first + __ffs(todo) - 1, lane);
   }
   __syncwarp();
   if (*abort_flag) {
@@ -672,9 +746,9 @@ attn_grad_queries_tc(const __grid_constant__ b200_tmap map_q, const __grid_const
   }
   tc_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == kMma) {
     tc_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Sh::kColumns) : "memory");
   }
 }
 

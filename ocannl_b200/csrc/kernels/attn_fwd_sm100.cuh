@@ -8,8 +8,12 @@
 // grown by more than 2^8 (weights stay below that, sums and accumulators are single precision, so nothing is lost): after the
 // first tiles hardly ever.  With NQ = 2 the two tiles take turns on the tensor cores and on the arithmetic; with NQ = 1 two CTAs of an SM do.
 //
-// Key tiles that no query of a tile sees are skipped, and those that all see take no mask: the classes of all key tiles are made
-// first, from the rows' last keys and the range of document numbers in each tile.
+// Key tiles that no query of a tile sees are skipped, and those that all see take no mask: known from the rows' last keys alone, or, with
+// documents, from classes made first for all key tiles from the range of document numbers in each.
+//
+// Short sequences are bound by the chain from a CTA's start to its end (64 sequences of 256 positions, 8 heads of 64: 9600 cycles, of which
+// 1200 were the classes, 1800 the wait for the first operands, 1800 the way out): so the copies start before anything else, and every
+// warp sends its own 32 rows out.
 #ifndef B200_ATTN_FWD_SM100_CUH
 #define B200_ATTN_FWD_SM100_CUH
 #include "attn_terms.cuh"
@@ -35,6 +39,56 @@ __device__ __forceinline__ float rcp(float x) {
 }
 // tanh x = 1 - 2 / (e^2x + 1), of which 2 x log2(e) is given; off by a few 2^-24 (absolute), which a cap multiplies
 __device__ __forceinline__ float tanh_of(float two_x_log2e) { return fmaf(-2.f, rcp(ex2(two_x_log2e) + 1.f), 1.f); }
+
+// Pairs of single-precision values in one instruction (the multiply-add pipe takes both in the issue slot of one).
+struct Pair {
+  unsigned long long v;
+  __device__ __forceinline__ Pair() {}
+  __device__ __forceinline__ Pair(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+  __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+};
+__device__ __forceinline__ Pair fma2(const Pair& a, const Pair& b, const Pair& c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ Pair mul2(const Pair& a, const Pair& b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Pair add2(const Pair& a, const Pair& b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+
+// x = tanh(x scale) of 32 scores.  The exponential and the reciprocal of tanh_of pass through the unit that also has to make the
+// weights, at an eighth of the multiply-adds' rate, and would bound the kernel: where all of a warp's scores are at most the cap in
+// size, tanh y = y P(y^2) instead, with P the polynomial of degree 5 whose largest error of y P on [0, 1] is least (2.4e-7; fitted by
+// iterated weighted least squares; 3.0e-7 in single precision).  2 x 4096 positions, 16 heads of 128, causal: 301 us without, 172 with it.
+__device__ __forceinline__ void tanh_chunk(float (&x)[32], float scale) {
+  float top = 0.f;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) top = fmaxf(top, fabsf(x[j]));
+  if (__any_sync(0xffffffffu, top * scale > 1.f)) {
+    const float s = 2.f * kLog2e * scale;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) x[j] = tanh_of(x[j] * s);
+    return;
+  }
+  const Pair s(scale, scale);
+#pragma unroll
+  for (int j = 0; j < 32; j += 2) {
+    const Pair y = mul2(Pair(x[j], x[j + 1]), s), z = mul2(y, y);
+    Pair p = fma2(z, Pair(-0.0028394637629389763f, -0.0028394637629389763f), Pair(0.01611417718231678f, 0.01611417718231678f));
+    p = fma2(p, z, Pair(-0.05097286030650139f, -0.05097286030650139f));
+    p = fma2(p, z, Pair(0.13253524899482727f, 0.13253524899482727f));
+    p = fma2(p, z, Pair(-0.3332400321960449f, -0.3332400321960449f));
+    p = fma2(p, z, Pair(0.9999968409538269f, 0.9999968409538269f));
+    mul2(p, y).get(x[j], x[j + 1]);
+  }
+}
 
 // A from tensor memory: 16-bit elements, two to a column
 __device__ __forceinline__ void umma_ts(unsigned int d, unsigned int a, unsigned long long b, unsigned int idesc, unsigned int accumulate) {
@@ -67,6 +121,14 @@ __host__ __device__ constexpr unsigned int idesc_of(int m, int n, bool a_mn, boo
 struct AttnSpan {
   int last_min, last_max, doc_min, doc_max;
 };
+// of rows r0 .. r0 + n - 1, without documents
+__device__ __forceinline__ AttnSpan plain_span(const AttnArgs& a, const AttnSeq& q, int r0, int n) {
+  AttnSpan s;
+  s.last_min = r0 < a.S ? attn_last(a, q, r0) : 0x7fffffff;
+  s.last_max = r0 < a.S ? attn_last(a, q, min(r0 + n, a.S) - 1) : -1;
+  s.doc_min = s.doc_max = 0;
+  return s;
+}
 __device__ __forceinline__ AttnSpan span_of(bool ok, const AttnRow& w) {
   AttnSpan s;
   s.last_min = __reduce_min_sync(0xffffffffu, ok ? w.last : 0x7fffffff);
@@ -76,17 +138,18 @@ __device__ __forceinline__ AttnSpan span_of(bool ok, const AttnRow& w) {
   return s;
 }
 // 0: no row sees a key of the tile, 1: every row sees every key, 2: some
-__device__ __forceinline__ unsigned int tile_class(const AttnSpan& s, int j0, bool docs, int kmin, int kmax, bool negative) {
+__device__ __forceinline__ unsigned int tile_class(const AttnSpan& s, int j0, int width, bool docs, int kmin, int kmax, bool negative) {
   if (j0 > s.last_max) return 0u;
-  if (!docs) return j0 + 127 <= s.last_min ? 1u : 2u;
+  if (!docs) return j0 + width - 1 <= s.last_min ? 1u : 2u;
   if (kmax < s.doc_min || kmin > s.doc_max) return 0u;
-  return (j0 + 127 <= s.last_min && !negative && kmin == kmax && s.doc_min == s.doc_max && s.doc_min == kmin) ? 1u : 2u;
+  return (j0 + width - 1 <= s.last_min && !negative && kmin == kmax && s.doc_min == s.doc_max && s.doc_min == kmin) ? 1u : 2u;
 }
-// range of the non-negative documents of keys j0 .. j0 + 127 (a warp); `negative`: some are padding
+// range of the non-negative documents of W keys from j0 (a warp); `negative`: some are padding
+template <int W>
 __device__ __forceinline__ void key_documents(const AttnArgs& a, int b, int j0, unsigned int lane, int& kmin, int& kmax, bool& negative) {
   int lo = 0x7fffffff, hi = -1, bad = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < W / 32; ++i) {
     const int j = j0 + (int)lane + 32 * i;
     if (j < a.T) {
       const int d = a.kdoc[(long long)b * a.T + j];
@@ -98,17 +161,18 @@ __device__ __forceinline__ void key_documents(const AttnArgs& a, int b, int j0, 
   kmax = __reduce_max_sync(0xffffffffu, hi);
   negative = __any_sync(0xffffffffu, bad);
 }
-// Which of the 128 keys from j0 the lane's row sees, a bit each.  The rows of a warp belong to one document or a few: one round each.
-__device__ __forceinline__ void visible_words(const AttnArgs& a, int b, int j0, const AttnRow& w, unsigned int lane, unsigned int (&bits)[4]) {
+// Which of 32 N keys from j0 the lane's row sees, a bit each.  The rows of a warp belong to one document or a few: one round each.
+template <int N>
+__device__ __forceinline__ void visible_words(const AttnArgs& a, int b, int j0, const AttnRow& w, unsigned int lane, unsigned int (&bits)[N]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < N; ++i) {
     const int n = w.last + 1 - (j0 + 32 * i);       // keys of this word up to the last one
     bits[i] = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
   }
   if (!a.kdoc) return;
-  int d[4];
+  int d[N];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < N; ++i) {
     const int j = j0 + (int)lane + 32 * i;
     d[i] = j < a.T ? a.kdoc[(long long)b * a.T + j] : -1;
   }
@@ -117,7 +181,7 @@ __device__ __forceinline__ void visible_words(const AttnArgs& a, int b, int j0, 
     const int doc = __shfl_sync(0xffffffffu, w.doc, __ffs(todo) - 1);
     const bool mine = w.doc == doc;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < N; ++i) {
       const unsigned int same = __ballot_sync(0xffffffffu, d[i] == doc);
       if (mine) bits[i] &= same;
     }
@@ -125,51 +189,72 @@ __device__ __forceinline__ void visible_words(const AttnArgs& a, int b, int j0, 
   }
 }
 
-template <int DP, int NQ>
+// KW: keys of a tile.  With 64 the scores have two places in tensor memory, and those of the next tile are formed while the softmax of
+// this one runs; with 128 one, and they wait for its weights.
+template <int DP, int NQ, int KW>
 struct FwdShape {
-  static constexpr int kPanels = DP / 64;
-  static constexpr unsigned int kTile = kPanels * kTileBytes64;
-  // two slots each for keys and values; one, where two CTAs of 96 KB share an SM
-  static constexpr int kSlots = (DP == 128 && NQ == 1) ? 1 : 2;
+  static constexpr int kPanels = DP / 64, kScores = 128 / KW;
+  static constexpr unsigned int kTile = kPanels * kTileBytes64;              // queries
+  static constexpr unsigned int kPanel = KW * 128, kKeys = kPanels * kPanel; // keys or values
+  // slots for keys and for values: 64 KB together with two query tiles or two CTAs an SM
+  static constexpr int kSlots = (DP == 128 && NQ == 1) ? 128 / KW : 2 * 128 / KW;
   static constexpr unsigned int kThreads = NQ * 128 + 64;
-  static constexpr unsigned int kBytes = NQ * kTile + 2 * kSlots * kTile;
+  static constexpr unsigned int kBytes = NQ * kTile + 2 * kSlots * kKeys;
   static constexpr unsigned int kColumns = NQ * (128 + DP) <= 256 ? 256 : 512;
-  static constexpr size_t smem(int tiles) { return 1024 + kBytes + 256 + (size_t)tiles; }
+  static constexpr size_t smem(int tiles) { return 1024 + kBytes + 512 + (size_t)tiles; }
 };
 
-template <class T, int DP, int NQ, bool CAP, bool BIAS>
+template <class T, int DP, int NQ, int KW, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(NQ * 128 + 64, NQ == 1 ? 2 : 1)
 attn_forward_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant__ b200_tmap map_k, const __grid_constant__ b200_tmap map_v,
                 const __grid_constant__ b200_tmap map_o, const __grid_constant__ AttnArgs a) {
-  typedef FwdShape<DP, NQ> Sh;
+  typedef FwdShape<DP, NQ, KW> Sh;
   extern __shared__ __align__(128) unsigned char dyn[];
   const unsigned int base = (b200_smem_addr(dyn) + 1023u) & ~1023u;
   unsigned char* const gen = dyn + (base - b200_smem_addr(dyn));
-  const unsigned int q_at = base, k_at = base + NQ * Sh::kTile, v_at = k_at + Sh::kSlots * Sh::kTile;
+  const unsigned int q_at = base, k_at = base + NQ * Sh::kTile, v_at = k_at + Sh::kSlots * Sh::kKeys;
   unsigned long long* bars = (unsigned long long*)(gen + Sh::kBytes);
   const unsigned int bar0 = b200_smem_addr(bars);
-  const unsigned int bar_q = bar0, bar_kf = bar0 + 8, bar_ke = bar0 + 24, bar_vf = bar0 + 40, bar_ve = bar0 + 56;   // two each but bar_q
-  const unsigned int bar_s = bar0 + 72, bar_p = bar0 + 88, bar_o = bar0 + 104;                                       // a query tile each
-  volatile unsigned int* tmem_slot = (volatile unsigned int*)(bars + 16);
+  const unsigned int bar_q = bar0, bar_kf = bar0 + 8, bar_ke = bar0 + 40, bar_vf = bar0 + 72, bar_ve = bar0 + 104;   // four slots each but bar_q
+  const unsigned int bar_s = bar0 + 136, bar_p = bar0 + 168, bar_o = bar0 + 200;      // a query tile each; bar_s, bar_p: two places each
+  volatile unsigned int* tmem_slot = (volatile unsigned int*)(bars + 27);
   volatile unsigned int* abort_flag = tmem_slot + 1;
-  volatile unsigned int* repair = tmem_slot + 2;      // [2]: some row of the query tile came out infinite or undefined
-  AttnSpan* spans = (AttnSpan*)(bars + 18);           // [2], 16 bytes each
-  unsigned char* classes = (unsigned char*)(gen + Sh::kBytes + 256);
+  AttnSpan* spans = (AttnSpan*)(bars + 30);           // [2], 16 bytes each
+  unsigned char* classes = (unsigned char*)(gen + Sh::kBytes + 512);
 
   asm volatile("griddepcontrol.launch_dependents;");
   const unsigned int warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
   const unsigned int kLoad = NQ * 4, kMma = NQ * 4 + 1;
-  if (threadIdx.x == 0) {
+  // this CTA's queries: the last ones first, which under a causal mask see the most keys
+  const unsigned int heads = (unsigned int)a.B * (unsigned int)a.H;
+  const unsigned int tiles_q = (a.S + 128 * NQ - 1) / (128 * NQ);
+  const int r0 = (int)(tiles_q - 1 - blockIdx.x / heads) * 128 * NQ;
+  const unsigned int bh = blockIdx.x % heads;
+  const int b = (int)(bh / (unsigned int)a.H), h = (int)(bh % (unsigned int)a.H), hk = h / a.group;
+  const bool docs = a.kdoc != nullptr;
+
+  auto load_keys = [&](int t, unsigned int slot) {
+    b200_mbar_expect_tx(bar_kf + 8 * slot, Sh::kKeys);
+#pragma unroll
+    for (int p = 0; p < Sh::kPanels; ++p) b200_tma_load_4d(k_at + slot * Sh::kKeys + p * Sh::kPanel, &map_k, bar_kf + 8 * slot, p * 64, t * KW, hk, b);
+  };
+  auto load_values = [&](int t, unsigned int slot) {
+    b200_mbar_expect_tx(bar_vf + 8 * slot, Sh::kKeys);
+#pragma unroll
+    for (int p = 0; p < Sh::kPanels; ++p) b200_tma_load_4d(v_at + slot * Sh::kKeys + p * Sh::kPanel, &map_v, bar_vf + 8 * slot, p * 64, t * KW, hk, b);
+  };
+  if (threadIdx.x == kLoad * 32) {
     b200_mbar_init(bar_q, 1);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 4; ++i) {
       b200_mbar_init(bar_kf + 8 * i, 1);
       b200_mbar_init(bar_ke + 8 * i, 1);
       b200_mbar_init(bar_vf + 8 * i, 1);
       b200_mbar_init(bar_ve + 8 * i, 1);
       b200_mbar_init(bar_s + 8 * i, 1);
       b200_mbar_init(bar_p + 8 * i, 128);
+    }
+    for (int i = 0; i < 2; ++i) {
       b200_mbar_init(bar_o + 8 * i, 1);
-      repair[i] = 0u;
       spans[i].last_min = spans[i].doc_min = 0x7fffffff;
       spans[i].last_max = -1;
       spans[i].doc_max = -0x7fffffff - 1;
@@ -182,73 +267,85 @@ attn_forward_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant__
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
-
-  // this CTA's queries: the last ones first, which under a causal mask see the most keys
-  const unsigned int heads = (unsigned int)a.B * (unsigned int)a.H;
-  const unsigned int tiles_q = (a.S + 128 * NQ - 1) / (128 * NQ);
-  const int r0 = (int)(tiles_q - 1 - blockIdx.x / heads) * 128 * NQ;
-  const unsigned int bh = blockIdx.x % heads;
-  const int b = (int)(bh / (unsigned int)a.H), h = (int)(bh % (unsigned int)a.H), hk = h / a.group;
+  const AttnSeq seq = attn_seq(a, b);
+  AttnSpan span[NQ];
+  int n_tiles = 0;
+#pragma unroll
+  for (int i = 0; i < NQ; ++i) {
+    span[i] = plain_span(a, seq, r0 + 128 * i, 128);
+    n_tiles = max(n_tiles, (span[i].last_max + KW) / KW);
+  }
+  // the queries, and without documents the first keys and values, are on their way from here
+  if (threadIdx.x == kLoad * 32) {
+    b200_mbar_expect_tx(bar_q, NQ * Sh::kTile);
+#pragma unroll
+    for (int i = 0; i < NQ; ++i)
+#pragma unroll
+      for (int p = 0; p < Sh::kPanels; ++p) b200_tma_load_4d(q_at + i * Sh::kTile + p * kTileBytes64, &map_q, bar_q, p * 64, r0 + 128 * i, h, b);
+    if (!docs && n_tiles) {
+      load_keys(0, 0);
+      load_values(0, 0);
+    }
+  }
   const unsigned int g = warp >> 2;                        // query tile of a softmax warp
   const int r = r0 + (int)threadIdx.x;                     // row of a softmax thread
   AttnRow row;
   row.pos = 0; row.last = -1; row.doc = 0;
+  if (warp < kLoad && r < a.S) row = attn_row(a, b, r);
   tc_before();
   __syncthreads();
   tc_after();
-  if (warp < kLoad) {
-    if (r < a.S) row = attn_row(a, b, r);
-    const AttnSpan s = span_of(r < a.S, row);
-    if (lane == 0) {
-      atomicMin(&spans[g].last_min, s.last_min);
-      atomicMax(&spans[g].last_max, s.last_max);
-      atomicMin(&spans[g].doc_min, s.doc_min);
-      atomicMax(&spans[g].doc_max, s.doc_max);
+  if (docs) {
+    if (warp < kLoad) {
+      const AttnSpan s = span_of(r < a.S, row);
+      if (lane == 0) {
+        atomicMin(&spans[g].last_min, s.last_min);
+        atomicMax(&spans[g].last_max, s.last_max);
+        atomicMin(&spans[g].doc_min, s.doc_min);
+        atomicMax(&spans[g].doc_max, s.doc_max);
+      }
     }
-  }
-  __syncthreads();
-  int n_tiles = 0;
+    __syncthreads();
+    n_tiles = 0;
 #pragma unroll
-  for (int i = 0; i < NQ; ++i) n_tiles = max(n_tiles, (spans[i].last_max + 128) / 128);
-  for (int t = (int)warp; t < n_tiles; t += (int)(Sh::kThreads / 32)) {
-    int kmin = 0, kmax = 0;
-    bool negative = false;
-    if (a.kdoc) key_documents(a, b, t * 128, lane, kmin, kmax, negative);
-    unsigned int c = 0;
+    for (int i = 0; i < NQ; ++i) n_tiles = max(n_tiles, (spans[i].last_max + KW) / KW);
+    for (int t = (int)warp; t < n_tiles; t += (int)(Sh::kThreads / 32)) {
+      int kmin = 0, kmax = 0;
+      bool negative = false;
+      key_documents<KW>(a, b, t * KW, lane, kmin, kmax, negative);
+      unsigned int c = 0;
 #pragma unroll
-    for (int i = 0; i < NQ; ++i) c |= tile_class(spans[i], t * 128, a.kdoc != nullptr, kmin, kmax, negative) << (2 * i);
-    if (lane == 0) classes[t] = (unsigned char)c;
+      for (int i = 0; i < NQ; ++i) c |= tile_class(spans[i], t * KW, KW, true, kmin, kmax, negative) << (2 * i);
+      if (lane == 0) classes[t] = (unsigned char)c;
+    }
+    __syncthreads();
   }
-  __syncthreads();
+  // what query tile i sees of key tile t; what any does
+  auto class_of = [&](int t, int i) { return docs ? (classes[t] >> (2 * i)) & 3u : tile_class(span[i], t * KW, KW, false, 0, 0, false); };
+  auto seen_at = [&](int t) { return !docs || classes[t] != 0; };      // (without documents every tile up to the last one)
   const unsigned int tmem = *tmem_slot;
   const unsigned int acc_o = tmem + NQ * 128;              // output accumulators behind the scores
 
   if (warp == kLoad) {
-    if (b200_elect()) {
-      b200_mbar_expect_tx(bar_q, NQ * Sh::kTile);
-#pragma unroll
-      for (int i = 0; i < NQ; ++i)
-#pragma unroll
-        for (int p = 0; p < Sh::kPanels; ++p) b200_tma_load_4d(q_at + i * Sh::kTile + p * kTileBytes64, &map_q, bar_q, p * 64, r0 + 128 * i, h, b);
+    if (lane == 0) {
       unsigned int n = 0;
       bool live = true;
       for (int t = 0; t < n_tiles && live; ++t) {
-        if (!classes[t]) continue;
+        if (!seen_at(t)) continue;
         const unsigned int slot = n % Sh::kSlots, use = n / Sh::kSlots;
-        if (use) live = b200_wait(bar_ke + 8 * slot, (use - 1) & 1u, abort_flag, a.status, 21u);
-        if (!live) break;
-        b200_mbar_expect_tx(bar_kf + 8 * slot, Sh::kTile);
-#pragma unroll
-        for (int p = 0; p < Sh::kPanels; ++p) b200_tma_load_4d(k_at + slot * Sh::kTile + p * kTileBytes64, &map_k, bar_kf + 8 * slot, p * 64, t * 128, hk, b);
-        if (use) live = b200_wait(bar_ve + 8 * slot, (use - 1) & 1u, abort_flag, a.status, 22u);
-        if (!live) break;
-        b200_mbar_expect_tx(bar_vf + 8 * slot, Sh::kTile);
-#pragma unroll
-        for (int p = 0; p < Sh::kPanels; ++p) b200_tma_load_4d(v_at + slot * Sh::kTile + p * kTileBytes64, &map_v, bar_vf + 8 * slot, p * 64, t * 128, hk, b);
+        if (docs || n) {
+          if (use) live = b200_wait(bar_ke + 8 * slot, (use - 1) & 1u, abort_flag, a.status, 21u);
+          if (!live) break;
+          load_keys(t, slot);
+          if (use) live = b200_wait(bar_ve + 8 * slot, (use - 1) & 1u, abort_flag, a.status, 22u);
+          if (!live) break;
+          load_values(t, slot);
+        }
         ++n;
       }
       // the copies under way land before shared memory is given up, whatever happened to the others
-      if (n && *abort_flag) {
+      if (*abort_flag) {
+        for (int tries = 0; tries < 1 << 20 && !b200_mbar_try(bar_q, 0u); ++tries) {}
         for (unsigned int i = 0; i < Sh::kSlots && i < n; ++i) {
           const unsigned int last = (n - 1 - i) / Sh::kSlots, slot = (n - 1 - i) % Sh::kSlots;
           for (int tries = 0; tries < 1 << 20 && !b200_mbar_try(bar_kf + 8 * slot, last & 1u); ++tries) {}
@@ -259,65 +356,75 @@ attn_forward_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant__
     __syncwarp();
   } else if (warp == kMma) {
     if (b200_elect()) {
-      constexpr unsigned int idesc_s = idesc_of<T>(128, 128, false, false), idesc_o = idesc_of<T>(128, DP, false, true);
+      constexpr unsigned int idesc_s = idesc_of<T>(128, KW, false, false), idesc_o = idesc_of<T>(128, DP, false, true);
       bool live = b200_wait(bar_q, 0u, abort_flag, a.status, 23u);
-      auto scores = [&](int i, unsigned int slot) {
-#pragma unroll
-        for (int p = 0; p < Sh::kPanels; ++p) {
-          const unsigned long long dq = b200_smem_desc(q_at + i * Sh::kTile + p * kTileBytes64, 16u, 1024u);
-          const unsigned long long dk = b200_smem_desc(k_at + slot * Sh::kTile + p * kTileBytes64, 16u, 1024u);
-#pragma unroll
-          for (unsigned int ks = 0; ks < 4; ++ks) b200_umma(tmem + i * 128, dq + ks * 2, dk + ks * 2, idesc_s, (p || ks) ? 1u : 0u);
-        }
-        b200_umma_commit(bar_s + 8 * i);
-      };
-      unsigned int done[NQ];                     // tiles whose weights have been multiplied
+      unsigned int scored[NQ], done[NQ];         // tiles whose scores are queued, whose weights have been multiplied
       int last[NQ];                              // the last tile of keys that a query tile sees: its product is awaited
 #pragma unroll
       for (int i = 0; i < NQ; ++i) {
-        done[i] = 0;
-        for (last[i] = n_tiles - 1; last[i] >= 0 && !((classes[last[i]] >> (2 * i)) & 3u); --last[i]) {}
+        scored[i] = done[i] = 0;
+        for (last[i] = n_tiles - 1; last[i] >= 0 && !class_of(last[i], i); --last[i]) {}
       }
-      // the scores of a tile are queued behind the products of the tile before it, query tile by query tile
+      auto scores = [&](int i, unsigned int slot) {
+        const unsigned int place = scored[i]++ % Sh::kScores;
+#pragma unroll
+        for (int p = 0; p < Sh::kPanels; ++p) {
+          const unsigned long long dq = b200_smem_desc(q_at + i * Sh::kTile + p * kTileBytes64, 16u, 1024u);
+          const unsigned long long dk = b200_smem_desc(k_at + slot * Sh::kKeys + p * Sh::kPanel, 16u, 1024u);
+#pragma unroll
+          for (unsigned int ks = 0; ks < 4; ++ks) b200_umma(tmem + i * 128 + place * KW, dq + ks * 2, dk + ks * 2, idesc_s, (p || ks) ? 1u : 0u);
+        }
+        b200_umma_commit(bar_s + 16 * i + 8 * place);
+      };
       int t = 0, next = 0;
       unsigned int n = 0;
-      while (next < n_tiles && !classes[next]) ++next;
+      while (next < n_tiles && !seen_at(next)) ++next;
       if (live && next < n_tiles) {
         live = b200_wait(bar_kf, 0u, abort_flag, a.status, 24u);
         tc_after();
         if (live) {
 #pragma unroll
           for (int i = 0; i < NQ; ++i)
-            if ((classes[next] >> (2 * i)) & 3u) scores(i, 0);
+            if (class_of(next, i)) scores(i, 0);
           b200_umma_commit(bar_ke);
         }
       }
       while (live && next < n_tiles) {
         t = next;
-        for (++next; next < n_tiles && !classes[next]; ++next) {}
+        for (++next; next < n_tiles && !seen_at(next); ++next) {}
         const unsigned int slot = n % Sh::kSlots, ph = (n / Sh::kSlots) & 1u, slot1 = (n + 1) % Sh::kSlots, ph1 = ((n + 1) / Sh::kSlots) & 1u;
+        if (next < n_tiles) live = b200_wait(bar_kf + 8 * slot1, ph1, abort_flag, a.status, 26u);
+        if (!live) break;
+        tc_after();
+        // With two places the next tile's scores go ahead of this one's products (their place was given up with the weights before);
+        // with one they follow them, query tile by query tile.
+        if (Sh::kScores == 2 && next < n_tiles) {
+#pragma unroll
+          for (int i = 0; i < NQ; ++i)
+            if (class_of(next, i)) scores(i, slot1);
+          b200_umma_commit(bar_ke + 8 * slot1);
+        }
         live = b200_wait(bar_vf + 8 * slot, ph, abort_flag, a.status, 25u);
-        if (live && next < n_tiles) live = b200_wait(bar_kf + 8 * slot1, ph1, abort_flag, a.status, 26u);
         tc_after();
 #pragma unroll
         for (int i = 0; i < NQ; ++i) {
           if (!live) break;
-          if ((classes[t] >> (2 * i)) & 3u) {
-            live = b200_wait(bar_p + 8 * i, done[i] & 1u, abort_flag, a.status, 27u);
+          if (class_of(t, i)) {
+            live = b200_wait(bar_p + 16 * i + 8 * (done[i] % Sh::kScores), done[i] / Sh::kScores & 1u, abort_flag, a.status, 27u);
             tc_after();
             if (!live) break;
-            const unsigned long long dv = b200_smem_desc(v_at + slot * Sh::kTile, kTileBytes64, 1024u);
+            const unsigned int weights = tmem + i * 128 + done[i] % Sh::kScores * KW;
+            const unsigned long long dv = b200_smem_desc(v_at + slot * Sh::kKeys, Sh::kPanel, 1024u);
 #pragma unroll
-            for (unsigned int ks = 0; ks < 8; ++ks)
-              umma_ts(acc_o + i * DP, tmem + i * 128 + ks * 8, dv + ks * 128, idesc_o, (done[i] || ks) ? 1u : 0u);
-            if (t == last[i]) b200_umma_commit(bar_o + 8 * i);
+            for (unsigned int ks = 0; ks < KW / 16; ++ks) umma_ts(acc_o + i * DP, weights + ks * 8, dv + ks * 128, idesc_o, (done[i] || ks) ? 1u : 0u);
+            if (Sh::kScores == 2 || t == last[i]) b200_umma_commit(bar_o + 8 * i);
             ++done[i];
           }
           if (i == NQ - 1) b200_umma_commit(bar_ve + 8 * slot);
-          if (next < n_tiles && ((classes[next] >> (2 * i)) & 3u)) scores(i, slot1);
+          if (Sh::kScores == 1 && next < n_tiles && class_of(next, i)) scores(i, slot1);
         }
         if (!live) break;
-        if (next < n_tiles) b200_umma_commit(bar_ke + 8 * slot1);
+        if (Sh::kScores == 1 && next < n_tiles) b200_umma_commit(bar_ke + 8 * slot1);
         ++n;
       }
     }
@@ -326,34 +433,33 @@ attn_forward_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant__
     // ---------------------------------------------------------------- softmax: a thread a row
     const unsigned int mine = tmem + g * 128 + ((warp & 3u) << 21), mine_o = acc_o + g * DP + ((warp & 3u) << 21);
     const float c = CAP ? a.cap * kLog2e : a.scale * kLog2e;
-    const float to_tanh = CAP ? 2.f * kLog2e * a.scale / a.cap : 0.f;
+    const float to_tanh = CAP ? a.scale / a.cap : 0.f;
     const float slope2 = BIAS ? a.slopes[h] * kLog2e : 0.f;
+    const AttnSpan mine_span = NQ == 2 && g == 1u ? span[NQ - 1] : span[0];
     float m = -INFINITY, l = 0.f;      // m: in log 2 units without bias or cap scaled by c, see `unit`
     const float unit = BIAS ? 1.f : c;
     unsigned int seen = 0;
     bool live = true;
     for (int t = 0; t < n_tiles && live; ++t) {
-      const unsigned int cls = (classes[t] >> (2 * g)) & 3u;
+      const unsigned int cls = docs ? (classes[t] >> (2 * g)) & 3u : tile_class(mine_span, t * KW, KW, false, 0, 0, false);
       if (!cls) continue;
-      live = b200_wait(bar_s + 8 * g, seen & 1u, abort_flag, a.status, 28u);
+      const unsigned int place = seen % Sh::kScores, at = mine + place * KW;
+      live = b200_wait(bar_s + 16 * g + 8 * place, seen / Sh::kScores & 1u, abort_flag, a.status, 28u);
       if (!live) break;
       tc_after();
       // first pass: the row's maximum, 32 scores at a time; what cap, bias or mask have changed goes back
-      unsigned int bits[4] = {0u, 0u, 0u, 0u};
-      if (cls == 2u) visible_words(a, b, t * 128, row, lane, bits);
+      unsigned int bits[KW / 32];
+      if (cls == 2u) visible_words<KW / 32>(a, b, t * KW, row, lane, bits);
       float x[2][32], top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-      b200_tmem_ld32(mine, (unsigned int*)x[0]);
+      b200_tmem_ld32(at, (unsigned int*)x[0]);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < KW / 32; ++k) {
         float* y = x[k & 1];
         tmem_wait_ld();
-        if (k < 3) b200_tmem_ld32(mine + 32 * (k + 1), (unsigned int*)x[(k + 1) & 1]);
-        if constexpr (CAP) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) y[j] = tanh_of(y[j] * to_tanh);
-        }
+        if (k < KW / 32 - 1) b200_tmem_ld32(at + 32 * (k + 1), (unsigned int*)x[(k + 1) & 1]);
+        if constexpr (CAP) tanh_chunk(x[k & 1], to_tanh);
         if constexpr (BIAS) {
-          const float from = (float)(row.pos - t * 128 - 32 * k);
+          const float from = (float)(row.pos - t * KW - 32 * k);
 #pragma unroll
           for (int j = 0; j < 32; ++j) y[j] = fmaf(-slope2, fabsf(from - (float)j), y[j] * c);
         }
@@ -363,16 +469,21 @@ attn_forward_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant__
         }
 #pragma unroll
         for (int j = 0; j < 32; ++j) top[j & 3] = fmaxf(top[j & 3], y[j]);
-        if (CAP || BIAS || cls == 2u) b200_tmem_st32(mine + 32 * k, (const unsigned int*)y);
+        if (CAP || BIAS || cls == 2u) b200_tmem_st32(at + 32 * k, (const unsigned int*)y);
       }
       if (CAP || BIAS || cls == 2u) tmem_wait_st();
-      b200_tmem_ld32(mine, (unsigned int*)x[0]);
+      b200_tmem_ld32(at, (unsigned int*)x[0]);
       const float m_tile = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * unit;
       // the maximum in use moves when some row of the warp has outgrown it (or has had none)
       if (__any_sync(0xffffffffu, m_tile > m + 8.f || (m == -INFINITY && m_tile != -INFINITY))) {
         const float m_new = fmaxf(m, m_tile);
         const float by = m == -INFINITY ? 0.f : ex2(m - m_new);
         if (seen) {
+          // (with one place the scores came behind the product before; with two it may still run)
+          if (Sh::kScores == 2) {
+            live = b200_wait(bar_o + 8 * g, (seen - 1) & 1u, abort_flag, a.status, 30u);
+            tc_after();
+          }
 #pragma unroll
           for (int e = 0; e < DP; e += 32) {
             float o[32];
@@ -387,32 +498,38 @@ attn_forward_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant__
         m = m_new;
       }
       const float off = m == -INFINITY ? 0.f : -m;
-      float part[4] = {0.f, 0.f, 0.f, 0.f};
+      Pair part[2] = {Pair(0.f, 0.f), Pair(0.f, 0.f)};
+      const Pair unit2(unit, unit), off2(off, off);
       // second pass: the weights, over the scores that have been read
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < KW / 32; ++k) {
         const float* y = x[k & 1];
         tmem_wait_ld();
-        if (k < 3) b200_tmem_ld32(mine + 32 * (k + 1), (unsigned int*)x[(k + 1) & 1]);
+        if (k < KW / 32 - 1) b200_tmem_ld32(at + 32 * (k + 1), (unsigned int*)x[(k + 1) & 1]);
         unsigned int w[16];
 #pragma unroll
         for (int j = 0; j < 32; j += 2) {
-          const float p0 = ex2(fmaf(y[j], unit, off)), p1 = ex2(fmaf(y[j + 1], unit, off));
-          part[j & 2] += p0;
-          part[(j & 2) + 1] += p1;
+          float p0, p1;
+          fma2(Pair(y[j], y[j + 1]), unit2, off2).get(p0, p1);
+          p0 = ex2(p0);
+          p1 = ex2(p1);
+          part[j >> 1 & 1] = add2(part[j >> 1 & 1], Pair(p0, p1));
           w[j / 2] = pack2(p0, p1, T());
         }
-        tmem_st16(mine + 16 * k, w);
+        tmem_st16(at + 16 * k, w);
       }
-      l += (part[0] + part[1]) + (part[2] + part[3]);
+      float l0, l1;
+      add2(part[0], part[1]).get(l0, l1);
+      l += l0 + l1;
       tmem_wait_st();
       tc_before();
-      b200_mbar_arrive(bar_p + 8 * g);
+      // (a barrier a place: with two of them a warp may be a tile ahead of another)
+      b200_mbar_arrive(bar_p + 16 * g + 8 * place);
       ++seen;
     }
     // ---------------------------------------------------------------- output
     // (the output goes through the queries' tile, which has to have arrived even where nobody reads it)
-    if (live) live = b200_wait(seen ? bar_o + 8 * g : bar_q, 0u, abort_flag, a.status, 29u);
+    if (live) live = b200_wait(seen ? bar_o + 8 * g : bar_q, seen && Sh::kScores == 2 ? (seen - 1) & 1u : 0u, abort_flag, a.status, 29u);
     tc_after();
     const float by = l > 0.f || l != l ? 1.f / l : 0.f;
     float bad = 0.f;
@@ -437,22 +554,21 @@ attn_forward_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant__
         *(uint4*)(line + (((piece0 + p) ^ (in & 7u)) << 4)) =
             make_uint4(pack2(o[8 * p], o[8 * p + 1], T()), pack2(o[8 * p + 2], o[8 * p + 3], T()), pack2(o[8 * p + 4], o[8 * p + 5], T()), pack2(o[8 * p + 6], o[8 * p + 7], T()));
     }
-    const bool mend = live && r < a.S && bad != 0.f;     // (NaN)
-    if (mend) repair[g] = 1u;
     if (live && r < a.S && a.lse) a.lse[((long long)b * a.H + h) * a.S + r] = l > 0.f || l != l ? (m + log2f(l)) * kLn2 : -INFINITY;
+    // every warp sends its 32 rows; those with a value that is infinite or undefined are done again, one by one
+    const int first = r0 + (int)warp * 32;
+    const unsigned int mend = __ballot_sync(0xffffffffu, live && r < a.S && bad != 0.f);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    named_barrier(1 + (int)g, 128);
-    if ((threadIdx.x & 127u) == 0 && live) {
+    __syncwarp();
+    if (lane == 0 && live && first < a.S) {
 #pragma unroll
       for (int p = 0; p < Sh::kPanels; ++p)
-        if (p * 64 < a.D && r0 + 128 * (int)g < a.S) b200_tma_store_4d(&map_o, b200_smem_addr(tile) + p * kTileBytes64, p * 64, r0 + 128 * (int)g, h, b);
-      if (repair[g]) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        if (p * 64 < a.D) b200_tma_store_4d(&map_o, b200_smem_addr(tile) + p * kTileBytes64 + (warp & 3u) * 4096, p * 64, first, h, b);
+      if (mend) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
       else b200_tma_store_read_wait<0>();
     }
-    if (repair[g]) {
-      named_barrier(1 + (int)g, 128);
-      for (unsigned int todo = __ballot_sync(0xffffffffu, mend); todo; todo &= todo - 1) attn_forward_row<T>(a, b, h, r0 + (int)(warp * 32) + __ffs(todo) - 1, lane);
-    }
+    __syncwarp();
+    for (unsigned int todo = mend; todo; todo &= todo - 1) attn_forward_row<T>(a, b, h, first + __ffs(todo) - 1, lane);
   }
   // ------------------------------------------------------------------ teardown
   __syncwarp();

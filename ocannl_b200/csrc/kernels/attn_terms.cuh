@@ -31,14 +31,26 @@ struct AttnRow {
   int pos, last, doc;
 };
 
+// a sequence's number of keys, and its prefix (0: none)
+struct AttnSeq {
+  int len, prefix;
+};
+__device__ __forceinline__ AttnSeq attn_seq(const AttnArgs& a, int b) {
+  AttnSeq s;
+  s.len = a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
+  s.prefix = a.mask == B200_MASK_PREFIX ? max(a.prefix[b], 0) : 0;
+  return s;
+}
+// the last key that query r sees, documents aside: never less than that of the query before
+__device__ __forceinline__ int attn_last(const AttnArgs& a, const AttnSeq& s, int r) {
+  const int last = a.mask == B200_MASK_NONE ? s.len - 1 : min(s.len - 1, max(s.len - a.S + r, s.prefix - 1));
+  return max(last, -1);
+}
 __device__ __forceinline__ AttnRow attn_row(const AttnArgs& a, int b, int r) {
+  const AttnSeq s = attn_seq(a, b);
   AttnRow w;
-  const int len = a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
-  w.pos = len - a.S + r;
-  w.last = len - 1;
-  if (a.mask == B200_MASK_CAUSAL) w.last = min(w.last, w.pos);
-  if (a.mask == B200_MASK_PREFIX) w.last = min(w.last, max(w.pos, max(a.prefix[b], 0) - 1));
-  w.last = max(w.last, -1);
+  w.pos = s.len - a.S + r;
+  w.last = attn_last(a, s, r);
   w.doc = 0;
   if (a.qdoc) {
     w.doc = a.qdoc[(long long)b * a.S + r];

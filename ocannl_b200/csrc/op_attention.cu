@@ -148,32 +148,32 @@ FewKernel few_of(bool cap, bool bias) {
   if (cap) return bias ? attn_forward_few<T, DP, true, true> : attn_forward_few<T, DP, true, false>;
   return bias ? attn_forward_few<T, DP, false, true> : attn_forward_few<T, DP, false, false>;
 }
-template <class T, int DP>
+template <class T, int DP, int CW>
 KeysKernel keys_of(bool cap, bool bias) {
-  if (cap) return bias ? attn_grad_keys_tc<T, DP, true, true> : attn_grad_keys_tc<T, DP, true, false>;
-  return bias ? attn_grad_keys_tc<T, DP, false, true> : attn_grad_keys_tc<T, DP, false, false>;
+  if (cap) return bias ? attn_grad_keys_tc<T, DP, CW, true, true> : attn_grad_keys_tc<T, DP, CW, true, false>;
+  return bias ? attn_grad_keys_tc<T, DP, CW, false, true> : attn_grad_keys_tc<T, DP, CW, false, false>;
 }
-template <class T, int DP>
+template <class T, int DP, int CW>
 QueriesKernel queries_of(bool cap, bool bias) {
-  if (cap) return bias ? attn_grad_queries_tc<T, DP, true, true> : attn_grad_queries_tc<T, DP, true, false>;
-  return bias ? attn_grad_queries_tc<T, DP, false, true> : attn_grad_queries_tc<T, DP, false, false>;
+  if (cap) return bias ? attn_grad_queries_tc<T, DP, CW, true, true> : attn_grad_queries_tc<T, DP, CW, true, false>;
+  return bias ? attn_grad_queries_tc<T, DP, CW, false, true> : attn_grad_queries_tc<T, DP, CW, false, false>;
 }
 
 typedef void (*AttnKernel)(const AttnArgs);
 typedef void (*ForwardKernel)(const b200_tmap, const b200_tmap, const b200_tmap, const b200_tmap, const AttnArgs);
 
-template <class T, int DP, int NQ>
+template <class T, int DP, int NQ, int KW>
 ForwardKernel forward_of(bool cap, bool bias) {
-  if (cap) return bias ? attn_forward_tc<T, DP, NQ, true, true> : attn_forward_tc<T, DP, NQ, true, false>;
-  return bias ? attn_forward_tc<T, DP, NQ, false, true> : attn_forward_tc<T, DP, NQ, false, false>;
+  if (cap) return bias ? attn_forward_tc<T, DP, NQ, KW, true, true> : attn_forward_tc<T, DP, NQ, KW, true, false>;
+  return bias ? attn_forward_tc<T, DP, NQ, KW, false, true> : attn_forward_tc<T, DP, NQ, KW, false, false>;
 }
 
-// [batch, length, heads, d] in boxes of 128 positions x 64 elements of a head, swizzled as the tensor cores read them
-b200_tmap head_map(const void* p, int dtype, int batch, int length, int heads, int d, int ld) {
+// [batch, length, heads, d] in boxes of `box_rows` positions x 64 elements of a head, swizzled as the tensor cores read them
+b200_tmap head_map(const void* p, int dtype, int batch, int length, int heads, int d, int ld, int box_rows) {
   CUtensorMap map;
   const cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)length, (cuuint64_t)heads, (cuuint64_t)batch};
   const cuuint64_t strides[3] = {(cuuint64_t)heads * ld * 2, (cuuint64_t)ld * 2, (cuuint64_t)length * heads * ld * 2};
-  const cuuint32_t box[4] = {64, 128, 1, 1}, estr[4] = {1, 1, 1, 1};
+  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1}, estr[4] = {1, 1, 1, 1};
   const CUresult r = cu().cuTensorMapEncodeTiled_(&map, dtype == B200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, (void*)p,
                                                   dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                                                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -209,7 +209,7 @@ struct AttnOperator : b200_operator {
   int vec = 0;
   FewKernel few = nullptr;
   FewArgs few_args = {};
-  b200_tmap map_q, map_k, map_v, map_o, map_do, map_dq, map_dk, map_dv;
+  b200_tmap map_q, map_k, map_v, map_o, map_do, map_dq, map_dk, map_dv, own_q, own_k, own_v, own_do;
   unsigned int threads = 0, grid = 0, keys_grid = 0;
   size_t smem = 0, keys_smem = 0;
   // padded copies: what is copied before and after the kernels
@@ -352,20 +352,15 @@ struct AttnOperator : b200_operator {
     return (unsigned int)n;
   }
   void choose_tc() {
-    auto of_queries = [&](const void* p) { return head_map(p, dtype, a.B, a.S, a.H, a.D, a.ld); };
-    auto of_keys = [&](const void* p) { return head_map(p, dtype, a.B, a.T, a.HK, a.D, a.ld); };
-    map_q = of_queries(a.q);
-    map_k = of_keys(a.k);
-    map_v = of_keys(a.v);
+    // results leave 32 rows at a time
     if (grad) {
-      map_do = of_queries(a.d_out);
-      map_dq = of_queries(a.dq);
-      map_dk = of_keys(a.dk);
-      map_dv = of_keys(a.dv);
+      map_dq = of_queries(a.dq, 32);
+      map_dk = of_keys(a.dk, 32);
+      map_dv = of_keys(a.dv, 32);
     } else {
-      map_o = of_queries(a.out);
+      map_q = of_queries(a.q, 128);
+      map_o = of_queries(a.out, 32);
     }
-    const int tiles = (a.T + 127) / 128, tiles_q = (a.S + 127) / 128;
     const long long heads = (long long)a.B * a.H;
     // Heads of more than 64 elements: two query tiles a CTA share each key tile (64 KB per tile of 128 x 128 would otherwise
     // come in from L2 for 1024 cycles of products), unless that leaves SMs without work.
@@ -374,18 +369,18 @@ struct AttnOperator : b200_operator {
       typedef decltype(t) T;
       if constexpr (sizeof(T) == 2) {
         if (grad) {
-          if (a.D <= 64) set_grad<T, 64>(tiles, tiles_q);
-          else set_grad<T, 128>(tiles, tiles_q);
+          if (a.D <= 64) set_grad<T, 64, 64>();
+          else set_grad<T, 128, 128>();
         } else {
-          if (a.D <= 64) set<T, 64, 1>(tiles);
-          else if (two) set<T, 128, 2>(tiles);
-          else set<T, 128, 1>(tiles);
+          if (a.D <= 64) set<T, 64, 1, 64>();
+          else if (two) set<T, 128, 2, 128>();
+          else set<T, 128, 1, 64>();
         }
       }
       return 0;
     });
     grid = blocks_of(heads * ((a.S + 128 * (!grad && two ? 2 : 1) - 1) / (128 * (!grad && two ? 2 : 1))));
-    if (grad) keys_grid = blocks_of((long long)a.B * a.HK * tiles);
+    if (grad) keys_grid = blocks_of((long long)a.B * a.HK * ((a.T + 127) / 128));
     if (std::max(smem, keys_smem) > 227 * 1024) throw Error(B200_E_UNSUPPORTED, "attention: too many keys or queries");
     if (grad) {
       ready(keys, keys_smem);
@@ -394,20 +389,34 @@ struct AttnOperator : b200_operator {
       ready(forward, smem);
     }
   }
-  template <class T, int DP, int NQ>
-  void set(int tiles) {
-    forward = forward_of<T, DP, NQ>(a.cap > 0.f, a.slopes != nullptr);
-    threads = FwdShape<DP, NQ>::kThreads;
-    smem = FwdShape<DP, NQ>::smem(tiles);
+  template <class T, int DP, int NQ, int KW>
+  void set() {
+    forward = forward_of<T, DP, NQ, KW>(a.cap > 0.f, a.slopes != nullptr);
+    threads = FwdShape<DP, NQ, KW>::kThreads;
+    smem = FwdShape<DP, NQ, KW>::smem((a.T + KW - 1) / KW);
+    map_k = of_keys(a.k, KW);
+    map_v = of_keys(a.v, KW);
   }
-  template <class T, int DP>
-  void set_grad(int tiles, int tiles_q) {
-    keys = keys_of<T, DP>(a.cap > 0.f, a.slopes != nullptr);
-    queries = queries_of<T, DP>(a.cap > 0.f, a.slopes != nullptr);
-    threads = BwdShape<DP>::kThreads;
-    smem = BwdShape<DP>::smem(tiles);
-    keys_smem = BwdShape<DP>::smem(tiles_q);
+  template <class T, int DP, int CW>
+  void set_grad() {
+    typedef BwdShape<DP, CW> Sh;
+    keys = keys_of<T, DP, CW>(a.cap > 0.f, a.slopes != nullptr);
+    queries = queries_of<T, DP, CW>(a.cap > 0.f, a.slopes != nullptr);
+    threads = Sh::kThreads;
+    smem = Sh::smem((a.T + CW - 1) / CW);
+    keys_smem = Sh::smem((a.S + CW - 1) / CW);
+    // a CTA's own rows and the others' tiles, for either kernel
+    own_q = of_queries(a.q, 128);
+    own_do = of_queries(a.d_out, 128);
+    own_k = of_keys(a.k, 128);
+    own_v = of_keys(a.v, 128);
+    map_q = of_queries(a.q, CW);
+    map_do = of_queries(a.d_out, CW);
+    map_k = of_keys(a.k, CW);
+    map_v = of_keys(a.v, CW);
   }
+  b200_tmap of_queries(const void* p, int rows) const { return head_map(p, dtype, a.B, a.S, a.H, a.D, a.ld, rows); }
+  b200_tmap of_keys(const void* p, int rows) const { return head_map(p, dtype, a.B, a.T, a.HK, a.D, a.ld, rows); }
   void copy(const std::vector<Copy>& list, cudaStream_t s) {
     for (auto& c : list)
       launch(attn_copy_rows, (unsigned int)std::min<long long>((c.rows * head + 1023) / 1024, 16ll * dev->sm_count), 256, 0, s, (const unsigned short*)c.src,
@@ -418,8 +427,8 @@ struct AttnOperator : b200_operator {
     copy(before, s);
     if (grad && rows) launch(statistics, statistics_grid, 256, 0, s, a, by_heads, by_padded);
     if (tc && grad) {
-      launch(keys, keys_grid, threads, keys_smem, s, map_q, map_k, map_v, map_do, map_dk, map_dv, a);
-      launch(queries, grid, threads, smem, s, map_q, map_k, map_v, map_do, map_dq, a);
+      launch(keys, keys_grid, threads, keys_smem, s, map_q, own_k, own_v, map_do, map_dk, map_dv, a);
+      launch(queries, grid, threads, smem, s, own_q, map_k, map_v, own_do, map_dq, a);
     } else if (few) {
       launch(few, dim3(grid, (unsigned int)few_args.splits), kFewWarps * 32, smem, s, a, few_args);
     } else if (tc) {
