@@ -195,27 +195,40 @@ attn_grad_keys_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant
   tc_after();
   const float grad_unit = gradient_unit<T>(a, scratch);
   if (docs) {
-    int kmin = 0, kmax = 0;
-    bool negative = false;
-    key_documents<128>(a, b, j0, lane, kmin, kmax, negative);
-    for (int t = (int)warp; t < tiles; t += (int)Sh::kWarps) {
-      AttnSpan s;
-      s.last_min = s.doc_min = 0x7fffffff;
-      s.last_max = -1;
-      s.doc_max = -0x7fffffff - 1;
+    int kmin[1], kmax[1];
+    bool negative[1];
+    key_documents<128, 1>(a, b, j0 / 128, 0, lane, kmin, kmax, negative);
+    constexpr int kAhead = 4;
+    for (int t0 = (int)warp; t0 < tiles; t0 += kAhead * (int)Sh::kWarps) {
+      int d[kAhead][CW / 32];
 #pragma unroll
-      for (int i = 0; i < CW / 32; ++i) {
-        const int r = t * CW + 32 * i + (int)lane;
-        AttnRow w;
-        w.last = w.doc = 0;
-        if (r < a.S) w = attn_row(a, b, r);
-        const AttnSpan p = span_of(r < a.S, w);
-        s.last_min = min(s.last_min, p.last_min);
-        s.last_max = max(s.last_max, p.last_max);
-        s.doc_min = min(s.doc_min, p.doc_min);
-        s.doc_max = max(s.doc_max, p.doc_max);
+      for (int n = 0; n < kAhead; ++n)
+#pragma unroll
+        for (int i = 0; i < CW / 32; ++i) {
+          const long long r = (long long)(t0 + n * (int)Sh::kWarps) * CW + 32 * i + lane;
+          d[n][i] = r < a.S ? __ldg(a.qdoc + (long long)b * a.S + r) : -1;
+        }
+#pragma unroll
+      for (int n = 0; n < kAhead; ++n) {
+        const int t = t0 + n * (int)Sh::kWarps;
+        AttnSpan s;
+        s.last_min = s.doc_min = 0x7fffffff;
+        s.last_max = -1;
+        s.doc_max = -0x7fffffff - 1;
+#pragma unroll
+        for (int i = 0; i < CW / 32; ++i) {
+          const int r = t * CW + 32 * i + (int)lane;
+          AttnRow w;
+          w.doc = d[n][i];
+          w.last = w.doc < 0 ? -1 : attn_last(a, seq, r);
+          const AttnSpan p = span_of(t < tiles && r < a.S, w);
+          s.last_min = min(s.last_min, p.last_min);
+          s.last_max = max(s.last_max, p.last_max);
+          s.doc_min = min(s.doc_min, p.doc_min);
+          s.doc_max = max(s.doc_max, p.doc_max);
+        }
+        if (lane == 0 && t < tiles) classes[t] = (unsigned char)tile_class(s, j0, 128, true, kmin[0], kmax[0], negative[0]);
       }
-      if (lane == 0) classes[t] = (unsigned char)tile_class(s, j0, 128, true, kmin, kmax, negative);
     }
     __syncthreads();
   }
@@ -541,12 +554,17 @@ attn_grad_queries_tc(const __grid_constant__ b200_tmap map_q, const __grid_const
     }
     __syncthreads();
     tiles = (span->last_max + CW) / CW;
-    for (int t = (int)warp; t < tiles; t += (int)Sh::kWarps) {
-      int kmin = 0, kmax = 0;
-      bool negative = false;
-      key_documents<CW>(a, b, t * CW, lane, kmin, kmax, negative);
-      const unsigned int cls = tile_class(*span, t * CW, CW, true, kmin, kmax, negative);
-      if (lane == 0) classes[t] = (unsigned char)cls;
+    constexpr int kAhead = 4;
+    for (int t0 = (int)warp; t0 < tiles; t0 += kAhead * (int)Sh::kWarps) {
+      int kmin[kAhead], kmax[kAhead];
+      bool negative[kAhead];
+      key_documents<CW, kAhead>(a, b, t0, Sh::kWarps, lane, kmin, kmax, negative);
+#pragma unroll
+      for (int n = 0; n < kAhead; ++n) {
+        const int t = t0 + n * (int)Sh::kWarps;
+        const unsigned int cls = tile_class(*span, t * CW, CW, true, kmin[n], kmax[n], negative[n]);
+        if (lane == 0 && t < tiles) classes[t] = (unsigned char)cls;
+      }
     }
     __syncthreads();
   }

@@ -27,7 +27,8 @@ struct FewShape {
   static constexpr int kRing = kFewStages * kStage;                    // of a warp
   static constexpr int kWidth = DP + 4;
   static constexpr int kJoin = kFewWarps * kFewRows * kWidth * 4;
-  static constexpr int smem() { return kFewWarps * kRing > kJoin ? kFewWarps * kRing : kJoin; }
+  static constexpr int smem() { return kFewWarps * kRing; }
+  static_assert(kJoin + kFewWarps * DP * 4 <= kFewWarps * kRing, "the warps meet where the rings were");
 };
 
 template <class T>
@@ -89,16 +90,18 @@ __global__ void __launch_bounds__(kFewWarps * 32) attn_forward_few(const __grid_
   // the queries as the A operand, straight from memory: rows ra and rb, elements 2 (lane % 4) .. of each eight
   unsigned int q[KS][4];
 #pragma unroll
-  for (int ks = 0; ks < KS; ++ks)
+  for (int w = 0; w < 2; ++w) {
+    const bool on = first_row + (w ? rb : ra) < shared_rows;
+    const unsigned short* p = (const unsigned short*)a.q + (on ? attn_q_at(a, b, query_of(w ? rb : ra), head_of(w ? rb : ra)) : 0) + (lane & 3u) * 2;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int k = i & 1 ? rb : ra, e = ks * 16 + (i >> 1) * 8 + (int)(lane & 3u) * 2;
-      q[ks][i] = 0u;
-      if (first_row + k < shared_rows && e < a.D) {
-        const unsigned short* p = (const unsigned short*)a.q + attn_q_at(a, b, query_of(k), head_of(k)) + e;
-        q[ks][i] = (unsigned int)p[0] | (e + 1 < a.D ? (unsigned int)p[1] << 16 : 0u);
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int e = ks * 16 + i * 8;
+        // (rows lie on 16 bytes, zeros behind their end)
+        q[ks][2 * i + w] = on && e + (int)(lane & 3u) * 2 < a.D ? *(const unsigned int*)(p + e) : 0u;
       }
-    }
+  }
 
   float o[DP / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
@@ -110,31 +113,43 @@ __global__ void __launch_bounds__(kFewWarps * 32) attn_forward_few(const __grid_
   const int steps = j_end > j_begin ? (j_end - j_begin + kFewStep - 1) / kFewStep : 0;
   const int mine = steps > (int)warp ? (steps - (int)warp + kFewWarps - 1) / kFewWarps : 0;     // this warp's steps
 
+  // a lane copies the same 16 bytes of every kRowsApart-th row of a step, from pointers that move on with the steps
+  constexpr int kPieces = DP / 8, kRowsApart = 32 / kPieces;
+  const int my_row = (int)lane / kPieces, my_piece = (int)lane % kPieces;
+  const bool in_head = my_piece * 8 < a.D;
+  const long long stride = (long long)a.HK * a.ld;
+  int next_j = j_begin + (int)warp * kFewStep + my_row;
+  const unsigned short *next_k = (const unsigned short*)a.k + attn_k_at(a, b, 0, hk) + (long long)next_j * stride + my_piece * 8,
+                       *next_v = (const unsigned short*)a.v + attn_k_at(a, b, 0, hk) + (long long)next_j * stride + my_piece * 8;
+  const unsigned int my_slot = ring + (my_row * Sh::kRow + my_piece * 8) * 2;
+  unsigned int to = 0;               // the slot that is filled next
   auto fetch = [&](int n) {
     if (n < mine) {
-      const int j0 = j_begin + ((int)warp + n * kFewWarps) * kFewStep;
-      const unsigned int at = ring + (n % kFewStages) * Sh::kStage;
-      constexpr int pieces = DP / 8;
+      const unsigned int at = my_slot + to * Sh::kStage;
 #pragma unroll
-      for (int i = (int)lane; i < kFewStep * pieces; i += 32) {
-        const int r = i / pieces, p = i % pieces;
-        const bool on = j0 + r < j_end && p * 8 < a.D;
-        const long long src = on ? attn_k_at(a, b, j0 + r, hk) + p * 8 : 0;
-        const unsigned int dst = at + (r * Sh::kRow + p * 8) * 2;
-        copy16(dst, (const unsigned short*)a.k + src, on);
-        copy16(dst + kFewStep * Sh::kRow * 2, (const unsigned short*)a.v + src, on);
+      for (int i = 0; i < kFewStep / kRowsApart; ++i) {
+        const bool on = in_head && next_j + i * kRowsApart < j_end;
+        copy16(at + i * kRowsApart * Sh::kRow * 2, on ? next_k + i * kRowsApart * stride : (const unsigned short*)a.k, on);
+        copy16(at + (i * kRowsApart + kFewStep) * Sh::kRow * 2, on ? next_v + i * kRowsApart * stride : (const unsigned short*)a.v, on);
       }
+      next_j += kFewWarps * kFewStep;
+      next_k += kFewWarps * kFewStep * stride;
+      next_v += kFewWarps * kFewStep * stride;
+      to = to + 1 == kFewStages ? 0 : to + 1;
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 #pragma unroll
   for (int i = 0; i < kFewStages - 1; ++i) fetch(i);
+  const int all_see = __reduce_min_sync(0xffffffffu, min(first_row + ra < shared_rows ? row[0].last : 0x7fffffff, first_row + rb < shared_rows ? row[1].last : 0x7fffffff));
+  unsigned int slot = 0;
   for (int n = 0; n < mine; ++n) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kFewStages - 2) : "memory");
     __syncwarp();
     fetch(n + kFewStages - 1);        // into the slot of the step before, which the whole warp has left
     const int j0 = j_begin + ((int)warp + n * kFewWarps) * kFewStep;
-    const unsigned int k_at = ring + (n % kFewStages) * Sh::kStage, v_at = k_at + kFewStep * Sh::kRow * 2;
+    const unsigned int k_at = ring + slot * Sh::kStage, v_at = k_at + kFewStep * Sh::kRow * 2;
+    slot = slot + 1 == kFewStages ? 0 : slot + 1;
     float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
     // keys 0-7 and 8-15, elements 0-7 and 8-15 of each sixteen: four 8 x 8 blocks
     const unsigned int k_row = k_at + (((lane & 7u) + (lane >> 4) * 8) * Sh::kRow + ((lane >> 3) & 1u) * 8) * 2;
@@ -145,32 +160,51 @@ __global__ void __launch_bounds__(kFewWarps * 32) attn_forward_few(const __grid_
       mma16<T>(s[0], q[ks], y[0], y[1]);
       mma16<T>(s[1], q[ks], y[2], y[3]);
     }
-    float top[2] = {-INFINITY, -INFINITY};
+    if constexpr (CAP) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[h][i] = tanh_of(s[h][i] * to_tanh);
+    }
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int w = i >> 1, j = j0 + h * 8 + (int)(lane & 3u) * 2 + (i & 1);
-        float x = s[h][i];
-        if constexpr (CAP) x = tanh_of(x * to_tanh);
-        x *= c;
-        if constexpr (BIAS) x = fmaf(-slope2[w], fabsf((float)(row[w].pos - j)), x);
-        bool on = j <= row[w].last;
-        if (a.kdoc) on = on && a.kdoc[(long long)b * a.T + j] == row[w].doc;
-        s[h][i] = on ? x : -INFINITY;
-        top[w] = fmaxf(top[w], s[h][i]);
+        s[h][i] *= c;
+        if constexpr (BIAS) s[h][i] = fmaf(-slope2[i >> 1], fabsf((float)(row[i >> 1].pos - j0 - h * 8 - (int)(lane & 3u) * 2 - (i & 1))), s[h][i]);
       }
-    float by[2], off[2];
+    if (a.kdoc || j0 + kFewStep - 1 > all_see) {
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      top[w] = fmaxf(top[w], __shfl_xor_sync(0xffffffffu, top[w], 1));
-      top[w] = fmaxf(top[w], __shfl_xor_sync(0xffffffffu, top[w], 2));
-      const float next = fmaxf(m[w], top[w]);
-      by[w] = m[w] == next ? 1.f : m[w] == -INFINITY ? 0.f : ex2(m[w] - next);
-      m[w] = next;
-      off[w] = next == -INFINITY ? 0.f : next;
-      l[w] *= by[w];
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int w = i >> 1, j = j0 + h * 8 + (int)(lane & 3u) * 2 + (i & 1);
+          bool on = j <= row[w].last;
+          if (a.kdoc) on = on && a.kdoc[(long long)b * a.T + j] == row[w].doc;
+          s[h][i] = on ? s[h][i] : -INFINITY;
+        }
     }
+    // the maximum in use moves when a row has outgrown it by 2^8 (or has had none): hardly ever after the first steps
+    float top[2];
+#pragma unroll
+    for (int w = 0; w < 2; ++w) top[w] = fmaxf(fmaxf(s[0][2 * w], s[0][2 * w + 1]), fmaxf(s[1][2 * w], s[1][2 * w + 1]));
+    if (__any_sync(0xffffffffu, top[0] > m[0] + 8.f || top[1] > m[1] + 8.f)) {
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        top[w] = fmaxf(top[w], __shfl_xor_sync(0xffffffffu, top[w], 1));
+        top[w] = fmaxf(top[w], __shfl_xor_sync(0xffffffffu, top[w], 2));
+        const float next = fmaxf(m[w], top[w]);
+        const float by = m[w] == next ? 1.f : m[w] == -INFINITY ? 0.f : ex2(m[w] - next);
+        m[w] = next;
+        l[w] *= by;
+#pragma unroll
+        for (int i = 0; i < DP / 8; ++i) {
+          o[i][2 * w] *= by;
+          o[i][2 * w + 1] *= by;
+        }
+      }
+    }
+    const float off[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
     // weights as the A operand: rows ra, rb, keys 0-7 and 8-15
     unsigned int p[4];
 #pragma unroll
@@ -180,13 +214,6 @@ __global__ void __launch_bounds__(kFewWarps * 32) attn_forward_few(const __grid_
       l[1] += p2 + p3;
       p[2 * h] = pack2(p0, p1, T());
       p[2 * h + 1] = pack2(p2, p3, T());
-    }
-    if (__any_sync(0xffffffffu, by[0] != 1.f || by[1] != 1.f)) {
-#pragma unroll
-      for (int i = 0; i < DP / 8; ++i) {
-        o[i][0] *= by[0]; o[i][1] *= by[0];
-        o[i][2] *= by[1]; o[i][3] *= by[1];
-      }
     }
     // values: keys 0-7 and 8-15 of elements 0-7, then of elements 8-15, of each sixteen
     const unsigned int v_row = v_at + (((lane & 7u) + ((lane >> 3) & 1u) * 8) * Sh::kRow + (lane >> 4) * 8) * 2;
@@ -225,28 +252,43 @@ __global__ void __launch_bounds__(kFewWarps * 32) attn_forward_few(const __grid_
   // The maximum and the sum of `n` partial rows `step` apart, and in `weight` (n of them) what each is multiplied by: a warp.
   // (a part without visible keys counts nothing, whatever it holds)
   auto weigh = [&](const float* from, int n, long long step, float* weight, float& top, float& sum) {
+    float t[kFewMost / 32], u[kFewMost / 32];
     top = -INFINITY;
-    for (int i = (int)lane; i < n; i += 32) top = fmaxf(top, from[i * step + DP]);
+#pragma unroll
+    for (int k = 0; k < kFewMost / 32; ++k) {
+      const int i = (int)lane + 32 * k;
+      t[k] = i < n ? from[i * step + DP] : -INFINITY;
+      u[k] = i < n ? from[i * step + DP + 1] : 0.f;
+      top = fmaxf(top, t[k]);
+    }
 #pragma unroll
     for (int k = 16; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
     sum = 0.f;
-    for (int i = (int)lane; i < n; i += 32) {
-      const float t = from[i * step + DP], w = t == -INFINITY ? 0.f : ex2(t - top);
-      weight[i] = w;
-      if (w != 0.f) sum = fmaf(w, from[i * step + DP + 1], sum);
+#pragma unroll
+    for (int k = 0; k < kFewMost / 32; ++k) {
+      const float w = t[k] == -INFINITY ? 0.f : ex2(t[k] - top);
+      if ((int)lane + 32 * k < n) weight[lane + 32 * k] = w;
+      if (w != 0.f) sum = fmaf(w, u[k], sum);
     }
 #pragma unroll
     for (int k = 16; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
     __syncwarp();
   };
-  // four elements of the sum of the weighed parts
-  auto gather = [&](const float* from, int n, long long step, const float* weight, int e) {
+  // four elements of the sum of every `each`-th weighed part from `i0` on; eight loads under way together
+  auto gather = [&](const float* from, int n, long long step, const float* weight, int e, int i0, int each) {
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-    for (int i = 0; i < n; ++i) {
-      const float w = weight[i];
-      const float4 x = *(const float4*)(from + i * step + e);
-      if (w != 0.f) v = make_float4(fmaf(w, x.x, v.x), fmaf(w, x.y, v.y), fmaf(w, x.z, v.z), fmaf(w, x.w, v.w));
+    for (int i = i0; i < n; i += 8 * each) {
+      float4 x[8];
+      float w[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int at = i + k * each;
+        w[k] = at < n ? weight[at] : 0.f;
+        x[k] = *(const float4*)(from + (at < n ? at : i) * step + e);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (w[k] != 0.f) v = make_float4(fmaf(w[k], x[k].x, v.x), fmaf(w[k], x[k].y, v.y), fmaf(w[k], x[k].z, v.z), fmaf(w[k], x[k].w, v.w));
     }
     return v;
   };
@@ -272,7 +314,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) attn_forward_few(const __grid_
     for (int i = (int)warp; i < rows; i += kFewWarps) {
       float top, sum;
       weigh(join + i * W, kFewWarps, kFewRows * W, weights[warp], top, sum);
-      if ((int)lane < DP / 4) *(float4*)(parts + i * W + 4 * lane) = gather(join + i * W, kFewWarps, kFewRows * W, weights[warp], 4 * (int)lane);
+      if ((int)lane < DP / 4) *(float4*)(parts + i * W + 4 * lane) = gather(join + i * W, kFewWarps, kFewRows * W, weights[warp], 4 * (int)lane, 0, 1);
       if (lane == 0) {
         parts[i * W + DP] = top;
         parts[i * W + DP + 1] = sum;
@@ -288,11 +330,32 @@ __global__ void __launch_bounds__(kFewWarps * 32) attn_forward_few(const __grid_
   }
   const float* all = f.splits > 1 ? f.parts + (long long)pair * f.splits * kFewRows * W : join;
   const int n_parts = f.splits > 1 ? f.splits : kFewWarps;
+  // A single row is shared by the four warps: each adds every fourth part, the first adds the four sums.
+  if (rows == 1) {
+    float top, sum;
+    weigh(all, n_parts, kFewRows * W, weights[warp], top, sum);
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if ((int)lane < DP / 4) v = gather(all, n_parts, kFewRows * W, weights[warp], 4 * (int)lane, (int)warp, kFewWarps);
+    float4* meet = (float4*)(dyn + sizeof(float) * kFewWarps * kFewRows * W);       // (behind `join`, within the rings)
+    __syncthreads();
+    if ((int)lane < DP / 4) meet[warp * (DP / 4) + lane] = v;
+    __syncthreads();
+    if (warp) return;
+    if ((int)lane < DP / 4) {
+      for (int w = 1; w < kFewWarps; ++w) {
+        const float4 x = meet[w * (DP / 4) + lane];
+        v = make_float4(v.x + x.x, v.y + x.y, v.z + x.z, v.w + x.w);
+      }
+      finish(0, 4 * (int)lane, v, top, sum);
+    }
+    if (__any_sync(0xffffffffu, !fine)) attn_forward_row<T>(a, b, head_of(0), query_of(0), lane);
+    return;
+  }
   for (int i = (int)warp; i < rows; i += kFewWarps) {
     float top, sum;
     weigh(all + i * W, n_parts, kFewRows * W, weights[warp], top, sum);
     fine = true;
-    if ((int)lane < DP / 4) finish(i, 4 * (int)lane, gather(all + i * W, n_parts, kFewRows * W, weights[warp], 4 * (int)lane), top, sum);
+    if ((int)lane < DP / 4) finish(i, 4 * (int)lane, gather(all + i * W, n_parts, kFewRows * W, weights[warp], 4 * (int)lane, 0, 1), top, sum);
     if (__any_sync(0xffffffffu, !fine)) attn_forward_row<T>(a, b, head_of(i), query_of(i), lane);
   }
 }

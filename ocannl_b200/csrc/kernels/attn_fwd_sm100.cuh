@@ -144,22 +144,30 @@ __device__ __forceinline__ unsigned int tile_class(const AttnSpan& s, int j0, in
   if (kmax < s.doc_min || kmin > s.doc_max) return 0u;
   return (j0 + width - 1 <= s.last_min && !negative && kmin == kmax && s.doc_min == s.doc_max && s.doc_min == kmin) ? 1u : 2u;
 }
-// range of the non-negative documents of W keys from j0 (a warp); `negative`: some are padding
-template <int W>
-__device__ __forceinline__ void key_documents(const AttnArgs& a, int b, int j0, unsigned int lane, int& kmin, int& kmax, bool& negative) {
-  int lo = 0x7fffffff, hi = -1, bad = 0;
+// Ranges of the non-negative documents of the W keys of each of N tiles from tile t on, `step` apart (a warp); `negative`: some are
+// padding.  All loads are under way before the first is used.
+template <int W, int N>
+__device__ __forceinline__ void key_documents(const AttnArgs& a, int b, int t, int step, unsigned int lane, int (&kmin)[N], int (&kmax)[N], bool (&negative)[N]) {
+  int d[N][W / 32];
 #pragma unroll
-  for (int i = 0; i < W / 32; ++i) {
-    const int j = j0 + (int)lane + 32 * i;
-    if (j < a.T) {
-      const int d = a.kdoc[(long long)b * a.T + j];
-      if (d < 0) bad = 1;
-      else { lo = min(lo, d); hi = max(hi, d); }
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int i = 0; i < W / 32; ++i) {
+      const long long j = (long long)(t + n * step) * W + lane + 32 * i;
+      d[n][i] = j < a.T ? __ldg(a.kdoc + (long long)b * a.T + j) : -0x7fffffff - 1;      // (no key: neither a document nor padding)
     }
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    int lo = 0x7fffffff, hi = -1, bad = 0;
+#pragma unroll
+    for (int i = 0; i < W / 32; ++i) {
+      if (d[n][i] < 0) bad |= d[n][i] != -0x7fffffff - 1;
+      else { lo = min(lo, d[n][i]); hi = max(hi, d[n][i]); }
+    }
+    kmin[n] = __reduce_min_sync(0xffffffffu, lo);
+    kmax[n] = __reduce_max_sync(0xffffffffu, hi);
+    negative[n] = __any_sync(0xffffffffu, bad);
   }
-  kmin = __reduce_min_sync(0xffffffffu, lo);
-  kmax = __reduce_max_sync(0xffffffffu, hi);
-  negative = __any_sync(0xffffffffu, bad);
 }
 // Which of 32 N keys from j0 the lane's row sees, a bit each.  The rows of a warp belong to one document or a few: one round each.
 template <int N>
@@ -309,14 +317,19 @@ attn_forward_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant__
     n_tiles = 0;
 #pragma unroll
     for (int i = 0; i < NQ; ++i) n_tiles = max(n_tiles, (spans[i].last_max + KW) / KW);
-    for (int t = (int)warp; t < n_tiles; t += (int)(Sh::kThreads / 32)) {
-      int kmin = 0, kmax = 0;
-      bool negative = false;
-      key_documents<KW>(a, b, t * KW, lane, kmin, kmax, negative);
-      unsigned int c = 0;
+    constexpr int kWarps = Sh::kThreads / 32, kAhead = 4;
+    for (int t0 = (int)warp; t0 < n_tiles; t0 += kAhead * kWarps) {
+      int kmin[kAhead], kmax[kAhead];
+      bool negative[kAhead];
+      key_documents<KW, kAhead>(a, b, t0, kWarps, lane, kmin, kmax, negative);
 #pragma unroll
-      for (int i = 0; i < NQ; ++i) c |= tile_class(spans[i], t * KW, KW, true, kmin, kmax, negative) << (2 * i);
-      if (lane == 0) classes[t] = (unsigned char)c;
+      for (int n = 0; n < kAhead; ++n) {
+        const int t = t0 + n * kWarps;
+        unsigned int c = 0;
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) c |= tile_class(spans[i], t * KW, KW, true, kmin[n], kmax[n], negative[n]) << (2 * i);
+        if (lane == 0 && t < n_tiles) classes[t] = (unsigned char)c;
+      }
     }
     __syncthreads();
   }
@@ -444,12 +457,12 @@ attn_forward_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant__
       const unsigned int cls = docs ? (classes[t] >> (2 * g)) & 3u : tile_class(mine_span, t * KW, KW, false, 0, 0, false);
       if (!cls) continue;
       const unsigned int place = seen % Sh::kScores, at = mine + place * KW;
+      unsigned int bits[KW / 32];
+      if (cls == 2u) visible_words<KW / 32>(a, b, t * KW, row, lane, bits);     // (its loads pass while the scores are formed)
       live = b200_wait(bar_s + 16 * g + 8 * place, seen / Sh::kScores & 1u, abort_flag, a.status, 28u);
       if (!live) break;
       tc_after();
       // first pass: the row's maximum, 32 scores at a time; what cap, bias or mask have changed goes back
-      unsigned int bits[KW / 32];
-      if (cls == 2u) visible_words<KW / 32>(a, b, t * KW, row, lane, bits);
       float x[2][32], top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
       b200_tmem_ld32(at, (unsigned int*)x[0]);
 #pragma unroll

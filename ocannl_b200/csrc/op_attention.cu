@@ -126,14 +126,14 @@ __global__ void __launch_bounds__(256) attn_dkv_rows(const __grid_constant__ Att
   }
 }
 
-// ---- rows of `d` elements to or from rows of `ld` (heads that no tensor map describes pass through padded copies)
+// ---- rows of `d` elements to or from rows of `ld` (heads that no tensor map describes pass through padded copies); the padding is zeros
 __global__ void __launch_bounds__(256) attn_copy_rows(const unsigned short* src, unsigned short* dst, long long rows, int d, int from, int to) {
   grid_begin();
-  const long long n = rows * d;
+  const long long n = rows * to;
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
-    const long long row = i / d;
-    const int e = (int)(i - row * d);
-    dst[row * to + e] = src[row * from + e];
+    const long long row = i / to;
+    const int e = (int)(i - row * to);
+    dst[i] = e < d ? src[row * from + e] : (unsigned short)0;
   }
 }
 
@@ -365,6 +365,9 @@ struct AttnOperator : b200_operator {
     // Heads of more than 64 elements: two query tiles a CTA share each key tile (64 KB per tile of 128 x 128 would otherwise
     // come in from L2 for 1024 cycles of products), unless that leaves SMs without work.
     const bool two = a.D > 64 && heads * ((a.S + 255) / 256) >= dev->sm_count;
+    // Key tiles of 64, whose next scores are formed during the softmax of the ones before, where that takes long (capped scores: 2 x 4096
+    // positions, 16 heads of 128, causal 261 us with tiles of 128, 226 with 64) and for heads of up to 64 elements (239 and 228); tiles
+    // of 128 else (281 and 304 without a mask, 209 and 213 with a bias).
     by_type(dtype, [&](auto t) {
       typedef decltype(t) T;
       if constexpr (sizeof(T) == 2) {
@@ -373,6 +376,7 @@ struct AttnOperator : b200_operator {
           else set_grad<T, 128, 128>();
         } else {
           if (a.D <= 64) set<T, 64, 1, 64>();
+          else if (two && a.cap > 0.f) set<T, 128, 2, 64>();
           else if (two) set<T, 128, 2, 128>();
           else set<T, 128, 1, 64>();
         }
