@@ -22,7 +22,7 @@ struct AttnArgs {
   unsigned int* status;
   int B, S, T, H, HK, D, group, mask;
   int ld;                                // elements from one head of a row to the next: D, or more in padded copies
-  float scale, cap;
+  float scale, cap, over;                // over: scale / cap
 };
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -66,7 +66,7 @@ __device__ __forceinline__ long long attn_k_at(const AttnArgs& a, int b, int j, 
 __device__ __forceinline__ float attn_score(const AttnArgs& a, float x, float slope2, int pos, int j, float& th) {
   float s;
   if (a.cap > 0.f) {
-    th = tanhf(x * a.scale / a.cap);
+    th = tanhf(x * a.over);
     s = th * (a.cap * kLog2e);
   } else {
     th = 0.f;

@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(256) attn_copy_rows(const unsigned short* src,
 typedef void (*KeysKernel)(const b200_tmap, const b200_tmap, const b200_tmap, const b200_tmap, const b200_tmap, const b200_tmap, const AttnArgs);
 typedef void (*QueriesKernel)(const b200_tmap, const b200_tmap, const b200_tmap, const b200_tmap, const b200_tmap, const AttnArgs);
 
-typedef void (*SingleKernel)(const AttnArgs, int);
+typedef void (*SingleKernel)(const AttnArgs, int, int);
 typedef void (*FewKernel)(const AttnArgs, const FewArgs);
 
 template <class T, int DP>
@@ -206,6 +206,7 @@ struct AttnOperator : b200_operator {
   QueriesKernel queries = nullptr;
   SingleKernel single[2] = {nullptr, nullptr};      // forward, or the gradients' two
   size_t single_smem[2] = {0, 0};
+  int single_places[2] = {1, 1};
   int vec = 0;
   FewKernel few = nullptr;
   FewArgs few_args = {};
@@ -334,16 +335,31 @@ struct AttnOperator : b200_operator {
   void choose_single() {
     vec = a.D % 4 == 0;
     for (const void* p : {a.q, a.k, a.v, a.d_out}) vec &= ((size_t)p & 15) == 0;
+    // Blocks of 32 rows where 64 leave the machine few of them: more, and more even, shares.  Heads of up to 64 elements run two such
+    // blocks an SM and gain up to four blocks of 64 rows an SM (2 x 1024 positions, 8 heads of 64, gradients 437 -> 370 us), wider ones one
+    // block either way (heads of 128: 572 -> 795).
+    const bool wide = a.D > 64;
+    auto of_rows = [&](long long heads, long long n) {
+      const bool small = heads * ((n + 63) / 64) < (wide ? 1ll : 4ll) * dev->sm_count;
+      return std::make_pair(small ? 2 : 4, blocks_of(heads * ((n + (small ? 31 : 63)) / (small ? 32 : 64))));
+    };
+    const auto by_query = of_rows((long long)a.B * a.H, a.S), by_key = of_rows((long long)a.B * a.HK, a.T);
+    const int rq = by_query.first, rk = by_key.first;
+    grid = by_query.second;
+    keys_grid = by_key.second;
+    auto room = [&](int i, int r, int own, int weights) {
+      single_places[i] = SingleShape::smem(a.D, r, own, weights, 2) <= (size_t)(r == 2 && !wide ? 113 : 227) * 1024 ? 2 : 1;
+      single_smem[i] = SingleShape::smem(a.D, r, own, weights, single_places[i]);
+    };
     if (grad) {
-      single[0] = a.D <= 64 ? attn_grad_keys_single<1> : attn_grad_keys_single<2>;
-      single[1] = a.D <= 64 ? attn_grad_queries_single<1> : attn_grad_queries_single<2>;
-      single_smem[0] = single_smem[1] = SingleShape::smem(a.D, 4);
-      keys_grid = blocks_of((long long)a.B * a.HK * ((a.T + kSide - 1) / kSide));
+      single[0] = rk == 2 ? (wide ? attn_grad_keys_single<2, 2> : attn_grad_keys_single<1, 2>) : (wide ? attn_grad_keys_single<2, 4> : attn_grad_keys_single<1, 4>);
+      single[1] = rq == 2 ? (wide ? attn_grad_queries_single<2, 2> : attn_grad_queries_single<1, 2>) : (wide ? attn_grad_queries_single<2, 4> : attn_grad_queries_single<1, 4>);
+      room(0, rk, 2, 2);
+      room(1, rq, 2, 1);
     } else {
-      single[0] = a.D <= 64 ? attn_forward_single<1> : attn_forward_single<2>;
-      single_smem[0] = SingleShape::smem(a.D, 3);
+      single[0] = rq == 2 ? (wide ? attn_forward_single<2, 2> : attn_forward_single<1, 2>) : (wide ? attn_forward_single<2, 4> : attn_forward_single<1, 4>);
+      room(0, rq, 1, 1);
     }
-    grid = blocks_of((long long)a.B * a.H * ((a.S + kSide - 1) / kSide));
     for (int i = 0; i < 2; ++i)
       if (single[i]) ready(single[i], single_smem[i]);
   }
@@ -438,8 +454,8 @@ struct AttnOperator : b200_operator {
     } else if (tc) {
       launch(forward, grid, threads, smem, s, map_q, map_k, map_v, map_o, a);
     } else if (single[0]) {
-      launch(single[0], grad ? keys_grid : grid, 256, single_smem[0], s, a, vec);
-      if (grad) launch(single[1], grid, 256, single_smem[1], s, a, vec);
+      launch(single[0], grad ? keys_grid : grid, 256, single_smem[0], s, a, vec, single_places[0]);
+      if (grad) launch(single[1], grid, 256, single_smem[1], s, a, vec, single_places[1]);
     } else if (grad) {
       if (rows) launch(kernel(1), blocks(rows), 256, 0, s, a);
       if (key_rows) launch(kernel(2), blocks(key_rows), 256, 0, s, a);
@@ -502,6 +518,7 @@ void bind(const b200_attention& p, AttnOperator* op, bool grad) {
   a.mask = p.mask;
   a.scale = p.scale;
   a.cap = p.cap;
+  a.over = p.cap > 0.f ? p.scale / p.cap : 0.f;
   op->choose();
 }
 
