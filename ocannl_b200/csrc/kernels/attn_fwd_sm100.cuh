@@ -224,10 +224,10 @@ attn_forward_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant__
   unsigned long long* bars = (unsigned long long*)(gen + Sh::kBytes);
   const unsigned int bar0 = b200_smem_addr(bars);
   const unsigned int bar_q = bar0, bar_kf = bar0 + 8, bar_ke = bar0 + 40, bar_vf = bar0 + 72, bar_ve = bar0 + 104;   // four slots each but bar_q
-  const unsigned int bar_s = bar0 + 136, bar_p = bar0 + 168, bar_o = bar0 + 200;      // a query tile each; bar_s, bar_p: two places each
-  volatile unsigned int* tmem_slot = (volatile unsigned int*)(bars + 27);
+  const unsigned int bar_s = bar0 + 136, bar_p = bar0 + 168, bar_o = bar0 + 200, bar_f = bar0 + 216;      // a query tile each; bar_s, bar_p: two places each
+  volatile unsigned int* tmem_slot = (volatile unsigned int*)(bars + 29);
   volatile unsigned int* abort_flag = tmem_slot + 1;
-  AttnSpan* spans = (AttnSpan*)(bars + 30);           // [2], 16 bytes each
+  AttnSpan* spans = (AttnSpan*)(bars + 32);           // [2], 16 bytes each
   unsigned char* classes = (unsigned char*)(gen + Sh::kBytes + 512);
 
   asm volatile("griddepcontrol.launch_dependents;");
@@ -263,6 +263,7 @@ attn_forward_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant__
     }
     for (int i = 0; i < 2; ++i) {
       b200_mbar_init(bar_o + 8 * i, 1);
+      b200_mbar_init(bar_f + 8 * i, 1);
       spans[i].last_min = spans[i].doc_min = 0x7fffffff;
       spans[i].last_max = -1;
       spans[i].doc_max = -0x7fffffff - 1;
@@ -430,7 +431,9 @@ attn_forward_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant__
             const unsigned long long dv = b200_smem_desc(v_at + slot * Sh::kKeys, Sh::kPanel, 1024u);
 #pragma unroll
             for (unsigned int ks = 0; ks < KW / 16; ++ks) umma_ts(acc_o + i * DP, weights + ks * 8, dv + ks * 128, idesc_o, (done[i] || ks) ? 1u : 0u);
-            if (Sh::kScores == 2 || t == last[i]) b200_umma_commit(bar_o + 8 * i);
+            // the last product has a barrier of its own: the others' may be two phases behind when it is waited for
+            if (t == last[i]) b200_umma_commit(bar_f + 8 * i);
+            else if (Sh::kScores == 2) b200_umma_commit(bar_o + 8 * i);
             ++done[i];
           }
           if (i == NQ - 1) b200_umma_commit(bar_ve + 8 * slot);
@@ -492,7 +495,8 @@ attn_forward_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant__
         const float m_new = fmaxf(m, m_tile);
         const float by = m == -INFINITY ? 0.f : ex2(m - m_new);
         if (seen) {
-          // (with one place the scores came behind the product before; with two it may still run)
+          // (with one place the scores came behind the product before; with two it may still run, but not the one before it, which the
+          // scores came behind: the barrier is in this phase or past it)
           if (Sh::kScores == 2) {
             live = b200_wait(bar_o + 8 * g, (seen - 1) & 1u, abort_flag, a.status, 30u);
             tc_after();
@@ -542,7 +546,7 @@ attn_forward_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant__
     }
     // ---------------------------------------------------------------- output
     // (the output goes through the queries' tile, which has to have arrived even where nobody reads it)
-    if (live) live = b200_wait(seen ? bar_o + 8 * g : bar_q, seen && Sh::kScores == 2 ? (seen - 1) & 1u : 0u, abort_flag, a.status, 29u);
+    if (live) live = b200_wait(seen ? bar_f + 8 * g : bar_q, 0u, abort_flag, a.status, 29u);
     tc_after();
     const float by = l > 0.f || l != l ? 1.f / l : 0.f;
     float bad = 0.f;

@@ -1,4 +1,6 @@
 """Layer norm, rotary positions and attention as linked operators, against their definitions in 64 bits."""
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -160,19 +162,6 @@ def rotary_long(x, f, p, layout, inverse, mag):
     return y
 
 
-def test_rotary_frequencies():
-    f, m = bk.rotary_frequencies(64)
-    assert m == 1.0 and f[0] == 1.0 and abs(f[31] - 10000.0 ** (-62 / 64)) < 1e-18
-    g, _ = bk.rotary_frequencies(64, scaling="ntk", factor=8.0)
-    assert g[0] == 1.0 and abs(g[31] / f[31] * 8.0 - 1.0) < 1e-12
-    y, m = bk.rotary_frequencies(64, scaling="yarn", factor=8.0)
-    assert y[0] == f[0] and abs(y[31] / f[31] * 8.0 - 1.0) < 1e-12 and m > 1.0 and np.all(np.diff(y) < 0)
-    with pytest.raises(bk.UserError):
-        bk.rotary_frequencies(63)
-    with pytest.raises(bk.UserError):
-        bk.rotary_frequencies(64, scaling="unknown")
-
-
 # ------------------------------------------------------------------ attention
 def docs_of(rng, b, n):
     ids = np.cumsum(rng.random((b, n)) < 4.0 / max(n, 4), 1).astype(np.int32)
@@ -318,5 +307,373 @@ def test_attention_ignores_what_is_not_seen(device, case, prec):
     device.await_()
     for m, (v, bound) in zip(("dq", "dk", "dv"), want):
         R.within(nodes.read(m), v, bound, m)
+    op.free()
+    nodes.free()
+
+
+def test_attention_gradients_by_differences(device):
+    """The gradients that the operator gives against central differences of the forward operator, in single precision."""
+    case = (2, 70, 70, 4, 2, 24, "prefix", True, None, 8.0, True)
+    x, t, more, sl, seen, pos, scale = attention_case(case, "single")
+    nodes, fwd = link_attention(device, case, "single", {n: x[n] for n in "qkv"}, t, more, sl, "aligned")
+    fwd.run()
+    x["out"], x["lse"] = nodes.read("out"), nodes.read("lse")
+    grads, bwd = link_attention(device, case, "single", x, t, more, sl, "aligned", grad=True)
+    bwd.run()
+    rng = np.random.default_rng(3)
+    for name in "qkv":
+        got = grads.read("d" + name)
+        direction, step, vals = rng.standard_normal(x[name].shape), 2.0 ** -6, []
+        for sign in (1, -1):
+            nodes.context.from_host(name, (x[name] + sign * step * direction).astype(np.float32))
+            fwd.run()
+            vals.append((nodes.read("out") * x["d_out"]).sum())
+        nodes.context.from_host(name, x[name].astype(np.float32))
+        diff, want = (vals[0] - vals[1]) / (2 * step), (got * direction).sum()
+        # values in single precision (2^-15 of their sizes at most), divided by the step; the third derivative's share is step^2
+        # of a sum of products like the first's
+        size = np.abs(x["out"] * x["d_out"]).sum()
+        assert abs(diff - want) <= R.ARITH * np.sqrt(x["out"].size) * size / x["out"].size / step + 64 * step ** 2 * np.abs(got * direction).sum(), (name, diff, want)
+    for o in (fwd, bwd):
+        o.free()
+    nodes.free()
+    grads.free()
+
+
+def test_weights_of_16_bits_in_the_norm(device):
+    x, _, gamma, beta, _ = norm_case(9, 96, "bfloat16", 4, False)
+    gamma, beta = R.rounded("bfloat16", gamma), R.rounded("bfloat16", beta)
+    nodes = R.Nodes(device, dict(x=("bfloat16", (9, 96), x), gamma=("bfloat16", (96,), gamma), beta=("bfloat16", (96,), beta), y=("bfloat16", (9, 96), None)))
+    op = nodes.context.layer_norm("x", "y", gamma="gamma", beta="beta")
+    op.run()
+    y = R.layer_norm(x, gamma, beta)[0]
+    R.within(nodes.read("y"), y, R.EPS["bfloat16"] / 2 * np.abs(y) + 2.0 ** -14, "y")
+    op.free()
+    bare = nodes.context.layer_norm("x", "y")
+    bare.run()
+    y = R.layer_norm(x, 1.0, 0.0)[0]
+    R.within(nodes.read("y"), y, R.EPS["bfloat16"] / 2 * np.abs(y) + 2.0 ** -14, "y")
+    bare.free()
+    nodes.free()
+
+
+def test_memory_around_the_outputs_is_left_alone(device):
+    """Outputs between other nodes, aligned to their elements alone: what lies before and behind them keeps its values."""
+    for prec in PRECS:
+        case = (1, 70, 70, 2, 1, 40, "causal", True, None, 0.0, False)
+        x, t, more, sl, seen, pos, scale = attention_case(case, prec)
+        b, s, n, h, hk, d = case[:6]
+        out, lse, _, _ = R.attention(x["q"], x["k"], x["v"], seen, pos, scale)
+        mark = np.arange(5, dtype=np.float64) + 1
+        a = {m: (prec, v.shape, v) for m, v in x.items()}
+        a.update({m: ("int32", v.shape, v) for m, v in more.items()})
+        a.update(fwd_out=(prec, out.shape, None), lse=("single", lse.shape, R.rounded("single", lse)), out=(prec, out.shape, R.rounded(prec, out)))
+        for i, m in enumerate(("dq", "dk", "dv", "y")):
+            a["guard%d" % i] = (prec, (5,), mark)
+            a[m] = (prec, x["k" if m in ("dk", "dv") else "q"].shape, None)
+        a["guard9"] = (prec, (5,), mark)
+        nodes = R.Nodes(device, a, "tight", odd_first=True)
+        ctx, docs = nodes.context, ("qdoc", "kdoc")
+        ops = [ctx.attention("q", "k", "v", "fwd_out", documents=docs), ctx.attention_grad("q", "k", "v", "out", "lse", "d_out", "dq", "dk", "dv", documents=docs),
+               ctx.rotary([("q", "y")], bk.rotary_frequencies(20)[0])]
+        for o in ops:
+            o.run()
+        device.await_()
+        for g in ("guard0", "guard1", "guard2", "guard3", "guard9"):
+            assert np.array_equal(nodes.read(g), mark), g
+        assert np.array_equal(nodes.read("q"), x["q"]) and np.array_equal(nodes.read("k"), x["k"])
+        for o in ops:
+            o.free()
+        nodes.free()
+
+
+def test_captured_replayed_and_with_a_growing_cache(device):
+    """One operator captured into a CUDA graph: replays read the lengths and keys of their time; a second operator of the same
+    sizes runs between them."""
+    import torch
+    case = (3, 1, 400, 8, 2, 64, "causal", False, (5, 100, 250), 0.0, False)
+    x, t, more, sl, _, _, scale = attention_case(case, "bfloat16")
+    nodes, op = link_attention(device, case, "bfloat16", {n: x[n] for n in "qkv"}, t, more, sl, "aligned")
+    others, other = link_attention(device, case, "bfloat16", {n: x[n] * 0.5 for n in "qkv"}, t, more, sl, "aligned")
+    device.await_()
+    stream = torch.cuda.ExternalStream(device.stream_handle())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        op.run()
+    for lengths in ((5, 100, 250), (6, 101, 251), (400, 0, 399)):
+        nodes.context.from_host("lengths", np.array(lengths, np.int32))
+        with torch.cuda.stream(stream):
+            graph.replay()
+        other.run()
+        with torch.cuda.stream(stream):
+            graph.replay()
+        device.await_()
+        seen, pos = R.visible(3, 1, 400, "causal", lengths=lengths)
+        out, lse, size, flat = R.attention(x["q"], x["k"], x["v"], seen, pos, scale)
+        R.within(nodes.read("out"), out, out_bound("bfloat16", out, size, flat), "out")
+    del graph
+    for o in (op, other):
+        o.free()
+    nodes.free()
+    others.free()
+
+
+def test_runs_wait_for_uploads(device):
+    """With uploads on a second stream a run sees what was uploaded before it."""
+    rows, n = 4096, 1024
+    rng = np.random.default_rng(8)
+    x = rng.standard_normal((rows, n)).astype(np.float32)
+    nodes = R.Nodes(device, dict(x=("single", (rows, n), np.zeros((rows, n))), y=("single", (rows, n), None)))
+    op = nodes.context.layer_norm("x", "y")
+    device.set_async_uploads(True)
+    try:
+        pool, off, _ = nodes.context.arrays["x"]
+        buf = bk.PinnedBuffer((rows, n), np.float32)
+        buf.array[...] = x
+        device.from_host(pool, off, buf.array)
+        op.run()
+        got = nodes.read("y")
+    finally:
+        device.set_async_uploads(False)
+    y = R.layer_norm(x.astype(np.float64), 1.0, 0.0)[0]
+    R.within(got, y, 2.0 ** -17 * (1 + np.abs(y)), "y")
+    buf.free()
+    op.free()
+    nodes.free()
+
+
+@pytest.mark.parametrize("queries", [1, 20])
+def test_offsets_behind_two_to_the_31(device, queries):
+    """A cache of 2.1 million positions: 2^31 elements and more of keys and of values.  All keys are zero, so all weights are equal."""
+    n, hk, d = 2_100_000, 8, 128
+    assert n * hk * d > 2 ** 31
+    pools = [device.alloc_pool(n * hk * d * 2) for _ in range(2)]
+    for p in pools:
+        device.memset_zero(p, 0, n * hk * d * 2)
+    tail = 64
+    last = R.rounded("bfloat16", np.random.default_rng(1).standard_normal((tail, hk, d)) * n / 100)
+    from ocannl_b200.workloads import store
+    device.from_host(pools[1], (n - tail) * hk * d * 2, store("bfloat16", last.astype(np.float32)))
+    from ocannl_b200.low_level import Tnode
+    nodes = R.Nodes(device, dict(q=("bfloat16", (1, queries, hk, d), np.ones((1, queries, hk, d))), out=("bfloat16", (1, queries, hk, d), None)))
+    arrays = dict(nodes.context.arrays, k=(pools[0], 0, Tnode(90, "k", "bfloat16", (1, n, hk, d))), v=(pools[1], 0, Tnode(91, "v", "bfloat16", (1, n, hk, d))))
+    op = bk.Context(device, arrays).attention("q", "k", "v", "out", mask="none")
+    op.run()
+    want = last.sum(0) / n
+    # equal weights of one; sums of n of them and of 64 products in single precision, added in parts
+    R.within(nodes.read("out"), np.broadcast_to(want, (1, queries, hk, d)), R.EPS["bfloat16"] / 2 * np.abs(want) + 2.0 ** -12 * np.abs(last).sum(0) / n, "out")
+    op.free()
+    for p in pools:
+        device.free_pool(p)
+    nodes.free()
+
+
+def test_what_link_refuses(device):
+    nodes = R.Nodes(device, dict(x=("single", (64, 64), np.ones((64, 64))), q=("bfloat16", (2, 8, 4, 16), None), k=("bfloat16", (2, 8, 2, 16), None), o=("bfloat16", (2, 8, 4, 16), None)))
+    pool, off, _ = nodes.context.arrays["x"]
+
+    def linked(entry, spec):
+        return bk.Operator(device, entry, spec)
+
+    def norm(**kw):
+        base = dict(rows=4, n=16, dtype=0, weight_dtype=0, eps=1e-5, x=bk.Operand(pool, off), y=bk.Operand(pool, off + 1024))
+        return bk.LayerNormSpec(**dict(base, **kw))
+
+    def attn(**kw):
+        at = {n: bk.Operand(*nodes.context.arrays[n][:2]) for n in "qk"}
+        base = dict(batch=2, queries=8, keys=8, heads=4, kv_heads=2, d=16, dtype=1, mask=1, scale=0.25, cap=0.0, q=at["q"], k=at["k"], v=at["k"],
+                    out=bk.Operand(*nodes.context.arrays["o"][:2]))
+        return bk.AttentionSpec(**dict(base, **kw))
+
+    def rot(**kw):
+        f = (ctypes.c_double * 8)(*([1.0] * 8))
+        base = dict(batch=2, seq=8, heads=(4, 0), d=16, pairs=8, dtype=1, magnitude=1.0, frequencies=f, x=two("q"), y=two("o"))
+        return bk.RotarySpec(**dict(base, **kw))
+
+    def two(name):
+        return (bk.Operand * 2)(bk.Operand(*nodes.context.arrays[name][:2]), bk.Operand(-1, 0))
+
+    for entry, spec, code, words in [
+            ("b200_layer_norm_link", norm(y=bk.Operand(pool, off + 16)), -1, "overlaps"),
+            ("b200_layer_norm_link", norm(y=bk.Operand(pool, off)), -1, "overlaps"),
+            ("b200_layer_norm_link", norm(y=bk.Operand(pool, off + 1026)), -1, "multiple of its element"),
+            ("b200_layer_norm_link", norm(rows=1 << 20), -1, "exceeds pool"),
+            ("b200_layer_norm_link", norm(rows=1 << 60, n=1 << 29), -1, "too many"),
+            ("b200_layer_norm_link", norm(x=bk.Operand(987654, 0)), -1, "unknown pool"),
+            ("b200_layer_norm_link", norm(x=bk.Operand(-1, 0)), -1, "'x' is required"),
+            ("b200_layer_norm_link", norm(dtype=7), -1, "element type"),
+            ("b200_layer_norm_link", norm(weight_dtype=1), -1, "gamma and beta"),
+            ("b200_layer_norm_link", norm(n=0), -1, "n between"),
+            ("b200_layer_norm_link", norm(eps=-1.0), -1, "eps"),
+            ("b200_layer_norm_link", norm(total=bk.Operand(pool, off + 2048)), -1, "residual"),
+            ("b200_layer_norm_grad_link", norm(), -1, "required"),
+            ("b200_rotary_link", rot(pairs=9), -1, "2 * pairs"),
+            ("b200_rotary_link", rot(heads=(0, 0)), -1, "heads"),
+            ("b200_rotary_link", rot(magnitude=float("nan")), -1, "magnitude"),
+            ("b200_rotary_link", rot(frequencies=(ctypes.c_double * 8)(*([float("inf")] * 8))), -1, "frequency"),
+            ("b200_rotary_link", rot(heads=(4, 2)), -1, "'x[1]' is required"),
+            ("b200_attention_link", attn(d=129), -4, "128"),
+            ("b200_attention_link", attn(heads=3), -1, "multiple of kv_heads"),
+            ("b200_attention_link", attn(scale=0.0), -1, "scale"),
+            ("b200_attention_link", attn(scale=float("inf")), -1, "scale"),
+            ("b200_attention_link", attn(cap=-1.0), -1, "cap"),
+            ("b200_attention_link", attn(mask=3), -1, "mask"),
+            ("b200_attention_link", attn(mask=2), -1, "prefix"),
+            ("b200_attention_link", attn(query_documents=bk.Operand(pool, off)), -1, "documents"),
+            ("b200_attention_link", attn(out=bk.Operand(*nodes.context.arrays["q"][:2])), -1, "overlaps"),
+            ("b200_attention_link", attn(keys=-1), -1, "between 0"),
+            ("b200_attention_grad_link", attn(), -1, "'lse' is required")]:
+        with pytest.raises(bk.B200Error) as e:
+            linked(entry, spec)
+        assert e.value.code == code and words in str(e.value), (entry, words, str(e.value))
+    nodes.free()
+
+
+# ------------------------------------------------------------------ together
+def matmul_routine(name, terms, rows):
+    """out[r, o] = sum over (w, x, transposed) of sum_i w[o, i] (or w[i, o]) x[r, i], single precision."""
+    from ocannl_b200.low_level import Routine, Seq, Set, loops
+    from ocannl_b200.workloads import reduce_scope
+    r = Routine(name)
+    tns, body = {}, []
+
+    def tn(n, dims):
+        if n not in tns:
+            tns[n] = r.tn(n, "single", dims)
+        return tns[n]
+    for out, o_dim, w, x, i_dim, transposed in terms:
+        wt, xt, ot = tn(w, (i_dim, o_dim) if transposed else (o_dim, i_dim)), tn(x, (rows, i_dim)), tn(out, (rows, o_dim))
+        a, o, i = r.syms(3)
+        body.append(loops([(a, rows), (o, o_dim)], Set(ot, (a, o), reduce_scope(
+            r, out + "_mm", "single", [(i, i_dim)], lambda: (wt[i, o] if transposed else wt[o, i], xt[a, i]), orig=(a, o)))))
+    r.body = Seq(body)
+    return r
+
+
+def test_a_decoder_layer_forward_and_backward(device):
+    """Norm, projections (a routine), rotary positions, attention, projection, residual and norm; then all gradients back to the
+    input, with the operators and routines of the framework in turn on one stream.  Against the layer in 64 bits and the
+    central difference of its loss."""
+    from ocannl_b200.low_level import Tnode
+    b, s, h, hk, e = 2, 45, 4, 2, 16
+    dm, rows = 48, 2 * 45
+    rng = np.random.default_rng(12)
+    w = {n: R.rounded("single", rng.standard_normal(shape) / np.sqrt(shape[1])) for n, shape in
+         (("wq", (h * e, dm)), ("wk", (hk * e, dm)), ("wv", (hk * e, dm)), ("wo", (dm, h * e)))}
+    g1, b1, g2, b2 = (R.rounded("single", o + 0.2 * rng.standard_normal(dm)) for o in (1, 0, 1, 0))
+    x, dy = (R.rounded("single", rng.standard_normal((rows, dm))) for _ in range(2))
+    docs = docs_of(rng, b, s)
+    freq = bk.rotary_frequencies(e)[0]
+    seen, pos = R.visible(b, s, s, "causal", qdoc=docs, kdoc=docs)
+    seat = np.broadcast_to(np.arange(s), (b, s))
+
+    def model(x):
+        n1, _, m1, r1, _ = R.layer_norm(x, g1, b1)
+        q, k, v = ((n1 @ w[n].T).reshape(b, s, -1, e) for n in ("wq", "wk", "wv"))
+        out, _, _, _ = R.attention(R.rotary(q, freq, seat), R.rotary(k, freq, seat), v, seen, pos, 0.25, 20.0)
+        return R.layer_norm(x, g2, b2, residual=out.reshape(rows, h * e) @ w["wo"].T)[0]
+
+    single = lambda n, dims, v=None: (n, dims, v)  # noqa: E731
+    plan = [single("x", (rows, dm), x), single("dy", (rows, dm), dy)] + [single(n, v.shape, v) for n, v in w.items()]
+    plan += [single(n, (dm,), v) for n, v in (("g1", g1), ("b1", b1), ("g2", g2), ("b2", b2))]
+    plan += [single(n, (rows, dm)) for n in ("n1", "o", "t", "y", "dt", "dn_q", "dn_k", "dn_v", "dn", "dx")]
+    plan += [single(n, (rows,)) for n in ("m1", "r1", "m2", "r2")] + [single(n, (dm,)) for n in ("dg1", "db1", "dg2", "db2")]
+    plan += [single(n, (b, h, s)) for n in ("lse",)]
+    wide, narrow = ("q", "av", "d_av", "dq"), ("k", "v", "dk", "dv")
+    tns = [Tnode(i + 1, n, "single", d) for i, (n, d, _) in enumerate(plan)]
+    # the projections' rows and the heads that the operators see are the same memory
+    ctx = bk.Context(device).allocate(tns + [Tnode(100, "docs", "int32", (b, s))] + [Tnode(200 + i, n, "single", (b, s, h if n in wide else hk, e)) for i, n in enumerate(wide + narrow)])
+    flat = dict(ctx.arrays)
+    for n in wide + narrow:
+        p, off, t = flat[n]
+        flat[n] = (p, off, Tnode(t.id, n, "single", (rows, (h if n in wide else hk) * e)))
+    for n, _, v in plan:
+        if v is not None:
+            ctx.from_host(n, v.astype(np.float32))
+    ctx.from_host("docs", docs)
+    by_rows = bk.Context(device, flat)
+    from ocannl_b200.low_level import Routine, Set, loops
+    codes = [bk.Code(matmul_routine("proj", [("q", h * e, "wq", "n1", dm, False), ("k", hk * e, "wk", "n1", dm, False), ("v", hk * e, "wv", "n1", dm, False)], rows), "tf32=0"),
+             bk.Code(matmul_routine("out_proj", [("o", dm, "wo", "av", h * e, False)], rows), "tf32=0"),
+             bk.Code(matmul_routine("out_grad", [("d_av", h * e, "wo", "dt", dm, True)], rows), "tf32=0"),
+             bk.Code(matmul_routine("proj_grad", [("dn_q", dm, "wq", "dq", h * e, True), ("dn_k", dm, "wk", "dk", hk * e, True), ("dn_v", dm, "wv", "dv", hk * e, True)], rows), "tf32=0")]
+    add = Routine("add")
+    parts = [add.tn(n, "single", (rows, dm), read_only=True) for n in ("dn_q", "dn_k", "dn_v")]
+    dn = add.tn("dn", "single", (rows, dm))
+    i, j = add.syms(2)
+    add.body = loops([(i, rows), (j, dm)], Set(dn, (i, j), parts[0][i, j] + parts[1][i, j] + parts[2][i, j]))
+    codes.append(bk.Code(add))
+    proj, out_proj, out_grad, proj_grad, adding = (by_rows.link(c) for c in codes)
+    terms = dict(documents="docs", cap=20.0, scale=0.25)
+    av_as_heads, turned = ctx, [("q", "q"), ("k", "k")]
+    steps = [ctx.layer_norm("x", "n1", gamma="g1", beta="b1", mean="m1", rstd="r1"), proj, ctx.rotary(turned, freq),
+             av_as_heads.attention("q", "k", "v", "av", lse="lse", **terms), out_proj,
+             ctx.layer_norm("x", "y", gamma="g2", beta="b2", residual="o", total="t", mean="m2", rstd="r2"),
+             ctx.layer_norm_grad("t", "dy", "dt", "m2", "r2", gamma="g2", dgamma="dg2", dbeta="db2"), out_grad,
+             ctx.attention_grad("q", "k", "v", "av", "lse", "d_av", "dq", "dk", "dv", **terms),
+             ctx.rotary([("dq", "dq"), ("dk", "dk")], freq, inverse=True), proj_grad, adding,
+             ctx.layer_norm_grad("x", "dn", "dx", "m1", "r1", gamma="g1", dgamma="dg1", dbeta="db1", d_total="dt")]
+    first = None
+    for _ in range(2):
+        for st in steps:
+            st.run()
+        device.await_()
+        got = {n: ctx.to_host(n).astype(np.float64) for n in ("y", "dx", "dg1", "db2")}
+        first = first or got
+        assert all(np.array_equal(first[n], got[n]) for n in got), "the same inputs give the same bits"
+    want = model(x)
+    assert np.abs(got["y"] - want).max() <= 2.0 ** -14 * (1 + np.abs(want).max())
+    for _ in range(3):
+        direction, step = rng.standard_normal(x.shape), 1e-5
+        diff = ((model(x + step * direction) - model(x - step * direction)) * dy).sum() / (2 * step)
+        assert abs((got["dx"] * direction).sum() - diff) <= 2.0 ** -13 * np.abs(got["dx"] * direction).sum(), (diff, (got["dx"] * direction).sum())
+    for st in steps:
+        st.free()
+    for c in codes:
+        c.free()
+    for p in {p for p, _, _ in ctx.arrays.values()}:
+        device.free_pool(p)
+
+
+# many tiles in a row, where a wait that is missing or too early would show
+LONG = [
+    (2, 1030, 1030, 2, 1, 64, "causal", False, None, 0.0, False),
+    (3, 1030, 1030, 4, 2, 128, "causal", True, None, 30.0, False),
+    (40, 513, 513, 2, 2, 128, "none", False, None, 0.0, True),
+    (24, 640, 640, 4, 4, 128, "prefix", False, None, 20.0, True),
+    (30, 300, 900, 4, 1, 32, "causal", False, None, 0.0, False),
+]
+
+
+@pytest.mark.parametrize("prec", ("bfloat16", "half"))
+@pytest.mark.parametrize("case", LONG)
+def test_attention_over_many_tiles(device, case, prec):
+    x, t, more, sl, seen, pos, scale = attention_case(case, prec)
+    some = [0, case[0] // 2, case[0] - 1]          # sequences that are compared; all have to repeat their bits
+    part = {n: v[some] for n, v in x.items()}
+    out, lse, size, flat = R.attention(part["q"], part["k"], part["v"], seen[some], pos[some], scale, t["cap"], sl)
+    nodes, op = link_attention(device, case, prec, {n: x[n] for n in "qkv"}, t, more, sl, "aligned")
+    first = None
+    for _ in range(6):
+        op.run()
+        got = nodes.read("out"), nodes.read("lse")
+        first = first or got
+        assert all(np.array_equal(f, g) for f, g in zip(first, got)), "the same inputs give the same bits"
+    R.within(first[0][some], out, out_bound(prec, out, size, flat), "out")
+    R.within(first[1][some], lse, R.ARITH * (1 + np.abs(np.where(np.isinf(lse), 0, lse))), "lse")
+    x["out"], x["lse"] = first
+    op.free()
+    nodes.free()
+    part = {n: v[some] for n, v in x.items()}
+    want = R.attention_grad(part["q"], part["k"], part["v"], part["out"], part["lse"], part["d_out"], seen[some], pos[some], scale, t["cap"], sl, prec)
+    nodes, op = link_attention(device, case, prec, x, t, more, sl, "aligned", grad=True)
+    first = None
+    for _ in range(6):
+        op.run()
+        got = [nodes.read(n) for n in ("dq", "dk", "dv")]
+        first = first or got
+        assert all(np.array_equal(f, g) for f, g in zip(first, got)), "the same inputs give the same bits"
+    for n, got, (v, bound) in zip(("dq", "dk", "dv"), first, want):
+        R.within(got[some], v, bound, n)
     op.free()
     nodes.free()
