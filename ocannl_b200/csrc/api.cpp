@@ -856,7 +856,9 @@ int b200_operator_run(b200_operator* op) {
     op->dev->make_current(/*join=*/false);
     if (op->dev->uploads_pending)
       for (int p : op->pools_used) op->dev->join_pool_id(p);
+    const long long before = operator_launches;
     op->run((cudaStream_t)op->dev->stream);
+    op->dev->n_launches += operator_launches - before;
   });
 }
 

@@ -1,7 +1,8 @@
 // The gradients of attention for 16-bit heads on the tensor cores.
 //
-// Two kernels, each of which owns its outputs and adds to them in a fixed order (no atomic additions: the same bits every time), at
-// the price of forming the scores and their gradients twice: seven products a pair of tiles instead of five.
+// Two kinds of CTAs in one launch, each of which owns its outputs and adds to them in a fixed order (no atomic additions: the same bits every time), at
+// the price of forming the scores and their gradients twice: seven products a pair of tiles instead of five.  (As two launches
+// few rows left most SMs idle twice.)
 //
 //   keys     a CTA has 128 keys of one key head and walks the tiles of 128 queries that see them, of all query heads it
 //            serves.  s^T = k q^T and dp^T = v do^T have a thread per key; p^T and ds^T go back to tensor memory in 16 bits, as the
@@ -116,10 +117,8 @@ __device__ __forceinline__ float pair_score(float x, float c, float slope2, floa
 
 // ------------------------------------------------------------------ keys
 template <class T, int DP, int CW, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(BwdShape<DP, CW>::kThreads, CW == 64 ? 2 : 1)
-attn_grad_keys_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant__ b200_tmap map_k, const __grid_constant__ b200_tmap map_v,
-                  const __grid_constant__ b200_tmap map_do, const __grid_constant__ b200_tmap map_dk, const __grid_constant__ b200_tmap map_dv,
-                  const __grid_constant__ AttnArgs a) {
+__device__ __forceinline__ void attn_grad_keys(const b200_tmap& map_q, const b200_tmap& map_k, const b200_tmap& map_v, const b200_tmap& map_do,
+                                               const b200_tmap& map_dk, const b200_tmap& map_dv, const AttnArgs& a, unsigned int block) {
   typedef BwdShape<DP, CW> Sh;
   extern __shared__ __align__(128) unsigned char dyn[];
   const unsigned int base = (b200_smem_addr(dyn) + 1023u) & ~1023u;
@@ -139,8 +138,8 @@ attn_grad_keys_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant
   constexpr unsigned int kLoad = Sh::kWarps - 2, kMma = Sh::kWarps - 1;
   // this CTA's keys: the first ones first, which under a causal mask are seen by the most queries
   const unsigned int heads = (unsigned int)a.B * (unsigned int)a.HK;
-  const int j0 = (int)(blockIdx.x / heads) * 128;
-  const unsigned int bh = blockIdx.x % heads;
+  const int j0 = (int)(block / heads) * 128;
+  const unsigned int bh = block % heads;
   const int b = (int)(bh / (unsigned int)a.HK), hk = (int)(bh % (unsigned int)a.HK);
   const int tiles = (a.S + CW - 1) / CW, stat_tiles = (a.S + 127) / 128;
   const bool docs = a.kdoc != nullptr;
@@ -321,7 +320,7 @@ attn_grad_keys_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant
   } else {
     const unsigned int half = warp >> 2, in = (warp & 3u) * 32 + lane, lanes = (warp & 3u) << 21;
     const unsigned int my_s = t_s + 64 * half + lanes, my_dp = t_dp + 64 * half + lanes;
-    const float c = CAP ? a.cap * kLog2e : a.scale * kLog2e, to_tanh = CAP ? a.scale / a.cap : 0.f;
+    const float c = CAP ? a.cap * kLog2e : a.scale * kLog2e, to_tanh = CAP ? a.over : 0.f;
     const int j = j0 + (int)in;
     unsigned int n = 0;
     bool live = true;
@@ -465,9 +464,8 @@ attn_grad_keys_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant
 
 // ------------------------------------------------------------------ queries
 template <class T, int DP, int CW, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(BwdShape<DP, CW>::kThreads, CW == 64 ? 2 : 1)
-attn_grad_queries_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant__ b200_tmap map_k, const __grid_constant__ b200_tmap map_v,
-                     const __grid_constant__ b200_tmap map_do, const __grid_constant__ b200_tmap map_dq, const __grid_constant__ AttnArgs a) {
+__device__ __forceinline__ void attn_grad_queries(const b200_tmap& map_q, const b200_tmap& map_k, const b200_tmap& map_v, const b200_tmap& map_do,
+                                                  const b200_tmap& map_dq, const AttnArgs& a, unsigned int block) {
   typedef BwdShape<DP, CW> Sh;
   extern __shared__ __align__(128) unsigned char dyn[];
   const unsigned int base = (b200_smem_addr(dyn) + 1023u) & ~1023u;
@@ -488,8 +486,8 @@ attn_grad_queries_tc(const __grid_constant__ b200_tmap map_q, const __grid_const
   constexpr unsigned int kLoad = Sh::kWarps - 2, kMma = Sh::kWarps - 1;
   const unsigned int heads = (unsigned int)a.B * (unsigned int)a.H;
   const int tiles_q = (a.S + 127) / 128;
-  const int t_q = tiles_q - 1 - (int)(blockIdx.x / heads), r0 = t_q * 128;
-  const unsigned int bh = blockIdx.x % heads;
+  const int t_q = tiles_q - 1 - (int)(block / heads), r0 = t_q * 128;
+  const unsigned int bh = block % heads;
   const int b = (int)(bh / (unsigned int)a.H), h = (int)(bh % (unsigned int)a.H), hk = h / a.group;
   const bool docs = a.kdoc != nullptr;
   if (threadIdx.x == kLoad * 32) {
@@ -644,7 +642,7 @@ attn_grad_queries_tc(const __grid_constant__ b200_tmap map_q, const __grid_const
   } else {
     const unsigned int lanes = (warp & 3u) << 21;
     const unsigned int my_dp = t_dp + 64 * half + lanes;
-    const float c = CAP ? a.cap * kLog2e : a.scale * kLog2e, to_tanh = CAP ? a.scale / a.cap : 0.f;
+    const float c = CAP ? a.cap * kLog2e : a.scale * kLog2e, to_tanh = CAP ? a.over : 0.f;
     const float slope2 = BIAS ? a.slopes[h] * kLog2e : 0.f;
     const float* stat = a.stat + (((long long)b * a.H + h) * tiles_q + t_q) * 256 + in;
     const float lse2 = stat[0], delta = stat[128];
@@ -768,6 +766,19 @@ attn_grad_queries_tc(const __grid_constant__ b200_tmap map_q, const __grid_const
     tc_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Sh::kColumns) : "memory");
   }
+}
+
+// What both kinds of CTAs are given: a tensor map for the rows a CTA owns and one for the tiles it walks
+struct GradMaps {
+  b200_tmap q, k, v, d_out, own_q, own_k, own_v, own_d_out, dq, dk, dv;
+};
+
+// The keys' CTAs come first: theirs are the longer walks.
+template <class T, int DP, int CW, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(BwdShape<DP, CW>::kThreads, CW == 64 ? 2 : 1)
+attn_grad_tc(const __grid_constant__ GradMaps m, const __grid_constant__ AttnArgs a, unsigned int keys_grid) {
+  if (blockIdx.x < keys_grid) attn_grad_keys<T, DP, CW, CAP, BIAS>(m.q, m.own_k, m.own_v, m.d_out, m.dk, m.dv, a, blockIdx.x);
+  else attn_grad_queries<T, DP, CW, CAP, BIAS>(m.own_q, m.k, m.v, m.own_d_out, m.dq, a, blockIdx.x - keys_grid);
 }
 
 }  // namespace b200

@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) attn_forward_few(const __grid_
   for (int i = 0; i < DP / 8; ++i)
 #pragma unroll
     for (int k = 0; k < 4; ++k) o[i][k] = 0.f;
-  const float c = CAP ? a.cap * kLog2e : a.scale * kLog2e, to_tanh = CAP ? 2.f * kLog2e * a.scale / a.cap : 0.f;
+  const float c = CAP ? a.cap * kLog2e : a.scale * kLog2e, to_tanh = CAP ? a.over : 0.f;
   const unsigned int ring = b200_smem_addr(dyn) + warp * Sh::kRing;
   const int steps = j_end > j_begin ? (j_end - j_begin + kFewStep - 1) / kFewStep : 0;
   const int mine = steps > (int)warp ? (steps - (int)warp + kFewWarps - 1) / kFewWarps : 0;     // this warp's steps
@@ -161,10 +161,8 @@ __global__ void __launch_bounds__(kFewWarps * 32) attn_forward_few(const __grid_
       mma16<T>(s[1], q[ks], y[2], y[3]);
     }
     if constexpr (CAP) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[h][i] = tanh_of(s[h][i] * to_tanh);
+      tanh_chunk(s[0], to_tanh);
+      tanh_chunk(s[1], to_tanh);
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h)

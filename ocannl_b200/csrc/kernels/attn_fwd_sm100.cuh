@@ -63,30 +63,32 @@ __device__ __forceinline__ Pair add2(const Pair& a, const Pair& b) {
   return r;
 }
 
-// x = tanh(x scale) of 32 scores.  The exponential and the reciprocal of tanh_of pass through the unit that also has to make the
-// weights, at an eighth of the multiply-adds' rate, and would bound the kernel: where all of a warp's scores are at most the cap in
-// size, tanh y = y P(y^2) instead, with P the polynomial of degree 5 whose largest error of y P on [0, 1] is least (2.4e-7; fitted by
-// iterated weighted least squares; 3.0e-7 in single precision).  2 x 4096 positions, 16 heads of 128, causal: 301 us without, 172 with it.
-__device__ __forceinline__ void tanh_chunk(float (&x)[32], float scale) {
+// x = tanh(x scale) of N scores of each lane.  The exponential and the reciprocal of tanh_of pass through the unit that also has to make
+// the weights, at an eighth of the multiply-adds' rate, and would bound the kernel: where all of a warp's scores are at most the cap in
+// size, tanh y = y + y^3 Q(y^2) instead, with Q the polynomial of degree 5 whose largest error on [0, 1] is least (2.6e-8, 8e-8 in single
+// precision, 1.6e-7 relative; fitted by iterated weighted least squares).  2 x 4096 positions, 16 heads of 128, causal: 301 us without,
+// 226 with it and tiles of 64 keys.
+template <int N>
+__device__ __forceinline__ void tanh_chunk(float (&x)[N], float scale) {
   float top = 0.f;
 #pragma unroll
-  for (int j = 0; j < 32; ++j) top = fmaxf(top, fabsf(x[j]));
+  for (int j = 0; j < N; ++j) top = fmaxf(top, fabsf(x[j]));
   if (__any_sync(0xffffffffu, top * scale > 1.f)) {
     const float s = 2.f * kLog2e * scale;
 #pragma unroll
-    for (int j = 0; j < 32; ++j) x[j] = tanh_of(x[j] * s);
+    for (int j = 0; j < N; ++j) x[j] = tanh_of(x[j] * s);
     return;
   }
   const Pair s(scale, scale);
 #pragma unroll
-  for (int j = 0; j < 32; j += 2) {
+  for (int j = 0; j < N; j += 2) {
     const Pair y = mul2(Pair(x[j], x[j + 1]), s), z = mul2(y, y);
-    Pair p = fma2(z, Pair(-0.0028394637629389763f, -0.0028394637629389763f), Pair(0.01611417718231678f, 0.01611417718231678f));
-    p = fma2(p, z, Pair(-0.05097286030650139f, -0.05097286030650139f));
-    p = fma2(p, z, Pair(0.13253524899482727f, 0.13253524899482727f));
-    p = fma2(p, z, Pair(-0.3332400321960449f, -0.3332400321960449f));
-    p = fma2(p, z, Pair(0.9999968409538269f, 0.9999968409538269f));
-    mul2(p, y).get(x[j], x[j + 1]);
+    Pair p = fma2(z, Pair(0.0010059071937575936f, 0.0010059071937575936f), Pair(-0.00609551602974534f, -0.00609551602974534f));
+    p = fma2(p, z, Pair(0.020165905356407166f, 0.020165905356407166f));
+    p = fma2(p, z, Pair(-0.053391970694065094f, -0.053391970694065094f));
+    p = fma2(p, z, Pair(0.13323739171028137f, 0.13323739171028137f));
+    p = fma2(p, z, Pair(-0.3333275318145752f, -0.3333275318145752f));
+    fma2(mul2(y, z), p, y).get(x[j], x[j + 1]);
   }
 }
 
@@ -449,7 +451,7 @@ attn_forward_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant__
     // ---------------------------------------------------------------- softmax: a thread a row
     const unsigned int mine = tmem + g * 128 + ((warp & 3u) << 21), mine_o = acc_o + g * DP + ((warp & 3u) << 21);
     const float c = CAP ? a.cap * kLog2e : a.scale * kLog2e;
-    const float to_tanh = CAP ? a.scale / a.cap : 0.f;
+    const float to_tanh = CAP ? a.over : 0.f;
     const float slope2 = BIAS ? a.slopes[h] * kLog2e : 0.f;
     const AttnSpan mine_span = NQ == 2 && g == 1u ? span[NQ - 1] : span[0];
     float m = -INFINITY, l = 0.f;      // m: in log 2 units without bias or cap scaled by c, see `unit`

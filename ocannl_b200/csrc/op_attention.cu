@@ -137,9 +137,7 @@ __global__ void __launch_bounds__(256) attn_copy_rows(const unsigned short* src,
   }
 }
 
-typedef void (*KeysKernel)(const b200_tmap, const b200_tmap, const b200_tmap, const b200_tmap, const b200_tmap, const b200_tmap, const AttnArgs);
-typedef void (*QueriesKernel)(const b200_tmap, const b200_tmap, const b200_tmap, const b200_tmap, const b200_tmap, const AttnArgs);
-
+typedef void (*GradKernel)(const GradMaps, const AttnArgs, unsigned int);
 typedef void (*SingleKernel)(const AttnArgs, int, int);
 typedef void (*FewKernel)(const AttnArgs, const FewArgs);
 
@@ -149,23 +147,24 @@ FewKernel few_of(bool cap, bool bias) {
   return bias ? attn_forward_few<T, DP, false, true> : attn_forward_few<T, DP, false, false>;
 }
 template <class T, int DP, int CW>
-KeysKernel keys_of(bool cap, bool bias) {
-  if (cap) return bias ? attn_grad_keys_tc<T, DP, CW, true, true> : attn_grad_keys_tc<T, DP, CW, true, false>;
-  return bias ? attn_grad_keys_tc<T, DP, CW, false, true> : attn_grad_keys_tc<T, DP, CW, false, false>;
-}
-template <class T, int DP, int CW>
-QueriesKernel queries_of(bool cap, bool bias) {
-  if (cap) return bias ? attn_grad_queries_tc<T, DP, CW, true, true> : attn_grad_queries_tc<T, DP, CW, true, false>;
-  return bias ? attn_grad_queries_tc<T, DP, CW, false, true> : attn_grad_queries_tc<T, DP, CW, false, false>;
+GradKernel grad_of(bool cap, bool bias) {
+  if (cap) return bias ? attn_grad_tc<T, DP, CW, true, true> : attn_grad_tc<T, DP, CW, true, false>;
+  return bias ? attn_grad_tc<T, DP, CW, false, true> : attn_grad_tc<T, DP, CW, false, false>;
 }
 
 typedef void (*AttnKernel)(const AttnArgs);
 typedef void (*ForwardKernel)(const b200_tmap, const b200_tmap, const b200_tmap, const b200_tmap, const AttnArgs);
 
+// (two query tiles: key tiles of 64 where scores are capped, of 128 else)
 template <class T, int DP, int NQ, int KW>
 ForwardKernel forward_of(bool cap, bool bias) {
-  if (cap) return bias ? attn_forward_tc<T, DP, NQ, KW, true, true> : attn_forward_tc<T, DP, NQ, KW, true, false>;
-  return bias ? attn_forward_tc<T, DP, NQ, KW, false, true> : attn_forward_tc<T, DP, NQ, KW, false, false>;
+  if constexpr (NQ == 2) {
+    constexpr bool kCap = KW == 64;
+    return bias ? attn_forward_tc<T, DP, NQ, KW, kCap, true> : attn_forward_tc<T, DP, NQ, KW, kCap, false>;
+  } else {
+    if (cap) return bias ? attn_forward_tc<T, DP, NQ, KW, true, true> : attn_forward_tc<T, DP, NQ, KW, true, false>;
+    return bias ? attn_forward_tc<T, DP, NQ, KW, false, true> : attn_forward_tc<T, DP, NQ, KW, false, false>;
+  }
 }
 
 // [batch, length, heads, d] in boxes of `box_rows` positions x 64 elements of a head, swizzled as the tensor cores read them
@@ -202,17 +201,17 @@ struct AttnOperator : b200_operator {
   // tensor-core form
   bool tc = false;
   ForwardKernel forward = nullptr;
-  KeysKernel keys = nullptr;
-  QueriesKernel queries = nullptr;
+  GradKernel gradients = nullptr;
+  GradMaps maps;
   SingleKernel single[2] = {nullptr, nullptr};      // forward, or the gradients' two
   size_t single_smem[2] = {0, 0};
   int single_places[2] = {1, 1};
   int vec = 0;
   FewKernel few = nullptr;
   FewArgs few_args = {};
-  b200_tmap map_q, map_k, map_v, map_o, map_do, map_dq, map_dk, map_dv, own_q, own_k, own_v, own_do;
+  b200_tmap map_q, map_k, map_v, map_o;
   unsigned int threads = 0, grid = 0, keys_grid = 0;
-  size_t smem = 0, keys_smem = 0;
+  size_t smem = 0;
   // padded copies: what is copied before and after the kernels
   struct Copy {
     const void* src;
@@ -370,9 +369,9 @@ struct AttnOperator : b200_operator {
   void choose_tc() {
     // results leave 32 rows at a time
     if (grad) {
-      map_dq = of_queries(a.dq, 32);
-      map_dk = of_keys(a.dk, 32);
-      map_dv = of_keys(a.dv, 32);
+      maps.dq = of_queries(a.dq, 32);
+      maps.dk = of_keys(a.dk, 32);
+      maps.dv = of_keys(a.dv, 32);
     } else {
       map_q = of_queries(a.q, 128);
       map_o = of_queries(a.out, 32);
@@ -400,14 +399,13 @@ struct AttnOperator : b200_operator {
       return 0;
     });
     grid = blocks_of(heads * ((a.S + 128 * (!grad && two ? 2 : 1) - 1) / (128 * (!grad && two ? 2 : 1))));
-    if (grad) keys_grid = blocks_of((long long)a.B * a.HK * ((a.T + 127) / 128));
-    if (std::max(smem, keys_smem) > 227 * 1024) throw Error(B200_E_UNSUPPORTED, "attention: too many keys or queries");
     if (grad) {
-      ready(keys, keys_smem);
-      ready(queries, smem);
-    } else {
-      ready(forward, smem);
+      keys_grid = blocks_of((long long)a.B * a.HK * ((a.T + 127) / 128));
+      grid = blocks_of((long long)grid + keys_grid);
     }
+    if (smem > 227 * 1024) throw Error(B200_E_UNSUPPORTED, "attention: too many keys or queries");
+    if (grad) ready(gradients, smem);
+    else ready(forward, smem);
   }
   template <class T, int DP, int NQ, int KW>
   void set() {
@@ -420,20 +418,17 @@ struct AttnOperator : b200_operator {
   template <class T, int DP, int CW>
   void set_grad() {
     typedef BwdShape<DP, CW> Sh;
-    keys = keys_of<T, DP, CW>(a.cap > 0.f, a.slopes != nullptr);
-    queries = queries_of<T, DP, CW>(a.cap > 0.f, a.slopes != nullptr);
+    gradients = grad_of<T, DP, CW>(a.cap > 0.f, a.slopes != nullptr);
     threads = Sh::kThreads;
-    smem = Sh::smem((a.T + CW - 1) / CW);
-    keys_smem = Sh::smem((a.S + CW - 1) / CW);
-    // a CTA's own rows and the others' tiles, for either kernel
-    own_q = of_queries(a.q, 128);
-    own_do = of_queries(a.d_out, 128);
-    own_k = of_keys(a.k, 128);
-    own_v = of_keys(a.v, 128);
-    map_q = of_queries(a.q, CW);
-    map_do = of_queries(a.d_out, CW);
-    map_k = of_keys(a.k, CW);
-    map_v = of_keys(a.v, CW);
+    smem = Sh::smem((std::max(a.S, a.T) + CW - 1) / CW);
+    maps.own_q = of_queries(a.q, 128);
+    maps.own_d_out = of_queries(a.d_out, 128);
+    maps.own_k = of_keys(a.k, 128);
+    maps.own_v = of_keys(a.v, 128);
+    maps.q = of_queries(a.q, CW);
+    maps.d_out = of_queries(a.d_out, CW);
+    maps.k = of_keys(a.k, CW);
+    maps.v = of_keys(a.v, CW);
   }
   b200_tmap of_queries(const void* p, int rows) const { return head_map(p, dtype, a.B, a.S, a.H, a.D, a.ld, rows); }
   b200_tmap of_keys(const void* p, int rows) const { return head_map(p, dtype, a.B, a.T, a.HK, a.D, a.ld, rows); }
@@ -447,8 +442,7 @@ struct AttnOperator : b200_operator {
     copy(before, s);
     if (grad && rows) launch(statistics, statistics_grid, 256, 0, s, a, by_heads, by_padded);
     if (tc && grad) {
-      launch(keys, keys_grid, threads, keys_smem, s, map_q, own_k, own_v, map_do, map_dk, map_dv, a);
-      launch(queries, grid, threads, smem, s, own_q, map_k, map_v, own_do, map_dq, a);
+      launch(gradients, grid, threads, smem, s, maps, a, keys_grid);
     } else if (few) {
       launch(few, dim3(grid, (unsigned int)few_args.splits), kFewWarps * 32, smem, s, a, few_args);
     } else if (tc) {

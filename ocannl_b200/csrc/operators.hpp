@@ -97,6 +97,9 @@ inline void rt_check(cudaError_t e, const char* what) {
   if (e != cudaSuccess) throw Error((int)e, std::string(what) + ": " + cudaGetErrorString(e));
 }
 
+// launches of operators on this thread, for the device's count (api.cpp)
+inline thread_local long long operator_launches = 0;
+
 // Programmatic stream serialisation, as every launch of the library: the kernels release their dependents at entry and wait
 // for the grids ahead before they touch memory.
 template <class... P, class... A>
@@ -112,6 +115,7 @@ void launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   rt_check(cudaLaunchKernelEx(&cfg, kernel, P(args)...), "operator launch");
+  ++operator_launches;
 }
 
 // Loads a kernel's code now (nothing is loaded inside a run, which may be under capture) and allows it its shared memory.
