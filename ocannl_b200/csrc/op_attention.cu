@@ -138,7 +138,8 @@ __global__ void __launch_bounds__(256) attn_copy_rows(const unsigned short* src,
 }
 
 typedef void (*GradKernel)(const GradMaps, const AttnArgs, unsigned int);
-typedef void (*SingleKernel)(const AttnArgs, int, int);
+typedef void (*SingleKernel)(const AttnArgs, int, int, int);
+typedef void (*SingleGradKernel)(const AttnArgs, int, int, int, unsigned int);
 typedef void (*FewKernel)(const AttnArgs, const FewArgs);
 
 template <class T, int DP>
@@ -203,10 +204,9 @@ struct AttnOperator : b200_operator {
   ForwardKernel forward = nullptr;
   GradKernel gradients = nullptr;
   GradMaps maps;
-  SingleKernel single[2] = {nullptr, nullptr};      // forward, or the gradients' two
-  size_t single_smem[2] = {0, 0};
-  int single_places[2] = {1, 1};
-  int vec = 0;
+  SingleKernel single = nullptr;
+  SingleGradKernel single_grad = nullptr;
+  int vec = 0, places = 1, groups = 4;
   FewKernel few = nullptr;
   FewArgs few_args = {};
   b200_tmap map_q, map_k, map_v, map_o;
@@ -334,33 +334,25 @@ struct AttnOperator : b200_operator {
   void choose_single() {
     vec = a.D % 4 == 0;
     for (const void* p : {a.q, a.k, a.v, a.d_out}) vec &= ((size_t)p & 15) == 0;
-    // Blocks of 32 rows where 64 leave the machine few of them: more, and more even, shares.  Heads of up to 64 elements run two such
-    // blocks an SM and gain up to four blocks of 64 rows an SM (2 x 1024 positions, 8 heads of 64, gradients 437 -> 370 us), wider ones one
-    // block either way (heads of 128: 572 -> 795).
-    const bool wide = a.D > 64;
-    auto of_rows = [&](long long heads, long long n) {
-      const bool small = heads * ((n + 63) / 64) < (wide ? 1ll : 4ll) * dev->sm_count;
-      return std::make_pair(small ? 2 : 4, blocks_of(heads * ((n + (small ? 31 : 63)) / (small ? 32 : 64))));
-    };
-    const auto by_query = of_rows((long long)a.B * a.H, a.S), by_key = of_rows((long long)a.B * a.HK, a.T);
-    const int rq = by_query.first, rk = by_key.first;
-    grid = by_query.second;
-    keys_grid = by_key.second;
-    auto room = [&](int i, int r, int own, int weights) {
-      single_places[i] = SingleShape::smem(a.D, r, own, weights, 2) <= (size_t)(r == 2 && !wide ? 113 : 227) * 1024 ? 2 : 1;
-      single_smem[i] = SingleShape::smem(a.D, r, own, weights, single_places[i]);
-    };
+    // Blocks of 64 rows, two warps for 16 of them; where that leaves SMs without a block, of 16 rows and four warps (below that they read
+    // the others four times as often for nothing: gradients of 2 x 1024 positions, 8 heads of 64, 220 us and 309).
+    const long long blocks64 = (long long)a.B * (a.H * ((a.S + 63ll) / 64) + (grad ? a.HK * ((a.T + 63ll) / 64) : 0));
+    groups = blocks64 < dev->sm_count ? 1 : 4;
+    const int shares = groups == 1 ? 4 : 2, rows_each = 16 * groups, own = grad ? 2 : 1;
+    threads = (unsigned int)(32 * groups * shares);
+    keys_grid = grad ? blocks_of((long long)a.B * a.HK * ((a.T + rows_each - 1) / rows_each)) : 0;
+    grid = blocks_of((long long)a.B * a.H * ((a.S + rows_each - 1) / rows_each) + keys_grid);
+    // two places where that leaves heads of up to 64 elements two blocks an SM, and wider ones, which have one, room at all
+    places = SingleShape::smem(a.D, groups, shares, own, 2) <= (size_t)(a.D <= 64 ? 113 : 227) * 1024 ? 2 : 1;
+    smem = SingleShape::smem(a.D, groups, shares, own, places);
+    if (!SingleShape::room_to_meet(a.D, groups, shares, own, places, a.D <= 64 ? 8 : 16)) throw Error(B200_E_UNSUPPORTED, "attention: internal error: no room to meet");
     if (grad) {
-      single[0] = rk == 2 ? (wide ? attn_grad_keys_single<2, 2> : attn_grad_keys_single<1, 2>) : (wide ? attn_grad_keys_single<2, 4> : attn_grad_keys_single<1, 4>);
-      single[1] = rq == 2 ? (wide ? attn_grad_queries_single<2, 2> : attn_grad_queries_single<1, 2>) : (wide ? attn_grad_queries_single<2, 4> : attn_grad_queries_single<1, 4>);
-      room(0, rk, 2, 2);
-      room(1, rq, 2, 1);
+      single_grad = a.D <= 64 ? attn_grad_single<8> : attn_grad_single<16>;
+      ready(single_grad, smem);
     } else {
-      single[0] = rq == 2 ? (wide ? attn_forward_single<2, 2> : attn_forward_single<1, 2>) : (wide ? attn_forward_single<2, 4> : attn_forward_single<1, 4>);
-      room(0, rq, 1, 1);
+      single = a.D <= 64 ? attn_forward_single<8> : attn_forward_single<16>;
+      ready(single, smem);
     }
-    for (int i = 0; i < 2; ++i)
-      if (single[i]) ready(single[i], single_smem[i]);
   }
   unsigned int blocks_of(long long n) const {
     if (n >> 31) throw Error(B200_E_UNSUPPORTED, "attention: too many rows");
@@ -447,9 +439,10 @@ struct AttnOperator : b200_operator {
       launch(few, dim3(grid, (unsigned int)few_args.splits), kFewWarps * 32, smem, s, a, few_args);
     } else if (tc) {
       launch(forward, grid, threads, smem, s, map_q, map_k, map_v, map_o, a);
-    } else if (single[0]) {
-      launch(single[0], grad ? keys_grid : grid, 256, single_smem[0], s, a, vec, single_places[0]);
-      if (grad) launch(single[1], grid, 256, single_smem[1], s, a, vec, single_places[1]);
+    } else if (single) {
+      launch(single, grid, threads, smem, s, a, vec, places, groups);
+    } else if (single_grad) {
+      launch(single_grad, grid, threads, smem, s, a, vec, places, groups, keys_grid);
     } else if (grad) {
       if (rows) launch(kernel(1), blocks(rows), 256, 0, s, a);
       if (key_rows) launch(kernel(2), blocks(key_rows), 256, 0, s, a);

@@ -9,8 +9,8 @@
 // registers, at most 16 elements a thread, so that the squares of the distances from the mean are summed in a second pass over
 // registers (no difference of large sums).  The groups stride over the rows, the next row's loads under way while one is worked
 // on; the scale and the shift stay in shared memory.  In the gradient a thread keeps its sums over the rows of its columns in
-// registers; they meet in shared memory once per block and then in a second kernel that adds the blocks' partial sums in their order: the same bits every time.  Rows of more than 8192 elements
-// are read again for each pass, by 1024 threads (they come from L2 then), their column sums by a kernel of its own.
+// registers; they meet in shared memory once per block and then in a second kernel that adds the blocks' partial sums in their order: the same bits every time.  Longer rows (forward: of more than
+// 16384 elements) are read again for each pass, by 1024 threads (they come from L2 then), their column sums kept in shared memory.
 #include "kernels/op_common.cuh"
 #include "operators.hpp"
 
@@ -25,6 +25,7 @@ struct NormArgs {
   float *partial;                  // gradient: [2][blocks][n]
   unsigned long long rows;
   unsigned int n;
+  int own_columns;                 // wide gradient: the column sums are made along with dx
   int weight_f32;                  // gamma and beta in single precision, or in the rows' type
   float eps, inv_n;
 };
@@ -303,10 +304,16 @@ __global__ void __launch_bounds__(1024) norm_wide(const NormArgs a) {
   }
 }
 
+// `own_columns`: the block's column sums lie in shared memory, where a thread adds to those of its elements alone
 template <class T, int VEC>
 __global__ void __launch_bounds__(1024) norm_grad_wide(const NormArgs a) {
   __shared__ float sh[2 * 2 * 32];
+  extern __shared__ __align__(16) float columns[];
   grid_begin();
+  if (a.own_columns)
+    for (unsigned int e = threadIdx.x * VEC; e < a.n; e += 1024 * VEC)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) columns[e + i] = columns[a.n + e + i] = 0.f;
   int half = 0;
   for (unsigned long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const unsigned long long at = row * a.n;
@@ -335,12 +342,23 @@ __global__ void __launch_bounds__(1024) norm_grad_wide(const NormArgs a) {
       if (a.dh) Vec<T, VEC>::load((const T*)a.dh + at + e, d);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        const float g = w[i] * weight_at<T>(a.gamma, a.weight_f32, e + i, 1.f);
-        v[i] = fmaf(rstd, g - m0 - (v[i] - mean) * rstd * m1, d[i]);
+        const float g = w[i] * weight_at<T>(a.gamma, a.weight_f32, e + i, 1.f), u = (v[i] - mean) * rstd;
+        if (a.own_columns) {
+          columns[e + i] = fmaf(w[i], u, columns[e + i]);
+          columns[a.n + e + i] += w[i];
+        }
+        v[i] = fmaf(rstd, g - m0 - u * m1, d[i]);
       }
       Vec<T, VEC>::store((T*)a.dx + at + e, v);
     }
   }
+  if (a.own_columns && a.partial)
+    for (unsigned int e = threadIdx.x * VEC; e < a.n; e += 1024 * VEC)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        a.partial[(unsigned long long)blockIdx.x * a.n + e + i] = columns[e + i];
+        a.partial[((unsigned long long)gridDim.x + blockIdx.x) * a.n + e + i] = columns[a.n + e + i];
+      }
 }
 
 // column sums of wide rows: a thread per column, a slice of the rows per block; partial sums as above
@@ -407,6 +425,8 @@ NormPlan rows_of(bool grad, unsigned int n) {
 template <class T>
 NormPlan plan_of(bool grad, unsigned int n, bool vec) {
   constexpr int V = 16 / (int)sizeof(T);
+  // (forward rows of up to 16384 elements still fit the registers of 1024 threads)
+  if (!grad && vec && n > 8192 && n <= 16384) return {norm_rows<T, V, 16 / V, 1024>, 1024, 1024, 16};
   if (n > 8192) {
     if (vec) return {grad ? norm_grad_wide<T, V> : norm_wide<T, V>, 1024, 1024, 0};
     return {grad ? norm_grad_wide<T, 1> : norm_wide<T, 1>, 1024, 1024, 0};
@@ -432,9 +452,14 @@ struct NormOperator : b200_operator {
     for (const void* p : {a.x, a.r, a.dy, a.dh, (const void*)a.y, (const void*)a.h, (const void*)a.dx}) vec &= ((size_t)p & 15) == 0;
     plan = dtype == B200_F32 ? plan_of<float>(grad, a.n, vec) : dtype == B200_BF16 ? plan_of<__nv_bfloat16>(grad, a.n, vec) : plan_of<__half>(grad, a.n, vec);
     const unsigned int per_block = plan.block / plan.tpr;
-    const bool wide = plan.tpr == 1024;
+    const bool wide = plan.elements == 0;
     smem = wide ? 0 : (size_t)plan.tpr * plan.elements * 4 * (grad ? 1 : 2);
     if (grad && per_block > 1 && !wide) smem = std::max(smem, 2 * (size_t)per_block * a.n * 4);
+    // (up to 28000 elements; wider rows' column sums take a pass of their own)
+    if (wide && grad && (dgamma || dbeta) && (size_t)a.n * 8 <= 224 * 1024) {
+      a.own_columns = 1;
+      smem = (size_t)a.n * 8;
+    }
     ready(plan.kernel, smem);
     int resident = 0;
     rt_check(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, plan.kernel, (int)plan.block, smem), "occupancy");
@@ -443,7 +468,7 @@ struct NormOperator : b200_operator {
     if (grad && (dgamma || dbeta)) {
       ready(norm_grad_join);
       unsigned int partials = grid;
-      if (wide) {
+      if (wide && !a.own_columns) {
         // enough blocks for the machine, at least 32 rows each
         const unsigned int across = (a.n + 255) / 256;
         slices = (unsigned int)std::max<unsigned long long>(1, std::min<unsigned long long>(a.rows / 32, (8u * dev->sm_count + across - 1) / across));
@@ -461,7 +486,7 @@ struct NormOperator : b200_operator {
     if (grid) launch(plan.kernel, grid, plan.block, smem, s, a);
     if (!a.partial) return;
     unsigned int partials = grid;
-    if (plan.tpr == 1024 && a.rows) {
+    if (slices && a.rows) {
       const dim3 g((a.n + 255) / 256, slices);
       if (dtype == B200_F32) launch(norm_grad_columns<float>, g, 256, 0, s, a, slices);
       else if (dtype == B200_BF16) launch(norm_grad_columns<__nv_bfloat16>, g, 256, 0, s, a, slices);

@@ -123,7 +123,8 @@ template <class K>
 void ready(K kernel, size_t smem = 0) {
   cudaFuncAttributes a;
   rt_check(cudaFuncGetAttributes(&a, kernel), "cudaFuncGetAttributes");
-  if (smem) rt_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "cudaFuncSetAttribute");
+  // (never lowered: operators that were linked before may need more)
+  if ((int)smem > a.maxDynamicSharedSizeBytes) rt_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "cudaFuncSetAttribute");
 }
 
 // The body of a link entry point: `make` fills a new operator of class Op; nothing crosses the C boundary.

@@ -357,6 +357,32 @@ def test_weights_of_16_bits_in_the_norm(device):
     nodes.free()
 
 
+def test_operators_of_one_kernel_and_different_sizes(device):
+    """A later link of a smaller problem takes nothing from an earlier one of a larger, and the other way round."""
+    sizes = ((3, 8192), (3, 5000), (2, 8192))
+    made = []
+    for rows, n in sizes:
+        x, _, gamma, beta, _ = norm_case(rows, n, "single", n, False)
+        nodes = R.Nodes(device, dict(x=("single", (rows, n), x), g=("single", (n,), gamma), b=("single", (n,), beta), y=("single", (rows, n), None)))
+        made.append((nodes, nodes.context.layer_norm("x", "y", gamma="g", beta="b"), R.layer_norm(x, gamma, beta)[0]))
+    cases = [(1, 70, 70, 2, 2, 64, "causal", True, None, 0.0, False), (1, 20, 20000, 2, 2, 64, "causal", True, None, 0.0, False), ATTENTION[13]]
+    attn = []
+    for case in cases:
+        x, t, more, sl, seen, pos, scale = attention_case(case, "bfloat16")
+        out, _, size, flat = R.attention(x["q"], x["k"], x["v"], seen, pos, scale)
+        attn.append(link_attention(device, case, "bfloat16", {m: x[m] for m in "qkv"}, t, more, sl, "aligned") + (out, out_bound("bfloat16", out, size, flat)))
+    for nodes, op, y in made + made[::-1]:
+        op.run()
+        R.within(nodes.read("y"), y, 2.0 ** -16 * (1 + np.abs(y)), "y")
+    for nodes, op, out, bound in attn + attn[::-1]:
+        op.run()
+        device.await_()
+        R.within(nodes.read("out"), out, bound, "out")
+    for x in made + attn:
+        x[1].free()
+        x[0].free()
+
+
 def test_memory_around_the_outputs_is_left_alone(device):
     """Outputs between other nodes, aligned to their elements alone: what lies before and behind them keeps its values."""
     for prec in PRECS:
