@@ -40,29 +40,6 @@ __device__ __forceinline__ float rcp(float x) {
 // tanh x = 1 - 2 / (e^2x + 1), of which 2 x log2(e) is given; off by a few 2^-24 (absolute), which a cap multiplies
 __device__ __forceinline__ float tanh_of(float two_x_log2e) { return fmaf(-2.f, rcp(ex2(two_x_log2e) + 1.f), 1.f); }
 
-// Pairs of single-precision values in one instruction (the multiply-add pipe takes both in the issue slot of one).
-struct Pair {
-  unsigned long long v;
-  __device__ __forceinline__ Pair() {}
-  __device__ __forceinline__ Pair(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
-  __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-};
-__device__ __forceinline__ Pair fma2(const Pair& a, const Pair& b, const Pair& c) {
-  Pair r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return r;
-}
-__device__ __forceinline__ Pair mul2(const Pair& a, const Pair& b) {
-  Pair r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ Pair add2(const Pair& a, const Pair& b) {
-  Pair r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-
 // x = tanh(x scale) of N scores of each lane.  The exponential and the reciprocal of tanh_of pass through the unit that also has to make
 // the weights, at an eighth of the multiply-adds' rate, and would bound the kernel: where all of a warp's scores are at most the cap in
 // size, tanh y = y + y^3 Q(y^2) instead, with Q the polynomial of degree 5 whose largest error on [0, 1] is least (2.6e-8, 8e-8 in single

@@ -152,9 +152,12 @@ __global__ void __launch_bounds__(512, 1) norm_grad_rows(const NormArgs a) {
   const unsigned int t = threadIdx.x % TPR, sub = threadIdx.x / TPR, per_block = blockDim.x / TPR;
   constexpr unsigned int kSpan = TPR * E;
   for (unsigned int e = threadIdx.x; e < kSpan; e += blockDim.x) weights[e] = e < a.n ? weight_at<T>(a.gamma, a.weight_f32, e, 1.f) : 0.f;
-  float dg[E], db[E];
+  [[maybe_unused]] float dg[E], db[E];
+  [[maybe_unused]] Pair dg2[E / 2 + 1], db2[E / 2 + 1];
 #pragma unroll
   for (int i = 0; i < E; ++i) dg[i] = db[i] = 0.f;
+#pragma unroll
+  for (int i = 0; i < E / 2; ++i) dg2[i] = db2[i] = Pair(0.f, 0.f);
   // the next row is on its way while this one is worked on; a row's values are taken from its bits twice, before and after the sums
   struct Row {
     Raw<T, VEC> x[NV], dy[NV], dh[NV];
@@ -187,22 +190,45 @@ __global__ void __launch_bounds__(512, 1) norm_grad_rows(const NormArgs a) {
     now = next;
     fetch(row + step);
     float s[2] = {0.f, 0.f};
+    // (behind the row's end dy and gamma are zero)
+    if constexpr (VEC == 1) {
 #pragma unroll
-    for (int c = 0; c < NV; ++c) {
-      float u[VEC], dy[VEC];
-      now.x[c].values(u);
-      now.dy[c].values(dy);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const int k = c * VEC + i;
-        // (behind the row's end dy and gamma are zero)
-        u[i] = (u[i] - now.mean) * now.rstd;
-        const float g = dy[i] * weights[(c * TPR + t) * VEC + i];
+      for (int c = 0; c < NV; ++c) {
+        float u, dy;
+        now.x[c].values(&u);
+        now.dy[c].values(&dy);
+        u = (u - now.mean) * now.rstd;
+        const float g = dy * weights[c * TPR + t];
         s[0] += g;
-        s[1] = fmaf(g, u[i], s[1]);
-        dg[k] = fmaf(dy[i], u[i], dg[k]);
-        db[k] += dy[i];
+        s[1] = fmaf(g, u, s[1]);
+        dg[c] = fmaf(dy, u, dg[c]);
+        db[c] += dy;
       }
+    } else {
+      // two elements to an instruction: a third of the kernel's time was the issue of its arithmetic
+      const Pair shift(-now.mean, -now.mean), rstd2(now.rstd, now.rstd);
+      Pair s0(0.f, 0.f), s1(0.f, 0.f);
+#pragma unroll
+      for (int c = 0; c < NV; ++c) {
+        float x[VEC], dy[VEC];
+        now.x[c].values(x);
+        now.dy[c].values(dy);
+#pragma unroll
+        for (int i = 0; i < VEC; i += 2) {
+          const int k = (c * VEC + i) / 2;
+          const float2 w = *(const float2*)(weights + (c * TPR + t) * VEC + i);
+          const Pair d(dy[i], dy[i + 1]), u = mul2(add2(Pair(x[i], x[i + 1]), shift), rstd2), g = mul2(d, Pair(w.x, w.y));
+          s0 = add2(s0, g);
+          s1 = fma2(g, u, s1);
+          dg2[k] = fma2(d, u, dg2[k]);
+          db2[k] = add2(db2[k], d);
+        }
+      }
+      float even, odd;
+      s0.get(even, odd);
+      s[0] = even + odd;
+      s1.get(even, odd);
+      s[1] = even + odd;
     }
     row_sum<TPR>(s, sh, half);
     half ^= 1;
@@ -216,12 +242,28 @@ __global__ void __launch_bounds__(512, 1) norm_grad_rows(const NormArgs a) {
       now.x[c].values(v);
       now.dy[c].values(dy);
       now.dh[c].values(w);
+      if constexpr (VEC == 1) {
+        v[0] = fmaf(now.rstd, dy[0] * weights[e] - m0 - (v[0] - now.mean) * now.rstd * m1, w[0]);
+      } else {
+        const Pair shift(-now.mean, -now.mean), rstd2(now.rstd, now.rstd), less0(-m0, -m0), less1(-m1, -m1);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) v[i] = fmaf(now.rstd, dy[i] * weights[e + i] - m0 - (v[i] - now.mean) * now.rstd * m1, w[i]);
+        for (int i = 0; i < VEC; i += 2) {
+          const float2 ga = *(const float2*)(weights + e + i);
+          const Pair u = mul2(add2(Pair(v[i], v[i + 1]), shift), rstd2), g = fma2(Pair(dy[i], dy[i + 1]), Pair(ga.x, ga.y), less0);
+          fma2(rstd2, fma2(u, less1, g), Pair(w[i], w[i + 1])).get(v[i], v[i + 1]);
+        }
+      }
       Vec<T, VEC>::store((T*)a.dx + row * a.n + e, v);
     }
   }
   if (!a.partial) return;
+  if constexpr (VEC > 1) {
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i) {
+      dg2[i].get(dg[2 * i], dg[2 * i + 1]);
+      db2[i].get(db[2 * i], db[2 * i + 1]);
+    }
+  }
   // the block's groups of threads meet: columns[which][group][column]
   const unsigned int plane = per_block * a.n;
   if (per_block > 1) {
@@ -431,8 +473,12 @@ NormPlan plan_of(bool grad, unsigned int n, bool vec) {
     if (vec) return {grad ? norm_grad_wide<T, V> : norm_wide<T, V>, 1024, 1024, 0};
     return {grad ? norm_grad_wide<T, 1> : norm_wide<T, 1>, 1024, 1024, 0};
   }
-  // (single elements: 16 of them a thread, twice for the next row, would not fit its registers)
-  if (!vec) return n <= 4096 ? rows_of<T, 1, 8>(grad, n) : rows_of<T, 1, 16>(grad, n);
+  // 16 single elements a thread, or the gradient's 16 of single precision, twice for the next row, would not fit its registers (1999
+  // rows of 777 single elements: 19.5 us, 8.8 with 8 of them); between 4096 and 8192 they have to.
+  constexpr unsigned int kMost = 512;
+  if (!vec) return n <= kMost * 8 ? rows_of<T, 1, 8>(grad, n) : NormPlan{grad ? norm_grad_rows<T, 1, 16, kMost> : norm_rows<T, 1, 16, kMost>, kMost, kMost, 16};
+  if (sizeof(T) == 4 && grad)
+    return n <= kMost * 8 ? NormPlan(rows_of<T, V, 8 / V>(true, n)) : NormPlan{norm_grad_rows<T, V, 16 / V, kMost>, kMost, kMost, 16};
   const unsigned int g = n <= 128 ? 8 : n <= 512 ? 32 : n <= 2048 ? 128 : 512;
   return n <= g * 8 ? rows_of<T, V, 8 / V>(grad, n) : rows_of<T, V, 16 / V>(grad, n);
 }
