@@ -24,39 +24,37 @@ __global__ void __launch_bounds__(256) attn_forward_rows(const __grid_constant__
     attn_forward_row<T>(a, (int)(bs / a.S), (int)(i - bs * a.H), (int)(bs % a.S), lane);
   }
 }
-// What the gradients need of every row: its lse and <d_out, out>, tile by tile of 128 queries, G threads a row.  Bound by memory: out and
-// d_out are read once, kRowsAtOnce rows of a thread under way together.  Rows behind the last one and rows that see nothing get
-// weights of zero.
+// What the gradients need of every row: its lse and <d_out, out>, tile by tile of 128 queries, G threads a row.  out and d_out are read
+// once, kRowsAtOnce rows of a thread under way together; what bounds it is the arithmetic of indices around 32 bytes a lane, so that
+// is kept to 32 bits (64 x 256 positions, 8 heads of 64: 14.4 us with more of it).  Rows that see nothing get weights of zero; the places
+// behind the last row are filled at link.
 constexpr int kRowsAtOnce = 4;
 
 template <class T, int VEC, int G>
-__global__ void __launch_bounds__(256) attn_statistics(const __grid_constant__ AttnArgs a, const Divisor by_heads, const Divisor by_padded) {
+__global__ void __launch_bounds__(256) attn_statistics(const __grid_constant__ AttnArgs a, const Divisor by_heads, const Divisor by_length) {
   __shared__ float sh[8];
   grid_begin();
-  constexpr int rows = 256 / G, chunks = VEC > 1 ? 1 : 128 / G;
+  constexpr unsigned int rows = 256 / G;
+  constexpr int chunks = VEC > 1 ? 1 : 128 / G;
   const int lane = (int)threadIdx.x % G;
-  const unsigned int padded = by_padded.d, n = (unsigned int)a.B * padded * (unsigned int)a.H, step = gridDim.x * rows * kRowsAtOnce;
+  const unsigned int heads = (unsigned int)a.H, length = (unsigned int)a.S, tiles = (length + 127) / 128;
+  const unsigned int n = (unsigned int)a.B * length * heads, step = gridDim.x * rows * kRowsAtOnce;
   float top = 0.f;
-  for (unsigned int base = blockIdx.x * rows * kRowsAtOnce; base < n; base += step) {
+  for (unsigned int base = blockIdx.x * rows * kRowsAtOnce + threadIdx.x / G; base - threadIdx.x / G < n; base += step) {
     Raw<T, VEC> x[kRowsAtOnce][chunks], y[kRowsAtOnce][chunks];
     float lse[kRowsAtOnce];
-    long long stat[kRowsAtOnce];
+    unsigned int stat[kRowsAtOnce];
 #pragma unroll
     for (int k = 0; k < kRowsAtOnce; ++k) {
-      const unsigned int i = base + k * rows + threadIdx.x / G;
+      const unsigned int i = base + k * rows;
       lse[k] = -INFINITY;
-      stat[k] = -1;
 #pragma unroll
       for (int c = 0; c < chunks; ++c) {
         x[k][c].clear();
         y[k][c].clear();
       }
       if (i >= n) continue;
-      const unsigned int bs = by_heads.of(i), h = i - bs * (unsigned int)a.H, b = by_padded.of(bs), r = bs - b * padded;
-      stat[k] = attn_stat_at(a, (int)b, (int)h, (int)r);
-      if (r >= (unsigned int)a.S) continue;
-      lse[k] = a.lse[((long long)b * a.H + h) * a.S + r];
-      const long long at = attn_q_at(a, (int)b, (int)r, (int)h);
+      const unsigned long long at = (unsigned long long)i * (unsigned int)a.ld;      // (the rows lie in this order)
 #pragma unroll
       for (int c = 0; c < chunks; ++c) {
         const int e = (c * G + lane) * VEC;
@@ -64,6 +62,9 @@ __global__ void __launch_bounds__(256) attn_statistics(const __grid_constant__ A
         x[k][c].load((const T*)a.o + at + e);
         y[k][c].load((const T*)a.d_out + at + e);
       }
+      const unsigned int bs = by_heads.of(i), h = i - bs * heads, b = by_length.of(bs), r = bs - b * length, bh = b * heads + h;
+      lse[k] = a.lse[bh * length + r];
+      stat[k] = (bh * tiles + (r >> 7)) * 256 + (r & 127);
     }
 #pragma unroll
     for (int k = 0; k < kRowsAtOnce; ++k) {
@@ -75,19 +76,19 @@ __global__ void __launch_bounds__(256) attn_statistics(const __grid_constant__ A
         y[k][c].values(w);
 #pragma unroll
         for (int q = 0; q < VEC; ++q) {
-          if (VEC > 1 && (c * G + lane) * VEC + q >= a.D) continue;      // (padded copies)
+          // (rows of padded copies end in zeros)
           delta = fmaf(u[q], w[q], delta);
-          square = fmaf(w[q], w[q], square);
+          if constexpr (std::is_same<T, __half>::value) square = fmaf(w[q], w[q], square);
         }
       }
 #pragma unroll
       for (int o = G / 2; o > 0; o >>= 1) {
         delta += __shfl_xor_sync(0xffffffffu, delta, o);
-        square += __shfl_xor_sync(0xffffffffu, square, o);
+        if constexpr (std::is_same<T, __half>::value) square += __shfl_xor_sync(0xffffffffu, square, o);
       }
       const bool empty = lse[k] == -INFINITY;
       if (!empty) top = fmaxf(top, square);
-      if (lane == 0 && stat[k] >= 0) {
+      if (lane == 0 && base + k * rows < n) {
         a.stat[stat[k]] = empty ? INFINITY : lse[k] * kLog2e;
         a.stat[stat[k] + 128] = empty ? 0.f : delta;
       }
@@ -198,7 +199,7 @@ struct AttnOperator : b200_operator {
   long long rows = 0, key_rows = 0;
   StatisticsKernel statistics = nullptr;
   unsigned int statistics_grid = 0;
-  Divisor by_heads, by_padded;
+  Divisor by_heads, by_length;
   // tensor-core form
   bool tc = false;
   ForwardKernel forward = nullptr;
@@ -262,7 +263,7 @@ struct AttnOperator : b200_operator {
       const long long padded = (long long)a.B * a.H * ((a.S + 127) / 128) * 128;
       const int size = (int)dtype_bytes(dtype);
       const bool vec = tc || (a.D * size % 16 == 0 && (((size_t)a.o | (size_t)a.d_out) & 15) == 0);
-      if (padded >> 31) throw Error(B200_E_UNSUPPORTED, "attention: too many rows");
+      if (padded >> 30) throw Error(B200_E_UNSUPPORTED, "attention: too many rows");
       int group = 32;
       statistics = by_type(dtype, [&](auto t) -> StatisticsKernel {
         typedef decltype(t) T;
@@ -273,15 +274,17 @@ struct AttnOperator : b200_operator {
       });
       ready(statistics);
       by_heads = Divisor((unsigned int)a.H);
-      by_padded = Divisor((unsigned int)((a.S + 127) / 128 * 128));
+      by_length = Divisor((unsigned int)a.S);
       const long long at_once = 256 / group * kRowsAtOnce;
-      statistics_grid = (unsigned int)std::min<long long>((padded + at_once - 1) / at_once, 8ll * dev->sm_count);
+      statistics_grid = (unsigned int)std::min<long long>((rows + at_once - 1) / at_once, 8ll * dev->sm_count);
       stat = reserve((size_t)padded * 8);
       if (dtype == B200_F16) norms = reserve((size_t)statistics_grid * 4);
     }
     take_workspace(reserved);
     if (grad && rows) {
       a.stat = (float*)(workspace + stat);
+      // the places behind a head's last row: a finite lse beyond all scores (3.4e38), so that what lies there weighs nothing
+      cu_check(cu().cuMemsetD8Async_(workspace + stat, 0x7f, (size_t)a.B * a.H * ((a.S + 127) / 128) * 1024, dev->stream), "cuMemsetD8Async(statistics)");
       if (dtype == B200_F16) {
         a.norms = (float*)(workspace + norms);
         a.n_norms = (int)statistics_grid;
@@ -432,7 +435,7 @@ struct AttnOperator : b200_operator {
   unsigned int blocks(long long n) const { return (unsigned int)std::min<long long>((n + 7) / 8, 16ll * dev->sm_count); }
   void run(cudaStream_t s) override {
     copy(before, s);
-    if (grad && rows) launch(statistics, statistics_grid, 256, 0, s, a, by_heads, by_padded);
+    if (grad && rows) launch(statistics, statistics_grid, 256, 0, s, a, by_heads, by_length);
     if (tc && grad) {
       launch(gradients, grid, threads, smem, s, maps, a, keys_grid);
     } else if (few) {
