@@ -137,25 +137,15 @@ __device__ __forceinline__ void attn_grad_keys(const b200_tmap& map_q, const b20
   const unsigned int warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
   constexpr unsigned int kLoad = Sh::kWarps - 2, kMma = Sh::kWarps - 1;
   // this CTA's keys: the first ones first, which under a causal mask are seen by the most queries
-  const unsigned int heads = (unsigned int)a.B * (unsigned int)a.HK;
-  const int j0 = (int)(block / heads) * 128;
-  const unsigned int bh = block % heads;
-  const int b = (int)(bh / (unsigned int)a.HK), hk = (int)(bh % (unsigned int)a.HK);
+  const unsigned int tile_of = a.all_key_heads.of(block), bh = block - tile_of * a.all_key_heads.d;
+  const int j0 = (int)tile_of * 128, b = (int)a.key_heads.of(bh), hk = (int)bh - b * a.HK;
   const int tiles = (a.S + CW - 1) / CW, stat_tiles = (a.S + 127) / 128;
   const bool docs = a.kdoc != nullptr;
-  if (threadIdx.x == kLoad * 32) {
-    b200_mbar_init(bar_kv, 1);
-    for (int i = 0; i < 2; ++i) {
-      b200_mbar_init(bar_full + 8 * i, 1);
-      b200_mbar_init(bar_empty + 8 * i, 1);
-    }
-    b200_mbar_init(bar_s, 1);
-    b200_mbar_init(bar_dp, 1);
-    b200_mbar_init(bar_p, Sh::kGroups * 128);
-    b200_mbar_init(bar_ds, Sh::kGroups * 128);
-    b200_mbar_init(bar_done, 1);
-    *abort_flag = 0u;
+  if (warp == kLoad) {
+    if (lane < 10) b200_mbar_init(bar0 + 8 * lane, lane == 7 || lane == 8 ? Sh::kGroups * 128 : 1);      // (bar_p, bar_ds)
+    if (lane == 10) *abort_flag = 0u;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    __syncwarp();
   }
   if (warp == kMma) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(b200_smem_addr((const void*)tmem_slot)), "r"(Sh::kColumns) : "memory");
@@ -484,27 +474,20 @@ __device__ __forceinline__ void attn_grad_queries(const b200_tmap& map_q, const 
   asm volatile("griddepcontrol.launch_dependents;");
   const unsigned int warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
   constexpr unsigned int kLoad = Sh::kWarps - 2, kMma = Sh::kWarps - 1;
-  const unsigned int heads = (unsigned int)a.B * (unsigned int)a.H;
-  const int tiles_q = (a.S + 127) / 128;
-  const int t_q = tiles_q - 1 - (int)(block / heads), r0 = t_q * 128;
-  const unsigned int bh = block % heads;
-  const int b = (int)(bh / (unsigned int)a.H), h = (int)(bh % (unsigned int)a.H), hk = h / a.group;
+  const unsigned int from_last = a.all_heads.of(block), bh = block - from_last * a.all_heads.d;
+  const int tiles_q = (a.S + 127) / 128, t_q = tiles_q - 1 - (int)from_last, r0 = t_q * 128;
+  const int b = (int)a.heads.of(bh), h = (int)bh - b * a.H, hk = (int)a.per_key_head.of((unsigned int)h);
   const bool docs = a.kdoc != nullptr;
-  if (threadIdx.x == kLoad * 32) {
-    b200_mbar_init(bar_q, 1);
-    for (int i = 0; i < 2; ++i) {
-      b200_mbar_init(bar_full + 8 * i, 1);
-      b200_mbar_init(bar_empty + 8 * i, 1);
-      b200_mbar_init(bar_s + 8 * i, 1);
+  if (warp == kLoad) {
+    if (lane < 10) b200_mbar_init(bar0 + 8 * lane, lane == 8 ? Sh::kGroups * 128 : 1);      // (bar_ds)
+    if (lane == 10) {
+      span->last_min = span->doc_min = 0x7fffffff;
+      span->last_max = -1;
+      span->doc_max = -0x7fffffff - 1;
+      *abort_flag = 0u;
     }
-    b200_mbar_init(bar_dp, 1);
-    b200_mbar_init(bar_ds, Sh::kGroups * 128);
-    b200_mbar_init(bar_done, 1);
-    span->last_min = span->doc_min = 0x7fffffff;
-    span->last_max = -1;
-    span->doc_max = -0x7fffffff - 1;
-    *abort_flag = 0u;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    __syncwarp();
   }
   if (warp == kMma) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(b200_smem_addr((const void*)tmem_slot)), "r"(Sh::kColumns) : "memory");

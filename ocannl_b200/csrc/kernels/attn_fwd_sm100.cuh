@@ -213,11 +213,10 @@ attn_forward_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant__
   const unsigned int warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
   const unsigned int kLoad = NQ * 4, kMma = NQ * 4 + 1;
   // this CTA's queries: the last ones first, which under a causal mask see the most keys
-  const unsigned int heads = (unsigned int)a.B * (unsigned int)a.H;
-  const unsigned int tiles_q = (a.S + 128 * NQ - 1) / (128 * NQ);
-  const int r0 = (int)(tiles_q - 1 - blockIdx.x / heads) * 128 * NQ;
-  const unsigned int bh = blockIdx.x % heads;
-  const int b = (int)(bh / (unsigned int)a.H), h = (int)(bh % (unsigned int)a.H), hk = h / a.group;
+  const unsigned int tiles_q = (a.S + 128 * NQ - 1) / (128 * NQ), from_last = a.all_heads.of(blockIdx.x);
+  const int r0 = (int)(tiles_q - 1 - from_last) * 128 * NQ;
+  const unsigned int bh = blockIdx.x - from_last * a.all_heads.d;
+  const int b = (int)a.heads.of(bh), h = (int)bh - b * a.H, hk = (int)a.per_key_head.of((unsigned int)h);
   const bool docs = a.kdoc != nullptr;
 
   auto load_keys = [&](int t, unsigned int slot) {
@@ -230,25 +229,18 @@ attn_forward_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant__
 #pragma unroll
     for (int p = 0; p < Sh::kPanels; ++p) b200_tma_load_4d(v_at + slot * Sh::kKeys + p * Sh::kPanel, &map_v, bar_vf + 8 * slot, p * 64, t * KW, hk, b);
   };
-  if (threadIdx.x == kLoad * 32) {
-    b200_mbar_init(bar_q, 1);
-    for (int i = 0; i < 4; ++i) {
-      b200_mbar_init(bar_kf + 8 * i, 1);
-      b200_mbar_init(bar_ke + 8 * i, 1);
-      b200_mbar_init(bar_vf + 8 * i, 1);
-      b200_mbar_init(bar_ve + 8 * i, 1);
-      b200_mbar_init(bar_s + 8 * i, 1);
-      b200_mbar_init(bar_p + 8 * i, 128);
+  // (a barrier a lane: one thread would take some 600 cycles for all of them, ahead of the first copies)
+  if (warp == kLoad) {
+    constexpr unsigned int kBarriers = 29, kFirstP = 21, kLastP = 24;
+    if (lane < kBarriers) b200_mbar_init(bar0 + 8 * lane, lane >= kFirstP && lane <= kLastP ? 128 : 1);
+    if (lane < 2) {
+      spans[lane].last_min = spans[lane].doc_min = 0x7fffffff;
+      spans[lane].last_max = -1;
+      spans[lane].doc_max = -0x7fffffff - 1;
     }
-    for (int i = 0; i < 2; ++i) {
-      b200_mbar_init(bar_o + 8 * i, 1);
-      b200_mbar_init(bar_f + 8 * i, 1);
-      spans[i].last_min = spans[i].doc_min = 0x7fffffff;
-      spans[i].last_max = -1;
-      spans[i].doc_max = -0x7fffffff - 1;
-    }
-    *abort_flag = 0u;
+    if (lane == 2) *abort_flag = 0u;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    __syncwarp();
   }
   if (warp == kMma) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(b200_smem_addr((const void*)tmem_slot)), "r"(Sh::kColumns) : "memory");

@@ -23,6 +23,7 @@ struct AttnArgs {
   int B, S, T, H, HK, D, group, mask;
   int ld;                                // elements from one head of a row to the next: D, or more in padded copies
   float scale, cap, over;                // over: scale / cap
+  Divisor all_heads, heads, all_key_heads, key_heads, per_key_head;    // of a block's number: B H, H, B HK, HK, H / HK
 };
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;

@@ -509,6 +509,15 @@ void bind(const b200_attention& p, AttnOperator* op, bool grad) {
   a.scale = p.scale;
   a.cap = p.cap;
   a.over = p.cap > 0.f ? p.scale / p.cap : 0.f;
+  // (blocks are numbered by heads only where there are rows, and then less than 2^31 of them)
+  a.heads = Divisor((unsigned int)a.H);
+  a.key_heads = Divisor((unsigned int)a.HK);
+  a.per_key_head = Divisor((unsigned int)a.group);
+  const long long all = (long long)a.B * a.H;
+  if (all >= 1 && all < (1ll << 31)) {
+    a.all_heads = Divisor((unsigned int)all);
+    a.all_key_heads = Divisor((unsigned int)a.B * (unsigned int)a.HK);
+  }
   op->choose();
 }
 
