@@ -137,8 +137,11 @@ __device__ __forceinline__ void attn_grad_keys(const b200_tmap& map_q, const b20
   const unsigned int warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
   constexpr unsigned int kLoad = Sh::kWarps - 2, kMma = Sh::kWarps - 1;
   // this CTA's keys: the first ones first, which under a causal mask are seen by the most queries
-  const unsigned int tile_of = a.all_key_heads.of(block), bh = block - tile_of * a.all_key_heads.d;
+  // (blocks that share a key tile, each for some of the query heads, lie one behind the other)
+  const unsigned int share_of = a.all_key_heads.of(block), bh = block - share_of * a.all_key_heads.d;
+  const unsigned int tile_of = a.parts_of.of(share_of);
   const int j0 = (int)tile_of * 128, b = (int)a.key_heads.of(bh), hk = (int)bh - b * a.HK;
+  const int part = (int)(share_of - tile_of * a.parts_of.d), first_head = hk * a.group + part * a.part_heads;
   const int tiles = (a.S + CW - 1) / CW, stat_tiles = (a.S + 127) / 128;
   const bool docs = a.kdoc != nullptr;
   if (warp == kLoad) {
@@ -178,7 +181,7 @@ __device__ __forceinline__ void attn_grad_keys(const b200_tmap& map_q, const b20
   int early = -1;             // the tile that is on its way before the others are known
   if (!docs)
     for (early = 0; early < tiles && !class_without(early); ++early) {}
-  if (threadIdx.x == kLoad * 32 && early >= 0 && early < tiles) load(hk * a.group, early, 0);
+  if (threadIdx.x == kLoad * 32 && early >= 0 && early < tiles) load(first_head, early, 0);
   tc_before();
   __syncthreads();
   tc_after();
@@ -230,7 +233,7 @@ __device__ __forceinline__ void attn_grad_keys(const b200_tmap& map_q, const b20
     if (lane == 0) {
       unsigned int n = 0;
       bool live = true;
-      for (int h = hk * a.group; h < (hk + 1) * a.group && live; ++h)
+      for (int h = first_head; h < first_head + a.part_heads && live; ++h)
         for (int t = begin; t < tiles; ++t) {
           if (!class_of(t)) continue;
           if (docs || n) {
@@ -268,7 +271,7 @@ __device__ __forceinline__ void attn_grad_keys(const b200_tmap& map_q, const b20
       };
       int total = 0;
       for (int t = begin; t < tiles; ++t) total += class_of(t) != 0;
-      total *= a.group;
+      total *= a.part_heads;
       bool live = b200_wait(bar_kv, 0u, abort_flag, a.status, 32u);
       if (live && total) {
         live = b200_wait(bar_full, 0u, abort_flag, a.status, 33u);
@@ -314,7 +317,7 @@ __device__ __forceinline__ void attn_grad_keys(const b200_tmap& map_q, const b20
     const int j = j0 + (int)in;
     unsigned int n = 0;
     bool live = true;
-    for (int h = hk * a.group; h < (hk + 1) * a.group && live; ++h) {
+    for (int h = first_head; h < first_head + a.part_heads && live; ++h) {
       const float slope2 = BIAS ? a.slopes[h] * kLog2e : 0.f;
       for (int t = begin; t < tiles; ++t) {
         const unsigned int cls = class_of(t);
@@ -419,8 +422,16 @@ __device__ __forceinline__ void attn_grad_keys(const b200_tmap& map_q, const b20
         }
 #pragma unroll
         for (int i = 0; i < 32; ++i) o[i] = n ? o[i] * by : 0.f;
-        fine &= store_columns<T>(tile, in, e, o);
+        if (a.n_parts > 1) {         // joined with the other blocks' by a kernel of its own
+          float* to = a.parts + ((((long long)(2 * part + 1 - which) * a.B + b) * a.T + j) * a.HK + hk) * DP + e;
+          if (live && j < a.T)
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) *(float4*)(to + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+        } else {
+          fine &= store_columns<T>(tile, in, e, o);
+        }
       }
+      if (a.n_parts > 1) continue;
       mend[which] = __ballot_sync(0xffffffffu, live && j < a.T && !fine);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
@@ -748,6 +759,42 @@ __device__ __forceinline__ void attn_grad_queries(const b200_tmap& map_q, const 
   if (warp == kMma) {
     tc_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Sh::kColumns) : "memory");
+  }
+}
+
+// Adds the parts of every key's gradients in their order, a warp a row; DP: 64 or 128
+template <class T, int DP>
+__global__ void __launch_bounds__(256) attn_join_parts(const __grid_constant__ AttnArgs a) {
+  asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const unsigned int lane = threadIdx.x & 31u;
+  const long long rows = (long long)a.B * a.T * a.HK;
+  for (long long i = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); i < rows; i += (long long)gridDim.x * 8) {
+    int again = 0;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {          // dk, dv
+      float v[DP / 32];
+#pragma unroll
+      for (int k = 0; k < DP / 32; ++k) v[k] = 0.f;
+      for (int p = 0; p < a.n_parts; ++p) {
+        const float* from = a.parts + ((2 * p + which) * rows + i) * DP;
+#pragma unroll
+        for (int k = 0; k < DP / 32; ++k) v[k] += from[lane + 32 * k];
+      }
+      bool fine = true;
+      T* to = (T*)(which ? a.dv : a.dk) + i * a.ld;
+#pragma unroll
+      for (int k = 0; k < DP / 32; ++k)
+        if ((int)lane + 32 * k < a.D) {
+          from_float(v[k], to[lane + 32 * k]);
+          fine = fine && v[k] * 0.f == 0.f;
+        }
+      if (__any_sync(0xffffffffu, !fine)) again |= 1 << which;
+    }
+    if (again) {
+      const long long bt = i / a.HK;
+      attn_dkv_row<T>(a, (int)(bt / a.T), (int)(i - bt * a.HK), (int)(bt % a.T), lane, again);
+    }
   }
 }
 

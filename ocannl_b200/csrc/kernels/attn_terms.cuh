@@ -15,6 +15,8 @@ struct AttnArgs {
   void *out, *dq, *dk, *dv;
   float* lse;                            // [batch, heads, queries]
   float* stat;                           // gradient: a tile of 128 queries of a head: lse / log 2 of each, then <d_out, out>
+  float* parts;                          // gradient, with `n_parts` > 1: a part's dk, then dv, of [batch, keys, kv_heads] rows of 64 or 128
+  int n_parts, part_heads;               // blocks that share a key tile, query heads of each
   float* norms;                          // gradient, half: largest squares of a row of d_out, n_norms of them
   int n_norms;
   const int *lengths, *prefix, *qdoc, *kdoc;
@@ -23,7 +25,7 @@ struct AttnArgs {
   int B, S, T, H, HK, D, group, mask;
   int ld;                                // elements from one head of a row to the next: D, or more in padded copies
   float scale, cap, over;                // over: scale / cap
-  Divisor all_heads, heads, all_key_heads, key_heads, per_key_head;    // of a block's number: B H, H, B HK, HK, H / HK
+  Divisor all_heads, heads, all_key_heads, key_heads, per_key_head, parts_of;    // of a block's number: B H, H, B HK, HK, H / HK, n_parts
 };
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;

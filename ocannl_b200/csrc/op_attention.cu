@@ -204,6 +204,7 @@ struct AttnOperator : b200_operator {
   bool tc = false;
   ForwardKernel forward = nullptr;
   GradKernel gradients = nullptr;
+  AttnKernel join = nullptr;
   GradMaps maps;
   SingleKernel single = nullptr;
   SingleGradKernel single_grad = nullptr;
@@ -258,6 +259,18 @@ struct AttnOperator : b200_operator {
     if (pad)
       for (auto& n : nodes) n.at = reserve((size_t)(n.of_keys ? key_rows : rows) * ld * 2);
     size_t stat = 0, norms = 0, parts = 0, tickets = 0;
+    a.n_parts = 1;
+    a.part_heads = a.group;
+    if (tc && grad) {
+      // A block walks all query heads that share its keys.  Where that leaves SMs without a block (two for heads of up to 64
+      // elements), as many blocks share a key tile as divide the query heads and are needed, and their sums are joined.
+      const long long blocks = (long long)a.B * a.HK * ((a.T + 127) / 128), want = (a.D <= 64 ? 2ll : 1ll) * dev->sm_count;
+      while (a.n_parts < a.group && blocks * a.n_parts < want)
+        do ++a.n_parts; while (a.group % a.n_parts);
+      a.part_heads = a.group / a.n_parts;
+      if (a.n_parts > 1) parts = reserve((size_t)a.n_parts * 2 * key_rows * (a.D <= 64 ? 64 : 128) * 4);
+    }
+    a.parts_of = Divisor((unsigned int)a.n_parts);
     if (tc && !grad && few_rows()) choose_few(&parts, &tickets);
     if (grad && rows) {
       const long long padded = (long long)a.B * a.H * ((a.S + 127) / 128) * 128;
@@ -301,6 +314,15 @@ struct AttnOperator : b200_operator {
           if (*p == n.node) *p = copy;
       }
       a.ld = ld;
+    }
+    if (a.n_parts > 1) {
+      a.parts = (float*)(workspace + parts);
+      join = by_type(dtype, [&](auto t) -> AttnKernel {
+        typedef decltype(t) T;
+        if constexpr (sizeof(T) == 2) return a.D <= 64 ? attn_join_parts<T, 64> : attn_join_parts<T, 128>;
+        return nullptr;
+      });
+      ready(join);
     }
     if (few) {
       few_args.parts = (float*)(workspace + parts);
@@ -395,7 +417,7 @@ struct AttnOperator : b200_operator {
     });
     grid = blocks_of(heads * ((a.S + 128 * (!grad && two ? 2 : 1) - 1) / (128 * (!grad && two ? 2 : 1))));
     if (grad) {
-      keys_grid = blocks_of((long long)a.B * a.HK * ((a.T + 127) / 128));
+      keys_grid = blocks_of((long long)a.B * a.HK * ((a.T + 127) / 128) * a.n_parts);
       grid = blocks_of((long long)grid + keys_grid);
     }
     if (smem > 227 * 1024) throw Error(B200_E_UNSUPPORTED, "attention: too many keys or queries");
@@ -438,6 +460,7 @@ struct AttnOperator : b200_operator {
     if (grad && rows) launch(statistics, statistics_grid, 256, 0, s, a, by_heads, by_length);
     if (tc && grad) {
       launch(gradients, grid, threads, smem, s, maps, a, keys_grid);
+      if (join) launch(join, blocks(key_rows), 256, 0, s, a);
     } else if (few) {
       launch(few, dim3(grid, (unsigned int)few_args.splits), kFewWarps * 32, smem, s, a, few_args);
     } else if (tc) {

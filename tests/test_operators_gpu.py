@@ -668,6 +668,7 @@ LONG = [
     (40, 513, 513, 2, 2, 128, "none", False, None, 0.0, True),
     (24, 640, 640, 4, 4, 128, "prefix", False, None, 20.0, True),
     (30, 300, 900, 4, 1, 32, "causal", False, None, 0.0, False),
+    (3, 700, 700, 12, 2, 72, "prefix", True, None, 0.0, True),       # few key heads: their query heads are shared out and joined
 ]
 
 
