@@ -243,17 +243,19 @@ struct AttnOperator : b200_operator {
     else if (!tc)
       for (int i = 0; i < 3; ++i) ready(kernel(i));
     // Heads whose rows or addresses are no multiples of 16 bytes go through copies with padded rows.
+    // (each operand has a copy of its own: those that are read may be one node, of which each takes as many rows as it has)
     struct Padded {
-      const void* node;
+      const void** node;
       bool written, of_keys;
       size_t at;
     };
     std::vector<Padded> nodes;
-    for (auto& n : {Padded{a.q, false, false, 0}, {a.k, false, true, 0}, {a.v, false, true, 0}, {a.o, false, false, 0}, {a.d_out, false, false, 0},
-                    {a.out, true, false, 0}, {a.dq, true, false, 0}, {a.dk, true, true, 0}, {a.dv, true, true, 0}})
-      if (n.node) nodes.push_back(n);
+    for (auto& n : {Padded{&a.q, false, false, 0}, {&a.k, false, true, 0}, {&a.v, false, true, 0}, {&a.o, false, false, 0}, {&a.d_out, false, false, 0},
+                    {(const void**)&a.out, true, false, 0}, {(const void**)&a.dq, true, false, 0}, {(const void**)&a.dk, true, true, 0},
+                    {(const void**)&a.dv, true, true, 0}})
+      if (*n.node) nodes.push_back(n);
     bool plain = a.D % 8 == 0;
-    for (auto& n : nodes) plain &= ((size_t)n.node & 15) == 0;
+    for (auto& n : nodes) plain &= ((size_t)*n.node & 15) == 0;
     const int ld = (a.D + 7) / 8 * 8;
     const bool pad = tc && !plain;
     if (pad)
@@ -308,10 +310,9 @@ struct AttnOperator : b200_operator {
       for (auto& n : nodes) {
         void* copy = (void*)(workspace + n.at);
         const long long many = n.of_keys ? key_rows : rows;
-        if (n.written) after.push_back({copy, (void*)n.node, many, ld, a.D});
-        else before.push_back({n.node, copy, many, a.D, ld});
-        for (const void** p : {&a.q, &a.k, &a.v, &a.o, &a.d_out, (const void**)&a.out, (const void**)&a.dq, (const void**)&a.dk, (const void**)&a.dv})
-          if (*p == n.node) *p = copy;
+        if (n.written) after.push_back({copy, (void*)*n.node, many, ld, a.D});
+        else before.push_back({*n.node, copy, many, a.D, ld});
+        *n.node = copy;
       }
       a.ld = ld;
     }

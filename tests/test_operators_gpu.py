@@ -5,6 +5,7 @@ import numpy as np
 import pytest
 
 from ocannl_b200 import backend as bk
+from ocannl_b200.low_level import Tnode
 from tests import operators_reference as R
 
 pytestmark = pytest.mark.gpu
@@ -442,6 +443,37 @@ def test_captured_replayed_and_with_a_growing_cache(device):
         o.free()
     nodes.free()
     others.free()
+
+
+@pytest.mark.parametrize("prec", PRECS)
+@pytest.mark.parametrize("s,n", [(3, 60), (40, 300), (300, 40)])
+def test_one_node_as_queries_keys_and_values(device, s, n, prec):
+    """Inputs may be one node, each of the rows that its own shape says; heads of 20 elements take copies with padded rows."""
+    most = max(s, n)
+    rng = np.random.default_rng(17)
+    both = R.rounded(prec, rng.standard_normal((1, most, 2, 20)))
+    x = dict(q=both[:, :s], k=both[:, :n], v=both[:, :n], d_out=both[:, :s])
+    seen, pos = R.visible(1, s, n, "none")
+    scale = 1.0 / np.sqrt(20)
+    out, lse, size, flat = R.attention(x["q"], x["k"], x["v"], seen, pos, scale)
+    o, l = R.rounded(prec, out), R.rounded("single", lse)
+    want = R.attention_grad(x["q"], x["k"], x["v"], o, l, x["d_out"], seen, pos, scale, 0.0, None, prec)
+    nodes = R.Nodes(device, dict(both=(prec, both.shape, both), out=(prec, out.shape, None), lse=("single", lse.shape, None), o=(prec, out.shape, o),
+                                 l=("single", lse.shape, l), dq=(prec, x["q"].shape, None), dk=(prec, x["k"].shape, None), dv=(prec, x["k"].shape, None)))
+    pool, off, _ = nodes.context.arrays["both"]
+    for i, (name, rows) in enumerate((("queries", s), ("keys", n))):
+        nodes.context.arrays[name] = (pool, off, Tnode(90 + i, name, prec, (1, rows, 2, 20)))
+    ops = [nodes.context.attention("queries", "keys", "keys", "out", lse="lse", mask="none"),
+           nodes.context.attention_grad("queries", "keys", "keys", "o", "l", "queries", "dq", "dk", "dv", mask="none")]
+    for op in ops:
+        op.run()
+    device.await_()
+    R.within(nodes.read("out"), out, out_bound(prec, out, size, flat), "out")
+    for name, (v, bound) in zip(("dq", "dk", "dv"), want):
+        R.within(nodes.read(name), v, bound, name)
+    for op in ops:
+        op.free()
+    nodes.free()
 
 
 def test_runs_wait_for_uploads(device):
