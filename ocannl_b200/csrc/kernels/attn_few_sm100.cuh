@@ -5,7 +5,7 @@
 // head) are cut into `splits` ranges, one a block, so that a few sequences fill the machine; a block's four warps take
 // every fourth step of 16 keys, each with a ring of its own that cp.async fills two steps ahead, and its own running maximum, sum and
 // output.  The warps meet in shared memory, the blocks in the workspace: the block that comes last joins the ranges in their
-// order (the same bits whoever comes last).  Keys behind the last visible one are not read but zeroed in shared memory.
+// order (the same bits whoever comes last), or, where a warp of it would have several rows to join, a second launch with a block a row.  Keys behind the last visible one are not read but zeroed in shared memory.
 #ifndef B200_ATTN_FEW_SM100_CUH
 #define B200_ATTN_FEW_SM100_CUH
 #include "attn_fwd_sm100.cuh"
@@ -18,6 +18,7 @@ struct FewArgs {
   float* parts;            // [pair][split][16][DP + 4]: output (not divided), maximum, sum, and two floats that keep rows on 16 bytes
   unsigned int* tickets;   // [pair], zero between runs
   int splits, per_split;   // keys of a range, a multiple of 16 * 4
+  int join_later;          // the ranges are joined by a launch of its own
 };
 
 template <int DP>
@@ -49,6 +50,92 @@ __device__ __forceinline__ void ldmatrix4_t(unsigned int (&r)[4], unsigned int a
 // 16 bytes, zeros where not `on`
 __device__ __forceinline__ void copy16(unsigned int dst, const void* src, bool on) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+
+// The maximum and the sum of `n` partial rows `step` apart, and in `weight` (n of them) what each is multiplied by: a warp.
+// (a part without visible keys counts nothing, whatever it holds)
+template <int DP>
+__device__ __forceinline__ void few_weigh(const float* from, int n, long long step, float* weight, float& top, float& sum) {
+  const unsigned int lane = threadIdx.x & 31u;
+  float t[kFewMost / 32], u[kFewMost / 32];
+  top = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < kFewMost / 32; ++k) {
+    const int i = (int)lane + 32 * k;
+    t[k] = i < n ? from[i * step + DP] : -INFINITY;
+    u[k] = i < n ? from[i * step + DP + 1] : 0.f;
+    top = fmaxf(top, t[k]);
+  }
+#pragma unroll
+  for (int k = 16; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+  sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < kFewMost / 32; ++k) {
+    const float w = t[k] == -INFINITY ? 0.f : ex2(t[k] - top);
+    if ((int)lane + 32 * k < n) weight[lane + 32 * k] = w;
+    if (w != 0.f) sum = fmaf(w, u[k], sum);
+  }
+#pragma unroll
+  for (int k = 16; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+  __syncwarp();
+}
+// four elements of the sum of every `each`-th weighed part from `i0` on; eight loads under way together
+__device__ __forceinline__ float4 few_gather(const float* from, int n, long long step, const float* weight, int e, int i0, int each) {
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = i0; i < n; i += 8 * each) {
+    float4 x[8];
+    float w[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int at = i + k * each;
+      w[k] = at < n ? weight[at] : 0.f;
+      x[k] = *(const float4*)(from + (at < n ? at : i) * step + e);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (w[k] != 0.f) v = make_float4(fmaf(w[k], x[k].x, v.x), fmaf(w[k], x[k].y, v.y), fmaf(w[k], x[k].z, v.z), fmaf(w[k], x[k].w, v.w));
+  }
+  return v;
+}
+// Writes four elements of a row and, with the first, its lse.  False: one is infinite or undefined, and the row has to be mended (0 times
+// infinity from a hidden key among visible ones)
+template <class T>
+__device__ __forceinline__ bool few_finish(const AttnArgs& a, int b, int h, int r, int e, const float4& v, float top, float sum) {
+  const float by = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+  const float y[4] = {v.x * by, v.y * by, v.z * by, v.w * by};
+  T* to = (T*)a.out + attn_q_at(a, b, r, h) + e;
+  bool fine = true;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (e + k < a.D) {
+      from_float(y[k], to[k]);
+      fine = fine && y[k] * 0.f == 0.f;
+    }
+  if (e == 0 && a.lse) a.lse[((long long)b * a.H + h) * a.S + r] = by != 0.f ? (top + log2f(sum)) * kLn2 : -INFINITY;
+  return fine;
+}
+// One row by a block: each of the four warps adds every fourth part, the first adds the four sums.
+template <class T, int DP>
+__device__ __forceinline__ void few_row_of_block(const AttnArgs& a, int b, int h, int r, const float* from, int n, float* weight, float4* meet) {
+  constexpr int step = kFewRows * FewShape<DP>::kWidth;
+  const unsigned int warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+  float top, sum;
+  few_weigh<DP>(from, n, step, weight, top, sum);
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (lane < DP / 4) v = few_gather(from, n, step, weight, 4 * (int)lane, (int)warp, kFewWarps);
+  __syncthreads();
+  if (lane < DP / 4) meet[warp * (DP / 4) + lane] = v;
+  __syncthreads();
+  if (warp) return;
+  bool fine = true;
+  if (lane < DP / 4) {
+    for (int w = 1; w < kFewWarps; ++w) {
+      const float4 x = meet[w * (DP / 4) + lane];
+      v = make_float4(v.x + x.x, v.y + x.y, v.z + x.z, v.w + x.w);
+    }
+    fine = few_finish<T>(a, b, h, r, 4 * (int)lane, v, top, sum);
+  }
+  if (__any_sync(0xffffffffu, !fine)) attn_forward_row<T>(a, b, h, r, lane);
 }
 
 // blockIdx.x: (sequence, key head, sixteen of the rows that share it); blockIdx.y: range of keys
@@ -247,77 +334,21 @@ __global__ void __launch_bounds__(kFewWarps * 32) attn_forward_few(const __grid_
   }
   __syncthreads();
   const int rows = min(kFewRows, shared_rows - first_row);
-  // The maximum and the sum of `n` partial rows `step` apart, and in `weight` (n of them) what each is multiplied by: a warp.
-  // (a part without visible keys counts nothing, whatever it holds)
-  auto weigh = [&](const float* from, int n, long long step, float* weight, float& top, float& sum) {
-    float t[kFewMost / 32], u[kFewMost / 32];
-    top = -INFINITY;
-#pragma unroll
-    for (int k = 0; k < kFewMost / 32; ++k) {
-      const int i = (int)lane + 32 * k;
-      t[k] = i < n ? from[i * step + DP] : -INFINITY;
-      u[k] = i < n ? from[i * step + DP + 1] : 0.f;
-      top = fmaxf(top, t[k]);
-    }
-#pragma unroll
-    for (int k = 16; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
-    sum = 0.f;
-#pragma unroll
-    for (int k = 0; k < kFewMost / 32; ++k) {
-      const float w = t[k] == -INFINITY ? 0.f : ex2(t[k] - top);
-      if ((int)lane + 32 * k < n) weight[lane + 32 * k] = w;
-      if (w != 0.f) sum = fmaf(w, u[k], sum);
-    }
-#pragma unroll
-    for (int k = 16; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
-    __syncwarp();
-  };
-  // four elements of the sum of every `each`-th weighed part from `i0` on; eight loads under way together
-  auto gather = [&](const float* from, int n, long long step, const float* weight, int e, int i0, int each) {
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i = i0; i < n; i += 8 * each) {
-      float4 x[8];
-      float w[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int at = i + k * each;
-        w[k] = at < n ? weight[at] : 0.f;
-        x[k] = *(const float4*)(from + (at < n ? at : i) * step + e);
-      }
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (w[k] != 0.f) v = make_float4(fmaf(w[k], x[k].x, v.x), fmaf(w[k], x[k].y, v.y), fmaf(w[k], x[k].z, v.z), fmaf(w[k], x[k].w, v.w));
-    }
-    return v;
-  };
-  bool fine = true;
-  auto finish = [&](int i, int e, const float4& v, float top, float sum) {
-    const int h = head_of(i), r = query_of(i);
-    const float by = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-    const float y[4] = {v.x * by, v.y * by, v.z * by, v.w * by};
-    T* to = (T*)a.out + attn_q_at(a, b, r, h) + e;
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (e + k < a.D) {
-        from_float(y[k], to[k]);
-        fine = fine && y[k] * 0.f == 0.f;
-      }
-    if (e == 0 && a.lse) a.lse[((long long)b * a.H + h) * a.S + r] = by != 0.f ? (top + log2f(sum)) * kLn2 : -INFINITY;
-  };
+  const int lane_e = 4 * (int)lane;
   __shared__ float weights[kFewWarps][kFewMost];
   float* parts = f.parts + ((long long)pair * f.splits + split) * kFewRows * W;
-  // a warp takes every fourth row; rows with a value that is infinite or undefined are mended (0 times infinity from a hidden key
-  // among visible ones)
+  // a warp takes every fourth row
   if (f.splits > 1) {
     for (int i = (int)warp; i < rows; i += kFewWarps) {
       float top, sum;
-      weigh(join + i * W, kFewWarps, kFewRows * W, weights[warp], top, sum);
-      if ((int)lane < DP / 4) *(float4*)(parts + i * W + 4 * lane) = gather(join + i * W, kFewWarps, kFewRows * W, weights[warp], 4 * (int)lane, 0, 1);
+      few_weigh<DP>(join + i * W, kFewWarps, kFewRows * W, weights[warp], top, sum);
+      if (lane_e < DP) *(float4*)(parts + i * W + lane_e) = few_gather(join + i * W, kFewWarps, kFewRows * W, weights[warp], lane_e, 0, 1);
       if (lane == 0) {
         parts[i * W + DP] = top;
         parts[i * W + DP + 1] = sum;
       }
     }
+    if (f.join_later) return;
     __threadfence();
     __syncthreads();
     if (threadIdx.x == 0) last_block = atomicAdd(&f.tickets[pair], 1u) == (unsigned int)f.splits - 1u;
@@ -328,34 +359,31 @@ __global__ void __launch_bounds__(kFewWarps * 32) attn_forward_few(const __grid_
   }
   const float* all = f.splits > 1 ? f.parts + (long long)pair * f.splits * kFewRows * W : join;
   const int n_parts = f.splits > 1 ? f.splits : kFewWarps;
-  // A single row is shared by the four warps: each adds every fourth part, the first adds the four sums.
   if (rows == 1) {
-    float top, sum;
-    weigh(all, n_parts, kFewRows * W, weights[warp], top, sum);
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if ((int)lane < DP / 4) v = gather(all, n_parts, kFewRows * W, weights[warp], 4 * (int)lane, (int)warp, kFewWarps);
-    float4* meet = (float4*)(dyn + sizeof(float) * kFewWarps * kFewRows * W);       // (behind `join`, within the rings)
-    __syncthreads();
-    if ((int)lane < DP / 4) meet[warp * (DP / 4) + lane] = v;
-    __syncthreads();
-    if (warp) return;
-    if ((int)lane < DP / 4) {
-      for (int w = 1; w < kFewWarps; ++w) {
-        const float4 x = meet[w * (DP / 4) + lane];
-        v = make_float4(v.x + x.x, v.y + x.y, v.z + x.z, v.w + x.w);
-      }
-      finish(0, 4 * (int)lane, v, top, sum);
-    }
-    if (__any_sync(0xffffffffu, !fine)) attn_forward_row<T>(a, b, head_of(0), query_of(0), lane);
+    few_row_of_block<T, DP>(a, b, head_of(0), query_of(0), all, n_parts, weights[warp], (float4*)(dyn + sizeof(float) * kFewWarps * kFewRows * W));   // (behind `join`)
     return;
   }
   for (int i = (int)warp; i < rows; i += kFewWarps) {
     float top, sum;
-    weigh(all + i * W, n_parts, kFewRows * W, weights[warp], top, sum);
-    fine = true;
-    if ((int)lane < DP / 4) finish(i, 4 * (int)lane, gather(all + i * W, n_parts, kFewRows * W, weights[warp], 4 * (int)lane, 0, 1), top, sum);
+    few_weigh<DP>(all + i * W, n_parts, kFewRows * W, weights[warp], top, sum);
+    bool fine = true;
+    if (lane_e < DP) fine = few_finish<T>(a, b, head_of(i), query_of(i), lane_e, few_gather(all + i * W, n_parts, kFewRows * W, weights[warp], lane_e, 0, 1), top, sum);
     if (__any_sync(0xffffffffu, !fine)) attn_forward_row<T>(a, b, head_of(i), query_of(i), lane);
   }
+}
+
+// The join of the ranges of one row, a block; blockIdx.x as above, blockIdx.y: the row of its sixteen
+template <class T, int DP>
+__global__ void __launch_bounds__(kFewWarps * 32) attn_join_few(const __grid_constant__ AttnArgs a, const FewArgs f) {
+  __shared__ float weights[kFewWarps][kFewMost];
+  __shared__ float4 meet[kFewWarps * DP / 4];
+  asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int shared_rows = a.group * a.S, sixteens = (shared_rows + kFewRows - 1) / kFewRows;
+  const int pair = (int)blockIdx.x, unit = pair / sixteens, i = (int)blockIdx.y, row = pair % sixteens * kFewRows + i;
+  if (row >= shared_rows) return;
+  few_row_of_block<T, DP>(a, unit / a.HK, unit % a.HK * a.group + row / a.S, row % a.S, f.parts + ((long long)pair * f.splits * kFewRows + i) * FewShape<DP>::kWidth, f.splits,
+                          weights[threadIdx.x >> 5], meet);
 }
 
 }  // namespace b200

@@ -142,6 +142,7 @@ typedef void (*GradKernel)(const GradMaps, const AttnArgs, unsigned int);
 typedef void (*SingleKernel)(const AttnArgs, int, int, int);
 typedef void (*SingleGradKernel)(const AttnArgs, int, int, int, unsigned int);
 typedef void (*FewKernel)(const AttnArgs, const FewArgs);
+typedef void (*FewJoinKernel)(const AttnArgs, const FewArgs);
 
 template <class T, int DP>
 FewKernel few_of(bool cap, bool bias) {
@@ -210,6 +211,7 @@ struct AttnOperator : b200_operator {
   SingleGradKernel single_grad = nullptr;
   int vec = 0, places = 1, groups = 4;
   FewKernel few = nullptr;
+  FewJoinKernel few_join = nullptr;
   FewArgs few_args = {};
   b200_tmap map_q, map_k, map_v, map_o;
   unsigned int threads = 0, grid = 0, keys_grid = 0;
@@ -330,15 +332,20 @@ struct AttnOperator : b200_operator {
       few_args.tickets = (unsigned int*)(workspace + tickets);
       cu_check(cu().cuMemsetD8Async_(workspace + tickets, 0, (size_t)grid * 4, dev->stream), "cuMemsetD8Async(tickets)");
       ready(few, smem);
+      if (few_join) ready(few_join);
     } else if (tc) {
       choose_tc();
     }
   }
   // A tile of the tensor-core kernel has 128 queries of one head.  Up to 16 queries go sixteen rows at a time (of all heads that
-  // share the keys), the keys split over the machine.
-  bool few_rows() const { return a.S <= 16; }
+  // share the keys), the keys split over the machine, and so do up to 128 over many keys, whose tiles would leave most of the machine idle
+  // for the length of one walk: over 8192 keys a walk of tiles takes 100 us, and 17 queries of 8 heads of 64 take 16, 128 of them 29, 128 of
+  // 32 heads over 8 (256 sixteens) 70; of heads of 128 20, 48 and (64 queries, 128 sixteens) 79.  Over 2048 keys the walk takes 29, half as
+  // many sixteens 22 to 28; so the shorter the keys, the fewer.
+  long long sixteens() const { return (long long)a.B * a.HK * (((long long)a.group * a.S + kFewRows - 1) / kFewRows); }
+  bool few_rows() const { return a.S <= 16 || (a.S <= 128 && a.T >= 1024 && sixteens() * (a.D <= 64 ? 16 : 32) <= std::min(a.T, 4096)); }
   void choose_few(size_t* parts, size_t* tickets) {
-    const long long pairs = (long long)a.B * a.HK * ((a.group * a.S + kFewRows - 1) / kFewRows);
+    const long long pairs = sixteens();
     grid = blocks_of(pairs);
     by_type(dtype, [&](auto t) {
       typedef decltype(t) T;
@@ -353,6 +360,13 @@ struct AttnOperator : b200_operator {
     const int step = kFewStep * kFewWarps, splits = (int)std::max<long long>(1, std::min<long long>(std::min(most, want), kFewMost));
     few_args.per_split = ((a.T + splits - 1) / splits + step - 1) / step * step;
     few_args.splits = (a.T + few_args.per_split - 1) / few_args.per_split;
+    few_args.join_later = few_args.splits > 1 && a.group * a.S > kFewWarps;
+    if (few_args.join_later)
+      few_join = by_type(dtype, [&](auto t) -> FewJoinKernel {
+        typedef decltype(t) T;
+        if constexpr (sizeof(T) == 2) return a.D <= 64 ? attn_join_few<T, 64> : attn_join_few<T, 128>;
+        return nullptr;
+      });
     const int width = a.D <= 64 ? FewShape<64>::kWidth : FewShape<128>::kWidth;
     *parts = reserve(few_args.splits > 1 ? (size_t)pairs * few_args.splits * kFewRows * width * 4 : 0);
     *tickets = reserve((size_t)pairs * 4);
@@ -464,6 +478,7 @@ struct AttnOperator : b200_operator {
       if (join) launch(join, blocks(key_rows), 256, 0, s, a);
     } else if (few) {
       launch(few, dim3(grid, (unsigned int)few_args.splits), kFewWarps * 32, smem, s, a, few_args);
+      if (few_join) launch(few_join, dim3(grid, (unsigned int)std::min(kFewRows, a.group * a.S)), kFewWarps * 32, 0, s, a, few_args);
     } else if (tc) {
       launch(forward, grid, threads, smem, s, map_q, map_k, map_v, map_o, a);
     } else if (single) {

@@ -366,7 +366,8 @@ def test_operators_of_one_kernel_and_different_sizes(device):
         x, _, gamma, beta, _ = norm_case(rows, n, "single", n, False)
         nodes = R.Nodes(device, dict(x=("single", (rows, n), x), g=("single", (n,), gamma), b=("single", (n,), beta), y=("single", (rows, n), None)))
         made.append((nodes, nodes.context.layer_norm("x", "y", gamma="g", beta="b"), R.layer_norm(x, gamma, beta)[0]))
-    cases = [(1, 70, 70, 2, 2, 64, "causal", True, None, 0.0, False), (1, 20, 20000, 2, 2, 64, "causal", True, None, 0.0, False), ATTENTION[13]]
+    cases = [(1, 70, 70, 2, 2, 64, "causal", True, None, 0.0, False), (1, 20, 20000, 2, 2, 64, "causal", True, None, 0.0, False), ATTENTION[13],
+             (1, 130, 20000, 1, 1, 64, "causal", True, None, 0.0, False)]
     attn = []
     for case in cases:
         x, t, more, sl, seen, pos, scale = attention_case(case, "bfloat16")
@@ -701,6 +702,10 @@ LONG = [
     (24, 640, 640, 4, 4, 128, "prefix", False, None, 20.0, True),
     (30, 300, 900, 4, 1, 32, "causal", False, None, 0.0, False),
     (3, 700, 700, 12, 2, 72, "prefix", True, None, 0.0, True),       # few key heads: their query heads are shared out and joined
+    # up to 128 queries over many keys
+    (3, 100, 2100, 6, 2, 64, "causal", True, (2100, 1400, 60), 0.0, False),
+    (3, 128, 2304, 3, 1, 96, "prefix", True, None, 20.0, True),
+    (3, 17, 4099, 5, 5, 40, "none", False, (4099, 0, 3), 0.0, True),
 ]
 
 
