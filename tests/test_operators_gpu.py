@@ -312,6 +312,12 @@ def test_attention_ignores_what_is_not_seen(device, case, prec):
     nodes.free()
 
 
+@pytest.mark.parametrize("prec", ("bfloat16", "half"))
+@pytest.mark.parametrize("case", [(1, 60, 1100, 2, 1, 33, "causal", False, None, 0.0, False), (2, 20, 2048, 4, 2, 128, "causal", False, (2048, 40), 30.0, True)])
+def test_attention_over_split_keys_ignores_what_is_not_seen(device, case, prec):
+    test_attention_ignores_what_is_not_seen(device, case, prec)
+
+
 def test_attention_gradients_by_differences(device):
     """The gradients that the operator gives against central differences of the forward operator, in single precision."""
     case = (2, 70, 70, 4, 2, 24, "prefix", True, None, 8.0, True)
