@@ -53,7 +53,8 @@ __device__ __forceinline__ void copy16(unsigned int dst, const void* src, bool o
 }
 
 // The maximum and the sum of `n` partial rows `step` apart, and in `weight` (n of them) what each is multiplied by: a warp.
-// (a part without visible keys counts nothing, whatever it holds)
+// (a part without visible keys has a sum of exactly 0 and counts nothing, whatever else it holds; one whose visible scores are all
+// undefined has no maximum either, but an undefined sum, which has to reach the result)
 template <int DP>
 __device__ __forceinline__ void few_weigh(const float* from, int n, long long step, float* weight, float& top, float& sum) {
   const unsigned int lane = threadIdx.x & 31u;
@@ -71,7 +72,7 @@ __device__ __forceinline__ void few_weigh(const float* from, int n, long long st
   sum = 0.f;
 #pragma unroll
   for (int k = 0; k < kFewMost / 32; ++k) {
-    const float w = t[k] == -INFINITY ? 0.f : ex2(t[k] - top);
+    const float w = u[k] == 0.f ? 0.f : t[k] == -INFINITY ? 1.f : ex2(t[k] - top);
     if ((int)lane + 32 * k < n) weight[lane + 32 * k] = w;
     if (w != 0.f) sum = fmaf(w, u[k], sum);
   }
