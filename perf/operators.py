@@ -363,7 +363,8 @@ class _Program:
             f, magnitude = _frequencies(case)
             return ctx.rotary([("q", "q_out"), ("k", "k_out")], frequencies=f, magnitude=magnitude, positions="positions",
                               layout=case["layout"], inverse=case["grad"])
-        terms = dict(mask=case["mask"], prefix="prefix" if "prefix" in x else None, documents="docs" if "docs" in x else None,
+        documents = ("query_docs", "docs") if "query_docs" in x else "docs" if "docs" in x else None
+        terms = dict(mask=case["mask"], prefix="prefix" if "prefix" in x else None, documents=documents,
                      lengths="lengths" if "lengths" in x else None, slopes="slopes" if "slopes" in x else None, cap=case["cap"])
         if case["grad"]:
             return ctx.attention_grad("q", "k", "v", "out", "lse", "d_out", "dq", "dk", "dv", **terms)
@@ -397,7 +398,10 @@ def prepare(case, seed):
     s = _State()
     s.case, s.x = case, _inputs(case, seed)
     if own:
-        # the nodes lie in the context's pool, the operator is linked to them
+        # the nodes lie in the context's pool, the operator is linked to them; with lengths the queries' documents, which are those of
+        # the last entries and not of the queries' positions, are a node of their own
+        if "docs" in s.x and "lengths" in s.x:
+            s.x["query_docs"] = s.x["docs"][:, case["keys"] - case["queries"]:].contiguous()
         s.program = _Program(case, s.x)
         s.outputs = {n: s.program.view(n) for n in _results(case, s.x)}
         s.x = None
