@@ -257,7 +257,8 @@ int b200_rotary_link(b200_dev* dev, const b200_rotary* spec, b200_operator** out
  * in a row), 1 <= d <= 128.  Query r of sequence b lies at position len_b - queries + r, where len_b is lengths[b] (taken
  * between 0 and `keys`) or `keys`.  It sees key j if j < len_b, and
  *   B200_MASK_CAUSAL: j <= position;   B200_MASK_PREFIX: j <= position or j < prefix[b];
- *   and, with documents: key_documents[b, j] == query_documents[b, r] >= 0 (a negative document is padding).
+ *   and, with documents: key_documents[b, j] == query_documents[b, r] >= 0 (a negative document is padding).  Where no documents of
+ *   queries are given, a query has the document of the key at its position (and none, like padding, where its position is negative).
  * What lies at a key or a query that is not seen has no influence, whatever it holds.
  * The gradient takes out and lse of the forward pass and gives, with p = exp(s - lse),
  *   dv_j = sum_r p_rj d_out_r;  ds_rj = p_rj (<d_out_r, v_j> - <d_out_r, out_r>);  dx = ds (1 - (c / cap)^2)
@@ -275,8 +276,8 @@ typedef struct {
   b200_operand q, k, v, out;
   b200_operand lse;              /* [batch, heads, queries] single; optional in the forward pass */
   b200_operand lengths, prefix;  /* int32 [batch] */
-  b200_operand query_documents;  /* int32 [batch, queries], and ... */
-  b200_operand key_documents;    /* int32 [batch, keys]: both or neither; may be one node */
+  b200_operand query_documents;  /* int32 [batch, queries], optional beside ... */
+  b200_operand key_documents;    /* int32 [batch, keys] */
   b200_operand slopes;           /* single [heads] */
   b200_operand d_out, dq, dk, dv;
 } b200_attention;

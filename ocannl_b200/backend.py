@@ -545,7 +545,7 @@ class Context:
         (b, s, h, d), (n, hk) = t.dims, u.dims[1:3]
         spec = AttentionSpec(batch=b, queries=s, keys=n, heads=h, kv_heads=hk, d=d, dtype=DTYPE[t.prec], mask=MASKS[mask],
                              scale=1.0 / np.sqrt(d) if scale is None and d else scale or 0.0, cap=cap)
-        qdoc, kdoc = (documents, documents) if documents is None or isinstance(documents, str) else documents
+        qdoc, kdoc = (None, documents) if documents is None or isinstance(documents, str) else documents
         for names, prec, dims in ((dict(rows_like, q=q), t.prec, t.dims), (dict(keys_like, k=k), t.prec, (b, n, hk, d)),
                                   (dict(lse=lse), "single", (b, h, s)), (dict(prefix=prefix, lengths=lengths), "int32", (b,)),
                                   (dict(query_documents=qdoc), "int32", (b, s)), (dict(key_documents=kdoc), "int32", (b, n)),
@@ -559,8 +559,9 @@ class Context:
                   cap: float = 0.0) -> Operator:
         """out = softmax over the visible keys of the scores, times v; lse (single [batch, heads, queries]) is what
         `attention_grad` reads.  The queries are the last ones of each sequence's `lengths` (or all) keys.  mask: "none",
-        "causal" or "prefix" (keys before prefix[b] are seen by all).  documents: an int32 node of numbers per key -- or two, of
-        queries and keys; queries see keys of their own document, a negative number is padding.  slopes: bias by distance,
+        "causal" or "prefix" (keys before prefix[b] are seen by all).  documents: an int32 node of numbers per key, where
+        a query has the number of the key at its position -- or two nodes, of queries and keys; queries see keys of their own document, a
+        negative number is padding.  slopes: bias by distance,
         -slopes[h] * |position - key|.  scale: 1 / sqrt(d) by default.  cap: scores become cap * tanh(score / cap)."""
         return self._attention("attention", q, k, dict(out=out), dict(v=v), lse, mask, prefix, documents, lengths, slopes, scale, cap)
 

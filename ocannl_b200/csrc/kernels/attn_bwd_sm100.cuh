@@ -58,10 +58,10 @@ __device__ __forceinline__ void bulk_load(unsigned int dst, const void* src, uns
 // Which of the 64 queries from r0 see key j, a bit each (bits of queries behind the last one are of no account: their weights are zero).
 // Without documents a key is seen from one query on.
 __device__ __forceinline__ void visible_queries(const AttnArgs& a, int b, int r0, int j, unsigned int lane, unsigned int (&bits)[2]) {
-  const int len = a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
+  const AttnSeq seq = attn_seq(a, b);
   int first = 0;
-  if (j >= len) first = 0x7fffffff;
-  else if (a.mask == B200_MASK_CAUSAL || (a.mask == B200_MASK_PREFIX && j >= a.prefix[b])) first = max(0, j - (len - a.S));
+  if (j >= seq.len) first = 0x7fffffff;
+  else if (a.mask == B200_MASK_CAUSAL || (a.mask == B200_MASK_PREFIX && j >= seq.prefix)) first = max(0, j - (seq.len - a.S));
   int doc = 0;
   if (a.kdoc) {
     doc = j < a.T ? a.kdoc[(long long)b * a.T + j] : -1;
@@ -77,7 +77,7 @@ __device__ __forceinline__ void visible_queries(const AttnArgs& a, int b, int r0
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int r = r0 + (int)lane + 32 * i;
-    d[i] = r < a.S ? a.qdoc[(long long)b * a.S + r] : -1;
+    d[i] = r < a.S ? attn_query_document(a, seq, b, r) : -1;
   }
   unsigned int todo = 0xffffffffu;
   while (todo) {
@@ -198,7 +198,7 @@ __device__ __forceinline__ void attn_grad_keys(const b200_tmap& map_q, const b20
 #pragma unroll
         for (int i = 0; i < CW / 32; ++i) {
           const long long r = (long long)(t0 + n * (int)Sh::kWarps) * CW + 32 * i + lane;
-          d[n][i] = r < a.S ? __ldg(a.qdoc + (long long)b * a.S + r) : -1;
+          d[n][i] = r < a.S ? attn_query_document(a, seq, b, (int)r) : -1;
         }
 #pragma unroll
       for (int n = 0; n < kAhead; ++n) {

@@ -19,7 +19,7 @@ struct AttnArgs {
   int n_parts, part_heads;               // blocks that share a key tile, query heads of each
   float* norms;                          // gradient, half: largest squares of a row of d_out, n_norms of them
   int n_norms;
-  const int *lengths, *prefix, *qdoc, *kdoc;
+  const int *lengths, *prefix, *qdoc, *kdoc;   // (kdoc without qdoc: a query has the document of the key at its position)
   const float* slopes;
   unsigned int* status;
   int B, S, T, H, HK, D, group, mask;
@@ -49,14 +49,20 @@ __device__ __forceinline__ int attn_last(const AttnArgs& a, const AttnSeq& s, in
   const int last = a.mask == B200_MASK_NONE ? s.len - 1 : min(s.len - 1, max(s.len - a.S + r, s.prefix - 1));
   return max(last, -1);
 }
+// a query's document: its entry of the queries' documents, or that of the key at its position (no position, no document)
+__device__ __forceinline__ int attn_query_document(const AttnArgs& a, const AttnSeq& s, int b, int r) {
+  if (a.qdoc) return a.qdoc[(long long)b * a.S + r];
+  const int pos = s.len - a.S + r;
+  return pos < 0 ? -1 : a.kdoc[(long long)b * a.T + pos];
+}
 __device__ __forceinline__ AttnRow attn_row(const AttnArgs& a, int b, int r) {
   const AttnSeq s = attn_seq(a, b);
   AttnRow w;
   w.pos = s.len - a.S + r;
   w.last = attn_last(a, s, r);
   w.doc = 0;
-  if (a.qdoc) {
-    w.doc = a.qdoc[(long long)b * a.S + r];
+  if (a.kdoc) {
+    w.doc = attn_query_document(a, s, b, r);
     if (w.doc < 0) w.last = -1;
   }
   return w;

@@ -507,7 +507,7 @@ void bind(const b200_attention& p, AttnOperator* op, bool grad) {
   if (!(p.cap >= 0.f) || !std::isfinite(p.cap)) ops.refuse("the cap must be finite and not negative (0: none)");
   if (p.mask < B200_MASK_NONE || p.mask > B200_MASK_PREFIX) ops.refuse("unknown mask " + std::to_string(p.mask));
   if ((p.mask == B200_MASK_PREFIX) != (p.prefix.pool_id >= 0)) ops.refuse("'prefix' goes with the prefix mask");
-  if ((p.query_documents.pool_id >= 0) != (p.key_documents.pool_id >= 0)) ops.refuse("documents are given for queries and keys, or for neither");
+  if (p.query_documents.pool_id >= 0 && p.key_documents.pool_id < 0) ops.refuse("documents of queries go with documents of keys");
   const size_t size = dtype_bytes(p.dtype);
   const unsigned long long nq = extent_product({p.batch, p.queries, p.heads, p.d}, "attention");
   const unsigned long long nk = extent_product({p.batch, p.keys, p.kv_heads, p.d}, "attention");

@@ -57,3 +57,57 @@ def test_undefined_values_that_are_seen_show(device, case, what, prec):
         else:
             x["k"][i, :, 0, 0] = np.nan
     check_forward(device, case, prec, x, t, more, sl, seen, pos, scale, sorted({0, b - 1}))
+
+
+def relink(nodes, op, t, more, sl, grad, **kw):
+    """The operator of `link_attention`'s nodes with other arguments."""
+    op.free()
+    kw = dict(dict(mask=t["mask"], cap=t["cap"], prefix="prefix" if "prefix" in more else None, lengths="lengths" if "lengths" in more else None,
+                   slopes="slopes" if sl is not None else None), **kw)
+    if grad:
+        return nodes.context.attention_grad("q", "k", "v", "out", "lse", "d_out", "dq", "dk", "dv", **kw)
+    return nodes.context.attention("q", "k", "v", "out", lse="lse", **kw)
+
+
+# one node of documents: batch, queries, keys, heads, kv_heads, d, mask, documents, lengths, cap, slopes
+ONE_NODE = [
+    (3, 200, 200, 2, 1, 64, "causal", True, (200, 64, 131), 0.0, False),
+    (3, 260, 260, 2, 2, 128, "none", True, (0, 260, 77), 0.0, False),
+    (2, 140, 300, 4, 2, 40, "prefix", True, (170, 290), 20.0, True),
+    (2, 300, 140, 2, 2, 72, "causal", True, None, 0.0, False),         # more queries than keys: the first have no position
+    (4, 3, 90, 4, 2, 64, "causal", True, (1, 90, 50, 20), 0.0, False),
+    (2, 1, 900, 4, 4, 128, "causal", True, (700, 300), 0.0, True),
+    (2, 40, 1100, 2, 1, 64, "causal", True, (1000, 500), 0.0, False),
+]
+
+
+@pytest.mark.parametrize("prec", PRECS)
+@pytest.mark.parametrize("case", ONE_NODE)
+def test_documents_in_one_node_go_by_position(device, case, prec):
+    x, t, more, sl, _, _, scale = attention_case(case, prec, seed=23)
+    b, s, n = case[:3]
+    del more["qdoc"]
+    lengths = np.full(b, n) if "lengths" not in more else more["lengths"]
+    at = (lengths - s)[:, None] + np.arange(s)
+    qdoc = np.where(at < 0, -1, np.take_along_axis(more["kdoc"], np.maximum(at, 0), 1))
+    seen, pos = R.visible(b, s, n, case[6], more.get("prefix"), qdoc, more["kdoc"], more.get("lengths"))
+    out, lse, size, flat = R.attention(x["q"], x["k"], x["v"], seen, pos, scale, t["cap"], sl)
+    assert seen.any() and not np.isneginf(lse).all()
+    nodes, op = link_attention(device, case, prec, {m: x[m] for m in "qkv"}, t, more, sl, "aligned")
+    op = relink(nodes, op, t, more, sl, False, documents="kdoc")
+    op.run()
+    device.await_()
+    R.within(nodes.read("out"), out, out_bound(prec, out, size, flat), "out")
+    R.within(nodes.read("lse"), lse, R.ARITH * (1 + np.abs(np.where(np.isinf(lse), 0, lse))), "lse")
+    op.free()
+    nodes.free()
+    x["out"], x["lse"] = R.rounded(prec, out), R.rounded("single", lse)
+    want = R.attention_grad(x["q"], x["k"], x["v"], x["out"], x["lse"], x["d_out"], seen, pos, scale, t["cap"], sl, prec)
+    nodes, op = link_attention(device, case, prec, x, t, more, sl, "aligned", grad=True)
+    op = relink(nodes, op, t, more, sl, True, documents="kdoc")
+    op.run()
+    device.await_()
+    for m, (v, bound) in zip(("dq", "dk", "dv"), want):
+        R.within(nodes.read(m), v, bound, m)
+    op.free()
+    nodes.free()
