@@ -8,6 +8,9 @@
 // grown by more than 2^8 (weights stay below that, sums and accumulators are single precision, so nothing is lost): after the
 // first tiles hardly ever.  With NQ = 2 the two tiles take turns on the tensor cores and on the arithmetic; with NQ = 1 two CTAs of an SM do.
 //
+// Over more than kSumKeys keys (SUMS) the accumulators are added to sums in the workspace every so many tiles, and cleared.  (In all
+// kernels, never taken, the branch cost 5 % of the shorter rows' time.)
+//
 // Key tiles that no query of a tile sees are skipped, and those that all see take no mask: known from the rows' last keys alone, or, with
 // documents, from classes made first for all key tiles from the range of document numbers in each.
 //
@@ -191,7 +194,7 @@ struct FwdShape {
   static constexpr size_t smem(int tiles) { return 1024 + kBytes + 512 + (size_t)tiles; }
 };
 
-template <class T, int DP, int NQ, int KW, bool CAP, bool BIAS>
+template <class T, int DP, int NQ, int KW, bool CAP, bool BIAS, bool SUMS>
 __global__ void __launch_bounds__(NQ * 128 + 64, NQ == 1 ? 2 : 1)
 attn_forward_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant__ b200_tmap map_k, const __grid_constant__ b200_tmap map_v,
                 const __grid_constant__ b200_tmap map_o, const __grid_constant__ AttnArgs a) {
@@ -427,6 +430,11 @@ attn_forward_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant__
     const float unit = BIAS ? 1.f : c;
     unsigned int seen = 0;
     bool live = true;
+    // the sums in memory: the maximum that they are relative to, and what they have to be multiplied by
+    constexpr unsigned int kSumTiles = kSumKeys / KW;
+    [[maybe_unused]] float m_sum = -INFINITY;
+    [[maybe_unused]] auto sums_at = [&](int e) { return (float4*)(a.sums + (((long long)b * a.H + h) * a.S + r) * DP + e); };
+    [[maybe_unused]] auto since = [&]() { return m_sum == m ? 1.f : m_sum == -INFINITY ? 0.f : ex2(m_sum - m); };
     for (int t = 0; t < n_tiles && live; ++t) {
       const unsigned int cls = docs ? (classes[t] >> (2 * g)) & 3u : tile_class(mine_span, t * KW, KW, false, 0, 0, false);
       if (!cls) continue;
@@ -461,6 +469,32 @@ attn_forward_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant__
       if (CAP || BIAS || cls == 2u) tmem_wait_st();
       b200_tmem_ld32(at, (unsigned int*)x[0]);
       const float m_tile = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * unit;
+      if constexpr (SUMS)
+        if (seen && seen % kSumTiles == 0) {
+          // (the product before is waited for as below)
+          if (Sh::kScores == 2) {
+            live = b200_wait(bar_o + 8 * g, (seen - 1) & 1u, abort_flag, a.status, 49u);
+            tc_after();
+          }
+          const float by = since();
+#pragma unroll
+          for (int e = 0; e < DP; e += 32) {
+            float o[32];
+            b200_tmem_ld32(mine_o + e, (unsigned int*)o);
+            tmem_wait_ld();
+            if (r < a.S)
+#pragma unroll
+              for (int j = 0; j < 32; j += 4) {
+                float4* to = sums_at(e + j);
+                const float4 w = seen > kSumTiles && by != 0.f ? *to : make_float4(0.f, 0.f, 0.f, 0.f);
+                *to = make_float4(fmaf(w.x, by, o[j]), fmaf(w.y, by, o[j + 1]), fmaf(w.z, by, o[j + 2]), fmaf(w.w, by, o[j + 3]));
+              }
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] = 0.f;
+            b200_tmem_st32(mine_o + e, (unsigned int*)o);
+          }
+          m_sum = m;
+        }
       // the maximum in use moves when some row of the warp has outgrown it (or has had none)
       if (__any_sync(0xffffffffu, m_tile > m + 8.f || (m == -INFINITY && m_tile != -INFINITY))) {
         const float m_new = fmaxf(m, m_tile);
@@ -530,6 +564,19 @@ attn_forward_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant__
         b200_tmem_ld32(mine_o + e, (unsigned int*)o);
         tmem_wait_ld();
       }
+      if constexpr (SUMS)
+        if (seen > kSumTiles && r < a.S) {
+          const float before = since();
+          if (before != 0.f)
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) {
+              const float4 w = *sums_at(e + j);
+              o[j] = fmaf(w.x, before, o[j]);
+              o[j + 1] = fmaf(w.y, before, o[j + 1]);
+              o[j + 2] = fmaf(w.z, before, o[j + 2]);
+              o[j + 3] = fmaf(w.w, before, o[j + 3]);
+            }
+        }
 #pragma unroll
       for (int j = 0; j < 32; ++j) {
         o[j] = by == 0.f ? 0.f : o[j] * by;

@@ -15,6 +15,7 @@ struct AttnArgs {
   void *out, *dq, *dk, *dv;
   float* lse;                            // [batch, heads, queries]
   float* stat;                           // gradient: a tile of 128 queries of a head: lse / log 2 of each, then <d_out, out>
+  float* sums;                           // forward, over more than kSumKeys keys: [batch, heads, queries] rows of 64 or 128
   float* parts;                          // gradient, with `n_parts` > 1: a part's dk, then dv, of [batch, keys, kv_heads] rows of 64 or 128
   int n_parts, part_heads;               // blocks that share a key tile, query heads of each
   float* norms;                          // gradient, half: largest squares of a row of d_out, n_norms of them
@@ -27,6 +28,10 @@ struct AttnArgs {
   float scale, cap, over;                // over: scale / cap
   Divisor all_heads, heads, all_key_heads, key_heads, per_key_head, parts_of;    // of a block's number: B H, H, B HK, HK, H / HK, n_parts
 };
+
+// The tensor cores cut an accumulation off instead of rounding it: some 2^-22 for 16 keys, 0.7 % over a million of them where all
+// products have one sign.  So after this many keys the accumulators are added to sums in memory and start again: 2^-13 at most.
+constexpr int kSumKeys = 16384;
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 

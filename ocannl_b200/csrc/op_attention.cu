@@ -159,14 +159,14 @@ typedef void (*AttnKernel)(const AttnArgs);
 typedef void (*ForwardKernel)(const b200_tmap, const b200_tmap, const b200_tmap, const b200_tmap, const AttnArgs);
 
 // (two query tiles: key tiles of 64 where scores are capped, of 128 else)
-template <class T, int DP, int NQ, int KW>
+template <class T, int DP, int NQ, int KW, bool SUMS>
 ForwardKernel forward_of(bool cap, bool bias) {
   if constexpr (NQ == 2) {
     constexpr bool kCap = KW == 64;
-    return bias ? attn_forward_tc<T, DP, NQ, KW, kCap, true> : attn_forward_tc<T, DP, NQ, KW, kCap, false>;
+    return bias ? attn_forward_tc<T, DP, NQ, KW, kCap, true, SUMS> : attn_forward_tc<T, DP, NQ, KW, kCap, false, SUMS>;
   } else {
-    if (cap) return bias ? attn_forward_tc<T, DP, NQ, KW, true, true> : attn_forward_tc<T, DP, NQ, KW, true, false>;
-    return bias ? attn_forward_tc<T, DP, NQ, KW, false, true> : attn_forward_tc<T, DP, NQ, KW, false, false>;
+    if (cap) return bias ? attn_forward_tc<T, DP, NQ, KW, true, true, SUMS> : attn_forward_tc<T, DP, NQ, KW, true, false, SUMS>;
+    return bias ? attn_forward_tc<T, DP, NQ, KW, false, true, SUMS> : attn_forward_tc<T, DP, NQ, KW, false, false, SUMS>;
   }
 }
 
@@ -262,7 +262,7 @@ struct AttnOperator : b200_operator {
     const bool pad = tc && !plain;
     if (pad)
       for (auto& n : nodes) n.at = reserve((size_t)(n.of_keys ? key_rows : rows) * ld * 2);
-    size_t stat = 0, norms = 0, parts = 0, tickets = 0;
+    size_t stat = 0, norms = 0, parts = 0, tickets = 0, sums = 0;
     a.n_parts = 1;
     a.part_heads = a.group;
     if (tc && grad) {
@@ -276,6 +276,8 @@ struct AttnOperator : b200_operator {
     }
     a.parts_of = Divisor((unsigned int)a.n_parts);
     if (tc && !grad && few_rows()) choose_few(&parts, &tickets);
+    const bool summed = tc && !grad && !few && a.T > kSumKeys;
+    if (summed) sums = reserve((size_t)rows * (a.D <= 64 ? 64 : 128) * 4);
     if (grad && rows) {
       const long long padded = (long long)a.B * a.H * ((a.S + 127) / 128) * 128;
       const int size = (int)dtype_bytes(dtype);
@@ -318,6 +320,7 @@ struct AttnOperator : b200_operator {
       }
       a.ld = ld;
     }
+    if (summed) a.sums = (float*)(workspace + sums);
     if (a.n_parts > 1) {
       a.parts = (float*)(workspace + parts);
       join = by_type(dtype, [&](auto t) -> AttnKernel {
@@ -441,7 +444,7 @@ struct AttnOperator : b200_operator {
   }
   template <class T, int DP, int NQ, int KW>
   void set() {
-    forward = forward_of<T, DP, NQ, KW>(a.cap > 0.f, a.slopes != nullptr);
+    forward = a.sums ? forward_of<T, DP, NQ, KW, true>(a.cap > 0.f, a.slopes != nullptr) : forward_of<T, DP, NQ, KW, false>(a.cap > 0.f, a.slopes != nullptr);
     threads = FwdShape<DP, NQ, KW>::kThreads;
     smem = FwdShape<DP, NQ, KW>::smem((a.T + KW - 1) / KW);
     map_k = of_keys(a.k, KW);

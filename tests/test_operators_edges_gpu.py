@@ -111,3 +111,32 @@ def test_documents_in_one_node_go_by_position(device, case, prec):
         R.within(nodes.read(m), v, bound, m)
     op.free()
     nodes.free()
+
+
+@pytest.mark.parametrize("prec", ("bfloat16", "half"))
+@pytest.mark.parametrize("queries,d,heads", [(1, 8, 1), (130, 8, 1), (130, 72, 1), (260, 128, 149)])
+def test_sums_over_a_million_keys(device, queries, d, heads, prec):
+    """Equal weights of one: the output is the values' mean, rounded once, however many keys there are."""
+    n = 1_000_003 if heads == 1 else 100_003
+    rng = np.random.default_rng(37)
+    v = R.rounded(prec, 1.0 + rng.random((1, n, 1, d)))
+    zero, q = np.zeros((1, n, 1, d)), np.zeros((1, queries, heads, d))
+    nodes = R.Nodes(device, dict(q=(prec, q.shape, q), k=(prec, zero.shape, zero), v=(prec, v.shape, v), out=(prec, q.shape, None), lse=("single", (1, heads, queries), None)))
+    op = nodes.context.attention("q", "k", "v", "out", lse="lse", mask="none")
+    for _ in range(2):
+        op.run()
+    device.await_()
+    want = np.broadcast_to(v.mean(1, keepdims=True), q.shape)
+    R.within(nodes.read("out"), want, (R.EPS[prec] / 2 + 2.0 ** -12) * want, "out")
+    R.within(nodes.read("lse"), np.full((1, heads, queries), np.log(n)), R.ARITH * 15, "lse")
+    op.free()
+    nodes.free()
+
+
+@pytest.mark.parametrize("prec", ("bfloat16", "half"))
+@pytest.mark.parametrize("case", [(1, 150, 40000, 1, 1, 16, "causal", False, None, 0.0, True), (1, 130, 34000, 1, 1, 72, "prefix", True, None, 20.0, False)])
+def test_sums_over_many_keys_of_different_weights(device, case, prec):
+    """Maxima that move between the times when accumulators are added to the sums; places that are not seen."""
+    x, t, more, sl, seen, pos, scale = attention_case(case, prec, seed=41)
+    x["k"] = R.rounded(prec, x["k"] * np.linspace(0.2, 3.0, case[2])[None, :, None, None])
+    check_forward(device, case, prec, x, t, more, sl, seen, pos, scale)
