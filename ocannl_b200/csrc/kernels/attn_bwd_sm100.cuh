@@ -185,7 +185,7 @@ __device__ __forceinline__ void attn_grad_keys(const b200_tmap& map_q, const b20
   tc_before();
   __syncthreads();
   tc_after();
-  const float grad_unit = gradient_unit<T>(a, scratch);
+  const float grad_unit = gradient_unit<T>(a, scratch), to_unit = grad_unit * kWeightBack<T>;
   if (docs) {
     int kmin[1], kmax[1];
     bool negative[1];
@@ -383,7 +383,7 @@ __device__ __forceinline__ void attn_grad_keys(const b200_tmap& map_q, const b20
 #pragma unroll
               for (int q = 0; q < 4; ++q) {
                 float ds = w[32 * k + i + q] * (x[i + q] - delta[q]);
-                if constexpr (std::is_same<T, __half>::value) ds *= grad_unit;
+                if constexpr (std::is_same<T, __half>::value) ds *= to_unit;
                 if constexpr (M) ds = (bits[k] >> (i + q)) & 1u ? ds : 0.f;
                 x[i + q] = ds;
               }
@@ -411,7 +411,7 @@ __device__ __forceinline__ void attn_grad_keys(const b200_tmap& map_q, const b20
       if (Sh::kGroups == 2 && which != (int)half) continue;
       const unsigned int from = (which ? t_dk : t_dv) + lanes;
       unsigned char* tile = gen + (which ? 0 : Sh::kTile);
-      const float by = which ? a.scale / grad_unit : 1.f;
+      const float by = which ? a.scale / grad_unit : kWeightBack<T>;
       bool fine = true;
 #pragma unroll
       for (int e = 0; e < DP; e += 32) {
@@ -533,7 +533,7 @@ __device__ __forceinline__ void attn_grad_queries(const b200_tmap& map_q, const 
   tc_before();
   __syncthreads();
   tc_after();
-  const float grad_unit = gradient_unit<T>(a, scratch);
+  const float grad_unit = gradient_unit<T>(a, scratch), to_unit = grad_unit * kWeightBack<T>;
   if (docs) {
     if (warp < 4) {
       const AttnSpan s = span_of(r < a.S, row);
@@ -667,7 +667,7 @@ __device__ __forceinline__ void attn_grad_queries(const b200_tmap& map_q, const 
             if constexpr (!BIAS) p = ex2(fmaf(x[i], c, -lse2));
             else p = ex2(pair_score<BIAS>(x[i], c, slope2, far - (float)i) - lse2);
             if constexpr (M) p = (bits[k] >> i) & 1u ? p : 0.f;
-            if constexpr (std::is_same<T, __half>::value) p *= grad_unit;
+            if constexpr (std::is_same<T, __half>::value) p *= to_unit;
             w[32 * k + i] = CAP ? p * fmaf(-x[i], x[i], 1.f) : p;
           }
         }

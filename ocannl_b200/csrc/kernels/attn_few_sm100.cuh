@@ -15,7 +15,7 @@ namespace b200 {
 constexpr int kFewRows = 16, kFewStep = 16, kFewStages = 3, kFewWarps = 4, kFewMost = 256;   // (most ranges)
 
 struct FewArgs {
-  float* parts;            // [pair][split][16][DP + 4]: output (not divided), maximum, sum, and two floats that keep rows on 16 bytes
+  float* parts;            // [pair][split][16][DP + 4]: output (not divided), maximum, sum (both of half weights times 2^7), and two floats that keep rows on 16 bytes
   unsigned int* tickets;   // [pair], zero between runs
   int splits, per_split;   // keys of a range, a multiple of 16 * 4
   int join_later;          // the ranges are joined by a launch of its own
@@ -112,7 +112,7 @@ __device__ __forceinline__ bool few_finish(const AttnArgs& a, int b, int h, int 
       from_float(y[k], to[k]);
       fine = fine && y[k] * 0.f == 0.f;
     }
-  if (e == 0 && a.lse) a.lse[((long long)b * a.H + h) * a.S + r] = by != 0.f ? (top + log2f(sum)) * kLn2 : -INFINITY;
+  if (e == 0 && a.lse) a.lse[((long long)b * a.H + h) * a.S + r] = by != 0.f ? (top - kLift<T> + log2f(sum)) * kLn2 : -INFINITY;
   return fine;
 }
 // One row by a block: each of the four warps adds every fourth part, the first adds the four sums.
@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) attn_forward_few(const __grid_
         }
       }
     }
-    const float off[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+    const float off[2] = {m[0] == -INFINITY ? 0.f : m[0] - kLift<T>, m[1] == -INFINITY ? 0.f : m[1] - kLift<T>};
     // weights as the A operand: rows ra, rb, keys 0-7 and 8-15
     unsigned int p[4];
 #pragma unroll

@@ -72,6 +72,11 @@ __device__ __forceinline__ void tanh_chunk(float (&x)[N], float scale) {
   }
 }
 
+// Weights are at most 2^8 (the maximum in use may lag by that).  Half ones are multiplied by 2^7 more, which the row's sum has too: those
+// down to 2^-21 of the largest are then normal numbers.  (Many keys of 2^-20 beside one of 1 kept four bits: outputs were 3 % off.)
+template <class T>
+constexpr float kLift = std::is_same<T, __half>::value ? 7.f : 0.f;
+
 // A from tensor memory: 16-bit elements, two to a column
 __device__ __forceinline__ void umma_ts(unsigned int d, unsigned int a, unsigned long long b, unsigned int idesc, unsigned int accumulate) {
   asm volatile(
@@ -519,7 +524,7 @@ attn_forward_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant__
         l *= by;
         m = m_new;
       }
-      const float off = m == -INFINITY ? 0.f : -m;
+      const float off = m == -INFINITY ? 0.f : kLift<T> - m;
       Pair part[2] = {Pair(0.f, 0.f), Pair(0.f, 0.f)};
       const Pair unit2(unit, unit), off2(off, off);
       // second pass: the weights, over the scores that have been read
@@ -589,7 +594,7 @@ attn_forward_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant__
         *(uint4*)(line + (((piece0 + p) ^ (in & 7u)) << 4)) =
             make_uint4(pack2(o[8 * p], o[8 * p + 1], T()), pack2(o[8 * p + 2], o[8 * p + 3], T()), pack2(o[8 * p + 4], o[8 * p + 5], T()), pack2(o[8 * p + 6], o[8 * p + 7], T()));
     }
-    if (live && r < a.S && a.lse) a.lse[((long long)b * a.H + h) * a.S + r] = l > 0.f || l != l ? (m + log2f(l)) * kLn2 : -INFINITY;
+    if (live && r < a.S && a.lse) a.lse[((long long)b * a.H + h) * a.S + r] = l > 0.f || l != l ? (m - kLift<T> + log2f(l)) * kLn2 : -INFINITY;
     // every warp sends its 32 rows; those with a value that is infinite or undefined are done again, one by one
     const int first = r0 + (int)warp * 32;
     const unsigned int mend = __ballot_sync(0xffffffffu, live && r < a.S && bad != 0.f);

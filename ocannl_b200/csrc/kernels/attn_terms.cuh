@@ -89,7 +89,14 @@ __device__ __forceinline__ float attn_score(const AttnArgs& a, float x, float sl
   return fmaf(-slope2, fabsf((float)(pos - j)), s);
 }
 
-// Where a row's statistics lie: its lse (log 2 units; +infinity for a row that sees nothing: all weights are zero), 128 further <d_out, out>
+// Gradients of half heads have weights times 2^14, which their results give back: p is at most 1, and about 1 / keys in long rows (at a
+// million keys a half has four bits of it, and dv was 1.4 % off).  The factor comes with the statistics: lse less 14.
+template <class T>
+constexpr float kWeightLog = std::is_same<T, __half>::value ? 14.f : 0.f;
+template <class T>
+constexpr float kWeightBack = std::is_same<T, __half>::value ? 1.f / 16384.f : 1.f;
+
+// Where a row's statistics lie: its lse (log 2 units, less kWeightLog; +infinity for a row that sees nothing: all weights are zero), 128 further <d_out, out>
 __device__ __forceinline__ long long attn_stat_at(const AttnArgs& a, int b, int h, int r) {
   return (((long long)b * a.H + h) * ((a.S + 127) / 128) + (r >> 7)) * 256 + (r & 127);
 }
@@ -160,7 +167,7 @@ __device__ __noinline__ void attn_dq_row(const AttnArgs& a, int b, int h, int r,
   const float slope2 = a.slopes ? a.slopes[h] * kLog2e : 0.f;
   const int hk = h / a.group;
   const long long at = attn_q_at(a, b, r, h), stat = attn_stat_at(a, b, h, r);
-  const float lse2 = a.stat[stat], delta = a.stat[stat + 128];
+  const float lse2 = a.stat[stat] + kWeightLog<T>, delta = a.stat[stat + 128];
   float q[4], k[4], v[4], go[4], g[4] = {0.f, 0.f, 0.f, 0.f}, p, dx;
   attn_load_row<T>(a, a.q, at, lane, q);
   attn_load_row<T>(a, a.d_out, at, lane, go);
@@ -192,7 +199,7 @@ __device__ __noinline__ void attn_dkv_row(const AttnArgs& a, int b, int hk, int 
       const long long at = attn_q_at(a, b, r, h), stat = attn_stat_at(a, b, h, r);
       attn_load_row<T>(a, a.q, at, lane, q);
       attn_load_row<T>(a, a.d_out, at, lane, go);
-      attn_pair(a, attn_dot(q, k), attn_dot(go, v), slope2, w.pos, j, a.stat[stat], a.stat[stat + 128], p, dx);
+      attn_pair(a, attn_dot(q, k), attn_dot(go, v), slope2, w.pos, j, a.stat[stat] + kWeightLog<T>, a.stat[stat + 128], p, dx);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         gk[i] = fmaf(dx, q[i], gk[i]);

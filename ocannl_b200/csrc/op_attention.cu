@@ -89,7 +89,7 @@ __global__ void __launch_bounds__(256) attn_statistics(const __grid_constant__ A
       const bool empty = lse[k] == -INFINITY;
       if (!empty) top = fmaxf(top, square);
       if (lane == 0 && base + k * rows < n) {
-        a.stat[stat[k]] = empty ? INFINITY : lse[k] * kLog2e;
+        a.stat[stat[k]] = empty ? INFINITY : lse[k] * kLog2e - kWeightLog<T>;
         a.stat[stat[k] + 128] = empty ? 0.f : delta;
       }
     }

@@ -140,3 +140,47 @@ def test_sums_over_many_keys_of_different_weights(device, case, prec):
     x, t, more, sl, seen, pos, scale = attention_case(case, prec, seed=41)
     x["k"] = R.rounded(prec, x["k"] * np.linspace(0.2, 3.0, case[2])[None, :, None, None])
     check_forward(device, case, prec, x, t, more, sl, seen, pos, scale)
+
+
+@pytest.mark.parametrize("prec", ("bfloat16", "half"))
+@pytest.mark.parametrize("queries", (1, 130))
+def test_many_small_weights_beside_a_large_one(device, queries, prec):
+    """A million keys of weight 2^-20 of the largest, which has the value 0: small weights keep the bits of their type."""
+    n, d = 1_000_003, 8
+    rng = np.random.default_rng(29)
+    k, v = np.zeros((1, n, 1, d)), R.rounded(prec, 1.0 + rng.random((1, n, 1, d)))
+    q = np.zeros((1, queries, 1, d))
+    q[..., 0], k[0, 5, 0, 0], v[0, 5] = 1.0, 13.875, 0.0
+    nodes = R.Nodes(device, dict(q=(prec, q.shape, q), k=(prec, k.shape, k), v=(prec, v.shape, v), out=(prec, q.shape, None), lse=("single", (1, 1, queries), None)))
+    op = nodes.context.attention("q", "k", "v", "out", lse="lse", mask="none", scale=1.0)
+    op.run()
+    device.await_()
+    small = np.exp(-13.875)
+    total = 1.0 + (n - 1) * small
+    want = v.sum(1, keepdims=True) * small / total
+    # weights and the output are rounded once each; the sums in single precision
+    R.within(nodes.read("out"), np.broadcast_to(want, q.shape), (R.EPS[prec] + R.ARITH) * want, "out")
+    R.within(nodes.read("lse"), np.full((1, 1, queries), 13.875 + np.log(total)), R.ARITH * 15, "lse")
+    op.free()
+    nodes.free()
+
+
+@pytest.mark.parametrize("prec", ("bfloat16", "half"))
+def test_gradients_of_values_of_many_keys(device, prec):
+    """Weights of one in a million, alike for all keys: dv is the sum of d_out's rows over a million."""
+    n, s, d = 1_000_003, 130, 8
+    rng = np.random.default_rng(31)
+    do = R.rounded(prec, 1000.0 * (1.0 + rng.random((1, s, 1, d))))
+    v = R.rounded(prec, rng.standard_normal((1, n, 1, d)))
+    out = R.rounded(prec, np.broadcast_to(v.mean(1, keepdims=True), do.shape))
+    zero, q = np.zeros((1, n, 1, d)), np.zeros((1, s, 1, d))
+    nodes = R.Nodes(device, dict(q=(prec, q.shape, q), k=(prec, zero.shape, zero), v=(prec, v.shape, v), out=(prec, q.shape, out), d_out=(prec, q.shape, do),
+                                 lse=("single", (1, 1, s), np.full((1, 1, s), np.log(n))), dq=(prec, q.shape, None), dk=(prec, zero.shape, None), dv=(prec, zero.shape, None)))
+    op = nodes.context.attention_grad("q", "k", "v", "out", "lse", "d_out", "dq", "dk", "dv", mask="none")
+    op.run()
+    device.await_()
+    want = np.broadcast_to(do.sum(1, keepdims=True) / n, zero.shape)
+    R.within(nodes.read("dv"), want, (R.EPS[prec] + R.ARITH) * want, "dv")
+    assert not nodes.read("dq").any() and not nodes.read("dk").any()
+    op.free()
+    nodes.free()
