@@ -57,8 +57,7 @@ __device__ __forceinline__ void bulk_load(unsigned int dst, const void* src, uns
 
 // Which of the 64 queries from r0 see key j, a bit each (bits of queries behind the last one are of no account: their weights are zero).
 // Without documents a key is seen from one query on.
-__device__ __forceinline__ void visible_queries(const AttnArgs& a, int b, int r0, int j, unsigned int lane, unsigned int (&bits)[2]) {
-  const AttnSeq seq = attn_seq(a, b);
+__device__ __forceinline__ void visible_queries(const AttnArgs& a, const AttnSeq& seq, int b, int r0, int j, unsigned int lane, unsigned int (&bits)[2]) {
   int first = 0;
   if (j >= seq.len) first = 0x7fffffff;
   else if (a.mask == B200_MASK_CAUSAL || (a.mask == B200_MASK_PREFIX && j >= seq.prefix)) first = max(0, j - (seq.len - a.S));
@@ -73,11 +72,12 @@ __device__ __forceinline__ void visible_queries(const AttnArgs& a, int b, int r0
     bits[i] = n <= 0 ? 0xffffffffu : n >= 32 ? 0u : 0xffffffffu << n;
   }
   if (!a.kdoc) return;
+  const AttnQueryDocs theirs(a, seq, b);
   int d[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int r = r0 + (int)lane + 32 * i;
-    d[i] = r < a.S ? attn_query_document(a, seq, b, r) : -1;
+    d[i] = r < a.S ? theirs.of(r) : -1;
   }
   unsigned int todo = 0xffffffffu;
   while (todo) {
@@ -190,6 +190,7 @@ __device__ __forceinline__ void attn_grad_keys(const b200_tmap& map_q, const b20
     int kmin[1], kmax[1];
     bool negative[1];
     key_documents<128, 1>(a, b, j0 / 128, 0, lane, kmin, kmax, negative);
+    const AttnQueryDocs theirs(a, seq, b);
     constexpr int kAhead = 4;
     for (int t0 = (int)warp; t0 < tiles; t0 += kAhead * (int)Sh::kWarps) {
       int d[kAhead][CW / 32];
@@ -198,7 +199,7 @@ __device__ __forceinline__ void attn_grad_keys(const b200_tmap& map_q, const b20
 #pragma unroll
         for (int i = 0; i < CW / 32; ++i) {
           const long long r = (long long)(t0 + n * (int)Sh::kWarps) * CW + 32 * i + lane;
-          d[n][i] = r < a.S ? attn_query_document(a, seq, b, (int)r) : -1;
+          d[n][i] = r < a.S ? theirs.of((int)r) : -1;
         }
 #pragma unroll
       for (int n = 0; n < kAhead; ++n) {
@@ -325,7 +326,7 @@ __device__ __forceinline__ void attn_grad_keys(const b200_tmap& map_q, const b20
         const float* stat = (const float*)(gen + 2 * Sh::kTile + (n & 1u) * Sh::kStage + 2 * Sh::kStep) + 64 * half;
         unsigned int bits[2] = {0xffffffffu, 0xffffffffu};
         const int r0 = t * CW + 64 * (int)half;
-        if (cls == 2u) visible_queries(a, b, r0, j, lane, bits);
+        if (cls == 2u) visible_queries(a, seq, b, r0, j, lane, bits);
         live = b200_wait(bar_full + 8 * (n & 1u), (n >> 1) & 1u, abort_flag, a.status, 37u) && b200_wait(bar_s, n & 1u, abort_flag, a.status, 38u);
         if (!live) break;
         tc_after();

@@ -524,7 +524,7 @@ __device__ __forceinline__ void single_grad_keys(const AttnArgs& a, int vec, int
     next_last = next_doc = -1;
     if ((int)threadIdx.x < span && r < a.S) {
       next_last = attn_last(a, seq, r);
-      next_doc = a.kdoc ? attn_query_document(a, seq, b, r) : 0;
+      next_doc = a.kdoc ? AttnQueryDocs(a, seq, b).of(r) : 0;
       if (next_doc < 0) next_last = -1;
       next_lse2 = a.stat[attn_stat_at(a, b, h, r)];
       next_delta = a.stat[attn_stat_at(a, b, h, r) + 128];

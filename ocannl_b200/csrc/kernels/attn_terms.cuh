@@ -54,12 +54,14 @@ __device__ __forceinline__ int attn_last(const AttnArgs& a, const AttnSeq& s, in
   const int last = a.mask == B200_MASK_NONE ? s.len - 1 : min(s.len - 1, max(s.len - a.S + r, s.prefix - 1));
   return max(last, -1);
 }
-// a query's document: its entry of the queries' documents, or that of the key at its position (no position, no document)
-__device__ __forceinline__ int attn_query_document(const AttnArgs& a, const AttnSeq& s, int b, int r) {
-  if (a.qdoc) return a.qdoc[(long long)b * a.S + r];
-  const int pos = s.len - a.S + r;
-  return pos < 0 ? -1 : a.kdoc[(long long)b * a.T + pos];
-}
+// a sequence's queries' documents: their entries, or those of the keys at their positions (none before the first position)
+struct AttnQueryDocs {
+  const int* at;
+  int first;
+  __device__ __forceinline__ AttnQueryDocs(const AttnArgs& a, const AttnSeq& s, int b)
+      : at(a.qdoc ? a.qdoc + (long long)b * a.S : a.kdoc + ((long long)b * a.T + s.len - a.S)), first(a.qdoc ? 0 : a.S - s.len) {}
+  __device__ __forceinline__ int of(int r) const { return r >= first ? __ldg(at + r) : -1; }
+};
 __device__ __forceinline__ AttnRow attn_row(const AttnArgs& a, int b, int r) {
   const AttnSeq s = attn_seq(a, b);
   AttnRow w;
@@ -67,7 +69,7 @@ __device__ __forceinline__ AttnRow attn_row(const AttnArgs& a, int b, int r) {
   w.last = attn_last(a, s, r);
   w.doc = 0;
   if (a.kdoc) {
-    w.doc = attn_query_document(a, s, b, r);
+    w.doc = AttnQueryDocs(a, s, b).of(r);
     if (w.doc < 0) w.last = -1;
   }
   return w;
