@@ -32,23 +32,28 @@ struct BwdShape {
   static constexpr size_t smem(int tiles) { return 1024 + kBytes + 256 + (size_t)tiles; }
 };
 
-// Half gradients of scores are multiplied by a power of two before they are rounded, so that those of 2^-20 of the largest
-// row of d_out still lie in the normal range: 2^6 over the largest norm of a row of d_out (of the rows that see something).
-// `norms`: the squares of the largest norms, one a block of the statistics kernel.
-template <class T>
-__device__ __forceinline__ float gradient_unit(const AttnArgs& a, float* sh) {
-  if constexpr (std::is_same<T, __half>::value) {
-    float m = 0.f;
-    for (int i = (int)threadIdx.x; i < a.n_norms; i += (int)blockDim.x) m = fmaxf(m, a.norms[i]);
+// Half gradients of scores are multiplied by a power of two before they are rounded, a row's own: ds = p <d_out, v - out> is at most
+// |d_out| |v| + |d_out| |out|, and the power brings that bound between 2^13 and 2^14.  A query's row has its own |d_out| and the largest
+// |v| of the tiles it sees; a key's its own |v| and the largest |d_out| and |d_out| |out| of them.  So p may be 2^-20 before the first
+// bits are lost, whatever the sizes of d_out and v, and other rows, heads and sequences have no say in it.
+// (One power for the whole call, of the largest |d_out|, left 3 % of a gradient wrong beside a row 10^4 times as large.)
+__device__ __forceinline__ float unit_of(float bound) {
+  return bound > 0.f && bound < INFINITY ? exp2f(fminf(fmaxf(floorf(14.f - log2f(bound)), -60.f), 60.f)) : 1.f;
+}
+// the largest of each of N values of the softmax threads; `sh`: N floats a warp, used once
+template <int WARPS, int N>
+__device__ __forceinline__ void largest(float (&v)[N], float* sh) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if ((threadIdx.x & 31u) == 0) sh[threadIdx.x >> 5] = m;
-    __syncthreads();
-    for (unsigned int i = 0; i < blockDim.x / 32; ++i) m = fmaxf(m, sh[i]);
-    __syncthreads();
-    return m > 0.f && m < INFINITY ? exp2f(fminf(fmaxf(floorf(6.f - 0.5f * log2f(m)), -60.f), 60.f)) : 1.f;
+  for (int n = 0; n < N; ++n) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v[n] = fmaxf(v[n], __shfl_xor_sync(0xffffffffu, v[n], o));
+    if ((threadIdx.x & 31u) == 0) sh[n * WARPS + (threadIdx.x >> 5)] = v[n];
   }
-  return 1.f;
+  named_barrier(5, WARPS * 32);
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int i = 0; i < WARPS; ++i) v[n] = fmaxf(v[n], sh[n * WARPS + i]);
 }
 
 __device__ __forceinline__ void bulk_load(unsigned int dst, const void* src, unsigned int bytes, unsigned int bar) {
@@ -130,7 +135,7 @@ __device__ __forceinline__ void attn_grad_keys(const b200_tmap& map_q, const b20
   const unsigned int bar_s = bar0 + 40, bar_dp = bar0 + 48, bar_p = bar0 + 56, bar_ds = bar0 + 64, bar_done = bar0 + 72;
   volatile unsigned int* tmem_slot = (volatile unsigned int*)(bars + 10);
   volatile unsigned int* abort_flag = tmem_slot + 1;
-  float* scratch = (float*)(bars + 12);                   // [10]
+  float* scratch = (float*)(bars + 12);                   // [16]
   unsigned char* classes = (unsigned char*)(gen + Sh::kBytes + 256);
 
   asm volatile("griddepcontrol.launch_dependents;");
@@ -185,7 +190,6 @@ __device__ __forceinline__ void attn_grad_keys(const b200_tmap& map_q, const b20
   tc_before();
   __syncthreads();
   tc_after();
-  const float grad_unit = gradient_unit<T>(a, scratch), to_unit = grad_unit * kWeightBack<T>;
   if (docs) {
     int kmin[1], kmax[1];
     bool negative[1];
@@ -316,6 +320,24 @@ __device__ __forceinline__ void attn_grad_keys(const b200_tmap& map_q, const b20
     const unsigned int my_s = t_s + 64 * half + lanes, my_dp = t_dp + 64 * half + lanes;
     const float c = CAP ? a.cap * kLog2e : a.scale * kLog2e, to_tanh = CAP ? a.over : 0.f;
     const int j = j0 + (int)in;
+    float grad_unit = 1.f;
+    if constexpr (std::is_same<T, __half>::value) {
+      float most[2] = {0.f, 0.f};
+      for (int h = first_head; h < first_head + a.part_heads; ++h) {
+        const float2* sizes = a.row_sizes + ((long long)b * a.H + h) * stat_tiles * 128;
+#pragma unroll 8
+        for (int r = begin * CW + (int)threadIdx.x; r < tiles * CW; r += Sh::kGroups * 128)
+          if (!docs || classes[r / CW]) {
+            const float2 s = sizes[r];
+            most[0] = fmaxf(most[0], s.x);
+            most[1] = fmaxf(most[1], s.y);
+          }
+      }
+      const float of_v = j < a.T ? a.value_sizes[((long long)b * a.T + j) * a.HK + hk] : 0.f;
+      largest<Sh::kGroups * 4>(most, scratch);
+      grad_unit = unit_of(fmaf(most[0], of_v, most[1]));
+    }
+    const float to_unit = grad_unit * kWeightBack<T>;
     unsigned int n = 0;
     bool live = true;
     for (int h = first_head; h < first_head + a.part_heads && live; ++h) {
@@ -479,7 +501,7 @@ __device__ __forceinline__ void attn_grad_queries(const b200_tmap& map_q, const 
   const unsigned int bar_dp = bar0 + 56, bar_ds = bar0 + 64, bar_done = bar0 + 72;
   volatile unsigned int* tmem_slot = (volatile unsigned int*)(bars + 10);
   volatile unsigned int* abort_flag = tmem_slot + 1;
-  float* scratch = (float*)(bars + 12);
+  float* scratch = (float*)(bars + 12);                   // [8]
   AttnSpan* span = (AttnSpan*)(bars + 18);
   unsigned char* classes = (unsigned char*)(gen + Sh::kBytes + 256);
 
@@ -506,7 +528,8 @@ __device__ __forceinline__ void attn_grad_queries(const b200_tmap& map_q, const 
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const AttnSpan plain = plain_span(a, attn_seq(a, b), r0, 128);
+  const AttnSeq seq = attn_seq(a, b);
+  const AttnSpan plain = plain_span(a, seq, r0, 128);
   int tiles = (plain.last_max + CW) / CW;
   auto load = [&](int t, unsigned int n) {
     const unsigned int slot = n & 1u, at = ring + slot * Sh::kStage, bar = bar_full + 8 * slot;
@@ -534,7 +557,6 @@ __device__ __forceinline__ void attn_grad_queries(const b200_tmap& map_q, const 
   tc_before();
   __syncthreads();
   tc_after();
-  const float grad_unit = gradient_unit<T>(a, scratch), to_unit = grad_unit * kWeightBack<T>;
   if (docs) {
     if (warp < 4) {
       const AttnSpan s = span_of(r < a.S, row);
@@ -641,6 +663,19 @@ __device__ __forceinline__ void attn_grad_queries(const b200_tmap& map_q, const 
     const float slope2 = BIAS ? a.slopes[h] * kLog2e : 0.f;
     const float* stat = a.stat + (((long long)b * a.H + h) * tiles_q + t_q) * 256 + in;
     const float lse2 = stat[0], delta = stat[128];
+    float grad_unit = 1.f;
+    if constexpr (std::is_same<T, __half>::value) {
+      float of_v[1] = {0.f};
+      const float* sizes = a.value_sizes + (long long)b * a.T * a.HK + hk;
+      const int end = min(tiles * CW, seq.len);
+#pragma unroll 8
+      for (int j = (int)threadIdx.x; j < end; j += Sh::kGroups * 128)
+        if (!docs || classes[j / CW]) of_v[0] = fmaxf(of_v[0], sizes[(long long)j * a.HK]);
+      const float2 s = a.row_sizes[(((long long)b * a.H + h) * tiles_q + t_q) * 128 + in];
+      largest<Sh::kGroups * 4>(of_v, scratch);
+      grad_unit = unit_of(fmaf(s.x, of_v[0], s.y));
+    }
+    const float to_unit = grad_unit * kWeightBack<T>;
     unsigned int n = 0;
     bool live = true;
     for (int t = 0; t < tiles; ++t) {

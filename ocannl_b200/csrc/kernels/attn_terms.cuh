@@ -18,8 +18,8 @@ struct AttnArgs {
   float* sums;                           // forward, over more than kSumKeys keys: [batch, heads, queries] rows of 64 or 128
   float* parts;                          // gradient, with `n_parts` > 1: a part's dk, then dv, of [batch, keys, kv_heads] rows of 64 or 128
   int n_parts, part_heads;               // blocks that share a key tile, query heads of each
-  float* norms;                          // gradient, half: largest squares of a row of d_out, n_norms of them
-  int n_norms;
+  float2* row_sizes;                     // gradient, half, tiles of 128 queries of a head: |d_out|, then |d_out| |out|; zeros where nothing is seen
+  float* value_sizes;                    // gradient, half, [batch, keys, kv_heads]: |v|
   const int *lengths, *prefix, *qdoc, *kdoc;   // (kdoc without qdoc: a query has the document of the key at its position)
   const float* slopes;
   unsigned int* status;

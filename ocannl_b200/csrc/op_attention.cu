@@ -24,7 +24,7 @@ __global__ void __launch_bounds__(256) attn_forward_rows(const __grid_constant__
     attn_forward_row<T>(a, (int)(bs / a.S), (int)(i - bs * a.H), (int)(bs % a.S), lane);
   }
 }
-// What the gradients need of every row: its lse and <d_out, out>, tile by tile of 128 queries, G threads a row.  out and d_out are read
+// What the gradients need of every row: its lse and <d_out, out> (and of half heads the sizes of rows and values), tile by tile of 128 queries, G threads a row.  out and d_out are read
 // once, kRowsAtOnce rows of a thread under way together; what bounds it is the arithmetic of indices around 32 bytes a lane, so that
 // is kept to 32 bits (64 x 256 positions, 8 heads of 64: 14.4 us with more of it).  Rows that see nothing get weights of zero; the places
 // behind the last row are filled at link.
@@ -32,14 +32,13 @@ constexpr int kRowsAtOnce = 4;
 
 template <class T, int VEC, int G>
 __global__ void __launch_bounds__(256) attn_statistics(const __grid_constant__ AttnArgs a, const Divisor by_heads, const Divisor by_length) {
-  __shared__ float sh[8];
   grid_begin();
   constexpr unsigned int rows = 256 / G;
+  constexpr bool kSizes = std::is_same<T, __half>::value;
   constexpr int chunks = VEC > 1 ? 1 : 128 / G;
   const int lane = (int)threadIdx.x % G;
   const unsigned int heads = (unsigned int)a.H, length = (unsigned int)a.S, tiles = (length + 127) / 128;
   const unsigned int n = (unsigned int)a.B * length * heads, step = gridDim.x * rows * kRowsAtOnce;
-  float top = 0.f;
   for (unsigned int base = blockIdx.x * rows * kRowsAtOnce + threadIdx.x / G; base - threadIdx.x / G < n; base += step) {
     Raw<T, VEC> x[kRowsAtOnce][chunks], y[kRowsAtOnce][chunks];
     float lse[kRowsAtOnce];
@@ -68,7 +67,7 @@ __global__ void __launch_bounds__(256) attn_statistics(const __grid_constant__ A
     }
 #pragma unroll
     for (int k = 0; k < kRowsAtOnce; ++k) {
-      float delta = 0.f, square = 0.f;
+      float delta = 0.f, of_d_out = 0.f, of_out = 0.f;
 #pragma unroll
       for (int c = 0; c < chunks; ++c) {
         float u[VEC], w[VEC];
@@ -78,30 +77,60 @@ __global__ void __launch_bounds__(256) attn_statistics(const __grid_constant__ A
         for (int q = 0; q < VEC; ++q) {
           // (rows of padded copies end in zeros)
           delta = fmaf(u[q], w[q], delta);
-          if constexpr (std::is_same<T, __half>::value) square = fmaf(w[q], w[q], square);
+          if constexpr (kSizes) {
+            of_d_out = fmaf(w[q], w[q], of_d_out);
+            of_out = fmaf(u[q], u[q], of_out);
+          }
         }
       }
 #pragma unroll
       for (int o = G / 2; o > 0; o >>= 1) {
         delta += __shfl_xor_sync(0xffffffffu, delta, o);
-        if constexpr (std::is_same<T, __half>::value) square += __shfl_xor_sync(0xffffffffu, square, o);
+        if constexpr (kSizes) {
+          of_d_out += __shfl_xor_sync(0xffffffffu, of_d_out, o);
+          of_out += __shfl_xor_sync(0xffffffffu, of_out, o);
+        }
       }
       const bool empty = lse[k] == -INFINITY;
-      if (!empty) top = fmaxf(top, square);
       if (lane == 0 && base + k * rows < n) {
         a.stat[stat[k]] = empty ? INFINITY : lse[k] * kLog2e - kWeightLog<T>;
         a.stat[stat[k] + 128] = empty ? 0.f : delta;
+        if constexpr (kSizes) {
+          // (what is infinite or undefined has results that are done again: it is left out here)
+          const float x = sqrtf(of_d_out), y = x * sqrtf(of_out);
+          a.row_sizes[(stat[k] >> 8) * 128 + (stat[k] & 127u)] = make_float2(!empty && x < INFINITY ? x : 0.f, !empty && y < INFINITY ? y : 0.f);
+        }
       }
     }
   }
-  if (!a.norms) return;
+  if constexpr (kSizes) {
+    const long long keys = (long long)a.B * a.T * a.HK;
+    for (long long first = (long long)blockIdx.x * rows * kRowsAtOnce; first < keys; first += (long long)gridDim.x * rows * kRowsAtOnce) {
+      const long long i = first + threadIdx.x / G;
+      Raw<T, VEC> x[kRowsAtOnce][chunks];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if ((threadIdx.x & 31u) == 0) sh[threadIdx.x / 32] = top;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int i = 1; i < 8; ++i) top = fmaxf(top, sh[i]);
-    a.norms[blockIdx.x] = top;
+      for (int k = 0; k < kRowsAtOnce; ++k)
+#pragma unroll
+        for (int c = 0; c < chunks; ++c) {
+          const int e = (c * G + lane) * VEC;
+          x[k][c].clear();
+          if (i + k * rows < keys && e < a.D) x[k][c].load((const T*)a.v + (i + k * rows) * a.ld + e);
+        }
+#pragma unroll
+      for (int k = 0; k < kRowsAtOnce; ++k) {
+        float of_v = 0.f;
+#pragma unroll
+        for (int c = 0; c < chunks; ++c) {
+          float u[VEC];
+          x[k][c].values(u);
+#pragma unroll
+          for (int q = 0; q < VEC; ++q) of_v = fmaf(u[q], u[q], of_v);
+        }
+#pragma unroll
+        for (int o = G / 2; o > 0; o >>= 1) of_v += __shfl_xor_sync(0xffffffffu, of_v, o);
+        if (lane == 0 && i + k * rows < keys) a.value_sizes[i + k * rows] = of_v < INFINITY ? sqrtf(of_v) : 0.f;
+      }
+    }
   }
 }
 typedef void (*StatisticsKernel)(const AttnArgs, const Divisor, const Divisor);
@@ -262,7 +291,7 @@ struct AttnOperator : b200_operator {
     const bool pad = tc && !plain;
     if (pad)
       for (auto& n : nodes) n.at = reserve((size_t)(n.of_keys ? key_rows : rows) * ld * 2);
-    size_t stat = 0, norms = 0, parts = 0, tickets = 0, sums = 0;
+    size_t stat = 0, row_sizes = 0, value_sizes = 0, parts = 0, tickets = 0, sums = 0;
     a.n_parts = 1;
     a.part_heads = a.group;
     if (tc && grad) {
@@ -297,7 +326,10 @@ struct AttnOperator : b200_operator {
       const long long at_once = 256 / group * kRowsAtOnce;
       statistics_grid = (unsigned int)std::min<long long>((rows + at_once - 1) / at_once, 8ll * dev->sm_count);
       stat = reserve((size_t)padded * 8);
-      if (dtype == B200_F16) norms = reserve((size_t)statistics_grid * 4);
+      if (dtype == B200_F16) {
+        row_sizes = reserve((size_t)padded * 8);
+        value_sizes = reserve((size_t)key_rows * 4);
+      }
     }
     take_workspace(reserved);
     if (grad && rows) {
@@ -305,8 +337,9 @@ struct AttnOperator : b200_operator {
       // the places behind a head's last row: a finite lse beyond all scores (3.4e38), so that what lies there weighs nothing
       cu_check(cu().cuMemsetD8Async_(workspace + stat, 0x7f, (size_t)a.B * a.H * ((a.S + 127) / 128) * 1024, dev->stream), "cuMemsetD8Async(statistics)");
       if (dtype == B200_F16) {
-        a.norms = (float*)(workspace + norms);
-        a.n_norms = (int)statistics_grid;
+        a.row_sizes = (float2*)(workspace + row_sizes);
+        a.value_sizes = (float*)(workspace + value_sizes);
+        cu_check(cu().cuMemsetD8Async_(workspace + row_sizes, 0, (size_t)a.B * a.H * ((a.S + 127) / 128) * 1024, dev->stream), "cuMemsetD8Async(sizes)");
       }
     }
     if (pad) {

@@ -184,3 +184,61 @@ def test_gradients_of_values_of_many_keys(device, prec):
     assert not nodes.read("dq").any() and not nodes.read("dk").any()
     op.free()
     nodes.free()
+
+
+R.EPS["half, scaled"] = R.EPS["half"]       # a half's steps, without what the scales of gradients add: see below
+
+
+def scaled_grad(x, seen, pos, scale, cap, sl):
+    """The gradients of half heads and how far each may be: score gradients lie within 2^13 and 2^14 of the bound of their own row
+    (a query's |d_out| (max |v| + |out|); a key's max |d_out| |v| + max |d_out| |out|, over its sequence and the heads that share it), so
+    that half a step below the normal numbers, 2^-25, is 2^-38 of it; weights are stored times 2^14: 2^-39."""
+    b, s, h, d = x["q"].shape
+    n, hk = x["k"].shape[1:3]
+    want = R.attention_grad(x["q"], x["k"], x["v"], x["out"], x["lse"], x["d_out"], seen, pos, scale, cap, sl, "half, scaled")
+    of = {m: np.linalg.norm(x[m], axis=-1) for m in ("d_out", "out", "v")}
+    more = [np.zeros_like(a) for a, _ in want]
+    for i in range(b):
+        for g in range(h):
+            k = g // (h // hk)
+            rows, keys = seen[i].any(1), seen[i].any(0)
+            heads = slice(k * (h // hk), (k + 1) * (h // hk))
+            top = of["d_out"][i][rows][:, heads].max(initial=0.0)
+            both = (of["d_out"][i] * of["out"][i])[rows][:, heads].max(initial=0.0)
+            mine = of["d_out"][i, :, g] * (of["v"][i, keys, k].max(initial=0.0) + of["out"][i, :, g])
+            theirs = top * of["v"][i, :, k] + both
+            more[0][i, :, g] += scale * 2.0 ** -38 * mine[:, None] * (seen[i] @ np.abs(x["k"][i, :, k]))
+            more[1][i, :, k] += scale * 2.0 ** -38 * theirs[:, None] * (seen[i].T @ np.abs(x["q"][i, :, g]))
+            more[2][i, :, k] += 2.0 ** -39 * (seen[i].T @ np.abs(x["d_out"][i, :, g]))
+    return [(v, bound + m + 2.0 ** -25) for (v, bound), m in zip(want, more)]
+
+
+# batch, queries, keys, heads, kv_heads, d, mask, documents, lengths, cap, slopes
+SCALED = [
+    (2, 512, 512, 2, 2, 64, "none", False, None, 0.0, False),
+    (2, 700, 700, 2, 1, 128, "causal", False, None, 20.0, False),
+    (2, 300, 900, 3, 1, 40, "prefix", True, (900, 700), 0.0, True),
+]
+
+
+@pytest.mark.parametrize("of_v", (1.0, 2.0 ** -6, 100.0))
+@pytest.mark.parametrize("case", SCALED)
+def test_half_gradients_of_different_sizes(device, case, of_v):
+    """Rows, heads and sequences of d_out that differ by 10^4, small and large values: each keeps the bits that its own size allows."""
+    x, t, more, sl, seen, pos, scale = attention_case(case, "half", seed=43)
+    x["v"] = R.rounded("half", x["v"] * of_v)
+    rows = np.flatnonzero(seen[0].any(1))
+    x["d_out"] = x["d_out"] * 0.1
+    x["d_out"][0, rows[len(rows) // 2], 0] *= 1e4      # one row of a head
+    x["d_out"][1] *= 1e3                               # a sequence
+    x["d_out"] = R.rounded("half", x["d_out"])
+    out, lse, _, _ = R.attention(x["q"], x["k"], x["v"], seen, pos, scale, t["cap"], sl)
+    x["out"], x["lse"] = R.rounded("half", out), R.rounded("single", lse)
+    nodes, op = link_attention(device, case, "half", x, t, more, sl, "aligned", grad=True)
+    op.run()
+    device.await_()
+    for m, (v, bound) in zip(("dq", "dk", "dv"), scaled_grad(x, seen, pos, scale, t["cap"], sl)):
+        assert np.abs(v).max() < 65504.0, m
+        R.within(nodes.read(m), v, bound, m)
+    op.free()
+    nodes.free()
