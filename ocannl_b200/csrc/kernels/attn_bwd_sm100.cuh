@@ -825,7 +825,7 @@ __global__ void __launch_bounds__(256) attn_join_parts(const __grid_constant__ A
           from_float(v[k], to[lane + 32 * k]);
           fine = fine && v[k] * 0.f == 0.f;
         }
-      if (__any_sync(0xffffffffu, !fine)) again |= 1 << which;
+      if (attn_again(fine)) again |= 1 << which;
     }
     if (again) {
       const long long bt = i / a.HK;

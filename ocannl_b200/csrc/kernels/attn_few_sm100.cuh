@@ -70,6 +70,7 @@ __device__ __forceinline__ void few_weigh(const float* from, int n, long long st
 #pragma unroll
   for (int k = 16; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
   sum = 0.f;
+  __syncwarp();                     // (all lanes have read the weights of the row before)
 #pragma unroll
   for (int k = 0; k < kFewMost / 32; ++k) {
     const float w = u[k] == 0.f ? 0.f : t[k] == -INFINITY ? 1.f : ex2(t[k] - top);
@@ -136,7 +137,7 @@ __device__ __forceinline__ void few_row_of_block(const AttnArgs& a, int b, int h
     }
     fine = few_finish<T>(a, b, h, r, 4 * (int)lane, v, top, sum);
   }
-  if (__any_sync(0xffffffffu, !fine)) attn_forward_row<T>(a, b, h, r, lane);
+  if (attn_again(fine)) attn_forward_row<T>(a, b, h, r, lane);
 }
 
 // blockIdx.x: (sequence, key head, sixteen of the rows that share it); blockIdx.y: range of keys
@@ -369,7 +370,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) attn_forward_few(const __grid_
     few_weigh<DP>(all + i * W, n_parts, kFewRows * W, weights[warp], top, sum);
     bool fine = true;
     if (lane_e < DP) fine = few_finish<T>(a, b, head_of(i), query_of(i), lane_e, few_gather(all + i * W, n_parts, kFewRows * W, weights[warp], lane_e, 0, 1), top, sum);
-    if (__any_sync(0xffffffffu, !fine)) attn_forward_row<T>(a, b, head_of(i), query_of(i), lane);
+    if (attn_again(fine)) attn_forward_row<T>(a, b, head_of(i), query_of(i), lane);
   }
 }
 

@@ -190,9 +190,11 @@ __device__ __forceinline__ bool single_store(const float (&v)[DT][4], int second
     }
   return fine;
 }
-// lanes 4 g .. 4 g + 3 have rows g and g + 8: the rows, a bit each, of which some lane says no
+// lanes 4 g .. 4 g + 3 have rows g and g + 8: the rows, a bit each, of which some lane says no.  What the lanes have written of them lies
+// behind (a vote alone orders no memory): the rows are written again by other lanes.
 __device__ __forceinline__ unsigned int rows_not(bool fine) {
   unsigned int b = __ballot_sync(0xffffffffu, !fine), rows = 0u;
+  __syncwarp();
 #pragma unroll
   for (int g = 0; g < 8; ++g) rows |= (b >> (4 * g) & 15u ? 1u : 0u) << g;
   return rows;

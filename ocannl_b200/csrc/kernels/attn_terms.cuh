@@ -130,6 +130,13 @@ __device__ __forceinline__ float attn_dot(const float (&x)[4], const float (&y)[
   return warp_sum(s);
 }
 
+// Whether some lane's part of a row has to be done again; what the lanes have written of it lies behind (a vote alone orders no memory).
+__device__ __forceinline__ bool attn_again(bool fine) {
+  const bool again = __any_sync(0xffffffffu, !fine);
+  __syncwarp();
+  return again;
+}
+
 template <class T>
 __device__ __noinline__ void attn_forward_row(const AttnArgs& a, int b, int h, int r, unsigned int lane) {
   const AttnRow w = attn_row(a, b, r);
