@@ -471,7 +471,7 @@ struct AttnOperator : b200_operator {
       keys_grid = blocks_of((long long)a.B * a.HK * ((a.T + 127) / 128) * a.n_parts);
       grid = blocks_of((long long)grid + keys_grid);
     }
-    if (smem > 227 * 1024) throw Error(B200_E_UNSUPPORTED, "attention: too many keys or queries");
+    if (smem > 227 * 1024) throw Error(B200_E_UNSUPPORTED, "attention: too many keys or queries with documents");
     if (grad) ready(gradients, smem);
     else ready(forward, smem);
   }
@@ -479,7 +479,7 @@ struct AttnOperator : b200_operator {
   void set() {
     forward = a.sums ? forward_of<T, DP, NQ, KW, true>(a.cap > 0.f, a.slopes != nullptr) : forward_of<T, DP, NQ, KW, false>(a.cap > 0.f, a.slopes != nullptr);
     threads = FwdShape<DP, NQ, KW>::kThreads;
-    smem = FwdShape<DP, NQ, KW>::smem((a.T + KW - 1) / KW);
+    smem = FwdShape<DP, NQ, KW>::smem(a.kdoc ? (a.T + KW - 1) / KW : 0);      // (tiles have classes in memory with documents alone)
     map_k = of_keys(a.k, KW);
     map_v = of_keys(a.v, KW);
   }
@@ -488,7 +488,7 @@ struct AttnOperator : b200_operator {
     typedef BwdShape<DP, CW> Sh;
     gradients = grad_of<T, DP, CW>(a.cap > 0.f, a.slopes != nullptr);
     threads = Sh::kThreads;
-    smem = Sh::smem((std::max(a.S, a.T) + CW - 1) / CW);
+    smem = Sh::smem(a.kdoc ? (std::max(a.S, a.T) + CW - 1) / CW : 0);
     maps.own_q = of_queries(a.q, 128);
     maps.own_d_out = of_queries(a.d_out, 128);
     maps.own_k = of_keys(a.k, 128);

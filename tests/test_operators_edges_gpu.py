@@ -2,6 +2,7 @@
 import numpy as np
 import pytest
 
+from ocannl_b200 import backend as bk
 from tests import operators_reference as R
 from tests.test_operators_gpu import PRECS, attention_case, link_attention, out_bound
 
@@ -241,4 +242,31 @@ def test_half_gradients_of_different_sizes(device, case, of_v):
         assert np.abs(v).max() < 65504.0, m
         R.within(nodes.read(m), v, bound, m)
     op.free()
+    nodes.free()
+
+
+def test_keys_beyond_what_classes_of_tiles_have_room_for(device):
+    """Ten million keys: without documents nothing is kept of their tiles; with them the call is refused."""
+    n, s, d = 10_600_000, 130, 8
+    rng = np.random.default_rng(47)
+    q, do = np.zeros((1, s, 1, d)), R.rounded("bfloat16", 1e6 * (1.0 + rng.random((1, s, 1, d))))
+    nodes = R.Nodes(device, dict(q=("bfloat16", q.shape, q), out=("bfloat16", q.shape, None), lse=("single", (1, 1, s), None), d_out=("bfloat16", q.shape, do),
+                                 dq=("bfloat16", q.shape, None), docs=("int32", (1, n), np.zeros((1, n))),
+                                 **{m: ("bfloat16", (1, n, 1, d), None if m in ("dk", "dv") else np.full((1, n, 1, d), of)) for m, of in (("k", 0.0), ("v", 1.5), ("dk", 0.0), ("dv", 0.0))}))
+    ctx, args = nodes.context, ("q", "k", "v", "out")
+    back = args + ("lse", "d_out", "dq", "dk", "dv")
+    for refused in (lambda: ctx.attention(*args, documents="docs"), lambda: ctx.attention_grad(*back, documents="docs")):
+        with pytest.raises(bk.B200Error) as e:
+            refused()
+        assert e.value.code == -4 and "too many keys" in str(e.value)
+    ops = [ctx.attention(*args, lse="lse", mask="none"), ctx.attention_grad(*back, mask="none")]
+    for op in ops:
+        op.run()
+    device.await_()
+    assert np.array_equal(nodes.read("out"), np.full(q.shape, 1.5))
+    R.within(nodes.read("lse"), np.full((1, 1, s), np.log(n)), R.ARITH * 17, "lse")
+    want = np.broadcast_to(do.sum(1, keepdims=True) / n, (1, n, 1, d))
+    R.within(nodes.read("dv"), want, (R.EPS["bfloat16"] + 16 * R.ARITH) * want, "dv")      # (p from an lse of up to 16, in single precision)
+    for op in ops:
+        op.free()
     nodes.free()
