@@ -138,7 +138,6 @@ __device__ __forceinline__ void attn_grad_keys(const b200_tmap& map_q, const b20
   float* scratch = (float*)(bars + 12);                   // [16]
   unsigned char* classes = (unsigned char*)(gen + Sh::kBytes + 256);
 
-  asm volatile("griddepcontrol.launch_dependents;");
   const unsigned int warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
   constexpr unsigned int kLoad = Sh::kWarps - 2, kMma = Sh::kWarps - 1;
   // this CTA's keys: the first ones first, which under a causal mask are seen by the most queries
@@ -158,6 +157,7 @@ __device__ __forceinline__ void attn_grad_keys(const b200_tmap& map_q, const b20
   if (warp == kMma) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(b200_smem_addr((const void*)tmem_slot)), "r"(Sh::kColumns) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    tmem_taken();
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const AttnSeq seq = attn_seq(a, b);
@@ -505,7 +505,6 @@ __device__ __forceinline__ void attn_grad_queries(const b200_tmap& map_q, const 
   AttnSpan* span = (AttnSpan*)(bars + 18);
   unsigned char* classes = (unsigned char*)(gen + Sh::kBytes + 256);
 
-  asm volatile("griddepcontrol.launch_dependents;");
   const unsigned int warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
   constexpr unsigned int kLoad = Sh::kWarps - 2, kMma = Sh::kWarps - 1;
   const unsigned int from_last = a.all_heads.of(block), bh = block - from_last * a.all_heads.d;
@@ -526,6 +525,7 @@ __device__ __forceinline__ void attn_grad_queries(const b200_tmap& map_q, const 
   if (warp == kMma) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(b200_smem_addr((const void*)tmem_slot)), "r"(Sh::kColumns) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    tmem_taken();
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const AttnSeq seq = attn_seq(a, b);

@@ -98,6 +98,10 @@ __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::befor
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void named_barrier(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
+// The next kernel in the stream may be placed from here on, and not before this block has its tensor memory: one that took it first would
+// wait for this kernel's end, and this block for the memory.
+__device__ __forceinline__ void tmem_taken() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 template <class T>
 __host__ __device__ constexpr unsigned int idesc_of(int m, int n, bool a_mn, bool b_mn) {
   const unsigned int f = sizeof(T) == 2 ? (std::is_same<T, __nv_bfloat16>::value ? 1u : 0u) : 0u;
@@ -217,7 +221,6 @@ attn_forward_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant__
   AttnSpan* spans = (AttnSpan*)(bars + 32);           // [2], 16 bytes each
   unsigned char* classes = (unsigned char*)(gen + Sh::kBytes + 512);
 
-  asm volatile("griddepcontrol.launch_dependents;");
   const unsigned int warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
   const unsigned int kLoad = NQ * 4, kMma = NQ * 4 + 1;
   // this CTA's queries: the last ones first, which under a causal mask see the most keys
@@ -253,6 +256,7 @@ attn_forward_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant__
   if (warp == kMma) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(b200_smem_addr((const void*)tmem_slot)), "r"(Sh::kColumns) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    tmem_taken();
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const AttnSeq seq = attn_seq(a, b);
