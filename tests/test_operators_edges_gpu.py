@@ -3,8 +3,11 @@ import numpy as np
 import pytest
 
 from ocannl_b200 import backend as bk
+from ocannl_b200.low_level import Tnode
+from ocannl_b200.workloads import load, store
 from tests import operators_reference as R
 from tests.test_operators_gpu import PRECS, attention_case, link_attention, out_bound
+from tests import test_operators_gpu as T
 
 pytestmark = pytest.mark.gpu
 
@@ -269,4 +272,80 @@ def test_keys_beyond_what_classes_of_tiles_have_room_for(device):
     R.within(nodes.read("dv"), want, (R.EPS["bfloat16"] + 16 * R.ARITH) * want, "dv")      # (p from an lse of up to 16, in single precision)
     for op in ops:
         op.free()
+    nodes.free()
+
+
+# two tiles of queries a block, tiles of which one sees keys that the other does not, documents in all of them
+TWO_TILES = [
+    (20, 1030, 1030, 4, 2, 128, "causal", True, None, 30.0, False),
+    (20, 1030, 1030, 4, 2, 128, "causal", True, None, 0.0, False),
+    (19, 700, 900, 4, 1, 96, "prefix", True, None, 0.0, True),
+    (38, 513, 513, 2, 2, 72, "none", True, tuple(513 - 13 * i for i in range(38)), 20.0, True),
+]
+
+
+@pytest.mark.parametrize("prec", ("bfloat16", "half"))
+@pytest.mark.parametrize("case", TWO_TILES)
+def test_two_tiles_of_queries_with_documents(device, case, prec):
+    T.test_attention_over_many_tiles(device, case, prec)
+
+
+@pytest.mark.parametrize("prec", PRECS)
+@pytest.mark.parametrize("rows,n", [(2, 16400), (3, 20001), (1, 70000)])
+def test_wide_rows_of_the_norm(device, rows, n, prec):
+    T.test_layer_norm(device, rows, n, prec)
+
+
+@pytest.mark.parametrize("prec", PRECS)
+@pytest.mark.parametrize("rows,n", [(70, 28672), (70, 28680), (65, 30001), (3, 70000)])
+def test_wide_rows_of_the_norms_gradients(device, rows, n, prec):
+    T.test_layer_norm_grad(device, rows, n, prec)
+
+
+@pytest.mark.parametrize("prec", ("bfloat16", "half"))
+def test_tiles_and_gradients_behind_two_to_the_31(device, prec):
+    """130 queries over 2.1 million positions, 2^31 elements and more of k, v, dk and dv.  All keys are zero, so all weights are equal; all
+    values but the last are zero."""
+    n, hk, d, s, tail = 2_100_000, 8, 128, 130, 64
+    assert n * hk * d > 2 ** 31
+    rng = np.random.default_rng(53)
+    pools = {m: device.alloc_pool(n * hk * d * 2) for m in ("k", "v", "dk", "dv")}
+    for p in pools.values():
+        device.memset_zero(p, 0, n * hk * d * 2)
+    last = R.rounded(prec, rng.standard_normal((tail, hk, d)) * n / 1000)
+    device.from_host(pools["v"], (n - tail) * hk * d * 2, store(prec, last.astype(np.float32)))
+    do = R.rounded(prec, 1000.0 * rng.standard_normal((1, s, hk, d)))
+    mean = last.sum(0) / n
+    out = R.rounded(prec, np.broadcast_to(mean, (1, s, hk, d)))
+    nodes = R.Nodes(device, dict(q=(prec, do.shape, np.ones(do.shape)), out=(prec, do.shape, None), lse=("single", (1, hk, s), None), given=(prec, do.shape, out),
+                                 d_out=(prec, do.shape, do), dq=(prec, do.shape, None)))
+    arrays = dict(nodes.context.arrays, **{m: (p, 0, Tnode(90 + i, m, prec, (1, n, hk, d))) for i, (m, p) in enumerate(pools.items())})
+    ctx = bk.Context(device, arrays)
+    ops = [ctx.attention("q", "k", "v", "out", lse="lse", mask="none"), ctx.attention_grad("q", "k", "v", "given", "lse", "d_out", "dq", "dk", "dv", mask="none")]
+    for op in ops:
+        op.run()
+    device.await_()
+    half = R.EPS[prec] / 2
+    # equal weights of one; sums of n of them and of 64 products in single precision, added in parts
+    R.within(nodes.read("out"), np.broadcast_to(mean, do.shape), half * np.abs(mean) + 2.0 ** -12 * np.abs(last).sum(0) / n + 2.0 ** -25, "out")
+    R.within(nodes.read("lse"), np.full((1, hk, s), np.log(n)), R.ARITH * 16, "lse")
+    assert not nodes.read("dq").any()
+    delta = (do * out).sum(-1)[0]                                        # [s, hk]
+    for first, v in ((0, np.zeros((2, hk, d))), (n // 2, np.zeros((2, hk, d))), (n - tail - 2, np.concatenate([np.zeros((2, hk, d)), last]))):
+        rows = v.shape[0]
+        dp = np.einsum("rhd,jhd->rjh", do[0], v)
+        ds, size = (dp - delta[:, None]) / n, (np.abs(np.einsum("rhd,jhd->rjh", np.abs(do[0]), np.abs(v))) + np.abs(do * out).sum(-1)[0][:, None]) / n
+        want = {"dv": np.broadcast_to(do[0].sum(0) / n, v.shape), "dk": np.broadcast_to(ds.sum(0)[..., None] / np.sqrt(d), v.shape)}
+        # weights and score gradients are rounded once; p comes from an lse of 15 in single precision
+        off = {"dv": (half + 16 * R.ARITH) * np.abs(do[0]).sum(0) / n,
+               "dk": (((half + 16 * R.ARITH) * np.abs(ds) + 2.0 ** -20 * size).sum(0) / np.sqrt(d))[..., None]}
+        for m in ("dv", "dk"):
+            host = np.empty((rows, hk, d), np.float16 if prec == "half" else np.uint16)
+            device.to_host(pools[m], first * hk * d * 2, host)
+            device.await_()
+            R.within(load(prec, host), want[m], off[m] + half * np.abs(want[m]) + 2.0 ** -25, m)
+    for op in ops:
+        op.free()
+    for p in pools.values():
+        device.free_pool(p)
     nodes.free()
