@@ -9,8 +9,10 @@
 // registers, at most 16 elements a thread, so that the squares of the distances from the mean are summed in a second pass over
 // registers (no difference of large sums).  The groups stride over the rows, the next row's loads under way while one is worked
 // on; the scale and the shift stay in shared memory.  In the gradient a thread keeps its sums over the rows of its columns in
-// registers; they meet in shared memory once per block and then in a second kernel that adds the blocks' partial sums in their order: the same bits every time.  Longer rows (forward: of more than
-// 16384 elements) are read again for each pass, by 1024 threads (they come from L2 then), their column sums kept in shared memory.
+// registers; they meet in shared memory once per block and then in a second kernel that adds the blocks' partial sums in their order: the
+// same bits every time.  Sums of a thread's own rows are in single precision, those over threads and blocks in double.
+// Longer rows (forward: of more than 16384 elements) are read again for each pass, by 1024 threads (they come from L2 then), their column sums
+// kept in shared memory.
 #include "kernels/op_common.cuh"
 #include "operators.hpp"
 
@@ -280,9 +282,9 @@ __global__ void __launch_bounds__(512, 1) norm_grad_rows(const NormArgs a) {
     __syncthreads();
     for (unsigned int e = threadIdx.x; e < 2 * a.n; e += blockDim.x) {
       const unsigned int which = e >= a.n, col = e - which * a.n;
-      float v = 0.f;
-      for (unsigned int g = 0; g < per_block; ++g) v += columns[which * plane + g * a.n + col];
-      a.partial[((unsigned long long)which * gridDim.x + blockIdx.x) * a.n + col] = v;
+      double v = 0.;
+      for (unsigned int g = 0; g < per_block; ++g) v += (double)columns[which * plane + g * a.n + col];
+      a.partial[((unsigned long long)which * gridDim.x + blockIdx.x) * a.n + col] = (float)v;
     }
   } else {
 #pragma unroll
@@ -403,44 +405,44 @@ __global__ void __launch_bounds__(1024) norm_grad_wide(const NormArgs a) {
       }
 }
 
-// column sums of wide rows: a thread per column, a slice of the rows per block; partial sums as above
+// column sums of wide rows: a thread per column, a slice of the rows per block, which may be long: in double; partial sums as above
 template <class T>
 __global__ void __launch_bounds__(256) norm_grad_columns(const NormArgs a, unsigned int slices) {
   grid_begin();
   const unsigned int col = blockIdx.x * 256 + threadIdx.x, slice = blockIdx.y;
   if (col >= a.n) return;
   const unsigned long long first = a.rows * slice / slices, last = a.rows * (slice + 1) / slices;
-  float dg = 0.f, db = 0.f;
+  double dg = 0., db = 0.;
 #pragma unroll 4
   for (unsigned long long row = first; row < last; ++row) {
     const float dy = to_float(((const T*)a.dy)[row * a.n + col]);
     const float u = (to_float(((const T*)a.x)[row * a.n + col]) - a.mean[row]) * a.rstd[row];
-    dg = fmaf(dy, u, dg);
-    db += dy;
+    dg = fma((double)dy, (double)u, dg);
+    db += (double)dy;
   }
-  a.partial[(unsigned long long)slice * a.n + col] = dg;
-  a.partial[((unsigned long long)slices + slice) * a.n + col] = db;
+  a.partial[(unsigned long long)slice * a.n + col] = (float)dg;
+  a.partial[((unsigned long long)slices + slice) * a.n + col] = (float)db;
 }
 
 // Partial sums of `blocks` blocks, added in their order: 32 columns x 32 runs of blocks, then the runs.
 __global__ void __launch_bounds__(1024) norm_grad_join(const float* partial, unsigned int blocks, unsigned int n, float* dgamma, float* dbeta) {
-  __shared__ float sh[32][33];
+  __shared__ double sh[32][33];
   grid_begin();
   const unsigned int col = blockIdx.x * 32 + threadIdx.x, which = blockIdx.y;
   float* out = which ? dbeta : dgamma;
-  float v = 0.f;
+  double v = 0.;
   if (out && col < n) {
     const float* p = partial + (unsigned long long)which * blocks * n + col;
 #pragma unroll 4
-    for (unsigned int b = threadIdx.y; b < blocks; b += 32) v += p[(unsigned long long)b * n];
+    for (unsigned int b = threadIdx.y; b < blocks; b += 32) v += (double)p[(unsigned long long)b * n];
   }
   sh[threadIdx.y][threadIdx.x] = v;
   __syncthreads();
   if (threadIdx.y == 0 && out && col < n) {
-    float s = 0.f;
+    double s = 0.;
 #pragma unroll
     for (int i = 0; i < 32; ++i) s += sh[i][threadIdx.x];
-    out[col] = s;
+    out[col] = (float)s;
   }
 }
 

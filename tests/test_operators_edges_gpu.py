@@ -349,3 +349,19 @@ def test_tiles_and_gradients_behind_two_to_the_31(device, prec):
     for p in pools.values():
         device.free_pool(p)
     nodes.free()
+
+
+@pytest.mark.parametrize("rows,n", [(9472, 64), (9472, 40), (700, 28680)])
+def test_column_sums_of_the_norms_gradients(device, rows, n):
+    """Rows that are all alike, of a value whose last bits a running sum in single precision drops once it has reached 32."""
+    c = float(np.float32(1 + 2.0 ** -19 - 2.0 ** -23))
+    same = lambda v: ("single", (rows, n), np.full((rows, n), v, np.float32))  # noqa: E731
+    nodes = R.Nodes(device, dict(x=same(1.0), dy=same(c), dx=("single", (rows, n), None), mean=("single", (rows,), np.zeros(rows)), rstd=("single", (rows,), np.ones(rows)),
+                                 dg=("single", (n,), None), db=("single", (n,), None)))
+    op = nodes.context.layer_norm_grad("x", "dy", "dx", "mean", "rstd", dgamma="dg", dbeta="db")
+    op.run()
+    # a thread's own rows (one to four of them here, or a slice in double), a block's sum and the result are rounded
+    for name in ("dg", "db"):
+        R.within(nodes.read(name), np.full(n, rows * c), 6 * 2.0 ** -24 * rows * c, name)
+    op.free()
+    nodes.free()
