@@ -203,7 +203,7 @@ __device__ __forceinline__ unsigned int rows_not(bool fine) {
 // What describes the other rows of a step: keys' documents, or the queries
 struct SingleOthers {
   int last[kOthers * kMostShares], doc[kOthers * kMostShares], pos[kOthers * kMostShares];
-  float lse2[kOthers * kMostShares], delta[kOthers * kMostShares];
+  float lse[kOthers * kMostShares], delta[kOthers * kMostShares];
 };
 
 // The warps' part in the block: which 16 of its rows, which of the steps
@@ -406,21 +406,21 @@ __device__ __forceinline__ void single_grad_queries(const AttnArgs& a, int vec, 
   const unsigned int heads = (unsigned int)a.B * (unsigned int)a.H;
   const int tiles_q = (a.S + 16 * groups - 1) / (16 * groups), r0 = (tiles_q - 1 - (int)(block / heads)) * 16 * groups;
   const int b = (int)(block % heads) / a.H, h = (int)(block % heads) % a.H, hk = h / a.group;
-  const float slope2 = a.slopes ? a.slopes[h] * kLog2e : 0.f;
+  const float slope = a.slopes ? a.slopes[h] : 0.f;
   if (threadIdx.x == 0) *block_end = 0;
   const long long q_at = attn_q_at(a, b, 0, h), q_step = (long long)a.H * a.ld;
   single_load(q, 16 * groups, a.q, q_at, q_step, r0, a.S, a.D, ld, vec);
   single_load(go, 16 * groups, a.d_out, q_at, q_step, r0, a.S, a.D, ld, vec);
   SingleOwn own;
   own.fetch(a, b, r0 + 16 * me.group);
-  float lse2[2], delta[2];
+  float lse[2], delta[2];
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
     const int r = r0 + 16 * me.group + g + 8 * w;
-    lse2[w] = INFINITY;
+    lse[w] = INFINITY;
     delta[w] = 0.f;
     if (r < a.S) {
-      lse2[w] = a.stat[attn_stat_at(a, b, h, r)];
+      lse[w] = a.stat[attn_stat_at(a, b, h, r)];
       delta[w] = a.stat[attn_stat_at(a, b, h, r) + 128];
     }
   }
@@ -461,7 +461,7 @@ __device__ __forceinline__ void single_grad_queries(const AttnArgs& a, int vec, 
         const AttnRow& w = own.row[i >> 1];
         const int at = mine + 8 * c + 2 * t + (i & 1), j = j0 + at;
         const bool on = j <= w.last && (!a.kdoc || o_->doc[at] == w.doc);
-        attn_pair(a, x[c][i], y[c][i], slope2, w.pos, j, lse2[i >> 1], delta[i >> 1], p, dx);
+        attn_pair(a, x[c][i], y[c][i], slope, w.pos, j, lse[i >> 1], delta[i >> 1], p, dx);
         x[c][i] = on ? dx : 0.f;
       }
     single_add<DT>(acc, x, kt, ld, steps);
@@ -520,7 +520,7 @@ __device__ __forceinline__ void single_grad_keys(const AttnArgs& a, int vec, int
     for (int i = 0; i < 4; ++i) gk[e][i] = gv[e][i] = 0.f;
   // a thread's query of the next step, fetched ahead
   int next_last = -1, next_doc = -1;
-  float next_lse2 = INFINITY, next_delta = 0.f;
+  float next_lse = INFINITY, next_delta = 0.f;
   auto fetch = [&](int h, int r0) {
     const int r = r0 + (int)threadIdx.x;
     next_last = next_doc = -1;
@@ -528,7 +528,7 @@ __device__ __forceinline__ void single_grad_keys(const AttnArgs& a, int vec, int
       next_last = attn_last(a, seq, r);
       next_doc = a.kdoc ? AttnQueryDocs(a, seq, b).of(r) : 0;
       if (next_doc < 0) next_last = -1;
-      next_lse2 = a.stat[attn_stat_at(a, b, h, r)];
+      next_lse = a.stat[attn_stat_at(a, b, h, r)];
       next_delta = a.stat[attn_stat_at(a, b, h, r) + 128];
     }
   };
@@ -538,7 +538,7 @@ __device__ __forceinline__ void single_grad_keys(const AttnArgs& a, int vec, int
   }
   int n = 0;
   for (int h = hk * a.group; h <= last_head; ++h) {
-    const float slope2 = a.slopes ? a.slopes[h] * kLog2e : 0.f;
+    const float slope = a.slopes ? a.slopes[h] : 0.f;
     for (int r0 = begin; r0 < a.S; r0 += span, ++n) {
       __syncthreads();
       const bool more = r0 + span < a.S || h < last_head;
@@ -549,7 +549,7 @@ __device__ __forceinline__ void single_grad_keys(const AttnArgs& a, int vec, int
         o_->last[threadIdx.x] = next_last;
         o_->doc[threadIdx.x] = next_doc;
         o_->pos[threadIdx.x] = seq.len - a.S + r0 + (int)threadIdx.x;
-        o_->lse2[threadIdx.x] = next_lse2;
+        o_->lse[threadIdx.x] = next_lse;
         o_->delta[threadIdx.x] = next_delta;
       }
       if (more) fetch(next_h, next_r);
@@ -575,7 +575,7 @@ __device__ __forceinline__ void single_grad_keys(const AttnArgs& a, int vec, int
         for (int i = 0; i < 4; ++i) {
           const int at = mine + 8 * c + 2 * t + (i & 1);
           const bool on = key[i >> 1] <= o_->last[at] && (!a.kdoc || o_->doc[at] == doc[i >> 1]);
-          attn_pair(a, x[c][i], y[c][i], slope2, o_->pos[at], key[i >> 1], o_->lse2[at], o_->delta[at], p, dx);
+          attn_pair(a, x[c][i], y[c][i], slope, o_->pos[at], key[i >> 1], o_->lse[at], o_->delta[at], p, dx);
           x[c][i] = on ? p : 0.f;
           y[c][i] = on ? dx : 0.f;
         }

@@ -98,9 +98,16 @@ constexpr float kWeightLog = std::is_same<T, __half>::value ? 14.f : 0.f;
 template <class T>
 constexpr float kWeightBack = std::is_same<T, __half>::value ? 1.f / 16384.f : 1.f;
 
-// Where a row's statistics lie: its lse (log 2 units, less kWeightLog; +infinity for a row that sees nothing: all weights are zero), 128 further <d_out, out>
+// Where a row's statistics lie: its lse (of 16-bit heads in log 2 units, less kWeightLog; +infinity for a row that sees nothing: all weights are zero), 128 further <d_out, out>
 __device__ __forceinline__ long long attn_stat_at(const AttnArgs& a, int b, int h, int r) {
   return (((long long)b * a.H + h) * ((a.S + 127) / 128) + (r >> 7)) * 256 + (r & 127);
+}
+
+// the lse of a row's statistics as it was given (or +infinity)
+template <class T>
+__device__ __forceinline__ float attn_lse_of(float stat) {
+  if constexpr (std::is_same<T, float>::value) return stat;
+  return (stat + kWeightLog<T>) * kLn2;
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -161,11 +168,17 @@ __device__ __noinline__ void attn_forward_row(const AttnArgs& a, int b, int h, i
   if (a.lse && lane == 0) a.lse[((long long)b * a.H + h) * a.S + r] = (m + log2f(l)) * kLn2;
 }
 
-// p and dx of one pair, from the dot products <q, k> and <d_out, v>
-__device__ __forceinline__ void attn_pair(const AttnArgs& a, float qk, float dov, float slope2, int pos, int j, float lse2, float delta, float& p, float& dx) {
-  float th;
-  const float s = attn_score(a, qk, slope2, pos, j, th);
-  p = exp2f(s - lse2);
+// p and dx of one pair, from the dot products <q, k> and <d_out, v>.  Score and lse meet in their own unit, where their difference is all but
+// exact: each rounded in units of log 2 first, scores of 30 cost a third of p's accuracy in single precision.
+__device__ __forceinline__ void attn_pair(const AttnArgs& a, float qk, float dov, float slope, int pos, int j, float lse, float delta, float& p, float& dx) {
+  float th = 0.f, s;
+  if (a.cap > 0.f) {
+    th = tanhf(qk * a.over);
+    s = th * a.cap;
+  } else {
+    s = qk * a.scale;
+  }
+  p = exp2f((fmaf(-slope, fabsf((float)(pos - j)), s) - lse) * kLog2e);
   dx = p * (dov - delta) * a.scale;
   if (a.cap > 0.f) dx *= 1.f - th * th;
 }
@@ -173,10 +186,10 @@ __device__ __forceinline__ void attn_pair(const AttnArgs& a, float qk, float dov
 template <class T>
 __device__ __noinline__ void attn_dq_row(const AttnArgs& a, int b, int h, int r, unsigned int lane) {
   const AttnRow w = attn_row(a, b, r);
-  const float slope2 = a.slopes ? a.slopes[h] * kLog2e : 0.f;
+  const float slope = a.slopes ? a.slopes[h] : 0.f;
   const int hk = h / a.group;
   const long long at = attn_q_at(a, b, r, h), stat = attn_stat_at(a, b, h, r);
-  const float lse2 = a.stat[stat] + kWeightLog<T>, delta = a.stat[stat + 128];
+  const float lse = attn_lse_of<T>(a.stat[stat]), delta = a.stat[stat + 128];
   float q[4], k[4], v[4], go[4], g[4] = {0.f, 0.f, 0.f, 0.f}, p, dx;
   attn_load_row<T>(a, a.q, at, lane, q);
   attn_load_row<T>(a, a.d_out, at, lane, go);
@@ -185,7 +198,7 @@ __device__ __noinline__ void attn_dq_row(const AttnArgs& a, int b, int h, int r,
     const long long kat = attn_k_at(a, b, j, hk);
     attn_load_row<T>(a, a.k, kat, lane, k);
     attn_load_row<T>(a, a.v, kat, lane, v);
-    attn_pair(a, attn_dot(q, k), attn_dot(go, v), slope2, w.pos, j, lse2, delta, p, dx);
+    attn_pair(a, attn_dot(q, k), attn_dot(go, v), slope, w.pos, j, lse, delta, p, dx);
 #pragma unroll
     for (int i = 0; i < 4; ++i) g[i] = fmaf(dx, k[i], g[i]);
   }
@@ -201,14 +214,14 @@ __device__ __noinline__ void attn_dkv_row(const AttnArgs& a, int b, int hk, int 
   attn_load_row<T>(a, a.k, kat, lane, k);
   attn_load_row<T>(a, a.v, kat, lane, v);
   for (int h = hk * a.group; h < (hk + 1) * a.group; ++h) {
-    const float slope2 = a.slopes ? a.slopes[h] * kLog2e : 0.f;
+    const float slope = a.slopes ? a.slopes[h] : 0.f;
     for (int r = 0; r < a.S; ++r) {
       const AttnRow w = attn_row(a, b, r);
       if (j > w.last || (a.kdoc && doc != w.doc)) continue;
       const long long at = attn_q_at(a, b, r, h), stat = attn_stat_at(a, b, h, r);
       attn_load_row<T>(a, a.q, at, lane, q);
       attn_load_row<T>(a, a.d_out, at, lane, go);
-      attn_pair(a, attn_dot(q, k), attn_dot(go, v), slope2, w.pos, j, a.stat[stat] + kWeightLog<T>, a.stat[stat + 128], p, dx);
+      attn_pair(a, attn_dot(q, k), attn_dot(go, v), slope, w.pos, j, attn_lse_of<T>(a.stat[stat]), a.stat[stat + 128], p, dx);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         gk[i] = fmaf(dx, q[i], gk[i]);

@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(256) attn_statistics(const __grid_constant__ A
       }
       const bool empty = lse[k] == -INFINITY;
       if (lane == 0 && base + k * rows < n) {
-        a.stat[stat[k]] = empty ? INFINITY : lse[k] * kLog2e - kWeightLog<T>;
+        a.stat[stat[k]] = empty ? INFINITY : sizeof(T) == 4 ? lse[k] : lse[k] * kLog2e - kWeightLog<T>;
         a.stat[stat[k] + 128] = empty ? 0.f : delta;
         if constexpr (kSizes) {
           // (what is infinite or undefined has results that are done again: it is left out here)

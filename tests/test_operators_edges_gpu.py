@@ -365,3 +365,23 @@ def test_column_sums_of_the_norms_gradients(device, rows, n):
         R.within(nodes.read(name), np.full(n, rows * c), 6 * 2.0 ** -24 * rows * c, name)
     op.free()
     nodes.free()
+
+
+def test_single_precision_weights_of_large_scores(device):
+    """Every query sees one key, with scores of up to 60 and an lse that is the score: weights of one."""
+    n, d = 200, 16
+    rng = np.random.default_rng(59)
+    q, k = np.zeros((1, n, 1, d)), np.zeros((1, n, 1, d))
+    q[0, :, 0, 0], k[..., 0] = np.arange(n) + 1, 1.0
+    scale = np.float32(0.3)
+    lse = (q[0, :, 0, 0].astype(np.float32) * scale).astype(np.float32)
+    v, do = (R.rounded("single", rng.standard_normal((1, n, 1, d))) for _ in range(2))
+    single = lambda a: ("single", a.shape, a)  # noqa: E731
+    nodes = R.Nodes(device, dict(q=single(q), k=single(k), v=single(v), out=single(v), d_out=single(do), lse=single(lse.reshape(1, 1, n)), docs=("int32", (1, n), np.arange(n)[None]),
+                                 dq=("single", q.shape, None), dk=("single", q.shape, None), dv=("single", q.shape, None)))
+    op = nodes.context.attention_grad("q", "k", "v", "out", "lse", "d_out", "dq", "dk", "dv", documents="docs", scale=float(scale))
+    op.run()
+    # two tf32 parts keep 2^-21 of each operand
+    R.within(nodes.read("dv"), do, 2.0 ** -20 * np.abs(do) + 1e-30, "dv")
+    op.free()
+    nodes.free()
