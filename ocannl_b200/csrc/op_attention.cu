@@ -541,6 +541,9 @@ void bind(const b200_attention& p, AttnOperator* op, bool grad) {
   if (p.d > 128) ops.refuse("heads of more than 128 elements", B200_E_UNSUPPORTED);
   if (!(p.scale > 0.f) || !std::isfinite(p.scale)) ops.refuse("the scale must be positive and finite");
   if (!(p.cap >= 0.f) || !std::isfinite(p.cap)) ops.refuse("the cap must be finite and not negative (0: none)");
+  // (what the scores are multiplied by: infinite, or too small for all its bits, it would make every score undefined or rough)
+  if (!std::isfinite(p.scale * kLog2e)) ops.refuse("the scale is too large");
+  if (p.cap > 0.f && (!std::isfinite(p.cap * kLog2e) || !std::isnormal(p.scale / p.cap))) ops.refuse("the cap is too far from the scale");
   if (p.mask < B200_MASK_NONE || p.mask > B200_MASK_PREFIX) ops.refuse("unknown mask " + std::to_string(p.mask));
   if ((p.mask == B200_MASK_PREFIX) != (p.prefix.pool_id >= 0)) ops.refuse("'prefix' goes with the prefix mask");
   if (p.query_documents.pool_id >= 0 && p.key_documents.pool_id < 0) ops.refuse("documents of queries go with documents of keys");

@@ -385,3 +385,14 @@ def test_single_precision_weights_of_large_scores(device):
     R.within(nodes.read("dv"), do, 2.0 ** -20 * np.abs(do) + 1e-30, "dv")
     op.free()
     nodes.free()
+
+
+@pytest.mark.parametrize("scale,cap,words", [(3e38, 0.0, "scale is too large"), (0.125, 1e-45, "cap is too far"), (0.125, 1e38, "cap is too far"), (1e-30, 3e9, "cap is too far"),
+                                             (0.125, 3e38, "cap is too far")])
+def test_scales_and_caps_that_scores_cannot_have(device, scale, cap, words):
+    one = ("bfloat16", (1, 2, 1, 16), np.ones((1, 2, 1, 16)))
+    nodes = R.Nodes(device, dict(q=one, k=one, v=one, out=("bfloat16", (1, 2, 1, 16), None)))
+    with pytest.raises(bk.B200Error) as e:
+        nodes.context.attention("q", "k", "v", "out", scale=scale, cap=cap)
+    assert e.value.code == -1 and words in str(e.value)
+    nodes.free()
