@@ -563,7 +563,8 @@ attn_forward_tc(const __grid_constant__ b200_tmap map_q, const __grid_constant__
     if (live) live = b200_wait(seen ? bar_f + 8 * g : bar_q, 0u, abort_flag, a.status, 29u);
     tc_after();
     const float by = l > 0.f || l != l ? 1.f / l : 0.f;
-    float bad = 0.f;
+    // (of scores beyond 2^23 the product with `unit`, which is not rounded, and the maximum, which is, may lie far apart: such rows are done again)
+    float bad = !BIAS && fabsf(m) > 8388608.f && seen && m != -INFINITY ? 1.f : 0.f;
     unsigned char* tile = gen + g * Sh::kTile;     // the queries' tile: its last product is done
     const unsigned int in = (warp & 3u) * 32 + lane;
 #pragma unroll

@@ -396,3 +396,21 @@ def test_scales_and_caps_that_scores_cannot_have(device, scale, cap, words):
         nodes.context.attention("q", "k", "v", "out", scale=scale, cap=cap)
     assert e.value.code == -1 and words in str(e.value)
     nodes.free()
+
+
+@pytest.mark.parametrize("prec", PRECS)
+@pytest.mark.parametrize("scale,cap", [(1e-30, 1e-30), (1e30, 0.0), (0.125, 1e30)])
+def test_scales_and_caps_far_from_one(device, scale, cap, prec):
+    """Scores of 1e-30 weigh all keys alike; those of 1e30 the largest alone; a cap far above the scores changes none."""
+    rng = np.random.default_rng(61)
+    n, d = 40, 16
+    q, k, v = (R.rounded(prec, rng.standard_normal((1, n, 1, d))) for _ in range(3))
+    nodes = R.Nodes(device, dict(q=(prec, q.shape, q), k=(prec, k.shape, k), v=(prec, v.shape, v), out=(prec, q.shape, None)))
+    op = nodes.context.attention("q", "k", "v", "out", mask="none", scale=scale, cap=cap)
+    op.run()
+    device.await_()
+    seen, pos = R.visible(1, n, n, "none")
+    out, _, size, flat = R.attention(q, k, v, seen, pos, float(np.float32(scale)), float(np.float32(cap)))
+    R.within(nodes.read("out"), out, out_bound(prec, out, size, flat), "out")
+    op.free()
+    nodes.free()
