@@ -194,10 +194,11 @@ int b200_sum_f32_static(b200_dev* dev, int in_pool, size_t in_offset, size_t cou
  *      assignments.  An operator is linked to nodes once, like a routine -- arguments are checked, the kernels and the
  *      workspace chosen -- and keeps their addresses: free it before their pools.  A run queues kernels on the device's
  *      stream, in order with routines and copies; it allocates nothing, waits for nothing and may be captured into a CUDA graph.
- *      Every linked operator has a workspace of its own; runs of ONE operator may not overlap on the GPU.
+ *      Every linked operator has a workspace of its own; runs of ONE operator, and of the graphs that hold it, may not overlap
+ *      on the GPU, and a graph that holds it is released before the operator.
  *      Nodes are row-major and need only be aligned to their element size (16 bytes are faster).  An output may not overlap
- *      another operand, but where it says so.  Sums, statistics and softmax are held in single precision; 16-bit outputs are
- *      rounded once.  The same inputs give the same bits. */
+ *      another operand, but where it says so.  Sums, statistics and softmax are held in single precision or better; 16-bit outputs
+ *      are rounded once.  The same inputs give the same bits. */
 typedef struct b200_operator b200_operator;
 #define B200_F16 2               /* beside B200_F32 and B200_BF16 */
 typedef struct {
@@ -259,7 +260,12 @@ int b200_rotary_link(b200_dev* dev, const b200_rotary* spec, b200_operator** out
  *   B200_MASK_CAUSAL: j <= position;   B200_MASK_PREFIX: j <= position or j < prefix[b];
  *   and, with documents: key_documents[b, j] == query_documents[b, r] >= 0 (a negative document is padding).  Where no documents of
  *   queries are given, a query has the document of the key at its position (and none, like padding, where its position is negative).
- * What lies at a key or a query that is not seen has no influence, whatever it holds.
+ * What lies at a key or a query that is not seen has no influence, whatever it holds, beyond the last bits: with a cap the formula for
+ * tanh, and in the gradients of half heads the scale of a row, are chosen for a warp or a tile as a whole.
+ * Products: 16-bit heads multiply their own values exactly; weights, and in the gradients the gradients of scores, are rounded to
+ * the heads' type once more before they are multiplied (half ones scaled by powers of two, so that small ones keep their bits).
+ * Single heads are multiplied as two tf32 parts each, 2^-21 of a product; sums are in single precision.  lse is off by 2^-22 of its size, and
+ * the gradients' weights by as much as lse is: scores of thousands cost them bits.
  * The gradient takes out and lse of the forward pass and gives, with p = exp(s - lse),
  *   dv_j = sum_r p_rj d_out_r;  ds_rj = p_rj (<d_out_r, v_j> - <d_out_r, out_r>);  dx = ds (1 - (c / cap)^2)
  *   dq_r = scale * sum_j dx_rj k_j;  dk_j = scale * sum_r dx_rj q_r

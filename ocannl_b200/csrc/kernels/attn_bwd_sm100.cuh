@@ -9,7 +9,7 @@
 //            A operand of dv += p^T do and dk += ds^T q.
 //   queries  a CTA has 128 queries of one head and walks the tiles of keys they see: s = q k^T, dp = do v^T, dq += ds k.
 //
-// A thread does 64 columns of a row; one warp copies, one issues the products.  Weights are formed while the second product runs, the
+// A thread does 64 columns of a row; half score gradients are scaled, see unit_of; one warp copies, one issues the products.  Weights are formed while the second product runs, the
 // score gradients while the next tile's scores are.  Heads of more than 64 elements take tiles of 128 columns, two threads a row, and
 // all of tensor memory; those of up to 64 tiles of 64 columns, a thread a row, and half of it, so that two CTAs share an SM (short
 // sequences are bound by the chain from a CTA's start to its end).  Copies start before anything else.

@@ -15,7 +15,8 @@ namespace b200 {
 constexpr int kFewRows = 16, kFewStep = 16, kFewStages = 3, kFewWarps = 4, kFewMost = 256;   // (most ranges)
 
 struct FewArgs {
-  float* parts;            // [pair][split][16][DP + 4]: output (not divided), maximum, sum (both of half weights times 2^7), and two floats that keep rows on 16 bytes
+  float* parts;            // [pair][split][16][DP + 4]: output (not divided), maximum, sum (half weights times 2^7), and two floats that
+                           // keep rows on 16 bytes
   unsigned int* tickets;   // [pair], zero between runs
   int splits, per_split;   // keys of a range, a multiple of 16 * 4
   int join_later;          // the ranges are joined by a launch of its own

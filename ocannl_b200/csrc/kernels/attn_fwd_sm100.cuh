@@ -1,8 +1,9 @@
 // Attention for 16-bit heads on the tensor cores, any number of keys: softmax with a running maximum and sum.
 //
 // A CTA takes NQ tiles of 128 queries of one (sequence, head).  Roles: a warp that copies (TMA: the queries once, then tiles of
-// 128 keys and values through rings), a warp that issues tcgen05.mma, and four warps per query tile that do the softmax, a thread
-// a row.  Scores of a tile lie in tensor memory (128 columns); the thread loads its row of 128, applies cap, bias and mask, takes
+// 64 or 128 keys and values through rings), a warp that issues tcgen05.mma, and four warps per query tile that do the softmax, a thread
+// a row.  Scores of a tile lie in tensor memory (128 columns: one tile of 128 keys, or two of 64, of which the next one's scores are formed
+// during the softmax of this); the thread loads its row, 32 scores at a time, applies cap, bias and mask, takes
 // the maximum, writes the weights exp2(s - m) in 16 bits over the scores, and they are the A operand of the second product, which adds
 // to the output accumulators in tensor memory.  The accumulators are only multiplied by 2^(m_old - m_new) when a row's maximum has
 // grown by more than 2^8 (weights stay below that, sums and accumulators are single precision, so nothing is lost): after the
@@ -45,7 +46,7 @@ __device__ __forceinline__ float tanh_of(float two_x_log2e) { return fmaf(-2.f, 
 
 // x = tanh(x scale) of N scores of each lane.  The exponential and the reciprocal of tanh_of pass through the unit that also has to make
 // the weights, at an eighth of the multiply-adds' rate, and would bound the kernel: where all of a warp's scores are at most the cap in
-// size, tanh y = y + y^3 Q(y^2) instead, with Q the polynomial of degree 5 whose largest error on [0, 1] is least (2.6e-8, 8e-8 in single
+// size, tanh y = y + y^3 Q(y^2) instead, with Q the polynomial of degree 5 whose largest error on [0, 1] is least (3.0e-8, 8e-8 in single
 // precision, 1.6e-7 relative; fitted by iterated weighted least squares).  2 x 4096 positions, 16 heads of 128, causal: 301 us without,
 // 226 with it and tiles of 64 keys.
 template <int N>
