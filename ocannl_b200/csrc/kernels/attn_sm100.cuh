@@ -191,7 +191,6 @@ B200_ATTN_NAME(const __grid_constant__ b200_tmap map_q, const __grid_constant__ 
   volatile unsigned int* tmem_slot = (volatile unsigned int*)(bars + 4);
   volatile unsigned int* abort_flag = tmem_slot + 1;
 
-  asm volatile("griddepcontrol.launch_dependents;");
   const unsigned int warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
   const unsigned int quarter = warp & 3u, half = warp >> 2;
 #ifdef B200_TRACE
@@ -225,6 +224,8 @@ B200_ATTN_NAME(const __grid_constant__ b200_tmap map_q, const __grid_constant__ 
                  "r"((unsigned int)B200_ATTN_TMEM_COLS)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    // (not before the block has its tensor memory, which the next kernel's would wait for this one with)
+    asm volatile("griddepcontrol.launch_dependents;");
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");

@@ -170,8 +170,6 @@ B200_KERNEL_HEAD(B200_TMAP_PARAM map_a, B200_TMAP_PARAM map_b, const b200_gemm_s
   volatile unsigned int* tmem_slot = (volatile unsigned int*)(bars + 2 * B200_STAGES + 5 + B200_EPI_WARPS);
   volatile unsigned int* abort_flag = tmem_slot + 1;
 
-  // the next kernel in the stream may be placed as soon as every CTA of this one is running
-  asm volatile("griddepcontrol.launch_dependents;");
   const unsigned int warp = threadIdx.x >> 5;
   const unsigned int lane = threadIdx.x & 31u;
 #ifdef B200_TRACE
@@ -207,6 +205,9 @@ B200_KERNEL_HEAD(B200_TMAP_PARAM map_a, B200_TMAP_PARAM map_b, const b200_gemm_s
                  "r"((unsigned int)B200_TMEM_COLS)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit." B200_CG ".sync.aligned;" ::: "memory");
+    // The next kernel in the stream may be placed from here on, when every CTA of this one has its tensor memory: one that took it first
+    // would wait for this kernel's end, and this CTA for the memory.
+    asm volatile("griddepcontrol.launch_dependents;");
   }
   // Set-up touches no global memory and is over, block-wide barrier included, before the grids ahead of this one
   // end; the threads that read or write global memory (the producer, the epilogue) then wait for those grids
