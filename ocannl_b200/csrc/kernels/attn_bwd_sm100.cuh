@@ -34,7 +34,7 @@ struct BwdShape {
 
 // Half gradients of scores are multiplied by a power of two before they are rounded, a row's own: ds = p <d_out, v - out> is at most
 // |d_out| |v| + |d_out| |out|, and the power brings that bound between 2^13 and 2^14.  A query's row has its own |d_out| and the largest
-// |v| of the tiles it sees; a key's its own |v| and the largest |d_out| and |d_out| |out| of them.  So p may be 2^-20 before the first
+// |v| that its tile of queries sees; a key's its own |v| and the largest |d_out| and |d_out| |out| of the tiles that see it.  So p may be 2^-20 before the first
 // bits are lost, whatever the sizes of d_out and v, and other rows, heads and sequences have no say in it.
 // (One power for the whole call, of the largest |d_out|, left 3 % of a gradient wrong beside a row 10^4 times as large.)
 __device__ __forceinline__ float unit_of(float bound) {
@@ -528,8 +528,7 @@ __device__ __forceinline__ void attn_grad_queries(const b200_tmap& map_q, const 
     tmem_taken();
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const AttnSeq seq = attn_seq(a, b);
-  const AttnSpan plain = plain_span(a, seq, r0, 128);
+  const AttnSpan plain = plain_span(a, attn_seq(a, b), r0, 128);
   int tiles = (plain.last_max + CW) / CW;
   auto load = [&](int t, unsigned int n) {
     const unsigned int slot = n & 1u, at = ring + slot * Sh::kStage, bar = bar_full + 8 * slot;
@@ -665,12 +664,25 @@ __device__ __forceinline__ void attn_grad_queries(const b200_tmap& map_q, const 
     const float lse2 = stat[0], delta = stat[128];
     float grad_unit = 1.f;
     if constexpr (std::is_same<T, __half>::value) {
+      // (of keys that some row of the tile sees)
       float of_v[1] = {0.f};
       const float* sizes = a.value_sizes + (long long)b * a.T * a.HK + hk;
-      const int end = min(tiles * CW, seq.len);
+      if (!docs) {
 #pragma unroll 8
-      for (int j = (int)threadIdx.x; j < end; j += Sh::kGroups * 128)
-        if (!docs || classes[j / CW]) of_v[0] = fmaxf(of_v[0], sizes[(long long)j * a.HK]);
+        for (int j = (int)threadIdx.x; j <= plain.last_max; j += Sh::kGroups * 128) of_v[0] = fmaxf(of_v[0], sizes[(long long)j * a.HK]);
+      } else {
+        // tiles of which all is seen are shared out; of the others a warp takes what its own rows see
+        for (int t = 0; t < tiles; ++t) {
+          const unsigned int cls = classes[t];
+          if (!cls || (cls == 1u && (t & 3) != (int)(warp & 3u))) continue;
+          const int first = t * CW + 64 * (int)half;
+          unsigned int seen[2] = {0xffffffffu, 0xffffffffu};
+          if (cls == 2u) visible_words<2>(a, b, first, row, lane, seen);
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            if (__reduce_or_sync(0xffffffffu, seen[i]) >> lane & 1u) of_v[0] = fmaxf(of_v[0], sizes[(long long)(first + 32 * i + (int)lane) * a.HK]);
+        }
+      }
       const float2 s = a.row_sizes[(((long long)b * a.H + h) * tiles_q + t_q) * 128 + in];
       largest<Sh::kGroups * 4>(of_v, scratch);
       grad_unit = unit_of(fmaf(s.x, of_v[0], s.y));

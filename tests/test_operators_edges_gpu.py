@@ -414,3 +414,21 @@ def test_scales_and_caps_far_from_one(device, scale, cap, prec):
     R.within(nodes.read("out"), out, out_bound(prec, out, size, flat), "out")
     op.free()
     nodes.free()
+
+
+@pytest.mark.parametrize("case", [(2, 400, 400, 2, 1, 64, "causal", True, None, 0.0, False), (2, 300, 500, 2, 2, 128, "causal", True, (450, 333), 0.0, True)])
+def test_half_gradients_beside_large_values_that_are_not_seen(device, case):
+    """Values of 60000 at padding and behind the lengths take nothing from the gradients of values of 2^-8."""
+    x, t, more, sl, seen, pos, scale = attention_case(case, "half", seed=67)
+    keys = seen.any(1)
+    x["v"] = R.rounded("half", np.where(keys[:, :, None, None], x["v"] * 2.0 ** -8, 60000.0))
+    x["k"] = R.rounded("half", np.where(keys[:, :, None, None], x["k"], 200.0))
+    out, lse, _, _ = R.attention(x["q"], x["k"], x["v"], seen, pos, scale, t["cap"], sl)
+    x["out"], x["lse"] = R.rounded("half", out), R.rounded("single", lse)
+    nodes, op = link_attention(device, case, "half", x, t, more, sl, "aligned", grad=True)
+    op.run()
+    device.await_()
+    for m, (v, bound) in zip(("dq", "dk", "dv"), scaled_grad(x, seen, pos, scale, t["cap"], sl)):
+        R.within(nodes.read(m), v, bound, m)
+    op.free()
+    nodes.free()
