@@ -290,6 +290,87 @@ typedef struct {
 int b200_attention_link(b200_dev* dev, const b200_attention* spec, b200_operator** out);
 int b200_attention_grad_link(b200_dev* dev, const b200_attention* spec, b200_operator** out);
 
+/* A cache of keys and one of values in pages, for sequences of different lengths: [pages, kv_heads, page, d] each, of the type `dtype` or in 8
+ * bits (B200_E4M3: sign, 4 bits of exponent, 3 of mantissa, 448 the largest, no infinities) with a scale for each page and head, k = k_scale * code.
+ * Sequence b's tokens i * page .. (i + 1) * page - 1 lie in page page_table[b, i]; a number outside 0 .. pages - 1 is no page: nothing is written there
+ * and nobody sees its tokens (as with pages given back behind a window).  lengths[b] counts a sequence's tokens, the new ones included
+ * (negative: 0); tokens behind max_pages pages are not kept.  New tokens are rows of packed nodes: sequence b has rows starts[b] .. starts[b + 1] - 1
+ * (numbers taken between 0 and `tokens`, not falling), or, without starts, tokens / batch rows each.  Row i of n lies at position lengths[b] - n + i,
+ * and nowhere where that is negative.  Rows of no sequence are left as they were.  Pages may be shared between sequences, but for those that a call
+ * of cache_append writes. */
+#define B200_E4M3 3
+typedef struct {
+  int64_t batch, tokens;
+  int64_t pages, max_pages;      /* pages of the cache; of a sequence at most */
+  int32_t page;                  /* tokens of a page */
+  int32_t kv_heads, d;
+  int32_t dtype;                 /* of the cache: that of the new tokens, or B200_E4M3 */
+  b200_operand k, v;
+  b200_operand k_scale, v_scale; /* single [pages, kv_heads], with B200_E4M3: between 2^-40 and 2^40 */
+  b200_operand page_table;       /* int32 [batch, max_pages] */
+  b200_operand lengths;          /* int32 [batch] */
+  b200_operand starts;           /* int32 [batch + 1], optional */
+} b200_cache;
+
+/* New keys and values [tokens, kv_heads, d] go to their slots of the cache.  Keys, and with them queries [tokens, heads, d] if given, turn on the way
+ * as b200_rotary does it (pairs 0: they do not), by the token's position or by that of `positions`, and are rounded once to what holds them.
+ * 8 bits: a page's scale of a head is 2^e, the least power of two of at least 2^-40 with |x| <= 448 * 2^e for all values that the page has received;
+ * where it grows, the codes that the page holds are rounded again (which changes those alone that fall below the normal range).  A page whose
+ * first slot is written starts anew.  Values that are undefined, infinite or beyond 448 * 2^40 become the code of an undefined value. */
+typedef struct {
+  b200_cache cache;              /* k, v and the scales are written */
+  int32_t dtype;                 /* of k, v, q, q_out */
+  int32_t heads;                 /* of q; 0: no queries */
+  int32_t pairs;                 /* 2 * pairs <= d */
+  int32_t interleaved;
+  float magnitude;
+  const double* frequencies;     /* host, [pairs]: radians per position; copied at link */
+  b200_operand positions;        /* int32 [tokens], optional: what keys and queries turn by */
+  b200_operand k, v;
+  b200_operand q, q_out;         /* may be one node */
+} b200_cache_append;
+int b200_cache_append_link(b200_dev* dev, const b200_cache_append* spec, b200_operator** out);
+
+/* Attention of new tokens over a cache that holds them already (and all before them):
+ *   x_rj = scale * <q_r, k_j>;  c = cap * tanh(x / cap) (cap > 0) or x;  s = c - slope[h] * (position_r - j)
+ *   out_r = sum_j softmax_j(s_rj) v_j, lse_r = log(sum_j exp(s_rj)) over the tokens j that r sees;  none: 0 and -infinity
+ * Row r sees token j <= position_r whose page is there, if the window is 0, j > position_r - window, or j < sinks.
+ * q, out are [tokens, heads, d], each key head serves heads / kv_heads query heads in a row, 1 <= d <= 128.
+ * What lies at tokens that are not seen, behind the last one in a page among them, has no influence, whatever it holds, beyond the last bits.
+ * Products, weights and sums are those of b200_attention; codes of 8 bits are multiplied exactly, beside 16-bit heads with weights of 11 bits. */
+typedef struct {
+  b200_cache cache;              /* read */
+  int32_t dtype;                 /* of q, out */
+  int32_t heads;
+  float scale, cap;              /* cap 0: none */
+  int64_t window, sinks;         /* window 0: none */
+  b200_operand q, out;
+  b200_operand lse;              /* single [tokens, heads], optional */
+  b200_operand slopes;           /* single [heads], optional */
+} b200_cache_attention;
+int b200_cache_attention_link(b200_dev* dev, const b200_cache_attention* spec, b200_operator** out);
+
+/* Chooses a token for each row of logits x [rows, vocab]:  w_i = exp((x_i - max x) / temperature).  In the order of falling x (of equal ones: of
+ * rising i) the first n tokens are kept, n the least of top_k (0 or less: vocab), of the fewest whose w add up to at least top_p times the sum over the
+ * first top_k (1 or more: all; at least one), and of the number of w >= min_p (more than 1: 1).  The token is the first kept one, in the order of i, at which
+ * the running sum of w exceeds uniform * (the kept sum) (uniform below 0 or undefined: 0; the last kept one where none does).
+ * logprob = log(w_token / kept sum).  temperature 0 or less: the first largest, logprob 0.  Undefined logits count as -infinity, which is never chosen; where
+ * there are infinite ones, those have w = 1 and the others 0.  A row of nothing else: token -1, logprob -infinity.
+ * Every setting is one number for all rows or a node of one a row.  1 <= vocab < 2^31. */
+typedef struct {
+  int64_t rows, vocab;
+  int32_t dtype;                 /* of the logits */
+  int32_t top_k;
+  float temperature, top_p, min_p;
+  b200_operand logits;
+  b200_operand uniform;          /* single [rows] */
+  b200_operand temperatures, top_ps, min_ps;   /* single [rows], each optional, in the place of the number */
+  b200_operand top_ks;           /* int32 [rows], optional */
+  b200_operand tokens;           /* int32 [rows] */
+  b200_operand logprob;          /* single [rows], optional */
+} b200_sample;
+int b200_sample_link(b200_dev* dev, const b200_sample* spec, b200_operator** out);
+
 #ifdef __cplusplus
 }
 #endif

@@ -267,6 +267,8 @@ def _spec(name: str, *fields):
                 setattr(self, f, Operand(-1, 0))
             elif t is Operand * 2:
                 setattr(self, f, t(Operand(-1, 0), Operand(-1, 0)))
+            elif issubclass(t, ctypes.Structure):
+                setattr(self, f, t())
         for k, v in values.items():
             setattr(self, k, v)
     cls.__init__ = init
@@ -284,7 +286,16 @@ AttentionSpec = _spec("AttentionSpec", ("batch", _i64), ("queries", _i64), ("key
                       ("dtype", _i32), ("mask", _i32), ("scale", _f32), ("cap", _f32),
                       *((n, Operand) for n in ("q", "k", "v", "out", "lse", "lengths", "prefix", "query_documents", "key_documents",
                                                "slopes", "d_out", "dq", "dk", "dv")))
+CacheSpec = _spec("CacheSpec", ("batch", _i64), ("tokens", _i64), ("pages", _i64), ("max_pages", _i64), ("page", _i32), ("kv_heads", _i32), ("d", _i32), ("dtype", _i32),
+                  *((n, Operand) for n in ("k", "v", "k_scale", "v_scale", "page_table", "lengths", "starts")))
+CacheAppendSpec = _spec("CacheAppendSpec", ("cache", CacheSpec), ("dtype", _i32), ("heads", _i32), ("pairs", _i32), ("interleaved", _i32), ("magnitude", _f32),
+                        ("frequencies", ctypes.POINTER(ctypes.c_double)), *((n, Operand) for n in ("positions", "k", "v", "q", "q_out")))
+CacheAttentionSpec = _spec("CacheAttentionSpec", ("cache", CacheSpec), ("dtype", _i32), ("heads", _i32), ("scale", _f32), ("cap", _f32), ("window", _i64), ("sinks", _i64),
+                           *((n, Operand) for n in ("q", "out", "lse", "slopes")))
+SampleSpec = _spec("SampleSpec", ("rows", _i64), ("vocab", _i64), ("dtype", _i32), ("top_k", _i32), ("temperature", _f32), ("top_p", _f32), ("min_p", _f32),
+                   *((n, Operand) for n in ("logits", "uniform", "temperatures", "top_ps", "min_ps", "top_ks", "tokens", "logprob")))
 DTYPE = {"single": 0, "bfloat16": 1, "half": 2}   # B200_F32, B200_BF16, B200_F16
+E4M3 = 3                                          # B200_E4M3: nodes of precision byte
 MASKS = {"none": 0, "causal": 1, "prefix": 2}
 
 
@@ -571,6 +582,94 @@ class Context:
         """The gradients of `attention`, from its inputs, its out and lse, and the gradient d_out of out."""
         return self._attention("attention_grad", q, k, dict(out=out, d_out=d_out, dq=dq), dict(v=v, dk=dk, dv=dv), lse, mask, prefix,
                                documents, lengths, slopes, scale, cap)
+
+    def _cache(self, what: str, prec: str, d: int, tokens: int, k_cache: str, v_cache: str, pages: str, lengths: str, starts, k_scale, v_scale) -> CacheSpec:
+        for n in (k_cache, pages, lengths):
+            if n not in self.arrays:
+                raise UserError(-5, "%s: the context holds no node '%s'" % (what, n))
+        c, table = self.arrays[k_cache][2], self.arrays[pages][2]
+        if len(c.dims) != 4 or c.dims[3] != d:
+            raise UserError(-5, "%s: node '%s' is not [pages, kv_heads, page, %d]" % (what, k_cache, d))
+        if len(table.dims) != 2:
+            raise UserError(-5, "%s: node '%s' is not [batch, max_pages]" % (what, pages))
+        coded = k_scale is not None or v_scale is not None
+        if coded and (k_scale is None or v_scale is None):
+            raise UserError(-5, "%s: k_scale and v_scale go together" % what)
+        (n, hk, page, _), b = c.dims, table.dims[0]
+        spec = CacheSpec(batch=b, tokens=tokens, pages=n, max_pages=table.dims[1], page=page, kv_heads=hk, d=d, dtype=E4M3 if coded else DTYPE[prec])
+        for names, p, dims in ((dict(k=k_cache, v=v_cache), "byte" if coded else prec, c.dims), (dict(k_scale=k_scale, v_scale=v_scale), "single", (n, hk)),
+                               (dict(page_table=pages), "int32", table.dims), (dict(lengths=lengths), "int32", (b,)), (dict(starts=starts), "int32", (b + 1,))):
+            for field, ident in names.items():
+                setattr(spec, field, self._operand(what, ident, p, dims))
+        return spec
+
+    def _rows_of_heads(self, what: str, ident: str) -> Tnode:
+        t = self._node(what, ident)
+        if len(t.dims) != 3:
+            raise UserError(-5, "%s: node '%s' is not [tokens, heads, d]" % (what, ident))
+        return t
+
+    def cache_append(self, k: str, v: str, k_cache: str, v_cache: str, pages: str, lengths: str, starts: Optional[str] = None,
+                     k_scale: Optional[str] = None, v_scale: Optional[str] = None, q: Optional[str] = None, q_out: Optional[str] = None,
+                     frequencies: Sequence[float] = (), magnitude: float = 1.0, positions: Optional[str] = None, layout: str = "half") -> Operator:
+        """New keys and values [tokens, kv_heads, d] go to their slots of a cache in pages [pages, kv_heads, page, d]; the keys, and queries
+        q [tokens, heads, d] (to q_out, which may be q), turn by their positions on the way as in `rotary` (no frequencies: they do not).
+        pages: an int32 node [batch, max_pages] of page numbers, lengths: int32 [batch], the new tokens included; starts: int32 [batch + 1],
+        the first row of each sequence's new tokens (without: as many rows each).  positions: int32 [tokens], others to turn by.
+        k_scale, v_scale: single nodes [pages, kv_heads]; with them the caches are nodes of precision byte that hold e4m3 codes."""
+        what = "cache_append"
+        if layout not in ("half", "interleaved"):
+            raise UserError(-5, "%s: unknown layout '%s'" % (what, layout))
+        if (q is None) != (q_out is None):
+            raise UserError(-5, "%s: q and q_out go together" % what)
+        t = self._rows_of_heads(what, k)
+        n, hk, d = t.dims
+        f = np.ascontiguousarray(frequencies, dtype=np.float64).reshape(-1)
+        spec = CacheAppendSpec(dtype=DTYPE[t.prec], pairs=f.size, interleaved=int(layout == "interleaved"), magnitude=magnitude,
+                               frequencies=f.ctypes.data_as(ctypes.POINTER(ctypes.c_double)), positions=self._operand(what, positions, "int32", (n,)),
+                               k=self._operand(what, k, t.prec, (n, hk, d)), v=self._operand(what, v, t.prec, (n, hk, d)))
+        if q is not None:
+            dims = (n, self._rows_of_heads(what, q).dims[1], d)
+            spec.heads, spec.q, spec.q_out = dims[1], self._operand(what, q, t.prec, dims), self._operand(what, q_out, t.prec, dims)
+        spec.cache = self._cache(what, t.prec, d, n, k_cache, v_cache, pages, lengths, starts, k_scale, v_scale)
+        if spec.cache.kv_heads != hk:
+            raise UserError(-5, "%s: node '%s' has %d heads, the cache %d" % (what, k, hk, spec.cache.kv_heads))
+        return Operator(self.device, "b200_cache_append_link", spec)
+
+    def cache_attention(self, q: str, k_cache: str, v_cache: str, out: str, pages: str, lengths: str, starts: Optional[str] = None,
+                        k_scale: Optional[str] = None, v_scale: Optional[str] = None, lse: Optional[str] = None, window: int = 0, sinks: int = 0,
+                        slopes: Optional[str] = None, scale: Optional[float] = None, cap: float = 0.0) -> Operator:
+        """Attention of new tokens q [tokens, heads, d] over a cache in pages that holds them (`cache_append`, which describes the cache's nodes).
+        A token sees those at its position and before it: all, or, with a window, the last `window` of them and the first `sinks`.
+        lse: single [tokens, heads].  slopes, scale, cap: as in `attention`."""
+        what = "cache_attention"
+        t = self._rows_of_heads(what, q)
+        n, h, d = t.dims
+        spec = CacheAttentionSpec(dtype=DTYPE[t.prec], heads=h, scale=1.0 / np.sqrt(d) if scale is None and d else scale or 0.0, cap=cap, window=window, sinks=sinks,
+                                  q=self._operand(what, q, t.prec, t.dims), out=self._operand(what, out, t.prec, t.dims),
+                                  lse=self._operand(what, lse, "single", (n, h)), slopes=self._operand(what, slopes, "single", (h,)),
+                                  cache=self._cache(what, t.prec, d, n, k_cache, v_cache, pages, lengths, starts, k_scale, v_scale))
+        return Operator(self.device, "b200_cache_attention_link", spec)
+
+    def sample(self, logits: str, uniform: str, tokens: str, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, logprob: Optional[str] = None) -> Operator:
+        """Chooses a token (int32 node `tokens`) for each row of logits [.., vocab] by the random number in [0, 1) of the single node
+        `uniform`, among the top_k largest (0: all) of them, the fewest that have top_p of their sum, and those of at least min_p times
+        the largest probability.  temperature 0: the largest.  Each setting is a number or a node of one a row (single, top_k int32).
+        logprob (single): the logarithm of the probability that the token had among those kept."""
+        what = "sample"
+        t = self._node(what, logits)
+        if not t.dims:
+            raise UserError(-5, "%s: node '%s' has no axis" % (what, logits))
+        rows, vocab = t.dims[:-1], t.dims[-1]
+        spec = SampleSpec(rows=t.num_elems // vocab if vocab else 0, vocab=vocab, dtype=DTYPE[t.prec], temperature=1.0, top_p=1.0,
+                          logits=self._operand(what, logits, t.prec, t.dims), uniform=self._operand(what, uniform, "single", rows),
+                          tokens=self._operand(what, tokens, "int32", rows), logprob=self._operand(what, logprob, "single", rows))
+        for field, value, prec in (("temperature", temperature, "single"), ("top_k", top_k, "int32"), ("top_p", top_p, "single"), ("min_p", min_p, "single")):
+            if isinstance(value, str):
+                setattr(spec, field + "s", self._operand(what, value, prec, rows))
+            else:
+                setattr(spec, field, value)
+        return Operator(self.device, "b200_sample_link", spec)
 
     # ---- host access (Context.set_values / get_values, arrayjit/lib/context.ml:322-395)
     def from_host(self, ident: str, arr: np.ndarray):

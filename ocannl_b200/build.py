@@ -12,8 +12,10 @@ used here to prove, at build time and without a GPU, that every kernel source co
 from __future__ import annotations
 
 import os
+import re
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -23,7 +25,7 @@ CUDA = os.environ.get("CUDA_HOME", "/usr/local/cuda")
 
 HOST_SOURCES = ["ir.cpp", "emit.cpp", "compile.cpp", "gemm_match.cpp", "attn_match.cpp", "driver.cpp", "runtime.cpp",
                 "gemm_launch.cpp", "api.cpp"]
-CUDA_SOURCES = ["sum_static.cu", "op_norm.cu", "op_rotary.cu", "op_attention.cu"]
+CUDA_SOURCES = ["sum_static.cu", "op_norm.cu", "op_rotary.cu", "op_attention.cu", "op_cache_append.cu", "op_cache_attention.cu", "op_sample.cu"]
 EMBED = {"kNumericsSource": "kernels/numerics.cuh", "kTcSource": "kernels/tc_sm100.cuh",
          "kGemmSource": "kernels/gemm_sm100.cuh", "kAttnSource": "kernels/attn_sm100.cuh",
          "kAttnRowsSource": "kernels/attn_rows.cuh"}
@@ -53,34 +55,49 @@ def _newer(target, deps):
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def _included(src, seen=None):
+    """The source and the files of this tree that it includes, at any depth."""
+    seen = set() if seen is None else seen
+    src = os.path.normpath(src)
+    if src in seen or not os.path.exists(src):
+        return seen
+    seen.add(src)
+    with open(src) as f:
+        for name in re.findall(r'^\s*#include "([^"]+)"', f.read(), re.M):
+            for folder in (os.path.dirname(src), CSRC):
+                _included(os.path.join(folder, name), seen)
+    return seen
+
+
+def _run_all(commands, verbose):
+    """Compilers, as many at a time as there are processors."""
+    def one(cmd):
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        subprocess.run(cmd, check=True)
+    with ThreadPoolExecutor(os.cpu_count() or 1) as pool:
+        list(pool.map(one, commands))
+
+
 def build_library(verbose=False) -> str:
     os.makedirs(OUT, exist_ok=True)
     emb = _embed()
-    srcs = [os.path.join(CSRC, s) for s in HOST_SOURCES] + [emb]
-    hdrs = [os.path.join(CSRC, h) for h in os.listdir(CSRC) if h.endswith(".hpp")]
-    hdrs.append(os.path.join(HERE, "..", "include", "b200.h"))
-    objs = []
-    for s in srcs:
+    objs, commands = [], []
+    for s in [os.path.join(CSRC, s) for s in HOST_SOURCES] + [emb]:
         o = os.path.join(OUT, os.path.basename(s)[:-4] + ".o")
-        if _newer(o, [s] + hdrs):
-            cmd = ["g++", "-std=c++17", "-O2", "-fPIC", "-Wall", "-Wno-unused-function", "-I", CSRC,
-                   "-I", os.path.join(CUDA, "include"), "-c", s, "-o", o]
-            if verbose:
-                print(" ".join(cmd))
-            subprocess.run(cmd, check=True)
+        if _newer(o, _included(s)):
+            commands.append(["g++", "-std=c++17", "-O2", "-fPIC", "-Wall", "-Wno-unused-function", "-I", CSRC,
+                             "-I", os.path.join(CUDA, "include"), "-c", s, "-o", o])
         objs.append(o)
     # translation units that hold ahead-of-time kernels: nvcc, sm_100a only
-    hdrs += [os.path.join(CSRC, "kernels", h) for h in os.listdir(os.path.join(CSRC, "kernels")) if h.endswith(".cuh")]
     for s in CUDA_SOURCES:
         src = os.path.join(CSRC, s)
         o = os.path.join(OUT, s[:-3] + ".o")
-        if _newer(o, [src] + hdrs):
-            cmd = [os.path.join(CUDA, "bin", "nvcc"), "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo",
-                   "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-I", CSRC, "-c", src, "-o", o]
-            if verbose:
-                print(" ".join(cmd))
-            subprocess.run(cmd, check=True)
+        if _newer(o, _included(src)):
+            commands.insert(0, [os.path.join(CUDA, "bin", "nvcc"), "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo",
+                                "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-I", CSRC, "-c", src, "-o", o])
         objs.append(o)
+    _run_all(commands, verbose)
     if _newer(LIB, objs):
         cmd = ["g++", "-shared", "-o", LIB] + objs + ["-L", os.path.join(CUDA, "lib64"), "-lcudart_static", "-lrt",
                                                        "-ldl", "-lpthread"]

@@ -196,17 +196,8 @@ extern "C" int b200_rotary_link(b200_dev* dev, const b200_rotary* p, b200_operat
     op->kernel = p->dtype == B200_F32 ? kernel_of<float>(vec, p->interleaved) : p->dtype == B200_BF16 ? kernel_of<__nv_bfloat16>(vec, p->interleaved) : kernel_of<__half>(vec, p->interleaved);
     ready(op->kernel);
     if (!a.pairs) return;
-    std::vector<unsigned long long> turns((size_t)a.pairs);
-    for (unsigned int i = 0; i < a.pairs; ++i) {
-      const long double whole = (long double)p->frequencies[i] / 6.283185307179586476925286766559005768L;
-      const long double part = whole - floorl(whole);               // the fraction of a turn, in [0, 1]
-      const long double scaled = roundl(part * 18446744073709551616.0L);
-      turns[i] = scaled >= 18446744073709551616.0L ? 0ull : (unsigned long long)scaled;
-    }
-    op->take_workspace(turns.size() * 8);
-    // (a copy from pageable memory has read its source when the call returns)
-    cu_check(cu().cuMemcpyHtoDAsync_(op->workspace, turns.data(), turns.size() * 8, dev->stream), "cuMemcpyHtoDAsync(frequencies)");
-    cu_check(cu().cuStreamSynchronize_(dev->stream), "cuStreamSynchronize");
+    op->take_workspace((size_t)a.pairs * 8);
+    write_turns(op, op->workspace, p->frequencies, p->pairs);
     a.turns = (const unsigned long long*)op->workspace;
   });
 }

@@ -4,6 +4,7 @@
 #pragma once
 #include <cuda_runtime.h>
 
+#include <cmath>
 #include <set>
 #include <string>
 #include <vector>
@@ -95,6 +96,20 @@ inline unsigned long long extent_product(std::initializer_list<long long> v, con
 
 inline void rt_check(cudaError_t e, const char* what) {
   if (e != cudaSuccess) throw Error((int)e, std::string(what) + ": " + cudaGetErrorString(e));
+}
+
+// Turns of pairs per position, [pairs], scaled by 2^64, into the operator's workspace at `at`.
+inline void write_turns(b200_operator* op, CUdeviceptr at, const double* frequencies, int pairs) {
+  std::vector<unsigned long long> turns((size_t)pairs);
+  for (int i = 0; i < pairs; ++i) {
+    const long double whole = (long double)frequencies[i] / 6.283185307179586476925286766559005768L;
+    const long double part = whole - floorl(whole);               // the fraction of a turn, in [0, 1]
+    const long double scaled = roundl(part * 18446744073709551616.0L);
+    turns[(size_t)i] = scaled >= 18446744073709551616.0L ? 0ull : (unsigned long long)scaled;
+  }
+  // (a copy from pageable memory has read its source when the call returns)
+  cu_check(cu().cuMemcpyHtoDAsync_(at, turns.data(), turns.size() * 8, op->dev->stream), "cuMemcpyHtoDAsync(frequencies)");
+  cu_check(cu().cuStreamSynchronize_(op->dev->stream), "cuStreamSynchronize");
 }
 
 // launches of operators on this thread, for the device's count (api.cpp)
