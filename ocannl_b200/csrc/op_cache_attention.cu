@@ -2,6 +2,7 @@
 #include <cmath>
 
 #include "cache.hpp"
+#include "kernels/cache_attn_few_sm100.cuh"
 #include "kernels/cache_attn_terms.cuh"
 
 using namespace b200;
@@ -36,24 +37,74 @@ __global__ void __launch_bounds__(256) cache_attention_rows(const __grid_constan
 }
 
 typedef void (*RowsKernel)(const CacheAttnArgs);
+typedef void (*FewKernel)(const CacheAttnArgs, const CacheFewArgs);
 
 struct CacheAttnOperator : b200_operator {
   CacheAttnArgs a = {};
   int dtype = 0;
   bool coded = false;
   RowsKernel rows = nullptr;
+  FewKernel few = nullptr;
+  CacheFewArgs few_args = {};
   unsigned int grid = 0;
+  size_t smem = 0;
+
+  template <class T>
+  void set_rows() { rows = coded ? cache_attention_rows<T, true> : cache_attention_rows<T, false>; }
+  template <class T, int DP>
+  void set_few() {
+    few = coded ? cache_attention_few<T, DP, true> : cache_attention_few<T, DP, false>;
+    smem = coded ? CacheFewShape<DP, true>::smem() : CacheFewShape<DP, false>::smem();
+  }
+  unsigned int blocks_of(long long n) const {
+    if (n >> 31) throw Error(B200_E_UNSUPPORTED, "cache_attention: too many rows");
+    return (unsigned int)n;
+  }
+  // whole 16-byte pieces of rows
+  bool pieces() const {
+    bool ok = dtype != B200_F32 && a.c.D % (coded ? 16 : 8) == 0 && ((long long)a.c.tokens * a.group >> 31) == 0;
+    for (const void* p : {a.q, (const void*)a.c.k, (const void*)a.c.v}) ok &= ((size_t)p & 15) == 0;
+    return ok;
+  }
   void choose() {
     const long long n = (long long)a.c.tokens * a.H;
     if (!n || !a.c.batch) return;
-    rows = dtype == B200_F32 ? (coded ? cache_attention_rows<float, true> : cache_attention_rows<float, false>)
-         : dtype == B200_BF16 ? (coded ? cache_attention_rows<__nv_bfloat16, true> : cache_attention_rows<__nv_bfloat16, false>)
-                              : (coded ? cache_attention_rows<__half, true> : cache_attention_rows<__half, false>);
+    if (pieces()) return choose_few();
+    if (dtype == B200_F32) set_rows<float>();
+    else if (dtype == B200_BF16) set_rows<__nv_bfloat16>();
+    else set_rows<__half>();
     ready(rows);
     grid = (unsigned int)std::min<long long>((n + 7) / 8, 16ll * dev->sm_count);
   }
+  void choose_few() {
+    const CacheArgs& c = a.c;
+    if (dtype == B200_BF16) c.D <= 64 ? set_few<__nv_bfloat16, 64>() : set_few<__nv_bfloat16, 128>();
+    else c.D <= 64 ? set_few<__half, 64>() : set_few<__half, 128>();
+    // Tiles of 16 rows: a sequence of n tokens has (n group + 15) / 16 of them.  Chunks of at least 256 tokens, as many as give every SM `kWaves` rounds of
+    // blocks; a tile adds one at most, those cut for their length aside.
+    const long long some = std::min(c.batch, c.tokens), tiles = ((long long)c.tokens * a.group + 15 * some) / 16 * c.HK;
+    const long long capacity = std::min<long long>((long long)c.max_pages * c.page, 0x7fffffff);
+    const int resident = smem <= 75 * 1024 ? 3 : 2, waves = 3;
+    few_args.target = (long long)dev->sm_count * resident * waves;
+    few_args.least = 256;
+    few_args.most = kFewMost;
+    few_args.by_group = Divisor((unsigned int)a.group);
+    few_args.by_key_heads = Divisor((unsigned int)c.HK);
+    const unsigned __int128 walk = (unsigned __int128)tiles * (unsigned long long)(capacity + 64);
+    const long long long_ones = walk / kCacheChunk > (1ull << 31) ? (1ll << 31) : (long long)(walk / kCacheChunk);
+    grid = blocks_of(std::min<long long>(std::max(few_args.target, long_ones) + tiles, (long long)std::min<unsigned __int128>(walk / 256 + (unsigned long long)tiles, 1ull << 31)));
+    const int width = c.D <= 64 ? 68 : 132;
+    const size_t parts = (size_t)grid * 16 * width * 4;
+    take_workspace(parts + (size_t)grid * 4);
+    few_args.parts = (float*)workspace;
+    few_args.tickets = (unsigned int*)(workspace + parts);
+    cu_check(cu().cuMemsetD8Async_(workspace + parts, 0, (size_t)grid * 4, dev->stream), "cuMemsetD8Async(tickets)");
+    ready(few, smem);
+  }
   void run(cudaStream_t s) override {
-    if (grid) launch(rows, dim3(grid), 256, 0, s, a);
+    if (!grid) return;
+    if (few) launch(few, dim3(grid), kCacheFewThreads, smem, s, a, few_args);
+    else launch(rows, dim3(grid), 256, 0, s, a);
   }
 };
 
