@@ -48,13 +48,23 @@ struct CacheAttnOperator : b200_operator {
   CacheFewArgs few_args = {};
   unsigned int grid = 0;
   size_t smem = 0;
+  int tile = 16, width = 0, resident = 1;      // rows of a tile, floats of a row of its parts, blocks of an SM
 
   template <class T>
   void set_rows() { rows = coded ? cache_attention_rows<T, true> : cache_attention_rows<T, false>; }
-  template <class T, int DP>
+  template <class T, int DP, bool CODED, int NR>
   void set_few() {
-    few = coded ? cache_attention_few<T, DP, true> : cache_attention_few<T, DP, false>;
-    smem = coded ? CacheFewShape<DP, true>::smem() : CacheFewShape<DP, false>::smem();
+    typedef CacheFewShape<DP, CODED, NR> Sh;
+    few = a.c.page % 16 == 0 ? cache_attention_few<T, DP, CODED, NR, true> : cache_attention_few<T, DP, CODED, NR, false>;
+    smem = Sh::smem();
+    tile = Sh::kRows;
+    width = Sh::kWidth;
+    resident = std::min<int>(Sh::kBlocks, 226 * 1024 / (Sh::smem() + 6 * 1024));
+  }
+  template <class T, int DP>
+  void set_few(bool wide) {
+    if (coded) wide ? set_few<T, DP, true, 2>() : set_few<T, DP, true, 1>();
+    else wide ? set_few<T, DP, false, 2>() : set_few<T, DP, false, 1>();
   }
   unsigned int blocks_of(long long n) const {
     if (n >> 31) throw Error(B200_E_UNSUPPORTED, "cache_attention: too many rows");
@@ -78,23 +88,34 @@ struct CacheAttnOperator : b200_operator {
   }
   void choose_few() {
     const CacheArgs& c = a.c;
-    if (dtype == B200_BF16) c.D <= 64 ? set_few<__nv_bfloat16, 64>() : set_few<__nv_bfloat16, 128>();
-    else c.D <= 64 ? set_few<__half, 64>() : set_few<__half, 128>();
-    // Tiles of 16 rows: a sequence of n tokens has (n group + 15) / 16 of them.  Chunks of at least 256 tokens, as many as give every SM `kWaves` rounds of
-    // blocks; a tile adds one at most, those cut for their length aside.
-    const long long some = std::min(c.batch, c.tokens), tiles = ((long long)c.tokens * a.group + 15 * some) / 16 * c.HK;
+    // (rows of a sequence, on average: up to 8 take tiles of 8)
+    const bool wide = (long long)c.tokens * a.group > 8ll * std::min(c.batch, c.tokens);
+    if (dtype == B200_BF16) c.D <= 64 ? set_few<__nv_bfloat16, 64>(wide) : set_few<__nv_bfloat16, 128>(wide);
+    else c.D <= 64 ? set_few<__half, 64>(wide) : set_few<__half, 128>(wide);
+    // A sequence of n tokens has n group rows, in tiles.  Chunks of about 512 tokens at least, as many as give every SM three rounds of blocks; a
+    // tile adds one at most, those cut for their length aside.
+    const long long some = std::min(c.batch, c.tokens), tiles = ((long long)c.tokens * a.group + (tile - 1) * some) / tile * c.HK;
     const long long capacity = std::min<long long>((long long)c.max_pages * c.page, 0x7fffffff);
-    const int resident = smem <= 75 * 1024 ? 3 : 2, waves = 3;
-    few_args.target = (long long)dev->sm_count * resident * waves;
-    few_args.least = 256;
+    few_args.target = (long long)dev->sm_count * resident * 3;
+    few_args.least = 512;
     few_args.most = kFewMost;
+    few_args.single = capacity < few_args.least + few_args.least / 2;
     few_args.by_group = Divisor((unsigned int)a.group);
     few_args.by_key_heads = Divisor((unsigned int)c.HK);
-    const unsigned __int128 walk = (unsigned __int128)tiles * (unsigned long long)(capacity + 64);
-    const long long long_ones = walk / kCacheChunk > (1ull << 31) ? (1ll << 31) : (long long)(walk / kCacheChunk);
-    grid = blocks_of(std::min<long long>(std::max(few_args.target, long_ones) + tiles, (long long)std::min<unsigned __int128>(walk / 256 + (unsigned long long)tiles, 1ull << 31)));
-    const int width = c.D <= 64 ? 68 : 132;
-    const size_t parts = (size_t)grid * 16 * width * 4;
+    if (few_args.single) {
+      grid = blocks_of(tiles);
+      if (!c.starts) {
+        const long long each = ((long long)c.each * a.group + tile - 1) / tile * c.HK;
+        few_args.by_units = Divisor(blocks_of(each));
+        grid = blocks_of(each * c.batch);
+      }
+    } else {
+      // (the nearest number of chunks: up to one and a half times the size each)
+      const unsigned __int128 walk = (unsigned __int128)tiles * (unsigned long long)(capacity + 64);
+      const unsigned __int128 cut = std::max<unsigned __int128>((unsigned long long)few_args.target, walk / kCacheChunk), least = walk / few_args.least;
+      grid = blocks_of((long long)std::min<unsigned __int128>(std::min(cut, least) + (unsigned long long)tiles, 1ull << 31));
+    }
+    const size_t parts = few_args.single ? 0 : (size_t)grid * tile * width * 4;
     take_workspace(parts + (size_t)grid * 4);
     few_args.parts = (float*)workspace;
     few_args.tickets = (unsigned int*)(workspace + parts);
