@@ -44,16 +44,19 @@ __device__ __forceinline__ unsigned int key_of(float x) {
 __device__ __forceinline__ float of_key(unsigned int k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
 struct Share {                         // of a block, for the others of its cluster to read
-  unsigned long long list[kList];      // of the first block: what is sorted
+  unsigned long long list[kList];      // logits that may be at the border
+  unsigned int listed;                 // entries of the list (more than it holds: it is of no use)
+  unsigned int joined;                 // of the first block: entries of the list that all blocks' go to
+  unsigned int joined_from;            // where this block's begin there
   double sums[kBins];
   unsigned int counts[kBins];
   double warp_sums[kWarps];
   unsigned int warp_counts[kWarps];
   float largest;
   unsigned int first;                  // an index
-  unsigned int listed;                 // entries of the list
-  float border;                        // what the first block has found: the last logit that is kept, and its index
+  float border;                        // of the first block: the last logit that is kept, and its index
   unsigned int border_at;
+  unsigned int interval[2];
   float scratch[kWarps];
   double joined_sums[kBins];           // over all blocks
   unsigned int joined_counts[kBins];
@@ -65,73 +68,102 @@ struct Pick {                          // a histogram's bin
   double sum_above;
 };
 
-// The row as the blocks of its cluster hold it: E logits a thread in registers (0: they are read from memory every time), VEC neighbours a lane, a warp's
-// all in one piece.
-template <class T, int E, int VEC>
+// The row as the blocks of its cluster hold it: E logits a thread in registers (0: they are read again every time), VEC neighbours of 16 bytes a lane, a warp's
+// all in one piece.  Places count from the 16 bytes that the row begins in: `off` of them lie ahead of it.
+template <class T, int E>
 struct Logits {
-  float x[E ? E : VEC];
-  const T* row;
-  unsigned int n, begin, lane, count;  // begin: of this lane's first vector; count: vectors of a lane (in memory)
-  __device__ __forceinline__ void fetch(unsigned int at, float* v) const {
-    if (at + VEC <= n) Vec<T, VEC>::load(row + at, v);
-    else
+  static constexpr int VEC = 16 / (int)sizeof(T), kAtOnce = sizeof(T) == 4 ? 4 : 2;
+  float x[E ? E : 1];
+  const T* row;                        // place 0
+  unsigned int off, end, begin, count; // places of the row: off .. end - 1; begin: of this lane's first vector; count: vectors of a lane
+  __device__ __forceinline__ bool whole(unsigned int at) const { return at >= off && at + VEC <= end; }
+  __device__ __forceinline__ void some(unsigned int at, float (&v)[VEC]) const {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) v[i] = at + i < n ? to_float(row[at + i]) : -INFINITY;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) v[i] = v[i] != v[i] ? -INFINITY : v[i] + 0.f;       // (undefined ones count as none; one zero)
+    for (int i = 0; i < VEC; ++i) v[i] = at + i >= off && at + i < end ? to_float(row[at + i]) : -INFINITY;
   }
   __device__ __forceinline__ Logits(const SampleArgs& a, unsigned int r, unsigned int part) {
     row = (const T*)a.x + (unsigned long long)r * a.vocab;
-    n = a.vocab;
-    lane = threadIdx.x & 31u;
-    // (beyond 2^32 a warp has nothing)
+    off = (unsigned int)((size_t)row / sizeof(T)) % VEC;
+    row -= off;
+    end = a.vocab + off;
+    const unsigned int lane = threadIdx.x & 31u;
     const unsigned long long from = (unsigned long long)(part * kWarps + (threadIdx.x >> 5)) * a.span;
-    begin = (unsigned int)min(from, (unsigned long long)n) + lane * VEC;
-    count = from < n ? (unsigned int)((min((unsigned long long)a.span, n - from) + 32 * VEC - 1) / (32 * VEC)) : 0u;
+    begin = (unsigned int)min(from, (unsigned long long)end) + lane * VEC;
+    count = from < end ? (unsigned int)((min((unsigned long long)a.span, end - from) + 32 * VEC - 1) / (32 * VEC)) : 0u;
     if constexpr (E > 0) {
 #pragma unroll
       for (int v = 0; v < E / VEC; ++v) {
-        if (v < (int)count) fetch(begin + v * 32 * VEC, x + v * VEC);
-        else
+        float y[VEC];
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) x[v * VEC + i] = -INFINITY;
+        for (int i = 0; i < VEC; ++i) y[i] = -INFINITY;
+        if (v < (int)count) some(begin + v * 32 * VEC, y);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) x[v * VEC + i] = y[i];
+      }
+    }
+  }
+  static constexpr int kBatch = E ? E : kAtOnce * VEC;
+  // f(logits, index of each), kBatch at a time, which are under way together; -infinity ahead of the row and behind it, and where a lane has no more.  The
+  // lanes of a warp come here together.
+  template <class F>
+  __device__ __forceinline__ void batches(F f) const {
+    if constexpr (E > 0) {
+      f(x, [&](int e) { return begin + (e / VEC) * 32 * VEC + e % VEC - off; });
+    } else {
+      for (unsigned int v = 0; v < count; v += kAtOnce) {
+        float y[kBatch];
+        const unsigned int at = begin + v * 32 * VEC;
+        Raw<T, VEC> r[kAtOnce];
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k)
+          if (v + k < count && whole(at + k * 32 * VEC)) r[k].load(row + at + k * 32 * VEC);
+          else r[k].clear();
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) {
+          float z[VEC];
+          r[k].values(z);
+          // (the row's first and last 16 bytes, and what lies behind a lane's last vector)
+          if (v + k >= count || !whole(at + k * 32 * VEC)) {
+            if (v + k < count) some(at + k * 32 * VEC, z);
+            else
+#pragma unroll
+              for (int i = 0; i < VEC; ++i) z[i] = -INFINITY;
+          }
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) y[k * VEC + i] = z[i];
+        }
+        f(y, [&](int e) { return at + (e / VEC) * 32 * VEC + e % VEC - off; });
       }
     }
   }
   // f(logit, index), in the order of the indices of a lane
   template <class F>
   __device__ __forceinline__ void each(F f) const {
-    if constexpr (E > 0) {
+    batches([&](const float(&y)[kBatch], auto index) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) f(x[e], begin + (e / VEC) * 32 * VEC + e % VEC);
-    } else {
-      for (unsigned int v = 0; v < count; ++v) {
-        float y[VEC];
-        fetch(begin + v * 32 * VEC, y);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) f(y[i], begin + v * 32 * VEC + i);
-      }
-    }
+      for (int e = 0; e < kBatch; ++e) f(y[e], index(e));
+    });
   }
   // f(logits, index of the first): false ends it, for the whole warp
   template <class F>
   __device__ __forceinline__ void each_vector(F f) const {
+    bool go = true;
     if constexpr (E > 0) {
-      bool go = true;
 #pragma unroll
       for (int v = 0; v < E / VEC; ++v)
         if (go && v < (int)count) {
           float y[VEC];
 #pragma unroll
           for (int i = 0; i < VEC; ++i) y[i] = x[v * VEC + i];
-          go = f(y, begin + v * 32 * VEC);
+          go = f(y, begin + v * 32 * VEC - off);
         }
     } else {
-      bool go = true;
       for (unsigned int v = 0; go && v < count; ++v) {
+        const unsigned int at = begin + v * 32 * VEC;
         float y[VEC];
-        fetch(begin + v * 32 * VEC, y);
-        go = f(y, begin + v * 32 * VEC);
+        if (whole(at)) Vec<T, VEC>::load(row + at, y);
+        else some(at, y);
+        go = f(y, at - off);
       }
     }
   }
@@ -174,35 +206,52 @@ __device__ __forceinline__ double block_before(double v, double* scratch, double
   return before;
 }
 
-// rising; entries n .. n2 - 1 are filled here, n2 a power of two
-__device__ __forceinline__ void sort_list(unsigned long long* list, unsigned int n, unsigned int n2) {
-  for (unsigned int i = n + threadIdx.x; i < n2; i += kThreads) list[i] = ~0ull;
+// Rising, n of at most kList entries.  A thread has four neighbours: pairs of a bitonic network lie in it, in its warp, or, 128 entries and more apart, in shared memory.
+__device__ __forceinline__ void sort_list(unsigned long long* list, unsigned int n) {
+  static_assert(kList == 4 * kThreads, "four entries a thread");
+  const unsigned int n2 = n <= 2 ? 2u : 1u << (32 - __clz((int)n - 1)), i0 = threadIdx.x * 4;
+  unsigned long long r[4];
   __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 4; ++k) r[k] = i0 + k < n ? list[i0 + k] : ~0ull;
   for (unsigned int size = 2; size <= n2; size <<= 1)
     for (unsigned int step = size >> 1; step; step >>= 1) {
-      for (unsigned int t = threadIdx.x; t < n2 / 2; t += kThreads) {
-        const unsigned int i = (t / step) * 2 * step + t % step, j = i + step;
-        const unsigned long long u = list[i], v = list[j];
-        if ((u > v) == ((i & size) == 0)) {
-          list[i] = v;
-          list[j] = u;
-        }
+      unsigned long long p[4];
+      if (step >= 128) {
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 4; ++k) list[i0 + k] = r[k];
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 4; ++k) p[k] = list[(i0 + k) ^ step];
+      } else if (step >= 4) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) p[k] = __shfl_xor_sync(0xffffffffu, r[k], step >> 2);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) p[k] = step == 2 ? r[k ^ 2] : r[k ^ 1];
       }
-      // (a warp's 32 pairs lie in 64 entries of their own once they are less than 64 apart)
-      if (step > 32 || n2 > 64 * kWarps) __syncthreads();
-      else if (step == 1) __syncthreads();
-      else __syncwarp();
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const bool least = (((i0 + k) & size) == 0) == (((i0 + k) & step) == 0);
+        r[k] = (p[k] < r[k]) == least ? p[k] : r[k];
+      }
+      if (n2 <= 128 && threadIdx.x >= 32) break;
     }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (i0 + k < n) list[i0 + k] = r[k];
+  __syncthreads();
 }
-__device__ __forceinline__ unsigned int power_above(unsigned int n) { return n <= 2 ? 2u : 1u << (32 - __clz((int)n - 1)); }
-
-template <class T, int E, int VEC>
+template <class T, int E>
 __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __grid_constant__ SampleArgs a) {
   extern __shared__ __align__(16) uint2 bins[];       // [warp][bin][lane]: sum of weights, count
   __shared__ Share sh;
   grid_begin();
   const unsigned int parts = a.parts, part = blockIdx.x % parts, row = blockIdx.x / parts, warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-  const Logits<T, E, VEC> logits(a, row, part);
+  constexpr int VEC = Logits<T, E>::VEC;
+  const Logits<T, E> logits(a, row, part);
   const float temperature = a.temperatures ? a.temperatures[row] : a.temperature, top_p = a.top_ps ? a.top_ps[row] : a.top_p;
   const float min_p = a.min_ps ? a.min_ps[row] : a.min_p, uniform = a.uniform[row];
   const int top_k = a.top_ks ? a.top_ks[row] : a.top_k;
@@ -215,13 +264,17 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
   logits.each([&](float x, unsigned int) { top = fmaxf(top, x); });
   top = warp_join(top, larger);
   if (lane == 0) sh.scratch[warp] = top;
-  if (threadIdx.x == 0) sh.listed = 0;
+  if (threadIdx.x == 0) sh.listed = sh.joined = 0;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kWarps; ++i) top = fmaxf(top, sh.scratch[i]);
   if (threadIdx.x == 0) sh.largest = top;
   meet(parts);
-  for (unsigned int p = 0; p < parts; ++p) top = fmaxf(top, of_part(&sh, parts, p)->largest);
+  // (of all blocks at once: a value of another block is some 700 cycles away)
+  if (parts > 1) {
+    const float other = lane < parts ? of_part(&sh, parts, lane)->largest : -INFINITY;
+    top = warp_join(other, larger);
+  }
   if (top == -INFINITY) {
     if (part == 0 && threadIdx.x == 0) {
       a.tokens[row] = -1;
@@ -250,37 +303,46 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
     meet(parts);
     return;
   }
-  // (never zero, so that -infinity stays that)
-  const float rate = fmaxf((float)(1.4426950408889634 / (double)temperature), 1e-37f);
+  // Binades below the largest weight.  (The rate is never zero, so that -infinity stays that, and never infinite, so that the largest has zero.)
+  const float rate = fminf(fmaxf((float)(1.4426950408889634 / (double)temperature), 1e-37f), 3e38f);
   const bool endless = top == INFINITY;
-  auto below = [&](float x) -> float { return x == top ? 0.f : endless ? INFINITY : (top - x) * rate; };      // binades below the largest weight
-  auto weight = [&](float x) -> float {
+  auto below = [&](float x) -> float {
+    if (endless) return x == top ? 0.f : INFINITY;        // (the same for all of a row)
+    return (top - x) * rate;
+  };
+  auto weight_at = [&](float z) -> float {
     float w;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(-below(x)));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(-z));
     return w;
   };
+  auto weight = [&](float x) -> float { return weight_at(below(x)); };
 
   // ---- the border: kept are logits above it, and those equal to it up to an index
   float border = -INFINITY;
-  unsigned int border_at = 0xffffffffu;
-  auto kept = [&](float x, unsigned int i) { return x > border || (x == border && i <= border_at && x != -INFINITY); };
+  unsigned int border_to = 0;          // indices of ties below it
+  // (without branches, as all that every logit passes)
+  auto kept = [&](float x, unsigned int i) { return (x > border) | ((x == border) & (i < border_to)); };
   bool by_count = top_k > 0 && (unsigned int)top_k < a.vocab;
   const bool by_sum = top_p < 1.f;
   const double share = fmax((double)top_p, 0.0);
 
-  // a histogram of the kept logits that `of` gives a bin (0: the highest); bins of all blocks, joined, in sh
-  auto histogram = [&](auto of) {
+  // the list that all blocks' entries go to, in the first one: where the histogram was
+  unsigned long long* const all_list = E > 0 ? sh.list : (unsigned long long*)bins;
+
+  // a histogram of the kept logits that `over` passes on and `of` gives a bin (0: the highest); bins of all blocks, joined, in sh
+  auto histogram = [&](auto over, auto of) {
     for (unsigned int i = threadIdx.x; i < kWarps * kBins * 32 / 2; i += kThreads) ((uint4*)bins)[i] = make_uint4(0u, 0u, 0u, 0u);
     __syncthreads();
     uint2* mine = bins + warp * kBins * 32 + lane;
-    logits.each([&](float x, unsigned int i) {
-      if (!kept(x, i)) return;
-      const int b = of(x);
-      if (b < 0) return;
-      uint2 v = mine[b * 32];
-      v.x = __float_as_uint(__uint_as_float(v.x) + weight(x));
-      ++v.y;
-      mine[b * 32] = v;
+    over([&](float x, unsigned int i) {
+      const float z = below(x), w = weight_at(z);
+      const int b = of(x, z);
+      if (kept(x, i) & (b >= 0)) {
+        uint2 v = mine[b * 32];
+        v.x = __float_as_uint(__uint_as_float(v.x) + w);
+        ++v.y;
+        mine[b * 32] = v;
+      }
     });
     __syncthreads();
     // eight threads a bin, a warp's columns each
@@ -289,10 +351,15 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
       double s = 0.0;
       unsigned int n = 0;
 #pragma unroll 4
-      for (unsigned int i = 0; i < 32; ++i) {
-        const uint2 v = bins[(w * kBins + b) * 32 + ((i + threadIdx.x) & 31u)];
-        s += (double)__uint_as_float(v.x);
-        n += v.y;
+      for (unsigned int i = 0; i < 32; i += 4) {
+        float some = 0.f;
+#pragma unroll
+        for (unsigned int k = 0; k < 4; ++k) {
+          const uint2 v = bins[(w * kBins + b) * 32 + ((i + k + threadIdx.x) & 31u)];
+          some += __uint_as_float(v.x);
+          n += v.y;
+        }
+        s += (double)some;
       }
 #pragma unroll
       for (int o = 4; o > 0; o >>= 1) {
@@ -306,58 +373,95 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
     }
     meet(parts);
     if (threadIdx.x < kBins) {
-      double s = 0.0;
-      unsigned int n = 0;
-      for (unsigned int p = 0; p < parts; ++p) {
-        const Share* o = of_part(&sh, parts, p);
-        s += o->sums[threadIdx.x];
-        n += o->counts[threadIdx.x];
+      double s = 0.0, of[kMostParts];
+      unsigned int n = 0, in[kMostParts];
+#pragma unroll
+      for (unsigned int p = 0; p < kMostParts; ++p) {
+        const Share* o = of_part(&sh, parts, p < parts ? p : 0);
+        of[p] = p < parts ? o->sums[threadIdx.x] : 0.0;
+        in[p] = p < parts ? o->counts[threadIdx.x] : 0u;
+      }
+#pragma unroll
+      for (unsigned int p = 0; p < kMostParts; ++p) {
+        s += of[p];
+        n += in[p];
       }
       sh.joined_sums[threadIdx.x] = s;
       sh.joined_counts[threadIdx.x] = n;
     }
     meet(parts);                       // (the shares are written again)
   };
+  auto whole_row = [&](auto f) { logits.each(f); };
+  // the count and the sum of all bins: a warp, a lane a bin
+  auto everything = [&](unsigned int& n, double& s) {
+    n = warp_join(sh.joined_counts[lane], add);
+    s = __shfl_sync(0xffffffffu, warp_up_to(sh.joined_sums[lane]), 31);
+  };
   // the bin in which a count, or a sum, is reached; the last one that holds anything where it never is
   auto find = [&](bool counting, double goal) {
-    Pick r = {0, 0, 0, 0.0};
-    unsigned int n = 0;
-    double s = 0.0;
-    for (unsigned int b = 0; b < kBins; ++b) {
-      const unsigned int m = sh.joined_counts[b];
-      if (!m) continue;
-      r.bin = b;
-      r.above = n;
-      r.in = m;
-      r.sum_above = s;
-      n += m;
-      s += sh.joined_sums[b];
-      if (counting ? (double)n >= goal : s >= goal) break;
-    }
+    const unsigned int m = sh.joined_counts[lane];
+    const double w = sh.joined_sums[lane];
+    const unsigned int n = warp_up_to(m);
+    const double s = warp_up_to(w);
+    const unsigned int any = __ballot_sync(0xffffffffu, m != 0u), far = __ballot_sync(0xffffffffu, m != 0u && (counting ? (double)n >= goal : s >= goal));
+    Pick r;
+    r.bin = far ? (unsigned int)__ffs((int)far) - 1u : any ? 31u - (unsigned int)__clz((int)any) : 0u;
+    r.in = __shfl_sync(0xffffffffu, m, r.bin);
+    r.above = __shfl_sync(0xffffffffu, n, r.bin) - r.in;
+    // (not the bin's sum taken off again, which would not give the one before exactly)
+    const double before = __shfl_up_sync(0xffffffffu, s, 1);
+    r.sum_above = __shfl_sync(0xffffffffu, lane ? before : 0.0, r.bin);
     return r;
   };
-  // puts the kept logits that `of` accepts into the first block's list
+  // puts the kept logits that `of` accepts into this block's list
   auto gather = [&](auto of) {
-    unsigned int n = 0;
-    logits.each([&](float x, unsigned int i) { n += kept(x, i) && of(x); });
-    const unsigned int up_to = warp_up_to(n);
-    unsigned int at = 0;
+    __syncthreads();
+    if (threadIdx.x == 0) sh.listed = 0;
+    __syncthreads();
+    logits.batches([&](const auto& y, auto index) {
+      unsigned int mask = 0;
+#pragma unroll
+      for (int e = 0; e < Logits<T, E>::kBatch; ++e) mask |= (kept(y[e], index(e)) & of(y[e])) ? 1u << e : 0u;
+      if (!__any_sync(0xffffffffu, mask)) return;
+      unsigned int at = mask ? atomicAdd(&sh.listed, (unsigned int)__popc((int)mask)) : 0u;
+#pragma unroll
+      for (int e = 0; e < Logits<T, E>::kBatch; ++e)
+        if (mask >> e & 1u) {
+          if (at < kList) sh.list[at] = (unsigned long long)~key_of(y[e] + 0.f) << 32 | index(e);       // (one zero)
+          ++at;
+        }
+    });
+    __syncthreads();
+  };
+  auto listed_logits = [&](auto f) {
+    for (unsigned int k = threadIdx.x; k < sh.listed; k += kThreads) f(of_key(~(unsigned int)(sh.list[k] >> 32)), (unsigned int)sh.list[k]);
+  };
+  // ... and those of the list that `of` accepts to the list of all blocks, kList in all
+  auto send = [&](auto of) {
+    if (E > 0) {
+      if (threadIdx.x == 0) sh.joined = sh.listed;
+      __syncthreads();
+      return;
+    }
     Share* first = of_part(&sh, parts, 0);
-    if (lane == 31 && up_to) at = atomicAdd(&first->listed, up_to);
-    at = __shfl_sync(0xffffffffu, at, 31) + up_to - n;
-    if (n)
-      logits.each([&](float x, unsigned int i) {
-        if (!kept(x, i) || !of(x)) return;
-        if (at < kList) first->list[at] = (unsigned long long)~key_of(x) << 32 | i;
-        ++at;
-      });
+    unsigned long long* to = parts > 1 ? cg::this_cluster().map_shared_rank(all_list, 0) : all_list;
+    const unsigned int n = min(sh.listed, (unsigned int)kList);
+    for (unsigned int k0 = 0; k0 < n; k0 += kThreads) {
+      const unsigned int k = k0 + threadIdx.x;
+      const bool on = k < n && of(of_key(~(unsigned int)(sh.list[k] >> 32)));
+      const unsigned int votes = __ballot_sync(0xffffffffu, on);
+      unsigned int at = 0;
+      if (lane == 0 && votes) at = atomicAdd(&first->joined, (unsigned int)__popc((int)votes));
+      at = __shfl_sync(0xffffffffu, at, 0) + (unsigned int)__popc((int)(votes & ((1u << lane) - 1u)));
+      if (on && at < kList) to[at] = sh.list[k];
+    }
     meet(parts);
   };
   auto logit_of = [&](unsigned long long entry) { return of_key(~(unsigned int)(entry >> 32)); };
   // The first n of the sorted list that reach a goal, by count or by sum: each thread has four entries.  `ahead`: the sum ahead of the list
   auto weights_of = [&](unsigned int n, float (&w)[4]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = threadIdx.x * 4 + i < n ? weight(logit_of(sh.list[threadIdx.x * 4 + i])) : 0.f;
+    for (int i = 0; i < 4; ++i) w[i] = threadIdx.x * 4 + i < n ? weight(logit_of(all_list[threadIdx.x * 4 + i])) : 0.f;
     return ((double)w[0] + w[1]) + ((double)w[2] + w[3]);
   };
   auto reach = [&](unsigned int n, double ahead, double goal) {
@@ -390,21 +494,26 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
   if (by_count || by_sum) {
     bool listed = false;               // the list holds all that may be kept
     double total = 0.0;                // of all logits' weights
-    auto level = [&](float x) { return min((int)(below(x) * 2.f), kBins - 1); };
+    // (half a binade a bin, rounded to the nearest by an addition)
+    auto level_at = [&](float z) { return (int)min(__float_as_uint(fmaf(z, 2.f, 8388608.f)) - 0x4b000000u, (unsigned int)(kBins - 1)); };
+    auto level = [&](float x) { return level_at(below(x)); };
+    auto by_level = [&](float, float z) { return level_at(z); };
     Pick at = {0, 0, 0, 0.0};
-    if (a.vocab <= kList) {
+    if (E > 0 || a.vocab <= kList) {
       gather([](float) { return true; });
+      send([](float) { return true; });
       listed = true;
     } else {
-      histogram(level);
-      unsigned int n = 0;
-      for (int b = 0; b < kBins; ++b) n += sh.joined_counts[b], total += sh.joined_sums[b];
+      histogram(whole_row, by_level);
+      unsigned int n;
+      everything(n, total);
       by_count = by_count && (unsigned int)top_k < n;
       if (by_count || by_sum) {
         at = find(by_count, by_count ? (double)top_k : share * total);
         if (at.above + at.in <= kList) {
           const int last = (int)at.bin;
           gather([&](float x) { return level(x) <= last; });
+          send([](float) { return true; });
           listed = true;
         }
       }
@@ -412,10 +521,10 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
     if (listed) {
       // ---- one block does the rest
       if (part != 0) return;
-      unsigned int n = min(sh.listed, (unsigned int)kList);
-      sort_list(sh.list, n, power_above(n));
+      unsigned int n = min(sh.joined, (unsigned int)kList);
+      sort_list(all_list, n);
       if (by_count) n = min(n, (unsigned int)top_k);
-      if (by_sum) n = reach(n, 0.0, share * (by_count || a.vocab <= kList ? sum_of(n) : total));
+      if (by_sum) n = reach(n, 0.0, share * (by_count || E > 0 || a.vocab <= kList ? sum_of(n) : total));
       float w[4];
       weights_of(n, w);
       // those above the least weight; in the order of the indices
@@ -424,7 +533,7 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const unsigned int k = threadIdx.x * 4 + i;
-        entry[i] = k < n ? sh.list[k] : 0ull;
+        entry[i] = k < n ? all_list[k] : 0ull;
         const bool on = k < n && w[i] > 0.f && (w[i] >= min_p || logit_of(entry[i]) == top);
         entry[i] = on ? entry[i] << 32 | entry[i] >> 32 : ~0ull;
         here += on;
@@ -432,19 +541,19 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (threadIdx.x * 4 + i < n) sh.list[threadIdx.x * 4 + i] = entry[i];
+        if (threadIdx.x * 4 + i < n) all_list[threadIdx.x * 4 + i] = entry[i];
       here = warp_join(here, add);
       if (lane == 0) sh.warp_counts[warp] = here;
       __syncthreads();
       here = 0;
 #pragma unroll
       for (int i = 0; i < kWarps; ++i) here += sh.warp_counts[i];
-      sort_list(sh.list, n, power_above(n));
+      sort_list(all_list, n);
       double all, up_to = 0.0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const unsigned int k = threadIdx.x * 4 + i;
-        w[i] = k < here ? weight(of_key(~(unsigned int)sh.list[k])) : 0.f;
+        w[i] = k < here ? weight(of_key(~(unsigned int)all_list[k])) : 0.f;
         up_to += w[i];
       }
       up_to = block_before(up_to, sh.block_sums, all);
@@ -462,7 +571,7 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
       __syncthreads();
       if (threadIdx.x == 0) {
         for (int i = 0; i < kWarps; ++i) found = min(found, sh.warp_counts[i]);
-        const unsigned long long e = sh.list[found];
+        const unsigned long long e = all_list[found];
         a.tokens[row] = (int)(unsigned int)(e >> 32);
         if (a.logprob) a.logprob[row] = (float)log((double)weight(of_key(~(unsigned int)e)) / all);
       }
@@ -474,69 +583,72 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
       double goal = (double)top_k;
       if (!counting) {
         if (by_count) {
-          histogram(level);
-          total = 0.0;
-          for (int b = 0; b < kBins; ++b) total += sh.joined_sums[b];
+          histogram(whole_row, by_level);
+          unsigned int n;
+          everything(n, total);
         }
         goal = share * total;
         at = find(false, goal);
       }
-      // the logits of the bin, as an interval of keys: where the bin's number changes (it never rises with the logit)
-      unsigned int lo = key_of(-INFINITY) + 1, hi = key_of(top);
-      {
-        unsigned int l = lo, h = hi;
-        while (l < h) {                // the least key of a bin up to this one
-          const unsigned int mid = l + (h - l) / 2;
-          if (level(of_key(mid)) <= (int)at.bin) h = mid;
-          else l = mid + 1;
+      // The logits of the bin, as an interval of keys: where the bin's number changes (it never rises with the logit).  A warp an end, 32 keys at a time.
+      if (warp < 2) {
+        const int bin = (int)at.bin - (int)warp;                         // the least key of a bin up to this one (none: one behind the largest)
+        unsigned int l = key_of(-INFINITY) + 1, h = key_of(top) + (bin < 0);
+        if (bin < 0) l = h;
+        while (l < h) {
+          const unsigned int step = (h - l) / 32 + 1, most = h - l, k = l + min(lane * step, most);
+          const unsigned int yes = __ballot_sync(0xffffffffu, level(of_key(k)) <= bin), n = yes ? (unsigned int)__ffs((int)yes) - 1u : 32u;
+          const unsigned int from = l;
+          if (n) l = from + min((n - 1u) * step, most) + 1u;             // (lanes before the first have a higher one)
+          if (n < 32u) h = from + min(n * step, most);
         }
-        const unsigned int least = l;
-        l = least, h = hi;
-        while (l < h) {                // the largest of this one
-          const unsigned int mid = h - (h - l) / 2;
-          if (level(of_key(mid)) >= (int)at.bin) l = mid;
-          else h = mid - 1;
-        }
-        lo = least;
-        hi = l;
+        if (lane == 0) sh.interval[warp] = h - warp;
       }
+      __syncthreads();
+      unsigned int lo = sh.interval[0], hi = sh.interval[1];
       unsigned int above = at.above;
       double sum_above = at.sum_above;
-      while (at.in > kList && lo < hi) {
+      bool have = false;               // the blocks' lists hold the interval
+      auto inside = [&](float x) { return (x >= of_key(lo)) & (x <= of_key(hi)); };
+      for (;;) {
+        // (where the lists are likely to hold it; an uneven row is passed again)
+        if (!have && (at.in <= kList || (lo < hi && at.in <= kList * parts / 4 * 3))) {
+          gather(inside);
+          meet(parts);
+          have = true;
+          have = __all_sync(0xffffffffu, lane >= parts || of_part(&sh, parts, lane)->listed <= kList);
+          meet(parts);
+        }
+        // (a few hundred are divided sooner than sorted, where no pass over the row is needed for it)
+        if (at.in <= (have ? kList / 4 : kList) || lo == hi) break;
         int bits = 0;
         while ((hi - lo) >> bits >= kBins) ++bits;
-        const unsigned int l = lo, h = hi;
-        histogram([&](float x) {
-          const unsigned int k = key_of(x);
-          return k < l || k > h ? -1 : (int)((h - k) >> bits);
-        });
+        auto split = [&](float x, float) { return inside(x) ? (int)((hi - key_of(x + 0.f)) >> bits) : -1; };
+        if (have) histogram(listed_logits, split);
+        else histogram(whole_row, split);
         at = find(counting, counting ? goal - above : goal - sum_above);
         above += at.above;
         sum_above += at.sum_above;
-        const unsigned int cut = h - (at.bin << bits);
-        lo = cut - l < (1u << bits) ? l : cut - (1u << bits) + 1;
+        const unsigned int cut = hi - (at.bin << bits);
+        lo = cut - lo < (1u << bits) ? lo : cut - (1u << bits) + 1;
         hi = cut;
       }
       if (at.in <= kList) {
-        const unsigned int l = lo, h = hi;
-        gather([&](float x) {
-          const unsigned int k = key_of(x);
-          return k >= l && k <= h;
-        });
+        send(inside);
         if (part == 0) {
-          const unsigned int n = min(sh.listed, (unsigned int)kList);
-          sort_list(sh.list, n, power_above(n));
+          const unsigned int n = min(sh.joined, (unsigned int)kList);
+          sort_list(all_list, n);
           const unsigned int many = counting ? min(max((unsigned int)top_k - above, 1u), n) : reach(n, sum_above, goal);
           if (threadIdx.x == 0) {
-            const unsigned long long e = sh.list[many - 1];
+            const unsigned long long e = all_list[many - 1];
             sh.border = logit_of(e);
             sh.border_at = (unsigned int)e;
-            sh.listed = 0;
+            sh.joined = 0;
           }
         }
         meet(parts);
         border = of_part(&sh, parts, 0)->border;
-        border_at = of_part(&sh, parts, 0)->border_at;
+        border_to = of_part(&sh, parts, 0)->border_at + 1u;
         meet(parts);
       } else {
         // many equal ones: as many as are wanted of them, in the order of their indices
@@ -569,7 +681,7 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
         }
         meet(parts);
         border = value;
-        border_at = of_part(&sh, parts, 0)->border_at;
+        border_to = of_part(&sh, parts, 0)->border_at + 1u;
         meet(parts);
       }
     }
@@ -577,26 +689,35 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
 
   // ---- the token: in which warp the running sum passes the goal, then where in it
   auto chance = [&](float x, unsigned int i) -> float {
-    if (!kept(x, i)) return 0.f;
     const float w = weight(x);
-    return w >= min_p || x == top ? w : 0.f;
+    return kept(x, i) & ((w >= min_p) | (x == top)) ? w : 0.f;
   };
   double mine = 0.0;
-  logits.each([&](float x, unsigned int i) { mine += (double)chance(x, i); });
+  logits.batches([&](const auto& y, auto index) {
+    float some = 0.f;
+#pragma unroll
+    for (int e = 0; e < Logits<T, E>::kBatch; ++e) some += chance(y[e], index(e));
+    mine += (double)some;
+  });
   mine = warp_join(mine, add);
   if (lane == 0) sh.warp_sums[warp] = mine;
   meet(parts);
-  double total = 0.0, before = 0.0;
-  unsigned int last_any = 0;           // the last warp that has any
-  for (unsigned int p = 0; p < parts; ++p)
-    for (unsigned int i = 0; i < kWarps; ++i) {
-      if (p == part && i == warp) before = total;
-      const double s = of_part(&sh, parts, p)->warp_sums[i];
-      if (s > 0.0) last_any = p * kWarps + i;
-      total += s;
-    }
-  const double goal = (uniform > 0.f ? (double)uniform : 0.0) * total;
-  const bool owner = goal < total ? before <= goal && before + mine > goal : part * kWarps + warp == last_any;
+  // two warps' sums a lane, and where they end; all warps count the same way
+  double two[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const unsigned int w = 2 * lane + k;
+    two[k] = w < parts * kWarps ? of_part(&sh, parts, w / kWarps)->warp_sums[w % kWarps] : 0.0;
+  }
+  const double up_to = warp_up_to(two[0] + two[1]), up_to_before = __shfl_up_sync(0xffffffffu, up_to, 1), ahead = lane ? up_to_before : 0.0, middle = ahead + two[0];
+  const double total = __shfl_sync(0xffffffffu, up_to, 31), goal = (uniform > 0.f ? (double)uniform : 0.0) * total;
+  // the first that passes the goal, or the last that has any
+  unsigned int which = warp_join(two[0] > 0.0 && middle > goal ? 2 * lane : two[1] > 0.0 && up_to > goal ? 2 * lane + 1u : 0xffffffffu, smaller);
+  const unsigned int last_any = warp_join(two[1] > 0.0 ? 2 * lane + 1u : two[0] > 0.0 ? 2 * lane : 0u, larger);
+  if (which == 0xffffffffu) which = last_any;
+  const double even = __shfl_sync(0xffffffffu, ahead, which / 2), odd = __shfl_sync(0xffffffffu, middle, which / 2);
+  double before = which & 1u ? odd : even;
+  const bool owner = part * kWarps + warp == which;
   if (owner) {
     unsigned int last = 0xffffffffu, found = 0xffffffffu;
     float last_w = 0.f, found_w = 0.f;
@@ -645,17 +766,17 @@ struct SampleOperator : b200_operator {
   size_t smem = 0;
 
   template <class T>
-  void choose(bool vec) {
-    constexpr int V = 16 / (int)sizeof(T);
-    // Rows of up to a list's length lie in registers, a block each.  Longer ones are read again in every pass, from L2: a block of 16384 logits where the
-    // rows fill the machine, of 4096 where they do not, eight at most.
+  void choose() {
+    constexpr unsigned int V = 16 / (unsigned int)sizeof(T), piece = 32 * V;
+    // Rows of up to a list's length lie in registers, a block each.  Longer ones are read again in every pass, from L2, by up to eight blocks of 2048 logits
+    // at least, seven blocks an SM: more of them wait for one another more often than the shorter passes gain (256 rows of 131072 logits: 1, 2, 4, 8 blocks
+    // a row take 339, 207, 188, 228 us).
     const unsigned int n = a.vocab;
-    const auto blocks = [&](unsigned int each) { return (unsigned int)std::min<unsigned long long>(kMostParts, ((unsigned long long)n + each - 1) / each); };
-    const bool small = n <= (unsigned int)kList;
-    a.parts = small ? 1u : (unsigned long long)a.rows * blocks(4096) <= 3ull * dev->sm_count ? blocks(4096) : blocks(16384);
-    const unsigned int piece = 32u * (vec ? (unsigned int)V : 1u);
-    a.span = small ? 32u * (V == 8 ? 8u : 4u) : (unsigned int)(((unsigned long long)n + a.parts * kWarps * piece - 1) / (a.parts * kWarps * piece) * piece);
-    kernel = small ? (vec ? sample_rows<T, V == 8 ? 8 : 4, V> : sample_rows<T, V == 8 ? 8 : 4, 1>) : (vec ? sample_rows<T, 0, V> : sample_rows<T, 0, 1>);
+    const bool small = n + V <= (unsigned int)kList;
+    const auto blocks = [&](unsigned long long each) { return (n + each - 1) / each; };
+    a.parts = small ? 1u : (unsigned int)std::max(1ull, std::min(std::min((unsigned long long)kMostParts, blocks(2048)), 7ull * (unsigned int)dev->sm_count / a.rows));
+    a.span = small ? 32u * 8u : (unsigned int)(((unsigned long long)n + V + a.parts * kWarps * piece - 1) / (a.parts * kWarps * piece) * piece);
+    kernel = small ? sample_rows<T, 8> : sample_rows<T, 0>;
     smem = small ? 0 : (size_t)kWarps * kBins * 32 * 8;
     ready(kernel, smem);
   }
@@ -706,11 +827,9 @@ extern "C" int b200_sample_link(b200_dev* dev, const b200_sample* p, b200_operat
     a.min_p = p->min_p;
     a.top_k = p->top_k;
     if (!a.rows) return;
-    const size_t size = dtype_bytes(p->dtype);
-    const bool vec = ((size_t)a.x & 15) == 0 && (size_t)a.vocab * size % 16 == 0;
-    if (p->dtype == B200_F32) op->choose<float>(vec);
-    else if (p->dtype == B200_BF16) op->choose<__nv_bfloat16>(vec);
-    else op->choose<__half>(vec);
+    if (p->dtype == B200_F32) op->choose<float>();
+    else if (p->dtype == B200_BF16) op->choose<__nv_bfloat16>();
+    else op->choose<__half>();
     if ((unsigned long long)a.rows * a.parts >> 31) ops.refuse("too many rows", B200_E_UNSUPPORTED);
   });
 }
