@@ -3,7 +3,20 @@
 #include "kernels/cache_terms.cuh"
 #include "operators.hpp"
 
+struct b200_tmap;
+
 namespace b200 {
+
+// The kernel of attention over a paged cache for many new tokens (op_cache_prompts.cu): of 16-bit types, for heads of up to 64 or 128 elements, one or two row
+// tiles a block.
+struct CacheAttnArgs;
+struct CacheTileArgs;
+struct CacheTiles {
+  void (*kernel)(const b200_tmap, const b200_tmap, const b200_tmap, const CacheAttnArgs, const CacheTileArgs);
+  unsigned int threads;
+  size_t smem;
+};
+CacheTiles cache_tiles(int dtype, bool coded, bool wide, bool two);
 
 // `written`: the caches and their scales are outputs
 inline CacheArgs bind_cache(Operands& ops, const b200_cache& p, int dtype, bool written) {

@@ -72,11 +72,6 @@ __device__ __forceinline__ unsigned int transpose8(unsigned int x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-// the values of four codes, as two pairs of halves
-__device__ __forceinline__ void e4m3_split(unsigned int w, unsigned int& lo, unsigned int& hi) {
-  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
-}
-
 // What a sequence's tiles look at: its rows of a key head, in tiles, and no fewer tokens than any of them sees, as they are walked
 struct CacheWalk {
   unsigned int tiles;

@@ -63,6 +63,10 @@ __device__ __forceinline__ unsigned int e4m3_halves(unsigned int w) {
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((unsigned short)w));
   return r;
 }
+// the values of four codes, as two pairs of halves
+__device__ __forceinline__ void e4m3_split(unsigned int w, unsigned int& lo, unsigned int& hi) {
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
+}
 __device__ __forceinline__ float2 e4m3_unpack2(unsigned int w) {
   const unsigned int r = e4m3_halves(w);
   return __half22float2(*(const __half2*)&r);

@@ -1,8 +1,10 @@
 // Attention over a paged cache (b200_cache_attention_link): the choice of kernels and their launch.
 #include <cmath>
+#include <cstring>
 
 #include "cache.hpp"
 #include "kernels/cache_attn_few_sm100.cuh"
+#include "kernels/cache_attn_fwd_sm100.cuh"
 #include "kernels/cache_attn_terms.cuh"
 
 using namespace b200;
@@ -39,6 +41,20 @@ __global__ void __launch_bounds__(256) cache_attention_rows(const __grid_constan
 typedef void (*RowsKernel)(const CacheAttnArgs);
 typedef void (*FewKernel)(const CacheAttnArgs, const CacheFewArgs);
 
+// [dims[3]][dims[2]][dims[1]][dims[0]] elements in boxes of box[0] x box[1] x 1 x box[3]; 16-bit ones swizzled as the tensor cores read them
+b200_tmap box_map(const void* p, CUtensorMapDataType type, int size, const cuuint64_t (&dims)[4], const cuuint32_t (&box)[4]) {
+  CUtensorMap map;
+  const cuuint64_t strides[3] = {dims[0] * size, dims[0] * dims[1] * size, dims[0] * dims[1] * dims[2] * size};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUresult r = cu().cuTensorMapEncodeTiled_(&map, type, 4, (void*)p, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                                  size == 1 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) throw Error(B200_E_UNSUPPORTED, "cache_attention: a node's layout cannot be described to the TMA unit (CUresult " + std::to_string((int)r) + ")");
+  static_assert(sizeof(b200_tmap) == sizeof(CUtensorMap), "tensor map");
+  b200_tmap m;
+  memcpy(&m, &map, sizeof m);
+  return m;
+}
+
 struct CacheAttnOperator : b200_operator {
   CacheAttnArgs a = {};
   int dtype = 0;
@@ -46,6 +62,9 @@ struct CacheAttnOperator : b200_operator {
   RowsKernel rows = nullptr;
   FewKernel few = nullptr;
   CacheFewArgs few_args = {};
+  CacheTiles tiles = {};
+  CacheTileArgs tile_args = {};
+  b200_tmap map_q, map_k, map_v;
   unsigned int grid = 0;
   size_t smem = 0;
   int tile = 16, width = 0, resident = 1;      // rows of a tile, floats of a row of its parts, blocks of an SM
@@ -79,12 +98,38 @@ struct CacheAttnOperator : b200_operator {
   void choose() {
     const long long n = (long long)a.c.tokens * a.H;
     if (!n || !a.c.batch) return;
-    if (pieces()) return choose_few();
+    if (pieces()) return many() ? choose_tiles() : choose_few();
     if (dtype == B200_F32) set_rows<float>();
     else if (dtype == B200_BF16) set_rows<__nv_bfloat16>();
     else set_rows<__half>();
     ready(rows);
     grid = (unsigned int)std::min<long long>((n + 7) / 8, 16ll * dev->sm_count);
+  }
+  // Whole prompts: tiles of 128 rows on the tensor cores, where sequences have them on average and the cache's pages are boxes of the TMA unit.
+  bool many() const {
+    const CacheArgs& c = a.c;
+    const bool boxes = c.n_pages && c.page % 16 == 0 && (c.page % 64 == 0 || 64 % c.page == 0);
+    return boxes && a.group <= 128 && ((size_t)a.out & 15) == 0 && (long long)c.tokens * a.group >= 128ll * std::min(c.batch, c.tokens);
+  }
+  void choose_tiles() {
+    const CacheArgs& c = a.c;
+    tile_args.tokens = 128 / a.group;
+    tile_args.box = c.page % 64 == 0 ? 64 : (int)c.page;
+    tile_args.by_group = Divisor((unsigned int)a.group);
+    tile_args.by_key_heads = Divisor((unsigned int)c.HK);
+    const long long capacity = (long long)c.max_pages * c.page, some = std::min(c.batch, c.tokens);
+    auto blocks = [&](int nq) { return (c.tokens + (nq * tile_args.tokens - 1) * some) / (nq * tile_args.tokens) * c.HK; };
+    tile_args.sums = capacity > kSumKeys;
+    // Two row tiles a block share their keys, unless that leaves SMs without a block, or there are sums beside the accumulators.
+    const bool two = !tile_args.sums && (long long)c.tokens / (2 * tile_args.tokens) * c.HK >= dev->sm_count;
+    tiles = cache_tiles(dtype, coded, c.D > 64, two);
+    grid = blocks_of(blocks(two ? 2 : 1));
+    const CUtensorMapDataType type = dtype == B200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const cuuint64_t of_q[4] = {(cuuint64_t)c.D, (cuuint64_t)a.group, (cuuint64_t)c.HK, (cuuint64_t)c.tokens}, of_c[4] = {(cuuint64_t)c.D, c.page, (cuuint64_t)c.HK, c.n_pages};
+    const cuuint32_t box_q[4] = {64, (cuuint32_t)a.group, 1, (cuuint32_t)tile_args.tokens}, box_c[4] = {coded ? (c.D > 64 ? 128u : 64u) : 64u, (cuuint32_t)tile_args.box, 1, 1};
+    map_q = box_map(a.q, type, 2, of_q, box_q);
+    map_k = box_map(c.k, coded ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : type, coded ? 1 : 2, of_c, box_c);
+    map_v = box_map(c.v, coded ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : type, coded ? 1 : 2, of_c, box_c);
   }
   void choose_few() {
     const CacheArgs& c = a.c;
@@ -124,7 +169,8 @@ struct CacheAttnOperator : b200_operator {
   }
   void run(cudaStream_t s) override {
     if (!grid) return;
-    if (few) launch(few, dim3(grid), kCacheFewThreads, smem, s, a, few_args);
+    if (tiles.kernel) launch(tiles.kernel, dim3(grid), tiles.threads, tiles.smem, s, map_q, map_k, map_v, a, tile_args);
+    else if (few) launch(few, dim3(grid), kCacheFewThreads, smem, s, a, few_args);
     else launch(rows, dim3(grid), 256, 0, s, a);
   }
 };

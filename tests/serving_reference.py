@@ -179,38 +179,45 @@ def attention(q, k_cache, v_cache, table, lengths, starts, page, prec, k_scale=N
     pages, hk = k_cache.shape[:2]
     coded = k_scale is not None
     scale = 1.0 / np.sqrt(d) if scale is None else scale
-    out, lse, off = np.full(q.shape, np.nan), np.full((n, h), np.nan), np.zeros(q.shape)
-    lse_off = np.zeros((n, h))
+    out, lse, off, lse_off = np.full(q.shape, np.nan), np.full((n, h), np.nan), np.zeros(q.shape), np.zeros((n, h))
     half = EPS[prec] / 2
+    of_weights = 0.0 if prec == "single" else 2.0 ** -11 if coded else half
     for b, (rows, pos0) in enumerate(rows_of(lengths, starts, n, table.shape[0])):
-        for i, r in enumerate(rows):
-            pos = pos0 + i
-            js = [j for j in range(min(pos + 1, table.shape[1] * page)) if (not window or j > pos - window or j < sinks) and place(table, pages, page, b, j)]
-            if not js:
-                out[r], lse[r] = 0.0, -np.inf
-                continue
-            at = [place(table, pages, page, b, j) for j in js]
-            p, s = np.array([a[0] for a in at]), np.array([a[1] for a in at])
-            for g in range(hk):
-                k, v = k_cache[p, g, s], v_cache[p, g, s]
-                flat = np.abs(v).sum(0)
-                if coded:
-                    k, v = decode(k) * k_scale[p, g][:, None], decode(v)
-                    flat = np.abs(v).sum(0) * v_scale[p, g].max()
-                    v = v * v_scale[p, g][:, None]
-                for hh in range(g * (h // hk), (g + 1) * (h // hk)):
-                    with np.errstate(all="ignore"):
-                        z = k @ q[r, hh] * scale
-                        z = cap * np.tanh(z / cap) if cap else z
-                        z = z - (0.0 if slopes is None else slopes[hh]) * (pos - np.array(js))
-                        top = z.max()
-                        e = np.exp(z - top)
-                        w = e / e.sum()
-                        out[r, hh], lse[r, hh] = w @ v, top + np.log(e.sum())
-                    size = w @ np.abs(v)
-                    of_weights = 0.0 if prec == "single" else 2.0 ** -11 if coded else half
-                    off[r, hh] = half * np.abs(out[r, hh]) + (of_weights + ARITH) * size + (2.0 ** -25 * (flat + 1) if prec == "half" or (coded and prec != "single") else 1e-30)
-                    lse_off[r, hh] = ARITH * (1 + abs(lse[r, hh])) if np.isfinite(lse[r, hh]) else 0.0
+        if not len(rows):
+            continue
+        rows, pos = np.array(rows), pos0 + np.arange(len(rows))[:, None]
+        j = np.arange(max(0, min(int(pos[-1, 0]) + 1, table.shape[1] * page)))
+        p = table[b, j // page]
+        there = (p >= 0) & (p < pages)
+        seen = (j <= pos) & there
+        if window:
+            seen &= (j > pos - window) | (j < sinks)
+        used = seen.any(0)
+        p, slot = np.where(used, p, 0), j % page
+        for g in range(hk):
+            k, v = k_cache[p, g, slot], v_cache[p, g, slot]
+            if coded:
+                k, v = decode(k) * k_scale[p, g][:, None], decode(v)
+            k, v = np.where(used[:, None], k, 0.0), np.where(used[:, None], v, 0.0)
+            # (rows below the largest weight of a half: sizes of all values that a row sees)
+            flat = seen @ np.abs(v)
+            if coded:
+                flat = flat * np.where(seen, v_scale[p, g], 0.0).max(1, initial=0.0)[:, None]
+                v = v * np.where(used, v_scale[p, g], 0.0)[:, None]
+            for hh in range(g * (h // hk), (g + 1) * (h // hk)):
+                with np.errstate(all="ignore"):
+                    z = q[rows, hh] @ k.T * scale
+                    z = cap * np.tanh(z / cap) if cap else z
+                    z = z - (0.0 if slopes is None else slopes[hh]) * (pos - j)
+                    z = np.where(seen, z, -np.inf)
+                    top = z.max(1, initial=-np.inf, keepdims=True)
+                    e = np.where(seen, np.exp(z - np.where(np.isinf(top), 0.0, top)), 0.0)
+                    total = e.sum(1, keepdims=True)
+                    w = e / np.where(total == 0.0, 1.0, total)
+                    out[rows, hh], lse[rows, hh] = w @ v, (top + np.log(total))[:, 0]
+                size = w @ np.abs(v)
+                off[rows, hh] = half * np.abs(out[rows, hh]) + (of_weights + ARITH) * size + (2.0 ** -25 * (flat + 1) if prec == "half" or (coded and prec != "single") else 1e-30)
+                lse_off[rows, hh] = np.where(np.isfinite(lse[rows, hh]), ARITH * (1 + np.abs(np.where(np.isfinite(lse[rows, hh]), lse[rows, hh], 0.0))), 0.0)
     return out, lse, off, lse_off
 
 

@@ -307,6 +307,42 @@ def test_attention_over_pages(device, case, prec, coded):
         nodes.free()
 
 
+# prompts: rows enough for tiles of 128 on the tensor cores
+PROMPTS = [
+    (1, 128, [128], 64, 2, 2, 128, 0, 0, 0.0, False),
+    (2, [100, 300], [700, 300], 16, 2, 8, 128, 0, 0, 0.0, False),
+    (3, [64, 0, 200], [64, 9, 1000], 32, 1, 5, 96, 150, 20, 0.0, True),
+    (2, [90, 33], [513, 129], 64, 2, 6, 64, 0, 0, 20.0, False),
+    (1, 260, [1000], 128, 1, 20, 80, 200, 70, 0.0, False),
+    (2, [200, 70], [190, 300], 64, 1, 4, 48, 0, 0, 5.0, True),
+    (5, 40, [40, 100, 300, 77, 64], 16, 4, 16, 64, 33, 2, 0.0, False),
+    (1, 1, [50], 16, 1, 128, 64, 0, 0, 0.0, False),
+    (2, [1300, 1100], [1300, 1900], 32, 2, 16, 64, 0, 0, 0.0, False),
+    (3, [700, 800, 900], [700, 2000, 900], 64, 2, 16, 128, 300, 5, 30.0, False),
+    (1, 130, [17000], 64, 1, 2, 64, 0, 0, 0.0, False),
+    (1, 70, [34000], 16, 1, 2, 128, 0, 0, 0.0, False),
+]
+
+
+@pytest.mark.parametrize("coded", [False, True])
+@pytest.mark.parametrize("prec", ["bfloat16", "half"])
+@pytest.mark.parametrize("case", PROMPTS)
+def test_prompts_over_pages(device, case, prec, coded):
+    x, table, lengths, starts, page, t = attend_case(case, prec, coded)
+    want = want_attend(x, table, lengths, starts, page, prec, t)
+    nodes = attend_nodes(device, x, prec, table, lengths, starts)
+    op = link_attend(nodes, x, starts, t)
+    op.run()
+    device.await_()
+    check_attend(nodes, want)
+    first = nodes.raw("out")
+    op.run()
+    device.await_()
+    assert nodes.raw("out").tobytes() == first.tobytes()
+    op.free()
+    nodes.free()
+
+
 # ------------------------------------------------------------------ choosing a token
 SAMPLE = [   # (rows, vocab, what the rows hold)
     (3, 1, "logits"), (7, 27, "logits"), (33, 27, "ties"), (5, 1000, "logits"), (4, 1023, "hidden"), (3, 5000, "ties"), (4, 4097, "flat"),
