@@ -92,6 +92,80 @@ __device__ __forceinline__ unsigned int cache_chunks(const CacheFewArgs& f, int 
   return min(max(n, 1u), (unsigned int)f.most);
 }
 
+// A block's chunk: of a sequence, a tile of its rows of a key head, and how the tile's tokens are walked.
+struct CachePlan {
+  int b, hk, first_row, rows;          // rows of the tile that there are
+  CacheSeq s;
+  unsigned int chunks, first_unit;     // of the tile; the number of its first block
+  int least_pos, most_pos, end;        // positions of its rows; tokens that some row sees lie before `end`
+  int sink_end, shift;                 // the walk: tokens 0 .. sink_end - 1, then those from sink_end + shift on
+  int begin, stop;                     // of the walk, this chunk's
+  __device__ __forceinline__ int token_of(int v) const { return v < sink_end ? v : v + shift; }
+};
+template <int NT, int ROWS>
+__device__ __forceinline__ bool cache_plan(const CacheAttnArgs& a, const CacheFewArgs& f, CachePlan& p) {
+  const CacheArgs& c = a.c;
+  __shared__ unsigned long long works[NT / 32];
+  unsigned int nth;
+  p.chunks = 1;
+  if (f.single && !c.starts) {
+    p.b = (int)f.by_units.of(blockIdx.x);
+    nth = blockIdx.x - (unsigned int)p.b * f.by_units.d;
+    if (p.b >= c.batch) return false;
+  } else {
+    int size = 0x7fffffff;
+    if (!f.single) {
+      unsigned long long work = 0;
+      for (int i = (int)threadIdx.x; i < c.batch; i += NT) {
+        const CacheSeq s = cache_seq(c, i);
+        if (s.count) {
+          const CacheWalk w = cache_walk<ROWS>(a, s);
+          work += (unsigned long long)w.tiles * (unsigned int)w.tokens;
+        }
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) work += __shfl_xor_sync(0xffffffffu, work, o);
+      if ((threadIdx.x & 31u) == 0) works[threadIdx.x >> 5] = work;
+      __syncthreads();
+      work = 0;
+#pragma unroll
+      for (int i = 0; i < NT / 32; ++i) work += works[i];
+      size = (int)min(max((long long)(work * (unsigned int)c.HK / (unsigned long long)f.target) + 1, (long long)f.least), (long long)kCacheChunk);
+    }
+    const bool found = find_unit<NT>(
+        c.batch, blockIdx.x,
+        [&](int i) {
+          const CacheSeq s = cache_seq(c, i);
+          if (!s.count) return 0u;
+          const CacheWalk w = cache_walk<ROWS>(a, s);
+          return w.tiles * (unsigned int)c.HK * (f.single ? 1u : cache_chunks(f, w.tokens, size));
+        },
+        p.b, nth);
+    if (!found) return false;
+    if (!f.single) p.chunks = cache_chunks(f, cache_walk<ROWS>(a, cache_seq(c, p.b)).tokens, size);
+  }
+  p.s = cache_seq(c, p.b);
+  const unsigned int pair = nth / p.chunks, chunk = nth - pair * p.chunks;
+  const unsigned int tile = f.by_key_heads.of(pair);
+  p.first_unit = blockIdx.x - chunk;
+  p.hk = (int)(pair - tile * (unsigned int)c.HK);
+  p.first_row = (int)tile * ROWS;
+  p.rows = min(ROWS, p.s.count * a.group - p.first_row);
+  p.least_pos = p.s.pos0 + (int)f.by_group.of((unsigned int)p.first_row);
+  p.most_pos = p.s.pos0 + (int)f.by_group.of((unsigned int)(p.first_row + p.rows - 1));
+  p.end = cache_last(a, p.most_pos) + 1;
+  p.sink_end = p.shift = 0;
+  if (a.window) {
+    p.sink_end = (int)min(((long long)min(a.sinks, max(p.end, 0)) + 15) & ~15ll, 0x7ffffff0ll);
+    p.shift = max((cache_first(a, p.least_pos) & ~15) - p.sink_end, 0);
+  }
+  const int n_tokens = p.shift ? max(p.end - p.shift, p.sink_end) : max(p.end, 0);       // (the window may lie behind the last page)
+  const int per = (int)((((long long)n_tokens + p.chunks - 1) / p.chunks + 63) & ~63ll);
+  p.begin = (int)min((long long)chunk * per, (long long)n_tokens);
+  p.stop = (int)min((long long)p.begin + per, (long long)n_tokens);
+  return true;
+}
+
 // Writes four elements of a row and, with the first, its lse; false: one is infinite or undefined, and the row has to be done again
 template <class T>
 __device__ __forceinline__ bool cache_finish(const CacheAttnArgs& a, int row, int h, int e, const float4& v, float top, float sum, float lift) {
@@ -119,81 +193,26 @@ __global__ void __launch_bounds__(kCacheFewThreads, (CacheFewShape<DP, CODED, NR
   constexpr int KS = DP / 16, W = Sh::kWidth, R = Sh::kRows;
   constexpr float kUp = kLift<M>;
   extern __shared__ __align__(128) unsigned char dyn[];
-  __shared__ unsigned long long works[kCacheFewWarps];
   __shared__ unsigned int last_block;
   const CacheArgs& c = a.c;
   const unsigned int warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, q4 = lane & 3u;
   grid_begin();
 
-  // ---- this block's chunk
-  int b;
-  unsigned int nth, chunks = 1;
-  if (f.single && !c.starts) {
-    b = (int)f.by_units.of(blockIdx.x);
-    nth = blockIdx.x - (unsigned int)b * f.by_units.d;
-    if (b >= c.batch) return;
-  } else {
-    int size = 0x7fffffff;
-    if (!f.single) {
-      unsigned long long work = 0;
-      for (int i = (int)threadIdx.x; i < c.batch; i += kCacheFewThreads) {
-        const CacheSeq s = cache_seq(c, i);
-        if (s.count) {
-          const CacheWalk w = cache_walk<R>(a, s);
-          work += (unsigned long long)w.tiles * (unsigned int)w.tokens;
-        }
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) work += __shfl_xor_sync(0xffffffffu, work, o);
-      if (lane == 0) works[warp] = work;
-      __syncthreads();
-      work = 0;
-#pragma unroll
-      for (int i = 0; i < kCacheFewWarps; ++i) work += works[i];
-      size = (int)min(max((long long)(work * (unsigned int)c.HK / (unsigned long long)f.target) + 1, (long long)f.least), (long long)kCacheChunk);
-    }
-    const bool found = find_unit<kCacheFewThreads>(
-        c.batch, blockIdx.x,
-        [&](int i) {
-          const CacheSeq s = cache_seq(c, i);
-          if (!s.count) return 0u;
-          const CacheWalk w = cache_walk<R>(a, s);
-          return w.tiles * (unsigned int)c.HK * (f.single ? 1u : cache_chunks(f, w.tokens, size));
-        },
-        b, nth);
-    if (!found) return;
-    if (!f.single) chunks = cache_chunks(f, cache_walk<R>(a, cache_seq(c, b)).tokens, size);
-  }
-  const CacheSeq s = cache_seq(c, b);
-  const unsigned int pair = nth / chunks, chunk = nth - pair * chunks;
-  const unsigned int tile = f.by_key_heads.of(pair), first_unit = blockIdx.x - chunk;
-  const int hk = (int)(pair - tile * (unsigned int)c.HK);
-  const int first_row = (int)tile * R, rows = min(R, s.count * a.group - first_row);
+  CachePlan plan;
+  if (!cache_plan<kCacheFewThreads, R>(a, f, plan)) return;
+  const CacheSeq& s = plan.s;
+  const int b = plan.b, hk = plan.hk, first_row = plan.first_row, rows = plan.rows, end = plan.end, v_begin = plan.begin, v_end = plan.stop;
+  const unsigned int chunks = plan.chunks, first_unit = plan.first_unit;
   auto query_of = [&](int i) { return (int)f.by_group.of((unsigned int)(first_row + i)); };
   auto head_of = [&](int i) { return hk * a.group + first_row + i - query_of(i) * a.group; };
-
-  // ---- what its rows see; this lane's columns are rows 8 r + 2 q4 and the next one
-  const int least_pos = s.pos0 + query_of(0), most_pos = s.pos0 + query_of(rows - 1);
-  const int end = cache_last(a, most_pos) + 1;                         // tokens that some row sees lie before it
-  const int all_see = cache_last(a, least_pos), all_from = cache_first(a, most_pos);
-  // the walk: tokens 0 .. sink_end - 1, then those from sink_end + shift on
-  int sink_end = 0, shift = 0;
-  if (a.window) {
-    sink_end = (int)min(((long long)min(a.sinks, max(end, 0)) + 15) & ~15ll, 0x7ffffff0ll);
-    shift = max((cache_first(a, least_pos) & ~15) - sink_end, 0);
-  }
-  const int n_tokens = shift ? max(end - shift, sink_end) : max(end, 0);       // (the window may lie behind the last page)
-  const int per = (int)((((long long)n_tokens + chunks - 1) / chunks + 63) & ~63ll);
-  const int v_begin = (int)min((long long)chunk * per, (long long)n_tokens), v_end = (int)min((long long)v_begin + per, (long long)n_tokens);
+  // (this lane's columns are rows 8 r + 2 q4 and the next one)
+  const int all_see = cache_last(a, plan.least_pos), all_from = cache_first(a, plan.most_pos);
 
   // ---- the ring: steps of 16 tokens, every fourth of them this warp's
   const unsigned int ring = b200_smem_addr(dyn) + warp * Sh::kRing;
   const int steps = v_end > v_begin ? (v_end - v_begin + 15) / 16 : 0;
   const int mine = steps > (int)warp ? (steps - (int)warp + kCacheFewWarps - 1) / kCacheFewWarps : 0;
-  auto token_of = [&](int n) {
-    const int v = v_begin + ((int)warp + n * kCacheFewWarps) * 16;
-    return v < sink_end ? v : v + shift;
-  };
+  auto token_of = [&](int n) { return plan.token_of(v_begin + ((int)warp + n * kCacheFewWarps) * 16); };
   auto page_of = [&](int j) { return cache_page_at(c, b, c.by_page.of((unsigned int)j)); };
   constexpr int kSize = CODED ? 1 : 2;
   const unsigned char *const keys = (const unsigned char*)c.k, *const values = (const unsigned char*)c.v;

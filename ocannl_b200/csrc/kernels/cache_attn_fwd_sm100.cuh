@@ -419,6 +419,7 @@ cache_attention_tc(const __grid_constant__ b200_tmap map_q, const __grid_constan
         }
         m_tile = fmaxf(m_tile, fmaf(fmaxf(top, other), mul[k], add[k]));
       }
+      if (!on) m_tile = -INFINITY;               // (what lies in a row of no token has no say in when the others' maxima move)
       if (NQ == 1 && f.sums && seen && seen % kSumTiles == 0) {
         // the accumulators are added to the sums (the product before is waited for as below)
         live = b200_wait(bar_o + 8 * g, (seen - 1) & 1u, abort_flag, a.status, 72u);

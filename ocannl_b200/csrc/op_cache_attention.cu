@@ -3,6 +3,7 @@
 #include <cstring>
 
 #include "cache.hpp"
+#include "kernels/cache_attn_any.cuh"
 #include "kernels/cache_attn_few_sm100.cuh"
 #include "kernels/cache_attn_fwd_sm100.cuh"
 #include "kernels/cache_attn_terms.cuh"
@@ -11,34 +12,7 @@ using namespace b200;
 
 namespace {
 
-// ---- row by row, a warp each
-template <class T, bool CODED>
-__global__ void __launch_bounds__(256) cache_attention_rows(const __grid_constant__ CacheAttnArgs a) {
-  grid_begin();
-  const unsigned int lane = threadIdx.x & 31u;
-  const CacheArgs& c = a.c;
-  const long long n = (long long)c.tokens * a.H;
-  for (long long i = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); i < n; i += (long long)gridDim.x * 8) {
-    const int row = (int)(i / a.H);
-    int b;
-    if (c.starts) {
-      int lo = 0, hi = c.batch;                  // the last sequence that starts at the row or before it
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (__ldg(c.starts + mid) <= row) lo = mid;
-        else hi = mid;
-      }
-      b = lo;
-    } else {
-      b = row / c.each;
-    }
-    const CacheSeq s = cache_seq(c, b);
-    if (row < s.first || row >= s.first + s.count) continue;
-    cache_attention_row<T, CODED>(a, b, (int)(i - (long long)row * a.H), row, s.pos0 + (row - s.first), lane);
-  }
-}
-
-typedef void (*RowsKernel)(const CacheAttnArgs);
+typedef void (*AnyKernel)(const CacheAttnArgs, const CacheFewArgs, int);
 typedef void (*FewKernel)(const CacheAttnArgs, const CacheFewArgs);
 
 // [dims[3]][dims[2]][dims[1]][dims[0]] elements in boxes of box[0] x box[1] x 1 x box[3]; 16-bit ones swizzled as the tensor cores read them
@@ -59,7 +33,8 @@ struct CacheAttnOperator : b200_operator {
   CacheAttnArgs a = {};
   int dtype = 0;
   bool coded = false;
-  RowsKernel rows = nullptr;
+  AnyKernel any = nullptr;
+  int vec = 0;
   FewKernel few = nullptr;
   CacheFewArgs few_args = {};
   CacheTiles tiles = {};
@@ -70,7 +45,7 @@ struct CacheAttnOperator : b200_operator {
   int tile = 16, width = 0, resident = 1;      // rows of a tile, floats of a row of its parts, blocks of an SM
 
   template <class T>
-  void set_rows() { rows = coded ? cache_attention_rows<T, true> : cache_attention_rows<T, false>; }
+  void set_any() { any = coded ? cache_attention_any<T, true> : cache_attention_any<T, false>; }
   template <class T, int DP, bool CODED, int NR>
   void set_few() {
     typedef CacheFewShape<DP, CODED, NR> Sh;
@@ -99,11 +74,51 @@ struct CacheAttnOperator : b200_operator {
     const long long n = (long long)a.c.tokens * a.H;
     if (!n || !a.c.batch) return;
     if (pieces()) return many() ? choose_tiles() : choose_few();
-    if (dtype == B200_F32) set_rows<float>();
-    else if (dtype == B200_BF16) set_rows<__nv_bfloat16>();
-    else set_rows<__half>();
-    ready(rows);
-    grid = (unsigned int)std::min<long long>((n + 7) / 8, 16ll * dev->sm_count);
+    choose_any();
+  }
+  // Rows in tiles, tokens in chunks of about `least` at least, as many as give every SM three rounds of blocks; a tile adds one chunk at most, those cut
+  // for their length aside.
+  void choose_chunks(int rows_of_tile, int floats, int blocks, int least) {
+    const CacheArgs& c = a.c;
+    // A sequence of n tokens has n group rows.
+    const long long some = std::min(c.batch, c.tokens), tiles = ((long long)c.tokens * a.group + (rows_of_tile - 1) * some) / rows_of_tile * c.HK;
+    const long long capacity = std::min<long long>((long long)c.max_pages * c.page, 0x7fffffff);
+    few_args.target = (long long)dev->sm_count * blocks * 3;
+    few_args.least = least;
+    few_args.most = kFewMost;
+    few_args.single = capacity < least + least / 2;
+    few_args.by_group = Divisor((unsigned int)a.group);
+    few_args.by_key_heads = Divisor((unsigned int)c.HK);
+    if (few_args.single) {
+      grid = blocks_of(tiles);
+      if (!c.starts) {
+        const long long each = ((long long)c.each * a.group + rows_of_tile - 1) / rows_of_tile * c.HK;
+        few_args.by_units = Divisor(blocks_of(each));
+        grid = blocks_of(each * c.batch);
+      }
+    } else {
+      // (the nearest number of chunks: up to one and a half times the size each)
+      const unsigned __int128 walk = (unsigned __int128)tiles * (unsigned long long)(capacity + 64);
+      const unsigned __int128 cut = std::max<unsigned __int128>((unsigned long long)few_args.target, walk / kCacheChunk), fewest = walk / (unsigned int)least;
+      grid = blocks_of((long long)std::min<unsigned __int128>(std::min(cut, fewest) + (unsigned long long)tiles, 1ull << 31));
+    }
+    const size_t parts = few_args.single ? 0 : (size_t)grid * rows_of_tile * floats * 4;
+    take_workspace(parts + (size_t)grid * 4);
+    few_args.parts = (float*)workspace;
+    few_args.tickets = (unsigned int*)(workspace + parts);
+    cu_check(cu().cuMemsetD8Async_(workspace + parts, 0, (size_t)grid * 4, dev->stream), "cuMemsetD8Async(tickets)");
+  }
+  void choose_any() {
+    const int size = coded ? 1 : (int)dtype_bytes(dtype), v = coded ? 4 : 16 / size;
+    vec = a.c.D % v == 0;
+    for (const void* p : {(const void*)a.c.k, (const void*)a.c.v}) vec &= ((size_t)p & 15) == 0;
+    if (((long long)a.c.tokens * a.group) >> 31) throw Error(B200_E_UNSUPPORTED, "cache_attention: too many rows");
+    if (dtype == B200_F32) set_any<float>();
+    else if (dtype == B200_BF16) set_any<__nv_bfloat16>();
+    else set_any<__half>();
+    smem = any_smem(a.c.D);
+    choose_chunks(kAnyRows, kAnyWidth, (int)std::min<size_t>(6, 220 * 1024 / (smem + 7 * 1024)), 256);
+    ready(any, smem);
   }
   // Whole prompts: tiles of 128 rows on the tensor cores, where sequences have them on average and the cache's pages are boxes of the TMA unit.
   bool many() const {
@@ -137,41 +152,14 @@ struct CacheAttnOperator : b200_operator {
     const bool wide = (long long)c.tokens * a.group > 8ll * std::min(c.batch, c.tokens);
     if (dtype == B200_BF16) c.D <= 64 ? set_few<__nv_bfloat16, 64>(wide) : set_few<__nv_bfloat16, 128>(wide);
     else c.D <= 64 ? set_few<__half, 64>(wide) : set_few<__half, 128>(wide);
-    // A sequence of n tokens has n group rows, in tiles.  Chunks of about 512 tokens at least, as many as give every SM three rounds of blocks; a
-    // tile adds one at most, those cut for their length aside.
-    const long long some = std::min(c.batch, c.tokens), tiles = ((long long)c.tokens * a.group + (tile - 1) * some) / tile * c.HK;
-    const long long capacity = std::min<long long>((long long)c.max_pages * c.page, 0x7fffffff);
-    few_args.target = (long long)dev->sm_count * resident * 3;
-    few_args.least = 512;
-    few_args.most = kFewMost;
-    few_args.single = capacity < few_args.least + few_args.least / 2;
-    few_args.by_group = Divisor((unsigned int)a.group);
-    few_args.by_key_heads = Divisor((unsigned int)c.HK);
-    if (few_args.single) {
-      grid = blocks_of(tiles);
-      if (!c.starts) {
-        const long long each = ((long long)c.each * a.group + tile - 1) / tile * c.HK;
-        few_args.by_units = Divisor(blocks_of(each));
-        grid = blocks_of(each * c.batch);
-      }
-    } else {
-      // (the nearest number of chunks: up to one and a half times the size each)
-      const unsigned __int128 walk = (unsigned __int128)tiles * (unsigned long long)(capacity + 64);
-      const unsigned __int128 cut = std::max<unsigned __int128>((unsigned long long)few_args.target, walk / kCacheChunk), least = walk / few_args.least;
-      grid = blocks_of((long long)std::min<unsigned __int128>(std::min(cut, least) + (unsigned long long)tiles, 1ull << 31));
-    }
-    const size_t parts = few_args.single ? 0 : (size_t)grid * tile * width * 4;
-    take_workspace(parts + (size_t)grid * 4);
-    few_args.parts = (float*)workspace;
-    few_args.tickets = (unsigned int*)(workspace + parts);
-    cu_check(cu().cuMemsetD8Async_(workspace + parts, 0, (size_t)grid * 4, dev->stream), "cuMemsetD8Async(tickets)");
+    choose_chunks(tile, width, resident, 512);
     ready(few, smem);
   }
   void run(cudaStream_t s) override {
     if (!grid) return;
     if (tiles.kernel) launch(tiles.kernel, dim3(grid), tiles.threads, tiles.smem, s, map_q, map_k, map_v, a, tile_args);
     else if (few) launch(few, dim3(grid), kCacheFewThreads, smem, s, a, few_args);
-    else launch(rows, dim3(grid), 256, 0, s, a);
+    else launch(any, dim3(grid), kCacheFewThreads, smem, s, a, few_args, vec);
   }
 };
 
