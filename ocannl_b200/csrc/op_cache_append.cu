@@ -23,11 +23,13 @@ struct AppendArgs {
   const unsigned long long* turns;     // [pairs], of a turn per position, scaled by 2^64
   unsigned int heads, d, pairs;
   unsigned int turn_items, items, v_items;     // accesses of a head that turn, all of a head that turns, of a value head
-  unsigned int plain_blocks, per_block;        // blocks of rows that need no scale, tokens of each
+  unsigned int per_block;              // tokens of a block of rows that need no scale
   unsigned int turned_rows, plain_items;       // of a token: rows that turn, and all accesses, of such a block
+  unsigned int code_blocks, pages_each;        // blocks that make codes; pages that a sequence's tokens touch at most, without starts
   unsigned int tile;                   // tokens of a table, of a block that makes codes
   unsigned int per_head;               // warps of a head there
-  Divisor by_pairs, by_items, by_v_items, by_plain;
+  unsigned int heads_each, groups;     // heads of such a block; blocks of a page's keys, or values
+  Divisor by_pairs, by_items, by_v_items, by_plain, by_pages_each, by_groups;
   float magnitude;
 };
 
@@ -42,6 +44,15 @@ __device__ __forceinline__ float2 turn_of(const AppendArgs& a, int position, uns
   sincospif((float)step * 4.656612873077393e-10f, &s, &c);
   return make_float2(c * a.magnitude, s * a.magnitude);
 }
+
+// The table's pairs as an access takes them: kPairs of an item side by side, and 16 bytes between items where that keeps the 16-byte reads of eight lanes,
+// each of an item of its own, out of one another's banks.
+template <int VEC, bool INTERLEAVED>
+struct Table {
+  static constexpr int kPairs = VEC == 1 ? 1 : INTERLEAVED ? VEC / 2 : VEC, kPitch = kPairs >= 4 ? kPairs + 2 : kPairs;
+  __host__ __device__ static constexpr unsigned int row(unsigned int pairs) { return pairs / kPairs * kPitch; }
+  __device__ static unsigned int at(unsigned int pair) { return pair / kPairs * kPitch + pair % kPairs; }
+};
 
 // One access of a head: a vector, or with pairs that lie apart two (the second `far` elements behind the first)
 template <class T, int VEC, bool INTERLEAVED>
@@ -59,26 +70,42 @@ struct Piece {
     if (kSplit && turns) w.load(row + at + far(pairs));
   }
   __device__ __forceinline__ unsigned int far(unsigned int pairs) const { return INTERLEAVED ? 1u : pairs; }
+  typedef Table<VEC, INTERLEAVED> Tab;
+  __device__ __forceinline__ void pairs_of(const float2* cs, float2 (&t)[Tab::kPairs]) const {
+    const float2* from = cs + item * Tab::kPitch;
+    if constexpr (Tab::kPairs == 1) {
+      t[0] = from[0];
+    } else {
+#pragma unroll
+      for (int q = 0; q < Tab::kPairs; q += 2) {
+        const float4 v = *(const float4*)(from + q);
+        t[q] = make_float2(v.x, v.y);
+        t[q + 1] = make_float2(v.z, v.w);
+      }
+    }
+  }
   // the values, turned; y only where pairs lie apart
   __device__ __forceinline__ void values(const float2* cs, float (&x)[VEC], float (&y)[VEC]) const {
     u.values(x);
     if (!turns) return;
     if constexpr (kSplit) {
       w.values(y);
+      float2 t[VEC];
+      pairs_of(cs, t);
 #pragma unroll
       for (int q = 0; q < VEC; ++q) {
-        const float2 t = cs[item * VEC + q];
         const float x0 = x[q], y0 = y[q];
-        x[q] = x0 * t.x - y0 * t.y;
-        y[q] = x0 * t.y + y0 * t.x;
+        x[q] = x0 * t[q].x - y0 * t[q].y;
+        y[q] = x0 * t[q].y + y0 * t[q].x;
       }
     } else {
+      float2 t[VEC / 2];
+      pairs_of(cs, t);
 #pragma unroll
       for (int q = 0; q < VEC / 2; ++q) {
-        const float2 t = cs[item * (VEC / 2) + q];
         const float x0 = x[2 * q], y0 = x[2 * q + 1];
-        x[2 * q] = x0 * t.x - y0 * t.y;
-        x[2 * q + 1] = x0 * t.y + y0 * t.x;
+        x[2 * q] = x0 * t[q].x - y0 * t[q].y;
+        x[2 * q + 1] = x0 * t[q].y + y0 * t[q].x;
       }
     }
   }
@@ -95,12 +122,12 @@ __device__ __forceinline__ void store_codes(unsigned char* to, const float (&x)[
 }
 
 template <class T, int VEC, bool INTERLEAVED>
-__device__ __forceinline__ void plain_rows(const AppendArgs& a, float2* table, bool coded) {
+__device__ __forceinline__ void plain_rows(const AppendArgs& a, unsigned int block, float2* table, bool coded) {
   typedef Piece<T, VEC, INTERLEAVED> P;
   const CacheArgs& c = a.c;
   __shared__ int positions[kThreads];            // of the block's tokens
   __shared__ long long slots[kThreads];          // elements of the cache ahead of head 0 of a token's slot; -1: no slot, -2: no sequence
-  const unsigned int first = blockIdx.x * a.per_block, n = min(a.per_block, (unsigned int)c.tokens - first), total = n * a.plain_items;
+  const unsigned int first = block * a.per_block, n = min(a.per_block, (unsigned int)c.tokens - first), total = n * a.plain_items;
   const unsigned int turned = a.turned_rows * a.items;
   P it[kAtOnce];
   unsigned int tok[kAtOnce], row[kAtOnce];
@@ -150,9 +177,10 @@ __device__ __forceinline__ void plain_rows(const AppendArgs& a, float2* table, b
     positions[threadIdx.x] = a.positions ? a.positions[t] : pos;
   }
   __syncthreads();
+  const unsigned int row_of_table = P::Tab::row(a.pairs);
   for (unsigned int i = threadIdx.x; i < n * a.pairs; i += kThreads) {
-    const unsigned int t = a.by_pairs.of(i);
-    table[i] = turn_of(a, positions[t], i - t * a.pairs);
+    const unsigned int t = a.by_pairs.of(i), pair = i - t * a.pairs;
+    table[t * row_of_table + P::Tab::at(pair)] = turn_of(a, positions[t], pair);
   }
   __syncthreads();
   const long long head = (long long)c.page * c.D;      // from one head of a page to the next
@@ -171,7 +199,7 @@ __device__ __forceinline__ void plain_rows(const AppendArgs& a, float2* table, b
         to = (T*)(value ? c.v : c.k) + slot + (long long)(row[k] - (value ? a.turned_rows : a.heads)) * head;
       }
       float x[VEC], y[VEC];
-      it[k].values(table + tok[k] * a.pairs, x, y);
+      it[k].values(table + tok[k] * row_of_table, x, y);
       Vec<T, VEC>::store(to + it[k].at, x);
       if (P::kSplit && it[k].turns) Vec<T, VEC>::store(to + it[k].at + it[k].far(a.pairs), y);
     }
@@ -187,8 +215,9 @@ __device__ __forceinline__ void page_codes(const AppendArgs& a, float2* table) {
   typedef Piece<T, VEC, INTERLEAVED> P;
   const CacheArgs& c = a.c;
   __shared__ float largest[kWarps];
-  const unsigned int unit = blockIdx.x - a.plain_blocks, warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-  const bool value = unit & 1u;
+  const unsigned int block = a.by_groups.of(blockIdx.x), first_head = (blockIdx.x - block * a.groups) * a.heads_each, warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+  const unsigned int unit = block >> 1;           // of pages
+  const bool value = block & 1u;
   // pages that a sequence's new tokens touch
   auto pages_of = [&](const CacheSeq& s) -> unsigned int {
     const int end = s.pos0 + s.count, begin = max(s.pos0, 0);
@@ -196,8 +225,14 @@ __device__ __forceinline__ void page_codes(const AppendArgs& a, float2* table) {
   };
   int b;
   unsigned int nth;
-  if (!find_unit<kThreads>(c.batch, unit >> 1, [&](int i) { return pages_of(cache_seq(c, i)); }, b, nth)) return;
+  if (c.starts) {
+    if (!find_unit<kThreads>(c.batch, unit, [&](int i) { return pages_of(cache_seq(c, i)); }, b, nth)) return;
+  } else {
+    b = (int)a.by_pages_each.of(unit);
+    nth = unit - (unsigned int)b * a.pages_each;
+  }
   const CacheSeq s = cache_seq(c, b);
+  if (nth >= pages_of(s)) return;
   const unsigned int begin0 = (unsigned int)max(s.pos0, 0), index = c.by_page.of(begin0) + nth;
   const int page = cache_page_at(c, b, index);
   if (page < 0) return;
@@ -209,40 +244,66 @@ __device__ __forceinline__ void page_codes(const AppendArgs& a, float2* table) {
   unsigned char* codes = (unsigned char*)(value ? c.v : c.k);
   const unsigned int items = value ? a.v_items : a.items, turn_items = value ? 0u : a.turn_items;
   const Divisor by_items = value ? a.by_v_items : a.by_items;
-  const unsigned int at_once = kWarps / a.per_head, share = warp % a.per_head;
+  const unsigned int heads = min(first_head + a.heads_each, (unsigned int)c.HK), at_once = kWarps / a.per_head, share = warp % a.per_head;
   const bool one_table = n <= a.tile;
+  const unsigned int row_of_table = P::Tab::row(a.pairs);
   auto make_table = [&](unsigned int t0) {
     if (!turn_items) return;
     __syncthreads();
     const unsigned int many = min(a.tile, n - t0) * a.pairs;
     for (unsigned int i = threadIdx.x; i < many; i += kThreads) {
-      const unsigned int t = a.by_pairs.of(i);
-      table[i] = turn_of(a, a.positions ? a.positions[row0 + t0 + t] : (int)(begin + t0 + t), i - t * a.pairs);
+      const unsigned int t = a.by_pairs.of(i), pair = i - t * a.pairs;
+      table[t * row_of_table + P::Tab::at(pair)] = turn_of(a, a.positions ? a.positions[row0 + t0 + t] : (int)(begin + t0 + t), pair);
     }
     __syncthreads();
   };
-  if (one_table) make_table(0);
-  for (unsigned int h0 = 0; h0 < (unsigned int)c.HK; h0 += at_once) {
+  // A few tokens: a lane keeps its pieces, which are under way while the table is made; more are read twice.
+  const bool kept = n * items <= 32 * a.per_head * kAtOnce;
+  P held[kAtOnce];
+  auto hold = [&](unsigned int h0) {
     const unsigned int h = h0 + warp / a.per_head;
-    const bool mine = h < (unsigned int)c.HK && warp < at_once * a.per_head;
+    if (h >= heads || warp >= at_once * a.per_head) return;
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      const unsigned int i = share * 32 + lane + 32 * a.per_head * k;
+      if (i >= n * items) continue;
+      const unsigned int t = by_items.of(i);
+      held[k].load(from + ((unsigned long long)(row0 + t) * (unsigned int)c.HK + h) * a.d, i - t * items, turn_items, turn_items ? a.pairs : 0u);
+    }
+  };
+  if (kept) hold(first_head);
+  if (one_table) make_table(0);
+  for (unsigned int h0 = first_head; h0 < heads; h0 += at_once) {
+    const unsigned int h = h0 + warp / a.per_head;
+    const bool mine = h < heads && warp < at_once * a.per_head;
+    const float before = mine && slot ? scales[h] : 0.f;
     // all pieces of this warp's share: f(piece, token of the page's new ones, cosines and sines of its token)
     auto each = [&](auto&& f) {
+      if (kept) {
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) {
+          const unsigned int i = share * 32 + lane + 32 * a.per_head * k;
+          if (!mine || i >= n * items) continue;
+          const unsigned int t = by_items.of(i);
+          f(held[k], t, table + t * row_of_table);
+        }
+        return;
+      }
       for (unsigned int t0 = 0; t0 < n; t0 += a.tile) {
         if (!one_table) make_table(t0);
         const unsigned int many = mine ? min(a.tile, n - t0) * items : 0u;
         for (unsigned int i0 = share * 32 + lane; i0 < many; i0 += 32 * a.per_head * kAtOnce) {
-          P it[kAtOnce];
           unsigned int tok[kAtOnce];
 #pragma unroll
           for (int k = 0; k < kAtOnce; ++k) {
             const unsigned int i = i0 + 32 * a.per_head * k;
             if (i >= many) continue;
             tok[k] = by_items.of(i);
-            it[k].load(from + ((unsigned long long)(row0 + t0 + tok[k]) * (unsigned int)c.HK + h) * a.d, i - tok[k] * items, turn_items, turn_items ? a.pairs : 0u);
+            held[k].load(from + ((unsigned long long)(row0 + t0 + tok[k]) * (unsigned int)c.HK + h) * a.d, i - tok[k] * items, turn_items, turn_items ? a.pairs : 0u);
           }
 #pragma unroll
           for (int k = 0; k < kAtOnce; ++k)
-            if (i0 + 32 * a.per_head * k < many) f(it[k], t0 + tok[k], table + tok[k] * a.pairs);
+            if (i0 + 32 * a.per_head * k < many) f(held[k], t0 + tok[k], table + tok[k] * row_of_table);
         }
       }
     };
@@ -256,7 +317,6 @@ __device__ __forceinline__ void page_codes(const AppendArgs& a, float2* table) {
         if (P::kSplit && p.turns && e4m3_has(y[i])) top = fmaxf(top, fabsf(y[i]));
       }
     });
-    const float before = mine && slot ? scales[h] : 0.f;
     top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));       // (of numbers that are not negative)
     if (lane == 0) largest[warp] = top;
     __syncthreads();
@@ -291,16 +351,18 @@ __device__ __forceinline__ void page_codes(const AppendArgs& a, float2* table) {
       if (P::kSplit && p.turns) store_codes<VEC>(to + p.far(a.pairs), y, by);
     });
     if (mine && share == 0 && lane == 0 && (grows || !slot)) scales[h] = scale;
+    if (kept && h0 + at_once < heads) hold(h0 + at_once);
     __syncthreads();                   // (`largest` is written again)
   }
 }
 
 template <class T, int VEC, bool INTERLEAVED, bool CODED>
-__global__ void __launch_bounds__(kThreads) cache_append(const __grid_constant__ AppendArgs a) {
-  extern __shared__ float2 table[];    // [token][pair]: cosine, sine, times the magnitude
+__global__ void __launch_bounds__(kThreads, 3) cache_append(const __grid_constant__ AppendArgs a) {
+  extern __shared__ __align__(16) float2 table[];    // [token][pair]: cosine, sine, times the magnitude
   grid_begin();
-  if (!CODED || blockIdx.x < a.plain_blocks) plain_rows<T, VEC, INTERLEAVED>(a, table, CODED);
-  else page_codes<T, VEC, INTERLEAVED>(a, table);
+  // (pages first: they take longer)
+  if (CODED && blockIdx.x < a.code_blocks) page_codes<T, VEC, INTERLEAVED>(a, table);
+  else plain_rows<T, VEC, INTERLEAVED>(a, blockIdx.x - a.code_blocks, table, CODED);
 }
 
 typedef void (*AppendKernel)(const AppendArgs);
@@ -369,6 +431,8 @@ extern "C" int b200_cache_append_link(b200_dev* dev, const b200_cache_append* p,
     a.by_pairs = Divisor(std::max(1u, a.pairs));
     a.by_items = Divisor(a.items);
     a.by_v_items = Divisor(a.v_items);
+    // (Table: pairs of an item, and the floats between items)
+    const unsigned int of_item = !vec ? 1 : p->interleaved ? V / 2 : V, row_of_table = a.pairs / of_item * (of_item >= 4 ? of_item + 2 : of_item);
     unsigned long long plain = 0, codes = 0;
     size_t table = 0;
     if (pc.tokens && pc.batch && per_token) {
@@ -382,19 +446,32 @@ extern "C" int b200_cache_append_link(b200_dev* dev, const b200_cache_append* p,
       a.plain_items = (unsigned int)per_token;
       a.by_plain = Divisor(a.plain_items);
       plain = ((unsigned long long)pc.tokens + tok - 1) / tok;
-      table = (size_t)tok * a.pairs * 8;
+      table = (size_t)tok * row_of_table * 8;
     }
     if (coded && pc.tokens && pc.batch) {
       // Of n >= 1 tokens a sequence touches at most (n - 2) / page + 2 pages (rounded down, 1 of one token)
       const long long some = std::min<long long>(pc.batch, pc.tokens), page = pc.page;
       codes = (unsigned long long)std::min<long long>(pc.tokens, (pc.tokens + some * (page - 2)) / page + some);
+      if (!a.c.starts) {
+        a.pages_each = (unsigned int)((a.c.each + page - 2) / page + 1);
+        codes = (unsigned long long)a.pages_each * (unsigned long long)pc.batch;
+      }
+      a.by_pages_each = Divisor(std::max(1u, a.pages_each));
       a.tile = (unsigned int)std::min<long long>(page, a.pairs ? std::max(1u, 8192u / a.pairs) : page);
-      table = std::max(table, (size_t)std::min<long long>(a.tile, pc.tokens) * a.pairs * 8);
-      a.per_head = pc.kv_heads >= 5 ? 1 : pc.kv_heads >= 3 ? 2 : pc.kv_heads == 2 ? 4 : 8;
+      table = std::max(table, (size_t)std::min<long long>(a.tile, pc.tokens) * row_of_table * 8);
+      // Warps of a head: no fewer than hold what a page receives of it, as many as there are where heads are few.  (A block a page and all its heads, each read
+      // twice by one warp: 75 us for 8192 tokens of 8 heads, pages of 64.)
+      const long long fill = std::min<long long>(page, pc.tokens / some) * a.v_items;
+      a.per_head = 1;
+      while (a.per_head < (unsigned int)kWarps && ((long long)a.per_head * 32 * kAtOnce < fill || (long long)kWarps / a.per_head >= 2ll * pc.kv_heads)) a.per_head *= 2;
+      a.heads_each = std::max(2u, (unsigned int)kWarps / a.per_head);
+      a.groups = ((unsigned int)pc.kv_heads + a.heads_each - 1) / a.heads_each;
+      a.by_groups = Divisor(a.groups);
     }
-    if ((plain + 2 * codes) >> 31) ops.refuse("too many tokens", B200_E_UNSUPPORTED);
-    a.plain_blocks = (unsigned int)plain;
-    op->grid = (unsigned int)(plain + 2 * codes);
+    codes *= 2 * a.groups;
+    if ((plain + codes) >> 31) ops.refuse("too many tokens", B200_E_UNSUPPORTED);
+    a.code_blocks = (unsigned int)codes;
+    op->grid = (unsigned int)(plain + codes);
     op->smem = table;
     op->kernel = p->dtype == B200_F32 ? kernel_of<float>(vec, p->interleaved, coded) : p->dtype == B200_BF16 ? kernel_of<__nv_bfloat16>(vec, p->interleaved, coded)
                                                                                                             : kernel_of<__half>(vec, p->interleaved, coded);
