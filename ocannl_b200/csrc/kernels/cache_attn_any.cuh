@@ -1,6 +1,6 @@
 // Attention of new tokens over a paged cache in single precision arithmetic: single heads, and 16-bit ones whose rows are no whole 16-byte pieces.
 //
-// A block takes 8 rows of a (sequence, key head) and a chunk of their tokens, as the tensor-core form for few rows does, 32 tokens at a time in
+// A block takes 8 rows of a (sequence, key head) and a part of their tokens, as the tensor-core form for few rows does, 32 tokens at a time in
 // shared memory as floats.  A warp has two rows: a lane a token for the scores, four elements for the output.  Bound by shared memory: a warp reads a
 // tile's keys and values once for two rows, some 350 accesses of 128 bytes each for heads of 128 elements, so four warps take 32 KB of cache in 1400 cycles,
 // which is the rate at which an SM gets them from memory; warps without rows read nothing.  Scores keep their own unit until the maximum is taken off: rounded
@@ -27,15 +27,18 @@ __global__ void __launch_bounds__(kCacheFewThreads) cache_attention_any(const __
   const CacheArgs& c = a.c;
   const unsigned int warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
   grid_begin();
-  CachePlan plan;
-  if (!cache_plan<kCacheFewThreads, kAnyRows>(a, f, plan)) return;
-  const int pitch = any_pitch(c.D), rows = plan.rows;
+  CachePart part;
+  if (!cache_part<kCacheFewThreads, kAnyRows>(a, f, part)) return;
+  const int pitch = any_pitch(c.D);
+  CachePiece plan;
+  for (; cache_piece<kAnyRows>(a, f, part, plan); cache_advance<kAnyRows>(a, part)) {
+  const int rows = plan.rows;
   float *const q = any_shared, *const keys = q + kAnyRows * pitch, *const values = keys + kAnyTokens * pitch;
   auto query_of = [&](int i) { return (int)f.by_group.of((unsigned int)(plan.first_row + i)); };
   auto head_of = [&](int i) { return plan.hk * a.group + plan.first_row + i - query_of(i) * a.group; };
   for (int i = (int)threadIdx.x; i < kAnyRows * pitch; i += kCacheFewThreads) {
     const int r = i / pitch, e = i - r * pitch;
-    q[i] = r < rows && e < c.D ? to_float(((const T*)a.q)[((long long)(plan.s.first + query_of(r)) * a.H + head_of(r)) * c.D + e]) : 0.f;
+    q[i] = r < rows && e < c.D ? to_float(((const T*)a.q)[((long long)(part.s.first + query_of(r)) * a.H + head_of(r)) * c.D + e]) : 0.f;
   }
   const int r0 = 2 * (int)warp;                     // this warp's rows are r0 and r0 + 1
   const bool mine = r0 < rows;
@@ -44,7 +47,7 @@ __global__ void __launch_bounds__(kCacheFewThreads) cache_attention_any(const __
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const int r = min(r0 + k, rows - 1);
-    pos[k] = plan.s.pos0 + query_of(r);
+    pos[k] = part.s.pos0 + query_of(r);
     slope[k] = a.slopes ? a.slopes[head_of(r)] : 0.f;
   }
   float o[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
@@ -56,7 +59,7 @@ __global__ void __launch_bounds__(kCacheFewThreads) cache_attention_any(const __
       float ks = 0.f, vs = 0.f;
       if (v < plan.stop && j < plan.end) {
         const unsigned int index = c.by_page.of((unsigned int)j);
-        const int page = cache_page_at(c, plan.b, index);
+        const int page = cache_page_at(c, part.b, index);
         if (page >= 0) {
           place = cache_at(c, page, plan.hk) + (long long)((unsigned int)j - index * c.page) * c.D;
           if (CODED) {
@@ -178,7 +181,7 @@ __global__ void __launch_bounds__(kCacheFewThreads) cache_attention_any(const __
   auto finish = [&](int i, const float4& v, float top, float sum) {
     const float by = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
     const float y[4] = {v.x * by, v.y * by, v.z * by, v.w * by};
-    const int row = plan.s.first + query_of(i), h = head_of(i);
+    const int row = part.s.first + query_of(i), h = head_of(i);
     const long long at = (long long)row * a.H + h;
     bool fine = true;
 #pragma unroll
@@ -188,56 +191,61 @@ __global__ void __launch_bounds__(kCacheFewThreads) cache_attention_any(const __
         fine = fine && y[k] * 0.f == 0.f;
       }
     if (lane == 0 && a.lse) a.lse[at] = by != 0.f ? top + logf(sum) : -INFINITY;
-    if (attn_again(fine)) cache_attention_row<T, CODED>(a, plan.b, h, row, plan.s.pos0 + query_of(i), lane);
+    if (attn_again(fine)) cache_attention_row<T, CODED>(a, part.b, h, row, part.s.pos0 + query_of(i), lane);
   };
-  if (plan.chunks == 1) {
+  if (plan.parts == 1) {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
       if (r0 + i < rows) finish(r0 + i, make_float4(o[i][0], o[i][1], o[i][2], o[i][3]), m[i], l[i]);
-    return;
-  }
-  float* parts = f.parts + (long long)blockIdx.x * kAnyRows * kAnyWidth;
+  } else {
+    float* parts = f.parts + cache_part_at(plan.first_block, plan.part) * kAnyRows * kAnyWidth;
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-    if (r0 + i < rows) {
-      float* row = parts + (r0 + i) * kAnyWidth;
-      *(float4*)(row + 4 * lane) = make_float4(o[i][0], o[i][1], o[i][2], o[i][3]);
-      if (lane == 0) {
-        row[128] = m[i];
-        row[129] = l[i];
+    for (int i = 0; i < 2; ++i)
+      if (r0 + i < rows) {
+        float* row = parts + (r0 + i) * kAnyWidth;
+        *(float4*)(row + 4 * lane) = make_float4(o[i][0], o[i][1], o[i][2], o[i][3]);
+        if (lane == 0) {
+          row[128] = m[i];
+          row[129] = l[i];
+        }
+      }
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      last_block = atomicAdd(&f.tickets[plan.first_block], 1u) == plan.parts - 1u;
+      if (last_block) f.tickets[plan.first_block] = 0u;        // for the next run
+    }
+    __syncthreads();
+    if (last_block) {
+      __threadfence();
+      const int n = (int)plan.parts;
+      for (int i = (int)warp; i < rows; i += kCacheFewWarps) {
+        // (the maxima are in the scores' unit; a part without visible tokens has a sum of exactly 0 and counts nothing)
+        const float* from = f.parts + cache_part_at(plan.first_block, 0) * kAnyRows * kAnyWidth + i * kAnyWidth;
+        float t[kFewMost / 32], u[kFewMost / 32], top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < kFewMost / 32; ++k) {
+          const int at = (int)lane + 32 * k;
+          t[k] = at < n ? cache_part_row<128, kAnyRows>(from, at)[128] : -INFINITY;
+          u[k] = at < n ? cache_part_row<128, kAnyRows>(from, at)[129] : 0.f;
+          top = fmaxf(top, t[k]);
+        }
+#pragma unroll
+        for (int k = 16; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < kFewMost / 32; ++k) {
+          const float w = u[k] == 0.f ? 0.f : t[k] == -INFINITY ? 1.f : exp2f((t[k] - top) * kCacheLog2e);
+          if ((int)lane + 32 * k < n) weigh[warp][lane + 32 * k] = w;
+          if (w != 0.f) sum = fmaf(w, u[k], sum);
+        }
+        sum = cache_sum(sum);
+        __syncwarp();
+        finish(i, cache_gather<128, kAnyRows>(from, n, weigh[warp], 4 * (int)lane), top, sum);
       }
     }
-  __threadfence();
-  __syncthreads();
-  if (threadIdx.x == 0) last_block = atomicAdd(&f.tickets[plan.first_unit], 1u) == plan.chunks - 1u;
-  __syncthreads();
-  if (!last_block) return;
-  if (threadIdx.x == 0) f.tickets[plan.first_unit] = 0u;     // for the next run
-  __threadfence();
-  const int n = (int)plan.chunks;
-  for (int i = (int)warp; i < rows; i += kCacheFewWarps) {
-    // (the maxima are in the scores' unit; a part without visible tokens has a sum of exactly 0 and counts nothing)
-    const float* from = f.parts + (long long)plan.first_unit * kAnyRows * kAnyWidth + i * kAnyWidth;
-    float t[kFewMost / 32], u[kFewMost / 32], top = -INFINITY, sum = 0.f;
-#pragma unroll
-    for (int k = 0; k < kFewMost / 32; ++k) {
-      const int at = (int)lane + 32 * k;
-      t[k] = at < n ? from[(long long)at * kAnyRows * kAnyWidth + 128] : -INFINITY;
-      u[k] = at < n ? from[(long long)at * kAnyRows * kAnyWidth + 129] : 0.f;
-      top = fmaxf(top, t[k]);
-    }
-#pragma unroll
-    for (int k = 16; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
-    __syncwarp();
-#pragma unroll
-    for (int k = 0; k < kFewMost / 32; ++k) {
-      const float w = u[k] == 0.f ? 0.f : t[k] == -INFINITY ? 1.f : exp2f((t[k] - top) * kCacheLog2e);
-      if ((int)lane + 32 * k < n) weigh[warp][lane + 32 * k] = w;
-      if (w != 0.f) sum = fmaf(w, u[k], sum);
-    }
-    sum = cache_sum(sum);
-    __syncwarp();
-    finish(i, few_gather(from, n, kAnyRows * kAnyWidth, weigh[warp], 4 * (int)lane, 0, 1), top, sum);
+  }
+  __syncthreads();                                  // (what is shared is written again)
   }
 }
 

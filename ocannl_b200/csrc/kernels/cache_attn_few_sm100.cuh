@@ -11,9 +11,10 @@
 // again: out = sum w code / sum (w / scale), so that weights stay in the range of a half whatever the scales.  (bfloat16 queries beside codes become
 // halves too, each row multiplied by the power of two that brings its largest to 2^14.)
 //
-// The tokens that a tile sees (with a window: the sinks' and the window's, as one range) are cut into chunks, so that sequences of all lengths fill the
-// machine evenly: every block sums the lengths of all sequences, from which all find the same size of a chunk and each its own.  The block of a tile that
-// comes last joins the chunks in their order: the same bits whoever comes last.
+// The tokens that all tiles see (with a window: the sinks' and the window's, as one range), tile behind tile, are one long walk, of which every block takes
+// an equal part: the end of one tile, some whole ones, the beginning of another.  Every block finds its part from the lengths of all sequences, so that sequences
+// of all lengths fill the machine evenly, in one round of blocks.  (Chunks of a tile a block, three rounds of them: 64 sequences of up to 8192 in 193 us.)  The
+// block of a tile that comes last joins its parts in their order: the same bits whoever comes last.
 #ifndef B200_CACHE_ATTN_FEW_SM100_CUH
 #define B200_CACHE_ATTN_FEW_SM100_CUH
 #include "attn_few_sm100.cuh"
@@ -22,16 +23,17 @@
 namespace b200 {
 
 struct CacheFewArgs {
-  float* parts;            // [unit][rows of a tile][DP + 4]: output (not divided), maximum, sum
-  unsigned int* tickets;   // [unit], zero between runs
-  long long target;        // chunks that fill the machine
-  int least, most;         // tokens of a chunk, about, at least; chunks of a tile at most
-  int single;              // one chunk a tile, whatever the lengths
-  Divisor by_group, by_key_heads, by_units;     // by_units: without starts, units of a sequence (single)
+  float* parts;            // [block][2][rows of a tile][DP + 4]: output (not divided), maximum, sum; of the tile that begins ahead of the block's part, then of
+                           // the one that ends behind it
+  unsigned int* tickets;   // [block], zero between runs: of the tile that begins in a block and ends in another
+  unsigned int blocks;     // that fill the machine
+  unsigned int least;      // 64s of tokens of a block at least
+  int single;              // a tile a block, whatever the lengths
+  Divisor by_group, by_key_heads, by_units;     // by_units: without starts, tiles of a sequence (single)
 };
 
 constexpr int kCacheFewWarps = 4, kCacheFewThreads = 32 * kCacheFewWarps;
-constexpr int kCacheChunk = 65536;     // tokens of a chunk at most, a quarter of them a warp's: its accumulators' cut-off sums lose 2^-13 (see kSumKeys)
+constexpr unsigned int kCachePart = 1024;     // 64s of tokens of a block at most, a quarter of them a warp's: its accumulators' cut-off sums lose 2^-13 (see kSumKeys)
 
 template <int DP, bool CODED, int NR>
 struct CacheFewShape {
@@ -72,98 +74,231 @@ __device__ __forceinline__ unsigned int transpose8(unsigned int x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-// What a sequence's tiles look at: its rows of a key head, in tiles, and no fewer tokens than any of them sees, as they are walked
+// What a sequence's tiles look at: its rows of a key head, in tiles, and no fewer 64s of tokens than any of them sees, as they are walked
 struct CacheWalk {
-  unsigned int tiles;
-  int tokens;
+  unsigned int tiles, length;
 };
 template <int ROWS>
 __device__ __forceinline__ CacheWalk cache_walk(const CacheAttnArgs& a, const CacheSeq& s) {
   CacheWalk w;
-  w.tiles = ((unsigned int)s.count * (unsigned int)a.group + (ROWS - 1)) / ROWS;
+  w.tiles = ((unsigned int)s.count * (unsigned int)a.group + (ROWS - 1)) / ROWS * (unsigned int)a.c.HK;
   long long n = (long long)cache_last(a, s.pos0 + s.count - 1) + 1;
   if (a.window) n = min(n, (long long)a.window + ((a.sinks + 15ll) & ~15ll) + ROWS / a.group + 17);
-  w.tokens = (int)max(n, 1ll);
+  w.length = (unsigned int)((max(n, 1ll) + 63) / 64);
   return w;
 }
-// chunks of about `size` tokens: the nearest number
-__device__ __forceinline__ unsigned int cache_chunks(const CacheFewArgs& f, int tokens, int size) {
-  const unsigned int n = ((unsigned int)tokens + (unsigned int)(size >> 1)) / (unsigned int)size;
-  return min(max(n, 1u), (unsigned int)f.most);
-}
 
-// A block's chunk: of a sequence, a tile of its rows of a key head, and how the tile's tokens are walked.
-struct CachePlan {
-  int b, hk, first_row, rows;          // rows of the tile that there are
+// A block's part of the walk over all tiles: where it begins, and how much is left of it.
+struct CachePart {
+  int b;
+  unsigned int tile, at, left;         // tile of the sequence (key heads beside each other); 64s
+  unsigned long long ahead, quota;     // of the sequence: 64s of the sequences before it; a block's part
   CacheSeq s;
-  unsigned int chunks, first_unit;     // of the tile; the number of its first block
+  CacheWalk walk;
+};
+// A piece of a tile: which rows of a key head, and which of the tokens that they see.
+struct CachePiece {
+  int hk, first_row, rows;             // rows of the tile that there are
   int least_pos, most_pos, end;        // positions of its rows; tokens that some row sees lie before `end`
   int sink_end, shift;                 // the walk: tokens 0 .. sink_end - 1, then those from sink_end + shift on
-  int begin, stop;                     // of the walk, this chunk's
+  int begin, stop;                     // of the walk, this piece's
+  unsigned int parts, part, first_block;     // of the tile
   __device__ __forceinline__ int token_of(int v) const { return v < sink_end ? v : v + shift; }
 };
+// a part's place: of the tile that begins in `first_block`
+__device__ __forceinline__ long long cache_part_at(unsigned int first_block, unsigned int part) { return ((long long)first_block + part) * 2 + (part == 0 ? 1 : 0); }
+
 template <int NT, int ROWS>
-__device__ __forceinline__ bool cache_plan(const CacheAttnArgs& a, const CacheFewArgs& f, CachePlan& p) {
+__device__ __forceinline__ bool cache_part(const CacheAttnArgs& a, const CacheFewArgs& f, CachePart& p) {
   const CacheArgs& c = a.c;
-  __shared__ unsigned long long works[NT / 32];
-  unsigned int nth;
-  p.chunks = 1;
-  if (f.single && !c.starts) {
-    p.b = (int)f.by_units.of(blockIdx.x);
-    nth = blockIdx.x - (unsigned int)p.b * f.by_units.d;
-    if (p.b >= c.batch) return false;
-  } else {
-    int size = 0x7fffffff;
-    if (!f.single) {
-      unsigned long long work = 0;
-      for (int i = (int)threadIdx.x; i < c.batch; i += NT) {
-        const CacheSeq s = cache_seq(c, i);
-        if (s.count) {
-          const CacheWalk w = cache_walk<ROWS>(a, s);
-          work += (unsigned long long)w.tiles * (unsigned int)w.tokens;
-        }
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) work += __shfl_xor_sync(0xffffffffu, work, o);
-      if ((threadIdx.x & 31u) == 0) works[threadIdx.x >> 5] = work;
-      __syncthreads();
-      work = 0;
-#pragma unroll
-      for (int i = 0; i < NT / 32; ++i) work += works[i];
-      size = (int)min(max((long long)(work * (unsigned int)c.HK / (unsigned long long)f.target) + 1, (long long)f.least), (long long)kCacheChunk);
+  if (f.single) {
+    unsigned int nth;
+    if (c.starts) {
+      if (!find_unit<NT>(c.batch, blockIdx.x, [&](int i) { return cache_walk<ROWS>(a, cache_seq(c, i)).tiles; }, p.b, nth)) return false;
+    } else {
+      p.b = (int)f.by_units.of(blockIdx.x);
+      nth = blockIdx.x - (unsigned int)p.b * f.by_units.d;
+      if (p.b >= c.batch) return false;
     }
-    const bool found = find_unit<NT>(
-        c.batch, blockIdx.x,
-        [&](int i) {
-          const CacheSeq s = cache_seq(c, i);
-          if (!s.count) return 0u;
-          const CacheWalk w = cache_walk<ROWS>(a, s);
-          return w.tiles * (unsigned int)c.HK * (f.single ? 1u : cache_chunks(f, w.tokens, size));
-        },
-        p.b, nth);
-    if (!found) return false;
-    if (!f.single) p.chunks = cache_chunks(f, cache_walk<ROWS>(a, cache_seq(c, p.b)).tokens, size);
+    p.s = cache_seq(c, p.b);
+    p.walk = cache_walk<ROWS>(a, p.s);
+    p.tile = nth;
+    p.at = 0;
+    p.left = p.walk.length;
+    p.ahead = p.quota = 0;
+    return true;
   }
+  __shared__ unsigned long long sums[NT / 32], found[2];
+  const unsigned int lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+  auto length_of = [&](int i) -> unsigned long long {
+    if (i >= c.batch) return 0ull;
+    const CacheSeq s = cache_seq(c, i);
+    if (!s.count) return 0ull;
+    const CacheWalk w = cache_walk<ROWS>(a, s);
+    return (unsigned long long)w.tiles * w.length;
+  };
+  // the whole walk; with a sequence a thread, one look at the lengths finds the block's own place as well
+  unsigned long long all = 0, mine = 0, before = 0;
+  for (int i0 = 0; i0 < c.batch; i0 += NT) {
+    mine = length_of(i0 + (int)threadIdx.x);
+    unsigned long long up_to = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned long long x = __shfl_up_sync(0xffffffffu, up_to, o);
+      if (lane >= (unsigned int)o) up_to += x;
+    }
+    __syncthreads();
+    if (lane == 31) sums[warp] = up_to;
+    __syncthreads();
+    before = all + up_to - mine;
+#pragma unroll
+    for (int w = 0; w < NT / 32; ++w) {
+      if (w < (int)warp) before += sums[w];
+      all += sums[w];
+    }
+  }
+  p.quota = min(max((all + f.blocks - 1) / f.blocks, (unsigned long long)f.least), (unsigned long long)kCachePart);
+  const unsigned long long from = p.quota * blockIdx.x;
+  if (from >= all) return false;
+  if (c.batch <= NT) {
+    if (before <= from && from < before + mine) {
+      found[0] = threadIdx.x;
+      found[1] = before;
+    }
+  } else {
+    unsigned long long sum = 0;
+    for (int i0 = 0; i0 < c.batch; i0 += NT) {
+      mine = length_of(i0 + (int)threadIdx.x);
+      unsigned long long up_to = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned long long x = __shfl_up_sync(0xffffffffu, up_to, o);
+        if (lane >= (unsigned int)o) up_to += x;
+      }
+      __syncthreads();
+      if (lane == 31) sums[warp] = up_to;
+      __syncthreads();
+      before = sum + up_to - mine;
+#pragma unroll
+      for (int w = 0; w < NT / 32; ++w) {
+        if (w < (int)warp) before += sums[w];
+        sum += sums[w];
+      }
+      if (before <= from && from < before + mine) {
+        found[0] = (unsigned long long)(i0 + (int)threadIdx.x);
+        found[1] = before;
+      }
+    }
+  }
+  __syncthreads();
+  p.b = (int)found[0];
+  p.ahead = found[1];
   p.s = cache_seq(c, p.b);
-  const unsigned int pair = nth / p.chunks, chunk = nth - pair * p.chunks;
-  const unsigned int tile = f.by_key_heads.of(pair);
-  p.first_unit = blockIdx.x - chunk;
-  p.hk = (int)(pair - tile * (unsigned int)c.HK);
-  p.first_row = (int)tile * ROWS;
-  p.rows = min(ROWS, p.s.count * a.group - p.first_row);
-  p.least_pos = p.s.pos0 + (int)f.by_group.of((unsigned int)p.first_row);
-  p.most_pos = p.s.pos0 + (int)f.by_group.of((unsigned int)(p.first_row + p.rows - 1));
-  p.end = cache_last(a, p.most_pos) + 1;
-  p.sink_end = p.shift = 0;
-  if (a.window) {
-    p.sink_end = (int)min(((long long)min(a.sinks, max(p.end, 0)) + 15) & ~15ll, 0x7ffffff0ll);
-    p.shift = max((cache_first(a, p.least_pos) & ~15) - p.sink_end, 0);
-  }
-  const int n_tokens = p.shift ? max(p.end - p.shift, p.sink_end) : max(p.end, 0);       // (the window may lie behind the last page)
-  const int per = (int)((((long long)n_tokens + p.chunks - 1) / p.chunks + 63) & ~63ll);
-  p.begin = (int)min((long long)chunk * per, (long long)n_tokens);
-  p.stop = (int)min((long long)p.begin + per, (long long)n_tokens);
+  p.walk = cache_walk<ROWS>(a, p.s);
+  const unsigned long long rest = from - p.ahead;
+  p.tile = (unsigned int)(rest / p.walk.length);
+  p.at = (unsigned int)(rest - (unsigned long long)p.tile * p.walk.length);
+  p.left = (unsigned int)min(p.quota, all - from);
   return true;
+}
+// the next piece of the part; false: there is none
+template <int ROWS>
+__device__ __forceinline__ bool cache_piece(const CacheAttnArgs& a, const CacheFewArgs& f, CachePart& p, CachePiece& piece) {
+  const CacheArgs& c = a.c;
+  if (!p.left) return false;
+  const unsigned int take = min(p.left, p.walk.length - p.at), tile = f.by_key_heads.of(p.tile);
+  piece.hk = (int)(p.tile - tile * (unsigned int)c.HK);
+  piece.first_row = (int)tile * ROWS;
+  piece.rows = min(ROWS, p.s.count * a.group - piece.first_row);
+  piece.least_pos = p.s.pos0 + (int)f.by_group.of((unsigned int)piece.first_row);
+  piece.most_pos = p.s.pos0 + (int)f.by_group.of((unsigned int)(piece.first_row + piece.rows - 1));
+  piece.end = cache_last(a, piece.most_pos) + 1;
+  piece.sink_end = piece.shift = 0;
+  if (a.window) {
+    piece.sink_end = (int)min(((long long)min(a.sinks, max(piece.end, 0)) + 15) & ~15ll, 0x7ffffff0ll);
+    piece.shift = max((cache_first(a, piece.least_pos) & ~15) - piece.sink_end, 0);
+  }
+  const int n_tokens = piece.shift ? max(piece.end - piece.shift, piece.sink_end) : max(piece.end, 0);       // (the window may lie behind the last page)
+  piece.begin = (int)min((long long)p.at * 64, (long long)n_tokens);
+  piece.stop = (int)min((long long)(p.at + take) * 64, (long long)n_tokens);
+  piece.parts = 1;
+  piece.part = 0;
+  piece.first_block = blockIdx.x;
+  if (take < p.walk.length) {
+    const unsigned long long from = p.ahead + (unsigned long long)p.tile * p.walk.length;
+    piece.first_block = (unsigned int)(from / p.quota);
+    piece.parts = (unsigned int)((from + p.walk.length - 1) / p.quota) - piece.first_block + 1;
+    piece.part = blockIdx.x - piece.first_block;
+  }
+  return true;
+}
+// ... and on behind it
+template <int ROWS>
+__device__ __forceinline__ void cache_advance(const CacheAttnArgs& a, CachePart& p) {
+  p.left -= min(p.left, p.walk.length - p.at);
+  p.at = 0;
+  if (!p.left || ++p.tile < p.walk.tiles) return;
+  p.tile = 0;
+  p.ahead += (unsigned long long)p.walk.tiles * p.walk.length;
+  do {
+    p.s = cache_seq(a.c, ++p.b);
+  } while (!p.s.count && p.b + 1 < a.c.batch);
+  p.walk = cache_walk<ROWS>(a, p.s);
+}
+
+// The parts of a row: the first lies a place behind the others' line, (2 k - 1) places on for k > 0
+template <int DP, int R>
+__device__ __forceinline__ const float* cache_part_row(const float* first, int k) { return first + (k ? (2 * k - 1) : 0) * (long long)(R * (DP + 4)); }
+// their maximum and sum, and in `weight` what each is multiplied by: a warp (see few_weigh)
+template <int DP, int R>
+__device__ __forceinline__ void cache_weigh(const float* first, int n, float* weight, float& top, float& sum) {
+  const unsigned int lane = threadIdx.x & 31u;
+  float t[kFewMost / 32], u[kFewMost / 32];
+  top = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < kFewMost / 32; ++k) {
+    const int i = (int)lane + 32 * k;
+    t[k] = -INFINITY;
+    u[k] = 0.f;
+    if (i < n) {
+      const float* row = cache_part_row<DP, R>(first, i);
+      t[k] = row[DP];
+      u[k] = row[DP + 1];
+    }
+    top = fmaxf(top, t[k]);
+  }
+#pragma unroll
+  for (int k = 16; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+  sum = 0.f;
+  __syncwarp();                     // (all lanes have read the weights of the row before)
+#pragma unroll
+  for (int k = 0; k < kFewMost / 32; ++k) {
+    const float w = u[k] == 0.f ? 0.f : t[k] == -INFINITY ? 1.f : ex2(t[k] - top);
+    if ((int)lane + 32 * k < n) weight[lane + 32 * k] = w;
+    if (w != 0.f) sum = fmaf(w, u[k], sum);
+  }
+#pragma unroll
+  for (int k = 16; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+  __syncwarp();
+}
+// four elements of their weighed sum, in their order; eight loads under way together
+template <int DP, int R>
+__device__ __forceinline__ float4 cache_gather(const float* first, int n, const float* weight, int e) {
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = 0; i < n; i += 8) {
+    float4 x[8];
+    float w[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int at = i + k;
+      w[k] = at < n ? weight[at] : 0.f;
+      x[k] = *(const float4*)(cache_part_row<DP, R>(first, at < n ? at : i) + e);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (w[k] != 0.f) v = make_float4(fmaf(w[k], x[k].x, v.x), fmaf(w[k], x[k].y, v.y), fmaf(w[k], x[k].z, v.z), fmaf(w[k], x[k].w, v.w));
+  }
+  return v;
 }
 
 // Writes four elements of a row and, with the first, its lse; false: one is infinite or undefined, and the row has to be done again
@@ -198,11 +333,12 @@ __global__ void __launch_bounds__(kCacheFewThreads, (CacheFewShape<DP, CODED, NR
   const unsigned int warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, q4 = lane & 3u;
   grid_begin();
 
-  CachePlan plan;
-  if (!cache_plan<kCacheFewThreads, R>(a, f, plan)) return;
-  const CacheSeq& s = plan.s;
-  const int b = plan.b, hk = plan.hk, first_row = plan.first_row, rows = plan.rows, end = plan.end, v_begin = plan.begin, v_end = plan.stop;
-  const unsigned int chunks = plan.chunks, first_unit = plan.first_unit;
+  CachePart part;
+  if (!cache_part<kCacheFewThreads, R>(a, f, part)) return;
+  CachePiece plan;
+  for (; cache_piece<R>(a, f, part, plan); cache_advance<R>(a, part)) {
+  const CacheSeq s = part.s;
+  const int b = part.b, hk = plan.hk, first_row = plan.first_row, rows = plan.rows, end = plan.end, v_begin = plan.begin, v_end = plan.stop;
   auto query_of = [&](int i) { return (int)f.by_group.of((unsigned int)(first_row + i)); };
   auto head_of = [&](int i) { return hk * a.group + first_row + i - query_of(i) * a.group; };
   // (this lane's columns are rows 8 r + 2 q4 and the next one)
@@ -221,18 +357,36 @@ __global__ void __launch_bounds__(kCacheFewThreads, (CacheFewShape<DP, CODED, NR
   auto key_bytes = [&](int p) { return (int)q4 * 16 + p * 64 < line ? 16 : 0; };
   auto value_bytes = [&](int p) { return (int)g * Sh::kValueBytes + p * 16 < line ? Sh::kValueWidth : 0; };
   const int key_at = (int)g * line + (int)q4 * 16, value_at = (int)q4 * 2 * line + (int)g * Sh::kValueBytes;
-  int ahead = 0 < mine ? page_of(token_of(0)) : -1;  // the page of the step that is fetched next
+  // WHOLE: where 32 steps lie, a lane each (bytes; -1: not there), and their pages' scales; and the same of the 32 steps behind them
+  long long where[2] = {-1, -1};
+  float ks[2] = {1.f, 1.f}, vs[2] = {1.f, 1.f};
+  auto look = [&](int n0, int k) {
+    const int n = n0 + (int)lane;
+    where[k] = -1;
+    if (n >= mine) return;
+    const int j = token_of(n);
+    const unsigned int index = c.by_page.of((unsigned int)j);
+    const int page = cache_page_at(c, b, index);
+    if (page < 0) return;
+    where[k] = (cache_at(c, page, hk) + (long long)((unsigned int)j - index * c.page) * c.D) * kSize;
+    if constexpr (CODED) {
+      ks[k] = __ldg(c.k_scale + (long long)page * c.HK + hk);
+      vs[k] = __ldg(c.v_scale + (long long)page * c.HK + hk);
+    }
+  };
+  if (WHOLE) {
+    look(0, 0);
+    if (mine > 32) look(32, 1);
+  }
   unsigned int to = 0;                               // the slot that is filled next
+  int first_of = 0;                                  // the step that where[0] begins with
   auto fetch = [&](int n) {
     if (n < mine) {
       const int j0 = token_of(n);
       const unsigned int at_k = ring + to * Sh::kStage + lane * 16, at_v = ring + to * Sh::kStage + Sh::kKeys + lane * Sh::kValueWidth;
-      const int page = ahead;
       if (WHOLE) {
-        if (n + 1 < mine) ahead = page_of(token_of(n + 1));
-        const unsigned int slot0 = (unsigned int)j0 - c.by_page.of((unsigned int)j0) * c.page;
-        const long long from = page >= 0 ? (cache_at(c, page, hk) + (long long)slot0 * c.D) * kSize : 0;
-        const int left = page >= 0 ? end - j0 : 0;   // tokens of the step that are there
+        const long long from0 = __shfl_sync(0xffffffffu, n - first_of < 32 ? where[0] : where[1], n & 31), from = max(from0, 0ll);
+        const int left = from0 >= 0 ? end - j0 : 0;  // tokens of the step that are there
         const unsigned char *const k0 = keys + from + key_at, *const v0 = values + from + value_at;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
@@ -357,45 +511,51 @@ __global__ void __launch_bounds__(kCacheFewThreads, (CacheFewShape<DP, CODED, NR
     for (int k = 0; k < 2; ++k) m[r][k] = -INFINITY, l[r][k] = 0.f;
   }
 
-  // the page of the step at hand, or (not WHOLE) those of this lane's tokens g and g + 8, and their scales: a step ahead
-  int there[2] = {-1, -1};
-  float ks[2] = {1.f, 1.f}, vs[2] = {1.f, 1.f};
-  auto look = [&](int n) {
+  // (not WHOLE: of this lane's tokens g and g + 8 of the step at hand, a step ahead)
+  bool there[2] = {false, false};
+  auto look_at = [&](int n) {
     if (n >= mine) return;
-    const int j0 = token_of(n);
 #pragma unroll
-    for (int k = 0; k < (WHOLE ? 1 : 2); ++k) {
-      const int j = WHOLE ? j0 : j0 + (int)g + 8 * k;
-      there[k] = j < end ? page_of(j) : -1;
-      if (CODED && there[k] >= 0) {
-        ks[k] = __ldg(c.k_scale + (long long)there[k] * c.HK + hk);
-        vs[k] = __ldg(c.v_scale + (long long)there[k] * c.HK + hk);
+    for (int k = 0; k < 2; ++k) {
+      const int j = token_of(n) + (int)g + 8 * k, page = j < end ? page_of(j) : -1;
+      there[k] = page >= 0;
+      if (CODED && page >= 0) {
+        ks[k] = __ldg(c.k_scale + (long long)page * c.HK + hk);
+        vs[k] = __ldg(c.v_scale + (long long)page * c.HK + hk);
       }
     }
   };
-  look(0);
+  if (!WHOLE) look_at(0);
   unsigned int slot = 0;
   for (int n = 0; n < mine; ++n) {
     const int j0 = token_of(n);
-    const int here[2] = {there[0], WHOLE ? there[0] : there[1]};
+    if (WHOLE && n - first_of == 32) {
+      // (copies are at most a few steps ahead: in the second 32)
+      first_of = n;
+      where[0] = where[1];
+      ks[0] = ks[1];
+      vs[0] = vs[1];
+      if (mine - n > 32) look(n + 32, 1);
+    }
+    const bool here[2] = {WHOLE ? __shfl_sync(0xffffffffu, (int)(where[0] >= 0), n & 31) != 0 : there[0], there[1]};
     // scale of the keys; of the values its inverse and its logarithm
     float down[2] = {1.f, 1.f}, back[2] = {1.f, 1.f}, raise[2] = {0.f, 0.f};
     if constexpr (CODED) {
 #pragma unroll
       for (int k = 0; k < (WHOLE ? 1 : 2); ++k) {
-        down[k] = cache_scale(ks[k]);
-        const float v = cache_scale(vs[k]);
+        down[k] = cache_scale(WHOLE ? __shfl_sync(0xffffffffu, ks[0], n & 31) : ks[k]);
+        const float v = cache_scale(WHOLE ? __shfl_sync(0xffffffffu, vs[0], n & 31) : vs[k]);
         back[k] = rcp(v);
         asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(raise[k]) : "f"(v));
       }
       if (WHOLE) down[1] = down[0], back[1] = back[0], raise[1] = raise[0];
     }
-    look(n + 1);
+    if (!WHOLE) look_at(n + 1);
     asm volatile("cp.async.wait_group %0;" ::"n"(Sh::kStages - 2) : "memory");
     fetch(n + Sh::kStages - 1);       // into the slot of the step before, which this lane alone reads
     const unsigned int at_k = ring + slot * Sh::kStage + lane * 16, at_v = ring + slot * Sh::kStage + Sh::kKeys + lane * Sh::kValueWidth;
     slot = slot + 1 == Sh::kStages ? 0 : slot + 1;
-    if (WHOLE && here[0] < 0) continue;
+    if (WHOLE && !here[0]) continue;
     // scores of tokens g (x[.][.][0, 1]) and g + 8 ([2, 3]); two sums, so that one product need not wait for the other
     float x[NR][4], x2[NR][4];
 #pragma unroll
@@ -449,7 +609,7 @@ __global__ void __launch_bounds__(kCacheFewThreads, (CacheFewShape<DP, CODED, NR
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const int j = j0 + (int)g + 8 * (k >> 1), at = pos[r][k & 1];
-          const bool on = j <= at && j < end && (j >= cache_first(a, at) || j < a.sinks) && here[k >> 1] >= 0;
+          const bool on = j <= at && j < end && (j >= cache_first(a, at) || j < a.sinks) && here[WHOLE ? 0 : k >> 1];
           x[r][k] = on ? x[r][k] : -INFINITY;
         }
       top[r][0] = fmaxf(x[r][0], x[r][2]);
@@ -555,9 +715,10 @@ __global__ void __launch_bounds__(kCacheFewThreads, (CacheFewShape<DP, CODED, NR
   __syncthreads();
   const int lane_e = 4 * (int)lane;
   __shared__ float weights[kCacheFewWarps][kFewMost];
-  float* parts = f.parts + (long long)blockIdx.x * R * W;
   // a warp takes every fourth row
-  if (chunks > 1) {
+  bool last = true;
+  if (plan.parts > 1) {
+    float* parts = f.parts + cache_part_at(plan.first_block, plan.part) * R * W;
     for (int i = (int)warp; i < rows; i += kCacheFewWarps) {
       float most, sum;
       few_weigh<DP>(join + i * W, kCacheFewWarps, R * W, weights[warp], most, sum);
@@ -569,20 +730,35 @@ __global__ void __launch_bounds__(kCacheFewThreads, (CacheFewShape<DP, CODED, NR
     }
     __threadfence();
     __syncthreads();
-    if (threadIdx.x == 0) last_block = atomicAdd(&f.tickets[first_unit], 1u) == chunks - 1u;
+    if (threadIdx.x == 0) {
+      last_block = atomicAdd(&f.tickets[plan.first_block], 1u) == plan.parts - 1u;
+      if (last_block) f.tickets[plan.first_block] = 0u;       // for the next run
+    }
     __syncthreads();
-    if (!last_block) return;
-    if (threadIdx.x == 0) f.tickets[first_unit] = 0u;       // for the next run
+    last = last_block != 0u;
     __threadfence();
   }
-  const float* all = chunks > 1 ? f.parts + (long long)first_unit * R * W : join;
-  const int n_parts = chunks > 1 ? (int)chunks : kCacheFewWarps;
-  for (int i = (int)warp; i < rows; i += kCacheFewWarps) {
-    float most, sum;
-    few_weigh<DP>(all + i * W, n_parts, R * W, weights[warp], most, sum);
-    bool fine = true;
-    if (lane_e < DP) fine = cache_finish<T>(a, s.first + query_of(i), head_of(i), lane_e, few_gather(all + i * W, n_parts, R * W, weights[warp], lane_e, 0, 1), most, sum, kUp);
-    if (attn_again(fine)) cache_attention_row<T, CODED>(a, b, head_of(i), s.first + query_of(i), s.pos0 + query_of(i), lane);
+  if (last) {
+    // (parts lie two a block apart, but for the first, which is the second of its block)
+    const bool joined = plan.parts > 1;
+    const float* all = joined ? f.parts + cache_part_at(plan.first_block, 0) * R * W : join;
+    const int n_parts = joined ? (int)plan.parts : kCacheFewWarps;
+    for (int i = (int)warp; i < rows; i += kCacheFewWarps) {
+      float most, sum;
+      bool fine = true;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (joined) {
+        cache_weigh<DP, R>(all + i * W, n_parts, weights[warp], most, sum);
+        if (lane_e < DP) v = cache_gather<DP, R>(all + i * W, n_parts, weights[warp], lane_e);
+      } else {
+        few_weigh<DP>(all + i * W, n_parts, R * W, weights[warp], most, sum);
+        if (lane_e < DP) v = few_gather(all + i * W, n_parts, R * W, weights[warp], lane_e, 0, 1);
+      }
+      if (lane_e < DP) fine = cache_finish<T>(a, s.first + query_of(i), head_of(i), lane_e, v, most, sum, kUp);
+      if (attn_again(fine)) cache_attention_row<T, CODED>(a, b, head_of(i), s.first + query_of(i), s.pos0 + query_of(i), lane);
+    }
+  }
+  __syncthreads();                    // (the rings, and what lies where they were, are written again)
   }
 }
 

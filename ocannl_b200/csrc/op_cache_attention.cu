@@ -76,17 +76,16 @@ struct CacheAttnOperator : b200_operator {
     if (pieces()) return many() ? choose_tiles() : choose_few();
     choose_any();
   }
-  // Rows in tiles, tokens in chunks of about `least` at least, as many as give every SM three rounds of blocks; a tile adds one chunk at most, those cut
-  // for their length aside.
-  void choose_chunks(int rows_of_tile, int floats, int blocks, int least) {
+  // Rows in tiles, whose tokens are dealt out evenly to as many blocks as the machine holds, `least` 64s of them at least.
+  void choose_parts(int rows_of_tile, int floats, int blocks, int least) {
     const CacheArgs& c = a.c;
     // A sequence of n tokens has n group rows.
     const long long some = std::min(c.batch, c.tokens), tiles = ((long long)c.tokens * a.group + (rows_of_tile - 1) * some) / rows_of_tile * c.HK;
-    const long long capacity = std::min<long long>((long long)c.max_pages * c.page, 0x7fffffff);
-    few_args.target = (long long)dev->sm_count * blocks * 3;
-    few_args.least = least;
-    few_args.most = kFewMost;
-    few_args.single = capacity < least + least / 2;
+    const long long capacity = (std::min<long long>((long long)c.max_pages * c.page, 0x7fffffff) + 127) / 64;       // 64s
+    few_args.blocks = (unsigned int)(dev->sm_count * blocks);
+    few_args.least = (unsigned int)std::max<long long>(least, capacity / (kFewMost - 4) + 1);
+    // Short sequences: a tile a block.
+    few_args.single = capacity <= (long long)few_args.least + few_args.least / 2;
     few_args.by_group = Divisor((unsigned int)a.group);
     few_args.by_key_heads = Divisor((unsigned int)c.HK);
     if (few_args.single) {
@@ -96,13 +95,13 @@ struct CacheAttnOperator : b200_operator {
         few_args.by_units = Divisor(blocks_of(each));
         grid = blocks_of(each * c.batch);
       }
-    } else {
-      // (the nearest number of chunks: up to one and a half times the size each)
-      const unsigned __int128 walk = (unsigned __int128)tiles * (unsigned long long)(capacity + 64);
-      const unsigned __int128 cut = std::max<unsigned __int128>((unsigned long long)few_args.target, walk / kCacheChunk), fewest = walk / (unsigned int)least;
-      grid = blocks_of((long long)std::min<unsigned __int128>(std::min(cut, fewest) + (unsigned long long)tiles, 1ull << 31));
+      return;
     }
-    const size_t parts = few_args.single ? 0 : (size_t)grid * rows_of_tile * floats * 4;
+    // (more blocks only where an even share would be longer than a part may be; fewer where there is not that much)
+    const unsigned __int128 walk = (unsigned __int128)blocks_of(tiles) * (unsigned long long)capacity;
+    const unsigned __int128 cut = std::max<unsigned __int128>(few_args.blocks, walk / kCachePart + 1), most = walk / few_args.least + 1;
+    grid = blocks_of((long long)std::min<unsigned __int128>(std::min(cut, most), 1ull << 31));
+    const size_t parts = ((size_t)grid + 1) * 2 * rows_of_tile * floats * 4;
     take_workspace(parts + (size_t)grid * 4);
     few_args.parts = (float*)workspace;
     few_args.tickets = (unsigned int*)(workspace + parts);
@@ -117,7 +116,7 @@ struct CacheAttnOperator : b200_operator {
     else if (dtype == B200_BF16) set_any<__nv_bfloat16>();
     else set_any<__half>();
     smem = any_smem(a.c.D);
-    choose_chunks(kAnyRows, kAnyWidth, (int)std::min<size_t>(6, 220 * 1024 / (smem + 7 * 1024)), 256);
+    choose_parts(kAnyRows, kAnyWidth, (int)std::min<size_t>(6, 220 * 1024 / (smem + 7 * 1024)), 4);
     ready(any, smem);
   }
   // Whole prompts: tiles of 128 rows on the tensor cores, where sequences have them on average and the cache's pages are boxes of the TMA unit.
@@ -152,7 +151,7 @@ struct CacheAttnOperator : b200_operator {
     const bool wide = (long long)c.tokens * a.group > 8ll * std::min(c.batch, c.tokens);
     if (dtype == B200_BF16) c.D <= 64 ? set_few<__nv_bfloat16, 64>(wide) : set_few<__nv_bfloat16, 128>(wide);
     else c.D <= 64 ? set_few<__half, 64>(wide) : set_few<__half, 128>(wide);
-    choose_chunks(tile, width, resident, 512);
+    choose_parts(tile, width, resident, 4);
     ready(few, smem);
   }
   void run(cudaStream_t s) override {
