@@ -51,6 +51,11 @@ struct CacheFewShape {
   static constexpr int kBlocks = NR == 1 ? 4 : 3;                      // of an SM
 };
 
+template <int BYTES>
+__device__ __forceinline__ void copy_whole(unsigned int dst, const void* src) {
+  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
+}
 // BYTES from memory, of which those behind `bytes` are zeros
 template <int BYTES>
 __device__ __forceinline__ void copy_in(unsigned int dst, const void* src, int bytes) {
@@ -359,7 +364,15 @@ __global__ void __launch_bounds__(kCacheFewThreads, (CacheFewShape<DP, CODED, NR
   const int key_at = (int)g * line + (int)q4 * 16, value_at = (int)q4 * 2 * line + (int)g * Sh::kValueBytes;
   // WHOLE: where 32 steps lie, a lane each (bytes; -1: not there), and their pages' scales; and the same of the 32 steps behind them
   long long where[2] = {-1, -1};
-  float ks[2] = {1.f, 1.f}, vs[2] = {1.f, 1.f};
+  struct Scales {
+    float down, back, raise;                         // of the keys; of the values its inverse and its logarithm
+    __device__ __forceinline__ void of(const CacheArgs& c, long long at) {
+      down = cache_scale(__ldg(c.k_scale + at));
+      const float v = cache_scale(__ldg(c.v_scale + at));
+      back = rcp(v);
+      asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(raise) : "f"(v));
+    }
+  } scales[2] = {{1.f, 1.f, 0.f}, {1.f, 1.f, 0.f}};
   auto look = [&](int n0, int k) {
     const int n = n0 + (int)lane;
     where[k] = -1;
@@ -369,10 +382,7 @@ __global__ void __launch_bounds__(kCacheFewThreads, (CacheFewShape<DP, CODED, NR
     const int page = cache_page_at(c, b, index);
     if (page < 0) return;
     where[k] = (cache_at(c, page, hk) + (long long)((unsigned int)j - index * c.page) * c.D) * kSize;
-    if constexpr (CODED) {
-      ks[k] = __ldg(c.k_scale + (long long)page * c.HK + hk);
-      vs[k] = __ldg(c.v_scale + (long long)page * c.HK + hk);
-    }
+    if constexpr (CODED) scales[k].of(c, (long long)page * c.HK + hk);
   };
   if (WHOLE) {
     look(0, 0);
@@ -388,22 +398,36 @@ __global__ void __launch_bounds__(kCacheFewThreads, (CacheFewShape<DP, CODED, NR
         const long long from0 = __shfl_sync(0xffffffffu, n - first_of < 32 ? where[0] : where[1], n & 31), from = max(from0, 0ll);
         const int left = from0 >= 0 ? end - j0 : 0;  // tokens of the step that are there
         const unsigned char *const k0 = keys + from + key_at, *const v0 = values + from + value_at;
+        if (left >= 16 && c.D == DP) {
+          // (all but a tile's last step, of heads that fill their pieces: places known beforehand)
+          constexpr int kLine = DP * kSize;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const bool on = (int)g + 8 * k < left;
+          for (int k = 0; k < 2; ++k)
 #pragma unroll
-          for (int p = 0; p < Sh::kPerKey; ++p) {
-            const int bytes = on ? key_bytes(p) : 0;
-            copy_in<16>(at_k + (k * Sh::kPerKey + p) * 512, bytes ? k0 + k * 8 * line + p * 64 : keys, bytes);
+            for (int p = 0; p < Sh::kPerKey; ++p) copy_whole<16>(at_k + (k * Sh::kPerKey + p) * 512, k0 + k * 8 * kLine + p * 64);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int p = 0; p < Sh::kPerValue; ++p)
+              copy_whole<Sh::kValueWidth>(at_v + (k * Sh::kPerValue + p) * 32 * Sh::kValueWidth, v0 + ((k & 1) + 8 * (k >> 1)) * kLine + p * 16);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const bool on = (int)g + 8 * k < left;
+#pragma unroll
+            for (int p = 0; p < Sh::kPerKey; ++p) {
+              const int bytes = on ? key_bytes(p) : 0;
+              copy_in<16>(at_k + (k * Sh::kPerKey + p) * 512, bytes ? k0 + k * 8 * line + p * 64 : keys, bytes);
+            }
           }
-        }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const bool on = (int)q4 * 2 + (k & 1) + 8 * (k >> 1) < left;
+          for (int k = 0; k < 4; ++k) {
+            const bool on = (int)q4 * 2 + (k & 1) + 8 * (k >> 1) < left;
 #pragma unroll
-          for (int p = 0; p < Sh::kPerValue; ++p) {
-            const int bytes = on ? value_bytes(p) : 0;
-            copy_in<Sh::kValueWidth>(at_v + (k * Sh::kPerValue + p) * 32 * Sh::kValueWidth, bytes ? v0 + ((k & 1) + 8 * (k >> 1)) * line + p * 16 : values, bytes);
+            for (int p = 0; p < Sh::kPerValue; ++p) {
+              const int bytes = on ? value_bytes(p) : 0;
+              copy_in<Sh::kValueWidth>(at_v + (k * Sh::kPerValue + p) * 32 * Sh::kValueWidth, bytes ? v0 + ((k & 1) + 8 * (k >> 1)) * line + p * 16 : values, bytes);
+            }
           }
         }
       } else {
@@ -500,7 +524,7 @@ __global__ void __launch_bounds__(kCacheFewThreads, (CacheFewShape<DP, CODED, NR
     }
 
   // element g * DP / 8 + 2 i + (k >> 1) of column k & 1 is o[r][i][k]
-  float o[NR][DP / 16][4], m[NR][2], l[NR][2];
+  float o[NR][DP / 16][4], m[NR][2], l[NR][2], limit[NR][2], off[NR][2];       // (the maximum in use, what outgrows it, what is taken off)
 #pragma unroll
   for (int r = 0; r < NR; ++r) {
 #pragma unroll
@@ -508,7 +532,7 @@ __global__ void __launch_bounds__(kCacheFewThreads, (CacheFewShape<DP, CODED, NR
 #pragma unroll
       for (int k = 0; k < 4; ++k) o[r][i][k] = 0.f;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) m[r][k] = -INFINITY, l[r][k] = 0.f;
+    for (int k = 0; k < 2; ++k) m[r][k] = limit[r][k] = -INFINITY, l[r][k] = off[r][k] = 0.f;
   }
 
   // (not WHOLE: of this lane's tokens g and g + 8 of the step at hand, a step ahead)
@@ -519,10 +543,7 @@ __global__ void __launch_bounds__(kCacheFewThreads, (CacheFewShape<DP, CODED, NR
     for (int k = 0; k < 2; ++k) {
       const int j = token_of(n) + (int)g + 8 * k, page = j < end ? page_of(j) : -1;
       there[k] = page >= 0;
-      if (CODED && page >= 0) {
-        ks[k] = __ldg(c.k_scale + (long long)page * c.HK + hk);
-        vs[k] = __ldg(c.v_scale + (long long)page * c.HK + hk);
-      }
+      if (CODED && page >= 0) scales[k].of(c, (long long)page * c.HK + hk);
     }
   };
   if (!WHOLE) look_at(0);
@@ -533,22 +554,23 @@ __global__ void __launch_bounds__(kCacheFewThreads, (CacheFewShape<DP, CODED, NR
       // (copies are at most a few steps ahead: in the second 32)
       first_of = n;
       where[0] = where[1];
-      ks[0] = ks[1];
-      vs[0] = vs[1];
+      scales[0] = scales[1];
       if (mine - n > 32) look(n + 32, 1);
     }
     const bool here[2] = {WHOLE ? __shfl_sync(0xffffffffu, (int)(where[0] >= 0), n & 31) != 0 : there[0], there[1]};
-    // scale of the keys; of the values its inverse and its logarithm
     float down[2] = {1.f, 1.f}, back[2] = {1.f, 1.f}, raise[2] = {0.f, 0.f};
     if constexpr (CODED) {
 #pragma unroll
-      for (int k = 0; k < (WHOLE ? 1 : 2); ++k) {
-        down[k] = cache_scale(WHOLE ? __shfl_sync(0xffffffffu, ks[0], n & 31) : ks[k]);
-        const float v = cache_scale(WHOLE ? __shfl_sync(0xffffffffu, vs[0], n & 31) : vs[k]);
-        back[k] = rcp(v);
-        asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(raise[k]) : "f"(v));
+      for (int k = 0; k < 2; ++k) {
+        const Scales& of = scales[WHOLE ? 0 : k];
+        if (WHOLE && k == 1) {
+          down[1] = down[0], back[1] = back[0], raise[1] = raise[0];
+        } else {
+          down[k] = WHOLE ? __shfl_sync(0xffffffffu, of.down, n & 31) : of.down;
+          back[k] = WHOLE ? __shfl_sync(0xffffffffu, of.back, n & 31) : of.back;
+          raise[k] = WHOLE ? __shfl_sync(0xffffffffu, of.raise, n & 31) : of.raise;
+        }
       }
-      if (WHOLE) down[1] = down[0], back[1] = back[0], raise[1] = raise[0];
     }
     if (!WHOLE) look_at(n + 1);
     asm volatile("cp.async.wait_group %0;" ::"n"(Sh::kStages - 2) : "memory");
@@ -556,12 +578,12 @@ __global__ void __launch_bounds__(kCacheFewThreads, (CacheFewShape<DP, CODED, NR
     const unsigned int at_k = ring + slot * Sh::kStage + lane * 16, at_v = ring + slot * Sh::kStage + Sh::kKeys + lane * Sh::kValueWidth;
     slot = slot + 1 == Sh::kStages ? 0 : slot + 1;
     if (WHOLE && !here[0]) continue;
-    // scores of tokens g (x[.][.][0, 1]) and g + 8 ([2, 3]); two sums, so that one product need not wait for the other
-    float x[NR][4], x2[NR][4];
+    // scores of tokens g (x[.][0, 1]) and g + 8 ([2, 3])
+    float x[NR][4];
 #pragma unroll
     for (int r = 0; r < NR; ++r)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) x[r][k] = x2[r][k] = 0.f;
+      for (int k = 0; k < 4; ++k) x[r][k] = 0.f;
 #pragma unroll
     for (int p = 0; p < Sh::kPerKey; ++p) {
       const uint4 u = from_shared16(at_k + p * 512), w = from_shared16(at_k + (Sh::kPerKey + p) * 512);
@@ -573,14 +595,14 @@ __global__ void __launch_bounds__(kCacheFewThreads, (CacheFewShape<DP, CODED, NR
           e4m3_split(uu[t], y[0], y[2]);
           e4m3_split(ww[t], y[1], y[3]);
 #pragma unroll
-          for (int r = 0; r < NR; ++r) mma16<M>(t & 1 ? x2[r] : x[r], y, q[r][4 * p + t][0], q[r][4 * p + t][1]);
+          for (int r = 0; r < NR; ++r) mma16<M>(x[r], y, q[r][4 * p + t][0], q[r][4 * p + t][1]);
         }
       } else {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           const unsigned int y[4] = {uu[2 * t], ww[2 * t], uu[2 * t + 1], ww[2 * t + 1]};
 #pragma unroll
-          for (int r = 0; r < NR; ++r) mma16<M>(t & 1 ? x2[r] : x[r], y, q[r][2 * p + t][0], q[r][2 * p + t][1]);
+          for (int r = 0; r < NR; ++r) mma16<M>(x[r], y, q[r][2 * p + t][0], q[r][2 * p + t][1]);
         }
       }
     }
@@ -589,12 +611,15 @@ __global__ void __launch_bounds__(kCacheFewThreads, (CacheFewShape<DP, CODED, NR
     float top[NR][2];
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) x[r][k] = (x[r][k] + x2[r][k]) * (CODED ? unit[r][k & 1] * down[k >> 1] : unit[r][k & 1]);
       if (a.cap > 0.f) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[r][k] *= CODED ? unit[r][k & 1] * down[k >> 1] : unit[r][k & 1];
         tanh_chunk(x[r], 1.f);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) x[r][k] *= to_log2;
+        for (int k = 0; k < 4; ++k) x[r][k] = CODED ? fmaf(x[r][k], to_log2, raise[k >> 1]) : x[r][k] * to_log2;
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[r][k] = CODED ? fmaf(x[r][k], unit[r][k & 1] * down[k >> 1], raise[k >> 1]) : x[r][k] * unit[r][k & 1];
       }
       if (a.slopes)
 #pragma unroll
@@ -602,9 +627,6 @@ __global__ void __launch_bounds__(kCacheFewThreads, (CacheFewShape<DP, CODED, NR
           const int i = min(8 * r + 2 * (int)q4 + (k & 1), rows - 1);
           x[r][k] = fmaf(-a.slopes[head_of(i)] * kCacheLog2e, (float)(pos[r][k & 1] - j0 - (int)g - 8 * (k >> 1)), x[r][k]);
         }
-      if constexpr (CODED)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) x[r][k] += raise[k >> 1];
       if (some_hidden)
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -614,7 +636,7 @@ __global__ void __launch_bounds__(kCacheFewThreads, (CacheFewShape<DP, CODED, NR
         }
       top[r][0] = fmaxf(x[r][0], x[r][2]);
       top[r][1] = fmaxf(x[r][1], x[r][3]);
-      grows = grows || top[r][0] > m[r][0] + 8.f || top[r][1] > m[r][1] + 8.f;
+      grows = grows || top[r][0] > limit[r][0] || top[r][1] > limit[r][1];
     }
     // the maximum in use moves when a row has outgrown it by 2^8 (or has had none): hardly ever after the first steps
     if (__any_sync(0xffffffffu, grows)) {
@@ -627,6 +649,8 @@ __global__ void __launch_bounds__(kCacheFewThreads, (CacheFewShape<DP, CODED, NR
           const float next = fmaxf(m[r][k], top[r][k]);
           const float by = m[r][k] == next ? 1.f : m[r][k] == -INFINITY ? 0.f : ex2(m[r][k] - next);
           m[r][k] = next;
+          limit[r][k] = next + 8.f;
+          off[r][k] = next == -INFINITY ? 0.f : next - kUp;
           l[r][k] *= by;
 #pragma unroll
           for (int i = 0; i < DP / 16; ++i) {
@@ -639,8 +663,7 @@ __global__ void __launch_bounds__(kCacheFewThreads, (CacheFewShape<DP, CODED, NR
     unsigned int wt[NR][2];
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
-      const float off0 = m[r][0] == -INFINITY ? 0.f : m[r][0] - kUp, off1 = m[r][1] == -INFINITY ? 0.f : m[r][1] - kUp;
-      const float p0 = ex2(x[r][0] - off0), p1 = ex2(x[r][1] - off1), p2 = ex2(x[r][2] - off0), p3 = ex2(x[r][3] - off1);
+      const float p0 = ex2(x[r][0] - off[r][0]), p1 = ex2(x[r][1] - off[r][1]), p2 = ex2(x[r][2] - off[r][0]), p3 = ex2(x[r][3] - off[r][1]);
       if constexpr (CODED) {
         l[r][0] = fmaf(p0, back[0], fmaf(p2, back[1], l[r][0]));
         l[r][1] = fmaf(p1, back[0], fmaf(p3, back[1], l[r][1]));
