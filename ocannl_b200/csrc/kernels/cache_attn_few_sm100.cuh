@@ -4,8 +4,9 @@
 // has no tile of 8 or 16 rows): scores' = K q', 16 tokens at a time, and out' = V' weights', so that 8 rows, as many as heads usually share a key, waste
 // nothing, and take half the registers and products of a tile of 16.  A product does not care in which order its elements are added, so the order is
 // chosen for the loads: of the 16 elements of a step each of the four lanes that share a token has four neighbours, and the rows of the second product
-// are dealt out as neighbours to a lane too, so that every operand is read as whole 16-byte pieces by the lane that multiplies it.  A lane's cp.async
-// ring is its own, with no barrier between lanes; codes of 8 bits become halves in registers, two to an instruction; a transposed pair of values is one byte
+// are dealt out as neighbours to a lane too, so that every operand is read as whole 16-byte pieces by the lane that multiplies it.  A warp's ring is
+// its own, with no barrier between warps: pages that hold whole steps of 16 tokens arrive as boxes of the TMA unit, two or four a step (by 16-byte copies of
+// all lanes, 64 sequences of up to 8192 took 182 us with their products and 183 without), others by cp.async.  Codes of 8 bits become halves in registers, two to an instruction; a transposed pair of values is one byte
 // permutation, and the weights turn from scores' to operand's layout by a transpose of 8 x 8 between lanes.  Codes are multiplied as they are: a
 // page's scale of the keys goes onto its scores, the logarithm of its scale of the values onto the exponents of its weights, which the row's sum takes off
 // again: out = sum w code / sum (w / scale), so that weights stay in the range of a half whatever the scales.  (bfloat16 queries beside codes become
@@ -43,19 +44,15 @@ struct CacheFewShape {
   static constexpr int kValueWidth = kValueBytes < 16 ? kValueBytes : 16, kPerValue = kValueBytes / kValueWidth;
   static constexpr int kKeys = 2 * kPerKey * 512, kValues = 4 * kPerValue * 32 * kValueWidth;
   static constexpr int kStage = kKeys + kValues;                       // bytes of a warp
-  static constexpr int kStages = CODED ? (DP == 64 ? 4 : 3) : DP == 64 ? 3 : 2;
+  static constexpr int kStages = kStage <= 4096 ? 4 : 3;
   static constexpr int kRing = kStages * kStage;
   static constexpr int kWidth = DP + 4;
   static constexpr int kJoin = kCacheFewWarps * kRows * kWidth * 4;
-  static constexpr int smem() { return kCacheFewWarps * kRing > kJoin ? kCacheFewWarps * kRing : kJoin; }
-  static constexpr int kBlocks = NR == 1 ? 4 : 3;                      // of an SM
+  static constexpr int smem() { return 1024 + (kCacheFewWarps * kRing > kJoin ? kCacheFewWarps * kRing : kJoin); }     // (boxes lie on 1024 bytes)
+  static constexpr int kLine = DP * (CODED ? 1 : 2) < 128 ? DP * (CODED ? 1 : 2) : 128, kPanels = DP * (CODED ? 1 : 2) / kLine;   // a box: 16 rows of so many bytes
+  static constexpr int kBlocks = kStage > 4096 ? 2 : NR == 1 && DP == 64 ? 4 : 3;      // of an SM
 };
 
-template <int BYTES>
-__device__ __forceinline__ void copy_whole(unsigned int dst, const void* src) {
-  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
-}
 // BYTES from memory, of which those behind `bytes` are zeros
 template <int BYTES>
 __device__ __forceinline__ void copy_in(unsigned int dst, const void* src, int bytes) {
@@ -326,7 +323,9 @@ __device__ __forceinline__ bool cache_finish(const CacheAttnArgs& a, int row, in
 
 // WHOLE: pages hold a multiple of 16 tokens, so that a step's tokens lie in one
 template <class T, int DP, bool CODED, int NR, bool WHOLE>
-__global__ void __launch_bounds__(kCacheFewThreads, (CacheFewShape<DP, CODED, NR>::kBlocks)) cache_attention_few(const __grid_constant__ CacheAttnArgs a,
+__global__ void __launch_bounds__(kCacheFewThreads, (CacheFewShape<DP, CODED, NR>::kBlocks)) cache_attention_few(const __grid_constant__ b200_tmap map_k,
+                                                                                                               const __grid_constant__ b200_tmap map_v,
+                                                                                                               const __grid_constant__ CacheAttnArgs a,
                                                                                                                const __grid_constant__ CacheFewArgs f) {
   typedef CacheFewShape<DP, CODED, NR> Sh;
   typedef typename std::conditional<CODED, __half, T>::type M;          // what is multiplied
@@ -334,9 +333,20 @@ __global__ void __launch_bounds__(kCacheFewThreads, (CacheFewShape<DP, CODED, NR
   constexpr float kUp = kLift<M>;
   extern __shared__ __align__(128) unsigned char dyn[];
   __shared__ unsigned int last_block;
+  __shared__ unsigned long long arrived[kCacheFewWarps][Sh::kStages];
+  __shared__ volatile unsigned int abort_flag;
   const CacheArgs& c = a.c;
   const unsigned int warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, q4 = lane & 3u;
+  const unsigned int dyn_at = (b200_smem_addr(dyn) + 1023u) & ~1023u, bars = b200_smem_addr(arrived[warp]);
+  unsigned char* const gen = dyn + (dyn_at - b200_smem_addr(dyn));
+  if constexpr (WHOLE) {
+    if (lane < (unsigned int)Sh::kStages) b200_mbar_init(bars + 8 * lane, 1);
+    if (threadIdx.x == 0) abort_flag = 0u;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    __syncthreads();
+  }
   grid_begin();
+  unsigned int filled = 0, taken = 0;                  // steps that this warp has asked for, and used
 
   CachePart part;
   if (!cache_part<kCacheFewThreads, R>(a, f, part)) return;
@@ -350,7 +360,7 @@ __global__ void __launch_bounds__(kCacheFewThreads, (CacheFewShape<DP, CODED, NR
   const int all_see = cache_last(a, plan.least_pos), all_from = cache_first(a, plan.most_pos);
 
   // ---- the ring: steps of 16 tokens, every fourth of them this warp's
-  const unsigned int ring = b200_smem_addr(dyn) + warp * Sh::kRing;
+  const unsigned int ring = dyn_at + warp * Sh::kRing;
   const int steps = v_end > v_begin ? (v_end - v_begin + 15) / 16 : 0;
   const int mine = steps > (int)warp ? (steps - (int)warp + kCacheFewWarps - 1) / kCacheFewWarps : 0;
   auto token_of = [&](int n) { return plan.token_of(v_begin + ((int)warp + n * kCacheFewWarps) * 16); };
@@ -361,9 +371,8 @@ __global__ void __launch_bounds__(kCacheFewThreads, (CacheFewShape<DP, CODED, NR
   // bytes that this lane takes at its keys' and its values' pieces (none behind the head's end)
   auto key_bytes = [&](int p) { return (int)q4 * 16 + p * 64 < line ? 16 : 0; };
   auto value_bytes = [&](int p) { return (int)g * Sh::kValueBytes + p * 16 < line ? Sh::kValueWidth : 0; };
-  const int key_at = (int)g * line + (int)q4 * 16, value_at = (int)q4 * 2 * line + (int)g * Sh::kValueBytes;
-  // WHOLE: where 32 steps lie, a lane each (bytes; -1: not there), and their pages' scales; and the same of the 32 steps behind them
-  long long where[2] = {-1, -1};
+  // WHOLE: the pages of 32 steps, a lane each (-1: none), their slots there, and their pages' scales; and the same of the 32 steps behind them
+  int where[2] = {-1, -1}, slots[2] = {0, 0};
   struct Scales {
     float down, back, raise;                         // of the keys; of the values its inverse and its logarithm
     __device__ __forceinline__ void of(const CacheArgs& c, long long at) {
@@ -380,57 +389,34 @@ __global__ void __launch_bounds__(kCacheFewThreads, (CacheFewShape<DP, CODED, NR
     const int j = token_of(n);
     const unsigned int index = c.by_page.of((unsigned int)j);
     const int page = cache_page_at(c, b, index);
-    if (page < 0) return;
-    where[k] = (cache_at(c, page, hk) + (long long)((unsigned int)j - index * c.page) * c.D) * kSize;
-    if constexpr (CODED) scales[k].of(c, (long long)page * c.HK + hk);
+    where[k] = page;
+    slots[k] = (int)((unsigned int)j - index * c.page);
+    if (CODED && page >= 0) scales[k].of(c, (long long)page * c.HK + hk);
   };
   if (WHOLE) {
     look(0, 0);
     if (mine > 32) look(32, 1);
   }
-  unsigned int to = 0;                               // the slot that is filled next
   int first_of = 0;                                  // the step that where[0] begins with
   auto fetch = [&](int n) {
     if (n < mine) {
-      const int j0 = token_of(n);
-      const unsigned int at_k = ring + to * Sh::kStage + lane * 16, at_v = ring + to * Sh::kStage + Sh::kKeys + lane * Sh::kValueWidth;
-      if (WHOLE) {
-        const long long from0 = __shfl_sync(0xffffffffu, n - first_of < 32 ? where[0] : where[1], n & 31), from = max(from0, 0ll);
-        const int left = from0 >= 0 ? end - j0 : 0;  // tokens of the step that are there
-        const unsigned char *const k0 = keys + from + key_at, *const v0 = values + from + value_at;
-        if (left >= 16 && c.D == DP) {
-          // (all but a tile's last step, of heads that fill their pieces: places known beforehand)
-          constexpr int kLine = DP * kSize;
+      const unsigned int to = filled++ % Sh::kStages;
+      if constexpr (WHOLE) {
+        const bool near = n - first_of < 32;
+        const int page = __shfl_sync(0xffffffffu, near ? where[0] : where[1], n & 31), at = __shfl_sync(0xffffffffu, near ? slots[0] : slots[1], n & 31);
+        if (b200_elect()) {
+          const unsigned int bar = bars + 8 * to, dst = ring + to * Sh::kStage;
+          b200_mbar_expect_tx(bar, Sh::kStage);
+          // (no page: a box outside the cache, zeros)
 #pragma unroll
-          for (int k = 0; k < 2; ++k)
-#pragma unroll
-            for (int p = 0; p < Sh::kPerKey; ++p) copy_whole<16>(at_k + (k * Sh::kPerKey + p) * 512, k0 + k * 8 * kLine + p * 64);
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-#pragma unroll
-            for (int p = 0; p < Sh::kPerValue; ++p)
-              copy_whole<Sh::kValueWidth>(at_v + (k * Sh::kPerValue + p) * 32 * Sh::kValueWidth, v0 + ((k & 1) + 8 * (k >> 1)) * kLine + p * 16);
-        } else {
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const bool on = (int)g + 8 * k < left;
-#pragma unroll
-            for (int p = 0; p < Sh::kPerKey; ++p) {
-              const int bytes = on ? key_bytes(p) : 0;
-              copy_in<16>(at_k + (k * Sh::kPerKey + p) * 512, bytes ? k0 + k * 8 * line + p * 64 : keys, bytes);
-            }
-          }
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const bool on = (int)q4 * 2 + (k & 1) + 8 * (k >> 1) < left;
-#pragma unroll
-            for (int p = 0; p < Sh::kPerValue; ++p) {
-              const int bytes = on ? value_bytes(p) : 0;
-              copy_in<Sh::kValueWidth>(at_v + (k * Sh::kPerValue + p) * 32 * Sh::kValueWidth, bytes ? v0 + ((k & 1) + 8 * (k >> 1)) * line + p * 16 : values, bytes);
-            }
+          for (int p = 0; p < Sh::kPanels; ++p) {
+            b200_tma_load_4d(dst + p * 16 * Sh::kLine, &map_k, bar, p * 64, at, hk, page < 0 ? (int)c.n_pages : page);
+            b200_tma_load_4d(dst + Sh::kKeys + p * 16 * Sh::kLine, &map_v, bar, p * 64, at, hk, page < 0 ? (int)c.n_pages : page);
           }
         }
       } else {
+        const int j0 = token_of(n);
+        const unsigned int at_k = ring + to * Sh::kStage + lane * 16, at_v = ring + to * Sh::kStage + Sh::kKeys + lane * Sh::kValueWidth;
         // byte of a token's row, -1: not there
         auto place = [&](int j) -> long long {
           if (j >= end) return -1;
@@ -457,9 +443,8 @@ __global__ void __launch_bounds__(kCacheFewThreads, (CacheFewShape<DP, CODED, NR
           }
         }
       }
-      to = to + 1 == Sh::kStages ? 0 : to + 1;
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
+    if (!WHOLE) asm volatile("cp.async.commit_group;" ::: "memory");
   };
 #pragma unroll
   for (int i = 0; i < Sh::kStages - 1; ++i) fetch(i);
@@ -547,13 +532,19 @@ __global__ void __launch_bounds__(kCacheFewThreads, (CacheFewShape<DP, CODED, NR
     }
   };
   if (!WHOLE) look_at(0);
-  unsigned int slot = 0;
-  for (int n = 0; n < mine; ++n) {
+  // where a lane's pieces lie in a stage: boxes swizzled by the copies, or a piece of all lanes behind the other
+  auto box_at = [&](unsigned int row, unsigned int byte) {
+    const unsigned int chunk = byte % Sh::kLine / 16, turn = Sh::kLine == 128 ? row & 7u : row >> 1 & 3u;
+    return byte / Sh::kLine * (16 * Sh::kLine) + row * Sh::kLine + ((chunk ^ turn) << 4) + byte % 16;
+  };
+  bool live = true;
+  for (int n = 0; n < mine && live; ++n) {
     const int j0 = token_of(n);
     if (WHOLE && n - first_of == 32) {
       // (copies are at most a few steps ahead: in the second 32)
       first_of = n;
       where[0] = where[1];
+      slots[0] = slots[1];
       scales[0] = scales[1];
       if (mine - n > 32) look(n + 32, 1);
     }
@@ -573,10 +564,16 @@ __global__ void __launch_bounds__(kCacheFewThreads, (CacheFewShape<DP, CODED, NR
       }
     }
     if (!WHOLE) look_at(n + 1);
-    asm volatile("cp.async.wait_group %0;" ::"n"(Sh::kStages - 2) : "memory");
-    fetch(n + Sh::kStages - 1);       // into the slot of the step before, which this lane alone reads
-    const unsigned int at_k = ring + slot * Sh::kStage + lane * 16, at_v = ring + slot * Sh::kStage + Sh::kKeys + lane * Sh::kValueWidth;
-    slot = slot + 1 == Sh::kStages ? 0 : slot + 1;
+    const unsigned int slot = taken % Sh::kStages, stage = ring + slot * Sh::kStage;
+    if constexpr (WHOLE) {
+      live = b200_wait(bars + 8 * slot, taken / Sh::kStages & 1u, &abort_flag, a.status, 81u);
+      live = __all_sync(0xffffffffu, live);         // (and all lanes have read the step before)
+    } else {
+      asm volatile("cp.async.wait_group %0;" ::"n"(Sh::kStages - 2) : "memory");
+    }
+    ++taken;
+    if (live) fetch(n + Sh::kStages - 1);           // into the slot of the step before
+    if (!live) break;
     if (WHOLE && !here[0]) continue;
     // scores of tokens g (x[.][0, 1]) and g + 8 ([2, 3])
     float x[NR][4];
@@ -586,7 +583,8 @@ __global__ void __launch_bounds__(kCacheFewThreads, (CacheFewShape<DP, CODED, NR
       for (int k = 0; k < 4; ++k) x[r][k] = 0.f;
 #pragma unroll
     for (int p = 0; p < Sh::kPerKey; ++p) {
-      const uint4 u = from_shared16(at_k + p * 512), w = from_shared16(at_k + (Sh::kPerKey + p) * 512);
+      const uint4 u = from_shared16(stage + (WHOLE ? box_at(g, q4 * 16 + p * 64) : p * 512 + lane * 16)),
+                  w = from_shared16(stage + (WHOLE ? box_at(g + 8, q4 * 16 + p * 64) : (Sh::kPerKey + p) * 512 + lane * 16));
       const unsigned int uu[4] = {u.x, u.y, u.z, u.w}, ww[4] = {w.x, w.y, w.z, w.w};
       if constexpr (CODED) {
 #pragma unroll
@@ -606,6 +604,7 @@ __global__ void __launch_bounds__(kCacheFewThreads, (CacheFewShape<DP, CODED, NR
         }
       }
     }
+    const bool beyond = j0 + 15 >= end;
     const bool some_hidden = !WHOLE || j0 + 15 > all_see || (a.window && j0 < all_from && j0 + 15 >= a.sinks);
     bool grows = false;
     float top[NR][2];
@@ -681,7 +680,8 @@ __global__ void __launch_bounds__(kCacheFewThreads, (CacheFewShape<DP, CODED, NR
       unsigned int y[4][4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const unsigned int from = at_v + (k * Sh::kPerValue + piece) * 32 * Sh::kValueWidth;
+        const unsigned int token = q4 * 2 + (k & 1) + 8 * (k >> 1);
+        const unsigned int from = stage + Sh::kKeys + (WHOLE ? box_at(token, g * Sh::kValueBytes + piece * 16) : (k * Sh::kPerValue + piece) * 32 * Sh::kValueWidth + lane * Sh::kValueWidth);
         if constexpr (kWords == 4) {
           const uint4 v = from_shared16(from);
           y[k][0] = v.x; y[k][1] = v.y; y[k][2] = v.z; y[k][3] = v.w;
@@ -689,6 +689,10 @@ __global__ void __launch_bounds__(kCacheFewThreads, (CacheFewShape<DP, CODED, NR
           const uint2 v = from_shared8(from);
           y[k][0] = v.x; y[k][1] = v.y;
         }
+        // (a box has its page's slots behind the last token too)
+        if (WHOLE && beyond)
+#pragma unroll
+          for (int i = 0; i < kWords; ++i) y[k][i] = j0 + (int)token < end ? y[k][i] : 0u;
       }
 #pragma unroll
       for (int i = 0; i < kWords; ++i) {
@@ -714,7 +718,14 @@ __global__ void __launch_bounds__(kCacheFewThreads, (CacheFewShape<DP, CODED, NR
       }
     }
   }
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  if constexpr (WHOLE) {
+    // (after a wait that gave up, what is under way lands before shared memory has another use)
+    if (!live)
+      for (; taken != filled; ++taken)
+        for (int tries = 0; tries < 1 << 20 && !b200_mbar_try(bars + 8 * (taken % Sh::kStages), taken / Sh::kStages & 1u); ++tries) {}
+  } else {
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+  }
 #pragma unroll
   for (int r = 0; r < NR; ++r)
 #pragma unroll
@@ -722,7 +733,7 @@ __global__ void __launch_bounds__(kCacheFewThreads, (CacheFewShape<DP, CODED, NR
 #pragma unroll
       for (int d = 4; d < 32; d <<= 1) l[r][k] += __shfl_xor_sync(0xffffffffu, l[r][k], d);
   __syncthreads();                    // the rings become the place where the warps meet
-  float* join = (float*)dyn;
+  float* join = (float*)gen;
 #pragma unroll
   for (int r = 0; r < NR; ++r)
 #pragma unroll
@@ -781,6 +792,7 @@ __global__ void __launch_bounds__(kCacheFewThreads, (CacheFewShape<DP, CODED, NR
       if (attn_again(fine)) cache_attention_row<T, CODED>(a, b, head_of(i), s.first + query_of(i), s.pos0 + query_of(i), lane);
     }
   }
+  if constexpr (WHOLE) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   __syncthreads();                    // (the rings, and what lies where they were, are written again)
   }
 }

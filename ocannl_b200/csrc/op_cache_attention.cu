@@ -13,15 +13,15 @@ using namespace b200;
 namespace {
 
 typedef void (*AnyKernel)(const CacheAttnArgs, const CacheFewArgs, int);
-typedef void (*FewKernel)(const CacheAttnArgs, const CacheFewArgs);
+typedef void (*FewKernel)(const b200_tmap, const b200_tmap, const CacheAttnArgs, const CacheFewArgs);
 
-// [dims[3]][dims[2]][dims[1]][dims[0]] elements in boxes of box[0] x box[1] x 1 x box[3]; 16-bit ones swizzled as the tensor cores read them
-b200_tmap box_map(const void* p, CUtensorMapDataType type, int size, const cuuint64_t (&dims)[4], const cuuint32_t (&box)[4]) {
+// [dims[3]][dims[2]][dims[1]][dims[0]] elements in boxes of box[0] x box[1] x 1 x box[3]
+b200_tmap box_map(const void* p, CUtensorMapDataType type, int size, const cuuint64_t (&dims)[4], const cuuint32_t (&box)[4], CUtensorMapSwizzle swizzle) {
   CUtensorMap map;
   const cuuint64_t strides[3] = {dims[0] * size, dims[0] * dims[1] * size, dims[0] * dims[1] * dims[2] * size};
   const cuuint32_t estr[4] = {1, 1, 1, 1};
   const CUresult r = cu().cuTensorMapEncodeTiled_(&map, type, 4, (void*)p, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                                                  size == 1 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                                                  swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) throw Error(B200_E_UNSUPPORTED, "cache_attention: a node's layout cannot be described to the TMA unit (CUresult " + std::to_string((int)r) + ")");
   static_assert(sizeof(b200_tmap) == sizeof(CUtensorMap), "tensor map");
   b200_tmap m;
@@ -49,11 +49,11 @@ struct CacheAttnOperator : b200_operator {
   template <class T, int DP, bool CODED, int NR>
   void set_few() {
     typedef CacheFewShape<DP, CODED, NR> Sh;
-    few = a.c.page % 16 == 0 ? cache_attention_few<T, DP, CODED, NR, true> : cache_attention_few<T, DP, CODED, NR, false>;
+    few = a.c.page % 16 == 0 && a.c.n_pages ? cache_attention_few<T, DP, CODED, NR, true> : cache_attention_few<T, DP, CODED, NR, false>;
     smem = Sh::smem();
     tile = Sh::kRows;
     width = Sh::kWidth;
-    resident = std::min<int>(Sh::kBlocks, 226 * 1024 / (Sh::smem() + 6 * 1024));
+    resident = std::min<int>(Sh::kBlocks, 227 * 1024 / (Sh::smem() + 6 * 1024));
   }
   template <class T, int DP>
   void set_few(bool wide) {
@@ -138,12 +138,19 @@ struct CacheAttnOperator : b200_operator {
     const bool two = !tile_args.sums && (long long)c.tokens / (2 * tile_args.tokens) * c.HK >= dev->sm_count;
     tiles = cache_tiles(dtype, coded, c.D > 64, two);
     grid = blocks_of(blocks(two ? 2 : 1));
-    const CUtensorMapDataType type = dtype == B200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    const cuuint64_t of_q[4] = {(cuuint64_t)c.D, (cuuint64_t)a.group, (cuuint64_t)c.HK, (cuuint64_t)c.tokens}, of_c[4] = {(cuuint64_t)c.D, c.page, (cuuint64_t)c.HK, c.n_pages};
-    const cuuint32_t box_q[4] = {64, (cuuint32_t)a.group, 1, (cuuint32_t)tile_args.tokens}, box_c[4] = {coded ? (c.D > 64 ? 128u : 64u) : 64u, (cuuint32_t)tile_args.box, 1, 1};
-    map_q = box_map(a.q, type, 2, of_q, box_q);
-    map_k = box_map(c.k, coded ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : type, coded ? 1 : 2, of_c, box_c);
-    map_v = box_map(c.v, coded ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : type, coded ? 1 : 2, of_c, box_c);
+    const cuuint64_t of_q[4] = {(cuuint64_t)c.D, (cuuint64_t)a.group, (cuuint64_t)c.HK, (cuuint64_t)c.tokens};
+    const cuuint32_t box_q[4] = {64, (cuuint32_t)a.group, 1, (cuuint32_t)tile_args.tokens};
+    map_q = box_map(a.q, type(), 2, of_q, box_q, CU_TENSOR_MAP_SWIZZLE_128B);
+    // (codes are made halves where they lie: rows one behind the other)
+    cache_maps(tile_args.box, coded ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B);
+  }
+  CUtensorMapDataType type() const { return dtype == B200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16; }
+  void cache_maps(int rows, CUtensorMapSwizzle swizzle) {
+    const CacheArgs& c = a.c;
+    const cuuint64_t of_c[4] = {(cuuint64_t)c.D, c.page, (cuuint64_t)c.HK, c.n_pages};
+    const cuuint32_t box_c[4] = {coded && c.D > 64 ? 128u : 64u, (cuuint32_t)rows, 1, 1};
+    map_k = box_map(c.k, coded ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : type(), coded ? 1 : 2, of_c, box_c, swizzle);
+    map_v = box_map(c.v, coded ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : type(), coded ? 1 : 2, of_c, box_c, swizzle);
   }
   void choose_few() {
     const CacheArgs& c = a.c;
@@ -152,12 +159,14 @@ struct CacheAttnOperator : b200_operator {
     if (dtype == B200_BF16) c.D <= 64 ? set_few<__nv_bfloat16, 64>(wide) : set_few<__nv_bfloat16, 128>(wide);
     else c.D <= 64 ? set_few<__half, 64>(wide) : set_few<__half, 128>(wide);
     choose_parts(tile, width, resident, 4);
+    // (one box a step; codes of heads of up to 64 elements have rows of 64 bytes)
+    if (c.page % 16 == 0 && c.n_pages) cache_maps(16, coded && c.D <= 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
     ready(few, smem);
   }
   void run(cudaStream_t s) override {
     if (!grid) return;
     if (tiles.kernel) launch(tiles.kernel, dim3(grid), tiles.threads, tiles.smem, s, map_q, map_k, map_v, a, tile_args);
-    else if (few) launch(few, dim3(grid), kCacheFewThreads, smem, s, a, few_args);
+    else if (few) launch(few, dim3(grid), kCacheFewThreads, smem, s, map_k, map_v, a, few_args);
     else launch(any, dim3(grid), kCacheFewThreads, smem, s, a, few_args, vec);
   }
 };
