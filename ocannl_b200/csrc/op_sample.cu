@@ -48,8 +48,8 @@ struct Share {                         // of a block, for the others of its clus
   unsigned int listed;                 // entries of the list (more than it holds: it is of no use)
   unsigned int joined;                 // of the first block: entries of the list that all blocks' go to
   unsigned int joined_from;            // where this block's begin there
-  double sums[kBins];
-  unsigned int counts[kBins];
+  double sums[2][kBins];               // of one histogram and the next
+  unsigned int counts[2][kBins];
   double warp_sums[kWarps];
   unsigned int warp_counts[kWarps];
   float largest;
@@ -206,8 +206,37 @@ __device__ __forceinline__ double block_before(double v, double* scratch, double
   return before;
 }
 
-// Rising, n of at most kList entries.  A thread has four neighbours: pairs of a bitonic network lie in it, in its warp, or, 128 entries and more apart, in shared memory.
+// Rising, n of at most kThreads entries, one a thread: pairs of a bitonic network lie in a warp, or, 32 entries and more apart, in shared memory.
+__device__ __forceinline__ void sort_few(unsigned long long* list, unsigned int n) {
+  const unsigned int n2 = n <= 2 ? 2u : 1u << (32 - __clz((int)n - 1)), i = threadIdx.x;
+  __syncthreads();
+  unsigned long long r = i < n ? list[i] : ~0ull;
+  // (a warp behind the last power of two has nothing to do but to come to the barriers)
+  for (unsigned int size = 2; size <= n2; size <<= 1)
+    for (unsigned int step = size >> 1; step; step >>= 1) {
+      unsigned long long p;
+      if (step >= 32) {
+        __syncthreads();
+        list[i] = r;
+        __syncthreads();
+        p = list[i ^ step];
+      } else {
+        if ((threadIdx.x & ~31u) >= n2) continue;
+        p = __shfl_xor_sync(0xffffffffu, r, step);
+      }
+      const bool least = ((i & size) == 0) == ((i & step) == 0);
+      r = (p < r) == least ? p : r;
+    }
+  __syncthreads();
+  if (i < n) list[i] = r;
+  __syncthreads();
+}
+// Rising, n of at most kList entries.  A thread has four neighbours: pairs lie in it, in its warp, or, 128 entries and more apart, in shared memory.
 __device__ __forceinline__ void sort_list(unsigned long long* list, unsigned int n) {
+  if (n <= (unsigned int)kThreads) {
+    sort_few(list, n);
+    return;
+  }
   static_assert(kList == 4 * kThreads, "four entries a thread");
   const unsigned int n2 = n <= 2 ? 2u : 1u << (32 - __clz((int)n - 1)), i0 = threadIdx.x * 4;
   unsigned long long r[4];
@@ -236,7 +265,6 @@ __device__ __forceinline__ void sort_list(unsigned long long* list, unsigned int
         const bool least = (((i0 + k) & size) == 0) == (((i0 + k) & step) == 0);
         r[k] = (p[k] < r[k]) == least ? p[k] : r[k];
       }
-      if (n2 <= 128 && threadIdx.x >= 32) break;
     }
   __syncthreads();
 #pragma unroll
@@ -329,8 +357,10 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
   // the list that all blocks' entries go to, in the first one: where the histogram was
   unsigned long long* const all_list = E > 0 ? sh.list : (unsigned long long*)bins;
 
+  unsigned int histograms = 0;
   // a histogram of the kept logits that `over` passes on and `of` gives a bin (0: the highest); bins of all blocks, joined, in sh
   auto histogram = [&](auto over, auto of) {
+    const unsigned int set = histograms++ & 1u;
     for (unsigned int i = threadIdx.x; i < kWarps * kBins * 32 / 2; i += kThreads) ((uint4*)bins)[i] = make_uint4(0u, 0u, 0u, 0u);
     __syncthreads();
     uint2* mine = bins + warp * kBins * 32 + lane;
@@ -367,8 +397,8 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
         n += __shfl_xor_sync(0xffffffffu, n, o);
       }
       if (w == 0) {
-        sh.sums[b] = s;
-        sh.counts[b] = n;
+        sh.sums[set][b] = s;
+        sh.counts[set][b] = n;
       }
     }
     meet(parts);
@@ -378,8 +408,8 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
 #pragma unroll
       for (unsigned int p = 0; p < kMostParts; ++p) {
         const Share* o = of_part(&sh, parts, p < parts ? p : 0);
-        of[p] = p < parts ? o->sums[threadIdx.x] : 0.0;
-        in[p] = p < parts ? o->counts[threadIdx.x] : 0u;
+        of[p] = p < parts ? o->sums[set][threadIdx.x] : 0.0;
+        in[p] = p < parts ? o->counts[set][threadIdx.x] : 0u;
       }
 #pragma unroll
       for (unsigned int p = 0; p < kMostParts; ++p) {
@@ -389,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
       sh.joined_sums[threadIdx.x] = s;
       sh.joined_counts[threadIdx.x] = n;
     }
-    meet(parts);                       // (the shares are written again)
+    __syncthreads();                   // (this set of shares is written again two histograms on, with a meeting between)
   };
   auto whole_row = [&](auto f) { logits.each(f); };
   // the count and the sum of all bins: a warp, a lane a bin
