@@ -476,15 +476,26 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
     Share* first = of_part(&sh, parts, 0);
     unsigned long long* to = parts > 1 ? cg::this_cluster().map_shared_rank(all_list, 0) : all_list;
     const unsigned int n = min(sh.listed, (unsigned int)kList);
-    for (unsigned int k0 = 0; k0 < n; k0 += kThreads) {
-      const unsigned int k = k0 + threadIdx.x;
-      const bool on = k < n && of(of_key(~(unsigned int)(sh.list[k] >> 32)));
-      const unsigned int votes = __ballot_sync(0xffffffffu, on);
-      unsigned int at = 0;
-      if (lane == 0 && votes) at = atomicAdd(&first->joined, (unsigned int)__popc((int)votes));
-      at = __shfl_sync(0xffffffffu, at, 0) + (unsigned int)__popc((int)(votes & ((1u << lane) - 1u)));
-      if (on && at < kList) to[at] = sh.list[k];
+    // (a place in another block's list is some 1500 cycles away: one question a warp)
+    unsigned long long mine[kList / kThreads];
+    unsigned int many = 0;
+#pragma unroll
+    for (int k = 0; k < kList / kThreads; ++k) {
+      const unsigned int i = threadIdx.x + k * kThreads;
+      mine[k] = i < n ? sh.list[i] : ~0ull;
+      if (i < n && !of(of_key(~(unsigned int)(mine[k] >> 32)))) mine[k] = ~0ull;
+      many += mine[k] != ~0ull;
     }
+    const unsigned int up_to = warp_up_to(many);
+    unsigned int at = 0;
+    if (lane == 31 && up_to) at = atomicAdd(&first->joined, up_to);
+    at = __shfl_sync(0xffffffffu, at, 31) + up_to - many;
+#pragma unroll
+    for (int k = 0; k < kList / kThreads; ++k)
+      if (mine[k] != ~0ull) {
+        if (at < kList) to[at] = mine[k];
+        ++at;
+      }
     meet(parts);
   };
   auto logit_of = [&](unsigned long long entry) { return of_key(~(unsigned int)(entry >> 32)); };
