@@ -200,10 +200,13 @@ def attention(q, k_cache, v_cache, table, lengths, starts, page, prec, k_scale=N
                 k, v = decode(k) * k_scale[p, g][:, None], decode(v)
             k, v = np.where(used[:, None], k, 0.0), np.where(used[:, None], v, 0.0)
             # (rows below the largest weight of a half: sizes of all values that a row sees)
-            flat = seen @ np.abs(v)
+            fine = np.where(np.isfinite(v), v, 0.0)
+            odd = np.flatnonzero(~np.isfinite(v).all(1))       # (added below, for the rows that see them)
+            flat = seen @ np.abs(fine)
             if coded:
                 flat = flat * np.where(seen, v_scale[p, g], 0.0).max(1, initial=0.0)[:, None]
-                v = v * np.where(used, v_scale[p, g], 0.0)[:, None]
+                by = np.where(used, v_scale[p, g], 0.0)[:, None]
+                v, fine = v * by, fine * by
             for hh in range(g * (h // hk), (g + 1) * (h // hk)):
                 with np.errstate(all="ignore"):
                     z = q[rows, hh] @ k.T * scale
@@ -211,11 +214,14 @@ def attention(q, k_cache, v_cache, table, lengths, starts, page, prec, k_scale=N
                     z = z - (0.0 if slopes is None else slopes[hh]) * (pos - j)
                     z = np.where(seen, z, -np.inf)
                     top = z.max(1, initial=-np.inf, keepdims=True)
-                    e = np.where(seen, np.exp(z - np.where(np.isinf(top), 0.0, top)), 0.0)
+                    e = np.where(seen, np.exp(z - np.where(np.isneginf(top), 0.0, top)), 0.0)
                     total = e.sum(1, keepdims=True)
                     w = e / np.where(total == 0.0, 1.0, total)
-                    out[rows, hh], lse[rows, hh] = w @ v, (top + np.log(total))[:, 0]
-                size = w @ np.abs(v)
+                    out[rows, hh], lse[rows, hh] = w @ fine, (top + np.log(total))[:, 0]
+                    for i in odd:
+                        at = np.flatnonzero(seen[:, i])
+                        out[rows[at], hh] += w[at, i][:, None] * np.where(np.isfinite(v[i]), 0.0, v[i])
+                size = w @ np.abs(fine)
                 off[rows, hh] = half * np.abs(out[rows, hh]) + (of_weights + ARITH) * size + (2.0 ** -25 * (flat + 1) if prec == "half" or (coded and prec != "single") else 1e-30)
                 lse_off[rows, hh] = np.where(np.isfinite(lse[rows, hh]), ARITH * (1 + np.abs(np.where(np.isfinite(lse[rows, hh]), lse[rows, hh], 0.0))), 0.0)
     return out, lse, off, lse_off
