@@ -29,11 +29,13 @@ struct CacheFewArgs {
   unsigned int* tickets;   // [block], zero between runs: of the tile that begins in a block and ends in another
   unsigned int blocks;     // that fill the machine
   unsigned int least;      // 64s of tokens of a block at least
+  unsigned int enough;     // tiles that need not be cut for the machine to be busy
   int single;              // a tile a block, whatever the lengths
   Divisor by_group, by_key_heads, by_units;     // by_units: without starts, tiles of a sequence (single)
 };
 
 constexpr int kCacheFewWarps = 4, kCacheFewThreads = 32 * kCacheFewWarps;
+constexpr unsigned int kCacheShort = 24;      // 64s of tokens of tiles that are not cut, on average
 constexpr unsigned int kCachePart = 1024;     // 64s of tokens of a block at most, a quarter of them a warp's: its accumulators' cut-off sums lose 2^-13 (see kSumKeys)
 
 template <int DP, bool CODED, int NR>
@@ -97,6 +99,7 @@ struct CachePart {
   unsigned long long ahead, quota;     // of the sequence: 64s of the sequences before it; a block's part
   CacheSeq s;
   CacheWalk walk;
+  bool whole;                          // no tile is cut: a walk of tiles, each of length 1
 };
 // A piece of a tile: which rows of a key head, and which of the tokens that they see.
 struct CachePiece {
@@ -109,6 +112,11 @@ struct CachePiece {
 };
 // a part's place: of the tile that begins in `first_block`
 __device__ __forceinline__ long long cache_part_at(unsigned int first_block, unsigned int part) { return ((long long)first_block + part) * 2 + (part == 0 ? 1 : 0); }
+
+// (64-bit quotients take some 100 instructions, and walks are hardly ever that long)
+__device__ __forceinline__ unsigned long long quotient(unsigned long long n, unsigned long long d) {
+  return (n | d) >> 32 ? n / d : (unsigned long long)((unsigned int)n / (unsigned int)d);
+}
 
 template <int NT, int ROWS>
 __device__ __forceinline__ bool cache_part(const CacheAttnArgs& a, const CacheFewArgs& f, CachePart& p) {
@@ -128,38 +136,58 @@ __device__ __forceinline__ bool cache_part(const CacheAttnArgs& a, const CacheFe
     p.at = 0;
     p.left = p.walk.length;
     p.ahead = p.quota = 0;
+    p.whole = false;
     return true;
   }
-  __shared__ unsigned long long sums[NT / 32], found[2];
+  __shared__ unsigned long long sums[2][NT / 32], found[2];
   const unsigned int lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
-  auto length_of = [&](int i) -> unsigned long long {
-    if (i >= c.batch) return 0ull;
-    const CacheSeq s = cache_seq(c, i);
-    if (!s.count) return 0ull;
-    const CacheWalk w = cache_walk<ROWS>(a, s);
-    return (unsigned long long)w.tiles * w.length;
-  };
-  // the whole walk; with a sequence a thread, one look at the lengths finds the block's own place as well
-  unsigned long long all = 0, mine = 0, before = 0;
-  for (int i0 = 0; i0 < c.batch; i0 += NT) {
-    mine = length_of(i0 + (int)threadIdx.x);
-    unsigned long long up_to = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const unsigned long long x = __shfl_up_sync(0xffffffffu, up_to, o);
-      if (lane >= (unsigned int)o) up_to += x;
+  // of NT sequences from i0 on: 64s and tiles, this thread's, those before it, and added to all
+  auto sums_of = [&](int i0, unsigned long long& all, unsigned long long& tiles, unsigned long long& mine, unsigned long long& mine_tiles, unsigned long long& before,
+                     unsigned long long& before_tiles) {
+    const int i = i0 + (int)threadIdx.x;
+    mine = mine_tiles = 0;
+    if (i < c.batch) {
+      const CacheSeq s = cache_seq(c, i);
+      if (s.count) {
+        const CacheWalk w = cache_walk<ROWS>(a, s);
+        mine_tiles = w.tiles;
+        mine = mine_tiles * w.length;
+      }
     }
+    unsigned long long up_to[2] = {mine, mine_tiles};
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned long long x = __shfl_up_sync(0xffffffffu, up_to[k], o);
+        if (lane >= (unsigned int)o) up_to[k] += x;
+      }
     __syncthreads();
-    if (lane == 31) sums[warp] = up_to;
+    if (lane == 31) sums[0][warp] = up_to[0], sums[1][warp] = up_to[1];
     __syncthreads();
-    before = all + up_to - mine;
+    before = all + up_to[0] - mine;
+    before_tiles = tiles + up_to[1] - mine_tiles;
 #pragma unroll
     for (int w = 0; w < NT / 32; ++w) {
-      if (w < (int)warp) before += sums[w];
-      all += sums[w];
+      if (w < (int)warp) before += sums[0][w], before_tiles += sums[1][w];
+      all += sums[0][w];
+      tiles += sums[1][w];
     }
+  };
+  // the whole walk, and its tiles; with a sequence a thread, one look at the lengths finds the block's own place as well
+  unsigned long long all = 0, tiles = 0, mine = 0, mine_tiles = 0, before = 0, before_tiles = 0;
+  for (int i0 = 0; i0 < c.batch; i0 += NT) {
+    sums_of(i0, all, tiles, mine, mine_tiles, before, before_tiles);
   }
-  p.quota = min(max((all + f.blocks - 1) / f.blocks, (unsigned long long)f.least), (unsigned long long)kCachePart);
+  // Short tiles, and enough of them for the machine: none is cut (32 sequences of 8 key heads, 1044 tokens each: 25.8 us, 27.2 cut).
+  p.whole = tiles >= f.enough && all <= tiles * kCacheShort;
+  if (p.whole) {
+    all = tiles;
+    mine = mine_tiles;
+    before = before_tiles;
+  }
+  p.quota = quotient(all + f.blocks - 1, f.blocks);
+  if (!p.whole) p.quota = min(max(p.quota, (unsigned long long)f.least), (unsigned long long)kCachePart);
   const unsigned long long from = p.quota * blockIdx.x;
   if (from >= all) return false;
   if (c.batch <= NT) {
@@ -168,23 +196,12 @@ __device__ __forceinline__ bool cache_part(const CacheAttnArgs& a, const CacheFe
       found[1] = before;
     }
   } else {
-    unsigned long long sum = 0;
+    unsigned long long sum = 0, sum_tiles = 0;
     for (int i0 = 0; i0 < c.batch; i0 += NT) {
-      mine = length_of(i0 + (int)threadIdx.x);
-      unsigned long long up_to = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const unsigned long long x = __shfl_up_sync(0xffffffffu, up_to, o);
-        if (lane >= (unsigned int)o) up_to += x;
-      }
-      __syncthreads();
-      if (lane == 31) sums[warp] = up_to;
-      __syncthreads();
-      before = sum + up_to - mine;
-#pragma unroll
-      for (int w = 0; w < NT / 32; ++w) {
-        if (w < (int)warp) before += sums[w];
-        sum += sums[w];
+      sums_of(i0, sum, sum_tiles, mine, mine_tiles, before, before_tiles);
+      if (p.whole) {
+        mine = mine_tiles;
+        before = before_tiles;
       }
       if (before <= from && from < before + mine) {
         found[0] = (unsigned long long)(i0 + (int)threadIdx.x);
@@ -197,8 +214,9 @@ __device__ __forceinline__ bool cache_part(const CacheAttnArgs& a, const CacheFe
   p.ahead = found[1];
   p.s = cache_seq(c, p.b);
   p.walk = cache_walk<ROWS>(a, p.s);
+  if (p.whole) p.walk.length = 1;
   const unsigned long long rest = from - p.ahead;
-  p.tile = (unsigned int)(rest / p.walk.length);
+  p.tile = (unsigned int)quotient(rest, p.walk.length);
   p.at = (unsigned int)(rest - (unsigned long long)p.tile * p.walk.length);
   p.left = (unsigned int)min(p.quota, all - from);
   return true;
@@ -222,14 +240,14 @@ __device__ __forceinline__ bool cache_piece(const CacheAttnArgs& a, const CacheF
   }
   const int n_tokens = piece.shift ? max(piece.end - piece.shift, piece.sink_end) : max(piece.end, 0);       // (the window may lie behind the last page)
   piece.begin = (int)min((long long)p.at * 64, (long long)n_tokens);
-  piece.stop = (int)min((long long)(p.at + take) * 64, (long long)n_tokens);
+  piece.stop = p.whole ? n_tokens : (int)min((long long)(p.at + take) * 64, (long long)n_tokens);
   piece.parts = 1;
   piece.part = 0;
   piece.first_block = blockIdx.x;
   if (take < p.walk.length) {
     const unsigned long long from = p.ahead + (unsigned long long)p.tile * p.walk.length;
-    piece.first_block = (unsigned int)(from / p.quota);
-    piece.parts = (unsigned int)((from + p.walk.length - 1) / p.quota) - piece.first_block + 1;
+    piece.first_block = (unsigned int)quotient(from, p.quota);
+    piece.parts = (unsigned int)quotient(from + p.walk.length - 1, p.quota) - piece.first_block + 1;
     piece.part = blockIdx.x - piece.first_block;
   }
   return true;
@@ -246,6 +264,7 @@ __device__ __forceinline__ void cache_advance(const CacheAttnArgs& a, CachePart&
     p.s = cache_seq(a.c, ++p.b);
   } while (!p.s.count && p.b + 1 < a.c.batch);
   p.walk = cache_walk<ROWS>(a, p.s);
+  if (p.whole) p.walk.length = 1;
 }
 
 // The parts of a row: the first lies a place behind the others' line, (2 k - 1) places on for k > 0
@@ -359,6 +378,31 @@ __global__ void __launch_bounds__(kCacheFewThreads, (CacheFewShape<DP, CODED, NR
   // (this lane's columns are rows 8 r + 2 q4 and the next one)
   const int all_see = cache_last(a, plan.least_pos), all_from = cache_first(a, plan.most_pos);
 
+  // ---- the queries as the B operand, in the order of the keys' pieces: row 8 r + g.  Under way before the pages are looked up.
+  unsigned int q[NR][KS][2];
+  float unit[NR][2];                                 // what a column's products have to be multiplied by
+  {
+    constexpr int kRun = CODED ? 16 : 8;             // neighbouring elements of a lane
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      const int i = (int)g + 8 * r;
+      const bool on = i < rows;
+      const unsigned short* from = (const unsigned short*)a.q + (on ? ((long long)(s.first + query_of(i)) * a.H + head_of(i)) * c.D : 0);
+#pragma unroll
+      for (int p = 0; p < DP / (4 * kRun); ++p)
+#pragma unroll
+        for (int t = 0; t < kRun / 8; ++t) {
+          const int e = p * 4 * kRun + (int)q4 * kRun + t * 8, ks = p * (kRun / 4) + 2 * t;
+          uint4 v = make_uint4(0u, 0u, 0u, 0u);
+          if (on && e < c.D) v = *(const uint4*)(from + e);
+          q[r][ks][0] = v.x;
+          q[r][ks][1] = v.y;
+          q[r][ks + 1][0] = v.z;
+          q[r][ks + 1][1] = v.w;
+        }
+    }
+  }
+
   // ---- the ring: steps of 16 tokens, every fourth of them this warp's
   const unsigned int ring = dyn_at + warp * Sh::kRing;
   const int steps = v_end > v_begin ? (v_end - v_begin + 15) / 16 : 0;
@@ -449,28 +493,10 @@ __global__ void __launch_bounds__(kCacheFewThreads, (CacheFewShape<DP, CODED, NR
 #pragma unroll
   for (int i = 0; i < Sh::kStages - 1; ++i) fetch(i);
 
-  // ---- the queries as the B operand, in the order of the keys' pieces: row 8 r + g
-  unsigned int q[NR][KS][2];
-  float unit[NR][2];                                 // what a column's products have to be multiplied by
+  // (their conversion, once the first copies are under way)
   {
-    constexpr int kRun = CODED ? 16 : 8;             // neighbouring elements of a lane
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
-      const int i = (int)g + 8 * r;
-      const bool on = i < rows;
-      const unsigned short* from = (const unsigned short*)a.q + (on ? ((long long)(s.first + query_of(i)) * a.H + head_of(i)) * c.D : 0);
-#pragma unroll
-      for (int p = 0; p < DP / (4 * kRun); ++p)
-#pragma unroll
-        for (int t = 0; t < kRun / 8; ++t) {
-          const int e = p * 4 * kRun + (int)q4 * kRun + t * 8, ks = p * (kRun / 4) + 2 * t;
-          uint4 v = make_uint4(0u, 0u, 0u, 0u);
-          if (on && e < c.D) v = *(const uint4*)(from + e);
-          q[r][ks][0] = v.x;
-          q[r][ks][1] = v.y;
-          q[r][ks + 1][0] = v.z;
-          q[r][ks + 1][1] = v.w;
-        }
       float mine_unit = 1.f;
       if constexpr (CODED && std::is_same<T, __nv_bfloat16>::value) {
         unsigned int most = 0;

@@ -84,6 +84,7 @@ struct CacheAttnOperator : b200_operator {
     const long long capacity = (std::min<long long>((long long)c.max_pages * c.page, 0x7fffffff) + 127) / 64;       // 64s
     few_args.blocks = (unsigned int)(dev->sm_count * blocks);
     few_args.least = (unsigned int)std::max<long long>(least, capacity / (kFewMost - 4) + 1);
+    few_args.enough = (unsigned int)dev->sm_count;
     // Short sequences: a tile a block.
     few_args.single = capacity <= (long long)few_args.least + few_args.least / 2;
     few_args.by_group = Divisor((unsigned int)a.group);
