@@ -13,6 +13,7 @@
 #include <cooperative_groups.h>
 
 #include <cmath>
+#include <type_traits>
 
 #include "kernels/op_common.cuh"
 #include "operators.hpp"
@@ -34,7 +35,7 @@ struct SampleArgs {
   int top_k;
 };
 
-constexpr int kThreads = 256, kWarps = kThreads / 32, kBins = 32, kList = 1024, kMostParts = 8;
+constexpr int kThreads = 256, kWarps = kThreads / 32, kBins = 32, kList = 1024, kLocal = 2 * kList, kMostParts = 8;
 
 // rises with the value
 __device__ __forceinline__ unsigned int key_of(float x) {
@@ -44,7 +45,10 @@ __device__ __forceinline__ unsigned int key_of(float x) {
 __device__ __forceinline__ float of_key(unsigned int k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
 struct Share {                         // of a block, for the others of its cluster to read
-  unsigned long long list[kList];      // logits that may be at the border
+  union {
+    unsigned int local[kLocal];        // indices of logits of this block's that may be at the border
+    unsigned long long list[kList];    // (rows in registers) the logits themselves, as they are sorted
+  };
   unsigned int listed;                 // entries of the list (more than it holds: it is of no use)
   unsigned int joined;                 // of the first block: entries of the list that all blocks' go to
   unsigned int joined_from;            // where this block's begin there
@@ -359,7 +363,8 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
 
   unsigned int histograms = 0;
   // a histogram of the kept logits that `over` passes on and `of` gives a bin (0: the highest); bins of all blocks, joined, in sh
-  auto histogram = [&](auto over, auto of) {
+  // (`fresh`: nothing but -infinity has been left out yet)
+  auto histogram_of = [&](auto fresh, auto over, auto of) {
     const unsigned int set = histograms++ & 1u;
     for (unsigned int i = threadIdx.x; i < kWarps * kBins * 32 / 2; i += kThreads) ((uint4*)bins)[i] = make_uint4(0u, 0u, 0u, 0u);
     __syncthreads();
@@ -367,7 +372,7 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
     over([&](float x, unsigned int i) {
       const float z = below(x), w = weight_at(z);
       const int b = of(x, z);
-      if (kept(x, i) & (b >= 0)) {
+      if ((fresh.value ? x > -INFINITY : kept(x, i)) & (b >= 0)) {
         uint2 v = mine[b * 32];
         v.x = __float_as_uint(__uint_as_float(v.x) + w);
         ++v.y;
@@ -421,6 +426,10 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
     }
     __syncthreads();                   // (this set of shares is written again two histograms on, with a meeting between)
   };
+  auto histogram = [&](auto over, auto of) {
+    if (border == -INFINITY) histogram_of(std::true_type(), over, of);
+    else histogram_of(std::false_type(), over, of);
+  };
   auto whole_row = [&](auto f) { logits.each(f); };
   // the count and the sum of all bins: a warp, a lane a bin
   auto everything = [&](unsigned int& n, double& s) {
@@ -444,59 +453,71 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
     return r;
   };
   // puts the kept logits that `of` accepts into this block's list
-  auto gather = [&](auto of) {
+  auto gather_of = [&](auto fresh, auto of) {
     __syncthreads();
     if (threadIdx.x == 0) sh.listed = 0;
     __syncthreads();
     logits.batches([&](const auto& y, auto index) {
       unsigned int mask = 0;
 #pragma unroll
-      for (int e = 0; e < Logits<T, E>::kBatch; ++e) mask |= (kept(y[e], index(e)) & of(y[e])) ? 1u << e : 0u;
+      for (int e = 0; e < Logits<T, E>::kBatch; ++e) mask |= ((fresh.value ? y[e] > -INFINITY : kept(y[e], index(e))) & of(y[e])) ? 1u << e : 0u;
       if (!__any_sync(0xffffffffu, mask)) return;
       unsigned int at = mask ? atomicAdd(&sh.listed, (unsigned int)__popc((int)mask)) : 0u;
 #pragma unroll
       for (int e = 0; e < Logits<T, E>::kBatch; ++e)
         if (mask >> e & 1u) {
-          if (at < kList) sh.list[at] = (unsigned long long)~key_of(y[e] + 0.f) << 32 | index(e);       // (one zero)
+          if constexpr (E > 0) {
+            if (at < kList) sh.list[at] = (unsigned long long)~key_of(y[e] + 0.f) << 32 | index(e);      // (one zero)
+          } else {
+            if (at < kLocal) sh.local[at] = index(e);
+          }
           ++at;
         }
     });
     __syncthreads();
   };
+  auto gather = [&](auto of) {
+    if (border == -INFINITY) gather_of(std::true_type(), of);
+    else gather_of(std::false_type(), of);
+  };
+  auto logit_at = [&](unsigned int i) { return to_float(logits.row[logits.off + i]); };
   auto listed_logits = [&](auto f) {
-    for (unsigned int k = threadIdx.x; k < sh.listed; k += kThreads) f(of_key(~(unsigned int)(sh.list[k] >> 32)), (unsigned int)sh.list[k]);
+    for (unsigned int k = threadIdx.x; k < sh.listed; k += kThreads) f(logit_at(sh.local[k]), sh.local[k]);
   };
   // ... and those of the list that `of` accepts to the list of all blocks, kList in all
   auto send = [&](auto of) {
-    if (E > 0) {
+    if constexpr (E > 0) {
       if (threadIdx.x == 0) sh.joined = sh.listed;
       __syncthreads();
-      return;
-    }
-    Share* first = of_part(&sh, parts, 0);
-    unsigned long long* to = parts > 1 ? cg::this_cluster().map_shared_rank(all_list, 0) : all_list;
-    const unsigned int n = min(sh.listed, (unsigned int)kList);
-    // (a place in another block's list is some 1500 cycles away: one question a warp)
-    unsigned long long mine[kList / kThreads];
-    unsigned int many = 0;
+    } else {
+      Share* first = of_part(&sh, parts, 0);
+      unsigned long long* to = parts > 1 ? cg::this_cluster().map_shared_rank(all_list, 0) : all_list;
+      const unsigned int n = min(sh.listed, (unsigned int)kLocal);
+      // (a place in another block's list is some 1500 cycles away: one question a warp)
+      unsigned long long mine[kLocal / kThreads];
+      unsigned int many = 0;
 #pragma unroll
-    for (int k = 0; k < kList / kThreads; ++k) {
-      const unsigned int i = threadIdx.x + k * kThreads;
-      mine[k] = i < n ? sh.list[i] : ~0ull;
-      if (i < n && !of(of_key(~(unsigned int)(mine[k] >> 32)))) mine[k] = ~0ull;
-      many += mine[k] != ~0ull;
-    }
-    const unsigned int up_to = warp_up_to(many);
-    unsigned int at = 0;
-    if (lane == 31 && up_to) at = atomicAdd(&first->joined, up_to);
-    at = __shfl_sync(0xffffffffu, at, 31) + up_to - many;
-#pragma unroll
-    for (int k = 0; k < kList / kThreads; ++k)
-      if (mine[k] != ~0ull) {
-        if (at < kList) to[at] = mine[k];
-        ++at;
+      for (int k = 0; k < kLocal / kThreads; ++k) {
+        const unsigned int i = threadIdx.x + k * kThreads;
+        mine[k] = ~0ull;
+        if (i < n) {
+          const unsigned int at = sh.local[i];
+          const float x = logit_at(at);
+          if (of(x)) mine[k] = (unsigned long long)~key_of(x + 0.f) << 32 | at, ++many;                   // (one zero)
+        }
       }
-    meet(parts);
+      const unsigned int up_to = warp_up_to(many);
+      unsigned int at = 0;
+      if (lane == 31 && up_to) at = atomicAdd(&first->joined, up_to);
+      at = __shfl_sync(0xffffffffu, at, 31) + up_to - many;
+#pragma unroll
+      for (int k = 0; k < kLocal / kThreads; ++k)
+        if (mine[k] != ~0ull) {
+          if (at < kList) to[at] = mine[k];
+          ++at;
+        }
+      meet(parts);
+    }
   };
   auto logit_of = [&](unsigned long long entry) { return of_key(~(unsigned int)(entry >> 32)); };
   // The first n of the sorted list that reach a goal, by count or by sum: each thread has four entries.  `ahead`: the sum ahead of the list
@@ -653,11 +674,11 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
       auto inside = [&](float x) { return (x >= of_key(lo)) & (x <= of_key(hi)); };
       for (;;) {
         // (where the lists are likely to hold it; an uneven row is passed again)
-        if (!have && (at.in <= kList || (lo < hi && at.in <= kList * parts / 4 * 3))) {
+        if (!have && (at.in <= kList || (lo < hi && at.in <= kLocal * parts / 4 * 3))) {
           gather(inside);
           meet(parts);
           have = true;
-          have = __all_sync(0xffffffffu, lane >= parts || of_part(&sh, parts, lane)->listed <= kList);
+          have = __all_sync(0xffffffffu, lane >= parts || of_part(&sh, parts, lane)->listed <= kLocal);
           meet(parts);
         }
         // (a few hundred are divided sooner than sorted, where no pass over the row is needed for it)
