@@ -120,11 +120,15 @@ struct CacheAttnOperator : b200_operator {
     choose_parts(kAnyRows, kAnyWidth, (int)std::min<size_t>(6, 220 * 1024 / (smem + 7 * 1024)), 4);
     ready(any, smem);
   }
-  // Whole prompts: tiles of 128 rows on the tensor cores, where sequences have them on average and the cache's pages are boxes of the TMA unit.
+  // Tiles of 128 rows walk all their tokens in one block, some 0.85 us for 64 of them; tiles of 16 spread them over the machine, which gets through some
+  // 18000 tokens of a tile in a us in 8 bits, 10000 else.  So there have to be tiles of 128 enough, and rows enough in them (measured, us by sixteens and by
+  // 128s: 64 new tokens of 32 heads over 8 key heads and 8192 tokens, 8 bits, 31 and 108; 300 each of four sequences, 8 over 1, 4096, 8 bits, 70 and 56; 512 of 8 over
+  // 8, 2048 tokens, 24 and 22; 64 each of eight, 32 over 8, 2048 tokens, 102 and 33).
   bool many() const {
     const CacheArgs& c = a.c;
     const bool boxes = c.n_pages && c.page % 16 == 0 && (c.page % 64 == 0 || 64 % c.page == 0);
-    return boxes && a.group <= 128 && ((size_t)a.out & 15) == 0 && (long long)c.tokens * a.group >= 128ll * std::min(c.batch, c.tokens);
+    const long long rows = (long long)c.tokens * a.group;
+    return boxes && a.group <= 128 && ((size_t)a.out & 15) == 0 && rows >= 32ll * std::min(c.batch, c.tokens) && rows * c.HK >= 128ll * (coded ? 72 : 32);
   }
   void choose_tiles() {
     const CacheArgs& c = a.c;

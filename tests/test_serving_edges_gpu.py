@@ -6,7 +6,7 @@ import pytest
 from ocannl_b200 import backend as bk
 from ocannl_b200.low_level import Tnode
 from tests import serving_reference as R
-from tests.test_serving_gpu import ATTEND, PROMPTS, append_case, append_nodes, attend_case, attend_nodes, check_attend, link_append, link_attend, want_attend
+from tests.test_serving_gpu import ATTEND, PROMPTS, TILES, append_case, append_nodes, attend_case, attend_nodes, check_attend, link_append, link_attend, want_attend
 
 pytestmark = pytest.mark.gpu
 
@@ -117,7 +117,7 @@ def test_a_prompt_and_the_tokens_behind_it(device, prec, coded):
         s.free()
 
 
-EVERY = [ATTEND[1], ATTEND[3], ATTEND[5], ATTEND[8], ATTEND[9], PROMPTS[1], PROMPTS[4], PROMPTS[9]]
+EVERY = [ATTEND[1], ATTEND[3], ATTEND[5], ATTEND[8], ATTEND[9], PROMPTS[1], PROMPTS[4], PROMPTS[9], TILES[1], TILES[4]]
 
 
 @pytest.mark.parametrize("coded", [False, True])
@@ -152,7 +152,7 @@ def test_undefined_values_that_are_seen(device, case, what, prec, coded):
 
 
 @pytest.mark.parametrize("coded", [False, True])
-@pytest.mark.parametrize("case", [ATTEND[1], ATTEND[4], PROMPTS[1]])
+@pytest.mark.parametrize("case", [ATTEND[1], ATTEND[4], PROMPTS[1], TILES[1]])
 def test_pages_of_several_sequences(device, case, coded):
     """Two sequences with one beginning."""
     case = (2,) + case[1:] if isinstance(case[1], int) else (2, case[1][:2]) + case[2:]

@@ -307,7 +307,7 @@ def test_attention_over_pages(device, case, prec, coded):
         nodes.free()
 
 
-# prompts: rows enough for tiles of 128 on the tensor cores
+# prompts, in tiles of 16 rows
 PROMPTS = [
     (1, 128, [128], 64, 2, 2, 128, 0, 0, 0.0, False),
     (2, [100, 300], [700, 300], 16, 2, 8, 128, 0, 0, 0.0, False),
@@ -322,11 +322,24 @@ PROMPTS = [
     (1, 130, [17000], 64, 1, 2, 64, 0, 0, 0.0, False),
     (1, 70, [34000], 16, 1, 2, 128, 0, 0, 0.0, False),
 ]
+# key heads, and rows of them, enough for tiles of 128
+TILES = [
+    (1, 128, [128], 64, 72, 72, 64, 0, 0, 0.0, False),
+    (2, [100, 300], [700, 300], 16, 12, 24, 128, 0, 0, 0.0, False),
+    (3, [64, 0, 200], [64, 9, 1000], 32, 8, 40, 96, 150, 20, 0.0, True),
+    (2, [90, 33], [513, 129], 64, 26, 78, 64, 0, 0, 20.0, False),
+    (1, 260, [1000], 128, 2, 40, 80, 200, 70, 0.0, False),
+    (2, [200, 70], [190, 300], 64, 9, 36, 48, 0, 0, 5.0, True),
+    (5, 40, [40, 100, 300, 77, 64], 16, 12, 48, 64, 33, 2, 0.0, False),
+    (1, 1, [50], 16, 72, 9216, 64, 0, 0, 0.0, False),
+    (1, 140, [34000], 16, 34, 68, 16, 0, 0, 0.0, False),
+    (2, [700, 900], [60, 900], 64, 4, 16, 112, 0, 0, 0.0, False),
+]
 
 
 @pytest.mark.parametrize("coded", [False, True])
 @pytest.mark.parametrize("prec", ["bfloat16", "half"])
-@pytest.mark.parametrize("case", PROMPTS)
+@pytest.mark.parametrize("case", PROMPTS + TILES)
 def test_prompts_over_pages(device, case, prec, coded):
     x, table, lengths, starts, page, t = attend_case(case, prec, coded)
     want = want_attend(x, table, lengths, starts, page, prec, t)
