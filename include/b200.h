@@ -356,7 +356,8 @@ int b200_cache_attention_link(b200_dev* dev, const b200_cache_attention* spec, b
  * the running sum of w exceeds uniform * (the kept sum) (uniform below 0 or undefined: 0; the last kept one where none does).
  * logprob = log(w_token / kept sum).  temperature 0 or less: the first largest, logprob 0.  Undefined logits count as -infinity, which is never chosen; where
  * there are infinite ones, those have w = 1 and the others 0.  A row of nothing else: token -1, logprob -infinity.
- * Every setting is one number for all rows or a node of one a row.  1 <= vocab < 2^31. */
+ * Every setting is one number for all rows or a node of one a row (there an undefined temperature is 0, an undefined top_p 1, an undefined min_p 0).
+ * 1 <= vocab < 2^31. */
 typedef struct {
   int64_t rows, vocab;
   int32_t dtype;                 /* of the logits */

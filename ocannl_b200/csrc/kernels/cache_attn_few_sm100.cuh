@@ -35,7 +35,7 @@ struct CacheFewArgs {
 };
 
 constexpr int kCacheFewWarps = 4, kCacheFewThreads = 32 * kCacheFewWarps;
-constexpr unsigned int kCacheShort = 24;      // 64s of tokens of tiles that are not cut, on average
+constexpr unsigned int kCacheShort = 24;      // 64s of tokens, at most, of tiles that are not cut
 constexpr unsigned int kCachePart = 1024;     // 64s of tokens of a block at most, a quarter of them a warp's: its accumulators' cut-off sums lose 2^-13 (see kSumKeys)
 
 template <int DP, bool CODED, int NR>
@@ -140,10 +140,12 @@ __device__ __forceinline__ bool cache_part(const CacheAttnArgs& a, const CacheFe
     return true;
   }
   __shared__ unsigned long long sums[2][NT / 32], found[2];
+  __shared__ unsigned int longest_of[NT / 32];
   const unsigned int lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
   // of NT sequences from i0 on: 64s and tiles, this thread's, those before it, and added to all
   auto sums_of = [&](int i0, unsigned long long& all, unsigned long long& tiles, unsigned long long& mine, unsigned long long& mine_tiles, unsigned long long& before,
-                     unsigned long long& before_tiles) {
+                     unsigned long long& before_tiles, unsigned int& longest) {
+    unsigned int length = 0;
     const int i = i0 + (int)threadIdx.x;
     mine = mine_tiles = 0;
     if (i < c.batch) {
@@ -151,7 +153,8 @@ __device__ __forceinline__ bool cache_part(const CacheAttnArgs& a, const CacheFe
       if (s.count) {
         const CacheWalk w = cache_walk<ROWS>(a, s);
         mine_tiles = w.tiles;
-        mine = mine_tiles * w.length;
+        length = w.length;
+        mine = mine_tiles * length;
       }
     }
     unsigned long long up_to[2] = {mine, mine_tiles};
@@ -163,7 +166,8 @@ __device__ __forceinline__ bool cache_part(const CacheAttnArgs& a, const CacheFe
         if (lane >= (unsigned int)o) up_to[k] += x;
       }
     __syncthreads();
-    if (lane == 31) sums[0][warp] = up_to[0], sums[1][warp] = up_to[1];
+    length = __reduce_max_sync(0xffffffffu, length);
+    if (lane == 31) sums[0][warp] = up_to[0], sums[1][warp] = up_to[1], longest_of[warp] = length;
     __syncthreads();
     before = all + up_to[0] - mine;
     before_tiles = tiles + up_to[1] - mine_tiles;
@@ -172,15 +176,17 @@ __device__ __forceinline__ bool cache_part(const CacheAttnArgs& a, const CacheFe
       if (w < (int)warp) before += sums[0][w], before_tiles += sums[1][w];
       all += sums[0][w];
       tiles += sums[1][w];
+      longest = max(longest, longest_of[w]);
     }
   };
   // the whole walk, and its tiles; with a sequence a thread, one look at the lengths finds the block's own place as well
   unsigned long long all = 0, tiles = 0, mine = 0, mine_tiles = 0, before = 0, before_tiles = 0;
+  unsigned int longest = 0;
   for (int i0 = 0; i0 < c.batch; i0 += NT) {
-    sums_of(i0, all, tiles, mine, mine_tiles, before, before_tiles);
+    sums_of(i0, all, tiles, mine, mine_tiles, before, before_tiles, longest);
   }
   // Short tiles, and enough of them for the machine: none is cut (32 sequences of 8 key heads, 1044 tokens each: 25.8 us, 27.2 cut).
-  p.whole = tiles >= f.enough && all <= tiles * kCacheShort;
+  p.whole = tiles >= f.enough && longest <= kCacheShort;
   if (p.whole) {
     all = tiles;
     mine = mine_tiles;
@@ -198,7 +204,7 @@ __device__ __forceinline__ bool cache_part(const CacheAttnArgs& a, const CacheFe
   } else {
     unsigned long long sum = 0, sum_tiles = 0;
     for (int i0 = 0; i0 < c.batch; i0 += NT) {
-      sums_of(i0, sum, sum_tiles, mine, mine_tiles, before, before_tiles);
+      sums_of(i0, sum, sum_tiles, mine, mine_tiles, before, before_tiles, longest);
       if (p.whole) {
         mine = mine_tiles;
         before = before_tiles;

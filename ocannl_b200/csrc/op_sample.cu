@@ -285,7 +285,7 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
   constexpr int VEC = Logits<T, E>::VEC;
   const Logits<T, E> logits(a, row, part);
   const float temperature = a.temperatures ? a.temperatures[row] : a.temperature, top_p = a.top_ps ? a.top_ps[row] : a.top_p;
-  const float min_p = a.min_ps ? a.min_ps[row] : a.min_p, uniform = a.uniform[row];
+  const float min_p = fmaxf(a.min_ps ? a.min_ps[row] : a.min_p, 0.f), uniform = a.uniform[row];
   const int top_k = a.top_ks ? a.top_ks[row] : a.top_k;
   auto larger = [](auto u, auto v) { return u > v ? u : v; };
   auto smaller = [](auto u, auto v) { return u < v ? u : v; };

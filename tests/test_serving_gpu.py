@@ -430,6 +430,16 @@ def test_settings_as_numbers(device, given):
     check_sample(run_sample(device, "half", x, u, given), x, u, given)
 
 
+def test_settings_that_are_undefined(device):
+    """In a node: a temperature is 0 then, top_p 1, min_p 0; negative ones count as none."""
+    rng = np.random.default_rng(12)
+    x, u = logits(rng, "single", 8, 1500, "logits"), R.rounded("single", rng.random(8))
+    nan, ones = np.full(8, np.nan), np.ones(8)
+    for given, same in ((dict(temperature=nan), dict(temperature=0.0)), (dict(top_p=nan), {}), (dict(min_p=nan), {}), (dict(top_p=-ones, min_p=-ones, top_k=-ones), dict(top_p=0.0)),
+                        (dict(temperature=-ones), dict(temperature=0.0)), (dict(top_k=2e9 * ones), {})):
+        check_sample(run_sample(device, "single", x, u, given), x, u, same)
+
+
 def test_random_numbers_at_the_ends(device):
     """0, just below 1, and those outside: the first and the last kept token."""
     rng = np.random.default_rng(9)
