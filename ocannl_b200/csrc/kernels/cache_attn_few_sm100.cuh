@@ -5,8 +5,8 @@
 // nothing, and take half the registers and products of a tile of 16.  A product does not care in which order its elements are added, so the order is
 // chosen for the loads: of the 16 elements of a step each of the four lanes that share a token has four neighbours, and the rows of the second product
 // are dealt out as neighbours to a lane too, so that every operand is read as whole 16-byte pieces by the lane that multiplies it.  A warp's ring is
-// its own, with no barrier between warps: pages that hold whole steps of 16 tokens arrive as boxes of the TMA unit, two or four a step (by 16-byte copies of
-// all lanes, 64 sequences of up to 8192 took 182 us with their products and 183 without), others by cp.async.  Codes of 8 bits become halves in registers, two to an instruction; a transposed pair of values is one byte
+// its own, with no barrier between warps: pages that hold whole steps of 16 tokens arrive as boxes of the TMA unit, two or four a step (64
+// sequences of up to 8192, 32 heads over 8 of 128, codes: 145 us, 5.5 TB/s; by 16-byte copies of all lanes 182, and 183 without the products), others by cp.async.  Codes of 8 bits become halves in registers, two to an instruction; a transposed pair of values is one byte
 // permutation, and the weights turn from scores' to operand's layout by a transpose of 8 x 8 between lanes.  Codes are multiplied as they are: a
 // page's scale of the keys goes onto its scores, the logarithm of its scale of the values onto the exponents of its weights, which the row's sum takes off
 // again: out = sum w code / sum (w / scale), so that weights stay in the range of a half whatever the scales.  (bfloat16 queries beside codes become
@@ -14,7 +14,7 @@
 //
 // The tokens that all tiles see (with a window: the sinks' and the window's, as one range), tile behind tile, are one long walk, of which every block takes
 // an equal part: the end of one tile, some whole ones, the beginning of another.  Every block finds its part from the lengths of all sequences, so that sequences
-// of all lengths fill the machine evenly, in one round of blocks.  (Chunks of a tile a block, three rounds of them: 64 sequences of up to 8192 in 193 us.)  The
+// of all lengths fill the machine evenly, in one round of blocks.  (Chunks of a tile a block, three rounds of them, with copies of all lanes: 193 us, parts 182.)  The
 // block of a tile that comes last joins its parts in their order: the same bits whoever comes last.
 #ifndef B200_CACHE_ATTN_FEW_SM100_CUH
 #define B200_CACHE_ATTN_FEW_SM100_CUH
@@ -35,7 +35,7 @@ struct CacheFewArgs {
 };
 
 constexpr int kCacheFewWarps = 4, kCacheFewThreads = 32 * kCacheFewWarps;
-constexpr unsigned int kCacheShort = 24;      // 64s of tokens, at most, of tiles that are not cut
+constexpr unsigned int kCacheShort = 24;      // 64s of tokens, at most, of tiles that are not cut (32 sequences with a window of 1024: 25 us, 27 cut)
 constexpr unsigned int kCachePart = 1024;     // 64s of tokens of a block at most, a quarter of them a warp's: its accumulators' cut-off sums lose 2^-13 (see kSumKeys)
 
 template <int DP, bool CODED, int NR>

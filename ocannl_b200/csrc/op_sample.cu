@@ -3,13 +3,14 @@
 //   w_i = exp((x_i - max) / T);  kept: the first n in the order of falling x, of rising i among equal ones;  token: where the running sum of the kept, in the
 //   order of i, passes uniform * its end
 //
-// Bound by memory: a row is read once, and again from L2 in two or three more passes.  A cluster of up to eight blocks takes it and exchanges sums through
+// A row is read once, and again from L2 in two or three more passes.  A cluster of up to eight blocks takes it and exchanges sums through
 // shared memory.  What is kept is all logits above a border and, of those equal to it, the ones up to an index: no sort of the row.  The border is found by a
 // histogram of 32 bins, half a binade of weight each, of counts and sums of weights; every lane has columns of its own, so that nothing is added atomically and
 // sums come out the same every time.  A bin that bounds what is kept, with all above it, is usually a few hundred logits: these go to one block, which
 // sorts them and does the rest.  Where they are more than 1024, the bin is divided again by the bits of its logits, until it is small or of one value,
 // and the row is passed once more for the token.  Weights are summed in double precision beyond a lane's, so that borders lie where they do in 64 bits but
-// for 2^-22 of a weight.
+// for 2^-22 of a weight.  Measured: 256 rows of 131072 logits 192 us, 64 of 50021 in bfloat16 40 us: bound by instructions and by the
+// blocks' waits for one another (the bytes alone: 20 us).
 #include <cooperative_groups.h>
 
 #include <cmath>
