@@ -89,6 +89,7 @@ __device__ __forceinline__ bool find_unit(int batch, unsigned int target, F unit
       if (lane >= (unsigned int)o) up_to += x;
     }
     if (lane == 31) warps[warp] = up_to;
+    if (threadIdx.x == 0) found[0] = 0xffffffffu;
     __syncthreads();
     unsigned int before = 0, all = 0;
 #pragma unroll
@@ -106,7 +107,7 @@ __device__ __forceinline__ bool find_unit(int batch, unsigned int target, F unit
       b = (int)found[0];
       rest = found[1];
       __syncthreads();
-      return true;
+      return b >= 0;                  // (sums that pass 32 bits, of starts that fall: nobody's)
     }
     target -= all;
     __syncthreads();                  // (the sums are written again)
