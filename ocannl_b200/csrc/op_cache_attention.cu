@@ -139,8 +139,11 @@ struct CacheAttnOperator : b200_operator {
     const long long capacity = (long long)c.max_pages * c.page, some = std::min(c.batch, c.tokens);
     auto blocks = [&](int nq) { return (c.tokens + (nq * tile_args.tokens - 1) * some) / (nq * tile_args.tokens) * c.HK; };
     tile_args.sums = capacity > kSumKeys;
-    // Two row tiles a block share their keys, unless that leaves SMs without a block, or there are sums beside the accumulators.
-    const bool two = !tile_args.sums && (long long)c.tokens / (2 * tile_args.tokens) * c.HK >= dev->sm_count;
+    // Two row tiles a block share their keys and wait in turn: they take hardly longer than one.  One a block where all blocks run at once that way, or there
+    // are sums beside the accumulators.  (us, one and two: 700 tokens of 32 heads over 8 of 128, codes, 176 blocks and 88, 295 and 150; 1100 of heads of 64 in 16 bits, two
+    // blocks of one tile an SM, 280 and 144, 137 and 166.)
+    const long long about = (c.tokens + tile_args.tokens / 2 * some) / tile_args.tokens * c.HK;
+    const bool two = !tile_args.sums && about > (long long)dev->sm_count * (c.D <= 64 && !coded ? 2 : 1);
     tiles = cache_tiles(dtype, coded, c.D > 64, two);
     grid = blocks_of(blocks(two ? 2 : 1));
     const cuuint64_t of_q[4] = {(cuuint64_t)c.D, (cuuint64_t)a.group, (cuuint64_t)c.HK, (cuuint64_t)c.tokens};
