@@ -668,7 +668,7 @@ class Context:
             if isinstance(value, str):
                 setattr(spec, field + "s", self._operand(what, value, prec, rows))
             else:
-                setattr(spec, field, min(value, 2 ** 31 - 1) if field == "top_k" else value)
+                setattr(spec, field, max(-1, min(value, 2 ** 31 - 1)) if field == "top_k" else value)
         return Operator(self.device, "b200_sample_link", spec)
 
     # ---- host access (Context.set_values / get_values, arrayjit/lib/context.ml:322-395)

@@ -312,3 +312,17 @@ def test_refusals(device):
             call()
         assert e.value.code == code and words in str(e.value), words
     nodes.free()
+
+
+def test_numbers_to_keep_that_pass_32_bits(device):
+    """As many as there are, or none: all."""
+    rng = np.random.default_rng(47)
+    x, u = R.rounded("single", rng.normal(size=(4, 300))), R.rounded("single", np.full(4, 0.97))
+    nodes = R.Nodes(device, {"x": ("single", x.shape, x), "u": ("single", u.shape, u), "t": ("int32", u.shape, None)})
+    for top_k in (2 ** 32 + 2, 2 ** 31, -2 ** 32 + 2, -2 ** 31 - 1):
+        op = nodes.context.sample("x", "u", "t", top_k=top_k)
+        op.run()
+        device.await_()
+        assert nodes.read("t").tolist() == [R.sample(x[r], u[r])[0] for r in range(4)]
+        op.free()
+    nodes.free()
