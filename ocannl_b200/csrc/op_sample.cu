@@ -38,9 +38,9 @@ struct SampleArgs {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32, kBins = 32, kList = 1024, kLocal = 2 * kList, kMostParts = 8;
 
-// rises with the value
+// Rises with the value; one key for both zeros, as they are equal.  What is undefined lies outside the keys of -infinity and infinity.
 __device__ __forceinline__ unsigned int key_of(float x) {
-  const unsigned int u = __float_as_uint(x);
+  const unsigned int u = __float_as_uint(x + 0.f);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 __device__ __forceinline__ float of_key(unsigned int k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
@@ -308,6 +308,7 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
     const float other = lane < parts ? of_part(&sh, parts, lane)->largest : -INFINITY;
     top = warp_join(other, larger);
   }
+  top += 0.f;                          // (one zero, whichever lane or block it came from: ends of intervals are made of its bits)
   if (top == -INFINITY) {
     if (part == 0 && threadIdx.x == 0) {
       a.tokens[row] = -1;
@@ -373,7 +374,7 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
     over([&](float x, unsigned int i) {
       const float z = below(x), w = weight_at(z);
       const int b = of(x, z);
-      if ((fresh.value ? x > -INFINITY : kept(x, i)) & (b >= 0)) {
+      if ((fresh.value ? x > -INFINITY : kept(x, i)) & ((unsigned int)b < (unsigned int)kBins)) {
         uint2 v = mine[b * 32];
         v.x = __float_as_uint(__uint_as_float(v.x) + w);
         ++v.y;
@@ -468,7 +469,7 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
       for (int e = 0; e < Logits<T, E>::kBatch; ++e)
         if (mask >> e & 1u) {
           if constexpr (E > 0) {
-            if (at < kList) sh.list[at] = (unsigned long long)~key_of(y[e] + 0.f) << 32 | index(e);      // (one zero)
+            if (at < kList) sh.list[at] = (unsigned long long)~key_of(y[e]) << 32 | index(e);
           } else {
             if (at < kLocal) sh.local[at] = index(e);
           }
@@ -504,7 +505,7 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
         if (i < n) {
           const unsigned int at = sh.local[i];
           const float x = logit_at(at);
-          if (of(x)) mine[k] = (unsigned long long)~key_of(x + 0.f) << 32 | at, ++many;                   // (one zero)
+          if (of(x)) mine[k] = (unsigned long long)~key_of(x) << 32 | at, ++many;
         }
       }
       const unsigned int up_to = warp_up_to(many);
@@ -672,7 +673,11 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
       unsigned int above = at.above;
       double sum_above = at.sum_above;
       bool have = false;               // the blocks' lists hold the interval
-      auto inside = [&](float x) { return (x >= of_key(lo)) & (x <= of_key(hi)); };
+      // (by keys, as the bins are, so that what is inside has one)
+      auto inside = [&](float x) {
+        const unsigned int k = key_of(x);
+        return (k >= lo) & (k <= hi);
+      };
       for (;;) {
         // (where the lists are likely to hold it; an uneven row is passed again)
         if (!have && (at.in <= kList || (lo < hi && at.in <= kLocal * parts / 4 * 3))) {
@@ -686,7 +691,7 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
         if (at.in <= (have ? kList / 4 : kList) || lo == hi) break;
         int bits = 0;
         while ((hi - lo) >> bits >= kBins) ++bits;
-        auto split = [&](float x, float) { return inside(x) ? (int)((hi - key_of(x + 0.f)) >> bits) : -1; };
+        auto split = [&](float x, float) { return inside(x) ? (int)((hi - key_of(x)) >> bits) : -1; };
         if (have) histogram(listed_logits, split);
         else histogram(whole_row, split);
         at = find(counting, counting ? goal - above : goal - sum_above);

@@ -1,0 +1,44 @@
+"""Choices of a token over long rows where the border is hard to find: zeros of both signs as the largest logits, many equal logits, borders far down."""
+import numpy as np
+import pytest
+
+from tests import serving_reference as R
+from tests.test_serving_gpu import PRECS, check_sample, run_sample
+
+pytestmark = pytest.mark.gpu
+
+
+def repeated(rows, *arrays):
+    """The same few rows again and again, up to `rows` of them: their number decides how many blocks a row has."""
+    return [np.resize(a, (rows,) + a.shape[1:]) for a in arrays]
+
+
+def check_repeated(got, few, rows, x, u, given):
+    """The first `few` rows against the restatement, all others bit for bit against those."""
+    check_sample([a[:few] for a in got], x[:few], u[:few], {n: v[:few] if np.ndim(v) else v for n, v in given.items()})
+    for a in got:
+        assert a.tobytes() == np.resize(a[:few], a.shape).tobytes()
+
+
+# (vocab, rows): one to eight blocks a row
+ZEROS = [(1500, 5), (5000, 5), (5000, 600), (20011, 150), (20011, 300), (20011, 600), (131072, 5)]
+
+
+@pytest.mark.parametrize("prec", PRECS)
+@pytest.mark.parametrize("vocab,rows", ZEROS)
+def test_zeros_are_the_largest(device, vocab, rows, prec):
+    """Rows of -0 alone, of both zeros, of negated costs with thousands of zeros, and a -0 above all others."""
+    rng = np.random.default_rng(vocab + rows)
+    x = np.empty((5, vocab))
+    x[0] = -0.0
+    x[1] = np.where(rng.random(vocab) < 0.5, 0.0, -0.0)
+    x[2] = -np.maximum(rng.standard_normal(vocab), 0.0)
+    x[3] = -np.abs(rng.standard_normal(vocab))
+    x[3, vocab // 3] = -0.0
+    x[4] = np.where(rng.random(vocab) < 0.6, -0.0, -5.0)
+    x, u = R.rounded(prec, x), R.rounded("single", rng.random(5))
+    assert np.signbit(x[0]).all() and np.signbit(x[2][x[2] == 0]).all()
+    x, u = repeated(rows, x, u)
+    for given in (dict(top_k=50), dict(top_p=0.9), dict(top_k=1100, top_p=0.5, temperature=5.0), dict(min_p=0.5, temperature=0.5), dict(temperature=0.0)):
+        given = {n: float(np.float32(v)) if n != "top_k" else v for n, v in given.items()}
+        check_repeated(run_sample(device, prec, x, u, given), 5, rows, x, u, given)
