@@ -222,26 +222,9 @@ __global__ void __launch_bounds__(kCacheFewThreads) cache_attention_any(const __
       for (int i = (int)warp; i < rows; i += kCacheFewWarps) {
         // (the maxima are in the scores' unit; a part without visible tokens has a sum of exactly 0 and counts nothing)
         const float* from = f.parts + cache_part_at(plan.first_block, 0) * kAnyRows * kAnyWidth + i * kAnyWidth;
-        float t[kFewMost / 32], u[kFewMost / 32], top = -INFINITY, sum = 0.f;
-#pragma unroll
-        for (int k = 0; k < kFewMost / 32; ++k) {
-          const int at = (int)lane + 32 * k;
-          t[k] = at < n ? cache_part_row<128, kAnyRows>(from, at)[128] : -INFINITY;
-          u[k] = at < n ? cache_part_row<128, kAnyRows>(from, at)[129] : 0.f;
-          top = fmaxf(top, t[k]);
-        }
-#pragma unroll
-        for (int k = 16; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
-        __syncwarp();
-#pragma unroll
-        for (int k = 0; k < kFewMost / 32; ++k) {
-          const float w = u[k] == 0.f ? 0.f : t[k] == -INFINITY ? 1.f : exp2f((t[k] - top) * kCacheLog2e);
-          if ((int)lane + 32 * k < n) weigh[warp][lane + 32 * k] = w;
-          if (w != 0.f) sum = fmaf(w, u[k], sum);
-        }
-        sum = cache_sum(sum);
-        __syncwarp();
-        finish(i, cache_gather<128, kAnyRows>(from, n, weigh[warp], 4 * (int)lane), top, sum);
+        float top, sum;
+        const float4 v = cache_join<128, kAnyRows>([](float x) { return exp2f(x * kCacheLog2e); }, from, n, weigh[warp], true, 4 * (int)lane, top, sum);
+        finish(i, v, top, sum);
       }
     }
   }

@@ -18,6 +18,7 @@
 // block of a tile that comes last joins its parts in their order: the same bits whoever comes last.
 #ifndef B200_CACHE_ATTN_FEW_SM100_CUH
 #define B200_CACHE_ATTN_FEW_SM100_CUH
+#include "../cache_plan.hpp"
 #include "attn_few_sm100.cuh"
 #include "cache_attn_terms.cuh"
 
@@ -36,7 +37,6 @@ struct CacheFewArgs {
 
 constexpr int kCacheFewWarps = 4, kCacheFewThreads = 32 * kCacheFewWarps;
 constexpr unsigned int kCacheShort = 24;      // 64s of tokens, at most, of tiles that are not cut (32 sequences with a window of 1024: 25 us, 27 cut)
-constexpr unsigned int kCachePart = 1024;     // 64s of tokens of a block at most, a quarter of them a warp's: its accumulators' cut-off sums lose 2^-13 (see kSumKeys)
 
 template <int DP, bool CODED, int NR>
 struct CacheFewShape {
@@ -193,7 +193,7 @@ __device__ __forceinline__ bool cache_part(const CacheAttnArgs& a, const CacheFe
     before = before_tiles;
   }
   p.quota = quotient(all + f.blocks - 1, f.blocks);
-  if (!p.whole) p.quota = min(max(p.quota, (unsigned long long)f.least), (unsigned long long)kCachePart);
+  if (!p.whole) p.quota = cache_quota(p.quota, f.least);
   const unsigned long long from = p.quota * blockIdx.x;
   if (from >= all) return false;
   if (c.batch <= NT) {
@@ -276,9 +276,14 @@ __device__ __forceinline__ void cache_advance(const CacheAttnArgs& a, CachePart&
 // The parts of a row: the first lies a place behind the others' line, (2 k - 1) places on for k > 0
 template <int DP, int R>
 __device__ __forceinline__ const float* cache_part_row(const float* first, int k) { return first + (k ? (2 * k - 1) : 0) * (long long)(R * (DP + 4)); }
-// their maximum and sum, and in `weight` what each is multiplied by: a warp (see few_weigh)
-template <int DP, int R>
-__device__ __forceinline__ void cache_weigh(const float* first, int n, float* weight, float& top, float& sum) {
+// what a part counts for beside the largest maximum: see few_weigh.  `ex`: a weight from a difference in the scores' unit
+template <class Ex>
+__device__ __forceinline__ float cache_part_weight(Ex ex, float part_top, float part_sum, float top) {
+  return part_sum == 0.f ? 0.f : part_top == -INFINITY ? 1.f : ex(part_top - top);
+}
+// the maximum and sum of n of them (kFewMost at most) from k0 on, and in `weight` what each is multiplied by: a warp
+template <int DP, int R, class Ex>
+__device__ __forceinline__ void cache_weigh(Ex ex, const float* first, int k0, int n, float* weight, float& top, float& sum) {
   const unsigned int lane = threadIdx.x & 31u;
   float t[kFewMost / 32], u[kFewMost / 32];
   top = -INFINITY;
@@ -288,7 +293,7 @@ __device__ __forceinline__ void cache_weigh(const float* first, int n, float* we
     t[k] = -INFINITY;
     u[k] = 0.f;
     if (i < n) {
-      const float* row = cache_part_row<DP, R>(first, i);
+      const float* row = cache_part_row<DP, R>(first, k0 + i);
       t[k] = row[DP];
       u[k] = row[DP + 1];
     }
@@ -300,7 +305,7 @@ __device__ __forceinline__ void cache_weigh(const float* first, int n, float* we
   __syncwarp();                     // (all lanes have read the weights of the row before)
 #pragma unroll
   for (int k = 0; k < kFewMost / 32; ++k) {
-    const float w = u[k] == 0.f ? 0.f : t[k] == -INFINITY ? 1.f : ex2(t[k] - top);
+    const float w = cache_part_weight(ex, t[k], u[k], top);
     if ((int)lane + 32 * k < n) weight[lane + 32 * k] = w;
     if (w != 0.f) sum = fmaf(w, u[k], sum);
   }
@@ -310,7 +315,7 @@ __device__ __forceinline__ void cache_weigh(const float* first, int n, float* we
 }
 // four elements of their weighed sum, in their order; eight loads under way together
 template <int DP, int R>
-__device__ __forceinline__ float4 cache_gather(const float* first, int n, const float* weight, int e) {
+__device__ __forceinline__ float4 cache_gather(const float* first, int k0, int n, const float* weight, int e) {
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int i = 0; i < n; i += 8) {
     float4 x[8];
@@ -319,11 +324,33 @@ __device__ __forceinline__ float4 cache_gather(const float* first, int n, const 
     for (int k = 0; k < 8; ++k) {
       const int at = i + k;
       w[k] = at < n ? weight[at] : 0.f;
-      x[k] = *(const float4*)(cache_part_row<DP, R>(first, at < n ? at : i) + e);
+      x[k] = *(const float4*)(cache_part_row<DP, R>(first, k0 + (at < n ? at : i)) + e);
     }
 #pragma unroll
     for (int k = 0; k < 8; ++k)
       if (w[k] != 0.f) v = make_float4(fmaf(w[k], x[k].x, v.x), fmaf(w[k], x[k].y, v.y), fmaf(w[k], x[k].z, v.z), fmaf(w[k], x[k].w, v.w));
+  }
+  return v;
+}
+// A row of any number of parts by a warp: its maximum and sum, and elements e .. e + 3 (none where `on` is not set).  More than kFewMost, which only
+// sequences of some 16 million tokens have, are joined in turns, each to what the turns before have come to.
+template <int DP, int R, class Ex>
+__device__ __forceinline__ float4 cache_join(Ex ex, const float* first, int n, float* weight, bool on, int e, float& top, float& sum) {
+  const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
+  cache_weigh<DP, R>(ex, first, 0, min(n, kFewMost), weight, top, sum);
+  float4 v = on ? cache_gather<DP, R>(first, 0, min(n, kFewMost), weight, e) : none;
+  for (int k0 = kFewMost; k0 < n; k0 += kFewMost) {
+    float t, u;
+    cache_weigh<DP, R>(ex, first, k0, min(n - k0, kFewMost), weight, t, u);
+    const float4 x = on ? cache_gather<DP, R>(first, k0, min(n - k0, kFewMost), weight, e) : none;
+    const float next = fmaxf(top, t), by = cache_part_weight(ex, top, sum, next), w = cache_part_weight(ex, t, u, next);
+    v = by != 0.f ? make_float4(v.x * by, v.y * by, v.z * by, v.w * by) : none;
+    sum = by != 0.f ? sum * by : 0.f;
+    if (w != 0.f) {
+      v = make_float4(fmaf(w, x.x, v.x), fmaf(w, x.y, v.y), fmaf(w, x.z, v.z), fmaf(w, x.w, v.w));
+      sum = fmaf(w, u, sum);
+    }
+    top = next;
   }
   return v;
 }
@@ -814,8 +841,7 @@ __global__ void __launch_bounds__(kCacheFewThreads, (CacheFewShape<DP, CODED, NR
       bool fine = true;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
       if (joined) {
-        cache_weigh<DP, R>(all + i * W, n_parts, weights[warp], most, sum);
-        if (lane_e < DP) v = cache_gather<DP, R>(all + i * W, n_parts, weights[warp], lane_e);
+        v = cache_join<DP, R>([](float x) { return ex2(x); }, all + i * W, n_parts, weights[warp], lane_e < DP, lane_e, most, sum);
       } else {
         few_weigh<DP>(all + i * W, n_parts, R * W, weights[warp], most, sum);
         if (lane_e < DP) v = few_gather(all + i * W, n_parts, R * W, weights[warp], lane_e, 0, 1);

@@ -82,11 +82,12 @@ struct CacheAttnOperator : b200_operator {
     // A sequence of n tokens has n group rows.
     const long long some = std::min(c.batch, c.tokens), tiles = ((long long)c.tokens * a.group + (rows_of_tile - 1) * some) / rows_of_tile * c.HK;
     const long long capacity = (std::min<long long>((long long)c.max_pages * c.page, 0x7fffffff) + 127) / 64;       // 64s
-    few_args.blocks = (unsigned int)(dev->sm_count * blocks);
-    few_args.least = (unsigned int)std::max<long long>(least, capacity / (kFewMost - 4) + 1);
+    const CachePlan plan = cache_plan(blocks_of(tiles), (unsigned long long)capacity, (unsigned int)(dev->sm_count * blocks), (unsigned int)least, kFewMost);
+    few_args.blocks = plan.blocks;
+    few_args.least = plan.least;
     few_args.enough = (unsigned int)dev->sm_count;
     // Short sequences: a tile a block.
-    few_args.single = capacity <= (long long)few_args.least + few_args.least / 2;
+    few_args.single = plan.single;
     few_args.by_group = Divisor((unsigned int)a.group);
     few_args.by_key_heads = Divisor((unsigned int)c.HK);
     if (few_args.single) {
@@ -98,10 +99,7 @@ struct CacheAttnOperator : b200_operator {
       }
       return;
     }
-    // (more blocks only where an even share would be longer than a part may be; fewer where there is not that much)
-    const unsigned __int128 walk = (unsigned __int128)blocks_of(tiles) * (unsigned long long)capacity;
-    const unsigned __int128 cut = std::max<unsigned __int128>(few_args.blocks, walk / kCachePart + 1), most = walk / few_args.least + 1;
-    grid = blocks_of((long long)std::min<unsigned __int128>(std::min(cut, most), 1ull << 31));
+    grid = blocks_of((long long)plan.grid);
     const size_t parts = ((size_t)grid + 1) * 2 * rows_of_tile * floats * 4;
     take_workspace(parts + (size_t)grid * 4);
     few_args.parts = (float*)workspace;

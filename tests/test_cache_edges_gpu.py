@@ -1,0 +1,58 @@
+"""Attention over a paged cache at the ends of its range: sequences of tens of millions of tokens."""
+import numpy as np
+import pytest
+
+from tests import serving_reference as R
+from tests.test_serving_gpu import attend_nodes, link_attend
+
+pytestmark = pytest.mark.gpu
+
+
+def repeated_page(q, k, v, length, prec, coded, scale):
+    """(out, lse, bounds) of queries [h, d] that see `length` tokens, a page [page, d] again and again.  Bounds as in serving_reference.attention."""
+    page = k.shape[0]
+    times = length // page + (np.arange(page) < length % page)       # of every slot
+    z = q @ k.T * scale
+    top = np.where(times > 0, z, -np.inf).max(1, keepdims=True)
+    w = np.where(times > 0, np.exp(z - top), 0.0) * times
+    total = w.sum(1, keepdims=True)
+    out, lse = w / total @ v, (top + np.log(total))[:, 0]
+    half = R.EPS[prec] / 2
+    of_weights = 0.0 if prec == "single" else 2.0 ** -11 if coded else half
+    # (half weights below the normal range: 2^-25 of the largest, of all that a row sees)
+    tiny = 2.0 ** -25 * (times @ np.abs(v) + 1) / total if prec == "half" or (coded and prec != "single") else 1e-30
+    off = half * np.abs(out) + (of_weights + R.ARITH) * (w / total @ np.abs(v)) + tiny
+    return out, lse, off, R.ARITH * (1 + np.abs(lse))
+
+
+@pytest.mark.parametrize("lengths", [(17000011, 5000), (40000017, 3)])
+@pytest.mark.parametrize("prec,coded,page,d,heads", [("bfloat16", True, 1024, 64, 2), ("bfloat16", False, 1024, 128, 16), ("half", False, 1000, 64, 3), ("half", True, 1 << 16, 128, 1),
+                                                     ("single", False, 1000, 32, 2), ("single", True, 4096, 16, 9)])
+def test_sequences_of_millions_of_tokens(device, prec, coded, page, d, heads, lengths):
+    """More parts of a tile than are joined at once.  A table names one page throughout, so that the sums are known."""
+    rng = np.random.default_rng(page + d)
+    table = np.zeros((2, -(-max(lengths) // page) + 1), np.int64)
+    x = {"q": R.rounded(prec, rng.standard_normal((2, heads, d)))}
+    for g in "kv":
+        a = rng.standard_normal((1, 1, page, d))
+        if coded:
+            x[g + "_scale"] = np.full((1, 1), 2.0 ** R.exponent(np.abs(a).max()))
+            x[g + "_cache"] = R.encode(a / x[g + "_scale"][0, 0])
+        else:
+            x[g + "_cache"] = R.rounded(prec, a)
+    kv = [R.decode(x[g + "_cache"][0, 0]) * x[g + "_scale"][0, 0] if coded else x[g + "_cache"][0, 0] for g in "kv"]
+    nodes = attend_nodes(device, x, prec, table, np.array(lengths), None)
+    op = link_attend(nodes, x, None, {})
+    first = None
+    for _ in range(2):
+        op.run()
+        device.await_()
+        got, lse = nodes.read("out"), nodes.read("lse")
+        for b, n in enumerate(lengths):
+            want, want_lse, off, lse_off = repeated_page(x["q"][b], *kv, n, prec, coded, 1.0 / np.sqrt(d))
+            R.within(got[b], want, off, "out")
+            R.within(lse[b], want_lse, lse_off, "lse")
+        first = nodes.raw("out") if first is None else first
+        assert nodes.raw("out").tobytes() == first.tobytes()
+    op.free()
+    nodes.free()
