@@ -5,12 +5,12 @@
 //
 // A row is read once, and again from L2 in two or three more passes.  A cluster of up to eight blocks takes it and exchanges sums through
 // shared memory.  What is kept is all logits above a border and, of those equal to it, the ones up to an index: no sort of the row.  The border is found by a
-// histogram of 32 bins, half a binade of weight each, of counts and sums of weights; every lane has columns of its own, so that nothing is added atomically and
-// sums come out the same every time.  A bin that bounds what is kept, with all above it, is usually a few hundred logits: these go to one block, which
+// histogram of 32 bins, half a binade of weight each, of counts and sums of weights; every lane has columns of its own, so that nothing is added atomically, and
+// adds whole numbers, so that sums come out the same in whatever order and are exact but for a weight's own rounding.  A bin that bounds what is kept, with all above it, is usually a few hundred logits: these go to one block, which
 // sorts them and does the rest.  Where they are more than 1024, the bin is divided again by the bits of its logits, until it is small or of one value,
-// and the row is passed once more for the token.  Weights are summed in double precision beyond a lane's, so that borders lie where they do in 64 bits but
-// for 2^-22 of a weight.  Measured: 256 rows of 131072 logits 192 us, 64 of 50021 in bfloat16 40 us: bound by instructions and by the
-// blocks' waits for one another (the bytes alone: 20 us).
+// and the row is passed once more for the token.  A weight is
+// in single precision (some 2^-22 of it, more by the size of its exponent).  Measured: 256 rows of 131072 logits 240 us, 64 of 50021 in bfloat16 49 us: bound by
+// latency, three blocks an SM that wait for their logits' passes and for one another (the bytes alone: 20 us).
 #include <cooperative_groups.h>
 
 #include <cmath>
@@ -37,6 +37,12 @@ struct SampleArgs {
 };
 
 constexpr int kThreads = 256, kWarps = kThreads / 32, kBins = 32, kList = 1024, kLocal = 2 * kList, kMostParts = 8;
+
+// A column of a histogram is one 64-bit number: how many logits in its low bits, and above them the sum of their weights in steps of 2^-44 of the bin's unit.
+// Whole numbers do not care in which order they are added, and round only once, as a weight becomes one.
+constexpr int kCountBits = 10, kColumn = (1 << kCountBits) - 1, kFraction = 44;
+// a number between 0 and 1 in steps of 2^-44: the last bits of a sum with 256
+__device__ __forceinline__ unsigned long long fixed_of(double w) { return (unsigned long long)(__double_as_longlong(w + 256.0) - 0x4070000000000000ll); }
 
 // Rises with the value; one key for both zeros, as they are equal.  What is undefined lies outside the keys of -infinity and infinity.
 __device__ __forceinline__ unsigned int key_of(float x) {
@@ -108,14 +114,16 @@ struct Logits {
     }
   }
   static constexpr int kBatch = E ? E : kAtOnce * VEC;
+  // vectors of a lane that hold no more logits than a column of a histogram counts, a whole number of batches
+  static constexpr unsigned int kCounted = kColumn / kBatch * kAtOnce;
   // f(logits, index of each), kBatch at a time, which are under way together; -infinity ahead of the row and behind it, and where a lane has no more.  The
-  // lanes of a warp come here together.
+  // lanes of a warp come here together.  Of a lane's vectors those from v0 on, up to `end_v`.
   template <class F>
-  __device__ __forceinline__ void batches(F f) const {
+  __device__ __forceinline__ void batches(F f, unsigned int v0 = 0, unsigned int end_v = 0xffffffffu) const {
     if constexpr (E > 0) {
       f(x, [&](int e) { return begin + (e / VEC) * 32 * VEC + e % VEC - off; });
     } else {
-      for (unsigned int v = 0; v < count; v += kAtOnce) {
+      for (unsigned int v = v0; v < min(count, end_v); v += kAtOnce) {
         float y[kBatch];
         const unsigned int at = begin + v * 32 * VEC;
         Raw<T, VEC> r[kAtOnce];
@@ -143,11 +151,11 @@ struct Logits {
   }
   // f(logit, index), in the order of the indices of a lane
   template <class F>
-  __device__ __forceinline__ void each(F f) const {
+  __device__ __forceinline__ void each(F f, unsigned int v0 = 0, unsigned int end_v = 0xffffffffu) const {
     batches([&](const float(&y)[kBatch], auto index) {
 #pragma unroll
       for (int e = 0; e < kBatch; ++e) f(y[e], index(e));
-    });
+    }, v0, end_v);
   }
   // f(logits, index of the first): false ends it, for the whole warp
   template <class F>
@@ -279,7 +287,7 @@ __device__ __forceinline__ void sort_list(unsigned long long* list, unsigned int
 }
 template <class T, int E>
 __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __grid_constant__ SampleArgs a) {
-  extern __shared__ __align__(16) uint2 bins[];       // [warp][bin][lane]: sum of weights, count
+  extern __shared__ __align__(16) unsigned long long bins[];    // [warp][bin][lane]: columns of a histogram
   __shared__ Share sh;
   grid_begin();
   const unsigned int parts = a.parts, part = blockIdx.x % parts, row = blockIdx.x / parts, warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
@@ -361,52 +369,47 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
   const double share = fmax((double)top_p, 0.0);
 
   // the list that all blocks' entries go to, in the first one: where the histogram was
-  unsigned long long* const all_list = E > 0 ? sh.list : (unsigned long long*)bins;
+  unsigned long long* const all_list = E > 0 ? sh.list : bins;
 
   unsigned int histograms = 0;
   // a histogram of the kept logits that `over` passes on and `of` gives a bin (0: the highest); bins of all blocks, joined, in sh
-  // (`fresh`: nothing but -infinity has been left out yet)
-  auto histogram_of = [&](auto fresh, auto over, auto of) {
-    const unsigned int set = histograms++ & 1u;
-    for (unsigned int i = threadIdx.x; i < kWarps * kBins * 32 / 2; i += kThreads) ((uint4*)bins)[i] = make_uint4(0u, 0u, 0u, 0u);
-    __syncthreads();
-    uint2* mine = bins + warp * kBins * 32 + lane;
-    over([&](float x, unsigned int i) {
-      const float z = below(x), w = weight_at(z);
-      const int b = of(x, z);
-      if ((fresh.value ? x > -INFINITY : kept(x, i)) & ((unsigned int)b < (unsigned int)kBins)) {
-        uint2 v = mine[b * 32];
-        v.x = __float_as_uint(__uint_as_float(v.x) + w);
-        ++v.y;
-        mine[b * 32] = v;
-      }
-    });
-    __syncthreads();
-    // eight threads a bin, a warp's columns each
-    {
-      const unsigned int b = threadIdx.x / 8, w = threadIdx.x % 8;
-      double s = 0.0;
-      unsigned int n = 0;
+  // (`fresh`: nothing but -infinity has been left out yet; `weighed`: sums are wanted too; a bin's unit is 2^-unit(bin), no less than any of its weights)
+  auto histogram_of = [&](auto fresh, auto weighed, auto over, auto of, auto unit) {
+    const unsigned int set = histograms++ & 1u, b_mine = threadIdx.x / 8, w_mine = threadIdx.x % 8;
+    unsigned long long* mine = bins + warp * kBins * 32 + lane;
+    double s = 0.0;                    // eight threads a bin, a warp's columns each
+    unsigned int n = 0;
+    // (as many turns as it takes no column more than it counts; the same for all blocks)
+    for (unsigned int v0 = 0; v0 < a.span / (32 * VEC); v0 += Logits<T, E>::kCounted) {
+      __syncthreads();
+      for (unsigned int i = threadIdx.x; i < kWarps * kBins * 32 / 2; i += kThreads) ((uint4*)bins)[i] = make_uint4(0u, 0u, 0u, 0u);
+      __syncthreads();
+      const bool more = over(
+          [&](float x, unsigned int i) {
+            const float z = below(x);
+            const int b = of(x, z);
+            if ((fresh.value ? x > -INFINITY : kept(x, i)) & ((unsigned int)b < (unsigned int)kBins))
+              mine[b * 32] += weighed.value ? fixed_of((double)weight_at(z - (float)unit(b))) << kCountBits | 1u : 1u;
+          },
+          v0);
+      __syncthreads();
+      unsigned long long sum = 0;
 #pragma unroll 4
-      for (unsigned int i = 0; i < 32; i += 4) {
-        float some = 0.f;
-#pragma unroll
-        for (unsigned int k = 0; k < 4; ++k) {
-          const uint2 v = bins[(w * kBins + b) * 32 + ((i + k + threadIdx.x) & 31u)];
-          some += __uint_as_float(v.x);
-          n += v.y;
-        }
-        s += (double)some;
+      for (unsigned int i = 0; i < 32; ++i) {
+        const unsigned long long v = bins[(w_mine * kBins + b_mine) * 32 + ((i + threadIdx.x) & 31u)];
+        n += weighed.value ? (unsigned int)v & kColumn : (unsigned int)v;
+        sum += v >> kCountBits;
       }
 #pragma unroll
-      for (int o = 4; o > 0; o >>= 1) {
-        s += __shfl_xor_sync(0xffffffffu, s, o);
-        n += __shfl_xor_sync(0xffffffffu, n, o);
-      }
-      if (w == 0) {
-        sh.sums[set][b] = s;
-        sh.counts[set][b] = n;
-      }
+      for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (weighed.value) s += scalbn((double)sum, -kFraction - unit((int)b_mine));
+      if (!more) break;
+    }
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    if (w_mine == 0) {
+      sh.sums[set][b_mine] = s;
+      sh.counts[set][b_mine] = n;
     }
     meet(parts);
     if (threadIdx.x < kBins) {
@@ -428,11 +431,15 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
     }
     __syncthreads();                   // (this set of shares is written again two histograms on, with a meeting between)
   };
-  auto histogram = [&](auto over, auto of) {
-    if (border == -INFINITY) histogram_of(std::true_type(), over, of);
-    else histogram_of(std::false_type(), over, of);
+  auto histogram = [&](bool weighed, auto over, auto of, auto unit) {
+    if (border == -INFINITY) weighed ? histogram_of(std::true_type(), std::true_type(), over, of, unit) : histogram_of(std::true_type(), std::false_type(), over, of, unit);
+    else weighed ? histogram_of(std::false_type(), std::true_type(), over, of, unit) : histogram_of(std::false_type(), std::false_type(), over, of, unit);
   };
-  auto whole_row = [&](auto f) { logits.each(f); };
+  // f of the logits of a turn from a lane's vector v0 on; false: there are no more
+  auto whole_row = [&](auto f, unsigned int v0) {
+    logits.each(f, v0, v0 + Logits<T, E>::kCounted);
+    return true;
+  };
   // the count and the sum of all bins: a warp, a lane a bin
   auto everything = [&](unsigned int& n, double& s) {
     n = warp_join(sh.joined_counts[lane], add);
@@ -483,8 +490,9 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
     else gather_of(std::false_type(), of);
   };
   auto logit_at = [&](unsigned int i) { return to_float(logits.row[logits.off + i]); };
-  auto listed_logits = [&](auto f) {
+  auto listed_logits = [&](auto f, unsigned int) {
     for (unsigned int k = threadIdx.x; k < sh.listed; k += kThreads) f(logit_at(sh.local[k]), sh.local[k]);
+    return false;
   };
   // ... and those of the list that `of` accepts to the list of all blocks, kList in all
   auto send = [&](auto of) {
@@ -562,16 +570,24 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
     auto level_at = [&](float z) { return (int)min(__float_as_uint(fmaf(z, 2.f, 8388608.f)) - 0x4b000000u, (unsigned int)(kBins - 1)); };
     auto level = [&](float x) { return level_at(below(x)); };
     auto by_level = [&](float, float z) { return level_at(z); };
+    // (a bin's weights begin at 2^-(bin - 1/2) / 2, but for the last its own half binade)
+    auto level_unit = [](int b) { return max(b - 1, 0) >> 1; };
     Pick at = {0, 0, 0, 0.0};
     if (E > 0 || a.vocab <= kList) {
       gather([](float) { return true; });
       send([](float) { return true; });
       listed = true;
     } else {
-      histogram(whole_row, by_level);
       unsigned int n;
-      everything(n, total);
-      by_count = by_count && (unsigned int)top_k < n;
+      if (by_count) {
+        histogram(false, whole_row, by_level, level_unit);
+        everything(n, total);
+        by_count = (unsigned int)top_k < n;
+      }
+      if (!by_count && by_sum) {
+        histogram(true, whole_row, by_level, level_unit);
+        everything(n, total);
+      }
       if (by_count || by_sum) {
         at = find(by_count, by_count ? (double)top_k : share * total);
         if (at.above + at.in <= kList) {
@@ -647,7 +663,7 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
       double goal = (double)top_k;
       if (!counting) {
         if (by_count) {
-          histogram(whole_row, by_level);
+          histogram(true, whole_row, by_level, level_unit);
           unsigned int n;
           everything(n, total);
         }
@@ -692,8 +708,10 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
         int bits = 0;
         while ((hi - lo) >> bits >= kBins) ++bits;
         auto split = [&](float x, float) { return inside(x) ? (int)((hi - key_of(x)) >> bits) : -1; };
-        if (have) histogram(listed_logits, split);
-        else histogram(whole_row, split);
+        const int most = (int)fminf(below(of_key(hi)), 1e9f);
+        auto unit = [&](int) { return most; };
+        if (have) histogram(!counting, listed_logits, split, unit);
+        else histogram(!counting, whole_row, split, unit);
         at = find(counting, counting ? goal - above : goal - sum_above);
         above += at.above;
         sum_above += at.sum_above;

@@ -42,3 +42,32 @@ def test_zeros_are_the_largest(device, vocab, rows, prec):
     for given in (dict(top_k=50), dict(top_p=0.9), dict(top_k=1100, top_p=0.5, temperature=5.0), dict(min_p=0.5, temperature=0.5), dict(temperature=0.0)):
         given = {n: float(np.float32(v)) if n != "top_k" else v for n, v in given.items()}
         check_repeated(run_sample(device, prec, x, u, given), 5, rows, x, u, given)
+
+
+@pytest.mark.parametrize("vocab,rows,prec", [(131072, 3, "single"), (131072, 600, "bfloat16"), (1 << 24, 1, "single"), (3 << 22, 1, "half")])
+def test_one_logit_again_and_again_below_a_larger_one(device, vocab, rows, prec):
+    """The kept count is known: n is the least with 1 + (n - 1) w >= p (1 + (vocab - 1) w).  A random number of 1 takes the last kept one, which is
+    token n - 1, as equal logits are kept in the order of their indices."""
+    x = np.full((1, vocab), -0.37)
+    x[0, 0] = 0.0
+    x = R.rounded(prec, x)
+    w = np.exp(x[0, 1])
+    x, u = repeated(rows, x, np.ones(1))
+    for p in (0.3, 0.61, 0.9, 0.97):
+        p = float(np.float32(p))
+        need = (p * (1.0 + (vocab - 1) * w) - 1.0) / w
+        # (weights in steps of 2^-44 move the sums by vocab * 2^-45 at most, `need` by less than 2^24 * 2^-45 / w < 10^-6; sums in 64 bits by less still)
+        assert 0.001 < need % 1.0 < 0.999
+        tokens, _ = run_sample(device, prec, x, u, dict(top_p=p))
+        assert np.all(tokens == int(np.ceil(need))), (p, need, tokens[:4])
+
+
+def test_the_same_bits_every_time(device):
+    """Rows whose border is looked for in the blocks' lists, whose places are handed out in no order."""
+    rng = np.random.default_rng(77)
+    x, u = R.rounded("single", rng.standard_normal((40, 60000)) * 1.5), R.rounded("single", rng.random(40))
+    for given in (dict(top_p=float(np.float32(0.8))), dict(top_k=5000, top_p=0.5)):
+        first = run_sample(device, "single", x, u, given)
+        for _ in range(10):
+            again = run_sample(device, "single", x, u, given)
+            assert all(a.tobytes() == b.tobytes() for a, b in zip(first, again))
