@@ -6,11 +6,13 @@
 // A row is read once, and again from L2 in two or three more passes.  A cluster of up to eight blocks takes it and exchanges sums through
 // shared memory.  What is kept is all logits above a border and, of those equal to it, the ones up to an index: no sort of the row.  The border is found by a
 // histogram of 32 bins, half a binade of weight each, of counts and sums of weights; every lane has columns of its own, so that nothing is added atomically, and
-// adds whole numbers, so that sums come out the same in whatever order and are exact but for a weight's own rounding.  A bin that bounds what is kept, with all above it, is usually a few hundred logits: these go to one block, which
-// sorts them and does the rest.  Where they are more than 1024, the bin is divided again by the bits of its logits, until it is small or of one value,
-// and the row is passed once more for the token.  A weight is
-// in single precision (some 2^-22 of it, more by the size of its exponent).  Measured: 256 rows of 131072 logits 240 us, 64 of 50021 in bfloat16 49 us: bound by
-// latency, three blocks an SM that wait for their logits' passes and for one another (the bytes alone: 20 us).
+// adds whole numbers, so that sums come out the same in whatever order and are exact but for a weight's own rounding.  A bin that bounds what is kept, with all above
+// it, is usually a few hundred logits: these go to one block, which sorts them and does the rest in 64 bits.  Where they are more than 1024, the bin is divided
+// again by the bits of its logits, until it is small or of one value, and the row is passed once more for the token.
+// In the passes a weight is single (the exponential's 2^-22, and what its exponent's rounding makes: equal logits have equal weights, others' errors do not add up), with
+// the rate's rounding taken off, so that borders and tokens lie where 64 bits have them but for some 2^-10 of a weight in rows of 10^5 weights of one size.
+// Measured: 256 rows of 131072 logits 199 us, 64 of 50021 in bfloat16 43 us (in double precision throughout 312 and 55): 89 million instructions of warps at half of
+// the issue slots; three blocks an SM wait for their logits' passes and for one another (the bytes alone: 20 us).
 #include <cooperative_groups.h>
 
 #include <cmath>
@@ -38,11 +40,21 @@ struct SampleArgs {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32, kBins = 32, kList = 1024, kLocal = 2 * kList, kMostParts = 8;
 
-// A column of a histogram is one 64-bit number: how many logits in its low bits, and above them the sum of their weights in steps of 2^-44 of the bin's unit.
-// Whole numbers do not care in which order they are added, and round only once, as a weight becomes one.
-constexpr int kCountBits = 10, kColumn = (1 << kCountBits) - 1, kFraction = 44;
-// a number between 0 and 1 in steps of 2^-44: the last bits of a sum with 256
-__device__ __forceinline__ unsigned long long fixed_of(double w) { return (unsigned long long)(__double_as_longlong(w + 256.0) - 0x4070000000000000ll); }
+// A column of a histogram is two whole numbers, which do not care in which order they are added: the sum of weights in steps of 2^-22 of the bin's unit, and
+// what they were rounded by in steps of 2^-34 with the number of logits above it.  (Weights of a bin are below 1.25 of its unit, so 800 logits pass neither.)
+constexpr int kColumn = 800, kCountBits = 10;
+struct Column {
+  unsigned int sum, rest;
+  // w: in units of 2^-17 of the bin's.  A sum with 2^23 has the nearest whole number in its low bits; rests lie between -1/2 and 1/2 and are counted from there.
+  __device__ __forceinline__ void add(float w) {
+    const float whole = fmaf(w, 32.f, 8388608.f), left = fmaf(w, 32.f, 8388608.f - whole);
+    sum += __float_as_uint(whole) - 0x4b000000u;
+    rest += __float_as_uint(fmaf(left, 4096.f, 8388608.f + 2048.f)) - 0x4b000000u + (1u << (32 - kCountBits));
+  }
+  __device__ __forceinline__ unsigned int count() const { return rest >> (32 - kCountBits); }
+  // of `count` logits, in steps of 2^-34
+  __device__ __forceinline__ long long total() const { return ((long long)sum << 12) + (rest & ((1u << (32 - kCountBits)) - 1u)) - 2048ll * count(); }
+};
 
 // Rises with the value; one key for both zeros, as they are equal.  What is undefined lies outside the keys of -infinity and infinity.
 __device__ __forceinline__ unsigned int key_of(float x) {
@@ -287,7 +299,7 @@ __device__ __forceinline__ void sort_list(unsigned long long* list, unsigned int
 }
 template <class T, int E>
 __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __grid_constant__ SampleArgs a) {
-  extern __shared__ __align__(16) unsigned long long bins[];    // [warp][bin][lane]: columns of a histogram
+  extern __shared__ __align__(16) Column bins[];      // [warp][bin][lane]
   __shared__ Share sh;
   grid_begin();
   const unsigned int parts = a.parts, part = blockIdx.x % parts, row = blockIdx.x / parts, warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
@@ -296,6 +308,8 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
   const float temperature = a.temperatures ? a.temperatures[row] : a.temperature, top_p = a.top_ps ? a.top_ps[row] : a.top_p;
   const float min_p = fmaxf(a.min_ps ? a.min_ps[row] : a.min_p, 0.f), uniform = a.uniform[row];
   const int top_k = a.top_ks ? a.top_ks[row] : a.top_k;
+  // binades of weight of a logit (of short rows, while the logits are under way)
+  const double log2e = 1.4426950408889634, early_rate = E > 0 ? log2e / (double)temperature : 0.0;
   auto larger = [](auto u, auto v) { return u > v ? u : v; };
   auto smaller = [](auto u, auto v) { return u < v ? u : v; };
   auto add = [](auto u, auto v) { return u + v; };
@@ -345,19 +359,37 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
     meet(parts);
     return;
   }
-  // Binades below the largest weight.  (The rate is never zero, so that -infinity stays that, and never infinite, so that the largest has zero.)
-  const float rate = fminf(fmaxf((float)(1.4426950408889634 / (double)temperature), 1e-37f), 3e38f);
+  // Binades z below the largest weight: of a few logits in 64 bits, of whole rows in single precision, with what the rate was rounded by put onto the weight: it
+  // would move all of a row together against the largest.  (Differences are taken of logits halved where they could be infinite, and multiplied where
+  // temperatures are so small that rates could be.  Not of -infinity, which is left out everywhere.)
   const bool endless = top == INFINITY;
-  auto below = [&](float x) -> float {
-    if (endless) return x == top ? 0.f : INFINITY;        // (the same for all of a row)
-    return (top - x) * rate;
-  };
-  auto weight_at = [&](float z) -> float {
+  const float factor = top > 1e30f ? 0.5f : temperature < 1e-30f && fabsf(top) <= 1.f ? 1.2676506e30f : 1.f;      // (2^100)
+  const double top64 = (double)top, rate = E > 0 ? early_rate : log2e / (double)temperature;
+  const double rate_factor = endless ? 1.0 : fmin(factor == 1.f ? rate : factor < 1.f ? rate * 2.0 : rate * 7.888609052210118e-31, 3e38);
+  // (what a rate above 2^20 is rounded by is left out, where differences of 2^127 would not go with it)
+  const float rate_hi = (float)rate_factor, to_weight = rate_hi <= 1048576.f ? (float)(rate_factor - (double)rate_hi) * -0.69314718f : 0.f;
+  const float top_factor = endless ? 3.4028235e38f : top * factor;
+  // (where the largest is infinite: 0 for those, and 2^126 at least for all others)
+  auto difference = [&](float x) -> float { return fmaxf(fmaf(-x, factor, top_factor), 0.f); };
+  auto below = [&](float d) -> float { return __fmul_rn(d, rate_hi); };
+  // 2^-z for d's z
+  auto weight_at = [&](float d, float z) -> float {
     float w;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(-z));
-    return w;
+    return fmaf(w, d * to_weight, w);
   };
-  auto weight = [&](float x) -> float { return weight_at(below(x)); };
+  auto weight64 = [&](float x) -> double { return endless ? (x == top ? 1.0 : 0.0) : exp2(((double)x - top64) * rate); };
+
+  // the least logit whose weight is min_p: those below are not kept
+  float least = -INFINITY;
+  if (min_p > 0.f) {
+    least = top;
+    if (min_p < 1.f && !endless) {
+      const double at = top64 + log((double)min_p) * (double)temperature;
+      least = (float)at;
+      if ((double)least < at) least = of_key(key_of(least) + 1u);
+    }
+  }
 
   // ---- the border: kept are logits above it, and those equal to it up to an index
   float border = -INFINITY;
@@ -369,14 +401,14 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
   const double share = fmax((double)top_p, 0.0);
 
   // the list that all blocks' entries go to, in the first one: where the histogram was
-  unsigned long long* const all_list = E > 0 ? sh.list : bins;
+  unsigned long long* const all_list = E > 0 ? sh.list : (unsigned long long*)bins;
 
   unsigned int histograms = 0;
   // a histogram of the kept logits that `over` passes on and `of` gives a bin (0: the highest); bins of all blocks, joined, in sh
-  // (`fresh`: nothing but -infinity has been left out yet; `weighed`: sums are wanted too; a bin's unit is 2^-unit(bin), no less than any of its weights)
-  auto histogram_of = [&](auto fresh, auto weighed, auto over, auto of, auto unit) {
+  // (`fresh`: nothing but -infinity has been left out yet; `weighed`: sums are wanted too; a bin's unit is 2^-unit(bin), its weights are below 1.25 of it; scale_of(bin): 2^17 / unit)
+  auto histogram_of = [&](auto fresh, auto weighed, auto over, auto of, auto unit, auto scale_of) {
     const unsigned int set = histograms++ & 1u, b_mine = threadIdx.x / 8, w_mine = threadIdx.x % 8;
-    unsigned long long* mine = bins + warp * kBins * 32 + lane;
+    Column* mine = bins + warp * kBins * 32 + lane;
     double s = 0.0;                    // eight threads a bin, a warp's columns each
     unsigned int n = 0;
     // (as many turns as it takes no column more than it counts; the same for all blocks)
@@ -386,23 +418,29 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
       __syncthreads();
       const bool more = over(
           [&](float x, unsigned int i) {
-            const float z = below(x);
+            const float d = difference(x), z = below(d);
             const int b = of(x, z);
-            if ((fresh.value ? x > -INFINITY : kept(x, i)) & ((unsigned int)b < (unsigned int)kBins))
-              mine[b * 32] += weighed.value ? fixed_of((double)weight_at(z - (float)unit(b))) << kCountBits | 1u : 1u;
+            // (without branches, but for the last store)
+            const unsigned int at = min((unsigned int)b, (unsigned int)kBins - 1u);
+            Column v = mine[at * 32];
+            if (weighed.value) v.add(weight_at(d, z) * scale_of((int)at));
+            else ++v.sum;
+            if ((fresh.value ? x > -INFINITY : kept(x, i)) & ((unsigned int)b < (unsigned int)kBins)) mine[at * 32] = v;
           },
           v0);
       __syncthreads();
-      unsigned long long sum = 0;
+      long long sum = 0;
 #pragma unroll 4
       for (unsigned int i = 0; i < 32; ++i) {
-        const unsigned long long v = bins[(w_mine * kBins + b_mine) * 32 + ((i + threadIdx.x) & 31u)];
-        n += weighed.value ? (unsigned int)v & kColumn : (unsigned int)v;
-        sum += v >> kCountBits;
+        const Column v = bins[(w_mine * kBins + b_mine) * 32 + ((i + threadIdx.x) & 31u)];
+        n += weighed.value ? v.count() : v.sum;
+        if (weighed.value) sum += v.total();
       }
+      if (weighed.value) {
 #pragma unroll
-      for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (weighed.value) s += scalbn((double)sum, -kFraction - unit((int)b_mine));
+        for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        s += scalbn((double)sum, -34 - unit((int)b_mine));
+      }
       if (!more) break;
     }
 #pragma unroll
@@ -431,9 +469,9 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
     }
     __syncthreads();                   // (this set of shares is written again two histograms on, with a meeting between)
   };
-  auto histogram = [&](bool weighed, auto over, auto of, auto unit) {
-    if (border == -INFINITY) weighed ? histogram_of(std::true_type(), std::true_type(), over, of, unit) : histogram_of(std::true_type(), std::false_type(), over, of, unit);
-    else weighed ? histogram_of(std::false_type(), std::true_type(), over, of, unit) : histogram_of(std::false_type(), std::false_type(), over, of, unit);
+  auto histogram = [&](bool weighed, auto over, auto of, auto unit, auto scale_of) {
+    if (border == -INFINITY) weighed ? histogram_of(std::true_type(), std::true_type(), over, of, unit, scale_of) : histogram_of(std::true_type(), std::false_type(), over, of, unit, scale_of);
+    else weighed ? histogram_of(std::false_type(), std::true_type(), over, of, unit, scale_of) : histogram_of(std::false_type(), std::false_type(), over, of, unit, scale_of);
   };
   // f of the logits of a turn from a lane's vector v0 on; false: there are no more
   auto whole_row = [&](auto f, unsigned int v0) {
@@ -531,13 +569,13 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
   };
   auto logit_of = [&](unsigned long long entry) { return of_key(~(unsigned int)(entry >> 32)); };
   // The first n of the sorted list that reach a goal, by count or by sum: each thread has four entries.  `ahead`: the sum ahead of the list
-  auto weights_of = [&](unsigned int n, float (&w)[4]) {
+  auto weights_of = [&](unsigned int n, double (&w)[4]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = threadIdx.x * 4 + i < n ? weight(logit_of(all_list[threadIdx.x * 4 + i])) : 0.f;
-    return ((double)w[0] + w[1]) + ((double)w[2] + w[3]);
+    for (int i = 0; i < 4; ++i) w[i] = threadIdx.x * 4 + i < n ? weight64(logit_of(all_list[threadIdx.x * 4 + i])) : 0.0;
+    return (w[0] + w[1]) + (w[2] + w[3]);
   };
   auto reach = [&](unsigned int n, double ahead, double goal) {
-    float w[4];
+    double w[4];
     double all;
     const double own = weights_of(n, w);
     double up_to = ahead + block_before(own, sh.block_sums, all);
@@ -557,7 +595,7 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
     return max(found, 1u);
   };
   auto sum_of = [&](unsigned int n) {
-    float w[4];
+    double w[4];
     double all;
     block_before(weights_of(n, w), sh.block_sums, all);
     return all;
@@ -568,10 +606,10 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
     double total = 0.0;                // of all logits' weights
     // (half a binade a bin, rounded to the nearest by an addition)
     auto level_at = [&](float z) { return (int)min(__float_as_uint(fmaf(z, 2.f, 8388608.f)) - 0x4b000000u, (unsigned int)(kBins - 1)); };
-    auto level = [&](float x) { return level_at(below(x)); };
+    auto level = [&](float x) { return level_at(below(difference(x))); };
     auto by_level = [&](float, float z) { return level_at(z); };
-    // (a bin's weights begin at 2^-(bin - 1/2) / 2, but for the last its own half binade)
-    auto level_unit = [](int b) { return max(b - 1, 0) >> 1; };
+    auto level_unit = [](int b) { return b >> 1; };       // (z >= bin / 2 - 1/4)
+    auto level_scale = [](int b) { return __uint_as_float(((unsigned int)b << 22 & 0x07800000u) | 0x48000000u); };
     Pick at = {0, 0, 0, 0.0};
     if (E > 0 || a.vocab <= kList) {
       gather([](float) { return true; });
@@ -580,12 +618,12 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
     } else {
       unsigned int n;
       if (by_count) {
-        histogram(false, whole_row, by_level, level_unit);
+        histogram(false, whole_row, by_level, level_unit, level_scale);
         everything(n, total);
         by_count = (unsigned int)top_k < n;
       }
       if (!by_count && by_sum) {
-        histogram(true, whole_row, by_level, level_unit);
+        histogram(true, whole_row, by_level, level_unit, level_scale);
         everything(n, total);
       }
       if (by_count || by_sum) {
@@ -605,7 +643,7 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
       sort_list(all_list, n);
       if (by_count) n = min(n, (unsigned int)top_k);
       if (by_sum) n = reach(n, 0.0, share * (by_count || E > 0 || a.vocab <= kList ? sum_of(n) : total));
-      float w[4];
+      double w[4];
       weights_of(n, w);
       // those above the least weight; in the order of the indices
       unsigned int here = 0;
@@ -614,7 +652,7 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
       for (int i = 0; i < 4; ++i) {
         const unsigned int k = threadIdx.x * 4 + i;
         entry[i] = k < n ? all_list[k] : 0ull;
-        const bool on = k < n && w[i] > 0.f && (w[i] >= min_p || logit_of(entry[i]) == top);
+        const bool on = k < n && w[i] > 0.0 && logit_of(entry[i]) >= least;
         entry[i] = on ? entry[i] << 32 | entry[i] >> 32 : ~0ull;
         here += on;
       }
@@ -633,7 +671,7 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const unsigned int k = threadIdx.x * 4 + i;
-        w[i] = k < here ? weight(of_key(~(unsigned int)all_list[k])) : 0.f;
+        w[i] = k < here ? weight64(of_key(~(unsigned int)all_list[k])) : 0.0;
         up_to += w[i];
       }
       up_to = block_before(up_to, sh.block_sums, all);
@@ -653,7 +691,7 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
         for (int i = 0; i < kWarps; ++i) found = min(found, sh.warp_counts[i]);
         const unsigned long long e = all_list[found];
         a.tokens[row] = (int)(unsigned int)(e >> 32);
-        if (a.logprob) a.logprob[row] = (float)log((double)weight(of_key(~(unsigned int)e)) / all);
+        if (a.logprob) a.logprob[row] = (float)log(weight64(of_key(~(unsigned int)e)) / all);
       }
       return;
     }
@@ -663,7 +701,7 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
       double goal = (double)top_k;
       if (!counting) {
         if (by_count) {
-          histogram(true, whole_row, by_level, level_unit);
+          histogram(true, whole_row, by_level, level_unit, level_scale);
           unsigned int n;
           everything(n, total);
         }
@@ -689,11 +727,8 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
       unsigned int above = at.above;
       double sum_above = at.sum_above;
       bool have = false;               // the blocks' lists hold the interval
-      // (by keys, as the bins are, so that what is inside has one)
-      auto inside = [&](float x) {
-        const unsigned int k = key_of(x);
-        return (k >= lo) & (k <= hi);
-      };
+      // (no logit has the key of -0, so that an interval may end ahead of it: then, and only then, floats lie inside where their keys do)
+      auto inside = [&](float x) { return (x >= of_key(lo)) & (x <= of_key(hi)); };
       for (;;) {
         // (where the lists are likely to hold it; an uneven row is passed again)
         if (!have && (at.in <= kList || (lo < hi && at.in <= kLocal * parts / 4 * 3))) {
@@ -708,16 +743,17 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
         int bits = 0;
         while ((hi - lo) >> bits >= kBins) ++bits;
         auto split = [&](float x, float) { return inside(x) ? (int)((hi - key_of(x)) >> bits) : -1; };
-        const int most = (int)fminf(below(of_key(hi)), 1e9f);
+        const int most = (int)fminf(below(difference(of_key(hi))), 100.f);     // (weights from 2^-126 on are 0)
         auto unit = [&](int) { return most; };
-        if (have) histogram(!counting, listed_logits, split, unit);
-        else histogram(!counting, whole_row, split, unit);
+        auto scale_of = [&](int) { return __uint_as_float(((unsigned int)most << 23) + 0x48000000u); };
+        if (have) histogram(!counting, listed_logits, split, unit, scale_of);
+        else histogram(!counting, whole_row, split, unit, scale_of);
         at = find(counting, counting ? goal - above : goal - sum_above);
         above += at.above;
         sum_above += at.sum_above;
         const unsigned int cut = hi - (at.bin << bits);
         lo = cut - lo < (1u << bits) ? lo : cut - (1u << bits) + 1;
-        hi = cut;
+        hi = cut - (cut == 0x7fffffffu);
       }
       if (at.in <= kList) {
         send(inside);
@@ -739,7 +775,8 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
       } else {
         // many equal ones: as many as are wanted of them, in the order of their indices
         const float value = of_key(lo);
-        const double w = (double)weight(value), need = counting ? goal - above : w > 0.0 ? ceil((goal - sum_above) / w) : 1.0;
+        const float d = difference(value);
+        const double w = (double)weight_at(d, below(d)), need = counting ? goal - above : w > 0.0 ? ceil((goal - sum_above) / w) : 1.0;
         unsigned int want = need < 1.0 ? 1u : need > (double)at.in ? at.in : (unsigned int)need, ties = 0;
         logits.each([&](float x, unsigned int i) { ties += x == value && kept(x, i); });
         ties = warp_join(ties, add);
@@ -774,16 +811,26 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
   }
 
   // ---- the token: in which warp the running sum passes the goal, then where in it
+  if (least > border) {
+    const unsigned int k = key_of(least) - 1u;
+    border = of_key(k - (k == 0x7fffffffu));             // (not -0, which equals 0)
+    border_to = 0;
+  }
   auto chance = [&](float x, unsigned int i) -> float {
-    const float w = weight(x);
-    return kept(x, i) & ((w >= min_p) | (x == top)) ? w : 0.f;
+    const float d = difference(x), w = weight_at(d, below(d));
+    return kept(x, i) ? w : 0.f;
   };
   double mine = 0.0;
   logits.batches([&](const auto& y, auto index) {
-    float some = 0.f;
+    // (by halves, which adds equal weights exactly)
+    float some[Logits<T, E>::kBatch];
 #pragma unroll
-    for (int e = 0; e < Logits<T, E>::kBatch; ++e) some += chance(y[e], index(e));
-    mine += (double)some;
+    for (int e = 0; e < Logits<T, E>::kBatch; ++e) some[e] = chance(y[e], index(e));
+#pragma unroll
+    for (int h = Logits<T, E>::kBatch / 2; h > 0; h >>= 1)
+#pragma unroll
+      for (int e = 0; e < h; ++e) some[e] += some[e + h];
+    mine += (double)some[0];
   });
   mine = warp_join(mine, add);
   if (lane == 0) sh.warp_sums[warp] = mine;
@@ -806,7 +853,6 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
   const bool owner = part * kWarps + warp == which;
   if (owner) {
     unsigned int last = 0xffffffffu, found = 0xffffffffu;
-    float last_w = 0.f, found_w = 0.f;
     logits.each_vector([&](const float(&y)[VEC], unsigned int first) {
       double own = 0.0;
       float w[VEC];
@@ -814,7 +860,7 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
       for (int i = 0; i < VEC; ++i) {
         w[i] = chance(y[i], first + i);
         own += (double)w[i];
-        if (w[i] > 0.f) last = first + i, last_w = w[i];
+        if (w[i] > 0.f) last = first + i;
       }
       const double up_to = warp_up_to(own), all = __shfl_sync(0xffffffffu, up_to, 31);
       if (before + all > goal) {
@@ -822,23 +868,22 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
           s += (double)w[i];
-          if (found == 0xffffffffu && w[i] > 0.f && s > goal) found = first + i, found_w = w[i];
+          if (found == 0xffffffffu && w[i] > 0.f && s > goal) found = first + i;
         }
         if (__any_sync(0xffffffffu, found != 0xffffffffu)) return false;
       }
       before += all;
       return true;
     });
-    unsigned int least = warp_join(found, smaller);
-    if (least == 0xffffffffu) {
+    unsigned int chosen = warp_join(found, smaller);
+    if (chosen == 0xffffffffu) {
       // (rounding: the last of the warp)
-      least = warp_join(last == 0xffffffffu ? 0u : last + 1u, larger) - 1u;
+      chosen = warp_join(last == 0xffffffffu ? 0u : last + 1u, larger) - 1u;
       found = last;
-      found_w = last_w;
     }
-    if (found == least) {
+    if (found == chosen) {
       a.tokens[row] = (int)found;
-      if (a.logprob) a.logprob[row] = (float)log((double)found_w / total);
+      if (a.logprob) a.logprob[row] = (float)log(weight64(logit_at(found)) / total);
     }
   }
   meet(parts);

@@ -71,3 +71,42 @@ def test_the_same_bits_every_time(device):
         for _ in range(10):
             again = run_sample(device, "single", x, u, given)
             assert all(a.tobytes() == b.tobytes() for a, b in zip(first, again))
+
+
+@pytest.mark.parametrize("prec", PRECS)
+def test_borders_lie_where_64_bits_have_them(device, prec):
+    """Rows in falling order and a random number of 1: the token is the last kept one, the border itself."""
+    rng = np.random.default_rng(91)
+    rows, vocab = 24, 131072
+    x = -np.sort(-rng.standard_normal((rows, vocab)) * np.linspace(0.3, 4.0, rows)[:, None], 1)
+    x, u = R.rounded(prec, x), np.ones(rows)
+    single = {"temperature": rng.uniform(0.6, 1.5, rows), "top_p": rng.uniform(0.2, 0.995, rows), "min_p": 10.0 ** rng.uniform(-4, -1, rows)}
+    single = {n: R.rounded("single", v) for n, v in single.items()}
+    for given in (dict(single, min_p=0.0), dict(single, top_p=1.0), dict(single, top_k=rng.integers(10000, 100000, rows), min_p=0.0)):
+        check_sample(run_sample(device, prec, x, u, given), x, u, given)
+
+
+@pytest.mark.parametrize("prec", PRECS)
+def test_tokens_of_flat_rows(device, prec):
+    """A hundred thousand tokens of nearly equal weights: running sums that are off by a few millionths would choose others."""
+    rng = np.random.default_rng(92)
+    rows, vocab = 120, 100003
+    x = np.repeat(R.rounded(prec, rng.standard_normal((1, vocab)) * 2.0), rows, 0)
+    u = R.rounded("single", rng.random(rows))
+    for given in (dict(temperature=float(np.float32(3.3))), dict(top_p=float(np.float32(0.93)))):
+        check_sample(run_sample(device, prec, x, u, given), x, u, given)
+
+
+def test_differences_and_temperatures_at_the_ends(device):
+    """Logits whose difference single precision cannot hold, temperatures from the least number to infinity."""
+    x = np.tile(R.rounded("single", np.array([3e38, -3e38, 1e38, 0.0, -1e38, 2.9e38, 2e38])), (8, 1))
+    x[4:] = R.rounded("single", np.array([0.0, -1e-38, -3e-39, 1e-45, -1.0, -0.0, -2e-38]))
+    t = R.rounded("single", np.array([1e38, 3e38, 2e37, 1e30, 1e-45, 1e-38, 3e-39, 1.0]))
+    for u in (0.0, 0.3, 0.6, 0.9, 1.0):
+        u = R.rounded("single", np.full(8, u))
+        for given in (dict(temperature=t), dict(temperature=t, top_p=float(np.float32(0.7))), dict(temperature=t, top_k=3), dict(temperature=t, min_p=float(np.float32(0.05)))):
+            check_sample(run_sample(device, "single", x, u, given), x, u, given)
+    x = np.tile(x[:4], (1, 400))                      # rows of several blocks' passes
+    u, t = R.rounded("single", np.array([0.1, 0.4, 0.7, 1.0])), t[:4]
+    for given in (dict(temperature=t, top_p=float(np.float32(0.7))), dict(temperature=t, top_k=1500), dict(temperature=np.full(4, np.inf))):
+        check_sample(run_sample(device, "single", x, u, given), x, u, given)
