@@ -295,9 +295,9 @@ int b200_attention_grad_link(b200_dev* dev, const b200_attention* spec, b200_ope
  * Sequence b's tokens i * page .. (i + 1) * page - 1 lie in page page_table[b, i]; a number outside 0 .. pages - 1 is no page: nothing is written there
  * and nobody sees its tokens (as with pages given back behind a window).  lengths[b] counts a sequence's tokens, the new ones included
  * (negative: 0); tokens behind max_pages pages are not kept.  New tokens are rows of packed nodes: sequence b has rows starts[b] .. starts[b + 1] - 1
- * (numbers taken between 0 and `tokens`, not falling), or, without starts, tokens / batch rows each.  Row i of n lies at position lengths[b] - n + i,
- * and nowhere where that is negative.  Rows of no sequence are left as they were.  The table may name a page more than once, but for those that a
- * call of cache_append writes. */
+ * (numbers taken between 0 and `tokens`, not falling; where they fall, a run may take rows twice or leave them), or, without starts, tokens / batch
+ * rows each.  Row i of n lies at position lengths[b] - n + i, and nowhere where that is negative.  Rows of no sequence are left as they were.  The
+ * table may name a page more than once, but for those that a call of cache_append writes. */
 #define B200_E4M3 3
 typedef struct {
   int64_t batch, tokens;

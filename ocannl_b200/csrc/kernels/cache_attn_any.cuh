@@ -212,7 +212,7 @@ __global__ void __launch_bounds__(kCacheFewThreads) cache_attention_any(const __
     __threadfence();
     __syncthreads();
     if (threadIdx.x == 0) {
-      last_block = atomicAdd(&f.tickets[plan.first_block], 1u) == plan.parts - 1u;
+      last_block = plan.meets && atomicAdd(&f.tickets[plan.first_block], 1u) == plan.parts - 1u;
       if (last_block) f.tickets[plan.first_block] = 0u;        // for the next run
     }
     __syncthreads();

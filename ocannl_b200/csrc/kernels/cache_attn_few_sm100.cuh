@@ -108,6 +108,7 @@ struct CachePiece {
   int sink_end, shift;                 // the walk: tokens 0 .. sink_end - 1, then those from sink_end + shift on
   int begin, stop;                     // of the walk, this piece's
   unsigned int parts, part, first_block;     // of the tile
+  bool meets;                          // all its parts' blocks are in the grid (starts that fall may ask for more: such a tile is left, and takes no tickets)
   __device__ __forceinline__ int token_of(int v) const { return v < sink_end ? v : v + shift; }
 };
 // a part's place: of the tile that begins in `first_block`
@@ -250,11 +251,13 @@ __device__ __forceinline__ bool cache_piece(const CacheAttnArgs& a, const CacheF
   piece.parts = 1;
   piece.part = 0;
   piece.first_block = blockIdx.x;
+  piece.meets = true;
   if (take < p.walk.length) {
     const unsigned long long from = p.ahead + (unsigned long long)p.tile * p.walk.length;
     piece.first_block = (unsigned int)quotient(from, p.quota);
     piece.parts = (unsigned int)quotient(from + p.walk.length - 1, p.quota) - piece.first_block + 1;
     piece.part = blockIdx.x - piece.first_block;
+    piece.meets = (unsigned long long)piece.first_block + piece.parts <= gridDim.x;
   }
   return true;
 }
@@ -824,7 +827,7 @@ __global__ void __launch_bounds__(kCacheFewThreads, (CacheFewShape<DP, CODED, NR
     __threadfence();
     __syncthreads();
     if (threadIdx.x == 0) {
-      last_block = atomicAdd(&f.tickets[plan.first_block], 1u) == plan.parts - 1u;
+      last_block = plan.meets && atomicAdd(&f.tickets[plan.first_block], 1u) == plan.parts - 1u;
       if (last_block) f.tickets[plan.first_block] = 0u;       // for the next run
     }
     __syncthreads();

@@ -56,3 +56,40 @@ def test_sequences_of_millions_of_tokens(device, prec, coded, page, d, heads, le
         assert nodes.raw("out").tobytes() == first.tobytes()
     op.free()
     nodes.free()
+
+
+@pytest.mark.parametrize("prec,coded,d", [("bfloat16", True, 128), ("half", True, 128), ("single", False, 64)])
+def test_starts_that_fall_spoil_no_later_run(device, prec, coded, d):
+    """What a run writes for them is not defined, but the runs behind it are as ever: no tile waits for parts of an earlier run.  (With three blocks on each of 148
+    SMs, 444, the 32 tiles of 914432 tokens that falling starts make ask for 447, and the last of them begins in block 432; so does the last of eight
+    tiles whose lengths are those below.)"""
+    rng = np.random.default_rng(21)
+    batch, n, page, width = 64, 8, 1024, 893
+    x = {"q": R.rounded(prec, rng.standard_normal((n, 1, d)))}
+    for g in "kv":
+        a = rng.standard_normal((1, 1, page, d))
+        if coded:
+            x[g + "_scale"] = np.full((1, 1), 2.0 ** R.exponent(np.abs(a).max()))
+            x[g + "_cache"] = R.encode(a / x[g + "_scale"][0, 0])
+        else:
+            x[g + "_cache"] = R.rounded(prec, a)
+    kv = [R.decode(x[g + "_cache"][0, 0]) * x[g + "_scale"][0, 0] if coded else x[g + "_cache"][0, 0] for g in "kv"]
+    most = page * width
+    fine, falling = np.minimum(np.arange(batch + 1), n), np.where(np.arange(batch + 1) % 2, n, 0)
+    lengths = np.full(batch, most)
+    lengths[0], lengths[7] = most - 6400, 64 * 2300
+    nodes = attend_nodes(device, x, prec, np.zeros((batch, width), np.int64), lengths, fine)
+    op = link_attend(nodes, x, fine, {})
+    for starts in (fine, falling, fine, fine):
+        nodes.write("starts", starts)
+        nodes.write("lengths", lengths if starts is fine else np.full(batch, most))
+        nodes.write("out", np.full(x["q"].shape, np.nan))
+        op.run()
+        device.await_()
+        if starts is fine:
+            for b in range(n):
+                out, lse, off, lse_off = repeated_page(x["q"][b], *kv, int(lengths[b]), prec, coded, 1.0 / np.sqrt(d))
+                R.within(nodes.read("out")[b], out, off, "out")
+                R.within(nodes.read("lse")[b], lse, lse_off, "lse")
+    op.free()
+    nodes.free()
