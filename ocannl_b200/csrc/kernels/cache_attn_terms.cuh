@@ -26,7 +26,8 @@ constexpr float kCacheLog2e = 1.4426950408889634f, kCacheLn2 = 0.693147180559945
 __device__ __forceinline__ int cache_last(const CacheAttnArgs& a, int pos) {
   return (int)min((long long)pos, (long long)a.c.max_pages * a.c.page - 1);
 }
-__device__ __forceinline__ int cache_first(const CacheAttnArgs& a, int pos) { return a.window ? max(pos - a.window + 1, 0) : 0; }
+// (positions ahead of the first token less a window of nearly 2^31 would pass 32 bits)
+__device__ __forceinline__ int cache_first(const CacheAttnArgs& a, int pos) { return a.window ? max(max(pos, 0) - a.window + 1, 0) : 0; }
 
 // a scale as the arithmetic takes it (what lies outside the range that codes are written with would not fit the weights)
 __device__ __forceinline__ float cache_scale(float s) {

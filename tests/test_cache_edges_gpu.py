@@ -1,9 +1,9 @@
-"""Attention over a paged cache at the ends of its range: sequences of tens of millions of tokens."""
+"""Attention over a paged cache at the ends of its range: sequences of tens of millions of tokens and of 2^31, starts that fall, the widest windows."""
 import numpy as np
 import pytest
 
 from tests import serving_reference as R
-from tests.test_serving_gpu import attend_nodes, link_attend
+from tests.test_serving_gpu import attend_nodes, check_attend, link_attend, want_attend
 
 pytestmark = pytest.mark.gpu
 
@@ -91,5 +91,23 @@ def test_starts_that_fall_spoil_no_later_run(device, prec, coded, d):
                 out, lse, off, lse_off = repeated_page(x["q"][b], *kv, int(lengths[b]), prec, coded, 1.0 / np.sqrt(d))
                 R.within(nodes.read("out")[b], out, off, "out")
                 R.within(nodes.read("lse")[b], lse, lse_off, "lse")
+    op.free()
+    nodes.free()
+
+
+@pytest.mark.parametrize("prec,coded", [("single", False), ("half", True), ("bfloat16", False)])
+@pytest.mark.parametrize("window", [2 ** 31 - 2, 2 ** 31 - 1, 2 ** 62])
+@pytest.mark.parametrize("case", [(1, 8, [3], 16, 1, 4, 64), (2, [300, 200], [200, 210], 64, 1, 16, 64)])
+def test_the_widest_windows(device, case, window, prec, coded):
+    """... beside rows that lie ahead of the first token, which see nothing."""
+    from tests.test_serving_gpu import attend_case
+    x, table, lengths, starts, page, t = attend_case(case + (0, 0, 0.0, False), prec, coded)
+    t = dict(t, window=window)
+    want = want_attend(x, table, lengths, starts, page, prec, t)
+    nodes = attend_nodes(device, x, prec, table, lengths, starts)
+    op = link_attend(nodes, x, starts, t)
+    op.run()
+    device.await_()
+    check_attend(nodes, want)
     op.free()
     nodes.free()
