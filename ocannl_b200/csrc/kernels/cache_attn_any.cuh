@@ -51,13 +51,14 @@ __global__ void __launch_bounds__(kCacheFewThreads) cache_attention_any(const __
     slope[k] = a.slopes ? a.slopes[head_of(r)] : 0.f;
   }
   float o[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-  for (int v0 = plan.begin; v0 < plan.stop; v0 += kAnyTokens) {
+  for (unsigned int v0 = (unsigned int)plan.begin; v0 < (unsigned int)plan.stop; v0 += kAnyTokens) {      // (of up to 2^31 - 1 tokens: signed numbers would not end)
     __syncthreads();
     if (threadIdx.x < kAnyTokens) {
-      const int v = v0 + (int)threadIdx.x, j = plan.token_of(v);
+      const unsigned int v = v0 + threadIdx.x;
+      const int j = v < (unsigned int)plan.stop ? plan.token_of((int)v) : plan.end;
       long long place = -1;
       float ks = 0.f, vs = 0.f;
-      if (v < plan.stop && j < plan.end) {
+      if (j < plan.end) {
         const unsigned int index = c.by_page.of((unsigned int)j);
         const int page = cache_page_at(c, part.b, index);
         if (page >= 0) {
@@ -128,7 +129,7 @@ __global__ void __launch_bounds__(kCacheFewThreads) cache_attention_any(const __
 #pragma unroll
       for (int i = 0; i < 2; ++i) s[i] = (sum[i].x + sum[i].y) + (sum[i].z + sum[i].w);
     }
-    const int j = plan.token_of(v0 + (int)lane);
+    const int j = places[lane] >= 0 ? plan.token_of((int)(v0 + lane)) : 0;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       s[i] = a.cap > 0.f ? tanhf(s[i] * a.over) * a.cap : s[i] * a.scale;

@@ -115,7 +115,7 @@ cache_attention_tc(const __grid_constant__ b200_tmap map_q, const __grid_constan
     sink_end = (int)min(((long long)min(a.sinks, max(end, 0)) + 63) & ~63ll, 0x7fffffc0ll);
     shift = max((cache_first(a, least_pos) & ~63) - sink_end, 0);
   }
-  const int n_tokens = shift ? max(end - shift, sink_end) : max(end, 0), n_tiles = n_new ? (n_tokens + 63) / 64 : 0;
+  const int n_tokens = shift ? max(end - shift, sink_end) : max(end, 0), n_tiles = n_new ? n_tokens / 64 + (n_tokens % 64 != 0) : 0;
   auto token_of = [&](int t) { return t * 64 < sink_end ? t * 64 : t * 64 + shift; };
   // what row tile i sees of a tile of tokens: 0 nothing, 1 everything (pages aside), 2 some
   auto class_of = [&](int t, int i) -> unsigned int {

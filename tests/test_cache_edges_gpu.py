@@ -95,6 +95,60 @@ def test_starts_that_fall_spoil_no_later_run(device, prec, coded, d):
     nodes.free()
 
 
+def one_page(rng, prec, coded, page, d):
+    """A cache of one page, and its values."""
+    x, kv = {}, []
+    for g in "kv":
+        a = rng.standard_normal((1, 1, page, d))
+        if coded:
+            x[g + "_scale"] = np.full((1, 1), 2.0 ** R.exponent(np.abs(a).max()))
+            x[g + "_cache"] = R.encode(a / x[g + "_scale"][0, 0])
+        else:
+            x[g + "_cache"] = R.rounded(prec, a)
+        kv.append(R.decode(x[g + "_cache"][0, 0]) * x[g + "_scale"][0, 0] if coded else x[g + "_cache"][0, 0])
+    return x, kv
+
+
+@pytest.mark.parametrize("prec,coded,d", [("single", False, 1), ("half", True, 3), ("bfloat16", False, 8), ("half", True, 16)])
+def test_as_many_tokens_as_there_are_positions(device, prec, coded, d):
+    """2^31 - 1 tokens, and a few less, all of them seen."""
+    rng = np.random.default_rng(d)
+    page, lengths = 1 << 20, (2 ** 31 - 1, 2 ** 31 - 34)
+    x, kv = one_page(rng, prec, coded, page, d)
+    x["q"] = R.rounded(prec, rng.standard_normal((2, 2, d)))
+    nodes = attend_nodes(device, x, prec, np.zeros((2, 2048), np.int64), np.array(lengths), None)
+    op = link_attend(nodes, x, None, {})
+    op.run()
+    device.await_()
+    for b, n in enumerate(lengths):
+        out, lse, off, lse_off = repeated_page(x["q"][b], *kv, n, prec, coded, 1.0 / np.sqrt(d))
+        R.within(nodes.read("out")[b], out, off, "out")
+        R.within(nodes.read("lse")[b], lse, lse_off, "lse")
+    op.free()
+    nodes.free()
+
+
+@pytest.mark.parametrize("prec,coded,new,heads,d", [("single", False, 5, 3, 20), ("half", True, 3, 4, 64), ("bfloat16", False, 300, 16, 64), ("bfloat16", True, 300, 32, 32)])
+def test_windows_at_the_last_positions(device, prec, coded, new, heads, d):
+    rng = np.random.default_rng(new)
+    page, length, window = 4096, 2 ** 31 - 1, 500
+    x, (k, v) = one_page(rng, prec, coded, page, d)
+    x["q"] = R.rounded(prec, rng.standard_normal((new, heads, d)))
+    nodes = attend_nodes(device, x, prec, np.zeros((1, 2 ** 31 // page), np.int64), np.array([length]), None)
+    op = link_attend(nodes, x, None, dict(window=window))
+    op.run()
+    device.await_()
+    got, lse = nodes.read("out"), nodes.read("lse")
+    for r in range(new):
+        pos = length - new + r
+        at = np.arange(pos - window + 1, pos + 1) % page
+        want, want_lse, off, lse_off = repeated_page(x["q"][r], k[at], v[at], window, prec, coded, 1.0 / np.sqrt(d))
+        R.within(got[r], want, off, "out")
+        R.within(lse[r], want_lse, lse_off, "lse")
+    op.free()
+    nodes.free()
+
+
 @pytest.mark.parametrize("prec,coded", [("single", False), ("half", True), ("bfloat16", False)])
 @pytest.mark.parametrize("window", [2 ** 31 - 2, 2 ** 31 - 1, 2 ** 62])
 @pytest.mark.parametrize("case", [(1, 8, [3], 16, 1, 4, 64), (2, [300, 200], [200, 210], 64, 1, 16, 64)])
