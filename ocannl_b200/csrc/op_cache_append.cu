@@ -260,7 +260,7 @@ __device__ __forceinline__ void page_codes(const AppendArgs& a, float2* table) {
     __syncthreads();
   };
   // A few tokens: a lane keeps its pieces, which are under way while the table is made; more are read twice.
-  const bool kept = n * items <= 32 * a.per_head * kAtOnce;
+  const bool kept = n * items <= 32 * a.per_head * kAtOnce;        // (no more than a table is for)
   P held[kAtOnce];
   auto hold = [&](unsigned int h0) {
     const unsigned int h = h0 + warp / a.per_head;
@@ -438,7 +438,8 @@ extern "C" int b200_cache_append_link(b200_dev* dev, const b200_cache_append* p,
     unsigned long long plain = 0, codes = 0;
     size_t table = 0;
     if (pc.tokens && pc.batch && per_token) {
-      // About four accesses a thread, while that leaves the machine enough blocks; a table of at most 32 KB
+      // About four accesses a thread, while that leaves the machine enough blocks; a table of at most 4096 pairs (32 KB, and the gaps between
+      // items: 40 KB in 16 bits, 48 in single precision, where pairs lie apart)
       unsigned long long tok = std::max(1ull, 1024ull / per_token);
       tok = std::min(tok, std::max(1ull, (unsigned long long)pc.tokens / (2ull * (unsigned)dev->sm_count)));
       if (a.pairs) tok = std::min(tok, std::max(1ull, 4096ull / a.pairs));
@@ -459,7 +460,9 @@ extern "C" int b200_cache_append_link(b200_dev* dev, const b200_cache_append* p,
         codes = (unsigned long long)a.pages_each * (unsigned long long)pc.batch;
       }
       a.by_pages_each = Divisor(std::max(1u, a.pages_each));
-      a.tile = (unsigned int)std::min<long long>(page, a.pairs ? std::max(1u, 8192u / a.pairs) : page);
+      // A table of at most 8192 pairs, 64 to 96 KB (two blocks an SM then; three where pages of 64 tokens of 64 pairs need 40 KB), and no fewer tokens than lanes
+      // keep the pieces of, all of which look into one table.
+      a.tile = (unsigned int)std::min<long long>(page, a.pairs ? std::max(8192u / a.pairs, std::max(1u, (unsigned int)(kThreads * kAtOnce) / a.items)) : page);
       table = std::max(table, (size_t)std::min<long long>(a.tile, pc.tokens) * row_of_table * 8);
       // Warps of a head: no fewer than hold what a page receives of it, as many as there are where heads are few.  (A block a page and all its heads, each read
       // twice by one warp: 75 us for 8192 tokens of 8 heads, pages of 64.)

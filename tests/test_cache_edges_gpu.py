@@ -165,3 +165,22 @@ def test_the_widest_windows(device, case, window, prec, coded):
     check_attend(nodes, want)
     op.free()
     nodes.free()
+
+
+@pytest.mark.parametrize("coded", [False, True])
+@pytest.mark.parametrize("prec,page,d,pairs,layout", [("bfloat16", 256, 128, 64, "half"), ("single", 200, 256, 128, "half"), ("half", 700, 36, 13, "interleaved"),
+                                                      ("bfloat16", 129, 128, 64, "interleaved"), ("single", 90, 512, 96, "interleaved")])
+def test_pages_of_more_tokens_than_a_table(device, prec, page, d, pairs, layout, coded):
+    """New tokens of a page whose cosines and sines are made in turns."""
+    from tests.test_serving_gpu import append_case, append_nodes, check_append, link_append
+    new = [page + 3, 1, 2 * page - 1, 128]
+    x, table, lengths, starts, page, f, layout = append_case((4, new, [page + 3, 9, 2 * page + 40, 130], page, 3, 2, d, pairs, layout), prec, coded)
+    want, off = R.append(x, prec, table, lengths, starts, page, f, layout)
+    nodes = append_nodes(device, x, prec, table, lengths, starts)
+    op = link_append(nodes, x, starts, f, layout)
+    for _ in range(2):
+        op.run()
+        device.await_()
+        check_append(nodes, want, off, coded)
+    op.free()
+    nodes.free()
