@@ -184,3 +184,26 @@ def test_pages_of_more_tokens_than_a_table(device, prec, page, d, pairs, layout,
         check_append(nodes, want, off, coded)
     op.free()
     nodes.free()
+
+
+@pytest.mark.parametrize("prec,coded,d,tokens,heads,length", [("bfloat16", False, 128, 130, 72, 17100), ("bfloat16", True, 128, 130, 72, 17100), ("half", False, 128, 130, 72, 17100),
+                                                              ("half", True, 128, 130, 72, 17100), ("bfloat16", True, 72, 100, 96, 33100)])
+def test_long_walks_of_tiles(device, prec, coded, d, tokens, heads, length):
+    """More than 16384 tokens in tiles of 128 rows, heads of more than 64 elements: accumulators are added to sums beside them."""
+    from tests.test_serving_gpu import attend_case
+    x, table, lengths, starts, page, t = attend_case((1, tokens, [length], 64, 1, heads, d, 0, 0, 0.0, False), prec, coded)
+    # (values of one sign add up: what an accumulator cuts off would show)
+    x["v_cache"] = x["v_cache"] & 0x7f if coded else np.abs(x["v_cache"])
+    x["q"] = R.rounded(prec, x["q"] * 0.05)
+    want = want_attend(x, table, lengths, starts, page, prec, t)
+    nodes = attend_nodes(device, x, prec, table, lengths, starts)
+    op = link_attend(nodes, x, starts, t)
+    op.run()
+    device.await_()
+    check_attend(nodes, want)
+    first = nodes.raw("out")
+    op.run()
+    device.await_()
+    assert nodes.raw("out").tobytes() == first.tobytes()
+    op.free()
+    nodes.free()
