@@ -110,3 +110,21 @@ def test_differences_and_temperatures_at_the_ends(device):
     u, t = R.rounded("single", np.array([0.1, 0.4, 0.7, 1.0])), t[:4]
     for given in (dict(temperature=t, top_p=float(np.float32(0.7))), dict(temperature=t, top_k=1500), dict(temperature=np.full(4, np.inf))):
         check_sample(run_sample(device, "single", x, u, given), x, u, given)
+
+
+@pytest.mark.parametrize("prec", PRECS)
+@pytest.mark.parametrize("vocab", [1022, 1500, 9001])
+def test_infinite_and_undefined_logits_of_long_rows(device, vocab, prec):
+    rng = np.random.default_rng(vocab)
+    x = rng.standard_normal((7, vocab)) * 3.0
+    x[0, [3, vocab // 2, vocab - 1]] = np.inf
+    x[1, rng.random(vocab) < 0.9] = np.inf
+    x[2] = np.where(rng.random(vocab) < 0.5, np.nan, -np.inf)
+    x[3] = np.where(rng.random(vocab) < 0.9, np.nan, x[3])
+    x[4] = np.where(rng.random(vocab) < 0.9, -np.inf, x[4])
+    x[5] = np.where(rng.random(vocab) < 0.3, -np.nan, x[5])
+    x[6, ::2] = -np.inf
+    x, u = R.rounded(prec, x), R.rounded("single", rng.random(7))
+    for given in ({}, dict(top_k=2), dict(top_k=1100, top_p=0.5), dict(top_p=0.75), dict(min_p=0.5), dict(temperature=0.0), dict(top_p=0.0, min_p=2.0), dict(temperature=1e-3, top_p=0.5)):
+        given = {n: float(np.float32(v)) if n != "top_k" else v for n, v in given.items()}
+        check_sample(run_sample(device, prec, x, u, given), x, u, given)
