@@ -11,9 +11,9 @@
 // multiplies its scores, that of the values raises its weights' exponents and is taken off the sum.  (bfloat16 queries beside codes are made halves in
 // shared memory by the softmax's threads, each row brought to 2^14.)
 //
-// Bound by the chain product, weights, product of a tile: 4096 new tokens of sequences of 8192, 32 heads over 8 of 128, codes, take 402 us (867 TFLOP/s), tensor pipe
-// and exponential unit 41 % busy each over a grid of 3.6 uneven rounds.  (3000 half tokens, a window of
-// 700, 16 heads over 4: 52 us, 254 in tiles of 8 rows.)
+// Bound by the chain product, weights, product of a tile: 4096 new tokens of sequences of 8192, 32 heads over 8 of 128, codes, take 364 to 428 us on several machines
+// (958 to 815 TFLOP/s), tensor pipe and exponential unit 41 % busy each over a grid of 3.6 uneven rounds.  (3000 half tokens, a window of 700, 16 heads over 4, capped:
+// 52 to 73 us, 254 in tiles of 8 rows.)
 //
 // Over more than kSumKeys tokens the accumulators are added to sums in tensor memory of their own every so many tiles (NQ = 1, which has room for them).
 #ifndef B200_CACHE_ATTN_FWD_SM100_CUH

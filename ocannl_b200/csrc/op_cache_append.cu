@@ -7,8 +7,10 @@
 // table of cosines and sines serves them.  Rows that become codes are taken a page of a sequence a block (keys and values apart), since a page's scale
 // of a head needs all its values first: a warp (or a few) a head reads them twice, the second time from the caches, and no block has to wait for
 // another.  Scales are powers of two, so that codes a page holds already lose nothing when its scale grows.
-// Measured: prompts of 8192 tokens together, 32 heads over 8 of 128, codes, 58 us (floor 26; bound by instructions: keys turn twice, and a page makes its table);
-// 256 sequences' tokens, codes, 9.1 us.
+// Measured: prompts of 8192 tokens together, 32 heads over 8 of 128, codes, 59 to 65 us on several machines (floor 26): 37 million instructions of warps (keys turn
+// twice, and a page makes its table) at half of the issue slots, with a third of the warps that an SM has room for, and with pieces that 80 registers a thread do not
+// hold (524 bytes a thread go to memory and back); the same into a cache of 16 bits 40 us.  256 sequences' tokens, codes, 9.2 us: a chain of dependent
+// accesses, of which the codes of a page whose scale grows, four bytes a lane one after another, are the longest.
 #include <cmath>
 
 #include "cache.hpp"
