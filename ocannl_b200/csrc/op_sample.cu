@@ -10,8 +10,8 @@
 // it, is usually a few hundred logits: these go to one block, which sorts them and does the rest in 64 bits.  Where they are more than 1024, the bin is divided
 // again by the bits of its logits, until it is small or of one value, and the row is passed once more for the token.
 // In the passes a weight is single (the exponential's 2^-22, and what its exponent's rounding makes: equal logits have equal weights, others' errors do not add up), with
-// the rate's rounding taken off, so that borders and tokens lie where 64 bits have them but for some 2^-10 of a weight in rows of 10^5 weights of one size.
-// Measured: 256 rows of 131072 logits 199 us, 64 of 50021 in bfloat16 43 us (in double precision throughout 312 and 55): 89 million instructions of warps at half of
+// a rate in two parts, so that borders and tokens lie where 64 bits have them but for some 2^-10 of a weight in rows of 10^5 weights of one size.
+// Measured: 256 rows of 131072 logits 203 us, 64 of 50021 in bfloat16 44 us (in double precision throughout 312 and 55): 89 million instructions of warps at half of
 // the issue slots; three blocks an SM wait for their logits' passes and for one another (the bytes alone: 20 us).
 #include <cooperative_groups.h>
 
@@ -359,24 +359,24 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
     meet(parts);
     return;
   }
-  // Binades z below the largest weight: of a few logits in 64 bits, of whole rows in single precision, with what the rate was rounded by put onto the weight: it
-  // would move all of a row together against the largest.  (Differences are taken of logits halved where they could be infinite, and multiplied where
+  // Binades z below the largest weight: of a few logits in 64 bits, of whole rows in single precision, rounded once, by a rate in two parts: what it is
+  // rounded by would move all of a row together against the largest.  (Differences are taken of logits halved where they could be infinite, and multiplied where
   // temperatures are so small that rates could be.  Not of -infinity, which is left out everywhere.)
   const bool endless = top == INFINITY;
   const float factor = top > 1e30f ? 0.5f : temperature < 1e-30f && fabsf(top) <= 1.f ? 1.2676506e30f : 1.f;      // (2^100)
   const double top64 = (double)top, rate = E > 0 ? early_rate : log2e / (double)temperature;
   const double rate_factor = endless ? 1.0 : fmin(factor == 1.f ? rate : factor < 1.f ? rate * 2.0 : rate * 7.888609052210118e-31, 3e38);
   // (what a rate above 2^20 is rounded by is left out, where differences of 2^127 would not go with it)
-  const float rate_hi = (float)rate_factor, to_weight = rate_hi <= 1048576.f ? (float)(rate_factor - (double)rate_hi) * -0.69314718f : 0.f;
+  const float rate_hi = (float)rate_factor, rate_lo = rate_hi <= 1048576.f ? (float)(rate_factor - (double)rate_hi) : 0.f;
   const float top_factor = endless ? 3.4028235e38f : top * factor;
   // (where the largest is infinite: 0 for those, and 2^126 at least for all others)
   auto difference = [&](float x) -> float { return fmaxf(fmaf(-x, factor, top_factor), 0.f); };
-  auto below = [&](float d) -> float { return __fmul_rn(d, rate_hi); };
-  // 2^-z for d's z
-  auto weight_at = [&](float d, float z) -> float {
+  // (a multiplied difference may be infinite, and what is undefined then as far away)
+  auto below = [&](float d) -> float { return fminf(fmaf(d, rate_hi, d * rate_lo), 1e6f); };
+  auto weight_at = [&](float z) -> float {
     float w;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(-z));
-    return fmaf(w, d * to_weight, w);
+    return w;
   };
   auto weight64 = [&](float x) -> double { return endless ? (x == top ? 1.0 : 0.0) : exp2(((double)x - top64) * rate); };
 
@@ -418,12 +418,12 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
       __syncthreads();
       const bool more = over(
           [&](float x, unsigned int i) {
-            const float d = difference(x), z = below(d);
+            const float z = below(difference(x));
             const int b = of(x, z);
             // (without branches, but for the last store)
             const unsigned int at = min((unsigned int)b, (unsigned int)kBins - 1u);
             Column v = mine[at * 32];
-            if (weighed.value) v.add(weight_at(d, z) * scale_of((int)at));
+            if (weighed.value) v.add(weight_at(z) * scale_of((int)at));
             else ++v.sum;
             if ((fresh.value ? x > -INFINITY : kept(x, i)) & ((unsigned int)b < (unsigned int)kBins)) mine[at * 32] = v;
           },
@@ -775,8 +775,7 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
       } else {
         // many equal ones: as many as are wanted of them, in the order of their indices
         const float value = of_key(lo);
-        const float d = difference(value);
-        const double w = (double)weight_at(d, below(d)), need = counting ? goal - above : w > 0.0 ? ceil((goal - sum_above) / w) : 1.0;
+        const double w = (double)weight_at(below(difference(value))), need = counting ? goal - above : w > 0.0 ? ceil((goal - sum_above) / w) : 1.0;
         unsigned int want = need < 1.0 ? 1u : need > (double)at.in ? at.in : (unsigned int)need, ties = 0;
         logits.each([&](float x, unsigned int i) { ties += x == value && kept(x, i); });
         ties = warp_join(ties, add);
@@ -817,7 +816,7 @@ __global__ void __launch_bounds__(kThreads, E == 0 ? 3 : 4) sample_rows(const __
     border_to = 0;
   }
   auto chance = [&](float x, unsigned int i) -> float {
-    const float d = difference(x), w = weight_at(d, below(d));
+    const float w = weight_at(below(difference(x)));
     return kept(x, i) ? w : 0.f;
   };
   double mine = 0.0;

@@ -128,3 +128,18 @@ def test_infinite_and_undefined_logits_of_long_rows(device, vocab, prec):
     for given in ({}, dict(top_k=2), dict(top_k=1100, top_p=0.5), dict(top_p=0.75), dict(min_p=0.5), dict(temperature=0.0), dict(top_p=0.0, min_p=2.0), dict(temperature=1e-3, top_p=0.5)):
         given = {n: float(np.float32(v)) if n != "top_k" else v for n, v in given.items()}
         check_sample(run_sample(device, prec, x, u, given), x, u, given)
+
+
+@pytest.mark.parametrize("vocab", [9, 700, 3000, 40000])
+def test_masked_logits_beside_the_least_temperatures(device, vocab):
+    """Finite masks (-10^9, the lowest value) where differences are multiplied: their weight is 0, as that of all but the largest few."""
+    rng = np.random.default_rng(vocab)
+    x = np.zeros((6, vocab))
+    x[:, ::2] = -1e9
+    x[:, ::7] = -3.4e38
+    x[:, 1::2] = -np.abs(rng.standard_normal((6, len(x[0, 1::2])))) * np.array([1e-31, 1e-36, 1e-30, 0.5, 1e-29, 1e-40])[:, None]
+    x[3, 1] = 1.0
+    x, u = R.rounded("single", x), R.rounded("single", rng.random(6))
+    t = R.rounded("single", np.array([1e-31, 1e-36, 9e-31, 1e-33, 1e-20, 1e-40]))
+    for given in (dict(temperature=t), dict(temperature=t, top_k=3), dict(temperature=t, top_p=float(np.float32(0.6))), dict(temperature=t, top_p=float(np.float32(0.999)), min_p=float(np.float32(0.01)))):
+        check_sample(run_sample(device, "single", x, u, given), x, u, given)
