@@ -207,3 +207,28 @@ def test_long_walks_of_tiles(device, prec, coded, d, tokens, heads, length):
     assert nodes.raw("out").tobytes() == first.tobytes()
     op.free()
     nodes.free()
+
+
+@pytest.mark.parametrize("prec,coded,page,d", [("bfloat16", True, 1024, 64), ("half", False, 1000, 40), ("single", False, 1024, 16)])
+@pytest.mark.parametrize("there", [[0], [12000, 38000], [0, 1, 2, 20000, 38999, 39000], []])
+def test_long_tables_of_few_pages(device, prec, coded, page, d, there):
+    """Most parts of a tile see nothing, whole turns of their joining among them."""
+    rng = np.random.default_rng(page + len(there))
+    length, width = 39000 * page + 5, 39003
+    x, kv = one_page(rng, prec, coded, page, d)
+    x["q"] = R.rounded(prec, rng.standard_normal((1, 3, d)))
+    table = np.full((1, width), -1)
+    table[0, there] = 0
+    seen = sum(5 if i == 39000 else page for i in there)
+    nodes = attend_nodes(device, x, prec, table, np.array([length]), None)
+    op = link_attend(nodes, x, None, {})
+    op.run()
+    device.await_()
+    if not seen:
+        assert np.all(nodes.read("out") == 0.0) and np.all(nodes.read("lse") == -np.inf)
+    else:
+        out, lse, off, lse_off = repeated_page(x["q"][0], *kv, seen, prec, coded, 1.0 / np.sqrt(d))
+        R.within(nodes.read("out")[0], out, off, "out")
+        R.within(nodes.read("lse")[0], lse, lse_off, "lse")
+    op.free()
+    nodes.free()
